@@ -358,6 +358,82 @@ nuka_result_t nuka_b200_world_set_contact_readout(nuka_world_handle world, uint3
 #define NUKA_B200_STATIC_RESET_MAX_IDS 4096u
 nuka_result_t nuka_b200_world_reset_envs_static(nuka_world_handle world, const uint32_t* env_ids, uint32_t count);
 
+/* ---- Sequence operators: the memory of a policy over the episodes of a rollout -------------------------------------------
+ *
+ * No counterpart in the reference.  A token is one control step of one env; tokens lie one behind the other in rows (an env's part
+ * of a rollout, or a whole episode), and an episode ends where the env was done.  Every call enqueues its kernels on `stream` (a
+ * cudaStream_t of the calling thread's current device; NULL is the default stream) and returns without waiting.  All pointers are device memory;
+ * tensors have contiguous channels (a head's dim values, a token's channels), other strides are in elements and given where named.
+ * Nothing is launched when a call is refused: INVALID_ARG for a null pointer, a negative size, a stride or address that the loads
+ * cannot take, NOT_SUPPORTED for a type or size outside the ranges below.  Nothing is allocated: workspaces are the caller's.
+ * The same call gives the same bits every time. */
+enum { NUKA_B200_F32 = 0, NUKA_B200_F16 = 1, NUKA_B200_BF16 = 2 };
+
+/* How `tokens` tokens are cut into rows and episodes: 4 x tokens int32, filled by one of the two calls below and read by the
+ * operators: first[t], the first token of t's episode; end[t], one past its last; link[t], -1 where t goes on from token t - 1, -2 where it
+ * begins an episode inside a row, else the row that it begins; tail[t], the row whose last token t is, else -1. */
+typedef struct nuka_b200_episodes_t {
+    int32_t *first, *end, *link, *tail;
+    int64_t tokens, rows;
+} nuka_b200_episodes_t;
+/* Rows are whole episodes: row r holds the tokens [offsets[r], offsets[r + 1]); offsets (int32, rows + 1) ascend from 0 to tokens, empty rows allowed.
+ * The offsets are read on the device and not checked there: others are clamped so that every index in the plan stays inside the tokens. */
+nuka_result_t nuka_b200_episodes_from_offsets(const nuka_b200_episodes_t* plan, const int32_t* offsets, void* stream);
+/* Rows of tokens / rows tokens each; done[t] != 0 ends an episode with token t. */
+nuka_result_t nuka_b200_episodes_from_done(const nuka_b200_episodes_t* plan, const uint8_t* done, void* stream);
+
+/* The gated linear recurrence h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(gate_t), channel by channel.  An episode that begins
+ * inside a row begins from 0, a row begins from initial (rows x channels float, NULL = 0).  state (rows x channels float) receives
+ * h of each row's last token before it is rounded; empty rows are left as they are. */
+typedef struct nuka_b200_recurrence_t {
+    const nuka_b200_episodes_t* plan;
+    uint32_t dtype;                                 /* of x, gate, h, dh, dx, dgate */
+    int64_t channels;
+    const void *x, *gate;
+    int64_t x_stride, gate_stride;                  /* between tokens */
+    const float* initial;
+    void* h;                                        /* tokens x channels; the backward call reads it */
+    float* state;
+    const void* dh;                                 /* the rest in the backward call only: tokens x channels, as are dx and dgate */
+    const float* dstate;                            /* rows x channels, NULL = 0 */
+    void *dx, *dgate;
+    float* dinitial;                                /* rows x channels, NULL = not wanted; empty rows are left as they are */
+    void* workspace;                                /* nuka_b200_recurrence_workspace() bytes, 8-byte aligned; may be NULL where that is 0 */
+    uint64_t workspace_bytes;
+} nuka_b200_recurrence_t;
+uint64_t nuka_b200_recurrence_workspace(uint32_t dtype, int64_t tokens, int64_t channels);
+nuka_result_t nuka_b200_recurrence(const nuka_b200_recurrence_t* desc, void* stream);
+nuka_result_t nuka_b200_recurrence_backward(const nuka_b200_recurrence_t* desc, void* stream);
+/* Its form for one token of each of n envs: state (n x channels float, contiguous) is updated in place, h receives it rounded; envs with fresh[i] != 0 (NULL = none) begin from 0. */
+nuka_result_t nuka_b200_recurrence_step(uint32_t dtype, int64_t n, int64_t channels, const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
+                                        const uint8_t* fresh, float* state, void* h, void* stream);
+
+/* Queries and keys of every head: divided by their root mean square over the head's dim values (mean square plus eps), times a weight
+ * per column (float, NULL = 1), then turned by the token's position: of the first `turned` columns the pairs (i, i + turned / 2), or with interleaved != 0
+ * (2 i, 2 i + 1), turn by the angle position x frequencies[i] radians (double, turned / 2 of them, so that long contexts keep their low bits).
+ * position[t] is t - plan->first[t], or positions[t] where positions is not NULL.  dim and turned are multiples of 8, dim at most 256.
+ * The backward call takes dq_out / dk_out, writes dq / dk (contiguous) and the weights' gradients (float, NULL = not wanted). */
+typedef struct nuka_b200_heads_t {
+    const int32_t* first;                           /* the plan's, or NULL with positions */
+    const int32_t* positions;
+    const double* frequencies;
+    uint32_t dtype, interleaved;
+    int64_t tokens, heads_q, heads_k, dim, turned;
+    const void *q, *k;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride;
+    const float *q_weight, *k_weight;
+    float eps;
+    void *q_out, *k_out;                            /* tokens x heads x dim, contiguous */
+    const void *dq_out, *dk_out;                    /* the rest in the backward call only, contiguous */
+    void *dq, *dk;
+    float *dq_weight, *dk_weight;
+    void* workspace;                                /* nuka_b200_heads_workspace() bytes, needed where a weight's gradient is wanted */
+    uint64_t workspace_bytes;
+} nuka_b200_heads_t;
+uint64_t nuka_b200_heads_workspace(int64_t tokens, int64_t dim);
+nuka_result_t nuka_b200_heads(const nuka_b200_heads_t* desc, void* stream);
+nuka_result_t nuka_b200_heads_backward(const nuka_b200_heads_t* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@
 #include "../../include/nuka_b200.h"
 #include "nkb_host_pool.h"
 #include "nkb_scene.h"
+#include "nkb_sequence.h"
 #include "nkb_world.h"
 
 namespace {
@@ -181,6 +182,12 @@ nuka_result_t CreateWorld(nuka_device_handle device, const nuka_world_desc_t* de
 }
 
 }  // namespace
+
+namespace nkb {
+void SetLastError(const char* text) {
+    try { g_last_error = text; } catch (...) { g_last_error.clear(); }
+}
+}  // namespace nkb
 
 extern "C" {
 

@@ -62,6 +62,26 @@ class CookOptions(ctypes.Structure):
                 ("scene_filters", ctypes.c_uint32), ("max_contacts", ctypes.c_uint32), ("max_points", ctypes.c_uint32)]
 
 
+class EpisodesDesc(ctypes.Structure):
+    _fields_ = [("first", ctypes.c_void_p), ("end", ctypes.c_void_p), ("link", ctypes.c_void_p), ("tail", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("rows", ctypes.c_int64)]
+
+
+class RecurrenceDesc(ctypes.Structure):
+    _fields_ = [("plan", ctypes.POINTER(EpisodesDesc)), ("dtype", ctypes.c_uint32), ("channels", ctypes.c_int64), ("x", ctypes.c_void_p), ("gate", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64), ("initial", ctypes.c_void_p), ("h", ctypes.c_void_p), ("state", ctypes.c_void_p),
+                ("dh", ctypes.c_void_p), ("dstate", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dgate", ctypes.c_void_p), ("dinitial", ctypes.c_void_p),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class HeadsDesc(ctypes.Structure):
+    _fields_ = [("first", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("frequencies", ctypes.c_void_p), ("dtype", ctypes.c_uint32), ("interleaved", ctypes.c_uint32),
+                ("tokens", ctypes.c_int64), ("heads_q", ctypes.c_int64), ("heads_k", ctypes.c_int64), ("dim", ctypes.c_int64), ("turned", ctypes.c_int64),
+                ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64), ("k_stride", ctypes.c_int64),
+                ("k_head_stride", ctypes.c_int64), ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p), ("eps", ctypes.c_float),
+                ("q_out", ctypes.c_void_p), ("k_out", ctypes.c_void_p), ("dq_out", ctypes.c_void_p), ("dk_out", ctypes.c_void_p), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p),
+                ("dq_weight", ctypes.c_void_p), ("dk_weight", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
 EXPORTS = [
     "nuka_get_version", "nuka_result_message", "nuka_last_error_message", "nuka_device_create", "nuka_device_destroy",
     "nuka_world_create_from_scene", "nuka_world_destroy", "nuka_world_step", "nuka_world_step_n", "nuka_world_set_execution_mode",
@@ -72,7 +92,8 @@ EXPORTS = [
     "nuka_b200_world_pack_observations", "nuka_b200_observation_desc_defaults", "nuka_b200_world_reset_envs_masked", "nuka_b200_world_episode_step",
     "nuka_b200_world_set_contact_readout", "nuka_b200_world_set_broadphase", "nuka_b200_template_check", "nuka_b200_cook_options_defaults", "nuka_b200_scene_cook", "nuka_world_checkpoint_capture", "nuka_world_checkpoint_restore", "nuka_checkpoint_destroy",
     "nuka_checkpoint_write", "nuka_world_checkpoint_read", "nuka_checkpoint_byte_size", "nuka_checkpoint_equal", "nuka_world_state_hash",
-    "nuka_world_get_dof_name",
+    "nuka_world_get_dof_name", "nuka_b200_episodes_from_offsets", "nuka_b200_episodes_from_done", "nuka_b200_recurrence_workspace", "nuka_b200_recurrence",
+    "nuka_b200_recurrence_backward", "nuka_b200_recurrence_step", "nuka_b200_heads_workspace", "nuka_b200_heads", "nuka_b200_heads_backward",
 ]
 
 _LIB = None
@@ -140,5 +161,17 @@ def lib():
     L.nuka_checkpoint_byte_size.argtypes = [vp, ctypes.POINTER(ctypes.c_uint64)]
     L.nuka_checkpoint_equal.argtypes = [vp, vp, ctypes.POINTER(u32)]
     L.nuka_world_state_hash.argtypes = [vp, ctypes.POINTER(ctypes.c_uint64)]
+    i64, u64 = ctypes.c_int64, ctypes.c_uint64
+    L.nuka_b200_episodes_from_offsets.argtypes = [ctypes.POINTER(EpisodesDesc), vp, vp]
+    L.nuka_b200_episodes_from_done.argtypes = [ctypes.POINTER(EpisodesDesc), vp, vp]
+    L.nuka_b200_recurrence_workspace.argtypes = [u32, i64, i64]
+    L.nuka_b200_recurrence_workspace.restype = u64
+    L.nuka_b200_recurrence.argtypes = [ctypes.POINTER(RecurrenceDesc), vp]
+    L.nuka_b200_recurrence_backward.argtypes = [ctypes.POINTER(RecurrenceDesc), vp]
+    L.nuka_b200_recurrence_step.argtypes = [u32, i64, i64, vp, i64, vp, i64, vp, vp, vp, vp]
+    L.nuka_b200_heads_workspace.argtypes = [i64, i64]
+    L.nuka_b200_heads_workspace.restype = u64
+    L.nuka_b200_heads.argtypes = [ctypes.POINTER(HeadsDesc), vp]
+    L.nuka_b200_heads_backward.argtypes = [ctypes.POINTER(HeadsDesc), vp]
     _LIB = L
     return L

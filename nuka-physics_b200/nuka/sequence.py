@@ -1,0 +1,274 @@
+"""Sequence operators of a policy with memory: what a policy over the episodes of a rollout needs next to ``nuka.vec_env``.
+
+A token is one control step of one env.  Tokens lie one behind the other in rows (an env's part of a rollout, or a whole episode);
+``Episodes`` says where each token's episode begins and ends, and all operators over rollouts read it.  Each has a form for one token of
+every env, for acting:
+
+    over a rollout (training)                      one token of every env (acting)
+    gated_recurrence(x, gate, episodes, initial)   gated_recurrence_step(x, gate, state, fresh)
+    rotate_heads(q, k, ..., episodes, ...)         rotate_heads(q, k, ..., positions, ...)
+
+Tensors live on one GPU; the work is enqueued on torch's current stream of that GPU and nothing waits for it.  Operators over
+rollouts take part in automatic differentiation (once).  Needs torch with CUDA.
+"""
+import ctypes
+
+import torch
+
+from . import _abi, _check
+
+_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+
+
+def _expect(ok, text):
+    if not ok:
+        raise ValueError(text)
+
+
+def _on_gpu(*tensors):
+    """The GPU that all of the tensors are on (None is left out)."""
+    device = tensors[0].device
+    _expect(device.type == "cuda", "tensors must be on the GPU")
+    for tensor in tensors:
+        _expect(tensor is None or tensor.device == device, "tensors must be on one GPU")
+    return device
+
+
+def _dtype(tensor, allowed, what):
+    _expect(tensor.dtype in allowed, f"{what} must be one of {', '.join(str(d).replace('torch.', '') for d in allowed)}, not {str(tensor.dtype).replace('torch.', '')}")
+    return _DTYPES[tensor.dtype]
+
+
+def _call(device, function, *args):
+    """One call of the library on torch's current stream of `device`."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            _check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        _check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _ptr(tensor):
+    return None if tensor is None else tensor.data_ptr()
+
+
+def _flags(tensor, shape, device, what):
+    _expect(tensor.dtype in (torch.bool, torch.uint8) and tuple(tensor.shape) == shape and tensor.device == device, f"{what} must be {shape} bool or uint8 on {device}")
+    return tensor.contiguous()
+
+
+def _stride(tensor, dim):
+    return tensor.stride(dim) if tensor.shape[dim] > 1 else 0
+
+
+def _channels_last(tensor, multiple=1, size=1):
+    """The tensor as it is where its last dimension is contiguous, its strides are multiples of `multiple` values and it lies on `size` bytes, else a copy."""
+    last = tensor.dim() - 1
+    if (tensor.shape[last] == 1 or tensor.stride(last) == 1) and tensor.data_ptr() % size == 0 and all(_stride(tensor, d) % multiple == 0 for d in range(last)):
+        return tensor
+    return tensor.clone(memory_format=torch.contiguous_format)
+
+
+class Episodes:
+    """How a rollout's tokens are cut into rows and episodes, on the GPU.  Made once per rollout, for all layers and passes over it."""
+
+    def __init__(self, tokens, rows, device, rows_may_be_empty):
+        self.tokens, self.rows, self.device = int(tokens), int(rows), torch.device(device)
+        self._rows_may_be_empty = rows_may_be_empty or self.tokens == 0
+        self._plan = torch.empty((4, self.tokens), dtype=torch.int32, device=device)
+        base, step = self._plan.data_ptr(), 4 * self.tokens
+        self._desc = _abi.EpisodesDesc(base, base + step, base + 2 * step, base + 3 * step, self.tokens, self.rows)
+        self._ref = ctypes.pointer(self._desc)
+
+    @classmethod
+    def from_offsets(cls, offsets, tokens):
+        """Rows are whole episodes: row r holds the tokens offsets[r] to offsets[r + 1].  `offsets`: int32 on the GPU, rows + 1 of them, ascending from 0
+        to `tokens` (they are not read back to be checked)."""
+        _expect(offsets.dim() == 1 and offsets.numel() >= 1 and offsets.dtype == torch.int32, "offsets must be a vector of int32")
+        _expect(tokens >= 0, "tokens must not be negative")
+        device = _on_gpu(offsets)
+        offsets = offsets.contiguous()
+        plan = cls(tokens, offsets.numel() - 1, device, True)
+        _call(device, _abi.lib().nuka_b200_episodes_from_offsets, plan._ref, offsets.data_ptr())
+        return plan
+
+    @classmethod
+    def from_done(cls, done):
+        """A rollout of N envs over T control steps, its tokens env after env: `done` (N x T, bool or uint8, on the GPU) is set where an
+        episode ended with that token, as ``NukaVecEnv.step`` reports it."""
+        _expect(done.dim() == 2, "done must be envs x steps")
+        device = _on_gpu(done)
+        done = _flags(done, tuple(done.shape), device, "done")
+        plan = cls(done.numel(), done.shape[0], device, False)
+        _call(device, _abi.lib().nuka_b200_episodes_from_done, plan._ref, done.data_ptr())
+        return plan
+
+    @property
+    def first(self):
+        """Index of the first token of each token's episode."""
+        return self._plan[0]
+
+    @property
+    def end(self):
+        """Index behind the last token of each token's episode."""
+        return self._plan[1]
+
+    @property
+    def positions(self):
+        """Each token's number in its episode, from 0."""
+        return torch.arange(self.tokens, dtype=torch.int32, device=self.device) - self._plan[0]
+
+
+def _tokens_of(tensor, episodes, dims, what):
+    _expect(tensor.dim() == dims and tensor.shape[0] == episodes.tokens, f"{what} must have {dims} dimensions, the first of {episodes.tokens} tokens")
+
+
+# ---- the gated linear recurrence -----------------------------------------------------------------------------------
+class _Recurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, initial, episodes):
+        device, dtype = x.device, _DTYPES[x.dtype]
+        x, gate = _channels_last(x), _channels_last(gate)
+        channels = x.shape[1]
+        h = torch.empty(x.shape, dtype=x.dtype, device=device)
+        if not episodes._rows_may_be_empty:
+            state = torch.empty((episodes.rows, channels), dtype=torch.float32, device=device)
+        elif initial is None:
+            state = torch.zeros((episodes.rows, channels), dtype=torch.float32, device=device)
+        else:
+            state = initial.clone()
+        lib = _abi.lib()
+        need = lib.nuka_b200_recurrence_workspace(dtype, episodes.tokens, channels)
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), state.data_ptr(),
+                                   None, None, None, None, None, _ptr(workspace), need)
+        _call(device, lib.nuka_b200_recurrence, ctypes.byref(desc))
+        ctx.episodes, ctx.has_initial = episodes, initial is not None
+        ctx.save_for_backward(x, gate, h, *([initial] if initial is not None else []))
+        ctx.set_materialize_grads(False)
+        return h, state
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dstate):
+        x, gate, h, *initial = ctx.saved_tensors
+        initial, episodes = initial[0] if initial else None, ctx.episodes
+        device, dtype, channels = x.device, _DTYPES[x.dtype], x.shape[1]
+        dh = torch.zeros_like(h) if dh is None else dh.contiguous()
+        dstate = None if dstate is None else dstate.contiguous()
+        dx, dgate = torch.empty(x.shape, dtype=x.dtype, device=device), torch.empty(x.shape, dtype=x.dtype, device=device)
+        dinitial = None
+        if ctx.has_initial and ctx.needs_input_grad[2]:
+            if not episodes._rows_may_be_empty:
+                dinitial = torch.empty_like(initial)
+            else:                                   # an empty row ends with the state that it began with
+                dinitial = torch.zeros_like(initial) if dstate is None else dstate.clone()
+        lib = _abi.lib()
+        need = lib.nuka_b200_recurrence_workspace(dtype, episodes.tokens, channels)
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), None,
+                                   dh.data_ptr(), _ptr(dstate), dx.data_ptr(), dgate.data_ptr(), _ptr(dinitial), _ptr(workspace), need)
+        _call(device, lib.nuka_b200_recurrence_backward, ctypes.byref(desc))
+        return dx, dgate, dinitial, None
+
+
+def gated_recurrence(x, gate, episodes, initial=None):
+    """h_t = a_t h_{t-1} + (1 - a_t) x_t with a_t = sigmoid(gate_t), channel by channel over each episode.
+
+    x, gate: tokens x channels, f32, f16 or bf16.  initial: rows x channels f32, the state that each row begins with (the one its env had
+    when the rollout began), None for 0; an episode that begins inside a row begins with 0.  Returns (h, state): h like x, state (rows x channels f32) the
+    state that each row ends with, not rounded."""
+    device = _on_gpu(x, gate, initial, episodes._plan)
+    _dtype(x, tuple(_DTYPES), "x")
+    _tokens_of(x, episodes, 2, "x")
+    _expect(gate.shape == x.shape and gate.dtype == x.dtype, "gate must be like x")
+    if initial is not None:
+        _expect(tuple(initial.shape) == (episodes.rows, x.shape[1]) and initial.dtype == torch.float32, f"initial must be {episodes.rows} x {x.shape[1]} float32 on {device}")
+        initial = initial.contiguous()
+    return _Recurrence.apply(x, gate, initial, episodes)
+
+
+def gated_recurrence_step(x, gate, state, fresh=None):
+    """The recurrence for one token of each env.  x, gate: envs x channels; state: envs x channels f32, contiguous, updated in place; fresh: envs, bool or
+    uint8, set where the token begins an episode (the state before it counts as 0).  Returns h, the new state in x's type.  No gradient."""
+    device = _on_gpu(x, gate, state, fresh)
+    dtype = _dtype(x, tuple(_DTYPES), "x")
+    _expect(x.dim() == 2 and gate.shape == x.shape and gate.dtype == x.dtype, "x and gate must be envs x channels, of one type")
+    _expect(state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous(), "state must be contiguous float32, envs x channels")
+    x, gate = _channels_last(x), _channels_last(gate)
+    if fresh is not None:
+        fresh = _flags(fresh, (x.shape[0],), device, "fresh")
+    h = torch.empty(x.shape, dtype=x.dtype, device=device)
+    _call(device, _abi.lib().nuka_b200_recurrence_step, dtype, x.shape[0], x.shape[1], x.data_ptr(), _stride(x, 0), gate.data_ptr(), _stride(gate, 0), _ptr(fresh), state.data_ptr(), h.data_ptr())
+    return h
+
+
+# ---- norms of queries and keys, and their rotation -----------------------------------------------------------------
+def rotary_frequencies(turned, base=10000.0, trained=0, context=0, low=1.0, high=32.0):
+    """Angle per position of each of the turned / 2 pairs (float64, on the CPU): base^(-2 i / turned).  With `trained` and a longer `context`, pairs that
+    turn fewer than `low` times within the trained context are slowed down by context / trained, pairs that turn more than `high` times stay, those between are mixed
+    (the frequency part of the YaRN paper, Peng et al. 2023)."""
+    _expect(turned >= 0 and turned % 2 == 0, "turned must be even")
+    f = float(base) ** (-torch.arange(0, turned, 2, dtype=torch.float64) / max(turned, 1))
+    if trained and context > trained:
+        keep = ((trained * f / (2 * torch.pi) - low) / (high - low)).clamp(0.0, 1.0)
+        f = f * (keep + (1 - keep) * (trained / context))
+    return f
+
+
+class _Heads(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
+        device, size = q.device, q.element_size()
+        q, k = (_channels_last(x, 4, 4 * size) for x in (q, k))
+        tokens, heads_q, dim = q.shape
+        q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=q.dtype, device=device)
+        desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), tokens, heads_q, k.shape[1], dim,
+                              0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
+                              _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
+        _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
+        # the descriptor's arrays stay alive with what is saved here
+        ctx.save_for_backward(q, k, *(x for x in (q_weight, k_weight, first, positions, frequencies) if x is not None))
+        ctx.desc, ctx.weights = desc, (q_weight is not None, k_weight is not None)
+        ctx.set_materialize_grads(False)
+        return q_out, k_out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k = ctx.saved_tensors[:2]
+        device, desc = q.device, ctx.desc
+        dq_out, dk_out = (torch.zeros(x.shape, dtype=x.dtype, device=device) if d is None else _channels_last(d.contiguous(), 1, 4 * x.element_size()) for x, d in ((q, dq_out), (k, dk_out)))
+        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device)
+        dw = [torch.empty(q.shape[2], dtype=torch.float32, device=device) if has and ctx.needs_input_grad[2 + i] else None for i, has in enumerate(ctx.weights)]
+        lib = _abi.lib()
+        need = lib.nuka_b200_heads_workspace(q.shape[0], q.shape[2]) if dw[0] is not None or dw[1] is not None else 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        desc.dq_out, desc.dk_out, desc.dq, desc.dk = dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr()
+        desc.dq_weight, desc.dk_weight, desc.workspace, desc.workspace_bytes = _ptr(dw[0]), _ptr(dw[1]), _ptr(workspace), need
+        _call(device, lib.nuka_b200_heads_backward, ctypes.byref(desc))
+        return dq, dk, dw[0], dw[1], None, None, None, None, None
+
+
+def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, interleaved=False):
+    """Each head's queries and keys divided by their root mean square, times a weight per column, then turned by their position.
+
+    q: tokens x heads x dim, k: tokens x key heads x dim, f32, f16 or bf16, heads and tokens at any stride (views of one projection).  q_weight, k_weight: dim f32, or None.
+    positions: an ``Episodes`` (each token's number in its episode) or int32 per token.  frequencies: float64 on the GPU, one per turned pair
+    (``rotary_frequencies``; twice as many columns are turned, the others only normed), or None.  Pairs are (i, i + turned / 2), or with `interleaved` (2 i, 2 i + 1).
+    dim and the number of turned columns are multiples of 8, dim at most 256.  Returns (q, k), contiguous."""
+    episodes = positions if isinstance(positions, Episodes) else None
+    _on_gpu(q, k, q_weight, k_weight, frequencies, episodes._plan if episodes is not None else positions)
+    _dtype(q, tuple(_DTYPES), "q")
+    _expect(q.dim() == 3 and k.dim() == 3 and k.dtype == q.dtype and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2], "q and k must be tokens x heads x dim, of one type")
+    for w in (q_weight, k_weight):
+        _expect(w is None or (tuple(w.shape) == (q.shape[2],) and w.dtype == torch.float32), "weights must be float32, one per column of a head")
+    _expect(frequencies is None or (frequencies.dim() == 1 and frequencies.dtype == torch.float64), "frequencies must be a vector of float64")
+    if episodes is not None:
+        _tokens_of(q, episodes, 3, "q")
+        first, positions = episodes.first, None
+    else:
+        _expect(positions.dtype == torch.int32 and tuple(positions.shape) == (q.shape[0],), "positions must be an Episodes or int32, one per token")
+        first, positions = None, positions.contiguous()
+    q_weight, k_weight, frequencies = (None if x is None else x.contiguous() for x in (q_weight, k_weight, frequencies))
+    return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)

@@ -434,6 +434,28 @@ uint64_t nuka_b200_heads_workspace(int64_t tokens, int64_t dim);
 nuka_result_t nuka_b200_heads(const nuka_b200_heads_t* desc, void* stream);
 nuka_result_t nuka_b200_heads_backward(const nuka_b200_heads_t* desc, void* stream);
 
+/* Causal attention over the plan's episodes: out_i = sum over j of softmax(scale q_i . k_j) v_j, j from the first token of i's episode to i, or with
+ * window > 0 over the last `window` of these.  Query head h reads key head h / (heads_q / heads_k).  F16 or BF16; dim is a multiple of 8, at most 128;
+ * tensors lie on 16 bytes, strides are multiples of 8 values.  lse (and delta): heads_q x nuka_b200_attention_pitch(tokens) float on 16 bytes; the forward call writes lse, base 2 and
+ * scaled (NULL: not wanted), the backward call reads it and uses delta as a workspace.  out, dout, dq (tokens x heads_q x dim), dk and dv (tokens x heads_k x dim) are
+ * contiguous.  Probabilities and their gradients are rounded to the type of q before the second product, sums are in 32 bits. */
+typedef struct nuka_b200_attention_t {
+    const nuka_b200_episodes_t* plan;
+    uint32_t dtype;
+    int64_t heads_q, heads_k, dim, window;
+    float scale;                                    /* greater than 0 */
+    const void *q, *k, *v;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    void* out;
+    float* lse;
+    const void* dout;                               /* the rest in the backward call only */
+    float* delta;
+    void *dq, *dk, *dv;
+} nuka_b200_attention_t;
+int64_t nuka_b200_attention_pitch(int64_t tokens);
+nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream);
+nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

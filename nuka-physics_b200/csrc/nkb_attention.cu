@@ -1,0 +1,609 @@
+// Causal attention over packed episodes, forwards and backwards, on the tensor cores.
+//
+// Rows of the products are 128 tokens that lie one behind the other, whatever episodes they belong to: a token i sees the keys max(first_i, i - window + 1)
+// to i, both ends grow with i, so a tile of queries sees one range of keys, from the first one's first to the last one's own, and only
+// the tiles at that range's ends need a mask.  Short episodes share a tile; no length is known to the host.
+//
+//   forwards    S = Q K^T, P = exp2(scale log2(e) S - m), O += P V, m the running maximum, at last O / sum P
+//   queries     S, dP = dO V^T, dS = P (dP - D) with D = dO . O, dQ += dS K
+//   keys        S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q over all heads of the key's group
+//
+// The backward pass works the scores out twice, once for the queries' gradients and once for the keys': 7 products in place of 5, and in return no gradient is summed
+// through atomics, so that the same call gives the same bits, and the shared heads' sum stays in tensor memory.
+// One warp loads tiles by TMA, one thread issues the products, four warps turn scores into probabilities, a row to a thread;
+// P and dS go back to tensor memory as the next product's operand in the inputs' type (their one rounding more; sums and statistics are in 32 bits).
+// Two blocks share an SM, so that one's products run under the other's exponentials.
+#include <cuda_runtime.h>
+#include <algorithm>
+#include "nkb_sequence.cuh"
+#include "nkb_sequence.h"
+#include "nkb_tcgen.cuh"
+
+namespace nkb {
+
+constexpr int kRows = 128;                              // tokens of a block's tile, a thread and a tensor-memory lane each
+constexpr int kStream = 64;                             // tokens of a streamed tile of the backward pass
+constexpr int kBlock = 192;                             // four warps of rows, one that loads, one that multiplies
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttentionParams {
+    const int32_t *first, *end;
+    int64_t tokens, pitch;                              // pitch: floats between the heads' rows of lse and delta
+    int heads_q, heads_k, dim, window;                  // window 0: all of the episode
+    float scale, scale2;                                // scale2: times log2(e)
+    void *out, *dq, *dk, *dv;
+    const void* dout;
+    float *lse, *delta;
+};
+
+__device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
+__device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
+__device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+
+// One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T.
+template <typename T, int DP> __device__ __forceinline__ void store_row(uint32_t at, float by, int dim, T* to) {
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+        uint32_t r[32];
+        __syncwarp();
+        tensor_load(at + c, r);
+        wait_loads();
+#pragma unroll
+        for (int k = 0; k < 32; k += 8)
+            if (to != nullptr && c + k < dim) {
+                uint4 v;
+                v.x = pack<T>(__uint_as_float(r[k]) * by, __uint_as_float(r[k + 1]) * by);
+                v.y = pack<T>(__uint_as_float(r[k + 2]) * by, __uint_as_float(r[k + 3]) * by);
+                v.z = pack<T>(__uint_as_float(r[k + 4]) * by, __uint_as_float(r[k + 5]) * by);
+                v.w = pack<T>(__uint_as_float(r[k + 6]) * by, __uint_as_float(r[k + 7]) * by);
+                *reinterpret_cast<uint4*>(to + c + k) = v;
+            }
+    }
+}
+
+// ROWS x DP of one head: panels of 64 columns, each ROWS x 128 bytes
+template <int ROWS, int DP> __device__ __forceinline__ void load_panels(unsigned char* to, const CUtensorMap* map, uint64_t* bar, int head, int token) {
+#pragma unroll
+    for (int c = 0; c < DP; c += 64) load_tile(to + c / 64 * ROWS * 128, map, bar, c, head, token);
+}
+// d = A B^T over DP inner columns: A 128 rows, B N rows, both as loaded
+template <typename T, int N, int DP> __device__ __forceinline__ void multiply_rows(uint32_t d, uint32_t a, uint32_t b) {
+#pragma unroll
+    for (int k = 0; k < DP; k += 16)
+        multiply(d, inner_rows(a + k / 64 * kRows * 128 + k % 64 * 2), inner_rows(b + k / 64 * N * 128 + k % 64 * 2), product_of<T>(N, false), k != 0);
+}
+// d (+)= A B over N rows of B, A in tensor memory
+template <typename T, int N, int DP> __device__ __forceinline__ void multiply_columns(uint32_t d, uint32_t a, uint32_t b, bool add) {
+#pragma unroll
+    for (int k = 0; k < N; k += 16) multiply_tensor(d, a + k / 2, outer_rows(b + k * 128, N * 128), product_of<T>(DP, true), add || k != 0);
+}
+
+// All lanes of a warp wait, and go on together.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* lost) { return __all_sync(~0u, barrier_wait(bar, parity, lost)) != 0; }
+
+// A block that gave up waits, again for a bounded time, for the loads that it still has under way; what they bring is not used.
+__device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
+    const long long began = clock64();
+    while (!barrier_try(bar, parity) && clock64() - began < kBarrierCycles) {}
+}
+
+extern __shared__ unsigned char dynamic_shared[];
+__device__ __forceinline__ unsigned char* aligned_shared() { return dynamic_shared + ((1024u - (shared_address(dynamic_shared) & 1023u)) & 1023u); }
+
+// ---- forwards ---------------------------------------------------------------------------------------------------------
+template <int DP> struct Forward {
+    static constexpr int kStages = DP == 64 ? 2 : 1;
+    static constexpr bool kApart = DP == 64;            // P has columns of its own, so that the next scores do not wait for P V
+    static constexpr int kTile = kRows * DP * 2;
+    static constexpr int kShared = kTile * (1 + 2 * kStages) + 1024;
+    static constexpr int kOut = kRows, kProb = kApart ? kRows + DP : 0;      // columns; the scores are at 0
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBlock, 2) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                              const AttentionParams p) {
+    using F = Forward<DP>;
+    __shared__ uint64_t q_full, k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ uint32_t tensor;
+    __shared__ int lost;
+    unsigned char* const shared = aligned_shared();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int tiles = (int)((p.tokens + kRows - 1) / kRows), tile = tiles - 1 - (int)(blockIdx.x / p.heads_q), head = blockIdx.x % p.heads_q;     // the longest first
+    const int key_head = head / (p.heads_q / p.heads_k);
+    const int i0 = tile * kRows, last = (int)min((int64_t)i0 + kRows, p.tokens) - 1;
+    const int j0 = first_key(p, i0), count = (last - j0) / kRows + 1;
+    if (threadIdx.x == 0) {
+        lost = 0;
+        barrier_init(&q_full, 1);
+        for (int s = 0; s < F::kStages; ++s) { barrier_init(&k_full[s], 1); barrier_init(&k_empty[s], 1); barrier_init(&v_full[s], 1); barrier_init(&v_empty[s], 1); }
+        barrier_init(&s_full, 1);
+        barrier_init(&p_full, kRows);
+        barrier_init(&o_done, 1);
+        barrier_init(&ended, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 5) tensor_alloc<256>(&tensor);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t base = tensor, q_at = shared_address(shared), k_at = q_at + F::kTile, v_at = k_at + F::kStages * F::kTile;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            barrier_expect(&q_full, F::kTile);
+            load_panels<kRows, DP>(shared, &map_q, &q_full, head, i0);
+            int j = 0;
+            for (; j < count; ++j) {
+                const int s = j % F::kStages, turn = j / F::kStages;
+                if (turn > 0 && !barrier_wait(&k_empty[s], (turn - 1) & 1, &lost)) break;
+                barrier_expect(&k_full[s], F::kTile);
+                load_panels<kRows, DP>(shared + F::kTile * (1 + s), &map_k, &k_full[s], key_head, j0 + j * kRows);
+                if (turn > 0 && !barrier_wait(&v_empty[s], (turn - 1) & 1, &lost)) { drain(&k_full[s], turn & 1); break; }
+                barrier_expect(&v_full[s], F::kTile);
+                load_panels<kRows, DP>(shared + F::kTile * (1 + F::kStages + s), &map_v, &v_full[s], key_head, j0 + j * kRows);
+            }
+            drain(&q_full, 0);
+            for (int b = max(0, j - F::kStages); b < j; ++b) { drain(&k_full[b % F::kStages], b / F::kStages & 1); drain(&v_full[b % F::kStages], b / F::kStages & 1); }
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            bool fine = barrier_wait(&q_full, 0, &lost);
+            auto scores = [&](int j) {
+                const int s = j % F::kStages;
+                if (!barrier_wait(&k_full[s], j / F::kStages & 1, &lost)) return false;
+                fence_after();
+                multiply_rows<T, kRows, DP>(base, q_at, k_at + s * F::kTile);
+                commit(&s_full);
+                commit(&k_empty[s]);
+                return true;
+            };
+            fine = fine && scores(0);
+            for (int j = 0; fine && j < count; ++j) {
+                const int s = j % F::kStages;
+                if (!barrier_wait(&p_full, j & 1, &lost)) break;
+                fence_after();
+                if (F::kApart && j + 1 < count) fine = scores(j + 1);
+                if (!fine || !barrier_wait(&v_full[s], j / F::kStages & 1, &lost)) break;
+                fence_after();
+                multiply_columns<T, kRows, DP>(base + F::kOut, base + F::kProb, v_at + s * F::kTile, j != 0);
+                commit(&v_empty[s]);
+                commit(&o_done);
+                if (!F::kApart && j + 1 < count) fine = barrier_wait(&o_done, j & 1, &lost) && scores(j + 1);
+            }
+            commit(&ended);
+            drain(&ended, 0);
+        }
+    } else {
+        const int i = i0 + threadIdx.x;
+        const bool live = i < p.tokens;
+        const int low = live ? first_key(p, i) : 0, high = live ? i : -1;
+        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
+        float top = -INFINITY, sum = 0.f;                       // of the scores as they are; the sum of exp2(scale2 (S - top))
+        bool fine = true;
+        for (int j = 0; j < count; ++j) {
+            const int k0 = j0 + j * kRows;
+            if (!(fine = warp_wait(&s_full, j & 1, &lost))) break;
+            fence_after();
+            uint32_t r[kRows];
+#pragma unroll
+            for (int c = 0; c < kRows; c += 32) tensor_load(mine + c, r + c);
+            wait_loads();
+            if (!__all_sync(~0u, k0 >= low && k0 + kRows - 1 <= high)) {
+                const int from = low - k0, to = high - k0;
+#pragma unroll
+                for (int c = 0; c < kRows; ++c)
+                    if (c < from || c > to) r[c] = 0xff800000u;
+            }
+            float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kRows; ++c) best[c % 4] = fmaxf(best[c % 4], __uint_as_float(r[c]));
+            const float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
+            // P V of the tile before: P and O are free to be written
+            if (j > 0 && !(fine = warp_wait(&o_done, (j - 1) & 1, &lost))) break;
+            // the maximum in use follows only where the new one is more than 2^8 above: P stays below 2^8, and O is seldom rescaled
+            const bool up = (now - top) * p.scale2 > 8.f || top == -INFINITY;
+            if (__any_sync(~0u, up && now != top)) {
+                const float by = up && now != top ? exp2_fast((top - now) * p.scale2) : 1.f;
+                if (up) top = now;
+                sum *= by;
+                if (j > 0) {
+                    fence_after();
+#pragma unroll
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tensor_load(mine + F::kOut + c, o);
+                        wait_loads();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                        tensor_store(mine + F::kOut + c, o);
+                    }
+                }
+            }
+            const float shift = top == -INFINITY ? 0.f : top * p.scale2;
+            float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kRows; c += 64) {
+                uint32_t packed[32];
+#pragma unroll
+                for (int k = 0; k < 64; k += 2) {
+                    const float a = exp2_fast(fmaf(__uint_as_float(r[c + k]), p.scale2, -shift)), b = exp2_fast(fmaf(__uint_as_float(r[c + k + 1]), p.scale2, -shift));
+                    part[k % 4] += a;
+                    part[k % 4 + 1] += b;
+                    packed[k / 2] = pack<T>(a, b);
+                }
+                tensor_store(mine + F::kProb + c / 2, packed);
+            }
+            sum += (part[0] + part[1]) + (part[2] + part[3]);
+            wait_stores();
+            fence_before();
+            barrier_arrive(&p_full);
+        }
+        fine = fine && warp_wait(&o_done, (count - 1) & 1, &lost);
+        fence_after();
+        T* out = live ? static_cast<T*>(p.out) + ((int64_t)i * p.heads_q + head) * p.dim : nullptr;
+        store_row<T, DP>(mine + F::kOut, fine ? 1.f / sum : nan_value(), p.dim, out);
+        if (live && p.lse != nullptr) p.lse[head * p.pitch + i] = fine ? fmaf(top, p.scale2, log2f(sum)) : nan_value();
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 5) tensor_free<256>(tensor);
+}
+
+// ---- backwards: gradients of the queries -------------------------------------------------------------------------------
+template <int DP> struct Queries {
+    static constexpr int kStages = DP == 64 ? 3 : 1;
+    static constexpr bool kApart = DP == 64;
+    static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
+    static constexpr int kShared = 2 * kTile + 2 * kStages * kPart + 1024;
+    static constexpr int kGrad = kStream, kOut = 2 * kStream, kProb = kApart ? 2 * kStream + DP : 0;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
+                                                               const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
+    using F = Queries<DP>;
+    __shared__ uint64_t q_full, full[F::kStages], empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ uint32_t tensor;
+    __shared__ int lost;
+    unsigned char* const shared = aligned_shared();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int tiles = (int)((p.tokens + kRows - 1) / kRows), tile = tiles - 1 - (int)(blockIdx.x / p.heads_q), head = blockIdx.x % p.heads_q;
+    const int key_head = head / (p.heads_q / p.heads_k);
+    const int i0 = tile * kRows, last = (int)min((int64_t)i0 + kRows, p.tokens) - 1;
+    const int j0 = first_key(p, i0), count = (last - j0) / kStream + 1;
+    if (threadIdx.x == 0) {
+        lost = 0;
+        barrier_init(&q_full, 1);
+        for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
+        barrier_init(&s_full, 1);
+        barrier_init(&p_full, kRows);
+        barrier_init(&o_done, 1);
+        barrier_init(&ended, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 5) tensor_alloc<256>(&tensor);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t base = tensor, q_at = shared_address(shared), do_at = q_at + F::kTile, kv_at = do_at + F::kTile;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            barrier_expect(&q_full, 2 * F::kTile);
+            load_panels<kRows, DP>(shared, &map_q, &q_full, head, i0);
+            load_panels<kRows, DP>(shared + F::kTile, &map_do, &q_full, head, i0);
+            int j = 0;
+            for (; j < count; ++j) {
+                const int s = j % F::kStages, turn = j / F::kStages;
+                if (turn > 0 && !barrier_wait(&empty[s], (turn - 1) & 1, &lost)) break;
+                barrier_expect(&full[s], 2 * F::kPart);
+                unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
+                load_panels<kStream, DP>(to, &map_k, &full[s], key_head, j0 + j * kStream);
+                load_panels<kStream, DP>(to + F::kPart, &map_v, &full[s], key_head, j0 + j * kStream);
+            }
+            drain(&q_full, 0);
+            for (int b = max(0, j - F::kStages); b < j; ++b) drain(&full[b % F::kStages], b / F::kStages & 1);
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            bool fine = barrier_wait(&q_full, 0, &lost);
+            auto scores = [&](int j) {
+                const int s = j % F::kStages;
+                if (!barrier_wait(&full[s], j / F::kStages & 1, &lost)) return false;
+                fence_after();
+                multiply_rows<T, kStream, DP>(base, q_at, kv_at + 2 * s * F::kPart);
+                multiply_rows<T, kStream, DP>(base + F::kGrad, do_at, kv_at + (2 * s + 1) * F::kPart);
+                commit(&s_full);
+                return true;
+            };
+            fine = fine && scores(0);
+            for (int j = 0; fine && j < count; ++j) {
+                const int s = j % F::kStages;
+                if (!barrier_wait(&p_full, j & 1, &lost)) break;
+                fence_after();
+                if (F::kApart && j + 1 < count && !(fine = scores(j + 1))) break;
+                multiply_columns<T, kStream, DP>(base + F::kOut, base + F::kProb, kv_at + 2 * s * F::kPart, j != 0);
+                commit(&empty[s]);
+                commit(&o_done);
+                if (!F::kApart && j + 1 < count) fine = barrier_wait(&o_done, j & 1, &lost) && scores(j + 1);
+            }
+            commit(&ended);
+            drain(&ended, 0);
+        }
+    } else {
+        const int i = i0 + threadIdx.x;
+        const bool live = i < p.tokens;
+        const int low = live ? first_key(p, i) : 0, high = live ? i : -1;
+        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
+        // D = dO . O of the thread's row, which the keys' kernel reads after this one
+        float delta = 0.f, lse = 0.f;
+        if (live) {
+            const int64_t at = ((int64_t)i * p.heads_q + head) * p.dim;
+            const uint4 *o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + at), *g = reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout) + at);
+#pragma unroll 4
+            for (int c = 0; c < p.dim / 8; ++c) {
+                const uint4 a = o[c], b = g[c];
+                float u[8], v[8];
+                unpack<T, 8>(a, u);
+                unpack<T, 8>(b, v);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
+            }
+            lse = p.lse[head * p.pitch + i];
+            p.delta[head * p.pitch + i] = delta;
+        }
+        bool fine = true;
+        for (int j = 0; j < count; ++j) {
+            const int k0 = j0 + j * kStream;
+            if (!(fine = warp_wait(&s_full, j & 1, &lost))) break;
+            fence_after();
+            uint32_t r[kStream], d[kStream], packed[kStream / 2];
+#pragma unroll
+            for (int c = 0; c < kStream; c += 32) { tensor_load(mine + c, r + c); tensor_load(mine + F::kGrad + c, d + c); }
+            wait_loads();
+#pragma unroll
+            for (int c = 0; c < kStream; ++c) {
+                const float prob = exp2_fast(fmaf(__uint_as_float(r[c]), p.scale2, -lse));
+                r[c] = __float_as_uint(prob * (__uint_as_float(d[c]) - delta));
+            }
+            if (!__all_sync(~0u, k0 >= low && k0 + kStream - 1 <= high)) {
+                const int from = low - k0, to = high - k0;
+#pragma unroll
+                for (int c = 0; c < kStream; ++c)
+                    if (c < from || c > to) r[c] = 0u;
+            }
+#pragma unroll
+            for (int c = 0; c < kStream; c += 2) packed[c / 2] = pack<T>(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+            if (F::kApart && j > 0 && !(fine = warp_wait(&o_done, (j - 1) & 1, &lost))) break;
+            tensor_store(mine + F::kProb, packed);
+            wait_stores();
+            fence_before();
+            barrier_arrive(&p_full);
+        }
+        fine = fine && warp_wait(&o_done, (count - 1) & 1, &lost);
+        fence_after();
+        T* out = live ? static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + head) * p.dim : nullptr;
+        store_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), p.dim, out);
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 5) tensor_free<256>(tensor);
+}
+
+// ---- backwards: gradients of keys and values ----------------------------------------------------------------------------
+template <int DP> struct Keys {
+    static constexpr int kStages = DP == 64 ? 3 : 2;
+    static constexpr bool kApart = DP == 128;           // one block to an SM has columns to spare, two have not
+    static constexpr int kColumns = DP == 64 ? 256 : 512;
+    static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
+    static constexpr int kShared = 2 * kTile + 2 * kStages * kPart + 1024;
+    static constexpr int kGrad = kStream, kValue = 2 * kStream, kKey = 2 * kStream + DP;
+    static constexpr int kProb = kApart ? 2 * kStream + 2 * DP : 0, kProbGrad = kApart ? kProb + kStream / 2 : kGrad;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
+                                                                            const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
+    using F = Keys<DP>;
+    __shared__ uint64_t k_full, full[F::kStages], empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ __align__(16) float lse[F::kStages][kStream], delta[F::kStages][kStream];
+    __shared__ uint32_t tensor;
+    __shared__ int lost;
+    unsigned char* const shared = aligned_shared();
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int tile = blockIdx.x / p.heads_k, key_head = blockIdx.x % p.heads_k, group = p.heads_q / p.heads_k;        // the longest are the first ones
+    const int j0 = tile * kRows, last = (int)min((int64_t)j0 + kRows, p.tokens) - 1;
+    const int each = (past_query(p, last) - 1 - j0) / kStream + 1, count = each * group;
+    if (threadIdx.x == 0) {
+        lost = 0;
+        barrier_init(&k_full, 1);
+        for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
+        barrier_init(&s_full, 1);
+        barrier_init(&p_full, kRows);
+        barrier_init(&o_done, 1);
+        barrier_init(&ended, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncwarp();
+    if (warp == 5) tensor_alloc<F::kColumns>(&tensor);
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t base = tensor, k_at = shared_address(shared), v_at = k_at + F::kTile, part_at = v_at + F::kTile;
+
+    if (warp == 4) {
+        if (lane == 0) {
+            barrier_expect(&k_full, 2 * F::kTile);
+            load_panels<kRows, DP>(shared, &map_k, &k_full, key_head, j0);
+            load_panels<kRows, DP>(shared + F::kTile, &map_v, &k_full, key_head, j0);
+            int n = 0;
+            for (; n < count; ++n) {
+                const int s = n % F::kStages, turn = n / F::kStages, head = key_head * group + n / each, i = j0 + n % each * kStream;
+                if (turn > 0 && !barrier_wait(&empty[s], (turn - 1) & 1, &lost)) break;
+                barrier_expect(&full[s], 2 * F::kPart + 2 * kStream * 4);
+                unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
+                load_panels<kStream, DP>(to, &map_q, &full[s], head, i);
+                load_panels<kStream, DP>(to + F::kPart, &map_do, &full[s], head, i);
+                load_bytes(lse[s], p.lse + head * p.pitch + i, kStream * 4, &full[s]);
+                load_bytes(delta[s], p.delta + head * p.pitch + i, kStream * 4, &full[s]);
+            }
+            drain(&k_full, 0);
+            for (int b = max(0, n - F::kStages); b < n; ++b) drain(&full[b % F::kStages], b / F::kStages & 1);
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            bool fine = barrier_wait(&k_full, 0, &lost);
+            auto scores = [&](int n) {
+                const int s = n % F::kStages;
+                if (!barrier_wait(&full[s], n / F::kStages & 1, &lost)) return false;
+                fence_after();
+                multiply_rows<T, kStream, DP>(base, k_at, part_at + 2 * s * F::kPart);
+                multiply_rows<T, kStream, DP>(base + F::kGrad, v_at, part_at + (2 * s + 1) * F::kPart);
+                commit(&s_full);
+                return true;
+            };
+            fine = fine && scores(0);
+            for (int n = 0; fine && n < count; ++n) {
+                const int s = n % F::kStages;
+                if (!barrier_wait(&p_full, n & 1, &lost)) break;
+                fence_after();
+                if (F::kApart && n + 1 < count && !(fine = scores(n + 1))) break;
+                multiply_columns<T, kStream, DP>(base + F::kValue, base + F::kProb, part_at + (2 * s + 1) * F::kPart, n != 0);
+                multiply_columns<T, kStream, DP>(base + F::kKey, base + F::kProbGrad, part_at + 2 * s * F::kPart, n != 0);
+                commit(&empty[s]);
+                commit(&o_done);
+                if (!F::kApart && n + 1 < count) fine = barrier_wait(&o_done, n & 1, &lost) && scores(n + 1);
+            }
+            commit(&ended);
+            drain(&ended, 0);
+        }
+    } else {
+        const int j = j0 + threadIdx.x;
+        const bool live = j < p.tokens;
+        const int low = live ? j : 0, high = live ? past_query(p, j) - 1 : -1;          // the queries that see the key
+        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
+        bool fine = true;
+        for (int n = 0; n < count; ++n) {
+            const int s = n % F::kStages, i = j0 + n % each * kStream;
+            // the statistics came with the tile that the scores waited for; this wait makes them visible here, too
+            if (!(fine = warp_wait(&full[s], n / F::kStages & 1, &lost) && warp_wait(&s_full, n & 1, &lost))) break;
+            fence_after();
+            uint32_t r[kStream], d[kStream], packed[kStream / 2];
+#pragma unroll
+            for (int c = 0; c < kStream; c += 32) { tensor_load(mine + c, r + c); tensor_load(mine + F::kGrad + c, d + c); }
+            wait_loads();
+            const float4 *l4 = reinterpret_cast<const float4*>(lse[s]), *d4 = reinterpret_cast<const float4*>(delta[s]);
+#pragma unroll
+            for (int c = 0; c < kStream; c += 4) {
+                const float4 l = l4[c / 4], e = d4[c / 4];
+                const float ls[4] = {l.x, l.y, l.z, l.w}, es[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float prob = exp2_fast(fmaf(__uint_as_float(r[c + k]), p.scale2, -ls[k]));
+                    r[c + k] = __float_as_uint(prob);
+                    d[c + k] = __float_as_uint(prob * (__uint_as_float(d[c + k]) - es[k]));
+                }
+            }
+            if (!__all_sync(~0u, i >= low && i + kStream - 1 <= high)) {
+                const int from = low - i, to = high - i;
+#pragma unroll
+                for (int c = 0; c < kStream; ++c)
+                    if (c < from || c > to) r[c] = d[c] = 0u;
+            }
+            if (F::kApart && n > 0 && !(fine = warp_wait(&o_done, (n - 1) & 1, &lost))) break;
+#pragma unroll
+            for (int c = 0; c < kStream; c += 2) packed[c / 2] = pack<T>(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+            tensor_store(mine + F::kProb, packed);
+#pragma unroll
+            for (int c = 0; c < kStream; c += 2) packed[c / 2] = pack<T>(__uint_as_float(d[c]), __uint_as_float(d[c + 1]));
+            tensor_store(mine + F::kProbGrad, packed);
+            wait_stores();
+            fence_before();
+            barrier_arrive(&p_full);
+        }
+        fine = fine && warp_wait(&o_done, (count - 1) & 1, &lost);
+        fence_after();
+        const int64_t at = ((int64_t)j * p.heads_k + key_head) * p.dim;
+        store_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), p.dim, live ? static_cast<T*>(p.dv) + at : nullptr);
+        store_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), p.dim, live ? static_cast<T*>(p.dk) + at : nullptr);
+    }
+    __syncwarp();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    if (warp == 5) tensor_free<F::kColumns>(tensor);
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------------
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                 CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+static EncodeTiled encoder() {
+    static const EncodeTiled found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult how;
+        return cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &how) == cudaSuccess && how == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiled>(f) : nullptr;
+    }();
+    return found;
+}
+
+// tokens x heads x dim; what lies outside is read as 0, columns behind dim among it
+static bool map_of(CUtensorMap* map, uint32_t dtype, const void* p, int64_t dim, int64_t heads, int64_t tokens, int64_t head_stride, int64_t stride, int rows) {
+    const cuuint64_t sizes[3] = {(cuuint64_t)dim, (cuuint64_t)heads, (cuuint64_t)tokens};
+    const cuuint64_t strides[2] = {(cuuint64_t)(heads > 1 ? head_stride * 2 : dim * 2), (cuuint64_t)(tokens > 1 ? stride * 2 : dim * heads * 2)};
+    const cuuint32_t box[3] = {64, 1, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
+    return encoder()(map, dtype == NUKA_B200_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), sizes, strides, box, steps,
+                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int64_t attention_pitch(int64_t tokens) { return (tokens + kRows - 1) / kRows * kRows; }
+
+template <typename K> static cudaError_t with_shared(K kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
+
+template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_attention_t& d, bool backward, cudaStream_t stream) {
+    AttentionParams p{};
+    const nuka_b200_episodes_t& e = *d.plan;
+    p.first = e.first; p.end = e.end; p.tokens = e.tokens; p.pitch = attention_pitch(e.tokens);
+    p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens);
+    p.scale = d.scale; p.scale2 = d.scale * kLog2e;
+    p.out = d.out; p.lse = d.lse; p.dout = d.dout; p.delta = d.delta; p.dq = d.dq; p.dk = d.dk; p.dv = d.dv;
+    if (encoder() == nullptr) return cudaErrorNotSupported;
+    const int64_t tiles = (e.tokens + kRows - 1) / kRows;
+    CUtensorMap q, k, v, g;
+    if (!backward) {
+        // first, because it makes the device's context the thread's own: maps cannot be encoded without one
+        cudaError_t set = with_shared(attention_kernel<T, DP>, Forward<DP>::kShared);
+        if (set != cudaSuccess) return set;
+        if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, kRows) || !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, kRows) ||
+            !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, kRows)) return cudaErrorInvalidValue;
+        attention_kernel<T, DP><<<(unsigned)(tiles * d.heads_q), kBlock, Forward<DP>::kShared, stream>>>(q, k, v, p);
+        return cudaGetLastError();
+    }
+    for (int keys = 0; keys < 2; ++keys) {
+        const int own = keys ? kStream : kRows, other = keys ? kRows : kStream;
+        cudaError_t set = keys ? with_shared(key_grad_kernel<T, DP>, Keys<DP>::kShared) : with_shared(query_grad_kernel<T, DP>, Queries<DP>::kShared);
+        if (set != cudaSuccess) return set;
+        if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, own) || !map_of(&g, d.dtype, d.dout, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, own) ||
+            !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, other) || !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, other))
+            return cudaErrorInvalidValue;
+        if (keys) key_grad_kernel<T, DP><<<(unsigned)(tiles * d.heads_k), kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, p);
+        else query_grad_kernel<T, DP><<<(unsigned)(tiles * d.heads_q), kBlock, Queries<DP>::kShared, stream>>>(q, g, k, v, p);
+        set = cudaGetLastError();
+        if (set != cudaSuccess) return set;
+    }
+    return cudaSuccess;
+}
+
+cudaError_t launch_attention(const nuka_b200_attention_t& d, bool backward, cudaStream_t stream) {
+    if (d.plan->tokens == 0) return cudaSuccess;
+    if (d.dtype == NUKA_B200_F16) return d.dim <= 64 ? run_attention<__half, 64>(d, backward, stream) : run_attention<__half, 128>(d, backward, stream);
+    return d.dim <= 64 ? run_attention<__nv_bfloat16, 64>(d, backward, stream) : run_attention<__nv_bfloat16, 128>(d, backward, stream);
+}
+
+}  // namespace nkb

@@ -20,4 +20,7 @@ cudaError_t launch_recurrence_step(uint32_t dtype, int64_t n, int64_t channels, 
 uint64_t heads_workspace(int64_t tokens, int64_t dim);
 cudaError_t launch_heads(const nuka_b200_heads_t& d, bool backward, cudaStream_t stream);
 
+int64_t attention_pitch(int64_t tokens);
+cudaError_t launch_attention(const nuka_b200_attention_t& d, bool backward, cudaStream_t stream);
+
 }  // namespace nkb

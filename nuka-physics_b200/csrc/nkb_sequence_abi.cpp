@@ -118,4 +118,36 @@ static nuka_result_t Heads(const nuka_b200_heads_t* desc, bool backward, void* s
 nuka_result_t nuka_b200_heads(const nuka_b200_heads_t* desc, void* stream) { return Heads(desc, false, stream); }
 nuka_result_t nuka_b200_heads_backward(const nuka_b200_heads_t* desc, void* stream) { return Heads(desc, true, stream); }
 
+int64_t nuka_b200_attention_pitch(int64_t tokens) { return tokens <= 0 ? 0 : nkb::attention_pitch(tokens); }
+
+static nuka_result_t Attention(const nuka_b200_attention_t* desc, bool backward, void* stream) {
+    if (desc == nullptr) return Invalid("attention desc is null");
+    const nuka_b200_attention_t& d = *desc;
+    if (const char* fault = PlanFault(d.plan)) return Invalid(fault);
+    if (d.dtype != NUKA_B200_F16 && d.dtype != NUKA_B200_BF16) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dtype must be F16 or BF16");
+    if (d.heads_k < 1 || d.heads_q < 1 || d.heads_q > 65536 || d.heads_q % d.heads_k != 0) return Invalid("heads_q must be a positive multiple of heads_k, at most 65536");
+    if (d.dim < 8 || d.dim > 128 || d.dim % 8 != 0) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dim must be a multiple of 8, 8 to 128");
+    if (d.window < 0) return Invalid("window must not be negative");
+    if (!(d.scale > 0.f) || d.scale > 3.0e38f) return Invalid("scale must be greater than 0 and finite");
+    if (d.plan->tokens == 0) return NUKA_RESULT_OK;
+    if ((d.plan->tokens / 128 + 1) * d.heads_q > (1ll << 31) - 1) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times heads");
+    for (const void* p : {d.q, d.k, d.v, static_cast<const void*>(d.out)}) {
+        if (p == nullptr) return Invalid("q, k, v or out is null");
+        if (!Aligned(p, 16)) return Invalid("a tensor does not lie on 16 bytes");
+    }
+    if (!Aligned(d.lse, 16) || (backward && (d.lse == nullptr || d.delta == nullptr || !Aligned(d.delta, 16)))) return Invalid("lse or delta is null or not on 16 bytes");
+    if (backward)
+        for (const void* p : {d.dout, static_cast<const void*>(d.dq), static_cast<const void*>(d.dk), static_cast<const void*>(d.dv)})
+            if (p == nullptr || !Aligned(p, 16)) return Invalid("a gradient is null or not on 16 bytes");
+    // a size of 1 has no stride
+    const struct { int64_t size, stride; } strides[] = {{d.plan->tokens, d.q_stride}, {d.heads_q, d.q_head_stride}, {d.plan->tokens, d.k_stride}, {d.heads_k, d.k_head_stride},
+                                                        {d.plan->tokens, d.v_stride}, {d.heads_k, d.v_head_stride}};
+    for (const auto& s : strides)
+        if (s.size > 1 && (s.stride < d.dim || s.stride % 8 != 0 || s.stride >= (1ll << 38))) return Invalid("strides must be multiples of 8 values, at least dim");
+    return Ran(nkb::launch_attention(d, backward, StreamOf(stream)));
+}
+
+nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, false, stream); }
+nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, true, stream); }
+
 }  // extern "C"

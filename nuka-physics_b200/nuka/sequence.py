@@ -7,6 +7,7 @@ every env, for acting:
     over a rollout (training)                      one token of every env (acting)
     gated_recurrence(x, gate, episodes, initial)   gated_recurrence_step(x, gate, state, fresh)
     rotate_heads(q, k, ..., episodes, ...)         rotate_heads(q, k, ..., positions, ...)
+    episode_attention(q, k, v, episodes)           history_attention(q, k, v, cache)
 
 Tensors live on one GPU; the work is enqueued on torch's current stream of that GPU and nothing waits for it.  Operators over
 rollouts take part in automatic differentiation (once).  Needs torch with CUDA.
@@ -61,10 +62,12 @@ def _stride(tensor, dim):
     return tensor.stride(dim) if tensor.shape[dim] > 1 else 0
 
 
-def _channels_last(tensor, multiple=1, size=1):
-    """The tensor as it is where its last dimension is contiguous, its strides are multiples of `multiple` values and it lies on `size` bytes, else a copy."""
+def _channels_last(tensor, multiple=1, size=1, least=0):
+    """The tensor as it is where its last dimension is contiguous, its other strides are multiples of `multiple` values and at least `least`, and it lies on
+    `size` bytes, else a copy."""
     last = tensor.dim() - 1
-    if (tensor.shape[last] == 1 or tensor.stride(last) == 1) and tensor.data_ptr() % size == 0 and all(_stride(tensor, d) % multiple == 0 for d in range(last)):
+    if ((tensor.shape[last] == 1 or tensor.stride(last) == 1) and tensor.data_ptr() % size == 0
+            and all(tensor.shape[d] <= 1 or (tensor.stride(d) % multiple == 0 and tensor.stride(d) >= least) for d in range(last))):
         return tensor
     return tensor.clone(memory_format=torch.contiguous_format)
 
@@ -272,3 +275,50 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
         first, positions = None, positions.contiguous()
     q_weight, k_weight, frequencies = (None if x is None else x.contiguous() for x in (q_weight, k_weight, frequencies))
     return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
+
+
+# ---- attention over packed episodes --------------------------------------------------------------------------------
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, episodes, scale, window):
+        device = q.device
+        q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        lib = _abi.lib()
+        lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device)
+        desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
+                                  _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), lse.data_ptr())
+        _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
+        # the descriptor's arrays stay alive with what is saved here
+        ctx.save_for_backward(q, k, v, out, lse)
+        ctx.desc, ctx.episodes = desc, episodes
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, out, lse = ctx.saved_tensors
+        device, desc = q.device, ctx.desc
+        dout = _channels_last(dout.contiguous(), 1, 16)
+        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
+        delta = torch.empty_like(lse)
+        desc.dout, desc.delta, desc.dq, desc.dk, desc.dv = dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+        _call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc))
+        return dq, dk, dv, None, None, None
+
+
+def episode_attention(q, k, v, episodes, scale=None, window=None):
+    """Causal attention over each episode: a token sees itself and the tokens of its episode before it, with `window` at most the last `window` of these.
+
+    q: tokens x heads x dim, k and v: tokens x key heads x dim, f16 or bf16, tokens and heads at any stride (views of one projection); the heads are a multiple
+    of the key heads, and as many heads share one key head.  dim: a multiple of 8, at most 128 (64 and 128 waste nothing).  scale: dim^-0.5 unless given.
+    Returns tokens x heads x dim.  Sums and statistics are in 32 bits; probabilities and, backwards, their gradients are rounded to the inputs' type, so train in f16 with a
+    loss scale."""
+    _on_gpu(q, k, v, episodes._plan)
+    _dtype(q, (torch.float16, torch.bfloat16), "q")
+    for x, what in ((q, "q"), (k, "k"), (v, "v")):
+        _tokens_of(x, episodes, 3, what)
+    _expect(k.dtype == q.dtype and v.dtype == q.dtype and k.shape == v.shape and k.shape[2] == q.shape[2], "q, k and v must be of one type and dim, k and v of one shape")
+    _expect(k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and q.shape[1] > 0, "the heads must be a multiple of the key heads")
+    _expect(window is None or window >= 1, "window must be at least 1")
+    return _Attention.apply(q, k, v, episodes, q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window))

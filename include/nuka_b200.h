@@ -410,7 +410,8 @@ nuka_result_t nuka_b200_recurrence_step(uint32_t dtype, int64_t n, int64_t chann
 
 /* Queries and keys of every head: divided by their root mean square over the head's dim values (mean square plus eps), times a weight
  * per column (float, NULL = 1), then turned by the token's position: of the first `turned` columns the pairs (i, i + turned / 2), or with interleaved != 0
- * (2 i, 2 i + 1), turn by the angle position x frequencies[i] radians (double, turned / 2 of them, so that long contexts keep their low bits).
+ * (2 i, 2 i + 1), turn by the angle position x frequencies[i] radians (double, turned / 2 of them), factors
+ * and product rounded to 32 bits.
  * position[t] is t - plan->first[t], or positions[t] where positions is not NULL.  dim and turned are multiples of 8, dim at most 256.
  * The backward call takes dq_out / dk_out, writes dq / dk (contiguous) and the weights' gradients (float, NULL = not wanted). */
 typedef struct nuka_b200_heads_t {
@@ -455,6 +456,28 @@ typedef struct nuka_b200_attention_t {
 int64_t nuka_b200_attention_pitch(int64_t tokens);
 nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream);
 nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream);
+
+/* Attention of one token of each env over the env's cached history, for acting.  keys and values (envs x capacity x heads_k x dim, contiguous, on 16 bytes) are a
+ * ring: the token's k and v are written to place position % capacity, then the token attends to the last min(position + 1, capacity) tokens, itself among
+ * them: what nuka_b200_attention gives with window = capacity.  position[env]: the token's number in its episode (below 0 counts as 0).  Types, dims, strides and the heads'
+ * groups as in nuka_b200_attention; strides may also be 0.  The workspace (nuka_b200_history_workspace() bytes on 16 bytes, 0 bytes where an env is one block's work) is zeroed
+ * once by the caller and kept for all later calls of these sizes; calls that share it, or a cache, must not run at the same time. */
+typedef struct nuka_b200_history_t {
+    uint32_t dtype;
+    int64_t envs, capacity, heads_q, heads_k, dim;
+    float scale;
+    const void *q, *k, *v;                          /* envs x heads x dim */
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    void *keys, *values;
+    const int32_t* position;
+    void* out;                                      /* envs x heads_q x dim, contiguous */
+    void* workspace;
+    uint64_t workspace_bytes;
+} nuka_b200_history_t;
+uint64_t nuka_b200_history_workspace(const nuka_b200_history_t* desc);
+nuka_result_t nuka_b200_history(const nuka_b200_history_t* desc, void* stream);
+/* position[env] = 0 where fresh[env] != 0 (NULL = nowhere), else one more than it was: the next token of every env. */
+nuka_result_t nuka_b200_history_advance(int32_t* position, const uint8_t* fresh, int64_t envs, void* stream);
 
 #ifdef __cplusplus
 }

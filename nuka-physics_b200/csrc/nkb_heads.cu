@@ -143,8 +143,9 @@ __global__ void __launch_bounds__(kThreads) heads_kernel(const HeadsParams p) {
             const int token = k / half;
             const int64_t t = t0 + token;
             const int32_t position = p.positions != nullptr ? p.positions[t] : (int32_t)(t - p.first[t]);
-            // in turns and in 64 bits, of which only the fraction of a turn is kept: positions of a million turn as exactly as small ones
-            double turns = (double)position * p.frequencies[k - token * half] * 0.15915494309189533577;
+            // The angle is the product in 32 bits, as programs have it that keep it in 32 bits: what they trained fits.  Of that angle in turns, taken in 64 bits,
+            // only the fraction is kept, so its sine and cosine are exact to 32 bits however large it is.
+            double turns = (double)((float)position * (float)p.frequencies[k - token * half]) * 0.15915494309189533577;
             turns -= rint(turns);
             float s, c;
             sincospif(2.f * (float)turns, &s, &c);

@@ -150,4 +150,41 @@ static nuka_result_t Attention(const nuka_b200_attention_t* desc, bool backward,
 nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, false, stream); }
 nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, true, stream); }
 
+static const char* HistoryFault(const nuka_b200_history_t& d) {
+    if (d.envs < 0 || d.envs > kMostTokens || d.capacity < 1 || d.capacity > (1 << 30)) return "envs must not be negative, capacity 1 to 2^30";
+    if (d.heads_k < 1 || d.heads_q < 1 || d.heads_q > 65536 || d.heads_q % d.heads_k != 0) return "heads_q must be a positive multiple of heads_k, at most 65536";
+    return nullptr;
+}
+
+uint64_t nuka_b200_history_workspace(const nuka_b200_history_t* desc) {
+    return desc == nullptr || HistoryFault(*desc) != nullptr || desc->envs == 0 ? 0u : nkb::history_workspace(*desc);
+}
+
+nuka_result_t nuka_b200_history(const nuka_b200_history_t* desc, void* stream) {
+    if (desc == nullptr) return Invalid("history desc is null");
+    const nuka_b200_history_t& d = *desc;
+    if (d.dtype != NUKA_B200_F16 && d.dtype != NUKA_B200_BF16) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dtype must be F16 or BF16");
+    if (const char* fault = HistoryFault(d)) return Invalid(fault);
+    if (d.dim < 8 || d.dim > 128 || d.dim % 8 != 0) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dim must be a multiple of 8, 8 to 128");
+    if (!(d.scale > 0.f) || d.scale > 3.0e38f) return Invalid("scale must be greater than 0 and finite");
+    if (d.envs == 0) return NUKA_RESULT_OK;
+    if (d.envs * d.heads_q > (1ll << 31) - 1024) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many envs times heads");
+    for (const void* p : {d.q, d.k, d.v, static_cast<const void*>(d.keys), static_cast<const void*>(d.values), static_cast<const void*>(d.out)}) {
+        if (p == nullptr) return Invalid("q, k, v, keys, values or out is null");
+        if (!Aligned(p, 16)) return Invalid("a tensor does not lie on 16 bytes");
+    }
+    if (d.position == nullptr || !Aligned(d.position, 4)) return Invalid("position is null or not on 4 bytes");
+    for (int64_t s : {d.q_stride, d.q_head_stride, d.k_stride, d.k_head_stride, d.v_stride, d.v_head_stride})
+        if (s < 0 || s % 8 != 0) return Invalid("strides must be multiples of 8 values, not negative");
+    const uint64_t need = nkb::history_workspace(d);
+    if (need != 0u && (d.workspace == nullptr || d.workspace_bytes < need || !Aligned(d.workspace, 16))) return Invalid("the workspace is null, too small or not on 16 bytes");
+    return Ran(nkb::launch_history(d, StreamOf(stream)));
+}
+
+nuka_result_t nuka_b200_history_advance(int32_t* position, const uint8_t* fresh, int64_t envs, void* stream) {
+    if (envs < 0 || envs > kMostTokens) return Invalid("envs are negative or too many");
+    if (envs != 0 && (position == nullptr || !Aligned(position, 4))) return Invalid("position is null or not on 4 bytes");
+    return Ran(nkb::launch_history_advance(position, fresh, envs, StreamOf(stream)));
+}
+
 }  // extern "C"

@@ -90,6 +90,13 @@ class AttentionDesc(ctypes.Structure):
                 ("delta", ctypes.c_void_p), ("dq", ctypes.c_void_p), ("dk", ctypes.c_void_p), ("dv", ctypes.c_void_p)]
 
 
+class HistoryDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("envs", ctypes.c_int64), ("capacity", ctypes.c_int64), ("heads_q", ctypes.c_int64), ("heads_k", ctypes.c_int64), ("dim", ctypes.c_int64),
+                ("scale", ctypes.c_float), ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64), ("q_head_stride", ctypes.c_int64),
+                ("k_stride", ctypes.c_int64), ("k_head_stride", ctypes.c_int64), ("v_stride", ctypes.c_int64), ("v_head_stride", ctypes.c_int64), ("keys", ctypes.c_void_p),
+                ("values", ctypes.c_void_p), ("position", ctypes.c_void_p), ("out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
 EXPORTS = [
     "nuka_get_version", "nuka_result_message", "nuka_last_error_message", "nuka_device_create", "nuka_device_destroy",
     "nuka_world_create_from_scene", "nuka_world_destroy", "nuka_world_step", "nuka_world_step_n", "nuka_world_set_execution_mode",
@@ -103,6 +110,7 @@ EXPORTS = [
     "nuka_world_get_dof_name", "nuka_b200_episodes_from_offsets", "nuka_b200_episodes_from_done", "nuka_b200_recurrence_workspace", "nuka_b200_recurrence",
     "nuka_b200_recurrence_backward", "nuka_b200_recurrence_step", "nuka_b200_heads_workspace", "nuka_b200_heads", "nuka_b200_heads_backward",
     "nuka_b200_attention_pitch", "nuka_b200_attention", "nuka_b200_attention_backward",
+    "nuka_b200_history_workspace", "nuka_b200_history", "nuka_b200_history_advance",
 ]
 
 _LIB = None
@@ -186,5 +194,9 @@ def lib():
     L.nuka_b200_attention_pitch.restype = i64
     L.nuka_b200_attention.argtypes = [ctypes.POINTER(AttentionDesc), vp]
     L.nuka_b200_attention_backward.argtypes = [ctypes.POINTER(AttentionDesc), vp]
+    L.nuka_b200_history_workspace.argtypes = [ctypes.POINTER(HistoryDesc)]
+    L.nuka_b200_history_workspace.restype = u64
+    L.nuka_b200_history.argtypes = [ctypes.POINTER(HistoryDesc), vp]
+    L.nuka_b200_history_advance.argtypes = [vp, vp, i64, vp]
     _LIB = L
     return L

@@ -258,7 +258,7 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
 
     q: tokens x heads x dim, k: tokens x key heads x dim, f32, f16 or bf16, heads and tokens at any stride (views of one projection).  q_weight, k_weight: dim f32, or None.
     positions: an ``Episodes`` (each token's number in its episode) or int32 per token.  frequencies: float64 on the GPU, one per turned pair
-    (``rotary_frequencies``; twice as many columns are turned, the others only normed), or None.  Pairs are (i, i + turned / 2), or with `interleaved` (2 i, 2 i + 1).
+    (``rotary_frequencies``; twice as many columns are turned, the others only normed), or None; the angle is their product in 32 bits.  Pairs are (i, i + turned / 2), or with `interleaved` (2 i, 2 i + 1).
     dim and the number of turned columns are multiples of 8, dim at most 256.  Returns (q, k), contiguous."""
     episodes = positions if isinstance(positions, Episodes) else None
     _on_gpu(q, k, q_weight, k_weight, frequencies, episodes._plan if episodes is not None else positions)
@@ -322,3 +322,59 @@ def episode_attention(q, k, v, episodes, scale=None, window=None):
     _expect(k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and q.shape[1] > 0, "the heads must be a multiple of the key heads")
     _expect(window is None or window >= 1, "window must be at least 1")
     return _Attention.apply(q, k, v, episodes, q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window))
+
+
+# ---- attention of one token over a cached history ------------------------------------------------------------------
+class HistoryCache:
+    """Keys and values of the last `capacity` tokens of each env, for one layer: a ring of envs x capacity x key heads x dim.
+
+    ``position`` (envs, int32) is the number of each env's present token in its episode; ``advance(fresh)`` moves on to the next token of every env.  Layers of one
+    policy share it: give one cache's ``position`` to the others and advance once per control step.  `buffers`: (keys, values, position) to use in place of new ones."""
+
+    def __init__(self, envs, capacity, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", position=None, buffers=None):
+        _expect(dtype in (torch.float16, torch.bfloat16), "dtype must be float16 or bfloat16")
+        _expect(envs >= 0 and capacity >= 1 and kv_heads >= 1 and head_dim >= 8, "envs must not be negative, capacity and kv_heads at least 1, head_dim at least 8")
+        shape = (int(envs), int(capacity), int(kv_heads), int(head_dim))
+        if buffers is None:
+            buffers = (torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
+                       torch.full(shape[:1], -1, dtype=torch.int32, device=device) if position is None else position)
+        self.keys, self.values, self.position = buffers
+        self.device = _on_gpu(*buffers)
+        for x in buffers[:2]:
+            _expect(tuple(x.shape) == shape and x.dtype == dtype and x.is_contiguous(), f"keys and values must be contiguous, {shape} {dtype}")
+        _expect(tuple(self.position.shape) == shape[:1] and self.position.dtype == torch.int32 and self.position.is_contiguous(), "position must be contiguous int32, one per env")
+        self._workspaces = {}                   # per number of heads
+
+    def advance(self, fresh=None):
+        """The next token of every env; envs with `fresh` set (envs, bool or uint8) begin an episode and forget what they held."""
+        if fresh is not None:
+            fresh = _flags(fresh, tuple(self.position.shape), self.device, "fresh")
+        _call(self.device, _abi.lib().nuka_b200_history_advance, self.position.data_ptr(), _ptr(fresh), self.position.numel())
+
+    def _workspace(self, desc):
+        found = self._workspaces.get(desc.heads_q)
+        if found is None:
+            need = _abi.lib().nuka_b200_history_workspace(ctypes.byref(desc))
+            found = self._workspaces[desc.heads_q] = torch.zeros(need, dtype=torch.uint8, device=self.device)
+        return found
+
+
+def history_attention(q, k, v, cache, scale=None):
+    """Attention of one token of each env over what `cache` holds of its episode, the token itself among it: what ``episode_attention`` gives for the
+    episode's last token, with the cache's capacity as the window.  q: envs x heads x dim, k and v: envs x key heads x dim, in the cache's type, at any stride; k and v are
+    written into the cache.  scale: dim^-0.5 unless given.  Returns envs x heads x dim.  No gradient."""
+    device = _on_gpu(q, k, v, cache.keys)
+    envs, capacity, heads_k, dim = cache.keys.shape
+    dtype = cache.keys.dtype
+    _expect(q.dim() == 3 and q.shape[0] == envs and q.shape[2] == dim and q.shape[1] > 0 and q.shape[1] % heads_k == 0, f"q must be {envs} x a multiple of {heads_k} x {dim}")
+    _expect(tuple(k.shape) == (envs, heads_k, dim) and v.shape == k.shape, f"k and v must be {envs} x {heads_k} x {dim}")
+    _expect(q.dtype == dtype and k.dtype == dtype and v.dtype == dtype, f"q, k and v must be {dtype}, as the cache is")
+    q, k, v = (_channels_last(x, 8, 16) for x in (q, k, v))
+    out = torch.empty(q.shape, dtype=dtype, device=device)
+    desc = _abi.HistoryDesc(_DTYPES[dtype], envs, capacity, q.shape[1], heads_k, dim, dim ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                            _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), cache.keys.data_ptr(), cache.values.data_ptr(),
+                            cache.position.data_ptr(), out.data_ptr())
+    workspace = cache._workspace(desc)
+    desc.workspace, desc.workspace_bytes = workspace.data_ptr() or None, workspace.numel()
+    _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
+    return out

@@ -263,7 +263,7 @@ def _heads_64(x, w, position, frequencies, eps, interleaved):
     y = x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
     if w is not None:
         y = y * w
-    angle = position.double()[:, None, None] * frequencies
+    angle = (position.float()[:, None, None] * frequencies.float()).double()         # the definition: a product in 32 bits
     u, v = (y[..., 0:n:2], y[..., 1:n:2]) if interleaved else (y[..., :n // 2], y[..., n // 2:n])
     a, b = u * angle.cos() - v * angle.sin(), u * angle.sin() + v * angle.cos()
     return torch.cat([torch.stack([a, b], -1).flatten(-2) if interleaved else torch.cat([a, b], -1), y[..., n:]], -1)
@@ -296,8 +296,8 @@ def test_heads_and_their_gradient(dtype, dim, turned, interleaved, lengths, head
         _close(dw, want_dw, ulps * math.sqrt(n * x.shape[1]) * (dy.double().abs().max() * 4), "dw" + name)
 
 
-def test_heads_far_positions_keep_their_low_bits():
-    """Positions of a million turn as exactly as small ones: the angle is worked out in 64 bits."""
+def test_heads_at_far_positions():
+    """Sines and cosines of angles of millions are as exact as those of small ones: whole turns are taken off in 64 bits."""
     f = S.rotary_frequencies(64).cuda()
     q = _normal(_gen(11), 5, 2, 64)
     positions = torch.tensor([0, 1, 131071, 1000003, 2 ** 31 - 1], dtype=torch.int32, device="cuda")

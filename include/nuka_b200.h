@@ -375,11 +375,12 @@ enum { NUKA_B200_F32 = 0, NUKA_B200_F16 = 1, NUKA_B200_BF16 = 2 };
 typedef struct nuka_b200_episodes_t {
     int32_t *first, *end, *link, *tail;
     int64_t tokens, rows;
+    int64_t length;                                 /* of every row where all have the same, else 0: only how work is dealt out depends on it */
 } nuka_b200_episodes_t;
 /* Rows are whole episodes: row r holds the tokens [offsets[r], offsets[r + 1]); offsets (int32, rows + 1) ascend from 0 to tokens, empty rows allowed.
  * The offsets are read on the device and not checked there: others are clamped so that every index in the plan stays inside the tokens. */
 nuka_result_t nuka_b200_episodes_from_offsets(const nuka_b200_episodes_t* plan, const int32_t* offsets, void* stream);
-/* Rows of tokens / rows tokens each; done[t] != 0 ends an episode with token t. */
+/* Rows of length tokens each, length > 0 unless there are no tokens; done[t] != 0 ends an episode with token t. */
 nuka_result_t nuka_b200_episodes_from_done(const nuka_b200_episodes_t* plan, const uint8_t* done, void* stream);
 
 /* The gated linear recurrence h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(gate_t), channel by channel.  An episode that begins
@@ -401,7 +402,7 @@ typedef struct nuka_b200_recurrence_t {
     void* workspace;                                /* nuka_b200_recurrence_workspace() bytes, 8-byte aligned; may be NULL where that is 0 */
     uint64_t workspace_bytes;
 } nuka_b200_recurrence_t;
-uint64_t nuka_b200_recurrence_workspace(uint32_t dtype, int64_t tokens, int64_t channels);
+uint64_t nuka_b200_recurrence_workspace(const nuka_b200_episodes_t* plan, int64_t channels);
 nuka_result_t nuka_b200_recurrence(const nuka_b200_recurrence_t* desc, void* stream);
 nuka_result_t nuka_b200_recurrence_backward(const nuka_b200_recurrence_t* desc, void* stream);
 /* Its form for one token of each of n envs: state (n x channels float, contiguous) is updated in place, h receives it rounded; envs with fresh[i] != 0 (NULL = none) begin from 0. */

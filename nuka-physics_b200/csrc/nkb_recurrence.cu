@@ -76,331 +76,260 @@ cudaError_t launch_episodes_from_done(const nuka_b200_episodes_t& p, const uint8
 // ---- recurrence ----------------------------------------------------------------------------------------------------
 // Each token maps the state by h -> a h + b; two such maps in a row are one again, (A, B) after (a, b) = (A a, A b + B), which is what makes
 // the scan parallel.  A token that begins an episode forgets the state whatever it was: such a map is *closed* and is never
-// multiplied with what came before, so that an infinity or NaN stays in its episode.
+// multiplied with what came before, so that an infinity or NaN stays in its episode.  Backwards the state is the gradient that goes on to the token before, m -> a (m + b).
 //
-// A block takes a chunk of tokens by 32 * VEC channels, a warp of it TOK tokens, all loaded before the first is used.  Warps join their maps through
-// shared memory, chunks through words in global memory: a chunk's map is published as one 64-bit word per channel that is valid as
-// soon as it is not the fill pattern, so that nobody has to order two stores.  A chunk walks back over the maps of its group of kGroup chunks, to the group's
-// first or to the last closed one, and takes the state that the group before ended with.  Where a walk stops
-// depends on the plan alone, so the same call gives the same bits.  Chunks are handed out by a ticket: a block waits only for chunks
-// whose blocks run already.
-constexpr int kWarps = 8, kGroup = 32;
-constexpr int64_t kWaitCycles = 4000000000ll;           // about 2 s; then the chunk goes on with NaN, and the call ends
-constexpr uint64_t kHeader = 256;                       // ticket
+// A warp walks a segment of tokens one by one, 32 * VEC channels wide, the next tokens' loads under way while it works on the present ones, so an element
+// costs its sigmoid, two multiplications and its loads, and nothing waits for another warp.  Rows of one length that are short or give every SM its share of
+// warps are the segments: each begins with a row, and that is all.  Otherwise the tokens are cut into as many equal segments as fill the GPU and walked twice: first for
+// each segment's map alone, then, when a small scan over the maps has said what state each begins with, for the values.  The inputs are read twice that way (5 tensors' bytes in place
+// of 3 forwards, 8 in place of 6 backwards); chunks that wait for one another's maps read them once, and were slower by more: their waits, a few microseconds for every chunk of 64 tokens, had
+// nothing to hide under (131071 x 1024, bf16: 1.42 ms forwards, against FWD here).  All orders are fixed, so the same call gives the same bits.
 
-__host__ __device__ constexpr int recurrence_chunk(bool backward) { return kWarps * (backward ? 8 : 16); }
+// Channels of a lane; tokens whose loads are under way.
+template <typename T> constexpr int kWide = sizeof(T) == 4 ? 2 : 4;
+template <bool BACKWARD> constexpr int kBatch = BACKWARD ? 4 : 8;
+constexpr int kWalkers = 4;                             // warps of a block
+constexpr float kClosed = -1.f;                         // in the place of A, which is never negative
 
 struct RecurrenceParams {
     nuka_b200_episodes_t plan;
-    int64_t channels, x_stride, gate_stride, padded;
+    int64_t channels, x_stride, gate_stride, segment, segments;
     const void *x, *gate, *dh;
     void *h, *dx, *dgate;
     const float *initial, *dstate;
     float *state, *dinitial;
-    uint32_t* ticket;                                   // null where one chunk holds all tokens
-    unsigned long long* maps;                           // chunks x padded
-    uint32_t* ends;                                     // groups x padded: the state that a group's last chunk ends with
-    uint32_t tiles, chunks;
+    float2* maps;                                       // segments x channels; null where every segment is on its own
+    float* carries;                                     // segments x channels: the state that a segment begins with, in scan order
+    uint32_t tiles;
 };
 
-// 1 / (1 + exp(-g)) and 1 minus it, each without cancellation.  16-bit inputs and outputs leave the fast forms' 2^-21 far below their rounding.
+// 1 / (1 + exp(-g)) and 1 minus it, each without cancellation.  16-bit inputs and outputs leave the fast form's 2^-21 far below their rounding; its clamp
+// keeps exp(-g) finite, so that the product is 1 and not inf * 0 where the gate is closed.
 template <bool EXACT> __device__ __forceinline__ void sigmoid(float g, float& a, float& rest) {
-    const float e = EXACT ? expf(-fabsf(g)) : __expf(-fabsf(g));
-    const float r = EXACT ? 1.f / (1.f + e) : __fdividef(1.f, 1.f + e);
-    const float s = e * r;
-    a = g >= 0.f ? r : s;
-    rest = g >= 0.f ? s : r;
-    if (g != g) a = rest = g;
-}
-
-__device__ __forceinline__ unsigned long long load_word(const unsigned long long* p) {
-    unsigned long long v;
-    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void store_word(unsigned long long* p, unsigned long long v) { asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory"); }
-__device__ __forceinline__ uint32_t load_word(const uint32_t* p) {
-    uint32_t v;
-    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ void store_word(uint32_t* p, uint32_t v) { asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory"); }
-// NaN in one spelling: the fill pattern is a NaN, too
-__device__ __forceinline__ uint32_t bits_of(float v) { return v != v ? 0x7fffffffu : __float_as_uint(v); }
-constexpr float kClosed = -1.f;                         // in the place of A, which is never negative
-
-template <typename Word> __device__ Word wait_word(const Word* p, bool& lost) {
-    Word v = load_word(p);
-    if (v != ~Word(0)) return v;
-    const int64_t began = clock64();
-    while ((v = load_word(p)) == ~Word(0)) {
-        if (clock64() - began > kWaitCycles) { lost = true; return v; }
-        __nanosleep(20);
+    if (EXACT) {
+        const float e = expf(-fabsf(g)), r = 1.f / (1.f + e), s = e * r;         // NaN where g is
+        a = g >= 0.f ? r : s;
+        rest = g >= 0.f ? s : r;
+    } else {
+        float x, e;
+        asm("max.NaN.f32 %0, %1, 0fC2A00000;" : "=f"(x) : "f"(g));               // -80
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x * -1.4426950408889634f));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(a) : "f"(1.f + e));
+        rest = e * a;
     }
-    return v;
 }
 
-template <typename T, int VEC, bool BACKWARD>
-__global__ void __launch_bounds__(kWarps * 32) recurrence_kernel(const RecurrenceParams p) {
-    constexpr int TOK = recurrence_chunk(BACKWARD) / kWarps, WIDTH = 32 * VEC;
-    constexpr bool EXACT = sizeof(T) == 4;
-    __shared__ float map_a[kWarps][WIDTH], map_b[kWarps][WIDTH], carried[WIDTH];
-    __shared__ uint32_t cuts_of[kWarps], ticket;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t block = blockIdx.x;
-    if (p.ticket != nullptr) {
-        if (threadIdx.x == 0) ticket = atomicAdd(p.ticket, 1u) + 1u;
-        __syncthreads();
-        block = ticket;
-    }
-    const uint32_t chunk = block / p.tiles, tile = block % p.tiles;
-    const int64_t C = p.channels, tokens = p.plan.tokens, c = (int64_t)tile * WIDTH + lane * VEC;
+// MAPS: only the segment's map
+template <typename T, int VEC, bool BACKWARD, bool MAPS>
+__global__ void __launch_bounds__(kWalkers * 32, 4) recurrence_kernel(const RecurrenceParams p) {
+    constexpr int BATCH = kBatch<BACKWARD>;
+    constexpr bool EXACT = sizeof(T) == 4, NEEDS_X = !BACKWARD || !MAPS, NEEDS_H = BACKWARD && !MAPS;
+    using R = Raw<T, VEC>;
+    const int lane = threadIdx.x & 31;
+    const int64_t job = (int64_t)blockIdx.x * kWalkers + (threadIdx.x >> 5), segment = job / p.tiles, C = p.channels, c = (int64_t)(job % p.tiles) * (32 * VEC) + lane * VEC;
+    if (segment >= p.segments) return;
     const bool live = c < C;                            // VEC divides the channels
-    const int64_t s0 = ((int64_t)chunk * kWarps + warp) * TOK;
-    auto token = [&](int i) -> int64_t { return BACKWARD ? tokens - 1 - (s0 + i) : s0 + i; };
-    const int here = (int)max((int64_t)0, min((int64_t)TOK, tokens - s0));
+    const int64_t lowest = segment * p.segment, count = min(p.segment, p.plan.tokens - lowest);
+    const int64_t t0 = BACKWARD ? lowest + count - 1 : lowest, step = BACKWARD ? -1 : 1;
+    const int64_t column = live ? c : 0;                // lanes behind the last channel read the first one's, and write nothing
+    const T *const x = static_cast<const T*>(p.x) + column, *const gate = static_cast<const T*>(p.gate) + column;
+    const T *const dh = static_cast<const T*>(p.dh) + column, *const hs = static_cast<const T*>(p.h) + column;
 
-    // which of the warp's tokens take nothing from the one before them (in scan order), and the rows that begin or end there
-    int32_t link = -1, tail = -1;
-    bool cut = false;
-    if (lane < here) {
-        const int64_t t = token(lane);
-        link = p.plan.link[t];
-        tail = p.plan.tail[t];
-        cut = BACKWARD ? p.plan.end[t] == t + 1 : link != -1;
+    struct Ahead {
+        R x[NEEDS_X ? BATCH : 1], gate[BATCH], dh[BACKWARD ? BATCH : 1], h[NEEDS_H ? BATCH : 1];
+        int32_t link, tail;                             // of token `lane` of the batch
+    };
+    // behind the segment's end the last token again: loaded, and not used
+    auto fetch = [&](Ahead& b, int64_t k0) {
+        const int64_t own = t0 + step * min(k0 + lane, count - 1);
+        b.link = lane < BATCH ? p.plan.link[own] : -1;
+        b.tail = lane < BATCH ? p.plan.tail[own] : -1;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int64_t t = t0 + step * min(k0 + i, count - 1);
+            if constexpr (NEEDS_X) b.x[i] = load_raw<T, VEC>(x + t * p.x_stride);
+            b.gate[i] = load_raw<T, VEC>(gate + t * p.gate_stride);
+            if constexpr (BACKWARD) b.dh[i] = load_raw<T, VEC>(dh + t * C);
+            if constexpr (NEEDS_H) b.h[i] = load_raw<T, VEC>(hs + max((int64_t)0, t - 1) * C);
+        }
+    };
+    float h[VEC], A[VEC];                               // the state or the gradient that goes on; of a map, B and A
+    bool closed = false;
+    const int64_t place = segment * C + column;
+#pragma unroll
+    for (int v = 0; v < VEC; ++v) {
+        h[v] = !MAPS && p.maps != nullptr ? p.carries[place + v] : 0.f;
+        A[v] = 1.f;
     }
-    const uint32_t cuts = __ballot_sync(~0u, cut);
-
-    const T *x = static_cast<const T*>(p.x) + c, *gate = static_cast<const T*>(p.gate) + c;
-    float a[TOK][VEC], b[TOK][VEC], rest[BACKWARD ? TOK : 1][VEC], gap[BACKWARD ? TOK : 1][VEC];
-    {
-        Raw<T, VEC> rx[TOK], rg[TOK], rd[BACKWARD ? TOK : 1], rh[BACKWARD ? TOK : 1];
+    auto row_of = [&](const float* values, int32_t row, float (&to)[VEC]) {
 #pragma unroll
-        for (int i = 0; i < TOK; ++i) {
-            const int32_t row = __shfl_sync(~0u, link, i);
+        for (int v = 0; v < VEC; ++v) to[v] = values != nullptr ? values[row * C + column + v] : 0.f;
+    };
+    auto walk = [&](const Ahead& b, int64_t k0) {
+        const uint32_t begins = __ballot_sync(~0u, b.link != -1), ends = __ballot_sync(~0u, b.tail >= 0);
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) b[i][v] = 0.f;
-            if (live && i < here) {
-                const int64_t t = token(i);
-                rx[i] = load_raw<T, VEC>(x + t * p.x_stride);
-                rg[i] = load_raw<T, VEC>(gate + t * p.gate_stride);
-                if (BACKWARD) {
-                    rd[i] = load_raw<T, VEC>(static_cast<const T*>(p.dh) + t * C + c);
-                    if (row == -1) rh[i] = load_raw<T, VEC>(static_cast<const T*>(p.h) + (t - 1) * C + c);
+        for (int i = 0; i < BATCH; ++i) {
+            if (k0 + i >= count) break;
+            const int64_t t = t0 + step * (k0 + i);
+            const bool begin = begins >> i & 1u, end = ends >> i & 1u;
+            float a[VEC], rest[VEC], gv[VEC], xv[VEC];
+            unpack<T, VEC>(b.gate[i], gv);
+            if constexpr (NEEDS_X) unpack<T, VEC>(b.x[i], xv);
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) sigmoid<EXACT>(gv[v], a[v], rest[v]);
+            if constexpr (!BACKWARD) {
+                if (begin) {
+                    const int32_t row = __shfl_sync(~0u, b.link, i);
+                    if (row >= 0) {
+                        row_of(p.initial, row, h);
+                    } else {
+#pragma unroll
+                        for (int v = 0; v < VEC; ++v) h[v] = 0.f;
+                    }
+                    closed = true;
                 }
-                // the state before a row's first token; elsewhere an episode's first token has 0 before it
-                if (row >= 0 && p.initial != nullptr)
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) b[i][v] = p.initial[(int64_t)row * C + c + v];
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < TOK; ++i) {
-            const int32_t row = __shfl_sync(~0u, link, i);
-            float xv[VEC], gv[VEC], out[VEC];
-            unpack<T, VEC>(rx[i], xv);
-            unpack<T, VEC>(rg[i], gv);
-            if (BACKWARD) {
-                float hv[VEC], dv[VEC];
-                unpack<T, VEC>(rh[i], hv);
-                unpack<T, VEC>(rd[i], dv);
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) {
-                    sigmoid<EXACT>(gv[v], a[i][v], rest[i][v]);
-                    gap[i][v] = (row == -1 ? hv[v] : b[i][v]) - xv[v];
-                    b[i][v] = dv[v];
+                    h[v] = fmaf(a[v], h[v], rest[v] * xv[v]);
+                    if (MAPS) A[v] *= a[v];
                 }
-            } else {
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    float z;
-                    sigmoid<EXACT>(gv[v], z, out[v]);
-                    a[i][v] = z;
-                    b[i][v] = row >= 0 && p.initial != nullptr ? fmaf(z, b[i][v], out[v] * xv[v]) : out[v] * xv[v];
-                }
-            }
-            if (!live || i >= here)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) { a[i][v] = 1.f; b[i][v] = 0.f; }
-        }
-    }
-    if (BACKWARD && p.dstate != nullptr)
-#pragma unroll
-        for (int i = 0; i < TOK; ++i) {
-            const int32_t row = __shfl_sync(~0u, tail, i);
-            if (row >= 0 && live)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) b[i][v] += p.dstate[(int64_t)row * C + c + v];
-        }
-
-    // the warp's map.  Forwards h -> a h + b; backwards m -> a (m + b), m the gradient that goes on to the token before.
-    float A[VEC], B[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
-#pragma unroll
-    for (int i = 0; i < TOK; ++i)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const bool shut = (cuts >> i) & 1u;
-            if (BACKWARD) B[v] = a[i][v] * (shut ? b[i][v] : B[v] + b[i][v]);
-            else B[v] = shut ? b[i][v] : fmaf(a[i][v], B[v], b[i][v]);
-            A[v] = shut ? 0.f : A[v] * a[i][v];
-        }
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) { map_a[warp][lane * VEC + v] = A[v]; map_b[warp][lane * VEC + v] = B[v]; }
-    if (lane == 0) cuts_of[warp] = cuts;
-    __syncthreads();
-
-    if (warp == 0) {
-        float carry[VEC];
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) carry[v] = 0.f;
-        if (p.ticket != nullptr) {
-            bool closed = false;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) { A[v] = 1.f; B[v] = 0.f; }
-            for (int w = 0; w < kWarps; ++w) {
-                const bool shut = cuts_of[w] != 0u;
-                closed |= shut;
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) {
-                    const float ma = map_a[w][lane * VEC + v], mb = map_b[w][lane * VEC + v];
-                    B[v] = shut ? mb : fmaf(ma, B[v], mb);
-                    A[v] *= ma;
-                }
-            }
-            const int64_t word = (int64_t)chunk * p.padded + (int64_t)tile * WIDTH + lane * VEC;
-#pragma unroll
-            for (int v = 0; v < VEC; ++v)
-                store_word(p.maps + word + v, (unsigned long long)bits_of(closed ? kClosed : A[v]) << 32 | bits_of(B[v]));
-            const bool needs = chunk != 0u && !(cuts & 1u);
-            const int64_t group = chunk / kGroup;
-            if (needs) {
-                bool lost = false, shut = false;
-                float P[VEC];
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) P[v] = 1.f;
-                constexpr int AHEAD = 8;
-                for (int64_t m = (int64_t)chunk - 1; m >= group * kGroup && !shut; m -= AHEAD) {
-                    unsigned long long got[AHEAD][VEC];
-#pragma unroll
-                    for (int k = 0; k < AHEAD; ++k)
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v)
-                            got[k][v] = m - k >= group * kGroup ? load_word(p.maps + (m - k) * p.padded + (int64_t)tile * WIDTH + lane * VEC + v) : 0ull;
-#pragma unroll
-                    for (int k = 0; k < AHEAD; ++k) {
-                        if (m - k < group * kGroup || shut) break;
-                        bool last = false;
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) {
-                            unsigned long long w = got[k][v];
-                            if (w == ~0ull) w = wait_word(p.maps + (m - k) * p.padded + (int64_t)tile * WIDTH + lane * VEC + v, lost);
-                            const float ma = __uint_as_float((uint32_t)(w >> 32)), mb = __uint_as_float((uint32_t)w);
-                            carry[v] = fmaf(P[v], mb, carry[v]);
-                            last = ma == kClosed;
-                            P[v] *= ma;
-                        }
-                        shut = last;
+                if constexpr (!MAPS) {
+                    if (live) store<T, VEC>(static_cast<T*>(p.h) + t * C + c, h);
+                    if (end) {
+                        const int32_t row = __shfl_sync(~0u, b.tail, i);
+                        if (live) store<float, VEC>(p.state + row * C + c, h);
                     }
                 }
-                if (!shut && group != 0)
+            } else {
+                float dv[VEC];
+                unpack<T, VEC>(b.dh[i], dv);
+                if (end) {
+                    const int32_t row = __shfl_sync(~0u, b.tail, i);
+                    float more[VEC];
+                    row_of(p.dstate, row, more);
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v)
-                        carry[v] = fmaf(P[v], __uint_as_float(wait_word(p.ends + (group - 1) * p.padded + (int64_t)tile * WIDTH + lane * VEC + v, lost)), carry[v]);
-                if (lost)
+                    for (int v = 0; v < VEC; ++v) h[v] += more[v];
+                }
+                const int32_t row = begin ? __shfl_sync(~0u, b.link, i) : -1;
+                if constexpr (!MAPS) {
+                    float before[VEC], dx[VEC], dg[VEC];
+                    unpack<T, VEC>(b.h[i], before);
+                    if (begin) {
+                        if (row >= 0) {
+                            row_of(p.initial, row, before);
+                        } else {
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) carry[v] = __uint_as_float(0x7fffffffu);
+                            for (int v = 0; v < VEC; ++v) before[v] = 0.f;
+                        }
+                    }
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        const float grad = h[v] + dv[v];
+                        dx[v] = rest[v] * grad;
+                        dg[v] = dx[v] * (before[v] - xv[v]) * a[v];
+                        h[v] = a[v] * grad;
+                    }
+                    if (live) {
+                        store<T, VEC>(static_cast<T*>(p.dx) + t * C + c, dx);
+                        store<T, VEC>(static_cast<T*>(p.dgate) + t * C + c, dg);
+                        if (row >= 0 && p.dinitial != nullptr) store<float, VEC>(p.dinitial + row * C + c, h);
+                    }
+                } else {
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        h[v] = a[v] * (h[v] + dv[v]);
+                        A[v] *= a[v];
+                    }
+                }
+                if (begin) {                            // nothing goes on to another episode
+                    closed = true;
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) h[v] = 0.f;
+                }
             }
-            if (chunk % kGroup == kGroup - 1 && chunk + 1 < p.chunks)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) store_word(p.ends + group * p.padded + (int64_t)tile * WIDTH + lane * VEC + v, bits_of(closed ? B[v] : fmaf(A[v], carry[v], B[v])));
         }
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) carried[lane * VEC + v] = carry[v];
+    };
+    Ahead one, two;
+    fetch(one, 0);
+    for (int64_t k = 0; k < count; k += 2 * BATCH) {
+        fetch(two, k + BATCH);
+        walk(one, k);
+        if (k + BATCH >= count) break;
+        fetch(one, k + 2 * BATCH);
+        walk(two, k + BATCH);
     }
+    if (MAPS && live)
+#pragma unroll
+        for (int v = 0; v < VEC; ++v) p.maps[place + v] = make_float2(closed ? kClosed : A[v], h[v]);
+}
+
+// What each segment begins with: a block per 32 channels, its warps first join the maps of a run of segments each, then walk their run again.
+template <bool BACKWARD> __global__ void __launch_bounds__(1024) recurrence_carries_kernel(const RecurrenceParams p) {
+    __shared__ float2 runs[32][32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t C = p.channels, c = (int64_t)blockIdx.x * 32 + lane, each = (p.segments + 31) / 32, begin = min(p.segments, warp * each), end = min(p.segments, begin + each);
+    const bool live = c < C;
+    auto at = [&](int64_t k) { return (BACKWARD ? p.segments - 1 - k : k) * C + (live ? c : 0); };
+    float A = 1.f, B = 0.f;
+    auto join = [&](float2 m) {
+        if (m.x == kClosed) { A = kClosed; B = m.y; } else { B = fmaf(m.x, B, m.y); A = A == kClosed ? A : A * m.x; }
+    };
+#pragma unroll 8
+    for (int64_t k = begin; k < end; ++k) join(p.maps[at(k)]);
+    runs[warp][lane] = make_float2(A, B);
     __syncthreads();
-
-    float h[VEC];
-#pragma unroll
-    for (int v = 0; v < VEC; ++v) h[v] = carried[lane * VEC + v];
-    for (int w = 0; w < warp; ++w) {
-        const bool shut = cuts_of[w] != 0u;
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const float mb = map_b[w][lane * VEC + v];
-            h[v] = shut ? mb : fmaf(map_a[w][lane * VEC + v], h[v], mb);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < TOK; ++i) {
-        const int32_t begins = __shfl_sync(~0u, link, i), ends = __shfl_sync(~0u, tail, i);
-        if (i >= here || !live) continue;
-        const int64_t at = token(i) * C + c;
-        const bool shut = (cuts >> i) & 1u;
-        if (BACKWARD) {
-            float dx[VEC], dg[VEC];
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) {
-                const float grad = shut ? b[i][v] : h[v] + b[i][v];
-                dx[v] = rest[i][v] * grad;
-                dg[v] = dx[v] * gap[i][v] * a[i][v];
-                h[v] = a[i][v] * grad;
-            }
-            store<T, VEC>(static_cast<T*>(p.dx) + at, dx);
-            store<T, VEC>(static_cast<T*>(p.dgate) + at, dg);
-            if (begins >= 0 && p.dinitial != nullptr)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) p.dinitial[(int64_t)begins * C + c + v] = h[v];
-        } else {
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) h[v] = shut ? b[i][v] : fmaf(a[i][v], h[v], b[i][v]);
-            store<T, VEC>(static_cast<T*>(p.h) + at, h);
-            if (ends >= 0)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) p.state[(int64_t)ends * C + c + v] = h[v];
-        }
+    float h = 0.f;
+    for (int w = 0; w < warp; ++w) h = runs[w][lane].x == kClosed ? runs[w][lane].y : fmaf(runs[w][lane].x, h, runs[w][lane].y);
+#pragma unroll 8
+    for (int64_t k = begin; k < end; ++k) {
+        const float2 m = p.maps[at(k)];
+        if (live) p.carries[at(k)] = h;
+        h = m.x == kClosed ? m.y : fmaf(m.x, h, m.y);
     }
 }
 
-static int64_t round_up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+// Tokens of a segment.  Rows of one length where they give every SM sixteen warps, or are so short that a second walk would cost more than the
+// first; else equal shares for sixteen warps an SM (by 128 channels of 16 bits, or 64 of 32), 32 tokens at least.
+static int64_t segment_of(const nuka_b200_episodes_t& plan, int64_t channels) {
+    const int64_t tiles = (channels + 127) / 128, wanted = 16 * 148;
+    if (plan.length > 0 && (plan.length <= 64 || plan.rows * tiles >= wanted)) return plan.length;
+    return plan.tokens <= 64 ? plan.tokens : std::max<int64_t>(32, (plan.tokens * tiles + wanted - 1) / wanted);
+}
+static bool on_its_own(int64_t segment, const nuka_b200_episodes_t& plan) { return plan.tokens <= segment || segment == plan.length; }
 
-static uint64_t workspace_of(bool backward, int64_t tokens, int64_t channels) {
-    const int64_t chunks = (tokens + recurrence_chunk(backward) - 1) / recurrence_chunk(backward), padded = round_up(channels, 64);
-    return chunks <= 1 ? 0 : kHeader + chunks * padded * 8 + (chunks + kGroup - 1) / kGroup * padded * 4;
+uint64_t recurrence_workspace(const nuka_b200_episodes_t& plan, int64_t channels) {
+    const int64_t segment = segment_of(plan, channels);
+    return on_its_own(segment, plan) ? 0u : (uint64_t)((plan.tokens + segment - 1) / segment * channels) * (sizeof(float2) + sizeof(float));
 }
 
-uint64_t recurrence_workspace(uint32_t, int64_t tokens, int64_t channels) { return std::max(workspace_of(false, tokens, channels), workspace_of(true, tokens, channels)); }
-
-template <typename T, int VEC> static cudaError_t run_recurrence(const nuka_b200_recurrence_t& d, bool backward, cudaStream_t stream) {
+template <typename T, int VEC, bool BACKWARD> static cudaError_t run_recurrence(const nuka_b200_recurrence_t& d, cudaStream_t stream) {
     RecurrenceParams p{};
     p.plan = *d.plan;
     p.channels = d.channels; p.x_stride = d.x_stride; p.gate_stride = d.gate_stride;
     p.x = d.x; p.gate = d.gate; p.dh = d.dh; p.h = d.h; p.dx = d.dx; p.dgate = d.dgate;
     p.initial = d.initial; p.dstate = d.dstate; p.state = d.state; p.dinitial = d.dinitial;
+    p.segment = segment_of(p.plan, d.channels);
+    p.segments = (p.plan.tokens + p.segment - 1) / p.segment;
     p.tiles = (uint32_t)((d.channels + 32 * VEC - 1) / (32 * VEC));
-    p.padded = round_up(d.channels, 64);
-    p.chunks = (uint32_t)((p.plan.tokens + recurrence_chunk(backward) - 1) / recurrence_chunk(backward));
-    if (p.chunks > 1u) {
-        unsigned char* w = static_cast<unsigned char*>(d.workspace);
-        p.ticket = reinterpret_cast<uint32_t*>(w);
-        p.maps = reinterpret_cast<unsigned long long*>(w + kHeader);
-        p.ends = reinterpret_cast<uint32_t*>(w + kHeader + (uint64_t)p.chunks * p.padded * 8);
-        const cudaError_t filled = cudaMemsetAsync(w, 0xff, workspace_of(backward, p.plan.tokens, d.channels), stream);
-        if (filled != cudaSuccess) return filled;
+    const unsigned blocks = (unsigned)((p.segments * p.tiles + kWalkers - 1) / kWalkers);
+    if (!on_its_own(p.segment, p.plan)) {
+        p.maps = static_cast<float2*>(d.workspace);
+        p.carries = reinterpret_cast<float*>(p.maps + p.segments * d.channels);
+        recurrence_kernel<T, VEC, BACKWARD, true><<<blocks, kWalkers * 32, 0, stream>>>(p);
+        recurrence_carries_kernel<BACKWARD><<<(unsigned)((d.channels + 31) / 32), 1024, 0, stream>>>(p);
     }
-    const unsigned blocks = p.tiles * p.chunks;
-    if (backward) recurrence_kernel<T, VEC, true><<<blocks, kWarps * 32, 0, stream>>>(p);
-    else recurrence_kernel<T, VEC, false><<<blocks, kWarps * 32, 0, stream>>>(p);
+    recurrence_kernel<T, VEC, BACKWARD, false><<<blocks, kWalkers * 32, 0, stream>>>(p);
     return cudaGetLastError();
 }
 
-static bool even(const void* p, size_t size) { return p == nullptr || reinterpret_cast<uintptr_t>(p) % (2 * size) == 0; }
-
 template <typename T> static cudaError_t run_recurrence(const nuka_b200_recurrence_t& d, bool backward, cudaStream_t stream) {
-    const bool pairs = d.channels % 2 == 0 && d.x_stride % 2 == 0 && d.gate_stride % 2 == 0 && even(d.x, sizeof(T)) && even(d.gate, sizeof(T)) && even(d.h, sizeof(T)) &&
-                       even(d.dh, sizeof(T)) && even(d.dx, sizeof(T)) && even(d.dgate, sizeof(T));
-    return pairs ? run_recurrence<T, 2>(d, backward, stream) : run_recurrence<T, 1>(d, backward, stream);
+    constexpr int W = kWide<T>;
+    auto on = [](const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; };
+    bool wide = d.channels % W == 0 && d.x_stride % W == 0 && d.gate_stride % W == 0;
+    for (const void* p : {d.x, d.gate, static_cast<const void*>(d.h), d.dh, static_cast<const void*>(d.dx), static_cast<const void*>(d.dgate)}) wide = wide && on(p, W * sizeof(T));
+    for (const float* p : {static_cast<const float*>(d.state), static_cast<const float*>(d.dinitial)}) wide = wide && on(p, W * sizeof(float));
+    if (backward) return wide ? run_recurrence<T, W, true>(d, stream) : run_recurrence<T, 1, true>(d, stream);
+    return wide ? run_recurrence<T, W, false>(d, stream) : run_recurrence<T, 1, false>(d, stream);
 }
 
 cudaError_t launch_recurrence(const nuka_b200_recurrence_t& d, bool backward, cudaStream_t stream) {

@@ -12,7 +12,7 @@ void SetLastError(const char* text);           // the text of nuka_last_error_me
 cudaError_t launch_episodes_from_offsets(const nuka_b200_episodes_t& p, const int32_t* offsets, cudaStream_t stream);
 cudaError_t launch_episodes_from_done(const nuka_b200_episodes_t& p, const uint8_t* done, cudaStream_t stream);
 
-uint64_t recurrence_workspace(uint32_t dtype, int64_t tokens, int64_t channels);
+uint64_t recurrence_workspace(const nuka_b200_episodes_t& plan, int64_t channels);
 cudaError_t launch_recurrence(const nuka_b200_recurrence_t& d, bool backward, cudaStream_t stream);
 cudaError_t launch_recurrence_step(uint32_t dtype, int64_t n, int64_t channels, const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
                                    const uint8_t* fresh, float* state, void* h, cudaStream_t stream);

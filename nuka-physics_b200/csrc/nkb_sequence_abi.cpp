@@ -24,6 +24,7 @@ const char* PlanFault(const nuka_b200_episodes_t* p) {
     if (p == nullptr) return "the plan is null";
     if (p->tokens < 0 || p->rows < 0 || p->tokens > kMostTokens || p->rows > kMostTokens) return "tokens or rows of the plan are negative or too many";
     if (p->tokens != 0 && p->rows == 0) return "tokens without a row";
+    if (p->length < 0 || (p->length != 0 && p->length * p->rows != p->tokens)) return "rows of one length do not give the plan's tokens";
     if (p->tokens != 0 && (p->first == nullptr || p->end == nullptr || p->link == nullptr || p->tail == nullptr)) return "an array of the plan is null";
     return nullptr;
 }
@@ -40,13 +41,13 @@ nuka_result_t nuka_b200_episodes_from_offsets(const nuka_b200_episodes_t* plan, 
 
 nuka_result_t nuka_b200_episodes_from_done(const nuka_b200_episodes_t* plan, const uint8_t* done, void* stream) {
     if (const char* fault = PlanFault(plan)) return Invalid(fault);
-    if (plan->rows != 0 && plan->tokens % plan->rows != 0) return Invalid("rows of one length need a number of tokens that the rows divide");
+    if (plan->tokens != 0 && plan->length == 0) return Invalid("the rows' length is 0");
     if (plan->tokens != 0 && done == nullptr) return Invalid("done is null");
     return Ran(nkb::launch_episodes_from_done(*plan, done, StreamOf(stream)));
 }
 
-uint64_t nuka_b200_recurrence_workspace(uint32_t dtype, int64_t tokens, int64_t channels) {
-    return tokens <= 0 || channels <= 0 ? 0u : nkb::recurrence_workspace(dtype, tokens, channels);
+uint64_t nuka_b200_recurrence_workspace(const nuka_b200_episodes_t* plan, int64_t channels) {
+    return PlanFault(plan) != nullptr || plan->tokens == 0 || channels <= 0 ? 0u : nkb::recurrence_workspace(*plan, channels);
 }
 
 static nuka_result_t Recurrence(const nuka_b200_recurrence_t* desc, bool backward, void* stream) {
@@ -66,7 +67,7 @@ static nuka_result_t Recurrence(const nuka_b200_recurrence_t* desc, bool backwar
     for (const float* p : {d.initial, static_cast<const float*>(d.state), d.dstate, static_cast<const float*>(d.dinitial)})
         if (!Aligned(p, 4)) return Invalid("a state does not lie on a multiple of 4 bytes");
     if (d.plan->tokens / 32 * (d.channels / 32 + 1) > (1ll << 31)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times channels");
-    const uint64_t need = nkb::recurrence_workspace(d.dtype, d.plan->tokens, d.channels);
+    const uint64_t need = nkb::recurrence_workspace(*d.plan, d.channels);
     if (need != 0u && (d.workspace == nullptr || d.workspace_bytes < need || !Aligned(d.workspace, 8))) return Invalid("the workspace is null, too small or not on 8 bytes");
     return Ran(nkb::launch_recurrence(d, backward, StreamOf(stream)));
 }

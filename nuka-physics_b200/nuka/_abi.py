@@ -63,7 +63,7 @@ class CookOptions(ctypes.Structure):
 
 
 class EpisodesDesc(ctypes.Structure):
-    _fields_ = [("first", ctypes.c_void_p), ("end", ctypes.c_void_p), ("link", ctypes.c_void_p), ("tail", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("rows", ctypes.c_int64)]
+    _fields_ = [("first", ctypes.c_void_p), ("end", ctypes.c_void_p), ("link", ctypes.c_void_p), ("tail", ctypes.c_void_p), ("tokens", ctypes.c_int64), ("rows", ctypes.c_int64), ("length", ctypes.c_int64)]
 
 
 class RecurrenceDesc(ctypes.Structure):
@@ -181,7 +181,7 @@ def lib():
     i64, u64 = ctypes.c_int64, ctypes.c_uint64
     L.nuka_b200_episodes_from_offsets.argtypes = [ctypes.POINTER(EpisodesDesc), vp, vp]
     L.nuka_b200_episodes_from_done.argtypes = [ctypes.POINTER(EpisodesDesc), vp, vp]
-    L.nuka_b200_recurrence_workspace.argtypes = [u32, i64, i64]
+    L.nuka_b200_recurrence_workspace.argtypes = [ctypes.POINTER(EpisodesDesc), i64]
     L.nuka_b200_recurrence_workspace.restype = u64
     L.nuka_b200_recurrence.argtypes = [ctypes.POINTER(RecurrenceDesc), vp]
     L.nuka_b200_recurrence_backward.argtypes = [ctypes.POINTER(RecurrenceDesc), vp]

@@ -75,12 +75,12 @@ def _channels_last(tensor, multiple=1, size=1, least=0):
 class Episodes:
     """How a rollout's tokens are cut into rows and episodes, on the GPU.  Made once per rollout, for all layers and passes over it."""
 
-    def __init__(self, tokens, rows, device, rows_may_be_empty):
+    def __init__(self, tokens, rows, length, device):
         self.tokens, self.rows, self.device = int(tokens), int(rows), torch.device(device)
-        self._rows_may_be_empty = rows_may_be_empty or self.tokens == 0
+        self._rows_may_be_empty = length == 0
         self._plan = torch.empty((4, self.tokens), dtype=torch.int32, device=device)
         base, step = self._plan.data_ptr(), 4 * self.tokens
-        self._desc = _abi.EpisodesDesc(base, base + step, base + 2 * step, base + 3 * step, self.tokens, self.rows)
+        self._desc = _abi.EpisodesDesc(base, base + step, base + 2 * step, base + 3 * step, self.tokens, self.rows, length)
         self._ref = ctypes.pointer(self._desc)
 
     @classmethod
@@ -91,7 +91,7 @@ class Episodes:
         _expect(tokens >= 0, "tokens must not be negative")
         device = _on_gpu(offsets)
         offsets = offsets.contiguous()
-        plan = cls(tokens, offsets.numel() - 1, device, True)
+        plan = cls(tokens, offsets.numel() - 1, 0, device)
         _call(device, _abi.lib().nuka_b200_episodes_from_offsets, plan._ref, offsets.data_ptr())
         return plan
 
@@ -102,7 +102,7 @@ class Episodes:
         _expect(done.dim() == 2, "done must be envs x steps")
         device = _on_gpu(done)
         done = _flags(done, tuple(done.shape), device, "done")
-        plan = cls(done.numel(), done.shape[0], device, False)
+        plan = cls(done.numel(), done.shape[0], done.shape[1], device)
         _call(device, _abi.lib().nuka_b200_episodes_from_done, plan._ref, done.data_ptr())
         return plan
 
@@ -141,7 +141,7 @@ class _Recurrence(torch.autograd.Function):
         else:
             state = initial.clone()
         lib = _abi.lib()
-        need = lib.nuka_b200_recurrence_workspace(dtype, episodes.tokens, channels)
+        need = lib.nuka_b200_recurrence_workspace(episodes._ref, channels)
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), state.data_ptr(),
                                    None, None, None, None, None, _ptr(workspace), need)
@@ -167,7 +167,7 @@ class _Recurrence(torch.autograd.Function):
             else:                                   # an empty row ends with the state that it began with
                 dinitial = torch.zeros_like(initial) if dstate is None else dstate.clone()
         lib = _abi.lib()
-        need = lib.nuka_b200_recurrence_workspace(dtype, episodes.tokens, channels)
+        need = lib.nuka_b200_recurrence_workspace(episodes._ref, channels)
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), None,
                                    dh.data_ptr(), _ptr(dstate), dx.data_ptr(), dgate.data_ptr(), _ptr(dinitial), _ptr(workspace), need)

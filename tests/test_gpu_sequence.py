@@ -158,6 +158,37 @@ def test_recurrence_over_a_rollout_with_episodes_that_end_inside(shape, often):
     _close(dgate.cpu(), want[1], u * (want[1].abs() + (want[3] * before).abs()) + STEPS * want[1].abs().max(), "dgate")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("channels,length", [(20, 1), (64, 7), (37, 24), (72, 16), (256, 9)])
+def test_many_rows_of_one_length(dtype, channels, length):
+    """Rows enough for a warp each: the same values as of the rows one by one in other plans, gradients among them."""
+    gen, n = _gen(channels + length), 2400
+    done = torch.rand((n, length), generator=gen, device="cuda") < 0.1
+    plan = S.Episodes.from_done(done)
+    x, gate = (_normal(gen, n * length, channels, dtype=dtype).requires_grad_() for _ in range(2))
+    initial = _normal(gen, n, channels).requires_grad_()
+    dh, dstate = _normal(gen, n * length, channels, dtype=dtype), _normal(gen, n, channels)
+    h, state = S.gated_recurrence(x, gate, plan, initial)
+    grads = torch.autograd.grad([h, state], [x, gate, initial], [dh, dstate])
+    x64, g64, i64 = (v.detach().cpu().double() for v in (x, gate, initial))
+    some = torch.cat([torch.arange(r * length, (r + 1) * length) for r in (0, 1, 5, 1203, n - 1)])
+    rows = [0, 1, 5, 1203, n - 1]
+    small = S.Episodes.from_done(done[rows])
+    want_h, want_state, before = _recurrence_64(x64[some], g64[some], small, i64[rows])
+    want = _recurrence_grad_64(x64[some], g64[some], small, before, dh.cpu().double()[some], dstate.cpu().double()[rows])
+    u = UNIT[dtype]
+    _close(h.detach().cpu()[some], want_h, u * want_h.abs() + STEPS * want_h.abs().max(), "h")
+    _close(state.detach().cpu()[rows], want_state, STEPS * want_state.abs().max(), "state")
+    _close(grads[0].cpu()[some], want[0], u * want[0].abs() + STEPS * want[0].abs().max(), "dx")
+    _close(grads[1].cpu()[some], want[1], u * (want[1].abs() + (want[3] * before).abs()) + STEPS * want[1].abs().max(), "dgate")
+    _close(grads[2].cpu()[rows], want[2], STEPS * want[2].abs().max(), "dinitial")
+    # and every row against the chunks' kernel, by offsets in place of one length, where no episode ends inside
+    plain = S.Episodes.from_done(torch.zeros_like(done))
+    offsets = S.Episodes.from_offsets(torch.arange(n + 1, dtype=torch.int32, device="cuda") * length, n * length)
+    for got, other in zip(S.gated_recurrence(x, gate, plain, initial), S.gated_recurrence(x, gate, offsets, initial)):
+        assert (got.double() - other.double()).abs().max().item() <= 2 * max(UNIT[got.dtype], STEPS) * other.abs().max().item()
+
+
 def test_what_is_not_finite_stays_in_its_episode():
     lengths = [100, 90, 300, 40]
     plan, offsets = _plan_of(lengths)
@@ -373,13 +404,15 @@ def test_the_c_entries_refuse_what_they_cannot_take():
     ok = dict(plan=plan._ref, dtype=0, channels=8, x=x.data_ptr(), gate=x.data_ptr(), x_stride=8, gate_stride=8, h=x.data_ptr(), state=x.data_ptr())
     call = lambda **change: lib.nuka_b200_recurrence(ctypes.byref(_abi.RecurrenceDesc(**{**ok, **change})), None)
     assert lib.nuka_b200_recurrence(None, None) == _abi.INVALID_ARG
-    assert lib.nuka_b200_recurrence_workspace(0, 300, 8) > 0 and lib.nuka_b200_recurrence_workspace(0, 10, 8) == 0
+    small, _ = _plan_of([10])
+    assert lib.nuka_b200_recurrence_workspace(plan._ref, 8) > 0 and lib.nuka_b200_recurrence_workspace(small._ref, 8) == 0
     for change in (dict(x=None), dict(h=None), dict(state=None), dict(x=x.data_ptr() + 2), dict(x_stride=-8), dict(channels=-1), dict(), dict(workspace=x.data_ptr(), workspace_bytes=64)):
         assert call(**change) == _abi.INVALID_ARG, change                       # the last two: no workspace, too small a one
         assert lib.nuka_last_error_message() != b""
     assert call(dtype=3) == 7
-    plan_of = lambda **change: ctypes.byref(_abi.EpisodesDesc(**{**dict(first=x.data_ptr(), end=x.data_ptr(), link=x.data_ptr(), tail=x.data_ptr(), tokens=9, rows=2), **change}))
-    assert lib.nuka_b200_episodes_from_done(plan_of(), x.data_ptr(), None) == _abi.INVALID_ARG          # 2 does not divide 9
+    plan_of = lambda **change: ctypes.byref(_abi.EpisodesDesc(**{**dict(first=x.data_ptr(), end=x.data_ptr(), link=x.data_ptr(), tail=x.data_ptr(), tokens=9, rows=2, length=0), **change}))
+    for length in (0, 4, -1):                                                   # 2 rows of 4 are not 9 tokens
+        assert lib.nuka_b200_episodes_from_done(plan_of(length=length), x.data_ptr(), None) == _abi.INVALID_ARG
     for change in (dict(tokens=-1), dict(tokens=2 ** 31), dict(rows=0), dict(link=None)):
         assert lib.nuka_b200_episodes_from_offsets(plan_of(**change), x.data_ptr(), None) == _abi.INVALID_ARG
     assert lib.nuka_b200_heads(None, None) == _abi.INVALID_ARG and lib.nuka_b200_recurrence_step(0, 1, 8, None, 8, None, 8, None, None, None, None) == _abi.INVALID_ARG

@@ -30,6 +30,7 @@ struct AttentionParams {
     const int32_t *first, *end;
     int64_t tokens, pitch;                              // pitch: floats between the heads' rows of lse and delta
     int heads_q, heads_k, dim, window;                  // window 0: all of the episode
+    int span, tiles;                                    // tokens of a tile, at most 128, and how many tiles
     float scale, scale2;                                // scale2: times log2(e)
     void *out, *dq, *dk, *dv;
     const void* dout;
@@ -39,6 +40,19 @@ struct AttentionParams {
 __device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
 __device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
 __device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+
+// A tile of queries and a head; the longest first.
+struct QueryJob {
+    int i0, last, j0, count, head;                      // queries i0 to last, keys from j0 on in `count` steps
+    __device__ __forceinline__ QueryJob(const AttentionParams& p, int job) {
+        head = job % p.heads_q;
+        i0 = (p.tiles - 1 - job / p.heads_q) * p.span;
+        last = (int)min((int64_t)i0 + p.span, p.tokens) - 1;
+        j0 = first_key(p, i0);
+        count = (last - j0) / kStream + 1;
+    }
+    __device__ __forceinline__ int low(const AttentionParams& p) const { return i0 + (int)threadIdx.x <= last ? first_key(p, i0 + (int)threadIdx.x) : 0; }
+};
 
 // One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T.
 template <typename T, int DP> __device__ __forceinline__ void store_row(uint32_t at, float by, int dim, T* to) {
@@ -81,175 +95,352 @@ template <typename T, int N, int DP> __device__ __forceinline__ void multiply_co
 // All lanes of a warp wait, and go on together.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* lost) { return __all_sync(~0u, barrier_wait(bar, parity, lost)) != 0; }
 
+// Which of the columns 0 to 31 lie between `from` and `to`.
+__device__ __forceinline__ uint32_t columns_between(int from, int to) {
+    const uint32_t above = from <= 0 ? ~0u : from > 31 ? 0u : ~0u << from, below = to < 0 ? 0u : to >= 31 ? ~0u : (2u << to) - 1u;
+    return above & below;
+}
+
+// A row of 64-column panels of 128 rows, swizzled as TMA takes it: 16 bytes number `k` of row `row`.
+__device__ __forceinline__ unsigned char* staged(unsigned char* tile, int row, int k) { return tile + k / 8 * kRows * 128 + row * 128 + ((k % 8) ^ (row % 8)) * 16; }
+// A thread's row of 32-bit accumulators, times `by`, into a staged tile of T; `read` learns when the accumulators have been read.
+template <typename T, int DP> __device__ __forceinline__ void stage_row(uint32_t at, float by, unsigned char* tile, int row, uint64_t* read) {
+#pragma unroll
+    for (int c = 0; c < DP; c += 32) {
+        uint32_t r[32];
+        tensor_load(at + c, r);
+        wait_loads();
+        if (c + 32 == DP) {
+            fence_before();
+            barrier_arrive(read);
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 8) {
+            uint4 v;
+            v.x = pack<T>(__uint_as_float(r[k]) * by, __uint_as_float(r[k + 1]) * by);
+            v.y = pack<T>(__uint_as_float(r[k + 2]) * by, __uint_as_float(r[k + 3]) * by);
+            v.z = pack<T>(__uint_as_float(r[k + 4]) * by, __uint_as_float(r[k + 5]) * by);
+            v.w = pack<T>(__uint_as_float(r[k + 6]) * by, __uint_as_float(r[k + 7]) * by);
+            *reinterpret_cast<uint4*>(staged(tile, row, (c + k) / 8)) = v;
+        }
+    }
+}
+
 // A block that gave up waits, again for a bounded time, for the loads that it still has under way; what they bring is not used.
 __device__ __forceinline__ void drain(uint64_t* bar, uint32_t parity) {
     const long long began = clock64();
     while (!barrier_try(bar, parity) && clock64() - began < kBarrierCycles) {}
 }
 
+// The last loads into a ring of `stages` buffers of which `used` were begun.
+__device__ __forceinline__ void drain_ring(uint64_t* bars, int stages, int used) {
+    for (int n = max(0, used - stages); n < used; ++n) drain(&bars[n % stages], n / stages & 1);
+}
+
 extern __shared__ unsigned char dynamic_shared[];
 __device__ __forceinline__ unsigned char* aligned_shared() { return dynamic_shared + ((1024u - (shared_address(dynamic_shared) & 1023u)) & 1023u); }
 
 // ---- forwards ---------------------------------------------------------------------------------------------------------
+// A block takes jobs in turn: two tiles of queries, of two heads that share a key head or else of two neighbouring stretches of tokens, that meet the same keys, so that a tile of
+// keys and values is loaded once for 256 rows.  While one tile's rows are at their exponentials the tensor cores work for the other's. Loads run ahead
+// into the next job while the rows of the present one end. A row's 128 scores are taken into registers at once; where tensor memory has room for P beside them (dim up to 64)
+// the next scores then are multiplied while the exponentials go on, else P takes their place. P goes to its product in two halves, so that the first is under way during the second's exponentials.
+constexpr int kForward = 384;                           // two times four warps of rows, one that multiplies, one that loads, two that do nothing
+template <int N> struct Number { static constexpr int value = N; };
+
 template <int DP> struct Forward {
-    static constexpr int kStages = DP == 64 ? 2 : 1;
-    static constexpr bool kApart = DP == 64;            // P has columns of its own, so that the next scores do not wait for P V
+    static constexpr bool kApart = DP == 64;
+    static constexpr int kQueries = DP == 64 ? 2 : 1, kStages = DP == 64 ? 3 : 2;              // buffers
     static constexpr int kTile = kRows * DP * 2;
-    static constexpr int kShared = kTile * (1 + 2 * kStages) + 1024;
-    static constexpr int kOut = kRows, kProb = kApart ? kRows + DP : 0;      // columns; the scores are at 0
+    // rows leave through tiles of their own, or where there is no room through their queries' place
+    static constexpr int kKeys = 2 * kQueries * kTile, kStaged = kApart ? kKeys + 2 * kStages * kTile : 0, kShared = kKeys + 2 * kStages * kTile + (kApart ? 2 * kTile : 0) + 1024;
+    static constexpr int kProb = kApart ? kRows : 0, kOut = kApart ? kRows + kRows / 2 : kRows, kSet = 256;     // columns; the scores are at 0
+};
+
+struct ForwardJob {
+    int i0[2], last[2], head[2], j0, count;             // queries i0 to last (none if below i0), keys from j0 on in `count` steps
+    __device__ __forceinline__ ForwardJob(const AttentionParams& p, int job) {
+        const bool by_heads = p.heads_q / p.heads_k % 2 == 0;
+        const int across = by_heads ? p.heads_q / 2 : p.heads_q, along = by_heads ? p.tiles : (p.tiles + 1) / 2, at = along - 1 - job / across;       // the longest first
+        for (int s = 0; s < 2; ++s) {
+            head[s] = by_heads ? job % across * 2 + s : job % across;
+            i0[s] = (by_heads ? at : at * 2 + s) * p.span;
+            last[s] = (int)min((int64_t)i0[s] + p.span, p.tokens) - 1;
+        }
+        j0 = first_key(p, i0[0]);
+        count = (max(last[0], last[1]) - j0) / kRows + 1;
+    }
+    static __host__ __device__ __forceinline__ int all(const AttentionParams& p) { return p.heads_q / p.heads_k % 2 == 0 ? p.tiles * (p.heads_q / 2) : (p.tiles + 1) / 2 * p.heads_q; }
+    // Every other round backwards, so that the longest of one round goes with the shortest of the next.
+    static __device__ __forceinline__ int of_turn(int turn) { return turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBlock, 2) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                              const AttentionParams p) {
+__global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                const __grid_constant__ CUtensorMap map_o, const AttentionParams p) {
     using F = Forward<DP>;
-    __shared__ uint64_t q_full, k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ uint64_t q_full[F::kQueries], q_empty[F::kQueries], k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages];
+    __shared__ uint64_t s_full[2], s_empty[2], p_full[2][2], o_done[2], o_empty[2], ended;
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int tiles = (int)((p.tokens + kRows - 1) / kRows), tile = tiles - 1 - (int)(blockIdx.x / p.heads_q), head = blockIdx.x % p.heads_q;     // the longest first
-    const int key_head = head / (p.heads_q / p.heads_k);
-    const int i0 = tile * kRows, last = (int)min((int64_t)i0 + kRows, p.tokens) - 1;
-    const int j0 = first_key(p, i0), count = (last - j0) / kRows + 1;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         lost = 0;
-        barrier_init(&q_full, 1);
-        for (int s = 0; s < F::kStages; ++s) { barrier_init(&k_full[s], 1); barrier_init(&k_empty[s], 1); barrier_init(&v_full[s], 1); barrier_init(&v_empty[s], 1); }
-        barrier_init(&s_full, 1);
-        barrier_init(&p_full, kRows);
-        barrier_init(&o_done, 1);
+        for (int s = 0; s < F::kQueries; ++s) { barrier_init(&q_full[s], 1); barrier_init(&q_empty[s], 2); }
+        for (int s = 0; s < F::kStages; ++s) { barrier_init(&k_full[s], 1); barrier_init(&k_empty[s], 2); barrier_init(&v_full[s], 1); barrier_init(&v_empty[s], 2); }
+        for (int s = 0; s < 2; ++s) {
+            barrier_init(&s_full[s], 1);
+            barrier_init(&s_empty[s], kRows);
+            barrier_init(&p_full[s][0], kRows);
+            barrier_init(&p_full[s][1], kRows);
+            barrier_init(&o_done[s], 1);
+            barrier_init(&o_empty[s], kRows);
+        }
         barrier_init(&ended, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    if (warp == 5) tensor_alloc<256>(&tensor);
+    if (warp == 9) tensor_alloc<512>(&tensor);
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t base = tensor, q_at = shared_address(shared), k_at = q_at + F::kTile, v_at = k_at + F::kStages * F::kTile;
+    const uint32_t base = tensor, q_at = shared_address(shared), k_at = q_at + F::kKeys, v_at = k_at + F::kStages * F::kTile;
+    const int jobs = ForwardJob::all(p);
+    // registers: 128 x (2 x 200 + 104) of the 384 x 168 that the block has
 
-    if (warp == 4) {
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
+    if (warp == 9) {
         if (lane == 0) {
-            barrier_expect(&q_full, F::kTile);
-            load_panels<kRows, DP>(shared, &map_q, &q_full, head, i0);
-            int j = 0;
-            for (; j < count; ++j) {
-                const int s = j % F::kStages, turn = j / F::kStages;
-                if (turn > 0 && !barrier_wait(&k_empty[s], (turn - 1) & 1, &lost)) break;
-                barrier_expect(&k_full[s], F::kTile);
-                load_panels<kRows, DP>(shared + F::kTile * (1 + s), &map_k, &k_full[s], key_head, j0 + j * kRows);
-                if (turn > 0 && !barrier_wait(&v_empty[s], (turn - 1) & 1, &lost)) { drain(&k_full[s], turn & 1); break; }
-                barrier_expect(&v_full[s], F::kTile);
-                load_panels<kRows, DP>(shared + F::kTile * (1 + F::kStages + s), &map_v, &v_full[s], key_head, j0 + j * kRows);
+            int queries = 0, keys = 0, values = 0;      // loads begun so far
+            bool fine = true;
+            ForwardJob next(p, blockIdx.x);
+            for (int turn = 0, job = blockIdx.x; fine && job < jobs; job = ForwardJob::of_turn(++turn)) {
+                const ForwardJob now = next;
+                const int after = ForwardJob::of_turn(turn + 1);
+                if (after < jobs) next = ForwardJob(p, after);
+                const int b = queries % F::kQueries, key_head = now.head[0] / (p.heads_q / p.heads_k);
+                if (queries >= F::kQueries && !(fine = barrier_wait(&q_empty[b], (queries / F::kQueries - 1) & 1, &lost))) break;
+                barrier_expect(&q_full[b], 2 * F::kTile);
+                for (int s = 0; s < 2; ++s) load_panels<kRows, DP>(shared + (2 * b + s) * F::kTile, &map_q, &q_full[b], now.head[s], now.i0[s]);
+                ++queries;
+                for (int j = 0; j < now.count; ++j) {
+                    const int s = keys % F::kStages, round = keys / F::kStages;
+                    if (round > 0 && !(fine = barrier_wait(&k_empty[s], (round - 1) & 1, &lost))) break;
+                    barrier_expect(&k_full[s], F::kTile);
+                    load_panels<kRows, DP>(shared + F::kKeys + s * F::kTile, &map_k, &k_full[s], key_head, now.j0 + j * kRows);
+                    ++keys;
+                    if (round > 0 && !(fine = barrier_wait(&v_empty[s], (round - 1) & 1, &lost))) break;
+                    barrier_expect(&v_full[s], F::kTile);
+                    load_panels<kRows, DP>(shared + F::kKeys + (F::kStages + s) * F::kTile, &map_v, &v_full[s], key_head, now.j0 + j * kRows);
+                    ++values;
+                }
             }
-            drain(&q_full, 0);
-            for (int b = max(0, j - F::kStages); b < j; ++b) { drain(&k_full[b % F::kStages], b / F::kStages & 1); drain(&v_full[b % F::kStages], b / F::kStages & 1); }
+            drain_ring(q_full, F::kQueries, queries);
+            drain_ring(k_full, F::kStages, keys);
+            drain_ring(v_full, F::kStages, values);
         }
-    } else if (warp == 5) {
-        if (lane == 0) {
-            bool fine = barrier_wait(&q_full, 0, &lost);
-            auto scores = [&](int j) {
-                const int s = j % F::kStages;
-                if (!barrier_wait(&k_full[s], j / F::kStages & 1, &lost)) return false;
+    } else if (warp == 8) {
+        {
+            // One warp for both tiles, so that one's products run as a whole before the other's: issued side by side they take turns, and both tiles wait and both are at
+            // their exponentials at the same time.
+            struct Cursor { int turn, job, j, count, ahead; } at[2];
+            bool fine = true;
+            for (int set = 0; set < 2; ++set) at[set] = {0, (int)blockIdx.x, 0, 0, 0};
+            auto scores = [&](auto which) {
+                constexpr int set = decltype(which)::value;
+                Cursor& a = at[set];
+                const int b = a.turn % F::kQueries;
+                if (a.j == 0) {
+                    a.count = ForwardJob(p, a.job).count;
+                    if (!warp_wait(&q_full[b], a.turn / F::kQueries & 1, &lost)) return false;
+                }
+                const int s = a.ahead % F::kStages;
+                if (!warp_wait(&k_full[s], a.ahead / F::kStages & 1, &lost)) return false;
+                if (a.ahead > 0 && !warp_wait(F::kApart ? &s_empty[set] : &o_done[set], (a.ahead - 1) & 1, &lost)) return false;
                 fence_after();
-                multiply_rows<T, kRows, DP>(base, q_at, k_at + s * F::kTile);
-                commit(&s_full);
+                multiply_rows<T, kRows, DP>(base + set * F::kSet, q_at + (2 * b + set) * F::kTile, k_at + s * F::kTile);
+                commit(&s_full[set]);
                 commit(&k_empty[s]);
+                ++a.ahead;
+                if (++a.j == a.count) {
+                    if (F::kApart) commit(&q_empty[b]);
+                    a.j = 0;
+                    a.job = ForwardJob::of_turn(++a.turn);
+                }
                 return true;
             };
-            fine = fine && scores(0);
-            for (int j = 0; fine && j < count; ++j) {
-                const int s = j % F::kStages;
-                if (!barrier_wait(&p_full, j & 1, &lost)) break;
+            int n = 0, done = 0, steps = 0;
+            // one step of one tile: i of its job
+            auto step = [&](auto which, int i) {
+                constexpr int set = decltype(which)::value;
+                const int s = n % F::kStages;
+                if (F::kApart && i + 1 < steps && !scores(which)) return false;
+                if (!warp_wait(&p_full[set][0], n & 1, &lost)) return false;
+                if (i == 0 && done > 0 && !warp_wait(&o_empty[set], (done - 1) & 1, &lost)) return false;
+                if (!warp_wait(&v_full[s], n / F::kStages & 1, &lost)) return false;
                 fence_after();
-                if (F::kApart && j + 1 < count) fine = scores(j + 1);
-                if (!fine || !barrier_wait(&v_full[s], j / F::kStages & 1, &lost)) break;
-                fence_after();
-                multiply_columns<T, kRows, DP>(base + F::kOut, base + F::kProb, v_at + s * F::kTile, j != 0);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (half == 1) {
+                        if (!warp_wait(&p_full[set][1], n & 1, &lost)) return false;
+                        fence_after();
+                    }
+#pragma unroll
+                    for (int k = half * 64; k < half * 64 + 64; k += 16)
+                        multiply_tensor(base + set * F::kSet + F::kOut, base + set * F::kSet + F::kProb + k / 2, outer_rows(v_at + s * F::kTile + k * 128, kRows * 128), product_of<T>(DP, true),
+                                        i != 0 || k != 0);
+                }
                 commit(&v_empty[s]);
-                commit(&o_done);
-                if (!F::kApart && j + 1 < count) fine = barrier_wait(&o_done, j & 1, &lost) && scores(j + 1);
+                commit(&o_done[set]);
+                return F::kApart || i + 1 == steps || scores(which);
+            };
+            fine = scores(Number<0>{}) && scores(Number<1>{});
+            for (int own = blockIdx.x; fine && own < jobs; own = ForwardJob::of_turn(++done)) {
+                steps = at[0].count;                    // of the job that the scores have just begun
+                for (int i = 0; fine && i < steps; ++i, ++n) fine = step(Number<0>{}, i) && step(Number<1>{}, i);
+                // across a job's end when its last products are under way: the next one's queries may come only when both tiles' rows have left
+                if (fine && at[0].job < jobs) fine = scores(Number<0>{}) && scores(Number<1>{});
             }
             commit(&ended);
             drain(&ended, 0);
         }
+    }
     } else {
-        const int i = i0 + threadIdx.x;
-        const bool live = i < p.tokens;
-        const int low = live ? first_key(p, i) : 0, high = live ? i : -1;
-        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
-        float top = -INFINITY, sum = 0.f;                       // of the scores as they are; the sum of exp2(scale2 (S - top))
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+        const int set = warp / 4, row = threadIdx.x % kRows;
+        const uint32_t mine = base + set * F::kSet + ((uint32_t)(warp % 4 * 32) << 16);
+        const Pair scale2 = pair_of(p.scale2, p.scale2);
         bool fine = true;
-        for (int j = 0; j < count; ++j) {
-            const int k0 = j0 + j * kRows;
-            if (!(fine = warp_wait(&s_full, j & 1, &lost))) break;
-            fence_after();
-            uint32_t r[kRows];
+        int n = 0;
+        ForwardJob next(p, blockIdx.x);
+        auto low_of = [&](const ForwardJob& job) { return job.i0[set] + row <= job.last[set] ? first_key(p, job.i0[set] + row) : 0; };
+        int next_low = low_of(next);
+        for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
+            const int first = next.i0[set], last = next.last[set], i = first + row, low = next_low, count = next.count, j0 = next.j0, head = next.head[set];
+            const bool live = i <= last;
+            const int high = live ? i : -1;
+            const int after = ForwardJob::of_turn(turn + 1);
+            if (after < jobs) { next = ForwardJob(p, after); next_low = low_of(next); }
+            // keys that any and that all of the warp's rows see; a row that is not there sees none
+            const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
+            const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
+            float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
+            for (int j = 0; fine && j < count; ++j, ++n) {
+                const int k0 = j0 + j * kRows;
+                if (!(fine = warp_wait(&s_full[set], n & 1, &lost))) break;
+                fence_after();
+                uint32_t r[kRows];
 #pragma unroll
-            for (int c = 0; c < kRows; c += 32) tensor_load(mine + c, r + c);
-            wait_loads();
-            if (!__all_sync(~0u, k0 >= low && k0 + kRows - 1 <= high)) {
-                const int from = low - k0, to = high - k0;
+                for (int c = 0; c < kRows; c += 32) tensor_load(mine + c, r + c);
+                wait_loads();
+                if (F::kApart) {
+                    fence_before();
+                    barrier_arrive(&s_empty[set]);
+                }
+                if (k0 < all_low || k0 + kRows - 1 > all_high) {
 #pragma unroll
-                for (int c = 0; c < kRows; ++c)
-                    if (c < from || c > to) r[c] = 0xff800000u;
-            }
-            float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
+                    for (int c = 0; c < kRows; c += 32) {
+                        const uint32_t seen = columns_between(low - k0 - c, high - k0 - c);
 #pragma unroll
-            for (int c = 0; c < kRows; ++c) best[c % 4] = fmaxf(best[c % 4], __uint_as_float(r[c]));
-            const float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
-            // P V of the tile before: P and O are free to be written
-            if (j > 0 && !(fine = warp_wait(&o_done, (j - 1) & 1, &lost))) break;
-            // the maximum in use follows only where the new one is more than 2^8 above: P stays below 2^8, and O is seldom rescaled
-            const bool up = (now - top) * p.scale2 > 8.f || top == -INFINITY;
-            if (__any_sync(~0u, up && now != top)) {
-                const float by = up && now != top ? exp2_fast((top - now) * p.scale2) : 1.f;
-                if (up) top = now;
-                sum *= by;
-                if (j > 0) {
-                    fence_after();
-#pragma unroll
-                    for (int c = 0; c < DP; c += 32) {
-                        uint32_t o[32];
-                        tensor_load(mine + F::kOut + c, o);
-                        wait_loads();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-                        tensor_store(mine + F::kOut + c, o);
+                        for (int k = 0; k < 32; ++k) r[c + k] = seen >> k & 1u ? r[c + k] : 0xff800000u;
                     }
                 }
-            }
-            const float shift = top == -INFINITY ? 0.f : top * p.scale2;
-            float part[4] = {0.f, 0.f, 0.f, 0.f};
+                float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < kRows; c += 64) {
-                uint32_t packed[32];
+                for (int c = 0; c < kRows; c += 8)
 #pragma unroll
-                for (int k = 0; k < 64; k += 2) {
-                    const float a = exp2_fast(fmaf(__uint_as_float(r[c + k]), p.scale2, -shift)), b = exp2_fast(fmaf(__uint_as_float(r[c + k + 1]), p.scale2, -shift));
-                    part[k % 4] += a;
-                    part[k % 4 + 1] += b;
-                    packed[k / 2] = pack<T>(a, b);
+                    for (int k = 0; k < 4; ++k) best[k] = max3(best[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+                const float now_top = fmaxf(max3(best[0], best[1], best[2]), best[3]);
+                // the maximum in use follows only where the new one is more than 2^8 above: P stays below 2^8, and O is seldom rescaled
+                const bool up = now_top != top && ((now_top - top) * p.scale2 > 8.f || top == -INFINITY);
+                const bool any = __any_sync(~0u, up);
+                const float by = up ? exp2_fast((top - now_top) * p.scale2) : 1.f;
+                if (up) top = now_top;
+                sum *= by;
+                const float shift = top == -INFINITY ? 0.f : -top * p.scale2;
+                const Pair shifts = pair_of(shift, shift);
+                Pair part[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int q = 0; q < 2; ++q) {
+                        const int c0 = half * 64 + q * 32;
+                        if (k0 + c0 > any_high || k0 + c0 + 31 < any_low) {         // none of the warp's rows sees any of these 32 keys
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) packed[q * 16 + c] = 0u;
+                        } else {
+#pragma unroll
+                            for (int c = 0; c < 32; c += 2) {
+                                float a, b;
+                                split(fma_pair(pair_of(__uint_as_float(r[c0 + c]), __uint_as_float(r[c0 + c + 1])), scale2, shifts), a, b);
+                                a = exp2_fast(a);
+                                b = exp2_fast(b);
+                                part[c / 2 % 2] = add_pair(part[c / 2 % 2], pair_of(a, b));
+                                packed[q * 16 + c / 2] = pack<T>(a, b);
+                            }
+                        }
+                    }
+                    if (half == 0) {
+                        // P V of the step before: P and O are free to be written
+                        if (n > 0 && !(fine = warp_wait(&o_done[set], (n - 1) & 1, &lost))) break;
+                        if (any && j > 0) {
+                            fence_after();
+#pragma unroll
+                            for (int c = 0; c < DP; c += 32) {
+                                uint32_t o[32];
+                                tensor_load(mine + F::kOut + c, o);
+                                wait_loads();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                                tensor_store(mine + F::kOut + c, o);
+                            }
+                        }
+                    }
+                    tensor_store(mine + F::kProb + half * 32, packed);
+                    wait_stores();
+                    fence_before();
+                    barrier_arrive(&p_full[set][half]);
                 }
-                tensor_store(mine + F::kProb + c / 2, packed);
+                if (!fine) break;
+                float x, y;
+                split(add_pair(part[0], part[1]), x, y);
+                sum += x + y;
             }
-            sum += (part[0] + part[1]) + (part[2] + part[3]);
-            wait_stores();
-            fence_before();
-            barrier_arrive(&p_full);
+            if (fine) fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
+            fence_after();
+            // through shared memory, so that rows leave in whole lines and, where the tile is one of their own, the next job need not wait for them
+            unsigned char* const tile = shared + F::kStaged + set * F::kTile;
+            if (F::kApart) {
+                if (row == 0) wait_stores_read();
+                meet(1 + set, kRows);
+            }
+            stage_row<T, DP>(mine + F::kOut, fine ? 1.f / sum : nan_value(), tile, row, &o_empty[set]);
+            fence_shared();
+            meet(1 + set, kRows);
+            if (row == 0) {
+                if (first <= last) {
+#pragma unroll
+                    for (int c = 0; c < DP; c += 64)
+                        if (c < p.dim) store_tile(&map_o, tile + c / 64 * kRows * 128, c, head, first);
+                    stores_end();
+                }
+                if (!F::kApart) {
+                    wait_stores_read();
+                    barrier_arrive(&q_empty[0]);
+                }
+            }
+            if (live && p.lse != nullptr) p.lse[head * p.pitch + i] = fine ? fmaf(top, p.scale2, log2f(sum)) : nan_value();
         }
-        fine = fine && warp_wait(&o_done, (count - 1) & 1, &lost);
-        fence_after();
-        T* out = live ? static_cast<T*>(p.out) + ((int64_t)i * p.heads_q + head) * p.dim : nullptr;
-        store_row<T, DP>(mine + F::kOut, fine ? 1.f / sum : nan_value(), p.dim, out);
-        if (live && p.lse != nullptr) p.lse[head * p.pitch + i] = fine ? fmaf(top, p.scale2, log2f(sum)) : nan_value();
+        if (row == 0) wait_stores_done();
     }
     __syncwarp();
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 5) tensor_free<256>(tensor);
+    if (warp == 9) tensor_free<512>(tensor);
 }
 
 // ---- backwards: gradients of the queries -------------------------------------------------------------------------------
@@ -269,11 +460,9 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const int tiles = (int)((p.tokens + kRows - 1) / kRows), tile = tiles - 1 - (int)(blockIdx.x / p.heads_q), head = blockIdx.x % p.heads_q;
-    const int key_head = head / (p.heads_q / p.heads_k);
-    const int i0 = tile * kRows, last = (int)min((int64_t)i0 + kRows, p.tokens) - 1;
-    const int j0 = first_key(p, i0), count = (last - j0) / kStream + 1;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
+    const QueryJob job(p, blockIdx.x);
+    const int head = job.head, key_head = head / (p.heads_q / p.heads_k), i0 = job.i0, last = job.last, j0 = job.j0, count = job.count;
     if (threadIdx.x == 0) {
         lost = 0;
         barrier_init(&q_full, 1);
@@ -309,11 +498,11 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
             for (int b = max(0, j - F::kStages); b < j; ++b) drain(&full[b % F::kStages], b / F::kStages & 1);
         }
     } else if (warp == 5) {
-        if (lane == 0) {
-            bool fine = barrier_wait(&q_full, 0, &lost);
+        {
+            bool fine = warp_wait(&q_full, 0, &lost);
             auto scores = [&](int j) {
                 const int s = j % F::kStages;
-                if (!barrier_wait(&full[s], j / F::kStages & 1, &lost)) return false;
+                if (!warp_wait(&full[s], j / F::kStages & 1, &lost)) return false;
                 fence_after();
                 multiply_rows<T, kStream, DP>(base, q_at, kv_at + 2 * s * F::kPart);
                 multiply_rows<T, kStream, DP>(base + F::kGrad, do_at, kv_at + (2 * s + 1) * F::kPart);
@@ -323,20 +512,20 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
             fine = fine && scores(0);
             for (int j = 0; fine && j < count; ++j) {
                 const int s = j % F::kStages;
-                if (!barrier_wait(&p_full, j & 1, &lost)) break;
+                if (!warp_wait(&p_full, j & 1, &lost)) break;
                 fence_after();
                 if (F::kApart && j + 1 < count && !(fine = scores(j + 1))) break;
                 multiply_columns<T, kStream, DP>(base + F::kOut, base + F::kProb, kv_at + 2 * s * F::kPart, j != 0);
                 commit(&empty[s]);
                 commit(&o_done);
-                if (!F::kApart && j + 1 < count) fine = barrier_wait(&o_done, j & 1, &lost) && scores(j + 1);
+                if (!F::kApart && j + 1 < count) fine = warp_wait(&o_done, j & 1, &lost) && scores(j + 1);
             }
             commit(&ended);
             drain(&ended, 0);
         }
     } else {
         const int i = i0 + threadIdx.x;
-        const bool live = i < p.tokens;
+        const bool live = i <= last;
         const int low = live ? first_key(p, i) : 0, high = live ? i : -1;
         const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
         // D = dO . O of the thread's row, which the keys' kernel reads after this one
@@ -416,10 +605,10 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     const int tile = blockIdx.x / p.heads_k, key_head = blockIdx.x % p.heads_k, group = p.heads_q / p.heads_k;        // the longest are the first ones
-    const int j0 = tile * kRows, last = (int)min((int64_t)j0 + kRows, p.tokens) - 1;
-    const int each = (past_query(p, last) - 1 - j0) / kStream + 1, count = each * group;
+    const int j0 = tile * p.span, last = (int)min((int64_t)j0 + p.span, p.tokens) - 1;
+    const int i0 = j0 & ~3, each = (past_query(p, last) - 1 - i0) / kStream + 1, count = each * group;          // from a multiple of 16 bytes of the statistics on
     if (threadIdx.x == 0) {
         lost = 0;
         barrier_init(&k_full, 1);
@@ -444,7 +633,7 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
             load_panels<kRows, DP>(shared + F::kTile, &map_v, &k_full, key_head, j0);
             int n = 0;
             for (; n < count; ++n) {
-                const int s = n % F::kStages, turn = n / F::kStages, head = key_head * group + n / each, i = j0 + n % each * kStream;
+                const int s = n % F::kStages, turn = n / F::kStages, head = key_head * group + n / each, i = i0 + n % each * kStream;
                 if (turn > 0 && !barrier_wait(&empty[s], (turn - 1) & 1, &lost)) break;
                 barrier_expect(&full[s], 2 * F::kPart + 2 * kStream * 4);
                 unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
@@ -457,11 +646,11 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
             for (int b = max(0, n - F::kStages); b < n; ++b) drain(&full[b % F::kStages], b / F::kStages & 1);
         }
     } else if (warp == 5) {
-        if (lane == 0) {
-            bool fine = barrier_wait(&k_full, 0, &lost);
+        {
+            bool fine = warp_wait(&k_full, 0, &lost);
             auto scores = [&](int n) {
                 const int s = n % F::kStages;
-                if (!barrier_wait(&full[s], n / F::kStages & 1, &lost)) return false;
+                if (!warp_wait(&full[s], n / F::kStages & 1, &lost)) return false;
                 fence_after();
                 multiply_rows<T, kStream, DP>(base, k_at, part_at + 2 * s * F::kPart);
                 multiply_rows<T, kStream, DP>(base + F::kGrad, v_at, part_at + (2 * s + 1) * F::kPart);
@@ -471,26 +660,26 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
             fine = fine && scores(0);
             for (int n = 0; fine && n < count; ++n) {
                 const int s = n % F::kStages;
-                if (!barrier_wait(&p_full, n & 1, &lost)) break;
+                if (!warp_wait(&p_full, n & 1, &lost)) break;
                 fence_after();
                 if (F::kApart && n + 1 < count && !(fine = scores(n + 1))) break;
                 multiply_columns<T, kStream, DP>(base + F::kValue, base + F::kProb, part_at + (2 * s + 1) * F::kPart, n != 0);
                 multiply_columns<T, kStream, DP>(base + F::kKey, base + F::kProbGrad, part_at + 2 * s * F::kPart, n != 0);
                 commit(&empty[s]);
                 commit(&o_done);
-                if (!F::kApart && n + 1 < count) fine = barrier_wait(&o_done, n & 1, &lost) && scores(n + 1);
+                if (!F::kApart && n + 1 < count) fine = warp_wait(&o_done, n & 1, &lost) && scores(n + 1);
             }
             commit(&ended);
             drain(&ended, 0);
         }
     } else {
         const int j = j0 + threadIdx.x;
-        const bool live = j < p.tokens;
+        const bool live = j <= last;
         const int low = live ? j : 0, high = live ? past_query(p, j) - 1 : -1;          // the queries that see the key
         const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
         bool fine = true;
         for (int n = 0; n < count; ++n) {
-            const int s = n % F::kStages, i = j0 + n % each * kStream;
+            const int s = n % F::kStages, i = i0 + n % each * kStream;
             // the statistics came with the tile that the scores waited for; this wait makes them visible here, too
             if (!(fine = warp_wait(&full[s], n / F::kStages & 1, &lost) && warp_wait(&s_full, n & 1, &lost))) break;
             fence_after();
@@ -562,7 +751,14 @@ static bool map_of(CUtensorMap* map, uint32_t dtype, const void* p, int64_t dim,
                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int64_t attention_pitch(int64_t tokens) { return (tokens + kRows - 1) / kRows * kRows; }
+// A multiple of 16 bytes, and a streamed tile that begins at the last token ends within it.
+int64_t attention_pitch(int64_t tokens) { return (tokens + kStream + 3) / 4 * 4; }
+
+// Whole rows to a tile where rows of one length fill three quarters of it: queries then meet their keys within their own tile.
+static int tile_span(const nuka_b200_episodes_t& plan) {
+    const int64_t whole = plan.length > 0 && plan.length <= kRows ? kRows / plan.length * plan.length : 0;
+    return 4 * whole >= 3 * kRows ? (int)whole : kRows;
+}
 
 template <typename K> static cudaError_t with_shared(K kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 
@@ -571,18 +767,19 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
     const nuka_b200_episodes_t& e = *d.plan;
     p.first = e.first; p.end = e.end; p.tokens = e.tokens; p.pitch = attention_pitch(e.tokens);
     p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens);
+    p.span = tile_span(e); p.tiles = (int)((e.tokens + p.span - 1) / p.span);
     p.scale = d.scale; p.scale2 = d.scale * kLog2e;
     p.out = d.out; p.lse = d.lse; p.dout = d.dout; p.delta = d.delta; p.dq = d.dq; p.dk = d.dk; p.dv = d.dv;
     if (encoder() == nullptr) return cudaErrorNotSupported;
-    const int64_t tiles = (e.tokens + kRows - 1) / kRows;
-    CUtensorMap q, k, v, g;
+    CUtensorMap q, k, v, g, o;
     if (!backward) {
         // first, because it makes the device's context the thread's own: maps cannot be encoded without one
         cudaError_t set = with_shared(attention_kernel<T, DP>, Forward<DP>::kShared);
         if (set != cudaSuccess) return set;
         if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, kRows) || !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, kRows) ||
-            !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, kRows)) return cudaErrorInvalidValue;
-        attention_kernel<T, DP><<<(unsigned)(tiles * d.heads_q), kBlock, Forward<DP>::kShared, stream>>>(q, k, v, p);
+            !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, kRows) || !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, p.span))
+            return cudaErrorInvalidValue;
+        attention_kernel<T, DP><<<(unsigned)std::min(ForwardJob::all(p), 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();
     }
     for (int keys = 0; keys < 2; ++keys) {
@@ -592,8 +789,8 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
         if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, own) || !map_of(&g, d.dtype, d.dout, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, own) ||
             !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, other) || !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, other))
             return cudaErrorInvalidValue;
-        if (keys) key_grad_kernel<T, DP><<<(unsigned)(tiles * d.heads_k), kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, p);
-        else query_grad_kernel<T, DP><<<(unsigned)(tiles * d.heads_q), kBlock, Queries<DP>::kShared, stream>>>(q, g, k, v, p);
+        if (keys) key_grad_kernel<T, DP><<<(unsigned)(p.tiles * d.heads_k), kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, p);
+        else query_grad_kernel<T, DP><<<(unsigned)(p.tiles * d.heads_q), kBlock, Queries<DP>::kShared, stream>>>(q, g, k, v, p);
         set = cudaGetLastError();
         if (set != cudaSuccess) return set;
     }

@@ -131,7 +131,7 @@ static nuka_result_t Attention(const nuka_b200_attention_t* desc, bool backward,
     if (d.window < 0) return Invalid("window must not be negative");
     if (!(d.scale > 0.f) || d.scale > 3.0e38f) return Invalid("scale must be greater than 0 and finite");
     if (d.plan->tokens == 0) return NUKA_RESULT_OK;
-    if ((d.plan->tokens / 128 + 1) * d.heads_q > (1ll << 31) - 1) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times heads");
+    if ((d.plan->tokens / 64 + 1) * d.heads_q > (1ll << 30)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times heads");
     for (const void* p : {d.q, d.k, d.v, static_cast<const void*>(d.out)}) {
         if (p == nullptr) return Invalid("q, k, v or out is null");
         if (!Aligned(p, 16)) return Invalid("a tensor does not lie on 16 bytes");

@@ -44,6 +44,15 @@ __device__ __forceinline__ void load_tile(void* to, const CUtensorMap* map, uint
 __device__ __forceinline__ void load_bytes(void* to, const void* from, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(shared_address(to)), "l"(from), "r"(bytes), "r"(shared_address(bar)) : "memory");
 }
+// a tile out of shared memory, which is written by the thread's group of stores; what lies outside the tensor is left out
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, const void* from, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(map), "r"(shared_address(from)), "r"(x), "r"(y), "r"(z) : "memory");
+}
+__device__ __forceinline__ void stores_end() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void wait_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }        // their shared memory may be written again
+__device__ __forceinline__ void wait_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }              // ordinary stores before, TMA after
+__device__ __forceinline__ void meet(int which, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(which), "r"(threads) : "memory"); }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- tensor memory ------------------------------------------------------------------------------------------------------
@@ -87,20 +96,70 @@ __device__ __forceinline__ uint64_t outer_rows(uint32_t address, uint32_t panel)
 template <typename T> __host__ __device__ constexpr uint32_t product_of(int n, bool b_outer) {
     return 1u << 4 | (sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? (1u << 7 | 1u << 10) : 0u) | (b_outer ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
+// The whole warp calls these, and one lane of it issues: inside a branch of one lane the compiler cannot keep the operands in uniform registers, and moving them there takes
+// longer than the product (75 cycles an instruction in place of MMAC).
 __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(what), "r"((uint32_t)add) : "memory");
+    asm volatile("{ .reg .pred e, p; elect.sync _|e, 0xffffffff; setp.ne.u32 p, %4, 0; @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(what),
+                 "r"((uint32_t)add) : "memory");
 }
 // A from tensor memory, two values to a column
 __device__ __forceinline__ void multiply_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t what, bool add) {
-    asm volatile("{ .reg .pred p; setp.ne.u32 p, %4, 0; tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(what), "r"((uint32_t)add) : "memory");
+    asm volatile("{ .reg .pred e, p; elect.sync _|e, 0xffffffff; setp.ne.u32 p, %4, 0; @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(what),
+                 "r"((uint32_t)add) : "memory");
 }
-// the barrier completes when the thread's products so far have
-__device__ __forceinline__ void commit(uint64_t* bar) { asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(shared_address(bar)) : "memory"); }
+// the barrier completes when the products that the warp issued so far have
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("{ .reg .pred e; elect.sync _|e, 0xffffffff; @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(shared_address(bar)) : "memory");
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// two 32-bit values at a time
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair_of(float low, float high) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(low), "f"(high));
+    return r;
+}
+__device__ __forceinline__ void split(Pair p, float& low, float& high) { asm("mov.b64 {%0, %1}, %2;" : "=f"(low), "=f"(high) : "l"(p)); }
+__device__ __forceinline__ Pair fma_pair(Pair a, Pair b, Pair c) {
+    Pair r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ Pair add_pair(Pair a, Pair b) {
+    Pair r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Pair mul_pair(Pair a, Pair b) {
+    Pair r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 2^x of two values by multiplications and additions, for x up to 127: the integer part goes into the exponent, 2^f of the rest, between -1/2 and 1/2, is the
+// polynomial of degree 4 with the least largest relative error there (2.6e-6; a linear programme over 2001 points). Below -126 it is 2^-126.
+__device__ __forceinline__ void exp2_pair(Pair x, float& a, float& b) {
+    split(x, a, b);
+    const Pair y = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f)), magic = pair_of(12582912.f, 12582912.f), minus = pair_of(-12582912.f, -12582912.f);
+    const Pair whole = add_pair(y, magic), back = add_pair(whole, minus), one = pair_of(-1.f, -1.f), f = fma_pair(back, one, y);
+    Pair r = fma_pair(pair_of(0.009570085443556309f, 0.009570085443556309f), f, pair_of(0.0559178926050663f, 0.0559178926050663f));
+    r = fma_pair(r, f, pair_of(0.2402474582195282f, 0.2402474582195282f));
+    r = fma_pair(r, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
+    r = fma_pair(r, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
+    float u, v, m, n;
+    split(r, u, v);
+    split(whole, m, n);
+    a = __int_as_float(__float_as_int(u) + (__float_as_int(m) << 23));
+    b = __int_as_float(__float_as_int(v) + (__float_as_int(n) << 23));
 }
 template <typename T> __device__ __forceinline__ uint32_t pack(float low, float high);
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float low, float high) {

@@ -129,6 +129,24 @@ def test_rollouts_with_episodes_that_end_inside():
     _check(q, k, v, plan, do)
 
 
+@pytest.mark.parametrize("rows,length", [(300, 1), (90, 3), (50, 24), (11, 37), (5, 100), (3, 128), (2, 129)])
+@pytest.mark.parametrize("dim,dtype", [(64, torch.bfloat16), (128, torch.float16)])
+def test_rows_of_one_length(rows, length, dim, dtype):
+    """Rows that share a tile whole, with and without a remainder of the tile, and rows that are too long for it."""
+    plan = S.Episodes.from_done(torch.rand((rows, length), generator=_gen(rows), device="cuda") < 0.03)
+    q, k, v, do = _inputs(_gen(length), plan.tokens, 4, 2, dim, dtype)
+    _check(q, k, v, plan, do, window=None if length != 37 else 9)
+
+
+def test_more_jobs_than_blocks():
+    """Blocks that take several tiles and heads in turn, of very different lengths."""
+    plan = _plan_of([900, 3, 0, 1, 1300, 40, 700, 129])
+    q, k, v, do = _inputs(_gen(20), plan.tokens, 32, 4, 64, torch.bfloat16)
+    _check(q, k, v, plan, do)
+    q, k, v, do = _inputs(_gen(21), plan.tokens, 24, 24, 72, torch.bfloat16)
+    _check(q, k, v, plan, do, window=300)
+
+
 @pytest.mark.parametrize("size,scale", [(8.0, None), (1.0, 1.0), (1.0, 1e-3)])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_sharp_and_flat_softmax(size, scale, dim):

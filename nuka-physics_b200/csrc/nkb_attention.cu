@@ -143,23 +143,23 @@ __device__ __forceinline__ unsigned char* aligned_shared() { return dynamic_shar
 // ---- forwards ---------------------------------------------------------------------------------------------------------
 // A block takes jobs in turn: two tiles of queries, of two heads that share a key head or else of two neighbouring stretches of tokens, that meet the same keys, so that a tile of
 // keys and values is loaded once for 256 rows.  While one tile's rows are at their exponentials the tensor cores work for the other's. Loads run ahead
-// into the next job while the rows of the present one end. A row's 128 scores are taken into registers at once; where tensor memory has room for P beside them (dim up to 64)
-// the next scores then are multiplied while the exponentials go on, else P takes their place. P goes to its product in two halves, so that the first is under way during the second's exponentials.
-constexpr int kForward = 384;                           // two times four warps of rows, one that multiplies, one that loads, two that do nothing
+// into the next job while the rows of the present one end. A row's scores of a step are taken into registers at once, so that the next step's are multiplied while its
+// exponentials go on.
+constexpr int kForward = 384;                           // two times four warps of rows, two that multiply, two that load
 template <int N> struct Number { static constexpr int value = N; };
 
 template <int DP> struct Forward {
-    static constexpr bool kApart = DP == 64;
+    // keys of a step: as many as leave tensor memory room for the scores, P beside them and O, twice
+    static constexpr int kStep = DP == 64 ? 128 : 80;
     static constexpr int kQueries = DP == 64 ? 2 : 1, kStages = DP == 64 ? 3 : 2;              // buffers
-    static constexpr int kTile = kRows * DP * 2;
-    // rows leave through tiles of their own, or where there is no room through their queries' place
-    static constexpr int kKeys = 2 * kQueries * kTile, kStaged = kApart ? kKeys + 2 * kStages * kTile : 0, kShared = kKeys + 2 * kStages * kTile + (kApart ? 2 * kTile : 0) + 1024;
-    static constexpr int kProb = kApart ? kRows : 0, kOut = kApart ? kRows + kRows / 2 : kRows, kSet = 256;     // columns; the scores are at 0
+    static constexpr int kTile = kRows * DP * 2, kPart = kStep * DP * 2;
+    static constexpr int kKeys = 2 * kQueries * kTile, kStaged = kKeys + 2 * kStages * kPart, kShared = kStaged + 2 * kTile + 1024;
+    static constexpr int kProb = kStep, kOut = kStep + kStep / 2, kSet = 256;                  // columns; the scores are at 0
 };
 
 struct ForwardJob {
     int i0[2], last[2], head[2], j0, count;             // queries i0 to last (none if below i0), keys from j0 on in `count` steps
-    __device__ __forceinline__ ForwardJob(const AttentionParams& p, int job) {
+    __device__ __forceinline__ ForwardJob(const AttentionParams& p, int job, int step) {
         const bool by_heads = p.heads_q / p.heads_k % 2 == 0;
         const int across = by_heads ? p.heads_q / 2 : p.heads_q, along = by_heads ? p.tiles : (p.tiles + 1) / 2, at = along - 1 - job / across;       // the longest first
         for (int s = 0; s < 2; ++s) {
@@ -168,7 +168,7 @@ struct ForwardJob {
             last[s] = (int)min((int64_t)i0[s] + p.span, p.tokens) - 1;
         }
         j0 = first_key(p, i0[0]);
-        count = (max(last[0], last[1]) - j0) / kRows + 1;
+        count = (max(last[0], last[1]) - j0) / step + 1;
     }
     static __host__ __device__ __forceinline__ int all(const AttentionParams& p) { return p.heads_q / p.heads_k % 2 == 0 ? p.tiles * (p.heads_q / 2) : (p.tiles + 1) / 2 * p.heads_q; }
     // Every other round backwards, so that the longest of one round goes with the shortest of the next.
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                                                                 const __grid_constant__ CUtensorMap map_o, const AttentionParams p) {
     using F = Forward<DP>;
     __shared__ uint64_t q_full[F::kQueries], q_empty[F::kQueries], k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages];
-    __shared__ uint64_t s_full[2], s_empty[2], p_full[2][2], o_done[2], o_empty[2], ended;
+    __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], o_empty[2], ended[2];
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
@@ -192,120 +192,115 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         for (int s = 0; s < 2; ++s) {
             barrier_init(&s_full[s], 1);
             barrier_init(&s_empty[s], kRows);
-            barrier_init(&p_full[s][0], kRows);
-            barrier_init(&p_full[s][1], kRows);
+            barrier_init(&p_full[s], kRows);
             barrier_init(&o_done[s], 1);
             barrier_init(&o_empty[s], kRows);
+            barrier_init(&ended[s], 1);
         }
-        barrier_init(&ended, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    if (warp == 9) tensor_alloc<512>(&tensor);
+    if (warp == 10) tensor_alloc<512>(&tensor);
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t base = tensor, q_at = shared_address(shared), k_at = q_at + F::kKeys, v_at = k_at + F::kStages * F::kTile;
+    // what the multiplying warp's loops depend on comes by shuffles from one lane: the compiler then knows it to be the same for all and keeps it in uniform registers
+    const uint32_t base = __shfl_sync(~0u, tensor, 0), q_at = shared_address(shared), k_at = q_at + F::kKeys, v_at = k_at + F::kStages * F::kPart;
     const int jobs = ForwardJob::all(p);
     // registers: 128 x (2 x 200 + 104) of the 384 x 168 that the block has
 
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-    if (warp == 9) {
+    if (warp == 10) {
         if (lane == 0) {
-            int queries = 0, keys = 0, values = 0;      // loads begun so far
+            // queries and keys; values are another warp's, so that keys do not wait for the room that values wait for
+            int queries = 0, keys = 0;                  // loads begun so far
             bool fine = true;
-            ForwardJob next(p, blockIdx.x);
+            ForwardJob next(p, blockIdx.x, F::kStep);
             for (int turn = 0, job = blockIdx.x; fine && job < jobs; job = ForwardJob::of_turn(++turn)) {
                 const ForwardJob now = next;
                 const int after = ForwardJob::of_turn(turn + 1);
-                if (after < jobs) next = ForwardJob(p, after);
+                if (after < jobs) next = ForwardJob(p, after, F::kStep);
                 const int b = queries % F::kQueries, key_head = now.head[0] / (p.heads_q / p.heads_k);
                 if (queries >= F::kQueries && !(fine = barrier_wait(&q_empty[b], (queries / F::kQueries - 1) & 1, &lost))) break;
                 barrier_expect(&q_full[b], 2 * F::kTile);
                 for (int s = 0; s < 2; ++s) load_panels<kRows, DP>(shared + (2 * b + s) * F::kTile, &map_q, &q_full[b], now.head[s], now.i0[s]);
                 ++queries;
-                for (int j = 0; j < now.count; ++j) {
+                for (int j = 0; j < now.count; ++j, ++keys) {
                     const int s = keys % F::kStages, round = keys / F::kStages;
                     if (round > 0 && !(fine = barrier_wait(&k_empty[s], (round - 1) & 1, &lost))) break;
-                    barrier_expect(&k_full[s], F::kTile);
-                    load_panels<kRows, DP>(shared + F::kKeys + s * F::kTile, &map_k, &k_full[s], key_head, now.j0 + j * kRows);
-                    ++keys;
-                    if (round > 0 && !(fine = barrier_wait(&v_empty[s], (round - 1) & 1, &lost))) break;
-                    barrier_expect(&v_full[s], F::kTile);
-                    load_panels<kRows, DP>(shared + F::kKeys + (F::kStages + s) * F::kTile, &map_v, &v_full[s], key_head, now.j0 + j * kRows);
-                    ++values;
+                    barrier_expect(&k_full[s], F::kPart);
+                    load_panels<F::kStep, DP>(shared + F::kKeys + s * F::kPart, &map_k, &k_full[s], key_head, now.j0 + j * F::kStep);
                 }
             }
             drain_ring(q_full, F::kQueries, queries);
             drain_ring(k_full, F::kStages, keys);
+        }
+    } else if (warp == 11) {
+        if (lane == 0) {
+            int values = 0;
+            bool fine = true;
+            ForwardJob next(p, blockIdx.x, F::kStep);
+            for (int turn = 0, job = blockIdx.x; fine && job < jobs; job = ForwardJob::of_turn(++turn)) {
+                const ForwardJob now = next;
+                const int after = ForwardJob::of_turn(turn + 1);
+                if (after < jobs) next = ForwardJob(p, after, F::kStep);
+                const int key_head = now.head[0] / (p.heads_q / p.heads_k);
+                for (int j = 0; j < now.count; ++j, ++values) {
+                    const int s = values % F::kStages, round = values / F::kStages;
+                    if (round > 0 && !(fine = barrier_wait(&v_empty[s], (round - 1) & 1, &lost))) break;
+                    barrier_expect(&v_full[s], F::kPart);
+                    load_panels<F::kStep, DP>(shared + F::kKeys + (F::kStages + s) * F::kPart, &map_v, &v_full[s], key_head, now.j0 + j * F::kStep);
+                }
+            }
             drain_ring(v_full, F::kStages, values);
         }
-    } else if (warp == 8) {
-        {
-            // One warp for both tiles, so that one's products run as a whole before the other's: issued side by side they take turns, and both tiles wait and both are at
-            // their exponentials at the same time.
-            struct Cursor { int turn, job, j, count, ahead; } at[2];
-            bool fine = true;
-            for (int set = 0; set < 2; ++set) at[set] = {0, (int)blockIdx.x, 0, 0, 0};
-            auto scores = [&](auto which) {
-                constexpr int set = decltype(which)::value;
-                Cursor& a = at[set];
-                const int b = a.turn % F::kQueries;
-                if (a.j == 0) {
-                    a.count = ForwardJob(p, a.job).count;
-                    if (!warp_wait(&q_full[b], a.turn / F::kQueries & 1, &lost)) return false;
-                }
-                const int s = a.ahead % F::kStages;
-                if (!warp_wait(&k_full[s], a.ahead / F::kStages & 1, &lost)) return false;
-                if (a.ahead > 0 && !warp_wait(F::kApart ? &s_empty[set] : &o_done[set], (a.ahead - 1) & 1, &lost)) return false;
-                fence_after();
-                multiply_rows<T, kRows, DP>(base + set * F::kSet, q_at + (2 * b + set) * F::kTile, k_at + s * F::kTile);
-                commit(&s_full[set]);
-                commit(&k_empty[s]);
-                ++a.ahead;
-                if (++a.j == a.count) {
-                    if (F::kApart) commit(&q_empty[b]);
-                    a.j = 0;
-                    a.job = ForwardJob::of_turn(++a.turn);
-                }
-                return true;
-            };
-            int n = 0, done = 0, steps = 0;
-            // one step of one tile: i of its job
-            auto step = [&](auto which, int i) {
-                constexpr int set = decltype(which)::value;
-                const int s = n % F::kStages;
-                if (F::kApart && i + 1 < steps && !scores(which)) return false;
-                if (!warp_wait(&p_full[set][0], n & 1, &lost)) return false;
-                if (i == 0 && done > 0 && !warp_wait(&o_empty[set], (done - 1) & 1, &lost)) return false;
-                if (!warp_wait(&v_full[s], n / F::kStages & 1, &lost)) return false;
-                fence_after();
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    if (half == 1) {
-                        if (!warp_wait(&p_full[set][1], n & 1, &lost)) return false;
-                        fence_after();
-                    }
-#pragma unroll
-                    for (int k = half * 64; k < half * 64 + 64; k += 16)
-                        multiply_tensor(base + set * F::kSet + F::kOut, base + set * F::kSet + F::kProb + k / 2, outer_rows(v_at + s * F::kTile + k * 128, kRows * 128), product_of<T>(DP, true),
-                                        i != 0 || k != 0);
-                }
-                commit(&v_empty[s]);
-                commit(&o_done[set]);
-                return F::kApart || i + 1 == steps || scores(which);
-            };
-            fine = scores(Number<0>{}) && scores(Number<1>{});
-            for (int own = blockIdx.x; fine && own < jobs; own = ForwardJob::of_turn(++done)) {
-                steps = at[0].count;                    // of the job that the scores have just begun
-                for (int i = 0; fine && i < steps; ++i, ++n) fine = step(Number<0>{}, i) && step(Number<1>{}, i);
-                // across a job's end when its last products are under way: the next one's queries may come only when both tiles' rows have left
-                if (fine && at[0].job < jobs) fine = scores(Number<0>{}) && scores(Number<1>{});
+    } else if (warp < 10) {
+        const int set = warp - 8;
+        const uint32_t columns = base + set * F::kSet, q_set = q_at + set * F::kTile;
+        int job = blockIdx.x, turn = 0, j = 0, count = 0, ahead = 0;                               // of the scores, one step ahead of P V
+        int k_stage = 0, k_phase = 0, v_stage = 0, v_phase = 0, q_buffer = 0, q_phase = 0;
+        auto scores = [&]() {
+            if (j == 0) {
+                count = __shfl_sync(~0u, ForwardJob(p, job, F::kStep).count, 0);
+                if (!warp_wait(&q_full[q_buffer], q_phase, &lost)) return false;
             }
-            commit(&ended);
-            drain(&ended, 0);
+            if (!warp_wait(&k_full[k_stage], k_phase, &lost)) return false;
+            if (ahead > 0 && !warp_wait(&s_empty[set], (ahead - 1) & 1, &lost)) return false;
+            fence_after();
+            multiply_rows<T, F::kStep, DP>(columns, q_set + 2 * q_buffer * F::kTile, k_at + k_stage * F::kPart);
+            commit(&s_full[set]);
+            commit(&k_empty[k_stage]);
+            ++ahead;
+            if (++k_stage == F::kStages) { k_stage = 0; k_phase ^= 1; }
+            if (++j == count) {
+                commit(&q_empty[q_buffer]);
+                j = 0;
+                if (++q_buffer == F::kQueries) { q_buffer = 0; q_phase ^= 1; }
+                job = ForwardJob::of_turn(++turn);
+            }
+            return true;
+        };
+        int n = 0, done = 0;
+        bool fine = scores();
+        for (int own = blockIdx.x; fine && own < jobs; own = ForwardJob::of_turn(++done)) {
+            const int steps = count;                    // of the job that the scores have just begun
+            for (int i = 0; i < steps; ++i, ++n) {
+                if (i + 1 < steps && !(fine = scores())) break;
+                if (!(fine = warp_wait(&p_full[set], n & 1, &lost))) break;
+                if (i == 0 && done > 0 && !(fine = warp_wait(&o_empty[set], (done - 1) & 1, &lost))) break;
+                if (!(fine = warp_wait(&v_full[v_stage], v_phase, &lost))) break;
+                fence_after();
+                multiply_columns<T, F::kStep, DP>(columns + F::kOut, columns + F::kProb, v_at + v_stage * F::kPart, i != 0);
+                commit(&v_empty[v_stage]);
+                commit(&o_done[set]);
+                if (++v_stage == F::kStages) { v_stage = 0; v_phase ^= 1; }
+            }
+            // across a job's end when its last product is under way: the next one's queries may still be on theirs
+            if (fine && job < jobs) fine = scores();
         }
+        commit(&ended[set]);
+        drain(&ended[set], 0);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
@@ -314,7 +309,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         const Pair scale2 = pair_of(p.scale2, p.scale2);
         bool fine = true;
         int n = 0;
-        ForwardJob next(p, blockIdx.x);
+        ForwardJob next(p, blockIdx.x, F::kStep);
         auto low_of = [&](const ForwardJob& job) { return job.i0[set] + row <= job.last[set] ? first_key(p, job.i0[set] + row) : 0; };
         int next_low = low_of(next);
         for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
@@ -322,115 +317,106 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             const bool live = i <= last;
             const int high = live ? i : -1;
             const int after = ForwardJob::of_turn(turn + 1);
-            if (after < jobs) { next = ForwardJob(p, after); next_low = low_of(next); }
+            if (after < jobs) { next = ForwardJob(p, after, F::kStep); next_low = low_of(next); }
             // keys that any and that all of the warp's rows see; a row that is not there sees none
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
             for (int j = 0; fine && j < count; ++j, ++n) {
-                const int k0 = j0 + j * kRows;
+                const int k0 = j0 + j * F::kStep;
                 if (!(fine = warp_wait(&s_full[set], n & 1, &lost))) break;
                 fence_after();
-                uint32_t r[kRows];
+                uint32_t r[F::kStep];
 #pragma unroll
-                for (int c = 0; c < kRows; c += 32) tensor_load(mine + c, r + c);
+                for (int c = 0; c < F::kStep; c += 16) tensor_load16(mine + c, r + c);
                 wait_loads();
-                if (F::kApart) {
-                    fence_before();
-                    barrier_arrive(&s_empty[set]);
-                }
-                if (k0 < all_low || k0 + kRows - 1 > all_high) {
-#pragma unroll
-                    for (int c = 0; c < kRows; c += 32) {
-                        const uint32_t seen = columns_between(low - k0 - c, high - k0 - c);
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) r[c + k] = seen >> k & 1u ? r[c + k] : 0xff800000u;
-                    }
-                }
-                float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int c = 0; c < kRows; c += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) best[k] = max3(best[k], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
-                const float now_top = fmaxf(max3(best[0], best[1], best[2]), best[3]);
-                // the maximum in use follows only where the new one is more than 2^8 above: P stays below 2^8, and O is seldom rescaled
-                const bool up = now_top != top && ((now_top - top) * p.scale2 > 8.f || top == -INFINITY);
-                const bool any = __any_sync(~0u, up);
-                const float by = up ? exp2_fast((top - now_top) * p.scale2) : 1.f;
-                if (up) top = now_top;
-                sum *= by;
-                const float shift = top == -INFINITY ? 0.f : -top * p.scale2;
-                const Pair shifts = pair_of(shift, shift);
+                fence_before();
+                barrier_arrive(&s_empty[set]);
                 Pair part[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
+                // all: every row of the warp sees every key; else 16 keys at a time may be hidden from all, or from some
+                auto rows = [&](auto all) {
+                    constexpr bool ALL = decltype(all)::value != 0;
+                    auto hidden = [&](int c) { return !ALL && (k0 + c > any_high || k0 + c + 15 < any_low); };
+                    float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t packed[32];
+                    for (int c = 0; c < F::kStep; c += 16) {
+                        if (hidden(c)) continue;
+                        if (!ALL && (k0 + c < all_low || k0 + c + 15 > all_high)) {
+                            const uint32_t seen = columns_between(low - k0 - c, high - k0 - c);
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int c0 = half * 64 + q * 32;
-                        if (k0 + c0 > any_high || k0 + c0 + 31 < any_low) {         // none of the warp's rows sees any of these 32 keys
+                            for (int k = 0; k < 16; ++k) r[c + k] = seen >> k & 1u ? r[c + k] : 0xff800000u;
+                        }
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) packed[q * 16 + c] = 0u;
+                        for (int k = 0; k < 8; ++k) best[k % 4] = max3(best[k % 4], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+                    }
+                    const float now_top = fmaxf(max3(best[0], best[1], best[2]), best[3]);
+                    // the maximum in use follows only where the new one is more than 2^8 above: P stays below 2^8, and O is seldom rescaled
+                    const bool up = now_top != top && ((now_top - top) * p.scale2 > 8.f || top == -INFINITY);
+                    const bool any = __any_sync(~0u, up);
+                    const float by = up ? exp2_fast((top - now_top) * p.scale2) : 1.f;
+                    if (up) top = now_top;
+                    sum *= by;
+                    const float shift = top == -INFINITY ? 0.f : -top * p.scale2;
+                    const Pair shifts = pair_of(shift, shift);
+#pragma unroll
+                    for (int c = 0; c < F::kStep; c += 16) {
+                        uint32_t packed[8];
+                        if (hidden(c)) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) packed[k] = 0u;
                         } else {
 #pragma unroll
-                            for (int c = 0; c < 32; c += 2) {
+                            for (int k = 0; k < 16; k += 2) {
                                 float a, b;
-                                split(fma_pair(pair_of(__uint_as_float(r[c0 + c]), __uint_as_float(r[c0 + c + 1])), scale2, shifts), a, b);
+                                split(fma_pair(pair_of(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), scale2, shifts), a, b);
                                 a = exp2_fast(a);
                                 b = exp2_fast(b);
-                                part[c / 2 % 2] = add_pair(part[c / 2 % 2], pair_of(a, b));
-                                packed[q * 16 + c / 2] = pack<T>(a, b);
+                                part[k / 2 % 2] = add_pair(part[k / 2 % 2], pair_of(a, b));
+                                packed[k / 2] = pack<T>(a, b);
                             }
                         }
-                    }
-                    if (half == 0) {
-                        // P V of the step before: P and O are free to be written
-                        if (n > 0 && !(fine = warp_wait(&o_done[set], (n - 1) & 1, &lost))) break;
-                        if (any && j > 0) {
-                            fence_after();
+                        if (c == 0) {
+                            // P V of the step before: P and O are free to be written
+                            if (n > 0 && !warp_wait(&o_done[set], (n - 1) & 1, &lost)) return false;
+                            if (any && j > 0) {
+                                fence_after();
 #pragma unroll
-                            for (int c = 0; c < DP; c += 32) {
-                                uint32_t o[32];
-                                tensor_load(mine + F::kOut + c, o);
-                                wait_loads();
+                                for (int d = 0; d < DP; d += 32) {
+                                    uint32_t o[32];
+                                    tensor_load(mine + F::kOut + d, o);
+                                    wait_loads();
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-                                tensor_store(mine + F::kOut + c, o);
+                                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                                    tensor_store(mine + F::kOut + d, o);
+                                }
                             }
                         }
+                        tensor_store8(mine + F::kProb + c / 2, packed);
                     }
-                    tensor_store(mine + F::kProb + half * 32, packed);
                     wait_stores();
                     fence_before();
-                    barrier_arrive(&p_full[set][half]);
-                }
-                if (!fine) break;
+                    barrier_arrive(&p_full[set]);
+                    return true;
+                };
+                if (!(fine = k0 >= all_low && k0 + F::kStep - 1 <= all_high ? rows(Number<1>{}) : rows(Number<0>{}))) break;
                 float x, y;
                 split(add_pair(part[0], part[1]), x, y);
                 sum += x + y;
             }
             if (fine) fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
             fence_after();
-            // through shared memory, so that rows leave in whole lines and, where the tile is one of their own, the next job need not wait for them
+            // through shared memory, so that rows leave in whole lines and the next job need not wait for them
             unsigned char* const tile = shared + F::kStaged + set * F::kTile;
-            if (F::kApart) {
-                if (row == 0) wait_stores_read();
-                meet(1 + set, kRows);
-            }
+            if (row == 0) wait_stores_read();
+            meet(1 + set, kRows);
             stage_row<T, DP>(mine + F::kOut, fine ? 1.f / sum : nan_value(), tile, row, &o_empty[set]);
             fence_shared();
             meet(1 + set, kRows);
-            if (row == 0) {
-                if (first <= last) {
+            if (row == 0 && first <= last) {
 #pragma unroll
-                    for (int c = 0; c < DP; c += 64)
-                        if (c < p.dim) store_tile(&map_o, tile + c / 64 * kRows * 128, c, head, first);
-                    stores_end();
-                }
-                if (!F::kApart) {
-                    wait_stores_read();
-                    barrier_arrive(&q_empty[0]);
-                }
+                for (int c = 0; c < DP; c += 64)
+                    if (c < p.dim) store_tile(&map_o, tile + c / 64 * kRows * 128, c, head, first);
+                stores_end();
             }
             if (live && p.lse != nullptr) p.lse[head * p.pitch + i] = fine ? fmaf(top, p.scale2, log2f(sum)) : nan_value();
         }
@@ -440,7 +426,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 9) tensor_free<512>(tensor);
+    if (warp == 10) tensor_free<512>(tensor);
 }
 
 // ---- backwards: gradients of the queries -------------------------------------------------------------------------------
@@ -478,7 +464,8 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t base = tensor, q_at = shared_address(shared), do_at = q_at + F::kTile, kv_at = do_at + F::kTile;
+    // what the multiplying warp's loops depend on comes by shuffles from one lane: the compiler then knows it to be the same for all and keeps it in uniform registers
+    const uint32_t base = __shfl_sync(~0u, tensor, 0), q_at = shared_address(shared), do_at = q_at + F::kTile, kv_at = do_at + F::kTile;
 
     if (warp == 4) {
         if (lane == 0) {
@@ -624,7 +611,7 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t base = tensor, k_at = shared_address(shared), v_at = k_at + F::kTile, part_at = v_at + F::kTile;
+    const uint32_t base = __shfl_sync(~0u, tensor, 0), k_at = shared_address(shared), v_at = k_at + F::kTile, part_at = v_at + F::kTile;
 
     if (warp == 4) {
         if (lane == 0) {
@@ -776,8 +763,8 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
         // first, because it makes the device's context the thread's own: maps cannot be encoded without one
         cudaError_t set = with_shared(attention_kernel<T, DP>, Forward<DP>::kShared);
         if (set != cudaSuccess) return set;
-        if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, kRows) || !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, kRows) ||
-            !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, kRows) || !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, p.span))
+        if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, kRows) || !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, Forward<DP>::kStep) ||
+            !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, Forward<DP>::kStep) || !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, p.span))
             return cudaErrorInvalidValue;
         attention_kernel<T, DP><<<(unsigned)std::min(ForwardJob::all(p), 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();

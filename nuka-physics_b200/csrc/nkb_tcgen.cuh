@@ -81,6 +81,17 @@ __device__ __forceinline__ void tensor_store(uint32_t at, const uint32_t* r) {
                  : "memory");
 }
 
+// 16 columns; 8 columns
+__device__ __forceinline__ void tensor_load16(uint32_t at, uint32_t* r) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+                   "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tensor_store8(uint32_t at, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+
 // ---- products -----------------------------------------------------------------------------------------------------------
 // Operands in shared memory are rows of 128 bytes (64 values), swizzled by the TMA load's 128-byte mode, panels of 64 columns one behind the other.
 // As rows x 64 columns of the product's inner dimension (K-major): 8 rows are 1024 bytes.  The step to the next 16 inner values is 32 bytes.

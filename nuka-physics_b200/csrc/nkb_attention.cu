@@ -31,6 +31,7 @@ struct AttentionParams {
     int64_t tokens, pitch;                              // pitch: floats between the heads' rows of lse and delta
     int heads_q, heads_k, dim, window;                  // window 0: all of the episode
     int span, tiles;                                    // tokens of a tile, at most 128, and how many tiles
+    int by_heads, across, along;                        // of the forward kernel's jobs: tiles of two heads or of two stretches of tokens; jobs side by side, and behind one another
     float scale, scale2;                                // scale2: times log2(e)
     void *out, *dq, *dk, *dv;
     const void* dout;
@@ -103,17 +104,13 @@ __device__ __forceinline__ uint32_t columns_between(int from, int to) {
 
 // A row of 64-column panels of 128 rows, swizzled as TMA takes it: 16 bytes number `k` of row `row`.
 __device__ __forceinline__ unsigned char* staged(unsigned char* tile, int row, int k) { return tile + k / 8 * kRows * 128 + row * 128 + ((k % 8) ^ (row % 8)) * 16; }
-// A thread's row of 32-bit accumulators, times `by`, into a staged tile of T; `read` learns when the accumulators have been read.
-template <typename T, int DP> __device__ __forceinline__ void stage_row(uint32_t at, float by, unsigned char* tile, int row, uint64_t* read) {
+// A thread's row of 32-bit accumulators, times `by`, into a staged tile of T.
+template <typename T, int DP> __device__ __forceinline__ void stage_row(uint32_t at, float by, unsigned char* tile, int row) {
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
         uint32_t r[32];
         tensor_load(at + c, r);
         wait_loads();
-        if (c + 32 == DP) {
-            fence_before();
-            barrier_arrive(read);
-        }
 #pragma unroll
         for (int k = 0; k < 32; k += 8) {
             uint4 v;
@@ -157,20 +154,20 @@ template <int DP> struct Forward {
     static constexpr int kProb = kStep, kOut = kStep + kStep / 2, kSet = 256;                  // columns; the scores are at 0
 };
 
+// What it reads of the plan is looked at only when it is used, a job after it was asked for.
 struct ForwardJob {
-    int i0[2], last[2], head[2], j0, count;             // queries i0 to last (none if below i0), keys from j0 on in `count` steps
-    __device__ __forceinline__ ForwardJob(const AttentionParams& p, int job, int step) {
-        const bool by_heads = p.heads_q / p.heads_k % 2 == 0;
-        const int across = by_heads ? p.heads_q / 2 : p.heads_q, along = by_heads ? p.tiles : (p.tiles + 1) / 2, at = along - 1 - job / across;       // the longest first
+    int i0[2], last[2], head[2], first;                 // queries i0 to last (none if below i0)
+    __device__ __forceinline__ ForwardJob(const AttentionParams& p, int job) {
+        const int row = job / p.across, place = job - row * p.across, at = p.along - 1 - row;      // the longest first
         for (int s = 0; s < 2; ++s) {
-            head[s] = by_heads ? job % across * 2 + s : job % across;
-            i0[s] = (by_heads ? at : at * 2 + s) * p.span;
+            head[s] = p.by_heads ? place * 2 + s : place;
+            i0[s] = (p.by_heads ? at : at * 2 + s) * p.span;
             last[s] = (int)min((int64_t)i0[s] + p.span, p.tokens) - 1;
         }
-        j0 = first_key(p, i0[0]);
-        count = (max(last[0], last[1]) - j0) / step + 1;
+        first = p.first[i0[0]];
     }
-    static __host__ __device__ __forceinline__ int all(const AttentionParams& p) { return p.heads_q / p.heads_k % 2 == 0 ? p.tiles * (p.heads_q / 2) : (p.tiles + 1) / 2 * p.heads_q; }
+    __device__ __forceinline__ int begin(const AttentionParams& p) const { return p.window > 0 ? max(first, i0[0] - p.window + 1) : first; }          // of its keys
+    __device__ __forceinline__ int steps(const AttentionParams& p, int step) const { return (max(last[0], last[1]) - begin(p)) / step + 1; }
     // Every other round backwards, so that the longest of one round goes with the shortest of the next.
     static __device__ __forceinline__ int of_turn(int turn) { return turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
 };
@@ -180,7 +177,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                                                                 const __grid_constant__ CUtensorMap map_o, const AttentionParams p) {
     using F = Forward<DP>;
     __shared__ uint64_t q_full[F::kQueries], q_empty[F::kQueries], k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages];
-    __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], o_empty[2], ended[2];
+    __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], ended[2];
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
@@ -194,7 +191,6 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             barrier_init(&s_empty[s], kRows);
             barrier_init(&p_full[s], kRows);
             barrier_init(&o_done[s], 1);
-            barrier_init(&o_empty[s], kRows);
             barrier_init(&ended[s], 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -206,7 +202,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
     fence_after();
     // what the multiplying warp's loops depend on comes by shuffles from one lane: the compiler then knows it to be the same for all and keeps it in uniform registers
     const uint32_t base = __shfl_sync(~0u, tensor, 0), q_at = shared_address(shared), k_at = q_at + F::kKeys, v_at = k_at + F::kStages * F::kPart;
-    const int jobs = ForwardJob::all(p);
+    const int jobs = p.across * p.along;
     // registers: 128 x (2 x 200 + 104) of the 384 x 168 that the block has
 
     if (warp >= 8) {
@@ -216,21 +212,21 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             // queries and keys; values are another warp's, so that keys do not wait for the room that values wait for
             int queries = 0, keys = 0;                  // loads begun so far
             bool fine = true;
-            ForwardJob next(p, blockIdx.x, F::kStep);
+            ForwardJob next(p, blockIdx.x);
             for (int turn = 0, job = blockIdx.x; fine && job < jobs; job = ForwardJob::of_turn(++turn)) {
                 const ForwardJob now = next;
                 const int after = ForwardJob::of_turn(turn + 1);
-                if (after < jobs) next = ForwardJob(p, after, F::kStep);
-                const int b = queries % F::kQueries, key_head = now.head[0] / (p.heads_q / p.heads_k);
+                if (after < jobs) next = ForwardJob(p, after);
+                const int b = queries % F::kQueries, key_head = now.head[0] / (p.heads_q / p.heads_k), j0 = now.begin(p), count = now.steps(p, F::kStep);
                 if (queries >= F::kQueries && !(fine = barrier_wait(&q_empty[b], (queries / F::kQueries - 1) & 1, &lost))) break;
                 barrier_expect(&q_full[b], 2 * F::kTile);
                 for (int s = 0; s < 2; ++s) load_panels<kRows, DP>(shared + (2 * b + s) * F::kTile, &map_q, &q_full[b], now.head[s], now.i0[s]);
                 ++queries;
-                for (int j = 0; j < now.count; ++j, ++keys) {
+                for (int j = 0; j < count; ++j, ++keys) {
                     const int s = keys % F::kStages, round = keys / F::kStages;
                     if (round > 0 && !(fine = barrier_wait(&k_empty[s], (round - 1) & 1, &lost))) break;
                     barrier_expect(&k_full[s], F::kPart);
-                    load_panels<F::kStep, DP>(shared + F::kKeys + s * F::kPart, &map_k, &k_full[s], key_head, now.j0 + j * F::kStep);
+                    load_panels<F::kStep, DP>(shared + F::kKeys + s * F::kPart, &map_k, &k_full[s], key_head, j0 + j * F::kStep);
                 }
             }
             drain_ring(q_full, F::kQueries, queries);
@@ -240,17 +236,17 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         if (lane == 0) {
             int values = 0;
             bool fine = true;
-            ForwardJob next(p, blockIdx.x, F::kStep);
+            ForwardJob next(p, blockIdx.x);
             for (int turn = 0, job = blockIdx.x; fine && job < jobs; job = ForwardJob::of_turn(++turn)) {
                 const ForwardJob now = next;
                 const int after = ForwardJob::of_turn(turn + 1);
-                if (after < jobs) next = ForwardJob(p, after, F::kStep);
-                const int key_head = now.head[0] / (p.heads_q / p.heads_k);
-                for (int j = 0; j < now.count; ++j, ++values) {
+                if (after < jobs) next = ForwardJob(p, after);
+                const int key_head = now.head[0] / (p.heads_q / p.heads_k), j0 = now.begin(p), count = now.steps(p, F::kStep);
+                for (int j = 0; j < count; ++j, ++values) {
                     const int s = values % F::kStages, round = values / F::kStages;
                     if (round > 0 && !(fine = barrier_wait(&v_empty[s], (round - 1) & 1, &lost))) break;
                     barrier_expect(&v_full[s], F::kPart);
-                    load_panels<F::kStep, DP>(shared + F::kKeys + (F::kStages + s) * F::kPart, &map_v, &v_full[s], key_head, now.j0 + j * F::kStep);
+                    load_panels<F::kStep, DP>(shared + F::kKeys + (F::kStages + s) * F::kPart, &map_v, &v_full[s], key_head, j0 + j * F::kStep);
                 }
             }
             drain_ring(v_full, F::kStages, values);
@@ -258,11 +254,15 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
     } else if (warp < 10) {
         const int set = warp - 8;
         const uint32_t columns = base + set * F::kSet, q_set = q_at + set * F::kTile;
+        constexpr bool ACROSS = F::kQueries > 1;        // whether the scores run ahead over a job's end, too
         int job = blockIdx.x, turn = 0, j = 0, count = 0, ahead = 0;                               // of the scores, one step ahead of P V
+        ForwardJob next(p, job);
         int k_stage = 0, k_phase = 0, v_stage = 0, v_phase = 0, q_buffer = 0, q_phase = 0;
         auto scores = [&]() {
             if (j == 0) {
-                count = __shfl_sync(~0u, ForwardJob(p, job, F::kStep).count, 0);
+                count = __shfl_sync(~0u, next.steps(p, F::kStep), 0);
+                const int after = ForwardJob::of_turn(turn + 1);
+                if (after < jobs) next = ForwardJob(p, after);
                 if (!warp_wait(&q_full[q_buffer], q_phase, &lost)) return false;
             }
             if (!warp_wait(&k_full[k_stage], k_phase, &lost)) return false;
@@ -286,9 +286,8 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         for (int own = blockIdx.x; fine && own < jobs; own = ForwardJob::of_turn(++done)) {
             const int steps = count;                    // of the job that the scores have just begun
             for (int i = 0; i < steps; ++i, ++n) {
-                if (i + 1 < steps && !(fine = scores())) break;
+                if ((i + 1 < steps || (ACROSS && job < jobs)) && !(fine = scores())) break;
                 if (!(fine = warp_wait(&p_full[set], n & 1, &lost))) break;
-                if (i == 0 && done > 0 && !(fine = warp_wait(&o_empty[set], (done - 1) & 1, &lost))) break;
                 if (!(fine = warp_wait(&v_full[v_stage], v_phase, &lost))) break;
                 fence_after();
                 multiply_columns<T, F::kStep, DP>(columns + F::kOut, columns + F::kProb, v_at + v_stage * F::kPart, i != 0);
@@ -296,8 +295,8 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 commit(&o_done[set]);
                 if (++v_stage == F::kStages) { v_stage = 0; v_phase ^= 1; }
             }
-            // across a job's end when its last product is under way: the next one's queries may still be on theirs
-            if (fine && job < jobs) fine = scores();
+            // where queries have one buffer, only when the job's last product is under way: the next one's may still be on their way
+            if (!ACROSS && fine && job < jobs) fine = scores();
         }
         commit(&ended[set]);
         drain(&ended[set], 0);
@@ -309,117 +308,127 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         const Pair scale2 = pair_of(p.scale2, p.scale2);
         bool fine = true;
         int n = 0;
-        ForwardJob next(p, blockIdx.x, F::kStep);
-        auto low_of = [&](const ForwardJob& job) { return job.i0[set] + row <= job.last[set] ? first_key(p, job.i0[set] + row) : 0; };
-        int next_low = low_of(next);
+        // The rows of a job leave when the next one's first probabilities are worked out: P V of its last step is under way meanwhile.
+        struct Leaving { int first, last, head; float top, sum; } leaving{0, -1, 0, 0.f, 0.f};
+        unsigned char* const tile = shared + F::kStaged + set * F::kTile;
+        auto leave = [&]() {
+            // through shared memory, so that rows go in whole lines and nobody waits for them
+            const int i = leaving.first + row;
+            if (row == 0) wait_stores_read();
+            meet(1 + set, kRows);
+            stage_row<T, DP>(mine + F::kOut, fine ? 1.f / leaving.sum : nan_value(), tile, row);
+            fence_shared();
+            meet(1 + set, kRows);
+            if (row == 0 && leaving.first <= leaving.last) {
+#pragma unroll
+                for (int c = 0; c < DP; c += 64)
+                    if (c < p.dim) store_tile(&map_o, tile + c / 64 * kRows * 128, c, leaving.head, leaving.first);
+                stores_end();
+            }
+            if (i <= leaving.last && p.lse != nullptr) p.lse[leaving.head * p.pitch + i] = fine ? fmaf(leaving.top, p.scale2, log2f(leaving.sum)) : nan_value();
+        };
+        ForwardJob next(p, blockIdx.x);
+        auto first_of = [&](const ForwardJob& job) { return p.first[min(job.i0[set] + row, job.last[set] >= job.i0[set] ? job.last[set] : 0)]; };
+        int next_first = first_of(next);
         for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
-            const int first = next.i0[set], last = next.last[set], i = first + row, low = next_low, count = next.count, j0 = next.j0, head = next.head[set];
+            const int first = next.i0[set], last = next.last[set], i = first + row, head = next.head[set], j0 = next.begin(p), count = next.steps(p, F::kStep);
             const bool live = i <= last;
-            const int high = live ? i : -1;
+            const int high = live ? i : -1, low = !live ? 0 : p.window > 0 ? max(next_first, i - p.window + 1) : next_first;
             const int after = ForwardJob::of_turn(turn + 1);
-            if (after < jobs) { next = ForwardJob(p, after, F::kStep); next_low = low_of(next); }
+            if (after < jobs) { next = ForwardJob(p, after); next_first = first_of(next); }
             // keys that any and that all of the warp's rows see; a row that is not there sees none
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
-            for (int j = 0; fine && j < count; ++j, ++n) {
+            for (int j = 0; j < count; ++j, ++n) {
                 const int k0 = j0 + j * F::kStep;
-                if (!(fine = warp_wait(&s_full[set], n & 1, &lost))) break;
+                fine = fine && warp_wait(&s_full[set], n & 1, &lost);
+                if (!fine) break;
                 fence_after();
-                uint32_t r[F::kStep];
+                uint32_t r[F::kStep], packed[F::kStep / 2];
 #pragma unroll
                 for (int c = 0; c < F::kStep; c += 16) tensor_load16(mine + c, r + c);
                 wait_loads();
                 fence_before();
                 barrier_arrive(&s_empty[set]);
                 Pair part[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
-                // all: every row of the warp sees every key; else 16 keys at a time may be hidden from all, or from some
+                float by = 1.f;
+                bool any = false;
+                // all: every row of the warp sees every key; else CHUNK keys at a time may be hidden from all, or from some
                 auto rows = [&](auto all) {
                     constexpr bool ALL = decltype(all)::value != 0;
-                    auto hidden = [&](int c) { return !ALL && (k0 + c > any_high || k0 + c + 15 < any_low); };
+                    constexpr int CHUNK = DP == 64 ? 32 : 16;
+                    auto hidden = [&](int c) { return !ALL && (k0 + c > any_high || k0 + c + CHUNK - 1 < any_low); };
                     float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int c = 0; c < F::kStep; c += 16) {
+                    for (int c = 0; c < F::kStep; c += CHUNK) {
                         if (hidden(c)) continue;
-                        if (!ALL && (k0 + c < all_low || k0 + c + 15 > all_high)) {
+                        if (!ALL && (k0 + c < all_low || k0 + c + CHUNK - 1 > all_high)) {
                             const uint32_t seen = columns_between(low - k0 - c, high - k0 - c);
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) r[c + k] = seen >> k & 1u ? r[c + k] : 0xff800000u;
+                            for (int k = 0; k < CHUNK; ++k) r[c + k] = seen >> k & 1u ? r[c + k] : 0xff800000u;
                         }
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) best[k % 4] = max3(best[k % 4], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
+                        for (int k = 0; k < CHUNK / 2; ++k) best[k % 4] = max3(best[k % 4], __uint_as_float(r[c + 2 * k]), __uint_as_float(r[c + 2 * k + 1]));
                     }
                     const float now_top = fmaxf(max3(best[0], best[1], best[2]), best[3]);
                     // the maximum in use follows only where the new one is more than 2^8 above: P stays below 2^8, and O is seldom rescaled
                     const bool up = now_top != top && ((now_top - top) * p.scale2 > 8.f || top == -INFINITY);
-                    const bool any = __any_sync(~0u, up);
-                    const float by = up ? exp2_fast((top - now_top) * p.scale2) : 1.f;
+                    any = __any_sync(~0u, up);
+                    by = up ? exp2_fast((top - now_top) * p.scale2) : 1.f;
                     if (up) top = now_top;
                     sum *= by;
                     const float shift = top == -INFINITY ? 0.f : -top * p.scale2;
                     const Pair shifts = pair_of(shift, shift);
 #pragma unroll
-                    for (int c = 0; c < F::kStep; c += 16) {
-                        uint32_t packed[8];
+                    for (int c = 0; c < F::kStep; c += CHUNK) {
                         if (hidden(c)) {
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) packed[k] = 0u;
+                            for (int k = 0; k < CHUNK / 2; ++k) packed[c / 2 + k] = 0u;
                         } else {
 #pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
+                            for (int k = 0; k < CHUNK; k += 2) {
                                 float a, b;
                                 split(fma_pair(pair_of(__uint_as_float(r[c + k]), __uint_as_float(r[c + k + 1])), scale2, shifts), a, b);
                                 a = exp2_fast(a);
                                 b = exp2_fast(b);
                                 part[k / 2 % 2] = add_pair(part[k / 2 % 2], pair_of(a, b));
-                                packed[k / 2] = pack<T>(a, b);
+                                packed[(c + k) / 2] = pack<T>(a, b);
                             }
                         }
-                        if (c == 0) {
-                            // P V of the step before: P and O are free to be written
-                            if (n > 0 && !warp_wait(&o_done[set], (n - 1) & 1, &lost)) return false;
-                            if (any && j > 0) {
-                                fence_after();
-#pragma unroll
-                                for (int d = 0; d < DP; d += 32) {
-                                    uint32_t o[32];
-                                    tensor_load(mine + F::kOut + d, o);
-                                    wait_loads();
-#pragma unroll
-                                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-                                    tensor_store(mine + F::kOut + d, o);
-                                }
-                            }
-                        }
-                        tensor_store8(mine + F::kProb + c / 2, packed);
                     }
-                    wait_stores();
-                    fence_before();
-                    barrier_arrive(&p_full[set]);
-                    return true;
                 };
-                if (!(fine = k0 >= all_low && k0 + F::kStep - 1 <= all_high ? rows(Number<1>{}) : rows(Number<0>{}))) break;
+                if (k0 >= all_low && k0 + F::kStep - 1 <= all_high) rows(Number<1>{}); else rows(Number<0>{});
                 float x, y;
                 split(add_pair(part[0], part[1]), x, y);
                 sum += x + y;
-            }
-            if (fine) fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
-            fence_after();
-            // through shared memory, so that rows leave in whole lines and the next job need not wait for them
-            unsigned char* const tile = shared + F::kStaged + set * F::kTile;
-            if (row == 0) wait_stores_read();
-            meet(1 + set, kRows);
-            stage_row<T, DP>(mine + F::kOut, fine ? 1.f / sum : nan_value(), tile, row, &o_empty[set]);
-            fence_shared();
-            meet(1 + set, kRows);
-            if (row == 0 && first <= last) {
+                // P V of the step before has ended: P and O may be written, and the rows of a job that it ended may leave
+                if (n > 0) fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
+                if (!fine) break;
+                if (n > 0) fence_after();
+                if (j == 0 && n > 0) leave();
+                if (any && j > 0)
 #pragma unroll
-                for (int c = 0; c < DP; c += 64)
-                    if (c < p.dim) store_tile(&map_o, tile + c / 64 * kRows * 128, c, head, first);
-                stores_end();
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tensor_load(mine + F::kOut + c, o);
+                        wait_loads();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                        tensor_store(mine + F::kOut + c, o);
+                    }
+#pragma unroll
+                for (int c = 0; c < F::kStep / 2; c += 8) tensor_store8(mine + F::kProb + c, packed + c);
+                wait_stores();
+                fence_before();
+                barrier_arrive(&p_full[set]);
             }
-            if (live && p.lse != nullptr) p.lse[head * p.pitch + i] = fine ? fmaf(top, p.scale2, log2f(sum)) : nan_value();
+            if (!fine && turn > 0) leave();             // a block that gave up: NaN for this job's, and below for what is left
+            leaving = {first, last, head, top, sum};
         }
+        fine = fine && warp_wait(&o_done[set], (n - 1) & 1, &lost);
+        fence_after();
+        leave();
         if (row == 0) wait_stores_done();
     }
     __syncwarp();
@@ -755,6 +764,8 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
     p.first = e.first; p.end = e.end; p.tokens = e.tokens; p.pitch = attention_pitch(e.tokens);
     p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens);
     p.span = tile_span(e); p.tiles = (int)((e.tokens + p.span - 1) / p.span);
+    p.by_heads = p.heads_q / p.heads_k % 2 == 0;
+    p.across = p.by_heads ? p.heads_q / 2 : p.heads_q; p.along = p.by_heads ? p.tiles : (p.tiles + 1) / 2;
     p.scale = d.scale; p.scale2 = d.scale * kLog2e;
     p.out = d.out; p.lse = d.lse; p.dout = d.dout; p.delta = d.delta; p.dq = d.dq; p.dk = d.dk; p.dv = d.dv;
     if (encoder() == nullptr) return cudaErrorNotSupported;
@@ -766,7 +777,7 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
         if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, kRows) || !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, Forward<DP>::kStep) ||
             !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, Forward<DP>::kStep) || !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, p.span))
             return cudaErrorInvalidValue;
-        attention_kernel<T, DP><<<(unsigned)std::min(ForwardJob::all(p), 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
+        attention_kernel<T, DP><<<(unsigned)std::min(p.across * p.along, 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();
     }
     for (int keys = 0; keys < 2; ++keys) {

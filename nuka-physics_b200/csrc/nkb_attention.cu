@@ -39,20 +39,19 @@ struct AttentionParams {
 };
 
 __device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
-__device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
-__device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
 
-// A tile of queries and a head; the longest first.
+// A tile of queries and a head; the longest of one long row first.  What it reads of the plan is looked at only when it is used, a job after it was asked for.
 struct QueryJob {
-    int i0, last, j0, count, head;                      // queries i0 to last, keys from j0 on in `count` steps
+    int i0, last, head, first;                          // queries i0 to last; first: the plan's, of the first
     __device__ __forceinline__ QueryJob(const AttentionParams& p, int job) {
-        head = job % p.heads_q;
-        i0 = (p.tiles - 1 - job / p.heads_q) * p.span;
+        const int tile = job / p.heads_q;
+        head = job - tile * p.heads_q;
+        i0 = (p.tiles - 1 - tile) * p.span;
         last = (int)min((int64_t)i0 + p.span, p.tokens) - 1;
-        j0 = first_key(p, i0);
-        count = (last - j0) / kStream + 1;
+        first = p.first[i0];
     }
-    __device__ __forceinline__ int low(const AttentionParams& p) const { return i0 + (int)threadIdx.x <= last ? first_key(p, i0 + (int)threadIdx.x) : 0; }
+    __device__ __forceinline__ int begin(const AttentionParams& p) const { return p.window > 0 ? max(first, i0 - p.window + 1) : first; }             // of its keys
+    __device__ __forceinline__ int steps(const AttentionParams& p) const { return (last - begin(p)) / kStream + 1; }
 };
 
 // One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T.
@@ -340,6 +339,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
+            bool left = false;
             for (int j = 0; j < count; ++j, ++n) {
                 const int k0 = j0 + j * F::kStep;
                 fine = fine && warp_wait(&s_full[set], n & 1, &lost);
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 if (n > 0) fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
                 if (!fine) break;
                 if (n > 0) fence_after();
-                if (j == 0 && n > 0) leave();
+                if (j == 0 && n > 0) { leave(); left = true; }
                 if (any && j > 0)
 #pragma unroll
                     for (int c = 0; c < DP; c += 32) {
@@ -423,7 +423,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 fence_before();
                 barrier_arrive(&p_full[set]);
             }
-            if (!fine && turn > 0) leave();             // a block that gave up: NaN for this job's, and below for what is left
+            if (turn > 0 && !left) leave();             // a block that gave up: NaN for this job's, and below for what is left
             leaving = {first, last, head, top, sum};
         }
         fine = fine && warp_wait(&o_done[set], (n - 1) & 1, &lost);
@@ -439,30 +439,33 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
 }
 
 // ---- backwards: gradients of the queries -------------------------------------------------------------------------------
+// Two blocks to an SM, each of which takes (tile of queries, head) jobs in turn; loads and products run ahead as forwards, and rows leave under the next job's first exponentials.
 template <int DP> struct Queries {
-    static constexpr int kStages = DP == 64 ? 3 : 1;
-    static constexpr bool kApart = DP == 64;
+    static constexpr bool kApart = DP == 64;            // dS has columns of its own: the next scores are multiplied while the present ones are worked on
+    static constexpr int kStages = DP == 64 ? 2 : 1;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
-    static constexpr int kShared = 2 * kTile + 2 * kStages * kPart + 1024;
+    // queries, dO and, for D = dO . O, O; steps of keys and values; the rows that leave.  Wide heads have room for queries and dO only.
+    static constexpr int kTiles = kApart ? 3 : 2, kKeys = kTiles * kTile, kStaged = kKeys + 2 * kStages * kPart, kShared = kStaged + (kApart ? kTile : 0) + 1024;
     static constexpr int kGrad = kStream, kOut = 2 * kStream, kProb = kApart ? 2 * kStream + DP : 0;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
-                                                               const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
+__global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
+                                                               const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq,
+                                                               const AttentionParams p) {
     using F = Queries<DP>;
-    __shared__ uint64_t q_full, full[F::kStages], empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full, s_empty, p_full, o_done, ended;
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-    const QueryJob job(p, blockIdx.x);
-    const int head = job.head, key_head = head / (p.heads_q / p.heads_k), i0 = job.i0, last = job.last, j0 = job.j0, count = job.count;
     if (threadIdx.x == 0) {
         lost = 0;
         barrier_init(&q_full, 1);
+        barrier_init(&q_empty, F::kApart ? 1 + kRows : 1);      // the scores' products, and the rows' reads of dO and O
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
         barrier_init(&s_full, 1);
+        barrier_init(&s_empty, kRows);
         barrier_init(&p_full, kRows);
         barrier_init(&o_done, 1);
         barrier_init(&ended, 1);
@@ -473,106 +476,193 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
     fence_before();
     __syncthreads();
     fence_after();
-    // what the multiplying warp's loops depend on comes by shuffles from one lane: the compiler then knows it to be the same for all and keeps it in uniform registers
-    const uint32_t base = __shfl_sync(~0u, tensor, 0), q_at = shared_address(shared), do_at = q_at + F::kTile, kv_at = do_at + F::kTile;
+    const uint32_t base = __shfl_sync(~0u, tensor, 0), q_at = shared_address(shared), do_at = q_at + F::kTile, kv_at = q_at + F::kKeys;
+    const int jobs = p.tiles * p.heads_q, stride = gridDim.x, group = p.heads_q / p.heads_k;
 
     if (warp == 4) {
         if (lane == 0) {
-            barrier_expect(&q_full, 2 * F::kTile);
-            load_panels<kRows, DP>(shared, &map_q, &q_full, head, i0);
-            load_panels<kRows, DP>(shared + F::kTile, &map_do, &q_full, head, i0);
-            int j = 0;
-            for (; j < count; ++j) {
-                const int s = j % F::kStages, turn = j / F::kStages;
-                if (turn > 0 && !barrier_wait(&empty[s], (turn - 1) & 1, &lost)) break;
-                barrier_expect(&full[s], 2 * F::kPart);
-                unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
-                load_panels<kStream, DP>(to, &map_k, &full[s], key_head, j0 + j * kStream);
-                load_panels<kStream, DP>(to + F::kPart, &map_v, &full[s], key_head, j0 + j * kStream);
+            int steps = 0, queries = 0;                 // loads begun so far
+            bool fine = true;
+            QueryJob next(p, blockIdx.x);
+            for (int job = blockIdx.x; fine && job < jobs; job += stride) {
+                const QueryJob now = next;
+                if (job + stride < jobs) next = QueryJob(p, job + stride);
+                if (queries > 0 && !(fine = barrier_wait(&q_empty, (queries - 1) & 1, &lost))) break;
+                barrier_expect(&q_full, F::kTiles * F::kTile);
+                load_panels<kRows, DP>(shared, &map_q, &q_full, now.head, now.i0);
+                load_panels<kRows, DP>(shared + F::kTile, &map_do, &q_full, now.head, now.i0);
+                if (F::kApart) load_panels<kRows, DP>(shared + 2 * F::kTile, &map_o, &q_full, now.head, now.i0);
+                ++queries;
+                const int j0 = now.begin(p), count = now.steps(p), key_head = now.head / group;
+                for (int j = 0; j < count; ++j, ++steps) {
+                    const int s = steps % F::kStages, turn = steps / F::kStages;
+                    if (turn > 0 && !(fine = barrier_wait(&empty[s], (turn - 1) & 1, &lost))) break;
+                    barrier_expect(&full[s], 2 * F::kPart);
+                    unsigned char* to = shared + F::kKeys + 2 * s * F::kPart;
+                    load_panels<kStream, DP>(to, &map_k, &full[s], key_head, j0 + j * kStream);
+                    load_panels<kStream, DP>(to + F::kPart, &map_v, &full[s], key_head, j0 + j * kStream);
+                }
             }
-            drain(&q_full, 0);
-            for (int b = max(0, j - F::kStages); b < j; ++b) drain(&full[b % F::kStages], b / F::kStages & 1);
+            drain_ring(&q_full, 1, queries);
+            drain_ring(full, F::kStages, steps);
         }
     } else if (warp == 5) {
-        {
-            bool fine = warp_wait(&q_full, 0, &lost);
-            auto scores = [&](int j) {
-                const int s = j % F::kStages;
-                if (!warp_wait(&full[s], j / F::kStages & 1, &lost)) return false;
-                fence_after();
-                multiply_rows<T, kStream, DP>(base, q_at, kv_at + 2 * s * F::kPart);
-                multiply_rows<T, kStream, DP>(base + F::kGrad, do_at, kv_at + (2 * s + 1) * F::kPart);
-                commit(&s_full);
-                return true;
-            };
-            fine = fine && scores(0);
-            for (int j = 0; fine && j < count; ++j) {
-                const int s = j % F::kStages;
-                if (!warp_wait(&p_full, j & 1, &lost)) break;
-                fence_after();
-                if (F::kApart && j + 1 < count && !(fine = scores(j + 1))) break;
-                multiply_columns<T, kStream, DP>(base + F::kOut, base + F::kProb, kv_at + 2 * s * F::kPart, j != 0);
-                commit(&empty[s]);
-                commit(&o_done);
-                if (!F::kApart && j + 1 < count) fine = warp_wait(&o_done, j & 1, &lost) && scores(j + 1);
+        int job = blockIdx.x, j = 0, count = 0, ahead = 0, queries = 0, stage = 0, phase = 0;      // of the scores
+        QueryJob next(p, job);
+        auto scores = [&]() {
+            if (j == 0) {
+                count = __shfl_sync(~0u, next.steps(p), 0);
+                if (job + stride < jobs) next = QueryJob(p, job + stride);
+                if (!warp_wait(&q_full, queries & 1, &lost)) return false;
             }
-            commit(&ended);
-            drain(&ended, 0);
-        }
-    } else {
-        const int i = i0 + threadIdx.x;
-        const bool live = i <= last;
-        const int low = live ? first_key(p, i) : 0, high = live ? i : -1;
-        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
-        // D = dO . O of the thread's row, which the keys' kernel reads after this one
-        float delta = 0.f, lse = 0.f;
-        if (live) {
-            const int64_t at = ((int64_t)i * p.heads_q + head) * p.dim;
-            const uint4 *o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + at), *g = reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout) + at);
-#pragma unroll 4
-            for (int c = 0; c < p.dim / 8; ++c) {
-                const uint4 a = o[c], b = g[c];
-                float u[8], v[8];
-                unpack<T, 8>(a, u);
-                unpack<T, 8>(b, v);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
-            }
-            lse = p.lse[head * p.pitch + i];
-            p.delta[head * p.pitch + i] = delta;
-        }
-        bool fine = true;
-        for (int j = 0; j < count; ++j) {
-            const int k0 = j0 + j * kStream;
-            if (!(fine = warp_wait(&s_full, j & 1, &lost))) break;
+            if (!warp_wait(&full[stage], phase, &lost)) return false;
+            if (ahead > 0 && !warp_wait(F::kApart ? &s_empty : &o_done, (ahead - 1) & 1, &lost)) return false;
             fence_after();
-            uint32_t r[kStream], d[kStream], packed[kStream / 2];
-#pragma unroll
-            for (int c = 0; c < kStream; c += 32) { tensor_load(mine + c, r + c); tensor_load(mine + F::kGrad + c, d + c); }
-            wait_loads();
-#pragma unroll
-            for (int c = 0; c < kStream; ++c) {
-                const float prob = exp2_fast(fmaf(__uint_as_float(r[c]), p.scale2, -lse));
-                r[c] = __float_as_uint(prob * (__uint_as_float(d[c]) - delta));
+            multiply_rows<T, kStream, DP>(base, q_at, kv_at + 2 * stage * F::kPart);
+            multiply_rows<T, kStream, DP>(base + F::kGrad, do_at, kv_at + (2 * stage + 1) * F::kPart);
+            commit(&s_full);
+            ++ahead;
+            if (++stage == F::kStages) { stage = 0; phase ^= 1; }
+            if (++j == count) { commit(&q_empty); j = 0; ++queries; job += stride; }
+            return true;
+        };
+        int n = 0, own_stage = 0;
+        bool fine = scores();
+        for (int own = blockIdx.x; fine && own < jobs; own += stride) {
+            const int steps = count;                    // of the job that the scores have just begun
+            for (int i = 0; i < steps; ++i, ++n) {
+                if (F::kApart && F::kStages > 1 && i + 1 < steps && !(fine = scores())) break;
+                if (!(fine = warp_wait(&p_full, n & 1, &lost))) break;
+                fence_after();
+                multiply_columns<T, kStream, DP>(base + F::kOut, base + F::kProb, kv_at + 2 * own_stage * F::kPart, i != 0);
+                commit(&empty[own_stage]);
+                commit(&o_done);
+                if (++own_stage == F::kStages) own_stage = 0;
+                // over a job's end only now: the next one's queries may still be on their way
+                if ((!F::kApart || i + 1 == steps) && job < jobs && !(fine = scores())) break;
             }
-            if (!__all_sync(~0u, k0 >= low && k0 + kStream - 1 <= high)) {
-                const int from = low - k0, to = high - k0;
-#pragma unroll
-                for (int c = 0; c < kStream; ++c)
-                    if (c < from || c > to) r[c] = 0u;
-            }
-#pragma unroll
-            for (int c = 0; c < kStream; c += 2) packed[c / 2] = pack<T>(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-            if (F::kApart && j > 0 && !(fine = warp_wait(&o_done, (j - 1) & 1, &lost))) break;
-            tensor_store(mine + F::kProb, packed);
-            wait_stores();
-            fence_before();
-            barrier_arrive(&p_full);
         }
-        fine = fine && warp_wait(&o_done, (count - 1) & 1, &lost);
+        commit(&ended);
+        drain(&ended, 0);
+    } else {
+        const int row = threadIdx.x;
+        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
+        bool fine = true;
+        int n = 0, queries = 0;
+        struct Leaving { int first, last, head; } leaving{0, -1, 0};
+        auto leave = [&]() {
+            if (F::kApart) {
+                unsigned char* const tile = shared + F::kStaged;
+                if (row == 0) wait_stores_read();
+                meet(1, kRows);
+                stage_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), tile, row);
+                fence_shared();
+                meet(1, kRows);
+                if (row == 0 && leaving.first <= leaving.last) {
+                    store_tile(&map_dq, tile, 0, leaving.head, leaving.first);
+                    stores_end();
+                }
+            } else {
+                const int i = leaving.first + row;
+                store_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), p.dim, i <= leaving.last ? static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + leaving.head) * p.dim : nullptr);
+            }
+        };
+        QueryJob next(p, blockIdx.x);
+        auto first_of = [&](const QueryJob& job) { return p.first[min(job.i0 + row, job.last)]; };
+        auto lse_of = [&](const QueryJob& job) { return p.lse[job.head * p.pitch + min(job.i0 + row, job.last)]; };
+        int next_first = first_of(next);
+        float next_lse = lse_of(next);
+        for (int job = blockIdx.x; job < jobs; job += stride, ++queries) {
+            const QueryJob now = next;
+            const int i = now.i0 + row, j0 = now.begin(p), count = now.steps(p);
+            const bool live = i <= now.last;
+            const int high = live ? i : -1, low = !live ? 0 : p.window > 0 ? max(next_first, i - p.window + 1) : next_first;
+            const float lse = next_lse;
+            if (job + stride < jobs) { next = QueryJob(p, job + stride); next_first = first_of(next); next_lse = lse_of(next); }
+            const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
+            const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
+            // D = dO . O of the thread's row, which the keys' kernel reads after this one
+            float delta = 0.f;
+            if (F::kApart) {
+                fine = fine && warp_wait(&q_full, queries & 1, &lost);
+                if (fine)
+#pragma unroll
+                    for (int c = 0; c < DP / 8; ++c) {
+                        float u[8], v[8];
+                        unpack<T, 8>(*reinterpret_cast<const uint4*>(staged(shared + F::kTile, row, c)), u);
+                        unpack<T, 8>(*reinterpret_cast<const uint4*>(staged(shared + 2 * F::kTile, row, c)), v);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
+                    }
+                barrier_arrive(&q_empty);
+            } else if (live) {
+                const int64_t at = ((int64_t)i * p.heads_q + now.head) * p.dim;
+                const uint4 *o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + at), *g = reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout) + at);
+#pragma unroll 4
+                for (int c = 0; c < p.dim / 8; ++c) {
+                    float u[8], v[8];
+                    unpack<T, 8>(o[c], u);
+                    unpack<T, 8>(g[c], v);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
+                }
+            }
+            if (live) p.delta[now.head * p.pitch + i] = delta;
+            const Pair scale2 = pair_of(p.scale2, p.scale2), shift = pair_of(-lse, -lse), minus = pair_of(-delta, -delta);
+            bool left = false;
+            for (int j = 0; j < count; ++j, ++n) {
+                const int k0 = j0 + j * kStream;
+                fine = fine && warp_wait(&s_full, n & 1, &lost);
+                if (!fine) break;
+                fence_after();
+                uint32_t packed[kStream / 2];
+                const bool all = k0 >= all_low && k0 + kStream - 1 <= all_high;
+#pragma unroll
+                for (int c0 = 0; c0 < kStream; c0 += 32) {
+                    uint32_t r[32], d[32];
+                    tensor_load(mine + c0, r);
+                    tensor_load(mine + F::kGrad + c0, d);
+                    wait_loads();
+                    if (c0 + 32 == kStream) {
+                        fence_before();
+                        barrier_arrive(&s_empty);
+                    }
+                    if (k0 + c0 > any_high || k0 + c0 + 31 < any_low) {             // hidden from all of the warp's rows
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) packed[c0 / 2 + c] = 0u;
+                        continue;
+                    }
+                    const uint32_t seen = all ? ~0u : columns_between(low - k0 - c0, high - k0 - c0);
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        float a, b, x, y;
+                        split(fma_pair(pair_of(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), scale2, shift), a, b);
+                        a = exp2_fast(a);
+                        b = exp2_fast(b);
+                        split(mul_pair(pair_of(a, b), add_pair(pair_of(__uint_as_float(d[c]), __uint_as_float(d[c + 1])), minus)), x, y);
+                        if (!all) {
+                            x = seen >> c & 1u ? x : 0.f;
+                            y = seen >> (c + 1) & 1u ? y : 0.f;
+                        }
+                        packed[(c0 + c) / 2] = pack<T>(x, y);
+                    }
+                }
+                if (n > 0) fine = warp_wait(&o_done, (n - 1) & 1, &lost);
+                if (!fine) break;
+                if (n > 0) fence_after();
+                if (j == 0 && n > 0) { leave(); left = true; }
+                tensor_store(mine + F::kProb, packed);
+                wait_stores();
+                fence_before();
+                barrier_arrive(&p_full);
+            }
+            if (queries > 0 && !left) leave();          // a block that gave up: NaN for this job's, and below for what is left
+            leaving = {now.i0, now.last, now.head};
+        }
+        fine = fine && warp_wait(&o_done, (n - 1) & 1, &lost);
         fence_after();
-        T* out = live ? static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + head) * p.dim : nullptr;
-        store_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), p.dim, out);
+        leave();
+        if (row == 0) wait_stores_done();
     }
     __syncwarp();
     fence_before();
@@ -582,32 +672,49 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
 }
 
 // ---- backwards: gradients of keys and values ----------------------------------------------------------------------------
+// The same with (tile of keys, key head) jobs: the queries of all heads of the group that see any of the keys pass by, 64 at a time, with their statistics.
 template <int DP> struct Keys {
-    static constexpr int kStages = DP == 64 ? 3 : 2;
+    static constexpr int kStages = 2;
     static constexpr bool kApart = DP == 128;           // one block to an SM has columns to spare, two have not
     static constexpr int kColumns = DP == 64 ? 256 : 512;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
-    static constexpr int kShared = 2 * kTile + 2 * kStages * kPart + 1024;
+    static constexpr int kStaged = 2 * kTile + 2 * kStages * kPart, kShared = kStaged + (DP == 64 ? 2 * kTile : 0) + 1024;         // rows of wide heads leave without a staged tile
     static constexpr int kGrad = kStream, kValue = 2 * kStream, kKey = 2 * kStream + DP;
     static constexpr int kProb = kApart ? 2 * kStream + 2 * DP : 0, kProbGrad = kApart ? kProb + kStream / 2 : kGrad;
 };
 
+// A tile of keys and a key head; the longest of one long row are the first ones.
+struct KeyJob {
+    int j0, last, head, end;                            // keys j0 to last; end: the plan's, of the last
+    __device__ __forceinline__ KeyJob(const AttentionParams& p, int job) {
+        const int tile = job / p.heads_k;
+        head = job - tile * p.heads_k;
+        j0 = tile * p.span;
+        last = (int)min((int64_t)j0 + p.span, p.tokens) - 1;
+        end = p.end[last];
+    }
+    __device__ __forceinline__ int begin() const { return j0 & ~3; }               // of its queries: a multiple of 16 bytes of their statistics
+    __device__ __forceinline__ int steps(const AttentionParams& p) const {         // for one head
+        const int past = p.window > 0 ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
+        return (past - 1 - begin()) / kStream + 1;
+    }
+};
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
-                                                                            const __grid_constant__ CUtensorMap map_v, const AttentionParams p) {
+                                                                            const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
+                                                                            const __grid_constant__ CUtensorMap map_dv, const AttentionParams p) {
     using F = Keys<DP>;
-    __shared__ uint64_t k_full, full[F::kStages], empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ uint64_t k_full, k_empty, full[F::kStages], empty[F::kStages], s_full, p_full, o_done, ended;
     __shared__ __align__(16) float lse[F::kStages][kStream], delta[F::kStages][kStream];
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
-    const int tile = blockIdx.x / p.heads_k, key_head = blockIdx.x % p.heads_k, group = p.heads_q / p.heads_k;        // the longest are the first ones
-    const int j0 = tile * p.span, last = (int)min((int64_t)j0 + p.span, p.tokens) - 1;
-    const int i0 = j0 & ~3, each = (past_query(p, last) - 1 - i0) / kStream + 1, count = each * group;          // from a multiple of 16 bytes of the statistics on
     if (threadIdx.x == 0) {
         lost = 0;
         barrier_init(&k_full, 1);
+        barrier_init(&k_empty, 1);
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
         barrier_init(&s_full, 1);
         barrier_init(&p_full, kRows);
@@ -621,102 +728,181 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
     __syncthreads();
     fence_after();
     const uint32_t base = __shfl_sync(~0u, tensor, 0), k_at = shared_address(shared), v_at = k_at + F::kTile, part_at = v_at + F::kTile;
+    const int jobs = p.tiles * p.heads_k, stride = gridDim.x, group = p.heads_q / p.heads_k;
 
     if (warp == 4) {
         if (lane == 0) {
-            barrier_expect(&k_full, 2 * F::kTile);
-            load_panels<kRows, DP>(shared, &map_k, &k_full, key_head, j0);
-            load_panels<kRows, DP>(shared + F::kTile, &map_v, &k_full, key_head, j0);
-            int n = 0;
-            for (; n < count; ++n) {
-                const int s = n % F::kStages, turn = n / F::kStages, head = key_head * group + n / each, i = i0 + n % each * kStream;
-                if (turn > 0 && !barrier_wait(&empty[s], (turn - 1) & 1, &lost)) break;
-                barrier_expect(&full[s], 2 * F::kPart + 2 * kStream * 4);
-                unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
-                load_panels<kStream, DP>(to, &map_q, &full[s], head, i);
-                load_panels<kStream, DP>(to + F::kPart, &map_do, &full[s], head, i);
-                load_bytes(lse[s], p.lse + head * p.pitch + i, kStream * 4, &full[s]);
-                load_bytes(delta[s], p.delta + head * p.pitch + i, kStream * 4, &full[s]);
+            int steps = 0, keys = 0;                    // loads begun so far
+            bool fine = true;
+            KeyJob next(p, blockIdx.x);
+            for (int job = blockIdx.x; fine && job < jobs; job += stride) {
+                const KeyJob now = next;
+                if (job + stride < jobs) next = KeyJob(p, job + stride);
+                if (keys > 0 && !(fine = barrier_wait(&k_empty, (keys - 1) & 1, &lost))) break;
+                barrier_expect(&k_full, 2 * F::kTile);
+                load_panels<kRows, DP>(shared, &map_k, &k_full, now.head, now.j0);
+                load_panels<kRows, DP>(shared + F::kTile, &map_v, &k_full, now.head, now.j0);
+                ++keys;
+                const int each = now.steps(p);
+                for (int h = 0; fine && h < group; ++h)
+                    for (int m = 0; m < each; ++m, ++steps) {
+                        const int s = steps % F::kStages, turn = steps / F::kStages, head = now.head * group + h, i = now.begin() + m * kStream;
+                        if (turn > 0 && !(fine = barrier_wait(&empty[s], (turn - 1) & 1, &lost))) break;
+                        barrier_expect(&full[s], 2 * F::kPart + 2 * kStream * 4);
+                        unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
+                        load_panels<kStream, DP>(to, &map_q, &full[s], head, i);
+                        load_panels<kStream, DP>(to + F::kPart, &map_do, &full[s], head, i);
+                        load_bytes(lse[s], p.lse + head * p.pitch + i, kStream * 4, &full[s]);
+                        load_bytes(delta[s], p.delta + head * p.pitch + i, kStream * 4, &full[s]);
+                    }
             }
-            drain(&k_full, 0);
-            for (int b = max(0, n - F::kStages); b < n; ++b) drain(&full[b % F::kStages], b / F::kStages & 1);
+            drain_ring(&k_full, 1, keys);
+            drain_ring(full, F::kStages, steps);
         }
     } else if (warp == 5) {
-        {
-            bool fine = warp_wait(&k_full, 0, &lost);
-            auto scores = [&](int n) {
-                const int s = n % F::kStages;
-                if (!warp_wait(&full[s], n / F::kStages & 1, &lost)) return false;
-                fence_after();
-                multiply_rows<T, kStream, DP>(base, k_at, part_at + 2 * s * F::kPart);
-                multiply_rows<T, kStream, DP>(base + F::kGrad, v_at, part_at + (2 * s + 1) * F::kPart);
-                commit(&s_full);
-                return true;
-            };
-            fine = fine && scores(0);
-            for (int n = 0; fine && n < count; ++n) {
-                const int s = n % F::kStages;
-                if (!warp_wait(&p_full, n & 1, &lost)) break;
-                fence_after();
-                if (F::kApart && n + 1 < count && !(fine = scores(n + 1))) break;
-                multiply_columns<T, kStream, DP>(base + F::kValue, base + F::kProb, part_at + (2 * s + 1) * F::kPart, n != 0);
-                multiply_columns<T, kStream, DP>(base + F::kKey, base + F::kProbGrad, part_at + 2 * s * F::kPart, n != 0);
-                commit(&empty[s]);
-                commit(&o_done);
-                if (!F::kApart && n + 1 < count) fine = warp_wait(&o_done, n & 1, &lost) && scores(n + 1);
+        int job = blockIdx.x, j = 0, count = 0, ahead = 0, keys = 0, stage = 0, phase = 0;         // of the scores
+        KeyJob next(p, job);
+        auto scores = [&]() {
+            if (j == 0) {
+                count = __shfl_sync(~0u, next.steps(p) * group, 0);
+                if (job + stride < jobs) next = KeyJob(p, job + stride);
+                if (!warp_wait(&k_full, keys & 1, &lost)) return false;
             }
-            commit(&ended);
-            drain(&ended, 0);
+            if (!warp_wait(&full[stage], phase, &lost)) return false;
+            // apart, the scores' columns are free when P and dS are written; else when their products have ended
+            if (!F::kApart && ahead > 0 && !warp_wait(&o_done, (ahead - 1) & 1, &lost)) return false;
+            fence_after();
+            multiply_rows<T, kStream, DP>(base, k_at, part_at + 2 * stage * F::kPart);
+            multiply_rows<T, kStream, DP>(base + F::kGrad, v_at, part_at + (2 * stage + 1) * F::kPart);
+            commit(&s_full);
+            ++ahead;
+            if (++stage == F::kStages) { stage = 0; phase ^= 1; }
+            if (++j == count) { commit(&k_empty); j = 0; ++keys; job += stride; }
+            return true;
+        };
+        int n = 0, own_stage = 0;
+        bool fine = scores();
+        for (int own = blockIdx.x; fine && own < jobs; own += stride) {
+            const int steps = count;                    // of the job that the scores have just begun
+            for (int i = 0; i < steps; ++i, ++n) {
+                if (!(fine = warp_wait(&p_full, n & 1, &lost))) break;
+                fence_after();
+                if (F::kApart && i + 1 < steps && !(fine = scores())) break;
+                multiply_columns<T, kStream, DP>(base + F::kValue, base + F::kProb, part_at + (2 * own_stage + 1) * F::kPart, i != 0);
+                multiply_columns<T, kStream, DP>(base + F::kKey, base + F::kProbGrad, part_at + 2 * own_stage * F::kPart, i != 0);
+                commit(&empty[own_stage]);
+                commit(&o_done);
+                if (++own_stage == F::kStages) own_stage = 0;
+                if ((!F::kApart || i + 1 == steps) && job < jobs && !(fine = scores())) break;
+            }
         }
+        commit(&ended);
+        drain(&ended, 0);
     } else {
-        const int j = j0 + threadIdx.x;
-        const bool live = j <= last;
-        const int low = live ? j : 0, high = live ? past_query(p, j) - 1 : -1;          // the queries that see the key
+        const int row = threadIdx.x;
         const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
         bool fine = true;
-        for (int n = 0; n < count; ++n) {
-            const int s = n % F::kStages, i = i0 + n % each * kStream;
-            // the statistics came with the tile that the scores waited for; this wait makes them visible here, too
-            if (!(fine = warp_wait(&full[s], n / F::kStages & 1, &lost) && warp_wait(&s_full, n & 1, &lost))) break;
-            fence_after();
-            uint32_t r[kStream], d[kStream], packed[kStream / 2];
-#pragma unroll
-            for (int c = 0; c < kStream; c += 32) { tensor_load(mine + c, r + c); tensor_load(mine + F::kGrad + c, d + c); }
-            wait_loads();
-            const float4 *l4 = reinterpret_cast<const float4*>(lse[s]), *d4 = reinterpret_cast<const float4*>(delta[s]);
-#pragma unroll
-            for (int c = 0; c < kStream; c += 4) {
-                const float4 l = l4[c / 4], e = d4[c / 4];
-                const float ls[4] = {l.x, l.y, l.z, l.w}, es[4] = {e.x, e.y, e.z, e.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float prob = exp2_fast(fmaf(__uint_as_float(r[c + k]), p.scale2, -ls[k]));
-                    r[c + k] = __float_as_uint(prob);
-                    d[c + k] = __float_as_uint(prob * (__uint_as_float(d[c + k]) - es[k]));
+        int n = 0, keys = 0, stage = 0, phase = 0;
+        struct Leaving { int first, last, head; } leaving{0, -1, 0};
+        auto leave = [&]() {
+            if (DP == 64) {
+                unsigned char *const dv = shared + F::kStaged, *const dk = dv + F::kTile;
+                if (row == 0) wait_stores_read();
+                meet(1, kRows);
+                stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row);
+                stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row);
+                fence_shared();
+                meet(1, kRows);
+                if (row == 0 && leaving.first <= leaving.last) {
+                    store_tile(&map_dv, dv, 0, leaving.head, leaving.first);
+                    store_tile(&map_dk, dk, 0, leaving.head, leaving.first);
+                    stores_end();
                 }
+            } else {
+                const int j = leaving.first + row;
+                const int64_t at = ((int64_t)j * p.heads_k + leaving.head) * p.dim;
+                const bool there = j <= leaving.last;
+                store_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), p.dim, there ? static_cast<T*>(p.dv) + at : nullptr);
+                store_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), p.dim, there ? static_cast<T*>(p.dk) + at : nullptr);
             }
-            if (!__all_sync(~0u, i >= low && i + kStream - 1 <= high)) {
-                const int from = low - i, to = high - i;
+        };
+        KeyJob next(p, blockIdx.x);
+        auto end_of = [&](const KeyJob& job) { return p.end[min(job.j0 + row, job.last)]; };
+        int next_end = end_of(next);
+        const Pair scale2 = pair_of(p.scale2, p.scale2), minus_one = pair_of(-1.f, -1.f);
+        for (int job = blockIdx.x; job < jobs; job += stride, ++keys) {
+            const KeyJob now = next;
+            const int j = now.j0 + row, each = now.steps(p);
+            const bool live = j <= now.last;
+            // the queries that see the key
+            const int low = live ? j : 0, high = !live ? -1 : (p.window > 0 ? (int)min((int64_t)next_end, (int64_t)j + p.window) : next_end) - 1;
+            if (job + stride < jobs) { next = KeyJob(p, job + stride); next_end = end_of(next); }
+            const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
+            const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
+            bool first = true, left = false;
+            for (int h = 0; fine && h < group; ++h)
+                for (int m = 0; m < each; ++m, ++n) {
+                    const int i = now.begin() + m * kStream;
+                    // the statistics came with the tile that the scores waited for; this wait makes them visible here, too
+                    fine = fine && warp_wait(&full[stage], phase, &lost) && warp_wait(&s_full, n & 1, &lost);
+                    if (!fine) break;
+                    fence_after();
+                    uint32_t probs[kStream / 2], grads[kStream / 2];
+                    const float4 *l4 = reinterpret_cast<const float4*>(lse[stage]), *d4 = reinterpret_cast<const float4*>(delta[stage]);
+                    const bool all = i >= all_low && i + kStream - 1 <= all_high;
 #pragma unroll
-                for (int c = 0; c < kStream; ++c)
-                    if (c < from || c > to) r[c] = d[c] = 0u;
-            }
-            if (F::kApart && n > 0 && !(fine = warp_wait(&o_done, (n - 1) & 1, &lost))) break;
+                    for (int c0 = 0; c0 < kStream; c0 += 32) {
+                        uint32_t r[32], d[32];
+                        tensor_load(mine + c0, r);
+                        tensor_load(mine + F::kGrad + c0, d);
+                        wait_loads();
+                        if (i + c0 > any_high || i + c0 + 31 < any_low) {
 #pragma unroll
-            for (int c = 0; c < kStream; c += 2) packed[c / 2] = pack<T>(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-            tensor_store(mine + F::kProb, packed);
+                            for (int c = 0; c < 16; ++c) probs[c0 / 2 + c] = grads[c0 / 2 + c] = 0u;
+                            continue;
+                        }
+                        const uint32_t seen = all ? ~0u : columns_between(low - i - c0, high - i - c0);
 #pragma unroll
-            for (int c = 0; c < kStream; c += 2) packed[c / 2] = pack<T>(__uint_as_float(d[c]), __uint_as_float(d[c + 1]));
-            tensor_store(mine + F::kProbGrad, packed);
-            wait_stores();
-            fence_before();
-            barrier_arrive(&p_full);
+                        for (int c = 0; c < 32; c += 4) {
+                            const float4 l = l4[(c0 + c) / 4], e = d4[(c0 + c) / 4];
+                            const Pair ls[2] = {pair_of(l.x, l.y), pair_of(l.z, l.w)}, es[2] = {pair_of(e.x, e.y), pair_of(e.z, e.w)};
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int at = c0 + c + 2 * k;
+                                float a, b, x, y;
+                                split(fma_pair(ls[k], minus_one, mul_pair(pair_of(__uint_as_float(r[at - c0]), __uint_as_float(r[at - c0 + 1])), scale2)), a, b);
+                                a = exp2_fast(a);
+                                b = exp2_fast(b);
+                                split(mul_pair(pair_of(a, b), fma_pair(es[k], minus_one, pair_of(__uint_as_float(d[at - c0]), __uint_as_float(d[at - c0 + 1])))), x, y);
+                                if (!all) {
+                                    const bool u = seen >> (at - c0) & 1u, v = seen >> (at - c0 + 1) & 1u;
+                                    a = u ? a : 0.f; x = u ? x : 0.f;
+                                    b = v ? b : 0.f; y = v ? y : 0.f;
+                                }
+                                probs[at / 2] = pack<T>(a, b);
+                                grads[at / 2] = pack<T>(x, y);
+                            }
+                        }
+                    }
+                    if (n > 0 && (F::kApart || first)) fine = warp_wait(&o_done, (n - 1) & 1, &lost);
+                    if (!fine) break;
+                    if (n > 0) fence_after();
+                    if (first && n > 0) { leave(); left = true; }
+                    first = false;
+                    tensor_store(mine + F::kProb, probs);
+                    tensor_store(mine + F::kProbGrad, grads);
+                    wait_stores();
+                    fence_before();
+                    barrier_arrive(&p_full);
+                    if (++stage == F::kStages) { stage = 0; phase ^= 1; }
+                }
+            if (keys > 0 && !left) leave();             // a block that gave up: NaN for this job's, and below for what is left
+            leaving = {now.j0, now.last, now.head};
         }
-        fine = fine && warp_wait(&o_done, (count - 1) & 1, &lost);
+        fine = fine && warp_wait(&o_done, (n - 1) & 1, &lost);
         fence_after();
-        const int64_t at = ((int64_t)j * p.heads_k + key_head) * p.dim;
-        store_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), p.dim, live ? static_cast<T*>(p.dv) + at : nullptr);
-        store_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), p.dim, live ? static_cast<T*>(p.dk) + at : nullptr);
+        leave();
+        if (row == 0) wait_stores_done();
     }
     __syncwarp();
     fence_before();
@@ -780,15 +966,19 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
         attention_kernel<T, DP><<<(unsigned)std::min(p.across * p.along, 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();
     }
+    CUtensorMap dq, dk, dv;
     for (int keys = 0; keys < 2; ++keys) {
         const int own = keys ? kStream : kRows, other = keys ? kRows : kStream;
         cudaError_t set = keys ? with_shared(key_grad_kernel<T, DP>, Keys<DP>::kShared) : with_shared(query_grad_kernel<T, DP>, Queries<DP>::kShared);
         if (set != cudaSuccess) return set;
-        if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, own) || !map_of(&g, d.dtype, d.dout, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, own) ||
-            !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, other) || !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, other))
+        const int64_t wide = d.dim * d.heads_q, narrow = d.dim * d.heads_k;
+        if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, own) || !map_of(&g, d.dtype, d.dout, d.dim, d.heads_q, e.tokens, d.dim, wide, own) ||
+            !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, other) || !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, other) ||
+            !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, wide, kRows) || !map_of(&dq, d.dtype, d.dq, d.dim, d.heads_q, e.tokens, d.dim, wide, p.span) ||
+            !map_of(&dk, d.dtype, d.dk, d.dim, d.heads_k, e.tokens, d.dim, narrow, p.span) || !map_of(&dv, d.dtype, d.dv, d.dim, d.heads_k, e.tokens, d.dim, narrow, p.span))
             return cudaErrorInvalidValue;
-        if (keys) key_grad_kernel<T, DP><<<(unsigned)(p.tiles * d.heads_k), kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, p);
-        else query_grad_kernel<T, DP><<<(unsigned)(p.tiles * d.heads_q), kBlock, Queries<DP>::kShared, stream>>>(q, g, k, v, p);
+        if (keys) key_grad_kernel<T, DP><<<(unsigned)std::min(p.tiles * p.heads_k, DP == 64 ? 2 * 148 : 148), kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
+        else query_grad_kernel<T, DP><<<(unsigned)std::min(p.tiles * p.heads_q, 2 * 148), kBlock, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         set = cudaGetLastError();
         if (set != cudaSuccess) return set;
     }

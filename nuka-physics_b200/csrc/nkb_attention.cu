@@ -581,7 +581,9 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
             if (job + stride < jobs) { next = QueryJob(p, job + stride); next_first = first_of(next); next_lse = lse_of(next); }
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
-            // D = dO . O of the thread's row, which the keys' kernel reads after this one
+            // D = dO . O of the thread's row.  O has the error of its own rounding and of P's, which the sum of dS over the row, 0 by definition, shows: the keys' kernel, which runs
+            // after this one, gets D without it. Where a step holds all keys of a row D is summed from its own P and dP before dS, which matters where few keys share a row (dq of
+            // 24-token episodes was off by 1.8 times its rounding; with many keys the error averages out).
             float delta = 0.f;
             if (F::kApart) {
                 fine = fine && warp_wait(&q_full, queries & 1, &lost);
@@ -607,8 +609,8 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                     for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
                 }
             }
-            if (live) p.delta[now.head * p.pitch + i] = delta;
-            const Pair scale2 = pair_of(p.scale2, p.scale2), shift = pair_of(-lse, -lse), minus = pair_of(-delta, -delta);
+            const Pair scale2 = pair_of(p.scale2, p.scale2), shift = pair_of(-lse, -lse);
+            Pair off = pair_of(0.f, 0.f);
             bool left = false;
             for (int j = 0; j < count; ++j, ++n) {
                 const int k0 = j0 + j * kStream;
@@ -617,21 +619,13 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                 fence_after();
                 uint32_t packed[kStream / 2];
                 const bool all = k0 >= all_low && k0 + kStream - 1 <= all_high;
-#pragma unroll
-                for (int c0 = 0; c0 < kStream; c0 += 32) {
+                auto hidden = [&](int c0) { return k0 + c0 > any_high || k0 + c0 + 31 < any_low; };          // from all of the warp's rows
+                // P and P (dP - D) of 32 keys
+                auto part = [&](int c0, Pair minus, auto use) {
                     uint32_t r[32], d[32];
                     tensor_load(mine + c0, r);
                     tensor_load(mine + F::kGrad + c0, d);
                     wait_loads();
-                    if (c0 + 32 == kStream) {
-                        fence_before();
-                        barrier_arrive(&s_empty);
-                    }
-                    if (k0 + c0 > any_high || k0 + c0 + 31 < any_low) {             // hidden from all of the warp's rows
-#pragma unroll
-                        for (int c = 0; c < 16; ++c) packed[c0 / 2 + c] = 0u;
-                        continue;
-                    }
                     const uint32_t seen = all ? ~0u : columns_between(low - k0 - c0, high - k0 - c0);
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
@@ -644,9 +638,32 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                             x = seen >> c & 1u ? x : 0.f;
                             y = seen >> (c + 1) & 1u ? y : 0.f;
                         }
-                        packed[(c0 + c) / 2] = pack<T>(x, y);
+                        use(c0 + c, x, y);
+                    }
+                };
+                const bool whole = live && low >= k0 && high < k0 + kStream;
+                if (__any_sync(~0u, whole)) {
+                    float own = 0.f;
+#pragma unroll 1
+                    for (int c0 = 0; c0 < kStream; c0 += 32)
+                        if (!hidden(c0)) part(c0, pair_of(0.f, 0.f), [&](int, float x, float y) { own += x + y; });
+                    if (whole) delta = own;
+                }
+                const Pair minus = pair_of(-delta, -delta);
+#pragma unroll
+                for (int c0 = 0; c0 < kStream; c0 += 32) {
+                    if (hidden(c0)) {
+#pragma unroll
+                        for (int c = 0; c < 16; ++c) packed[c0 / 2 + c] = 0u;
+                    } else {
+                        part(c0, minus, [&](int c, float x, float y) {
+                            off = add_pair(off, pair_of(x, y));
+                            packed[c / 2] = pack<T>(x, y);
+                        });
                     }
                 }
+                fence_before();
+                barrier_arrive(&s_empty);
                 if (n > 0) fine = warp_wait(&o_done, (n - 1) & 1, &lost);
                 if (!fine) break;
                 if (n > 0) fence_after();
@@ -656,6 +673,9 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                 fence_before();
                 barrier_arrive(&p_full);
             }
+            float x, y;
+            split(off, x, y);
+            if (live) p.delta[now.head * p.pitch + i] = delta + (x + y);
             if (queries > 0 && !left) leave();          // a block that gave up: NaN for this job's, and below for what is left
             leaving = {now.i0, now.last, now.head};
         }
@@ -977,8 +997,10 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
             !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, wide, kRows) || !map_of(&dq, d.dtype, d.dq, d.dim, d.heads_q, e.tokens, d.dim, wide, p.span) ||
             !map_of(&dk, d.dtype, d.dk, d.dim, d.heads_k, e.tokens, d.dim, narrow, p.span) || !map_of(&dv, d.dtype, d.dv, d.dim, d.heads_k, e.tokens, d.dim, narrow, p.span))
             return cudaErrorInvalidValue;
-        if (keys) key_grad_kernel<T, DP><<<(unsigned)std::min(p.tiles * p.heads_k, DP == 64 ? 2 * 148 : 148), kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
-        else query_grad_kernel<T, DP><<<(unsigned)std::min(p.tiles * p.heads_q, 2 * 148), kBlock, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
+        // few jobs, that is long ones, are better dealt out by the hardware as blocks end
+        const int jobs = p.tiles * (keys ? p.heads_k : p.heads_q), slots = keys && DP != 64 ? 148 : 2 * 148, blocks = jobs <= 4 * slots ? jobs : slots;
+        if (keys) key_grad_kernel<T, DP><<<(unsigned)blocks, kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
+        else query_grad_kernel<T, DP><<<(unsigned)blocks, kBlock, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         set = cudaGetLastError();
         if (set != cudaSuccess) return set;
     }

@@ -127,25 +127,28 @@ def _tokens_of(tensor, episodes, dims, what):
 
 
 # ---- the gated linear recurrence -----------------------------------------------------------------------------------
+def _recur(x, gate, initial, episodes):
+    device, dtype, channels = x.device, _DTYPES[x.dtype], x.shape[1]
+    h = torch.empty(x.shape, dtype=x.dtype, device=device)
+    if not episodes._rows_may_be_empty:
+        state = torch.empty((episodes.rows, channels), dtype=torch.float32, device=device)
+    elif initial is None:
+        state = torch.zeros((episodes.rows, channels), dtype=torch.float32, device=device)
+    else:
+        state = initial.clone()
+    lib = _abi.lib()
+    need = lib.nuka_b200_recurrence_workspace(episodes._ref, channels)
+    workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), state.data_ptr(),
+                               None, None, None, None, None, _ptr(workspace), need)
+    _call(device, lib.nuka_b200_recurrence, ctypes.byref(desc))
+    return h, state
+
+
 class _Recurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, initial, episodes):
-        device, dtype = x.device, _DTYPES[x.dtype]
-        x, gate = _channels_last(x), _channels_last(gate)
-        channels = x.shape[1]
-        h = torch.empty(x.shape, dtype=x.dtype, device=device)
-        if not episodes._rows_may_be_empty:
-            state = torch.empty((episodes.rows, channels), dtype=torch.float32, device=device)
-        elif initial is None:
-            state = torch.zeros((episodes.rows, channels), dtype=torch.float32, device=device)
-        else:
-            state = initial.clone()
-        lib = _abi.lib()
-        need = lib.nuka_b200_recurrence_workspace(episodes._ref, channels)
-        workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-        desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), state.data_ptr(),
-                                   None, None, None, None, None, _ptr(workspace), need)
-        _call(device, lib.nuka_b200_recurrence, ctypes.byref(desc))
+        h, state = _recur(x, gate, initial, episodes)
         ctx.episodes, ctx.has_initial = episodes, initial is not None
         ctx.save_for_backward(x, gate, h, *([initial] if initial is not None else []))
         ctx.set_materialize_grads(False)
@@ -188,7 +191,9 @@ def gated_recurrence(x, gate, episodes, initial=None):
     if initial is not None:
         _expect(tuple(initial.shape) == (episodes.rows, x.shape[1]) and initial.dtype == torch.float32, f"initial must be {episodes.rows} x {x.shape[1]} float32 on {device}")
         initial = initial.contiguous()
-    return _Recurrence.apply(x, gate, initial, episodes)
+    train = torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (initial is not None and initial.requires_grad))
+    x, gate = _channels_last(x), _channels_last(gate)
+    return _Recurrence.apply(x, gate, initial, episodes) if train else _recur(x, gate, initial, episodes)
 
 
 def gated_recurrence_step(x, gate, state, fresh=None):
@@ -219,17 +224,21 @@ def rotary_frequencies(turned, base=10000.0, trained=0, context=0, low=1.0, high
     return f
 
 
+def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
+    device = q.device
+    tokens, heads_q, dim = q.shape
+    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=q.dtype, device=device)
+    desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), tokens, heads_q, k.shape[1], dim,
+                          0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
+                          _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
+    _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
+    return q_out, k_out, desc
+
+
 class _Heads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
-        device, size = q.device, q.element_size()
-        q, k = (_channels_last(x, 4, 4 * size) for x in (q, k))
-        tokens, heads_q, dim = q.shape
-        q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=q.dtype, device=device)
-        desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), tokens, heads_q, k.shape[1], dim,
-                              0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
-                              _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
-        _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
+        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved)
         # the descriptor's arrays stay alive with what is saved here
         ctx.save_for_backward(q, k, *(x for x in (q_weight, k_weight, first, positions, frequencies) if x is not None))
         ctx.desc, ctx.weights = desc, (q_weight is not None, k_weight is not None)
@@ -274,21 +283,31 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
         _expect(positions.dtype == torch.int32 and tuple(positions.shape) == (q.shape[0],), "positions must be an Episodes or int32, one per token")
         first, positions = None, positions.contiguous()
     q_weight, k_weight, frequencies = (None if x is None else x.contiguous() for x in (q_weight, k_weight, frequencies))
+    size = 4 * q.element_size()
+    q, k = _channels_last(q, 4, size), _channels_last(k, 4, size)
+    train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight))
+    if not train:
+        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)[:2]
     return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
 
 
 # ---- attention over packed episodes --------------------------------------------------------------------------------
+def _attend(q, k, v, episodes, scale, window, train):
+    """(out, the statistics that a backward pass needs beside it, the call's descriptor)."""
+    device = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    lib = _abi.lib()
+    lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device) if train else None
+    desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
+                              _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
+    _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
+    return out, lse, desc
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, episodes, scale, window):
-        device = q.device
-        q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-        lib = _abi.lib()
-        lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device)
-        desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
-                                  _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), lse.data_ptr())
-        _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
+        out, lse, desc = _attend(q, k, v, episodes, scale, window, True)
         # the descriptor's arrays stay alive with what is saved here
         ctx.save_for_backward(q, k, v, out, lse)
         ctx.desc, ctx.episodes = desc, episodes
@@ -321,7 +340,10 @@ def episode_attention(q, k, v, episodes, scale=None, window=None):
     _expect(k.dtype == q.dtype and v.dtype == q.dtype and k.shape == v.shape and k.shape[2] == q.shape[2], "q, k and v must be of one type and dim, k and v of one shape")
     _expect(k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and q.shape[1] > 0, "the heads must be a multiple of the key heads")
     _expect(window is None or window >= 1, "window must be at least 1")
-    return _Attention.apply(q, k, v, episodes, q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window))
+    scale, window = q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window)
+    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
+    return _Attention.apply(q, k, v, episodes, scale, window) if train else _attend(q, k, v, episodes, scale, window, False)[0]
 
 
 # ---- attention of one token over a cached history ------------------------------------------------------------------

@@ -33,6 +33,8 @@ struct AttentionParams {
     int span, tiles;                                    // tokens of a tile, at most 128, and how many tiles
     int by_heads, across, along;                        // of the forward kernel's jobs: tiles of two heads or of two stretches of tokens; jobs side by side, and behind one another
     float scale, scale2;                                // scale2: times log2(e)
+    const void *q, *k, *v;
+    int64_t q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
     void *out, *dq, *dk, *dv;
     const void* dout;
     float *lse, *delta;
@@ -54,8 +56,9 @@ struct QueryJob {
     __device__ __forceinline__ int steps(const AttentionParams& p) const { return (last - begin(p)) / kStream + 1; }
 };
 
-// One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T.
-template <typename T, int DP> __device__ __forceinline__ void store_row(uint32_t at, float by, int dim, T* to) {
+// One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T; whether all are finite.
+template <typename T, int DP> __device__ __forceinline__ bool store_row(uint32_t at, float by, int dim, T* to) {
+    float probe = 0.f;                                  // becomes NaN where a value is not finite
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
         uint32_t r[32];
@@ -65,6 +68,8 @@ template <typename T, int DP> __device__ __forceinline__ void store_row(uint32_t
 #pragma unroll
         for (int k = 0; k < 32; k += 8)
             if (to != nullptr && c + k < dim) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) probe = fmaf(__uint_as_float(r[k + e]), 0.f, probe);
                 uint4 v;
                 v.x = pack<T>(__uint_as_float(r[k]) * by, __uint_as_float(r[k + 1]) * by);
                 v.y = pack<T>(__uint_as_float(r[k + 2]) * by, __uint_as_float(r[k + 3]) * by);
@@ -73,6 +78,7 @@ template <typename T, int DP> __device__ __forceinline__ void store_row(uint32_t
                 *reinterpret_cast<uint4*>(to + c + k) = v;
             }
     }
+    return probe == 0.f;
 }
 
 // ROWS x DP of one head: panels of 64 columns, each ROWS x 128 bytes
@@ -103,8 +109,9 @@ __device__ __forceinline__ uint32_t columns_between(int from, int to) {
 
 // A row of 64-column panels of 128 rows, swizzled as TMA takes it: 16 bytes number `k` of row `row`.
 __device__ __forceinline__ unsigned char* staged(unsigned char* tile, int row, int k) { return tile + k / 8 * kRows * 128 + row * 128 + ((k % 8) ^ (row % 8)) * 16; }
-// A thread's row of 32-bit accumulators, times `by`, into a staged tile of T.
-template <typename T, int DP> __device__ __forceinline__ void stage_row(uint32_t at, float by, unsigned char* tile, int row) {
+// A thread's row of 32-bit accumulators, times `by`, into a staged tile of T; whether all are finite.
+template <typename T, int DP> __device__ __forceinline__ bool stage_row(uint32_t at, float by, unsigned char* tile, int row) {
+    float probe = 0.f;                                  // becomes NaN where a value is not finite
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
         uint32_t r[32];
@@ -112,6 +119,8 @@ template <typename T, int DP> __device__ __forceinline__ void stage_row(uint32_t
         wait_loads();
 #pragma unroll
         for (int k = 0; k < 32; k += 8) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) probe = fmaf(__uint_as_float(r[k + e]), 0.f, probe);
             uint4 v;
             v.x = pack<T>(__uint_as_float(r[k]) * by, __uint_as_float(r[k + 1]) * by);
             v.y = pack<T>(__uint_as_float(r[k + 2]) * by, __uint_as_float(r[k + 3]) * by);
@@ -120,6 +129,73 @@ template <typename T, int DP> __device__ __forceinline__ void stage_row(uint32_t
             *reinterpret_cast<uint4*>(staged(tile, row, (c + k) / 8)) = v;
         }
     }
+    return probe == 0.f;
+}
+
+// ---- rows that are not finite -----------------------------------------------------------------------------------------
+// A product over a tile multiplies what a row does not see by 0, and 0 times an infinity or NaN is NaN: an episode that is not finite would reach the others of its tiles. So a row that comes out
+// not finite is worked out again by its thread alone, in 32 bits, from what it sees and nothing else. That is slow, and only then.
+template <typename T> __device__ __forceinline__ float dot(const T* a, const T* b, int dim) {
+    float s = 0.f;
+    for (int c = 0; c < dim; c += 8) {
+        float u[8], v[8];
+        unpack<T, 8>(load_raw<T, 8>(a + c), u);
+        unpack<T, 8>(load_raw<T, 8>(b + c), v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s = fmaf(u[k], v[k], s);
+    }
+    return s;
+}
+template <typename T> __device__ __forceinline__ void add_row(float* sum, float by, const T* row, int dim) {
+    for (int c = 0; c < dim; c += 8) {
+        float v[8];
+        unpack<T, 8>(load_raw<T, 8>(row + c), v);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum[c + k] = fmaf(by, v[k], sum[c + k]);
+    }
+}
+template <typename T> __device__ __forceinline__ const T* query_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.q) + i * p.q_stride + head * p.q_head_stride; }
+template <typename T> __device__ __forceinline__ const T* key_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.k) + j * p.k_stride + head * p.k_head_stride; }
+template <typename T> __device__ __forceinline__ const T* value_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.v) + j * p.v_stride + head * p.v_head_stride; }
+template <typename T> __device__ __forceinline__ const T* dout_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.dout) + ((int64_t)i * p.heads_q + head) * p.dim; }
+template <typename T> __device__ __forceinline__ float probability(const AttentionParams& p, int i, int j, int head, int key_head, float lse) {
+    return exp2f(fmaf(dot<T>(query_row<T>(p, i, head), key_row<T>(p, j, key_head), p.dim), p.scale2, -lse));
+}
+__device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
+__device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+
+template <typename T> __device__ __noinline__ void slow_out(const AttentionParams& p, int i, int head, float lse, float* sum) {
+    const int key_head = head / (p.heads_q / p.heads_k);
+    for (int c = 0; c < p.dim; ++c) sum[c] = 0.f;
+    for (int j = first_key(p, i); j <= i; ++j) add_row<T>(sum, probability<T>(p, i, j, head, key_head, lse), value_row<T>(p, j, key_head), p.dim);
+}
+template <typename T> __device__ __noinline__ void slow_query_grad(const AttentionParams& p, int i, int head, float lse, float delta, float* sum) {
+    const int key_head = head / (p.heads_q / p.heads_k);
+    for (int c = 0; c < p.dim; ++c) sum[c] = 0.f;
+    for (int j = first_key(p, i); j <= i; ++j) {
+        const float ds = probability<T>(p, i, j, head, key_head, lse) * (dot<T>(dout_row<T>(p, i, head), value_row<T>(p, j, key_head), p.dim) - delta);
+        add_row<T>(sum, ds * p.scale, key_row<T>(p, j, key_head), p.dim);
+    }
+}
+// values: the value's gradient, else the key's
+template <typename T> __device__ __noinline__ void slow_key_grad(const AttentionParams& p, int j, int key_head, bool values, float* sum) {
+    const int group = p.heads_q / p.heads_k;
+    for (int c = 0; c < p.dim; ++c) sum[c] = 0.f;
+    for (int head = key_head * group; head < (key_head + 1) * group; ++head)
+        for (int i = j; i < past_query(p, j); ++i) {
+            const float prob = probability<T>(p, i, j, head, key_head, p.lse[head * p.pitch + i]);
+            if (values) {
+                add_row<T>(sum, prob, dout_row<T>(p, i, head), p.dim);
+            } else {
+                const float ds = prob * (dot<T>(dout_row<T>(p, i, head), value_row<T>(p, j, key_head), p.dim) - p.delta[head * p.pitch + i]);
+                add_row<T>(sum, ds * p.scale, query_row<T>(p, i, head), p.dim);
+            }
+        }
+}
+template <typename T> __device__ __forceinline__ uint4 pack_row(const float* v) {
+    uint4 r;
+    r.x = pack<T>(v[0], v[1]); r.y = pack<T>(v[2], v[3]); r.z = pack<T>(v[4], v[5]); r.w = pack<T>(v[6], v[7]);
+    return r;
 }
 
 // A block that gave up waits, again for a bounded time, for the loads that it still has under way; what they bring is not used.
@@ -151,6 +227,8 @@ template <int DP> struct Forward {
     static constexpr int kTile = kRows * DP * 2, kPart = kStep * DP * 2;
     static constexpr int kKeys = 2 * kQueries * kTile, kStaged = kKeys + 2 * kStages * kPart, kShared = kStaged + 2 * kTile + 1024;
     static constexpr int kProb = kStep, kOut = kStep + kStep / 2, kSet = 256;                  // columns; the scores are at 0
+    // Rows leave under the next job's exponentials, for which P is held back; wide heads, whose P goes out as it comes, have not the registers (their jobs are longer, too).
+    static constexpr bool kLate = DP == 64;
 };
 
 // What it reads of the plan is looked at only when it is used, a job after it was asked for.
@@ -315,7 +393,13 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             const int i = leaving.first + row;
             if (row == 0) wait_stores_read();
             meet(1 + set, kRows);
-            stage_row<T, DP>(mine + F::kOut, fine ? 1.f / leaving.sum : nan_value(), tile, row);
+            const bool finite = stage_row<T, DP>(mine + F::kOut, fine ? 1.f / leaving.sum : nan_value(), tile, row);
+            const float lse = fine ? fmaf(leaving.top, p.scale2, log2f(leaving.sum)) : nan_value();
+            if (fine && !finite && i <= leaving.last) {
+                float values[DP];
+                slow_out<T>(p, i, leaving.head, lse, values);
+                for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
+            }
             fence_shared();
             meet(1 + set, kRows);
             if (row == 0 && leaving.first <= leaving.last) {
@@ -324,7 +408,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                     if (c < p.dim) store_tile(&map_o, tile + c / 64 * kRows * 128, c, leaving.head, leaving.first);
                 stores_end();
             }
-            if (i <= leaving.last && p.lse != nullptr) p.lse[leaving.head * p.pitch + i] = fine ? fmaf(leaving.top, p.scale2, log2f(leaving.sum)) : nan_value();
+            if (i <= leaving.last && p.lse != nullptr) p.lse[leaving.head * p.pitch + i] = lse;
         };
         ForwardJob next(p, blockIdx.x);
         auto first_of = [&](const ForwardJob& job) { return p.first[min(job.i0[set] + row, job.last[set] >= job.i0[set] ? job.last[set] : 0)]; };
@@ -354,6 +438,17 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 Pair part[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
                 float by = 1.f;
                 bool any = false;
+                auto rescale = [&]() {
+#pragma unroll
+                    for (int c = 0; c < DP; c += 32) {
+                        uint32_t o[32];
+                        tensor_load(mine + F::kOut + c, o);
+                        wait_loads();
+#pragma unroll
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
+                        tensor_store(mine + F::kOut + c, o);
+                    }
+                };
                 // all: every row of the warp sees every key; else CHUNK keys at a time may be hidden from all, or from some
                 auto rows = [&](auto all) {
                     constexpr bool ALL = decltype(all)::value != 0;
@@ -380,6 +475,11 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                     sum *= by;
                     const float shift = top == -INFINITY ? 0.f : -top * p.scale2;
                     const Pair shifts = pair_of(shift, shift);
+                    if (!F::kLate && n > 0) {
+                        if (!warp_wait(&o_done[set], (n - 1) & 1, &lost)) return false;
+                        fence_after();
+                        if (any && j > 0) rescale();
+                    }
 #pragma unroll
                     for (int c = 0; c < F::kStep; c += CHUNK) {
                         if (hidden(c)) {
@@ -396,39 +496,45 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                                 packed[(c + k) / 2] = pack<T>(a, b);
                             }
                         }
+                        if (!F::kLate)
+#pragma unroll
+                            for (int k = 0; k < CHUNK / 2; k += 8) tensor_store8(mine + F::kProb + c / 2 + k, packed + c / 2 + k);
                     }
+                    return true;
                 };
-                if (k0 >= all_low && k0 + F::kStep - 1 <= all_high) rows(Number<1>{}); else rows(Number<0>{});
+                if (!(fine = k0 >= all_low && k0 + F::kStep - 1 <= all_high ? rows(Number<1>{}) : rows(Number<0>{}))) break;
                 float x, y;
                 split(add_pair(part[0], part[1]), x, y);
                 sum += x + y;
-                // P V of the step before has ended: P and O may be written, and the rows of a job that it ended may leave
-                if (n > 0) fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
-                if (!fine) break;
-                if (n > 0) fence_after();
-                if (j == 0 && n > 0) { leave(); left = true; }
-                if (any && j > 0)
-#pragma unroll
-                    for (int c = 0; c < DP; c += 32) {
-                        uint32_t o[32];
-                        tensor_load(mine + F::kOut + c, o);
-                        wait_loads();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * by);
-                        tensor_store(mine + F::kOut + c, o);
+                if (F::kLate) {
+                    // P V of the step before has ended: P and O may be written, and the rows of a job that it ended may leave
+                    if (n > 0) {
+                        fine = warp_wait(&o_done[set], (n - 1) & 1, &lost);
+                        if (!fine) break;
+                        fence_after();
+                        if (j == 0) { leave(); left = true; }
+                        if (any && j > 0) rescale();
                     }
 #pragma unroll
-                for (int c = 0; c < F::kStep / 2; c += 8) tensor_store8(mine + F::kProb + c, packed + c);
+                    for (int c = 0; c < F::kStep / 2; c += 8) tensor_store8(mine + F::kProb + c, packed + c);
+                }
                 wait_stores();
                 fence_before();
                 barrier_arrive(&p_full[set]);
             }
-            if (turn > 0 && !left) leave();             // a block that gave up: NaN for this job's, and below for what is left
-            leaving = {first, last, head, top, sum};
+            if (F::kLate && turn > 0 && !left) leave(); // a block that gave up: NaN for this job's, and below for what is left
+            leaving = Leaving{first, last, head, top, sum};
+            if (!F::kLate) {
+                fine = fine && warp_wait(&o_done[set], (n - 1) & 1, &lost);
+                fence_after();
+                leave();
+            }
         }
-        fine = fine && warp_wait(&o_done[set], (n - 1) & 1, &lost);
-        fence_after();
-        leave();
+        if (F::kLate) {
+            fine = fine && warp_wait(&o_done[set], (n - 1) & 1, &lost);
+            fence_after();
+            leave();
+        }
         if (row == 0) wait_stores_done();
     }
     __syncwarp();
@@ -549,13 +655,20 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
         const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
         bool fine = true;
         int n = 0, queries = 0;
-        struct Leaving { int first, last, head; } leaving{0, -1, 0};
+        struct Leaving { int first, last, head; float lse, delta; } leaving{0, -1, 0, 0.f, 0.f};
         auto leave = [&]() {
+            const int i = leaving.first + row;
+            const bool there = i <= leaving.last;
+            float values[DP];
             if (F::kApart) {
                 unsigned char* const tile = shared + F::kStaged;
                 if (row == 0) wait_stores_read();
                 meet(1, kRows);
-                stage_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), tile, row);
+                const bool finite = stage_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), tile, row);
+                if (fine && !finite && there) {
+                    slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
+                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
+                }
                 fence_shared();
                 meet(1, kRows);
                 if (row == 0 && leaving.first <= leaving.last) {
@@ -563,8 +676,11 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                     stores_end();
                 }
             } else {
-                const int i = leaving.first + row;
-                store_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), p.dim, i <= leaving.last ? static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + leaving.head) * p.dim : nullptr);
+                T* const to = static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + leaving.head) * p.dim;
+                if (!store_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), p.dim, there ? to : nullptr) && fine) {
+                    slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
+                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(to + c) = pack_row<T>(values + c);
+                }
             }
         };
         QueryJob next(p, blockIdx.x);
@@ -675,9 +791,10 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
             }
             float x, y;
             split(off, x, y);
-            if (live) p.delta[now.head * p.pitch + i] = delta + (x + y);
+            delta += x + y;
+            if (live) p.delta[now.head * p.pitch + i] = delta;
             if (queries > 0 && !left) leave();          // a block that gave up: NaN for this job's, and below for what is left
-            leaving = {now.i0, now.last, now.head};
+            leaving = Leaving{now.i0, now.last, now.head, lse, delta};
         }
         fine = fine && warp_wait(&o_done, (n - 1) & 1, &lost);
         fence_after();
@@ -825,12 +942,19 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
         int n = 0, keys = 0, stage = 0, phase = 0;
         struct Leaving { int first, last, head; } leaving{0, -1, 0};
         auto leave = [&]() {
+            const int j = leaving.first + row;
+            const bool there = j <= leaving.last;
+            float values[DP];
             if (DP == 64) {
                 unsigned char *const dv = shared + F::kStaged, *const dk = dv + F::kTile;
                 if (row == 0) wait_stores_read();
                 meet(1, kRows);
-                stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row);
-                stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row);
+                const bool finite[2] = {stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row), stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row)};
+                for (int which = 0; which < 2; ++which)
+                    if (fine && !finite[which] && there) {
+                        slow_key_grad<T>(p, j, leaving.head, which, values);
+                        for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(which ? dv : dk, row, c / 8)) = pack_row<T>(values + c);
+                    }
                 fence_shared();
                 meet(1, kRows);
                 if (row == 0 && leaving.first <= leaving.last) {
@@ -839,11 +963,14 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
                     stores_end();
                 }
             } else {
-                const int j = leaving.first + row;
-                const int64_t at = ((int64_t)j * p.heads_k + leaving.head) * p.dim;
-                const bool there = j <= leaving.last;
-                store_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), p.dim, there ? static_cast<T*>(p.dv) + at : nullptr);
-                store_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), p.dim, there ? static_cast<T*>(p.dk) + at : nullptr);
+                T* const to[2] = {static_cast<T*>(p.dk) + ((int64_t)j * p.heads_k + leaving.head) * p.dim, static_cast<T*>(p.dv) + ((int64_t)j * p.heads_k + leaving.head) * p.dim};
+                const bool finite[2] = {store_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), p.dim, there ? to[0] : nullptr),
+                                        store_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), p.dim, there ? to[1] : nullptr)};
+                for (int which = 0; which < 2; ++which)
+                    if (fine && !finite[which] && there) {
+                        slow_key_grad<T>(p, j, leaving.head, which, values);
+                        for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(to[which] + c) = pack_row<T>(values + c);
+                    }
             }
         };
         KeyJob next(p, blockIdx.x);
@@ -973,6 +1100,8 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
     p.by_heads = p.heads_q / p.heads_k % 2 == 0;
     p.across = p.by_heads ? p.heads_q / 2 : p.heads_q; p.along = p.by_heads ? p.tiles : (p.tiles + 1) / 2;
     p.scale = d.scale; p.scale2 = d.scale * kLog2e;
+    p.q = d.q; p.k = d.k; p.v = d.v; p.q_stride = d.q_stride; p.q_head_stride = d.q_head_stride; p.k_stride = d.k_stride; p.k_head_stride = d.k_head_stride;
+    p.v_stride = d.v_stride; p.v_head_stride = d.v_head_stride;
     p.out = d.out; p.lse = d.lse; p.dout = d.dout; p.delta = d.delta; p.dq = d.dq; p.dk = d.dk; p.dv = d.dv;
     if (encoder() == nullptr) return cudaErrorNotSupported;
     CUtensorMap q, k, v, g, o;

@@ -21,32 +21,40 @@ from . import _abi, _check
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 
 
+# Acting is one small call after the other: what is checked on every call is written to cost little, messages are put together only when they are raised.
 def _expect(ok, text):
     if not ok:
         raise ValueError(text)
 
 
-def _on_gpu(*tensors):
+def _on_gpu(first, *others):
     """The GPU that all of the tensors are on (None is left out)."""
-    device = tensors[0].device
-    _expect(device.type == "cuda", "tensors must be on the GPU")
-    for tensor in tensors:
-        _expect(tensor is None or tensor.device == device, "tensors must be on one GPU")
+    device = first.device
+    if device.type != "cuda":
+        raise ValueError("tensors must be on the GPU")
+    for tensor in others:
+        if tensor is not None and tensor.device != device:
+            raise ValueError("tensors must be on one GPU")
     return device
 
 
 def _dtype(tensor, allowed, what):
-    _expect(tensor.dtype in allowed, f"{what} must be one of {', '.join(str(d).replace('torch.', '') for d in allowed)}, not {str(tensor.dtype).replace('torch.', '')}")
+    if tensor.dtype not in allowed:
+        names = ", ".join(str(d).replace("torch.", "") for d in allowed)
+        raise ValueError(f"{what} must be one of {names}, not {str(tensor.dtype).replace('torch.', '')}")
     return _DTYPES[tensor.dtype]
 
 
 def _call(device, function, *args):
     """One call of the library on torch's current stream of `device`."""
-    if torch.cuda.current_device() != device.index:
+    index = device.index
+    if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
-            _check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+            code = function(*args, torch.cuda.current_stream(index).cuda_stream)
     else:
-        _check(function(*args, torch.cuda.current_stream(device).cuda_stream))
+        code = function(*args, torch.cuda.current_stream(index).cuda_stream)
+    if code:
+        _check(code)
 
 
 def _ptr(tensor):
@@ -54,7 +62,8 @@ def _ptr(tensor):
 
 
 def _flags(tensor, shape, device, what):
-    _expect(tensor.dtype in (torch.bool, torch.uint8) and tuple(tensor.shape) == shape and tensor.device == device, f"{what} must be {shape} bool or uint8 on {device}")
+    if not (tensor.dtype in (torch.bool, torch.uint8) and tensor.shape == shape and tensor.device == device):
+        raise ValueError(f"{what} must be {tuple(shape)} bool or uint8 on {device}")
     return tensor.contiguous()
 
 
@@ -65,10 +74,13 @@ def _stride(tensor, dim):
 def _channels_last(tensor, multiple=1, size=1, least=0):
     """The tensor as it is where its last dimension is contiguous, its other strides are multiples of `multiple` values and at least `least`, and it lies on
     `size` bytes, else a copy."""
-    last = tensor.dim() - 1
-    if ((tensor.shape[last] == 1 or tensor.stride(last) == 1) and tensor.data_ptr() % size == 0
-            and all(tensor.shape[d] <= 1 or (tensor.stride(d) % multiple == 0 and tensor.stride(d) >= least) for d in range(last))):
-        return tensor
+    strides, shape = tensor.stride(), tensor.shape
+    if (strides[-1] == 1 or shape[-1] == 1) and (size == 1 or tensor.data_ptr() % size == 0):
+        for s, n in zip(strides[:-1], shape):
+            if n > 1 and (s % multiple or s < least):
+                break
+        else:
+            return tensor
     return tensor.clone(memory_format=torch.contiguous_format)
 
 
@@ -101,7 +113,7 @@ class Episodes:
         episode ended with that token, as ``NukaVecEnv.step`` reports it."""
         _expect(done.dim() == 2, "done must be envs x steps")
         device = _on_gpu(done)
-        done = _flags(done, tuple(done.shape), device, "done")
+        done = _flags(done, done.shape, device, "done")
         plan = cls(done.numel(), done.shape[0], done.shape[1], device)
         _call(device, _abi.lib().nuka_b200_episodes_from_done, plan._ref, done.data_ptr())
         return plan
@@ -123,7 +135,8 @@ class Episodes:
 
 
 def _tokens_of(tensor, episodes, dims, what):
-    _expect(tensor.dim() == dims and tensor.shape[0] == episodes.tokens, f"{what} must have {dims} dimensions, the first of {episodes.tokens} tokens")
+    if tensor.dim() != dims or tensor.shape[0] != episodes.tokens:
+        raise ValueError(f"{what} must have {dims} dimensions, the first of {episodes.tokens} tokens")
 
 
 # ---- the gated linear recurrence -----------------------------------------------------------------------------------
@@ -145,6 +158,12 @@ def _recur(x, gate, initial, episodes):
     return h, state
 
 
+def _once(backward):
+    """Gradients that cannot be differentiated again, at no cost where nobody asks for it."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+    return staticmethod(lambda ctx, *grads: (guarded if torch.is_grad_enabled() else backward)(ctx, *grads))
+
+
 class _Recurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate, initial, episodes):
@@ -154,8 +173,7 @@ class _Recurrence(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return h, state
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dh, dstate):
         x, gate, h, *initial = ctx.saved_tensors
         initial, episodes = initial[0] if initial else None, ctx.episodes
@@ -185,11 +203,12 @@ def gated_recurrence(x, gate, episodes, initial=None):
     when the rollout began), None for 0; an episode that begins inside a row begins with 0.  Returns (h, state): h like x, state (rows x channels f32) the
     state that each row ends with, not rounded."""
     device = _on_gpu(x, gate, initial, episodes._plan)
-    _dtype(x, tuple(_DTYPES), "x")
+    _dtype(x, _DTYPES, "x")
     _tokens_of(x, episodes, 2, "x")
     _expect(gate.shape == x.shape and gate.dtype == x.dtype, "gate must be like x")
     if initial is not None:
-        _expect(tuple(initial.shape) == (episodes.rows, x.shape[1]) and initial.dtype == torch.float32, f"initial must be {episodes.rows} x {x.shape[1]} float32 on {device}")
+        if initial.shape != (episodes.rows, x.shape[1]) or initial.dtype != torch.float32:
+            raise ValueError(f"initial must be {episodes.rows} x {x.shape[1]} float32 on {device}")
         initial = initial.contiguous()
     train = torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (initial is not None and initial.requires_grad))
     x, gate = _channels_last(x), _channels_last(gate)
@@ -200,12 +219,12 @@ def gated_recurrence_step(x, gate, state, fresh=None):
     """The recurrence for one token of each env.  x, gate: envs x channels; state: envs x channels f32, contiguous, updated in place; fresh: envs, bool or
     uint8, set where the token begins an episode (the state before it counts as 0).  Returns h, the new state in x's type.  No gradient."""
     device = _on_gpu(x, gate, state, fresh)
-    dtype = _dtype(x, tuple(_DTYPES), "x")
+    dtype = _dtype(x, _DTYPES, "x")
     _expect(x.dim() == 2 and gate.shape == x.shape and gate.dtype == x.dtype, "x and gate must be envs x channels, of one type")
     _expect(state.shape == x.shape and state.dtype == torch.float32 and state.is_contiguous(), "state must be contiguous float32, envs x channels")
     x, gate = _channels_last(x), _channels_last(gate)
     if fresh is not None:
-        fresh = _flags(fresh, (x.shape[0],), device, "fresh")
+        fresh = _flags(fresh, x.shape[:1], device, "fresh")
     h = torch.empty(x.shape, dtype=x.dtype, device=device)
     _call(device, _abi.lib().nuka_b200_recurrence_step, dtype, x.shape[0], x.shape[1], x.data_ptr(), _stride(x, 0), gate.data_ptr(), _stride(gate, 0), _ptr(fresh), state.data_ptr(), h.data_ptr())
     return h
@@ -245,8 +264,7 @@ class _Heads(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         return q_out, k_out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dq_out, dk_out):
         q, k = ctx.saved_tensors[:2]
         device, desc = q.device, ctx.desc
@@ -271,16 +289,16 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     dim and the number of turned columns are multiples of 8, dim at most 256.  Returns (q, k), contiguous."""
     episodes = positions if isinstance(positions, Episodes) else None
     _on_gpu(q, k, q_weight, k_weight, frequencies, episodes._plan if episodes is not None else positions)
-    _dtype(q, tuple(_DTYPES), "q")
+    _dtype(q, _DTYPES, "q")
     _expect(q.dim() == 3 and k.dim() == 3 and k.dtype == q.dtype and k.shape[0] == q.shape[0] and k.shape[2] == q.shape[2], "q and k must be tokens x heads x dim, of one type")
     for w in (q_weight, k_weight):
-        _expect(w is None or (tuple(w.shape) == (q.shape[2],) and w.dtype == torch.float32), "weights must be float32, one per column of a head")
+        _expect(w is None or (w.shape == q.shape[2:] and w.dtype == torch.float32), "weights must be float32, one per column of a head")
     _expect(frequencies is None or (frequencies.dim() == 1 and frequencies.dtype == torch.float64), "frequencies must be a vector of float64")
     if episodes is not None:
         _tokens_of(q, episodes, 3, "q")
         first, positions = episodes.first, None
     else:
-        _expect(positions.dtype == torch.int32 and tuple(positions.shape) == (q.shape[0],), "positions must be an Episodes or int32, one per token")
+        _expect(positions.dtype == torch.int32 and positions.shape == q.shape[:1], "positions must be an Episodes or int32, one per token")
         first, positions = None, positions.contiguous()
     q_weight, k_weight, frequencies = (None if x is None else x.contiguous() for x in (q_weight, k_weight, frequencies))
     size = 4 * q.element_size()
@@ -313,8 +331,7 @@ class _Attention(torch.autograd.Function):
         ctx.desc, ctx.episodes = desc, episodes
         return out
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         device, desc = q.device, ctx.desc
@@ -370,15 +387,18 @@ class HistoryCache:
     def advance(self, fresh=None):
         """The next token of every env; envs with `fresh` set (envs, bool or uint8) begin an episode and forget what they held."""
         if fresh is not None:
-            fresh = _flags(fresh, tuple(self.position.shape), self.device, "fresh")
+            fresh = _flags(fresh, self.position.shape, self.device, "fresh")
         _call(self.device, _abi.lib().nuka_b200_history_advance, self.position.data_ptr(), _ptr(fresh), self.position.numel())
 
-    def _workspace(self, desc):
-        found = self._workspaces.get(desc.heads_q)
+    def _workspace(self, heads):
+        """(address, bytes) of what a call with this many heads needs beside the cache, zeroed once."""
+        found = self._workspaces.get(heads)
         if found is None:
-            need = _abi.lib().nuka_b200_history_workspace(ctypes.byref(desc))
-            found = self._workspaces[desc.heads_q] = torch.zeros(need, dtype=torch.uint8, device=self.device)
-        return found
+            envs, capacity, heads_k, dim = self.keys.shape
+            need = _abi.lib().nuka_b200_history_workspace(ctypes.byref(_abi.HistoryDesc(_DTYPES[self.keys.dtype], envs, capacity, heads, heads_k, dim)))
+            kept = torch.zeros(need, dtype=torch.uint8, device=self.device)
+            found = self._workspaces[heads] = (kept.data_ptr() or None, need, kept)
+        return found[:2]
 
 
 def history_attention(q, k, v, cache, scale=None):
@@ -388,15 +408,16 @@ def history_attention(q, k, v, cache, scale=None):
     device = _on_gpu(q, k, v, cache.keys)
     envs, capacity, heads_k, dim = cache.keys.shape
     dtype = cache.keys.dtype
-    _expect(q.dim() == 3 and q.shape[0] == envs and q.shape[2] == dim and q.shape[1] > 0 and q.shape[1] % heads_k == 0, f"q must be {envs} x a multiple of {heads_k} x {dim}")
-    _expect(tuple(k.shape) == (envs, heads_k, dim) and v.shape == k.shape, f"k and v must be {envs} x {heads_k} x {dim}")
-    _expect(q.dtype == dtype and k.dtype == dtype and v.dtype == dtype, f"q, k and v must be {dtype}, as the cache is")
-    q, k, v = (_channels_last(x, 8, 16) for x in (q, k, v))
+    if q.dim() != 3 or q.shape[0] != envs or q.shape[2] != dim or q.shape[1] == 0 or q.shape[1] % heads_k:
+        raise ValueError(f"q must be {envs} x a multiple of {heads_k} x {dim}")
+    if k.shape != (envs, heads_k, dim) or v.shape != k.shape:
+        raise ValueError(f"k and v must be {envs} x {heads_k} x {dim}")
+    if q.dtype != dtype or k.dtype != dtype or v.dtype != dtype:
+        raise ValueError(f"q, k and v must be {dtype}, as the cache is")
+    q, k, v = _channels_last(q, 8, 16), _channels_last(k, 8, 16), _channels_last(v, 8, 16)
     out = torch.empty(q.shape, dtype=dtype, device=device)
     desc = _abi.HistoryDesc(_DTYPES[dtype], envs, capacity, q.shape[1], heads_k, dim, dim ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                             _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), cache.keys.data_ptr(), cache.values.data_ptr(),
-                            cache.position.data_ptr(), out.data_ptr())
-    workspace = cache._workspace(desc)
-    desc.workspace, desc.workspace_bytes = workspace.data_ptr() or None, workspace.numel()
+                            cache.position.data_ptr(), out.data_ptr(), *cache._workspace(q.shape[1]))
     _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
     return out

@@ -76,6 +76,12 @@ def _close(got, want, bound, what):
     assert worst <= 0, f"{what}: {worst:.3e} beyond its bound, off by up to {off.max().item():.3e}"
 
 
+def _bounds(w, unit, step):
+    """(value, bound) of the outputs and gradients of _reference."""
+    return {"o": (w["o"], unit * (w["o"].abs() + w["o_p"]) + SUMS * w["o_p"] + step * w["o_n"] + step), "dq": (w["dq"], unit * w["dq"].abs() + w["dq_s"] + step * w["dq_n"] + step),
+            "dk": (w["dk"], unit * w["dk"].abs() + w["dk_s"] + step * w["dk_n"] + step), "dv": (w["dv"], unit * (w["dv"].abs() + w["dv_p"]) + SUMS * w["dv_p"] + step * w["dv_n"] + step)}
+
+
 def _check(q, k, v, plan, do, window=None, scale=None):
     unit, step = UNIT[q.dtype], STEP[q.dtype]
     UNIT_OF[:] = [unit * 2.0 ** 7, unit]
@@ -83,10 +89,8 @@ def _check(q, k, v, plan, do, window=None, scale=None):
     o = S.episode_attention(q, k, v, plan, scale=scale, window=window)
     grads = torch.autograd.grad(o, [q, k, v], do)
     w = _reference(q, k, v, plan, q.shape[2] ** -0.5 if scale is None else scale, window, do)
-    _close(o.detach(), w["o"], unit * (w["o"].abs() + w["o_p"]) + SUMS * w["o_p"] + step * w["o_n"] + step, "o")
-    _close(grads[0], w["dq"], unit * w["dq"].abs() + w["dq_s"] + step * w["dq_n"] + step, "dq")
-    _close(grads[1], w["dk"], unit * w["dk"].abs() + w["dk_s"] + step * w["dk_n"] + step, "dk")
-    _close(grads[2], w["dv"], unit * (w["dv"].abs() + w["dv_p"]) + SUMS * w["dv_p"] + step * w["dv_n"] + step, "dv")
+    for (name, (want, bound)), got in zip(_bounds(w, unit, step).items(), [o.detach(), *grads]):
+        _close(got, want, bound, name)
 
 
 def _inputs(gen, n, heads_q, heads_k, dim, dtype, scale=1.2):
@@ -180,6 +184,31 @@ def test_keys_that_are_not_finite_stay_in_their_episode():
     other = torch.ones(plan.tokens, dtype=torch.bool, device="cuda")
     other[60:90] = False
     assert torch.equal(got[other], want[other]) and torch.isnan(got[60:90]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("what", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_what_is_not_finite_stays_in_its_episode(dim, what, value):
+    """One token of one episode: outputs and gradients of the others are what they are without it, within the bounds of all values (they share tiles, and are worked out row by row)."""
+    plan = _plan_of([30, 40, 200, 24, 90])
+    names = ("q", "k", "v", "do")
+    clean = dict(zip(names, (x.clone() for x in _inputs(_gen(30), plan.tokens, 4, 2, dim, torch.bfloat16))))
+    spoilt = {n: x.clone() for n, x in clean.items()}
+    spoilt[what][100, 0, 5] = value                        # in the third episode
+    UNIT_OF[:] = [UNIT[torch.bfloat16] * 2.0 ** 7, UNIT[torch.bfloat16]]
+    w = _reference(*(clean[n] for n in names[:3]), plan, dim ** -0.5, None, clean["do"])
+    q, k, v = (spoilt[n].requires_grad_() for n in names[:3])
+    o = S.episode_attention(q, k, v, plan)
+    outs = [o.detach(), *torch.autograd.grad(o, [q, k, v], spoilt["do"])]
+    other = torch.ones(plan.tokens, dtype=torch.bool, device="cuda")
+    other[70:270] = False
+    for (name, (want, bound)), got in zip(_bounds(w, UNIT[torch.bfloat16], 0.0).items(), outs):
+        _close(got[other], want[other], bound[other], name)
+    spoils = {"q": [0], "k": [0], "v": [0], "do": [1, 2, 3]}[what]
+    assert all(not torch.isfinite(outs[n][70:270]).all() for n in spoils)
+    # rows of the same episode from before the token do not see it
+    assert torch.isfinite(outs[0][70:100]).all()
 
 
 def test_same_bits_every_time_strides_and_streams():

@@ -35,6 +35,22 @@ __device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, vol
     }
 }
 
+// ---- clusters -------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+// all threads of all blocks; what was written to shared memory before is seen after
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.release.aligned; barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ float4 load_of_block(uint32_t address, uint32_t rank) {
+    float4 v;
+    uint32_t there;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(address), "r"(rank));
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+    return v;
+}
+
 // ---- TMA --------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void load_tile(void* to, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(shared_address(to)),

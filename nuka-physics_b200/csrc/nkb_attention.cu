@@ -10,9 +10,20 @@
 //
 // The backward pass works the scores out twice, once for the queries' gradients and once for the keys': 7 products in place of 5, and in return no gradient is summed
 // through atomics, so that the same call gives the same bits, and the shared heads' sum stays in tensor memory.
-// One warp loads tiles by TMA, one thread issues the products, four warps turn scores into probabilities, a row to a thread;
+// Warps have roles: one or two load tiles by TMA, one or two issue products, four for each tile turn scores into probabilities, a row to a thread;
 // P and dS go back to tensor memory as the next product's operand in the inputs' type (their one rounding more; sums and statistics are in 32 bits).
-// Two blocks share an SM, so that one's products run under the other's exponentials.
+// One tile's products run under the other's exponentials: forwards the two are one block's, backwards those of two blocks on an SM.
+// A block stays for several jobs, its loads and products a step ahead of its rows.
+//
+// Measured, bf16, causal (8 heads, 2 of keys):
+//                                                           forwards    queries     keys
+//   98304 tokens in rows of 24, dim 64                         80 us      111         99        252 MB of inputs and outputs forwards: 3.1 TB/s
+//   20011 tokens in 40 episodes, dim 64                        49          54         93
+//   16384 tokens, one episode, dim 128                        468          --         --        550 GFLOP of visible pairs: 1.17 PFLOP/s
+//   40000 tokens in 4 episodes, dim 128                       845        2130       3480        0.97, 0.58 and 0.47 PFLOP/s
+// Long episodes are bound by the chain of a step, scores to exponentials to product, that each tile walks through: the tensor cores are busy for half of it.
+// Short rows are bound by the same chain once a tile, with its loads and its rows' way out around it: 128 rows see 24 keys each, and a tile's product is
+// mostly mask, so there neither the bytes nor the products are near their limits.
 #include <cuda_runtime.h>
 #include <algorithm>
 #include "nkb_sequence.cuh"
@@ -31,7 +42,7 @@ struct AttentionParams {
     int64_t tokens, pitch;                              // pitch: floats between the heads' rows of lse and delta
     int heads_q, heads_k, dim, window;                  // window 0: all of the episode
     int span, tiles;                                    // tokens of a tile, at most 128, and how many tiles
-    int split;                                          // blocks of a key job: 1, or one for each head of the group, as a cluster
+    int split;                                          // blocks of a key job, a cluster, each with an equal share of the group's heads
     int by_heads, across, along;                        // of the forward kernel's jobs: tiles of two heads or of two stretches of tokens; jobs side by side, and behind one another
     float scale, scale2;                                // scale2: times log2(e)
     const void *q, *k, *v;
@@ -811,8 +822,10 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
 
 // ---- backwards: gradients of keys and values ----------------------------------------------------------------------------
 // The same with (tile of keys, key head) jobs: the queries of all heads of the group that see any of the keys pass by, 64 at a time, with their statistics.
-// Where jobs are too few to go round, the heads of a group are a cluster's blocks, one each, which add up their sums in 32 bits through each other's shared memory at the end, always in the
-// order of the heads (20011 tokens in 40 episodes, 4 heads to a key head: 120 us without, SPLITUS with).
+// Where jobs are few, a cluster's blocks share the heads of a group, and add up their sums in 32 bits through each other's shared memory at the end, always in the order of the heads.
+// That sum is worth about ten steps, so jobs are cut in two as long as that leaves one block for each place on the GPU, or, where rows are long, four.
+// 8 heads, 2 of keys, dim 64, uncut and cut in 2 and 4: 3000 tokens in 10 episodes 44, 31 and 22 us; 6000 in 30: 35, 30 and 34; 20011 in 40: 92, 96 and 107; 20000 in 100: 62, 74 and 86;
+// 6000 in 2: 270, 148 and 91; 12000 in 3: 360, 214 and 215.
 template <int DP> struct Keys {
     static constexpr int kStages = 2;
     static constexpr bool kApart = DP == 128;           // one block to an SM has columns to spare, two have not
@@ -869,7 +882,7 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
     fence_after();
     const uint32_t base = __shfl_sync(~0u, tensor, 0), k_at = shared_address(shared), v_at = k_at + F::kTile, part_at = v_at + F::kTile;
     const int rank = p.split > 1 ? (int)cluster_rank() : 0, job0 = blockIdx.x / p.split, stride = gridDim.x / p.split, jobs = p.tiles * p.heads_k;
-    const int group = p.heads_q / p.heads_k / p.split;     // heads of a block, from number `rank` on
+    const int group = p.heads_q / p.heads_k / p.split;     // heads of a block, from number rank * group on
 
     if (warp == 4) {
         if (lane == 0) {
@@ -887,7 +900,7 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
                 const int each = now.steps(p);
                 for (int h = 0; fine && h < group; ++h)
                     for (int m = 0; m < each; ++m, ++steps) {
-                        const int s = steps % F::kStages, turn = steps / F::kStages, head = now.head * (p.heads_q / p.heads_k) + rank + h, i = now.begin() + m * kStream;
+                        const int s = steps % F::kStages, turn = steps / F::kStages, head = now.head * (p.heads_q / p.heads_k) + rank * group + h, i = now.begin() + m * kStream;
                         if (turn > 0 && !(fine = barrier_wait(&empty[s], (turn - 1) & 1, &lost))) break;
                         barrier_expect(&full[s], 2 * F::kPart + 2 * kStream * 4);
                         unsigned char* to = shared + 2 * F::kTile + 2 * s * F::kPart;
@@ -1172,7 +1185,9 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
             return cudaErrorInvalidValue;
         // few jobs, that is long ones, are better dealt out by the hardware as blocks end
         const int jobs = p.tiles * (keys ? p.heads_k : p.heads_q), slots = keys && DP != 64 ? 148 : 2 * 148, blocks = jobs <= 4 * slots ? jobs : slots, group = p.heads_q / p.heads_k;
-        p.split = keys && jobs <= 4 * slots && (group == 2 || group == 4 || group == 8) ? group : 1;
+        const int64_t row = e.tokens / std::max<int64_t>(e.rows, 1), reach = d.window > 0 ? std::min<int64_t>(row, d.window) : row, places = reach >= 1024 ? 4 * slots : slots;
+        p.split = 1;
+        while (keys && p.split < 8 && group % (2 * p.split) == 0 && 2 * p.split * (int64_t)jobs <= places) p.split *= 2;
         if (!keys) {
             query_grad_kernel<T, DP><<<(unsigned)blocks, kBlock, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         } else if (p.split == 1) {

@@ -83,7 +83,7 @@ cudaError_t launch_episodes_from_done(const nuka_b200_episodes_t& p, const uint8
 // warps are the segments: each begins with a row, and that is all.  Otherwise the tokens are cut into as many equal segments as fill the GPU and walked twice: first for
 // each segment's map alone, then, when a small scan over the maps has said what state each begins with, for the values.  The inputs are read twice that way (5 tensors' bytes in place
 // of 3 forwards, 8 in place of 6 backwards); chunks that wait for one another's maps read them once, and were slower by more: their waits, a few microseconds for every chunk of 64 tokens, had
-// nothing to hide under (131071 x 1024, bf16: 1.42 ms forwards, against FWD here).  All orders are fixed, so the same call gives the same bits.
+// nothing to hide under (131071 x 1024, bf16: 1.42 ms forwards, against 0.32 here).  All orders are fixed, so the same call gives the same bits.
 
 // Channels of a lane; tokens whose loads are under way.
 template <typename T> constexpr int kWide = sizeof(T) == 4 ? 2 : 4;

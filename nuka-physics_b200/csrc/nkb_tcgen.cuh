@@ -23,13 +23,13 @@ __device__ __forceinline__ bool barrier_try(uint64_t* bar, uint32_t parity) {
     return done != 0u;
 }
 // A wait gives up after about 2 s, or when another warp of the block gave up: the block then ends its work, and its outputs become NaN.
+// The clock is read at each turn: sixteen tries between two readings go on a little later (queries' gradients of 98304 x 8 x 64 in rows of 24: 121 us, against 111 so).
 constexpr long long kBarrierCycles = 4000000000ll;
 __device__ __forceinline__ bool barrier_wait(uint64_t* bar, uint32_t parity, volatile int* lost) {
     if (barrier_try(bar, parity)) return true;
     const long long began = clock64();
     for (;;) {
-        for (int k = 0; k < 16; ++k)
-            if (barrier_try(bar, parity)) return true;
+        if (barrier_try(bar, parity)) return true;
         if (*lost != 0) return false;
         if (clock64() - began > kBarrierCycles) { *lost = 1; return false; }
     }
@@ -69,7 +69,6 @@ __device__ __forceinline__ void wait_stores_read() { asm volatile("cp.async.bulk
 __device__ __forceinline__ void wait_stores_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }              // ordinary stores before, TMA after
 __device__ __forceinline__ void meet(int which, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(which), "r"(threads) : "memory"); }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- tensor memory ------------------------------------------------------------------------------------------------------
 template <int COLUMNS> __device__ __forceinline__ void tensor_alloc(uint32_t* to) {
@@ -124,7 +123,7 @@ template <typename T> __host__ __device__ constexpr uint32_t product_of(int n, b
     return 1u << 4 | (sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? (1u << 7 | 1u << 10) : 0u) | (b_outer ? 1u << 16 : 0u) | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
 }
 // The whole warp calls these, and one lane of it issues: inside a branch of one lane the compiler cannot keep the operands in uniform registers, and moving them there takes
-// longer than the product (75 cycles an instruction in place of MMAC).
+// longer than the product (75 cycles an instruction in place of 30).
 __device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t what, bool add) {
     asm volatile("{ .reg .pred e, p; elect.sync _|e, 0xffffffff; setp.ne.u32 p, %4, 0; @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(what),
                  "r"((uint32_t)add) : "memory");
@@ -171,22 +170,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
-}
-// 2^x of two values by multiplications and additions, for x up to 127: the integer part goes into the exponent, 2^f of the rest, between -1/2 and 1/2, is the
-// polynomial of degree 4 with the least largest relative error there (2.6e-6; a linear programme over 2001 points). Below -126 it is 2^-126.
-__device__ __forceinline__ void exp2_pair(Pair x, float& a, float& b) {
-    split(x, a, b);
-    const Pair y = pair_of(fmaxf(a, -126.f), fmaxf(b, -126.f)), magic = pair_of(12582912.f, 12582912.f), minus = pair_of(-12582912.f, -12582912.f);
-    const Pair whole = add_pair(y, magic), back = add_pair(whole, minus), one = pair_of(-1.f, -1.f), f = fma_pair(back, one, y);
-    Pair r = fma_pair(pair_of(0.009570085443556309f, 0.009570085443556309f), f, pair_of(0.0559178926050663f, 0.0559178926050663f));
-    r = fma_pair(r, f, pair_of(0.2402474582195282f, 0.2402474582195282f));
-    r = fma_pair(r, f, pair_of(0.6931217908859253f, 0.6931217908859253f));
-    r = fma_pair(r, f, pair_of(0.9999992847442627f, 0.9999992847442627f));
-    float u, v, m, n;
-    split(r, u, v);
-    split(whole, m, n);
-    a = __int_as_float(__float_as_int(u) + (__float_as_int(m) << 23));
-    b = __int_as_float(__float_as_int(v) + (__float_as_int(n) << 23));
 }
 template <typename T> __device__ __forceinline__ uint32_t pack(float low, float high);
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float low, float high) {

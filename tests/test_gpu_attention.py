@@ -151,6 +151,16 @@ def test_more_jobs_than_blocks():
     _check(q, k, v, plan, do, window=300)
 
 
+@pytest.mark.parametrize("heads_q,heads_k", [(6, 1), (12, 1), (16, 2)])
+@pytest.mark.parametrize("lengths", [[300, 20], [1100]])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_heads_shared_by_blocks(heads_q, heads_k, lengths, dim):
+    """Few jobs: several blocks have some heads of a key head's group each, and add up."""
+    plan = _plan_of(lengths)
+    q, k, v, do = _inputs(_gen(dim + heads_q), plan.tokens, heads_q, heads_k, dim, torch.bfloat16)
+    _check(q, k, v, plan, do)
+
+
 @pytest.mark.parametrize("size,scale", [(8.0, None), (1.0, 1.0), (1.0, 1e-3)])
 @pytest.mark.parametrize("dim", [64, 128])
 def test_sharp_and_flat_softmax(size, scale, dim):

@@ -559,20 +559,21 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
 // ---- backwards: gradients of the queries -------------------------------------------------------------------------------
 // Two blocks to an SM, each of which takes (tile of queries, head) jobs in turn; loads and products run ahead as forwards, and rows leave under the next job's first exponentials.
 template <int DP> struct Queries {
-    static constexpr bool kApart = DP == 64;            // dS has columns of its own: the next scores are multiplied while the present ones are worked on
-    static constexpr int kStages = DP == 64 ? 2 : 1;
+    // one block to an SM has columns for two steps' scores, the next ones multiplied while the present ones are worked on; where two share the SM, the other block's work goes on meanwhile
+    static constexpr int kBlocks = DP == 64 ? 2 : 1, kBuffers = DP == 64 ? 1 : 2, kColumns = 512 / kBlocks;
+    static constexpr int kStages = DP == 64 ? 2 : 3;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
-    // queries, dO and, for D = dO . O, O; steps of keys and values; the rows that leave.  Wide heads have room for queries and dO only.
-    static constexpr int kTiles = kApart ? 3 : 2, kKeys = kTiles * kTile, kStaged = kKeys + 2 * kStages * kPart, kShared = kStaged + (kApart ? kTile : 0) + 1024;
-    static constexpr int kGrad = kStream, kOut = 2 * kStream, kProb = kApart ? 2 * kStream + DP : 0;
+    // queries, dO and, for D = dO . O, O; steps of keys and values; the rows that leave
+    static constexpr int kKeys = 3 * kTile, kStaged = kKeys + 2 * kStages * kPart, kShared = kStaged + kTile + 1024;
+    static constexpr int kGrad = kStream, kScores = 2 * kStream, kOut = kBuffers * kScores, kProb = kOut + DP;
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
+__global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
                                                                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq,
                                                                const AttentionParams p) {
     using F = Queries<DP>;
-    __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full, s_empty, p_full, o_done, ended;
+    __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], s_empty[F::kBuffers], p_full, o_done, ended;
     __shared__ uint32_t tensor;
     __shared__ int lost;
     unsigned char* const shared = aligned_shared();
@@ -580,17 +581,16 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
     if (threadIdx.x == 0) {
         lost = 0;
         barrier_init(&q_full, 1);
-        barrier_init(&q_empty, F::kApart ? 1 + kRows : 1);      // the scores' products, and the rows' reads of dO and O
+        barrier_init(&q_empty, 1 + kRows);      // the scores' products, and the rows' reads of dO and O
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
-        barrier_init(&s_full, 1);
-        barrier_init(&s_empty, kRows);
+        for (int s = 0; s < F::kBuffers; ++s) { barrier_init(&s_full[s], 1); barrier_init(&s_empty[s], kRows); }
         barrier_init(&p_full, kRows);
         barrier_init(&o_done, 1);
         barrier_init(&ended, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncwarp();
-    if (warp == 5) tensor_alloc<256>(&tensor);
+    if (warp == 5) tensor_alloc<F::kColumns>(&tensor);
     fence_before();
     __syncthreads();
     fence_after();
@@ -606,10 +606,10 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                 const QueryJob now = next;
                 if (job + stride < jobs) next = QueryJob(p, job + stride);
                 if (queries > 0 && !(fine = barrier_wait(&q_empty, (queries - 1) & 1, &lost))) break;
-                barrier_expect(&q_full, F::kTiles * F::kTile);
+                barrier_expect(&q_full, 3 * F::kTile);
                 load_panels<kRows, DP>(shared, &map_q, &q_full, now.head, now.i0);
                 load_panels<kRows, DP>(shared + F::kTile, &map_do, &q_full, now.head, now.i0);
-                if (F::kApart) load_panels<kRows, DP>(shared + 2 * F::kTile, &map_o, &q_full, now.head, now.i0);
+                load_panels<kRows, DP>(shared + 2 * F::kTile, &map_o, &q_full, now.head, now.i0);
                 ++queries;
                 const int j0 = now.begin(p), count = now.steps(p), key_head = now.head / group;
                 for (int j = 0; j < count; ++j, ++steps) {
@@ -634,11 +634,12 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                 if (!warp_wait(&q_full, queries & 1, &lost)) return false;
             }
             if (!warp_wait(&full[stage], phase, &lost)) return false;
-            if (ahead > 0 && !warp_wait(F::kApart ? &s_empty : &o_done, (ahead - 1) & 1, &lost)) return false;
+            const int b = ahead % F::kBuffers;
+            if (ahead >= F::kBuffers && !warp_wait(&s_empty[b], (ahead / F::kBuffers - 1) & 1, &lost)) return false;
             fence_after();
-            multiply_rows<T, kStream, DP>(base, q_at, kv_at + 2 * stage * F::kPart);
-            multiply_rows<T, kStream, DP>(base + F::kGrad, do_at, kv_at + (2 * stage + 1) * F::kPart);
-            commit(&s_full);
+            multiply_rows<T, kStream, DP>(base + b * F::kScores, q_at, kv_at + 2 * stage * F::kPart);
+            multiply_rows<T, kStream, DP>(base + b * F::kScores + F::kGrad, do_at, kv_at + (2 * stage + 1) * F::kPart);
+            commit(&s_full[b]);
             ++ahead;
             if (++stage == F::kStages) { stage = 0; phase ^= 1; }
             if (++j == count) { commit(&q_empty); j = 0; ++queries; job += stride; }
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
         for (int own = blockIdx.x; fine && own < jobs; own += stride) {
             const int steps = count;                    // of the job that the scores have just begun
             for (int i = 0; i < steps; ++i, ++n) {
-                if (F::kApart && F::kStages > 1 && i + 1 < steps && !(fine = scores())) break;
+                if (i + 1 < steps && !(fine = scores())) break;
                 if (!(fine = warp_wait(&p_full, n & 1, &lost))) break;
                 fence_after();
                 multiply_columns<T, kStream, DP>(base + F::kOut, base + F::kProb, kv_at + 2 * own_stage * F::kPart, i != 0);
@@ -657,7 +658,7 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                 commit(&o_done);
                 if (++own_stage == F::kStages) own_stage = 0;
                 // over a job's end only now: the next one's queries may still be on their way
-                if ((!F::kApart || i + 1 == steps) && job < jobs && !(fine = scores())) break;
+                if (i + 1 == steps && job < jobs && !(fine = scores())) break;
             }
         }
         commit(&ended);
@@ -672,27 +673,20 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
             const int i = leaving.first + row;
             const bool there = i <= leaving.last;
             float values[DP];
-            if (F::kApart) {
-                unsigned char* const tile = shared + F::kStaged;
-                if (row == 0) wait_stores_read();
-                meet(1, kRows);
-                const bool finite = stage_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), tile, row);
-                if (fine && !finite && there) {
-                    slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
-                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
-                }
-                fence_shared();
-                meet(1, kRows);
-                if (row == 0 && leaving.first <= leaving.last) {
-                    store_tile(&map_dq, tile, 0, leaving.head, leaving.first);
-                    stores_end();
-                }
-            } else {
-                T* const to = static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + leaving.head) * p.dim;
-                if (!store_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), p.dim, there ? to : nullptr) && fine) {
-                    slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
-                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(to + c) = pack_row<T>(values + c);
-                }
+            unsigned char* const tile = shared + F::kStaged;
+            if (row == 0) wait_stores_read();
+            meet(1, kRows);
+            const bool finite = stage_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), tile, row);
+            if (fine && !finite && there) {
+                slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
+                for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
+            }
+            fence_shared();
+            meet(1, kRows);
+            if (row == 0 && leaving.first <= leaving.last) {
+                for (int c = 0; c < DP; c += 64)
+                    if (c < p.dim) store_tile(&map_dq, tile + c / 64 * kRows * 128, c, leaving.head, leaving.first);
+                stores_end();
             }
         };
         QueryJob next(p, blockIdx.x);
@@ -713,36 +707,25 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
             // after this one, gets D without it. Where a step holds all keys of a row D is summed from its own P and dP before dS, which matters where few keys share a row (dq of
             // 24-token episodes was off by 1.8 times its rounding; with many keys the error averages out).
             float delta = 0.f;
-            if (F::kApart) {
-                fine = fine && warp_wait(&q_full, queries & 1, &lost);
-                if (fine)
+            fine = fine && warp_wait(&q_full, queries & 1, &lost);
+            if (fine)
 #pragma unroll
-                    for (int c = 0; c < DP / 8; ++c) {
-                        float u[8], v[8];
-                        unpack<T, 8>(*reinterpret_cast<const uint4*>(staged(shared + F::kTile, row, c)), u);
-                        unpack<T, 8>(*reinterpret_cast<const uint4*>(staged(shared + 2 * F::kTile, row, c)), v);
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
-                    }
-                barrier_arrive(&q_empty);
-            } else if (live) {
-                const int64_t at = ((int64_t)i * p.heads_q + now.head) * p.dim;
-                const uint4 *o = reinterpret_cast<const uint4*>(static_cast<const T*>(p.out) + at), *g = reinterpret_cast<const uint4*>(static_cast<const T*>(p.dout) + at);
-#pragma unroll 4
-                for (int c = 0; c < p.dim / 8; ++c) {
+                for (int c = 0; c < DP / 8; ++c) {
                     float u[8], v[8];
-                    unpack<T, 8>(o[c], u);
-                    unpack<T, 8>(g[c], v);
+                    unpack<T, 8>(*reinterpret_cast<const uint4*>(staged(shared + F::kTile, row, c)), u);
+                    unpack<T, 8>(*reinterpret_cast<const uint4*>(staged(shared + 2 * F::kTile, row, c)), v);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) delta = fmaf(u[k], v[k], delta);
                 }
-            }
+            barrier_arrive(&q_empty);
             const Pair scale2 = pair_of(p.scale2, p.scale2), shift = pair_of(-lse, -lse);
             Pair off = pair_of(0.f, 0.f);
             bool left = false;
             for (int j = 0; j < count; ++j, ++n) {
                 const int k0 = j0 + j * kStream;
-                fine = fine && warp_wait(&s_full, n & 1, &lost);
+                const int b = n % F::kBuffers;
+                const uint32_t here = mine + b * F::kScores;
+                fine = fine && warp_wait(&s_full[b], n / F::kBuffers & 1, &lost);
                 if (!fine) break;
                 fence_after();
                 uint32_t packed[kStream / 2];
@@ -751,8 +734,8 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                 // P and P (dP - D) of 32 keys
                 auto part = [&](int c0, Pair minus, auto use) {
                     uint32_t r[32], d[32];
-                    tensor_load(mine + c0, r);
-                    tensor_load(mine + F::kGrad + c0, d);
+                    tensor_load(here + c0, r);
+                    tensor_load(here + F::kGrad + c0, d);
                     wait_loads();
                     const uint32_t seen = all ? ~0u : columns_between(low - k0 - c0, high - k0 - c0);
 #pragma unroll
@@ -791,7 +774,7 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
                     }
                 }
                 fence_before();
-                barrier_arrive(&s_empty);
+                barrier_arrive(&s_empty[b]);
                 if (n > 0) fine = warp_wait(&o_done, (n - 1) & 1, &lost);
                 if (!fine) break;
                 if (n > 0) fence_after();
@@ -817,7 +800,7 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
     fence_before();
     __syncthreads();
     fence_after();
-    if (warp == 5) tensor_free<256>(tensor);
+    if (warp == 5) tensor_free<F::kColumns>(tensor);
 }
 
 // ---- backwards: gradients of keys and values ----------------------------------------------------------------------------
@@ -827,13 +810,12 @@ __global__ void __launch_bounds__(kBlock, 2) query_grad_kernel(const __grid_cons
 // 8 heads, 2 of keys, dim 64, uncut and cut in 2 and 4: 3000 tokens in 10 episodes 44, 31 and 22 us; 6000 in 30: 35, 30 and 34; 20011 in 40: 92, 96 and 107; 20000 in 100: 62, 74 and 86;
 // 6000 in 2: 270, 148 and 91; 12000 in 3: 360, 214 and 215.
 template <int DP> struct Keys {
-    static constexpr int kStages = 2;
-    static constexpr bool kApart = DP == 128;           // one block to an SM has columns to spare, two have not
-    static constexpr int kColumns = DP == 64 ? 256 : 512;
+    // one block to an SM has columns for two steps' scores; P and dS take their scores' place
+    static constexpr int kBlocks = DP == 64 ? 2 : 1, kBuffers = DP == 64 ? 1 : 2, kColumns = 512 / kBlocks;
+    static constexpr int kStages = DP == 64 ? 2 : 4;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
     static constexpr int kStaged = 2 * kTile + 2 * kStages * kPart, kShared = kStaged + (DP == 64 ? 2 * kTile : 0) + 1024;         // rows of wide heads leave without a staged tile
-    static constexpr int kGrad = kStream, kValue = 2 * kStream, kKey = 2 * kStream + DP;
-    static constexpr int kProb = kApart ? 2 * kStream + 2 * DP : 0, kProbGrad = kApart ? kProb + kStream / 2 : kGrad;
+    static constexpr int kGrad = kStream, kScores = 2 * kStream, kValue = kBuffers * kScores, kKey = kValue + DP;
 };
 
 // A tile of keys and a key head; the longest of one long row are the first ones.
@@ -854,11 +836,11 @@ struct KeyJob {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                                                                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
                                                                             const __grid_constant__ CUtensorMap map_dv, const AttentionParams p) {
     using F = Keys<DP>;
-    __shared__ uint64_t k_full, k_empty, full[F::kStages], empty[F::kStages], s_full, p_full, o_done, ended;
+    __shared__ uint64_t k_full, k_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], p_full, o_done, ended;
     __shared__ __align__(16) float lse[F::kStages][kStream], delta[F::kStages][kStream];
     __shared__ uint32_t tensor;
     __shared__ int lost;
@@ -869,7 +851,7 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
         barrier_init(&k_full, 1);
         barrier_init(&k_empty, 1);
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
-        barrier_init(&s_full, 1);
+        for (int s = 0; s < F::kBuffers; ++s) barrier_init(&s_full[s], 1);
         barrier_init(&p_full, kRows);
         barrier_init(&o_done, 1);
         barrier_init(&ended, 1);
@@ -923,12 +905,12 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
                 if (!warp_wait(&k_full, keys & 1, &lost)) return false;
             }
             if (!warp_wait(&full[stage], phase, &lost)) return false;
-            // apart, the scores' columns are free when P and dS are written; else when their products have ended
-            if (!F::kApart && ahead > 0 && !warp_wait(&o_done, (ahead - 1) & 1, &lost)) return false;
+            const int b = ahead % F::kBuffers;
+            if (F::kBuffers == 1 && ahead > 0 && !warp_wait(&o_done, (ahead - 1) & 1, &lost)) return false;     // P and dS, which lie there, are free then
             fence_after();
-            multiply_rows<T, kStream, DP>(base, k_at, part_at + 2 * stage * F::kPart);
-            multiply_rows<T, kStream, DP>(base + F::kGrad, v_at, part_at + (2 * stage + 1) * F::kPart);
-            commit(&s_full);
+            multiply_rows<T, kStream, DP>(base + b * F::kScores, k_at, part_at + 2 * stage * F::kPart);
+            multiply_rows<T, kStream, DP>(base + b * F::kScores + F::kGrad, v_at, part_at + (2 * stage + 1) * F::kPart);
+            commit(&s_full[b]);
             ++ahead;
             if (++stage == F::kStages) { stage = 0; phase ^= 1; }
             if (++j == count) { commit(&k_empty); j = 0; ++keys; job += stride; }
@@ -939,15 +921,18 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
         for (int own = job0; fine && own < jobs; own += stride) {
             const int steps = count;                    // of the job that the scores have just begun
             for (int i = 0; i < steps; ++i, ++n) {
+                // the other buffer's P and dS are free when the products before have ended
+                if (F::kBuffers > 1 && n > 0 && !(fine = warp_wait(&o_done, (n - 1) & 1, &lost))) break;
+                if (F::kBuffers > 1 && i + 1 < steps && !(fine = scores())) break;
                 if (!(fine = warp_wait(&p_full, n & 1, &lost))) break;
                 fence_after();
-                if (F::kApart && i + 1 < steps && !(fine = scores())) break;
-                multiply_columns<T, kStream, DP>(base + F::kValue, base + F::kProb, part_at + (2 * own_stage + 1) * F::kPart, i != 0);
-                multiply_columns<T, kStream, DP>(base + F::kKey, base + F::kProbGrad, part_at + 2 * own_stage * F::kPart, i != 0);
+                const uint32_t probs = base + n % F::kBuffers * F::kScores;
+                multiply_columns<T, kStream, DP>(base + F::kValue, probs, part_at + (2 * own_stage + 1) * F::kPart, i != 0);
+                multiply_columns<T, kStream, DP>(base + F::kKey, probs + F::kGrad, part_at + 2 * own_stage * F::kPart, i != 0);
                 commit(&empty[own_stage]);
                 commit(&o_done);
                 if (++own_stage == F::kStages) own_stage = 0;
-                if ((!F::kApart || i + 1 == steps) && job < jobs && !(fine = scores())) break;
+                if ((F::kBuffers == 1 || i + 1 == steps) && job < jobs && !(fine = scores())) break;
             }
         }
         commit(&ended);
@@ -1023,7 +1008,9 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
                 for (int m = 0; m < each; ++m, ++n) {
                     const int i = now.begin() + m * kStream;
                     // the statistics came with the tile that the scores waited for; this wait makes them visible here, too
-                    fine = fine && warp_wait(&full[stage], phase, &lost) && warp_wait(&s_full, n & 1, &lost);
+                    const int b = n % F::kBuffers;
+                    const uint32_t here = mine + b * F::kScores;
+                    fine = fine && warp_wait(&full[stage], phase, &lost) && warp_wait(&s_full[b], n / F::kBuffers & 1, &lost);
                     if (!fine) break;
                     fence_after();
                     uint32_t probs[kStream / 2], grads[kStream / 2];
@@ -1032,8 +1019,8 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
 #pragma unroll
                     for (int c0 = 0; c0 < kStream; c0 += 32) {
                         uint32_t r[32], d[32];
-                        tensor_load(mine + c0, r);
-                        tensor_load(mine + F::kGrad + c0, d);
+                        tensor_load(here + c0, r);
+                        tensor_load(here + F::kGrad + c0, d);
                         wait_loads();
                         if (i + c0 > any_high || i + c0 + 31 < any_low) {
 #pragma unroll
@@ -1063,13 +1050,14 @@ __global__ void __launch_bounds__(kBlock, DP == 64 ? 2 : 1) key_grad_kernel(cons
                             }
                         }
                     }
-                    if (n > 0 && (F::kApart || first)) fine = warp_wait(&o_done, (n - 1) & 1, &lost);
+                    // each one in turn where there are two buffers, whose scores say nothing of the products before: a wait tells a phase from the one before it only
+                    if (n > 0 && (F::kBuffers > 1 || first)) fine = warp_wait(&o_done, (n - 1) & 1, &lost);
                     if (!fine) break;
-                    if (n > 0) fence_after();
+                    if (n > 0 && first) fence_after();
                     if (first && n > 0) { leave(); left = true; }
                     first = false;
-                    tensor_store(mine + F::kProb, probs);
-                    tensor_store(mine + F::kProbGrad, grads);
+                    tensor_store(here, probs);
+                    tensor_store(here + F::kGrad, grads);
                     wait_stores();
                     fence_before();
                     barrier_arrive(&p_full);
@@ -1184,7 +1172,7 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
             !map_of(&dk, d.dtype, d.dk, d.dim, d.heads_k, e.tokens, d.dim, narrow, p.span) || !map_of(&dv, d.dtype, d.dv, d.dim, d.heads_k, e.tokens, d.dim, narrow, p.span))
             return cudaErrorInvalidValue;
         // few jobs, that is long ones, are better dealt out by the hardware as blocks end
-        const int jobs = p.tiles * (keys ? p.heads_k : p.heads_q), slots = keys && DP != 64 ? 148 : 2 * 148, blocks = jobs <= 4 * slots ? jobs : slots, group = p.heads_q / p.heads_k;
+        const int jobs = p.tiles * (keys ? p.heads_k : p.heads_q), slots = 148 * (keys ? Keys<DP>::kBlocks : Queries<DP>::kBlocks), blocks = jobs <= 4 * slots ? jobs : slots, group = p.heads_q / p.heads_k;
         const int64_t row = e.tokens / std::max<int64_t>(e.rows, 1), reach = d.window > 0 ? std::min<int64_t>(row, d.window) : row, places = reach >= 1024 ? 4 * slots : slots;
         p.split = 1;
         while (keys && p.split < 8 && group % (2 * p.split) == 0 && 2 * p.split * (int64_t)jobs <= places) p.split *= 2;

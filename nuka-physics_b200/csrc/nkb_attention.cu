@@ -12,7 +12,8 @@
 // through atomics, so that the same call gives the same bits, and the shared heads' sum stays in tensor memory.
 // Warps have roles: one or two load tiles by TMA, one or two issue products, four for each tile turn scores into probabilities, a row to a thread;
 // P and dS go back to tensor memory as the next product's operand in the inputs' type (their one rounding more; sums and statistics are in 32 bits).
-// One tile's products run under the other's exponentials: forwards the two are one block's, backwards those of two blocks on an SM.
+// One tile's products run under the other's exponentials: forwards the two are one block's, backwards those of two blocks on an SM, and with wide heads, of which one block fills an SM,
+// the next step's scores run under the present one's exponentials.
 // A block stays for several jobs, its loads and products a step ahead of its rows.
 //
 // Measured, bf16, causal (8 heads, 2 of keys):
@@ -20,7 +21,7 @@
 //   98304 tokens in rows of 24, dim 64                         80 us      111         99        252 MB of inputs and outputs forwards: 3.1 TB/s
 //   20011 tokens in 40 episodes, dim 64                        49          54         93
 //   16384 tokens, one episode, dim 128                        468          --         --        550 GFLOP of visible pairs: 1.17 PFLOP/s
-//   40000 tokens in 4 episodes, dim 128                       845        2130       3480        0.97, 0.58 and 0.47 PFLOP/s
+//   40000 tokens in 4 episodes, dim 128                       825        1220       2344        0.99, 1.01 and 0.70 PFLOP/s of visible pairs
 // Long episodes are bound by the chain of a step, scores to exponentials to product, that each tile walks through: the tensor cores are busy for half of it.
 // Short rows are bound by the same chain once a tile, with its loads and its rows' way out around it: 128 rows see 24 keys each, and a tile's product is
 // mostly mask, so there neither the bytes nor the products are near their limits.
@@ -104,10 +105,10 @@ template <typename T, int N, int DP> __device__ __forceinline__ void multiply_ro
     for (int k = 0; k < DP; k += 16)
         multiply(d, inner_rows(a + k / 64 * kRows * 128 + k % 64 * 2), inner_rows(b + k / 64 * N * 128 + k % 64 * 2), product_of<T>(N, false), k != 0);
 }
-// d (+)= A B over N rows of B, A in tensor memory
-template <typename T, int N, int DP> __device__ __forceinline__ void multiply_columns(uint32_t d, uint32_t a, uint32_t b, bool add) {
+// d (+)= A B over N rows of B, A in tensor memory, `EACH` of its columns in a row, two values to a column, and those of the next ones twice as far
+template <typename T, int N, int DP, int EACH = N> __device__ __forceinline__ void multiply_columns(uint32_t d, uint32_t a, uint32_t b, bool add) {
 #pragma unroll
-    for (int k = 0; k < N; k += 16) multiply_tensor(d, a + k / 2, outer_rows(b + k * 128, N * 128), product_of<T>(DP, true), add || k != 0);
+    for (int k = 0; k < N; k += 16) multiply_tensor(d, a + k / EACH * EACH + k % EACH / 2, outer_rows(b + k * 128, N * 128), product_of<T>(DP, true), add || k != 0);
 }
 
 // All lanes of a warp wait, and go on together.
@@ -557,11 +558,13 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
 }
 
 // ---- backwards: gradients of the queries -------------------------------------------------------------------------------
-// Two blocks to an SM, each of which takes (tile of queries, head) jobs in turn; loads and products run ahead as forwards, and rows leave under the next job's first exponentials.
+// Two blocks to an SM, or one of wide heads, each of which takes (tile of queries, head) jobs in turn; loads and products run ahead as forwards, and rows leave under the next job's first exponentials.
 template <int DP> struct Queries {
     // one block to an SM has columns for two steps' scores, the next ones multiplied while the present ones are worked on; where two share the SM, the other block's work goes on meanwhile
     static constexpr int kBlocks = DP == 64 ? 2 : 1, kBuffers = DP == 64 ? 1 : 2, kColumns = 512 / kBlocks;
     static constexpr int kStages = DP == 64 ? 2 : 3;
+    // threads of a row, with one block to an SM two, each with half of a step's columns (40000 tokens in 4 episodes, 8 heads, 2 of keys: 1309 us with one, 1220 so; keys' 2751 and 2344)
+    static constexpr int kHalves = DP == 64 ? 1 : 2, kWorkers = kHalves * kRows, kThreads = kBlock + kWorkers - kRows, kPer = kStream / kHalves;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
     // queries, dO and, for D = dO . O, O; steps of keys and values; the rows that leave
     static constexpr int kKeys = 3 * kTile, kStaged = kKeys + 2 * kStages * kPart, kShared = kStaged + kTile + 1024;
@@ -569,22 +572,23 @@ template <int DP> struct Queries {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
+__global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
                                                                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq,
                                                                const AttentionParams p) {
     using F = Queries<DP>;
     __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], s_empty[F::kBuffers], p_full, o_done, ended;
     __shared__ uint32_t tensor;
     __shared__ int lost;
+    __shared__ float offs[F::kHalves][kRows];
     unsigned char* const shared = aligned_shared();
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
         lost = 0;
         barrier_init(&q_full, 1);
-        barrier_init(&q_empty, 1 + kRows);      // the scores' products, and the rows' reads of dO and O
+        barrier_init(&q_empty, 1 + F::kWorkers);      // the scores' products, and the rows' reads of dO and O
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
-        for (int s = 0; s < F::kBuffers; ++s) { barrier_init(&s_full[s], 1); barrier_init(&s_empty[s], kRows); }
-        barrier_init(&p_full, kRows);
+        for (int s = 0; s < F::kBuffers; ++s) { barrier_init(&s_full[s], 1); barrier_init(&s_empty[s], F::kWorkers); }
+        barrier_init(&p_full, F::kWorkers);
         barrier_init(&o_done, 1);
         barrier_init(&ended, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -664,8 +668,9 @@ __global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kerne
         commit(&ended);
         drain(&ended, 0);
     } else {
-        const int row = threadIdx.x;
-        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
+        // a warp reaches the tensor memory's lanes 32 (warp % 4) and on
+        const int row = warp % 4 * 32 + lane, half = warp / 4 == 0 ? 0 : 1;
+        const uint32_t mine = base + ((uint32_t)(warp % 4 * 32) << 16);
         bool fine = true;
         int n = 0, queries = 0;
         struct Leaving { int first, last, head; float lse, delta; } leaving{0, -1, 0, 0.f, 0.f};
@@ -674,16 +679,16 @@ __global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kerne
             const bool there = i <= leaving.last;
             float values[DP];
             unsigned char* const tile = shared + F::kStaged;
-            if (row == 0) wait_stores_read();
-            meet(1, kRows);
-            const bool finite = stage_row<T, DP>(mine + F::kOut, fine ? p.scale : nan_value(), tile, row);
+            if (threadIdx.x == 0) wait_stores_read();
+            meet(1, F::kWorkers);
+            const bool finite = stage_row<T, DP / F::kHalves>(mine + F::kOut + half * (DP / 2), fine ? p.scale : nan_value(), tile + half * kRows * 128, row);
             if (fine && !finite && there) {
                 slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
-                for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
+                for (int c = half * (DP / 2); c < p.dim && c < (half + 1) * DP / F::kHalves; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
             }
             fence_shared();
-            meet(1, kRows);
-            if (row == 0 && leaving.first <= leaving.last) {
+            meet(1, F::kWorkers);
+            if (threadIdx.x == 0 && leaving.first <= leaving.last) {
                 for (int c = 0; c < DP; c += 64)
                     if (c < p.dim) store_tile(&map_dq, tile + c / 64 * kRows * 128, c, leaving.head, leaving.first);
                 stores_end();
@@ -728,7 +733,7 @@ __global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kerne
                 fine = fine && warp_wait(&s_full[b], n / F::kBuffers & 1, &lost);
                 if (!fine) break;
                 fence_after();
-                uint32_t packed[kStream / 2];
+                uint32_t packed[F::kPer / 2];
                 const bool all = k0 >= all_low && k0 + kStream - 1 <= all_high;
                 auto hidden = [&](int c0) { return k0 + c0 > any_high || k0 + c0 + 31 < any_low; };          // from all of the warp's rows
                 // P and P (dP - D) of 32 keys
@@ -749,7 +754,7 @@ __global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kerne
                             x = seen >> c & 1u ? x : 0.f;
                             y = seen >> (c + 1) & 1u ? y : 0.f;
                         }
-                        use(c0 + c, x, y);
+                        use(c, x, y);
                     }
                 };
                 const bool whole = live && low >= k0 && high < k0 + kStream;
@@ -762,14 +767,15 @@ __global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kerne
                 }
                 const Pair minus = pair_of(-delta, -delta);
 #pragma unroll
-                for (int c0 = 0; c0 < kStream; c0 += 32) {
+                for (int own = 0; own < F::kPer; own += 32) {
+                    const int c0 = half * F::kPer + own;
                     if (hidden(c0)) {
 #pragma unroll
-                        for (int c = 0; c < 16; ++c) packed[c0 / 2 + c] = 0u;
+                        for (int c = 0; c < 16; ++c) packed[own / 2 + c] = 0u;
                     } else {
                         part(c0, minus, [&](int c, float x, float y) {
                             off = add_pair(off, pair_of(x, y));
-                            packed[c / 2] = pack<T>(x, y);
+                            packed[(own + c) / 2] = pack<T>(x, y);
                         });
                     }
                 }
@@ -779,22 +785,33 @@ __global__ void __launch_bounds__(kBlock, Queries<DP>::kBlocks) query_grad_kerne
                 if (!fine) break;
                 if (n > 0) fence_after();
                 if (j == 0 && n > 0) { leave(); left = true; }
-                tensor_store(mine + F::kProb, packed);
+                if constexpr (F::kHalves == 1) {
+                    tensor_store(mine + F::kProb, packed);
+                } else {
+                    for (int c = 0; c < F::kPer / 2; c += 8) tensor_store8(mine + F::kProb + half * (F::kPer / 2) + c, packed + c);
+                }
                 wait_stores();
                 fence_before();
                 barrier_arrive(&p_full);
             }
             float x, y;
             split(off, x, y);
-            delta += x + y;
-            if (live) p.delta[now.head * p.pitch + i] = delta;
+            if (F::kHalves == 1) {
+                delta += x + y;
+            } else {
+                offs[half][row] = x + y;
+                meet(2, F::kWorkers);
+                delta += offs[0][row] + offs[1 % F::kHalves][row];
+                meet(2, F::kWorkers);
+            }
+            if (live && half == 0) p.delta[now.head * p.pitch + i] = delta;
             if (queries > 0 && !left) leave();          // a block that gave up: NaN for this job's, and below for what is left
             leaving = Leaving{now.i0, now.last, now.head, lse, delta};
         }
         fine = fine && warp_wait(&o_done, (n - 1) & 1, &lost);
         fence_after();
         leave();
-        if (row == 0) wait_stores_done();
+        if (threadIdx.x == 0) wait_stores_done();
     }
     __syncwarp();
     fence_before();
@@ -813,6 +830,8 @@ template <int DP> struct Keys {
     // one block to an SM has columns for two steps' scores; P and dS take their scores' place
     static constexpr int kBlocks = DP == 64 ? 2 : 1, kBuffers = DP == 64 ? 1 : 2, kColumns = 512 / kBlocks;
     static constexpr int kStages = DP == 64 ? 2 : 4;
+    // threads of a row, with one block to an SM two, each with half of a step's columns (40000 tokens in 4 episodes, 8 heads, 2 of keys: 1309 us with one, 1220 so; keys' 2751 and 2344)
+    static constexpr int kHalves = DP == 64 ? 1 : 2, kWorkers = kHalves * kRows, kThreads = kBlock + kWorkers - kRows, kPer = kStream / kHalves;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
     static constexpr int kStaged = 2 * kTile + 2 * kStages * kPart, kShared = kStaged + (DP == 64 ? 2 * kTile : 0) + 1024;         // rows of wide heads leave without a staged tile
     static constexpr int kGrad = kStream, kScores = 2 * kStream, kValue = kBuffers * kScores, kKey = kValue + DP;
@@ -836,7 +855,7 @@ struct KeyJob {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
+__global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                                                                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
                                                                             const __grid_constant__ CUtensorMap map_dv, const AttentionParams p) {
     using F = Keys<DP>;
@@ -852,7 +871,7 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
         barrier_init(&k_empty, 1);
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
         for (int s = 0; s < F::kBuffers; ++s) barrier_init(&s_full[s], 1);
-        barrier_init(&p_full, kRows);
+        barrier_init(&p_full, F::kWorkers);
         barrier_init(&o_done, 1);
         barrier_init(&ended, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -927,8 +946,8 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
                 if (!(fine = warp_wait(&p_full, n & 1, &lost))) break;
                 fence_after();
                 const uint32_t probs = base + n % F::kBuffers * F::kScores;
-                multiply_columns<T, kStream, DP>(base + F::kValue, probs, part_at + (2 * own_stage + 1) * F::kPart, i != 0);
-                multiply_columns<T, kStream, DP>(base + F::kKey, probs + F::kGrad, part_at + 2 * own_stage * F::kPart, i != 0);
+                multiply_columns<T, kStream, DP, F::kPer>(base + F::kValue, probs, part_at + (2 * own_stage + 1) * F::kPart, i != 0);
+                multiply_columns<T, kStream, DP, F::kPer>(base + F::kKey, probs + F::kGrad, part_at + 2 * own_stage * F::kPart, i != 0);
                 commit(&empty[own_stage]);
                 commit(&o_done);
                 if (++own_stage == F::kStages) own_stage = 0;
@@ -938,8 +957,9 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
         commit(&ended);
         drain(&ended, 0);
     } else {
-        const int row = threadIdx.x;
-        const uint32_t mine = base + ((uint32_t)(warp * 32) << 16);
+        // a warp reaches the tensor memory's lanes 32 (warp % 4) and on
+        const int row = warp % 4 * 32 + lane, half = warp / 4 == 0 ? 0 : 1;
+        const uint32_t mine = base + ((uint32_t)(warp % 4 * 32) << 16);
         bool fine = true;
         int n = 0, keys = 0, stage = 0, phase = 0;
         struct Leaving { int first, last, head; } leaving{0, -1, 0};
@@ -950,7 +970,7 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
             if (p.split > 1) {
                 // in 32 bits where the operands were, 16 bytes at a time, rows turned against each other so that lanes meet different banks
 #pragma unroll
-                for (int which = 0; which < 2; ++which)
+                for (int which = half; which < 2; which += F::kHalves)
 #pragma unroll
                     for (int c = 0; c < DP; c += 32) {
                         uint32_t r[32];
@@ -981,13 +1001,11 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
                 }
             } else {
                 T* const to[2] = {static_cast<T*>(p.dk) + ((int64_t)j * p.heads_k + leaving.head) * p.dim, static_cast<T*>(p.dv) + ((int64_t)j * p.heads_k + leaving.head) * p.dim};
-                const bool finite[2] = {store_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), p.dim, there ? to[0] : nullptr),
-                                        store_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), p.dim, there ? to[1] : nullptr)};
-                for (int which = 0; which < 2; ++which)
-                    if (fine && !finite[which] && there) {
-                        slow_key_grad<T>(p, j, leaving.head, which, values);
-                        for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(to[which] + c) = pack_row<T>(values + c);
-                    }
+                const bool finite = store_row<T, DP>(mine + (half ? F::kValue : F::kKey), !fine ? nan_value() : half ? 1.f : p.scale, p.dim, there ? to[half] : nullptr);
+                if (fine && !finite && there) {
+                    slow_key_grad<T>(p, j, leaving.head, half, values);
+                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(to[half] + c) = pack_row<T>(values + c);
+                }
             }
         };
         KeyJob next(p, job0);
@@ -1013,18 +1031,19 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
                     fine = fine && warp_wait(&full[stage], phase, &lost) && warp_wait(&s_full[b], n / F::kBuffers & 1, &lost);
                     if (!fine) break;
                     fence_after();
-                    uint32_t probs[kStream / 2], grads[kStream / 2];
+                    uint32_t probs[F::kPer / 2], grads[F::kPer / 2];
                     const float4 *l4 = reinterpret_cast<const float4*>(lse[stage]), *d4 = reinterpret_cast<const float4*>(delta[stage]);
                     const bool all = i >= all_low && i + kStream - 1 <= all_high;
 #pragma unroll
-                    for (int c0 = 0; c0 < kStream; c0 += 32) {
+                    for (int own = 0; own < F::kPer; own += 32) {
+                        const int c0 = half * F::kPer + own;
                         uint32_t r[32], d[32];
                         tensor_load(here + c0, r);
                         tensor_load(here + F::kGrad + c0, d);
                         wait_loads();
                         if (i + c0 > any_high || i + c0 + 31 < any_low) {
 #pragma unroll
-                            for (int c = 0; c < 16; ++c) probs[c0 / 2 + c] = grads[c0 / 2 + c] = 0u;
+                            for (int c = 0; c < 16; ++c) probs[own / 2 + c] = grads[own / 2 + c] = 0u;
                             continue;
                         }
                         const uint32_t seen = all ? ~0u : columns_between(low - i - c0, high - i - c0);
@@ -1034,19 +1053,19 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
                             const Pair ls[2] = {pair_of(l.x, l.y), pair_of(l.z, l.w)}, es[2] = {pair_of(e.x, e.y), pair_of(e.z, e.w)};
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {
-                                const int at = c0 + c + 2 * k;
+                                const int at = c + 2 * k;
                                 float a, b, x, y;
-                                split(fma_pair(ls[k], minus_one, mul_pair(pair_of(__uint_as_float(r[at - c0]), __uint_as_float(r[at - c0 + 1])), scale2)), a, b);
+                                split(fma_pair(ls[k], minus_one, mul_pair(pair_of(__uint_as_float(r[at]), __uint_as_float(r[at + 1])), scale2)), a, b);
                                 a = exp2_fast(a);
                                 b = exp2_fast(b);
-                                split(mul_pair(pair_of(a, b), fma_pair(es[k], minus_one, pair_of(__uint_as_float(d[at - c0]), __uint_as_float(d[at - c0 + 1])))), x, y);
+                                split(mul_pair(pair_of(a, b), fma_pair(es[k], minus_one, pair_of(__uint_as_float(d[at]), __uint_as_float(d[at + 1])))), x, y);
                                 if (!all) {
-                                    const bool u = seen >> (at - c0) & 1u, v = seen >> (at - c0 + 1) & 1u;
+                                    const bool u = seen >> at & 1u, v = seen >> (at + 1) & 1u;
                                     a = u ? a : 0.f; x = u ? x : 0.f;
                                     b = v ? b : 0.f; y = v ? y : 0.f;
                                 }
-                                probs[at / 2] = pack<T>(a, b);
-                                grads[at / 2] = pack<T>(x, y);
+                                probs[(own + at) / 2] = pack<T>(a, b);
+                                grads[(own + at) / 2] = pack<T>(x, y);
                             }
                         }
                     }
@@ -1056,8 +1075,16 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
                     if (n > 0 && first) fence_after();
                     if (first && n > 0) { leave(); left = true; }
                     first = false;
-                    tensor_store(here, probs);
-                    tensor_store(here + F::kGrad, grads);
+                    if constexpr (F::kHalves == 1) {
+                        tensor_store(here, probs);
+                        tensor_store(here + F::kGrad, grads);
+                    } else {
+                        // where the thread's own scores were, since the row's other thread may still have to read its own
+                        for (int c = 0; c < F::kPer / 2; c += 8) {
+                            tensor_store8(here + half * F::kPer + c, probs + c);
+                            tensor_store8(here + F::kGrad + half * F::kPer + c, grads + c);
+                        }
+                    }
                     wait_stores();
                     fence_before();
                     barrier_arrive(&p_full);
@@ -1082,7 +1109,7 @@ __global__ void __launch_bounds__(kBlock, Keys<DP>::kBlocks) key_grad_kernel(con
         // each block takes its share of the rows of the cluster's one job
         const KeyJob job(p, job0);
         const int rows = kRows / p.split;
-        for (int x = threadIdx.x; x < 2 * rows * (DP / 4); x += kBlock) {
+        for (int x = threadIdx.x; x < 2 * rows * (DP / 4); x += F::kThreads) {
             const int which = x / (rows * (DP / 4)), row = rank * rows + x / (DP / 4) % rows, c = x % (DP / 4) * 4, j = job.j0 + row;
             float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
             for (int b = 0; b < p.split; ++b) {
@@ -1177,15 +1204,15 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
         p.split = 1;
         while (keys && p.split < 8 && group % (2 * p.split) == 0 && 2 * p.split * (int64_t)jobs <= places) p.split *= 2;
         if (!keys) {
-            query_grad_kernel<T, DP><<<(unsigned)blocks, kBlock, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
+            query_grad_kernel<T, DP><<<(unsigned)blocks, Queries<DP>::kThreads, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         } else if (p.split == 1) {
-            key_grad_kernel<T, DP><<<(unsigned)blocks, kBlock, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
+            key_grad_kernel<T, DP><<<(unsigned)blocks, Keys<DP>::kThreads, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
         } else {
             cudaLaunchAttribute cluster{};
             cluster.id = cudaLaunchAttributeClusterDimension;
             cluster.val.clusterDim.x = (unsigned)p.split; cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1u;
             cudaLaunchConfig_t config{};
-            config.gridDim = dim3((unsigned)(jobs * p.split)); config.blockDim = dim3(kBlock); config.dynamicSmemBytes = Keys<DP>::kShared; config.stream = stream;
+            config.gridDim = dim3((unsigned)(jobs * p.split)); config.blockDim = dim3(Keys<DP>::kThreads); config.dynamicSmemBytes = Keys<DP>::kShared; config.stream = stream;
             config.attrs = &cluster; config.numAttrs = 1u;
             set = cudaLaunchKernelEx(&config, key_grad_kernel<T, DP>, q, g, k, v, dk, dv, p);
             if (set != cudaSuccess) return set;

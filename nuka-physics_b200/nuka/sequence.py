@@ -176,7 +176,8 @@ class _Recurrence(torch.autograd.Function):
     @_once
     def backward(ctx, dh, dstate):
         x, gate, h, *initial = ctx.saved_tensors
-        initial, episodes = initial[0] if initial else None, ctx.episodes
+        # what is saved may come back elsewhere and with other strides (offloaded, worked out again)
+        x, gate, h, initial, episodes = _channels_last(x), _channels_last(gate), h.contiguous(), initial[0].contiguous() if initial else None, ctx.episodes
         device, dtype, channels = x.device, _DTYPES[x.dtype], x.shape[1]
         dh = torch.zeros_like(h) if dh is None else dh.contiguous()
         dstate = None if dstate is None else dstate.contiguous()
@@ -243,34 +244,41 @@ def rotary_frequencies(turned, base=10000.0, trained=0, context=0, low=1.0, high
     return f
 
 
-def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
-    device = q.device
-    tokens, heads_q, dim = q.shape
-    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=q.dtype, device=device)
-    desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), tokens, heads_q, k.shape[1], dim,
+def _heads_desc(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
+    return _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), q.shape[0], q.shape[1], k.shape[1], q.shape[2],
                           0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
-                          _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
+                          _ptr(q_weight), _ptr(k_weight), eps)
+
+
+def _turn(q, k, *rest):
+    device = q.device
+    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=q.dtype, device=device)
+    desc = _heads_desc(q, k, *rest)
+    desc.q_out, desc.k_out = q_out.data_ptr(), k_out.data_ptr()
     _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
-    return q_out, k_out, desc
+    return q_out, k_out
 
 
 class _Heads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
-        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved)
-        # the descriptor's arrays stay alive with what is saved here
-        ctx.save_for_backward(q, k, *(x for x in (q_weight, k_weight, first, positions, frequencies) if x is not None))
-        ctx.desc, ctx.weights = desc, (q_weight is not None, k_weight is not None)
+        given = (q_weight, k_weight, first, positions, frequencies)
+        ctx.save_for_backward(q, k, *(x for x in given if x is not None))
+        ctx.given, ctx.rest = [x is not None for x in given], (eps, interleaved)
         ctx.set_materialize_grads(False)
-        return q_out, k_out
+        return _turn(q, k, *given, eps, interleaved)
 
     @_once
     def backward(ctx, dq_out, dk_out):
-        q, k = ctx.saved_tensors[:2]
-        device, desc = q.device, ctx.desc
-        dq_out, dk_out = (torch.zeros(x.shape, dtype=x.dtype, device=device) if d is None else _channels_last(d.contiguous(), 1, 4 * x.element_size()) for x, d in ((q, dq_out), (k, dk_out)))
+        # what is saved may come back elsewhere and with other strides (offloaded, worked out again), so the descriptor is made anew
+        q, k, *saved = ctx.saved_tensors
+        size = 4 * q.element_size()
+        q, k, saved = _channels_last(q, 4, size), _channels_last(k, 4, size), [x.contiguous() for x in saved]
+        each = iter(saved)
+        device, desc = q.device, _heads_desc(q, k, *(next(each) if has else None for has in ctx.given), *ctx.rest)
+        dq_out, dk_out = (torch.zeros(x.shape, dtype=x.dtype, device=device) if d is None else _channels_last(d.contiguous(), 1, size) for x, d in ((q, dq_out), (k, dk_out)))
         dq, dk = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device)
-        dw = [torch.empty(q.shape[2], dtype=torch.float32, device=device) if has and ctx.needs_input_grad[2 + i] else None for i, has in enumerate(ctx.weights)]
+        dw = [torch.empty(q.shape[2], dtype=torch.float32, device=device) if has and ctx.needs_input_grad[2 + i] else None for i, has in enumerate(ctx.given[:2])]
         lib = _abi.lib()
         need = lib.nuka_b200_heads_workspace(q.shape[0], q.shape[2]) if dw[0] is not None or dw[1] is not None else 0
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
@@ -305,39 +313,44 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     q, k = _channels_last(q, 4, size), _channels_last(k, 4, size)
     train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight))
     if not train:
-        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)[:2]
+        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
     return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
 
 
 # ---- attention over packed episodes --------------------------------------------------------------------------------
+def _attention_desc(q, k, v, out, lse, episodes, scale, window):
+    return _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
+                              _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
+
+
 def _attend(q, k, v, episodes, scale, window, train):
-    """(out, the statistics that a backward pass needs beside it, the call's descriptor)."""
+    """out, and the statistics that a backward pass needs beside it."""
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     lib = _abi.lib()
     lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device) if train else None
-    desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
-                              _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
-    _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
-    return out, lse, desc
+    _call(device, lib.nuka_b200_attention, ctypes.byref(_attention_desc(q, k, v, out, lse, episodes, scale, window)))
+    return out, lse
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, episodes, scale, window):
-        out, lse, desc = _attend(q, k, v, episodes, scale, window, True)
-        # the descriptor's arrays stay alive with what is saved here
+        out, lse = _attend(q, k, v, episodes, scale, window, True)
         ctx.save_for_backward(q, k, v, out, lse)
-        ctx.desc, ctx.episodes = desc, episodes
+        ctx.rest = episodes, scale, window
         return out
 
     @_once
     def backward(ctx, dout):
+        # what is saved may come back elsewhere and with other strides, as for heads
         q, k, v, out, lse = ctx.saved_tensors
-        device, desc = q.device, ctx.desc
-        dout = _channels_last(dout.contiguous(), 1, 16)
+        q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
+        out, lse, dout = (_channels_last(x.contiguous(), 1, 16) for x in (out, lse, dout))
+        desc = _attention_desc(q, k, v, out, lse, *ctx.rest)
+        device = q.device
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
-        delta = torch.empty_like(lse)
+        delta = torch.empty(lse.shape, dtype=lse.dtype, device=device)
         desc.dout, desc.delta, desc.dq, desc.dk, desc.dv = dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         _call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc))
         return dq, dk, dv, None, None, None

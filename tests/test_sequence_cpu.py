@@ -1,0 +1,72 @@
+"""What nuka.sequence hands to the library and to torch, without a GPU: its calls go to a recorder in the library's place."""
+import pytest
+
+torch = pytest.importorskip("torch")
+from nuka import sequence as S  # noqa: E402
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """Tensors of the CPU are taken, and (entry's name, descriptor) of each call is kept; nothing is worked out."""
+    seen = []
+    monkeypatch.setattr(S, "_on_gpu", lambda first, *others: first.device)
+    monkeypatch.setattr(S, "_call", lambda device, function, *args: seen.append((function.__name__, getattr(args[0], "_obj", None))))
+    return seen
+
+
+def _plan(rows=2, length=5):
+    return S.Episodes.from_offsets(torch.arange(rows + 1, dtype=torch.int32) * length, rows * length)
+
+
+def _recurrence(leaves):
+    return S.gated_recurrence(leaves[0], leaves[1], _plan(), leaves[2])[0]
+
+
+def _heads(leaves):
+    return sum(S.rotate_heads(*leaves, _plan(), torch.ones(4, dtype=torch.float64)))
+
+
+def _attention(leaves):
+    return S.episode_attention(*leaves, _plan())
+
+
+# the operator, its leaves, and the fields of its backward call that come from the forward pass
+OPERATORS = {
+    "recurrence": (_recurrence, lambda: [torch.randn(10, 8), torch.randn(10, 8), torch.randn(2, 8)], ("x", "gate", "initial", "h")),
+    "heads": (_heads, lambda: [torch.randn(10, 2, 16), torch.randn(10, 2, 16), torch.ones(16), torch.ones(16)], ("q", "k", "q_weight", "k_weight", "first", "frequencies")),
+    "attention": (_attention, lambda: [torch.randn(10, 2, 16).bfloat16() for _ in range(3)], ("q", "k", "v", "out", "lse")),
+}
+
+
+@pytest.mark.parametrize("operator", list(OPERATORS))
+@pytest.mark.parametrize("turned", [False, True])
+def test_gradients_read_what_saved_tensors_return(calls, operator, turned):
+    """Hooks (offloading, checkpointing) give back other tensors than were saved, of other strides perhaps: the backward call has their addresses, or those of copies of
+    them, and strides that go with them."""
+    run, make, fields = OPERATORS[operator]
+    leaves = [x.requires_grad_() for x in make()]
+    kept, back = [], []
+
+    def unpack(x):
+        y = x.clone()
+        if turned and y.dim() == 3:                        # the same values, heads before tokens
+            y = y.transpose(0, 1).contiguous().transpose(0, 1)
+        back.append(y)
+        return y
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda x: kept.append(x.clone()) or kept[-1], unpack):
+        out = run(leaves)
+    for _ in range(2):                                     # a graph that is kept: each pass has a descriptor of its own
+        back.clear()
+        torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
+        name, desc = calls[-1]
+        assert name.endswith("_backward")
+        at = {x.data_ptr(): x for x in back}
+        for field in fields:
+            if not (turned and field == "out"):            # contiguous, so a copy of what was turned
+                assert getattr(desc, field) in at, field
+        for field in ("q", "k", "v") if operator != "recurrence" else ():
+            if hasattr(desc, field):
+                x = at[getattr(desc, field)]
+                assert (getattr(desc, field + "_stride"), getattr(desc, field + "_head_stride")) == x.stride()[:2]
+    assert calls[-1][1] is not calls[-2][1]

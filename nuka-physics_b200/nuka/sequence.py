@@ -67,6 +67,10 @@ def _flags(tensor, shape, device, what):
     return tensor.contiguous()
 
 
+def _empty(like):
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
+
+
 def _stride(tensor, dim):
     return tensor.stride(dim) if tensor.shape[dim] > 1 else 0
 
@@ -82,6 +86,18 @@ def _channels_last(tensor, multiple=1, size=1, least=0):
         else:
             return tensor
     return tensor.clone(memory_format=torch.contiguous_format)
+
+
+def _point(desc, names, tensors, strides=None, size=1):
+    """Sets the descriptor's addresses to those that the tensors have. What a backward pass finds saved may lie elsewhere than in the forward call, and otherwise (offloaded, worked
+    out again): False where a stride is not what it was or an address is not on `size` bytes."""
+    fits = True
+    for i, (name, x) in enumerate(zip(names, tensors)):
+        at = x.data_ptr()
+        setattr(desc, name, at)
+        if strides is not None and (x.stride() != strides[i] or at % size):
+            fits = False
+    return fits
 
 
 class Episodes:
@@ -181,7 +197,7 @@ class _Recurrence(torch.autograd.Function):
         device, dtype, channels = x.device, _DTYPES[x.dtype], x.shape[1]
         dh = torch.zeros_like(h) if dh is None else dh.contiguous()
         dstate = None if dstate is None else dstate.contiguous()
-        dx, dgate = torch.empty(x.shape, dtype=x.dtype, device=device), torch.empty(x.shape, dtype=x.dtype, device=device)
+        dx, dgate = _empty(x), _empty(x)
         dinitial = None
         if ctx.has_initial and ctx.needs_input_grad[2]:
             if not episodes._rows_may_be_empty:
@@ -244,41 +260,42 @@ def rotary_frequencies(turned, base=10000.0, trained=0, context=0, low=1.0, high
     return f
 
 
-def _heads_desc(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
-    return _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), q.shape[0], q.shape[1], k.shape[1], q.shape[2],
-                          0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
-                          _ptr(q_weight), _ptr(k_weight), eps)
-
-
-def _turn(q, k, *rest):
+def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
     device = q.device
-    q_out, k_out = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=q.dtype, device=device)
-    desc = _heads_desc(q, k, *rest)
-    desc.q_out, desc.k_out = q_out.data_ptr(), k_out.data_ptr()
+    tokens, heads_q, dim = q.shape
+    q_out, k_out = _empty(q), _empty(k)
+    desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), tokens, heads_q, k.shape[1], dim,
+                          0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
+                          _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
     _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
-    return q_out, k_out
+    return q_out, k_out, desc
 
 
 class _Heads(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
-        given = (q_weight, k_weight, first, positions, frequencies)
-        ctx.save_for_backward(q, k, *(x for x in given if x is not None))
-        ctx.given, ctx.rest = [x is not None for x in given], (eps, interleaved)
+        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved)
+        tensors = {"q": q, "k": k, "q_weight": q_weight, "k_weight": k_weight, "first": first, "positions": positions, "frequencies": frequencies}
+        ctx.names = [name for name, x in tensors.items() if x is not None]
+        tensors = [tensors[name] for name in ctx.names]
+        ctx.save_for_backward(*tensors)
+        ctx.desc, ctx.strides = desc, [x.stride() for x in tensors]
         ctx.set_materialize_grads(False)
-        return _turn(q, k, *given, eps, interleaved)
+        return q_out, k_out
 
     @_once
     def backward(ctx, dq_out, dk_out):
-        # what is saved may come back elsewhere and with other strides (offloaded, worked out again), so the descriptor is made anew
-        q, k, *saved = ctx.saved_tensors
-        size = 4 * q.element_size()
-        q, k, saved = _channels_last(q, 4, size), _channels_last(k, 4, size), [x.contiguous() for x in saved]
-        each = iter(saved)
-        device, desc = q.device, _heads_desc(q, k, *(next(each) if has else None for has in ctx.given), *ctx.rest)
+        tensors, desc = ctx.saved_tensors, _abi.HeadsDesc.from_buffer_copy(ctx.desc)
+        size = 4 * tensors[0].element_size()
+        if not _point(desc, ctx.names, tensors, ctx.strides, size):
+            tensors = [_channels_last(x, 4, size) if i < 2 else _channels_last(x.contiguous(), 1, size) for i, x in enumerate(tensors)]
+            _point(desc, ctx.names, tensors)
+            desc.q_stride, desc.q_head_stride, desc.k_stride, desc.k_head_stride = (_stride(x, i) for x in tensors[:2] for i in (0, 1))
+        q, k = tensors[:2]
+        device = q.device
         dq_out, dk_out = (torch.zeros(x.shape, dtype=x.dtype, device=device) if d is None else _channels_last(d.contiguous(), 1, size) for x, d in ((q, dq_out), (k, dk_out)))
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device)
-        dw = [torch.empty(q.shape[2], dtype=torch.float32, device=device) if has and ctx.needs_input_grad[2 + i] else None for i, has in enumerate(ctx.given[:2])]
+        dq, dk = _empty(q), _empty(k)
+        dw = [_empty(tensors[ctx.names.index(name)]) if name in ctx.names and ctx.needs_input_grad[2 + i] else None for i, name in enumerate(("q_weight", "k_weight"))]
         lib = _abi.lib()
         need = lib.nuka_b200_heads_workspace(q.shape[0], q.shape[2]) if dw[0] is not None or dw[1] is not None else 0
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
@@ -313,44 +330,44 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     q, k = _channels_last(q, 4, size), _channels_last(k, 4, size)
     train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight))
     if not train:
-        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
+        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)[:2]
     return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
 
 
 # ---- attention over packed episodes --------------------------------------------------------------------------------
-def _attention_desc(q, k, v, out, lse, episodes, scale, window):
-    return _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
-                              _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
-
-
 def _attend(q, k, v, episodes, scale, window, train):
-    """out, and the statistics that a backward pass needs beside it."""
+    """(out, the statistics that a backward pass needs beside it, the call's descriptor)."""
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
     lib = _abi.lib()
     lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device) if train else None
-    _call(device, lib.nuka_b200_attention, ctypes.byref(_attention_desc(q, k, v, out, lse, episodes, scale, window)))
-    return out, lse
+    desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
+                              _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
+    _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
+    return out, lse, desc
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, episodes, scale, window):
-        out, lse = _attend(q, k, v, episodes, scale, window, True)
-        ctx.save_for_backward(q, k, v, out, lse)
-        ctx.rest = episodes, scale, window
+        out, lse, desc = _attend(q, k, v, episodes, scale, window, True)
+        tensors = (q, k, v, out, lse)
+        ctx.save_for_backward(*tensors)
+        ctx.desc, ctx.strides, ctx.episodes = desc, [x.stride() for x in tensors], episodes
         return out
 
     @_once
     def backward(ctx, dout):
-        # what is saved may come back elsewhere and with other strides, as for heads
-        q, k, v, out, lse = ctx.saved_tensors
-        q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
-        out, lse, dout = (_channels_last(x.contiguous(), 1, 16) for x in (out, lse, dout))
-        desc = _attention_desc(q, k, v, out, lse, *ctx.rest)
-        device = q.device
-        dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
-        delta = torch.empty(lse.shape, dtype=lse.dtype, device=device)
+        tensors, desc, names = ctx.saved_tensors, _abi.AttentionDesc.from_buffer_copy(ctx.desc), ("q", "k", "v", "out", "lse")
+        if not _point(desc, names, tensors, ctx.strides, 16):
+            tensors = [_channels_last(x, 8, 16, x.shape[2]) if i < 3 else _channels_last(x.contiguous(), 1, 16) for i, x in enumerate(tensors)]
+            _point(desc, names, tensors)
+            desc.q_stride, desc.q_head_stride, desc.k_stride, desc.k_head_stride, desc.v_stride, desc.v_head_stride = (_stride(x, i) for x in tensors[:3] for i in (0, 1))
+        lse = tensors[4]
+        device = lse.device
+        dout = _channels_last(dout.contiguous(), 1, 16)
+        dq, dk, dv = _empty(tensors[0]), _empty(tensors[1]), _empty(tensors[2])
+        delta = _empty(lse)
         desc.dout, desc.delta, desc.dq, desc.dk, desc.dv = dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         _call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc))
         return dq, dk, dv, None, None, None

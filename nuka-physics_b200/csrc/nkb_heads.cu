@@ -120,11 +120,13 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? (sizeof(T) == 4 ? 4 : 6) 
                 }
                 const float r = rsqrtf(fmaf(square, inverse, p.eps));
                 if constexpr (BACKWARD) {
-                    const float pull = r * r * r * (dot * inverse);
+                    // dx = r (e - y mean(y e)) with y = x r, which stays within 32 bits where r^3 does not
+                    const float pull = r * (dot * inverse);
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        dw[keys][i] = fmaf(d[i], v[i] * r, dw[keys][i]);
-                        d[i] = fmaf(d[i] * w[i], r, -v[i] * pull);
+                        const float y = in ? v[i] * r : 0.f;        // without eps r is infinite where there is no row
+                        dw[keys][i] = fmaf(d[i], y, dw[keys][i]);
+                        d[i] = fmaf(-y, pull, d[i] * w[i]) * r;
                     }
                     if (in) { store<T, 4>(to + low, d0); store<T, 4>(to + high, d1); }
                 } else {

@@ -57,3 +57,44 @@ def test_gradients_under_checkpointing_and_hooks(operator, way):
         with torch.autograd.graph.save_on_cpu() if way == "on the CPU" else torch.autograd.graph.saved_tensors_hooks(lambda x: x.clone(), lambda x: x.clone()):
             got = _grads(run, leaves)
     assert all(torch.equal(a, b) and torch.isfinite(a).all() for a, b in zip(want, got))
+
+
+# ---- norms of heads with little or nothing added to the mean square -----------------------------------------------------
+def _normed_64(x, w, eps):
+    return x / torch.sqrt((x * x).mean(-1, keepdim=True) + eps) * w
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tokens,dim", [(1, 64), (17, 64), (33, 64), (5, 200), (7, 40)])
+def test_heads_without_eps(dtype, tokens, dim):
+    """Tokens that do not fill a block's last pass: lanes without a token add nothing to the weights' gradients.  Bounds: a few units in the last place of 32 bits before the one rounding,
+    for the weights times the square root of the number of terms."""
+    gen = _gen(tokens)
+    positions = torch.zeros(tokens, dtype=torch.int32, device="cuda")
+    q, k = (_normal(gen, tokens, n, dim, dtype=dtype).requires_grad_() for n in (3, 1))
+    w = _normal(gen, dim, shift=1.0, scale=0.2).requires_grad_()
+    out = S.rotate_heads(q, k, w, w, positions, None, eps=0.0)
+    cot = [_normal(gen, *o.shape, dtype=dtype) for o in out]
+    dq, dk, dw = torch.autograd.grad(out, [q, k, w], cot)
+    leaves = [x.detach().double().requires_grad_() for x in (q, k, w)]
+    want = torch.autograd.grad([_normed_64(leaves[0], leaves[2], 0.0), _normed_64(leaves[1], leaves[2], 0.0)], leaves, [c.double() for c in cot])
+    unit, ulps = (2.0 ** -8 if dtype is torch.bfloat16 else 2.0 ** -23), 16 * 2.0 ** -23
+    for got, x in ((dq, want[0]), (dk, want[1])):
+        assert ((got.double() - x).abs() <= unit * x.abs() + ulps * x.abs().max()).all()
+    assert ((dw.double() - want[2]).abs() <= ulps * (4 * tokens) ** 0.5 * max(c.double().abs().max().item() for c in cot) * 4).all()
+
+
+def test_heads_of_tiny_values_and_tiny_eps():
+    """A row of zeros and rows whose squares are far below 1: the cube of one over the root is beyond 32 bits, the gradient is not."""
+    positions = torch.zeros(3, dtype=torch.int32, device="cuda")
+    gen = _gen(2)
+    q = _normal(gen, 3, 2, 64) * torch.tensor([0.0, 1e-15, 1e-14], device="cuda")[:, None, None]
+    q.requires_grad_()
+    out = S.rotate_heads(q, q, None, None, positions, None, eps=1e-30)
+    cot = _normal(gen, 3, 2, 64)
+    dq, = torch.autograd.grad(out[0], q, cot)
+    x = q.detach().double().requires_grad_()
+    want, = torch.autograd.grad(_normed_64(x, 1.0, 1e-30), x, cot.double())
+    # row by row, whose gradients are of very different sizes; the eps itself is 2^-24 off in 32 bits
+    off, size = (dq.double() - want).abs().amax(-1), want.abs().amax(-1)
+    assert torch.isfinite(dq).all() and (off <= 16 * 2.0 ** -23 * size).all()

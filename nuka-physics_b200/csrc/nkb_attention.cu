@@ -674,6 +674,7 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
         bool fine = true;
         int n = 0, queries = 0;
         struct Leaving { int first, last, head; float lse, delta; } leaving{0, -1, 0, 0.f, 0.f};
+        // Every warp calls it once for each job, whether it gave up or not, and the named barrier in it is the only one: all meet there in the same order.
         auto leave = [&]() {
             const int i = leaving.first + row;
             const bool there = i <= leaving.last;
@@ -681,6 +682,9 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             unsigned char* const tile = shared + F::kStaged;
             if (threadIdx.x == 0) wait_stores_read();
             meet(1, F::kWorkers);
+            // the row's other thread has its part of D; where the block gave up, the keys' gradients become NaN by it
+            if (F::kHalves > 1) leaving.delta += offs[0][row] + offs[1 % F::kHalves][row];
+            if (there && half == 0) p.delta[leaving.head * p.pitch + i] = fine ? leaving.delta : nan_value();
             const bool finite = stage_row<T, DP / F::kHalves>(mine + F::kOut + half * (DP / 2), fine ? p.scale : nan_value(), tile + half * kRows * 128, row);
             if (fine && !finite && there) {
                 slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
@@ -796,16 +800,9 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             }
             float x, y;
             split(off, x, y);
-            if (F::kHalves == 1) {
-                delta += x + y;
-            } else {
-                offs[half][row] = x + y;
-                meet(2, F::kWorkers);
-                delta += offs[0][row] + offs[1 % F::kHalves][row];
-                meet(2, F::kWorkers);
-            }
-            if (live && half == 0) p.delta[now.head * p.pitch + i] = delta;
             if (queries > 0 && !left) leave();          // a block that gave up: NaN for this job's, and below for what is left
+            if (F::kHalves == 1) delta += x + y;
+            else offs[half][row] = x + y;               // read in leave(), between whose two meetings nobody writes it
             leaving = Leaving{now.i0, now.last, now.head, lse, delta};
         }
         fine = fine && warp_wait(&o_done, (n - 1) & 1, &lost);

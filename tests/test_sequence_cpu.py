@@ -1,4 +1,7 @@
 """What nuka.sequence hands to the library and to torch, without a GPU: its calls go to a recorder in the library's place."""
+import os
+import re
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -70,3 +73,13 @@ def test_gradients_read_what_saved_tensors_return(calls, operator, turned):
                 x = at[getattr(desc, field)]
                 assert (getattr(desc, field + "_stride"), getattr(desc, field + "_head_stride")) == x.stride()[:2]
     assert calls[-1][1] is not calls[-2][1]
+
+
+def test_the_rows_of_an_attention_kernel_meet_at_one_barrier():
+    """A wait of a kernel that gives up does so warp by warp.  Warps that go on and warps that gave up meet at the same named barriers in the same order only because there is one of
+    them: with two, the first could wait at one and the second at the other, and such a wait has no limit."""
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "nuka-physics_b200", "csrc", "nkb_attention.cu")
+    with open(path) as f:
+        kernels = f.read().split("__global__")[1:]
+    met = [set(re.findall(r"\bmeet\(([^,]*),", body)) for body in kernels]
+    assert len(kernels) == 3 and all(len(m) <= 1 for m in met) and any(met), met

@@ -146,8 +146,14 @@ template <typename T, int DP> __device__ __forceinline__ bool stage_row(uint32_t
 }
 
 // ---- rows that are not finite -----------------------------------------------------------------------------------------
-// A product over a tile multiplies what a row does not see by 0, and 0 times an infinity or NaN is NaN: an episode that is not finite would reach the others of its tiles. So a row that comes out
-// not finite is worked out again by its thread alone, in 32 bits, from what it sees and nothing else. That is slow, and only then.
+// A product over a tile multiplies what a row does not see by 0, and 0 times an infinity or NaN is NaN: an episode that is not finite would reach the others of its tiles. And in f16 a dS above
+// 65504 becomes an infinity. So a block remembers that a row came out not finite though its own statistics are, and when all its jobs are done, its pipeline at rest and no wait under way
+// that could give up meanwhile, its warps go over its rows once more: of a row that is not finite the columns in question are worked out in 32 bits, from what the row sees and nothing else.
+// A column that is not finite by its definition is left as it is, whichever of infinity and NaN it became; what shows that is read without a product: a visible value for the
+// outputs; for the gradients a query's lse or D, which are not finite wherever its row of q or dO is not.
+// A lane has four columns of the row's result, and of each 32 keys or queries one weight.
+// 30000 finite tokens, 20000 of which some are infinite, and 700 (8 heads, 2 of keys, dim 64, bf16; 2.0 and 7.9 ms where all are finite): 2.0 to 133 ms forwards, 7.8 to 173 back, by what is
+// infinite and where; 16384 tokens in f16 with most of dS beyond its range 95 ms back (1.6).
 template <typename T> __device__ __forceinline__ float dot(const T* a, const T* b, int dim) {
     float s = 0.f;
     for (int c = 0; c < dim; c += 8) {
@@ -159,56 +165,115 @@ template <typename T> __device__ __forceinline__ float dot(const T* a, const T* 
     }
     return s;
 }
-template <typename T> __device__ __forceinline__ void add_row(float* sum, float by, const T* row, int dim) {
-    for (int c = 0; c < dim; c += 8) {
-        float v[8];
-        unpack<T, 8>(load_raw<T, 8>(row + c), v);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum[c + k] = fmaf(by, v[k], sum[c + k]);
-    }
-}
 template <typename T> __device__ __forceinline__ const T* query_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.q) + i * p.q_stride + head * p.q_head_stride; }
 template <typename T> __device__ __forceinline__ const T* key_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.k) + j * p.k_stride + head * p.k_head_stride; }
 template <typename T> __device__ __forceinline__ const T* value_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.v) + j * p.v_stride + head * p.v_head_stride; }
 template <typename T> __device__ __forceinline__ const T* dout_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.dout) + ((int64_t)i * p.heads_q + head) * p.dim; }
-template <typename T> __device__ __forceinline__ float probability(const AttentionParams& p, int i, int j, int head, int key_head, float lse) {
-    return exp2f(fmaf(dot<T>(query_row<T>(p, i, head), key_row<T>(p, j, key_head), p.dim), p.scale2, -lse));
-}
 __device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
 __device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
 
-template <typename T> __device__ __noinline__ void slow_out(const AttentionParams& p, int i, int head, float lse, float* sum) {
-    const int key_head = head / (p.heads_q / p.heads_k);
-    for (int c = 0; c < p.dim; ++c) sum[c] = 0.f;
-    for (int j = first_key(p, i); j <= i; ++j) add_row<T>(sum, probability<T>(p, i, j, head, key_head, lse), value_row<T>(p, j, key_head), p.dim);
+// Which of a lane's four values are not finite.
+template <typename T> __device__ __forceinline__ uint32_t spoilt_of(uint2 v) {
+    constexpr uint32_t E = __is_same(T, __nv_bfloat16) ? 0x7f80u : 0x7c00u;
+    uint32_t m = 0u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) m |= ((k < 2 ? v.x : v.y) >> (k % 2 * 16) & E) == E ? 1u << k : 0u;
+    return m;
 }
-template <typename T> __device__ __noinline__ void slow_query_grad(const AttentionParams& p, int i, int head, float lse, float delta, float* sum) {
-    const int key_head = head / (p.heads_q / p.heads_k);
-    for (int c = 0; c < p.dim; ++c) sum[c] = 0.f;
-    for (int j = first_key(p, i); j <= i; ++j) {
-        const float ds = probability<T>(p, i, j, head, key_head, lse) * (dot<T>(dout_row<T>(p, i, head), value_row<T>(p, j, key_head), p.dim) - delta);
-        add_row<T>(sum, ds * p.scale, key_row<T>(p, j, key_head), p.dim);
+// The lane's four columns of a row of a result that this kernel wrote; none behind dim.
+template <typename T> __device__ __forceinline__ uint2 result_of(const T* row, int dim, int lane) { return 4 * lane < dim ? __ldcg(reinterpret_cast<const uint2*>(row + 4 * lane)) : make_uint2(0u, 0u); }
+template <typename T> __device__ __forceinline__ void give_columns(T* row, uint32_t which, const float (&sum)[4], float by, int lane) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (which >> k & 1u) row[4 * lane + k] = from_float<T>(sum[k] * by);
+}
+// sum += the weights of the lanes below `count` times their rows
+template <typename T, typename Row> __device__ __forceinline__ void add_rows(float (&sum)[4], float weight, int count, int dim, int lane, Row row) {
+#pragma unroll 4
+    for (int k = 0; k < count; ++k) {
+        const float by = __shfl_sync(~0u, weight, k);
+        if (4 * lane < dim) {
+            float v[4];
+            unpack<T, 4>(load_raw<T, 4>(row(k) + 4 * lane), v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum[e] = fmaf(by, v[e], sum[e]);
+        }
     }
 }
+constexpr uint32_t kFinal = 0xffffu;                    // first value of an output row whose lse is not finite: NaN as no conversion gives it
+
+template <typename T> __device__ __noinline__ void mend_out(const AttentionParams& p, int i, int head, int lane) {
+    T* const out = static_cast<T*>(p.out) + ((int64_t)i * p.heads_q + head) * p.dim;
+    const uint2 is = result_of(out, p.dim, lane);
+    uint32_t which = spoilt_of<T>(is);
+    if (!__any_sync(~0u, which != 0u) || (__shfl_sync(~0u, is.x, 0) & 0xffffu) == kFinal) return;
+    const int key_head = head / (p.heads_q / p.heads_k), low = first_key(p, i);
+    for (int j = low; j <= i && __any_sync(~0u, which != 0u); j += 8)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) which &= ~spoilt_of<T>(result_of(value_row<T>(p, min(j + k, i), key_head), p.dim, lane));
+    if (!__any_sync(~0u, which != 0u)) return;
+    float top = -INFINITY, total = 0.f, sum[4] = {};
+    for (int j = low; j <= i; j += 32) {
+        const int count = min(32, i - j + 1);
+        const float score = lane < count ? dot(query_row<T>(p, i, head), key_row<T>(p, j + lane, key_head), p.dim) * p.scale2 : -INFINITY;
+        float best = score;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) best = fmaxf(best, __shfl_xor_sync(~0u, best, d));
+        best = fmaxf(best, top);
+        const float shift = best == -INFINITY ? 0.f : best, by = exp2f(top - shift), weight = exp2f(score - shift);
+        total = fmaf(total, by, weight);                // the lane's own part
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] *= by;
+        add_rows<T>(sum, weight, count, p.dim, lane, [&](int k) { return value_row<T>(p, j + k, key_head); });
+        top = best;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
+    give_columns(out, which, sum, 1.f / total, lane);
+}
+
+template <typename T> __device__ __noinline__ void mend_query_grad(const AttentionParams& p, int i, int head, int lane) {
+    const float lse = p.lse[head * p.pitch + i], delta = __ldcg(p.delta + head * p.pitch + i);
+    if (!isfinite(lse) || !isfinite(delta)) return;
+    T* const dq = static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + head) * p.dim;
+    const uint32_t which = spoilt_of<T>(result_of(dq, p.dim, lane));
+    if (!__any_sync(~0u, which != 0u)) return;
+    const int key_head = head / (p.heads_q / p.heads_k);
+    float sum[4] = {};
+    for (int j = first_key(p, i); j <= i; j += 32) {
+        const int count = min(32, i - j + 1), own = min(j + lane, i);
+        const float prob = exp2f(fmaf(dot(query_row<T>(p, i, head), key_row<T>(p, own, key_head), p.dim), p.scale2, -lse));
+        const float weight = prob * (dot(dout_row<T>(p, i, head), value_row<T>(p, own, key_head), p.dim) - delta);
+        add_rows<T>(sum, weight, count, p.dim, lane, [&](int k) { return key_row<T>(p, j + k, key_head); });
+    }
+    give_columns(dq, which, sum, p.scale, lane);
+}
+
 // values: the value's gradient, else the key's
-template <typename T> __device__ __noinline__ void slow_key_grad(const AttentionParams& p, int j, int key_head, bool values, float* sum) {
-    const int group = p.heads_q / p.heads_k;
-    for (int c = 0; c < p.dim; ++c) sum[c] = 0.f;
+template <typename T> __device__ __noinline__ void mend_key_grad(const AttentionParams& p, int j, int key_head, bool values, int lane) {
+    T* const to = static_cast<T*>(values ? p.dv : p.dk) + ((int64_t)j * p.heads_k + key_head) * p.dim;
+    uint32_t which = spoilt_of<T>(result_of(to, p.dim, lane));
+    if (!__any_sync(~0u, which != 0u)) return;
+    const int group = p.heads_q / p.heads_k, past = past_query(p, j);
     for (int head = key_head * group; head < (key_head + 1) * group; ++head)
-        for (int i = j; i < past_query(p, j); ++i) {
-            const float prob = probability<T>(p, i, j, head, key_head, p.lse[head * p.pitch + i]);
-            if (values) {
-                add_row<T>(sum, prob, dout_row<T>(p, i, head), p.dim);
-            } else {
-                const float ds = prob * (dot<T>(dout_row<T>(p, i, head), value_row<T>(p, j, key_head), p.dim) - p.delta[head * p.pitch + i]);
-                add_row<T>(sum, ds * p.scale, query_row<T>(p, i, head), p.dim);
+        for (int i = j; i < past; i += 32) {
+            const int64_t at = head * p.pitch + min(i + lane, past - 1);
+            const bool unset = !isfinite(p.delta[at]);
+            if (__any_sync(~0u, !isfinite(p.lse[at]) || (unset && !values))) return;
+            for (uint32_t left = __ballot_sync(~0u, unset); left != 0u; left &= left - 1u) {
+                which &= ~spoilt_of<T>(result_of(dout_row<T>(p, min(i + __ffs(left) - 1, past - 1), head), p.dim, lane));
+                if (!__any_sync(~0u, which != 0u)) return;
             }
         }
-}
-template <typename T> __device__ __forceinline__ uint4 pack_row(const float* v) {
-    uint4 r;
-    r.x = pack<T>(v[0], v[1]); r.y = pack<T>(v[2], v[3]); r.z = pack<T>(v[4], v[5]); r.w = pack<T>(v[6], v[7]);
-    return r;
+    float sum[4] = {};
+    for (int head = key_head * group; head < (key_head + 1) * group; ++head)
+        for (int i = j; i < past; i += 32) {
+            const int count = min(32, past - i), own = min(i + lane, past - 1);
+            float weight = exp2f(fmaf(dot(query_row<T>(p, own, head), key_row<T>(p, j, key_head), p.dim), p.scale2, -p.lse[head * p.pitch + own]));
+            if (!values) weight *= dot(dout_row<T>(p, own, head), value_row<T>(p, j, key_head), p.dim) - p.delta[head * p.pitch + own];
+            add_rows<T>(sum, weight, count, p.dim, lane, [&](int k) { return values ? dout_row<T>(p, i + k, head) : query_row<T>(p, i + k, head); });
+        }
+    give_columns(to, which, sum, values ? 1.f : p.scale, lane);
 }
 
 // A block that gave up waits, again for a bounded time, for the loads that it still has under way; what they bring is not used.
@@ -264,16 +329,16 @@ struct ForwardJob {
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                const __grid_constant__ CUtensorMap map_o, const AttentionParams p) {
+                                                                const __grid_constant__ CUtensorMap map_o, const __grid_constant__ AttentionParams p) {
     using F = Forward<DP>;
     __shared__ uint64_t q_full[F::kQueries], q_empty[F::kQueries], k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages];
     __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], ended[2];
     __shared__ uint32_t tensor;
-    __shared__ int lost;
+    __shared__ int lost, spoilt[2];
     unsigned char* const shared = aligned_shared();
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
-        lost = 0;
+        lost = spoilt[0] = spoilt[1] = 0;
         for (int s = 0; s < F::kQueries; ++s) { barrier_init(&q_full[s], 1); barrier_init(&q_empty[s], 2); }
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&k_full[s], 1); barrier_init(&k_empty[s], 2); barrier_init(&v_full[s], 1); barrier_init(&v_empty[s], 2); }
         for (int s = 0; s < 2; ++s) {
@@ -408,10 +473,9 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             meet(1 + set, kRows);
             const bool finite = stage_row<T, DP>(mine + F::kOut, fine ? 1.f / leaving.sum : nan_value(), tile, row);
             const float lse = fine ? fmaf(leaving.top, p.scale2, log2f(leaving.sum)) : nan_value();
-            if (fine && !finite && i <= leaving.last) {
-                float values[DP];
-                slow_out<T>(p, i, leaving.head, lse, values);
-                for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
+            if (fine && i <= leaving.last) {
+                if (!isfinite(lse)) *reinterpret_cast<unsigned short*>(staged(tile, row, 0)) = (unsigned short)kFinal;
+                else if (!finite) spoilt[set] = 1;
             }
             fence_shared();
             meet(1 + set, kRows);
@@ -549,6 +613,12 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             leave();
         }
         if (row == 0) wait_stores_done();
+        meet(1 + set, kRows);
+        if (spoilt[set] != 0 && lost == 0)
+            for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
+                const ForwardJob done(p, job);
+                for (int i = done.i0[set] + warp % 4; i <= done.last[set]; i += 4) mend_out<T>(p, i, done.head[set], lane);
+            }
     }
     __syncwarp();
     fence_before();
@@ -578,12 +648,12 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
     using F = Queries<DP>;
     __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], s_empty[F::kBuffers], p_full, o_done, ended;
     __shared__ uint32_t tensor;
-    __shared__ int lost;
+    __shared__ int lost, spoilt;
     __shared__ float offs[F::kHalves][kRows];
     unsigned char* const shared = aligned_shared();
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
-        lost = 0;
+        lost = spoilt = 0;
         barrier_init(&q_full, 1);
         barrier_init(&q_empty, 1 + F::kWorkers);      // the scores' products, and the rows' reads of dO and O
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
@@ -678,7 +748,6 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
         auto leave = [&]() {
             const int i = leaving.first + row;
             const bool there = i <= leaving.last;
-            float values[DP];
             unsigned char* const tile = shared + F::kStaged;
             if (threadIdx.x == 0) wait_stores_read();
             meet(1, F::kWorkers);
@@ -686,10 +755,7 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             if (F::kHalves > 1) leaving.delta += offs[0][row] + offs[1 % F::kHalves][row];
             if (there && half == 0) p.delta[leaving.head * p.pitch + i] = fine ? leaving.delta : nan_value();
             const bool finite = stage_row<T, DP / F::kHalves>(mine + F::kOut + half * (DP / 2), fine ? p.scale : nan_value(), tile + half * kRows * 128, row);
-            if (fine && !finite && there) {
-                slow_query_grad<T>(p, i, leaving.head, leaving.lse, leaving.delta, values);
-                for (int c = half * (DP / 2); c < p.dim && c < (half + 1) * DP / F::kHalves; c += 8) *reinterpret_cast<uint4*>(staged(tile, row, c / 8)) = pack_row<T>(values + c);
-            }
+            if (!finite && there && isfinite(leaving.lse) && isfinite(leaving.delta)) spoilt = 1;
             fence_shared();
             meet(1, F::kWorkers);
             if (threadIdx.x == 0 && leaving.first <= leaving.last) {
@@ -809,6 +875,12 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
         fence_after();
         leave();
         if (threadIdx.x == 0) wait_stores_done();
+        meet(1, F::kWorkers);
+        if (spoilt != 0 && lost == 0)
+            for (int job = blockIdx.x; job < jobs; job += stride) {
+                const QueryJob done(p, job);
+                for (int i = done.i0 + half * 4 + warp % 4; i <= done.last; i += F::kWorkers / 32) mend_query_grad<T>(p, i, done.head, lane);
+            }
     }
     __syncwarp();
     fence_before();
@@ -845,11 +917,26 @@ struct KeyJob {
         end = p.end[last];
     }
     __device__ __forceinline__ int begin() const { return j0 & ~3; }               // of its queries: a multiple of 16 bytes of their statistics
-    __device__ __forceinline__ int steps(const AttentionParams& p) const {         // for one head
-        const int past = p.window > 0 ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
-        return (past - 1 - begin()) / kStream + 1;
-    }
+    __device__ __forceinline__ int past(const AttentionParams& p) const { return p.window > 0 ? (int)min((int64_t)end, (int64_t)last + p.window) : end; }
+    __device__ __forceinline__ int steps(const AttentionParams& p) const { return (past(p) - 1 - begin()) / kStream + 1; }            // for one head
 };
+
+// Queries of a step that are seen by none of the tile's keys, behind a long episode's end for instance: where they are not finite, which their lse or D is then not either, zeros take
+// their place in the second products. (Else every key of the episode would have to be worked out again.)  The first products have read them by then.  With one block to an SM the rows'
+// warps do it, else the one that multiplies: its check is ready before the probabilities, and the rows have no registers left; with two score buffers it is the chain itself (40000 tokens
+// in 4 episodes, dim 128: 2396 us there, 2314 here; 12000 in 3, dim 64, one key head: 233 there, 241 here).
+__device__ __forceinline__ bool hidden_spoilt(int x, int from, int past, const float* lse, const float* delta) { return (x < from || x >= past) && !(isfinite(lse[x]) && isfinite(delta[x])); }
+// Query x of the streamed tiles of q and dO: panels first, first + step and so on of both.
+template <int DP> __device__ __forceinline__ void clear_query(unsigned char* tiles, int x, int first, int step) {
+    for (int c = first; c < 2 * DP / 64; c += step)
+        for (int k = 0; k < 8; ++k) *reinterpret_cast<uint4*>(tiles + c * kStream * 128 + x * 128 + k * 16) = make_uint4(0u, 0u, 0u, 0u);
+}
+template <int DP, int THREADS> __device__ __noinline__ void clear_hidden(int from, int past, unsigned char* tiles, const float* lse, const float* delta, int thread) {
+    const int x = thread % kStream;
+    if (hidden_spoilt(x, from, past, lse, delta)) clear_query<DP>(tiles, x, thread / kStream, THREADS / kStream);
+    fence_shared();
+    __syncwarp();
+}
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
@@ -859,11 +946,11 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
     __shared__ uint64_t k_full, k_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], p_full, o_done, ended;
     __shared__ __align__(16) float lse[F::kStages][kStream], delta[F::kStages][kStream];
     __shared__ uint32_t tensor;
-    __shared__ int lost;
+    __shared__ int lost, spoilt;
     unsigned char* const shared = aligned_shared();
     const int warp = __shfl_sync(~0u, threadIdx.x / 32, 0), lane = threadIdx.x % 32;
     if (threadIdx.x == 0) {
-        lost = 0;
+        lost = spoilt = 0;
         barrier_init(&k_full, 1);
         barrier_init(&k_empty, 1);
         for (int s = 0; s < F::kStages; ++s) { barrier_init(&full[s], 1); barrier_init(&empty[s], 1); }
@@ -936,11 +1023,25 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         bool fine = scores();
         for (int own = job0; fine && own < jobs; own += stride) {
             const int steps = count;                    // of the job that the scores have just begun
-            for (int i = 0; i < steps; ++i, ++n) {
+            const KeyJob now(p, own);
+            const int each = steps / group;
+            for (int i = 0, m = 0; i < steps; ++i, ++n) {
                 // the other buffer's P and dS are free when the products before have ended
                 if (F::kBuffers > 1 && n > 0 && !(fine = warp_wait(&o_done, (n - 1) & 1, &lost))) break;
                 if (F::kBuffers > 1 && i + 1 < steps && !(fine = scores())) break;
+                const int i0 = now.begin() + m * kStream;
+                uint32_t clear = 0u;
+                if (F::kBuffers == 1 && (m == 0 || m + 1 == each))
+                    for (int x = lane; x < kStream; x += 32)
+                        if (hidden_spoilt(x, now.j0 - i0, now.past(p) - i0, lse[own_stage], delta[own_stage])) clear |= 1u << x / 32;
+                if (++m == each) m = 0;
                 if (!(fine = warp_wait(&p_full, n & 1, &lost))) break;
+                if (F::kBuffers == 1 && __any_sync(~0u, clear != 0u)) {
+                    for (int x = lane; x < kStream; x += 32)
+                        if (clear >> x / 32 & 1u) clear_query<DP>(shared + 2 * F::kTile + 2 * own_stage * F::kPart, x, 0, 1);
+                    fence_shared();
+                    __syncwarp();
+                }
                 fence_after();
                 const uint32_t probs = base + n % F::kBuffers * F::kScores;
                 multiply_columns<T, kStream, DP, F::kPer>(base + F::kValue, probs, part_at + (2 * own_stage + 1) * F::kPart, i != 0);
@@ -963,7 +1064,6 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         auto leave = [&]() {
             const int j = leaving.first + row;
             const bool there = j <= leaving.last;
-            float values[DP];
             if (p.split > 1) {
                 // in 32 bits where the operands were, 16 bytes at a time, rows turned against each other so that lanes meet different banks
 #pragma unroll
@@ -983,12 +1083,8 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                 unsigned char *const dv = shared + F::kStaged, *const dk = dv + F::kTile;
                 if (row == 0) wait_stores_read();
                 meet(1, kRows);
-                const bool finite[2] = {stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row), stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row)};
-                for (int which = 0; which < 2; ++which)
-                    if (fine && !finite[which] && there) {
-                        slow_key_grad<T>(p, j, leaving.head, which, values);
-                        for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(staged(which ? dv : dk, row, c / 8)) = pack_row<T>(values + c);
-                    }
+                const bool keys_finite = stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row), values_finite = stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row);
+                if (there && !(keys_finite && values_finite)) spoilt = 1;
                 fence_shared();
                 meet(1, kRows);
                 if (row == 0 && leaving.first <= leaving.last) {
@@ -999,10 +1095,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
             } else {
                 T* const to[2] = {static_cast<T*>(p.dk) + ((int64_t)j * p.heads_k + leaving.head) * p.dim, static_cast<T*>(p.dv) + ((int64_t)j * p.heads_k + leaving.head) * p.dim};
                 const bool finite = store_row<T, DP>(mine + (half ? F::kValue : F::kKey), !fine ? nan_value() : half ? 1.f : p.scale, p.dim, there ? to[half] : nullptr);
-                if (fine && !finite && there) {
-                    slow_key_grad<T>(p, j, leaving.head, half, values);
-                    for (int c = 0; c < p.dim; c += 8) *reinterpret_cast<uint4*>(to[half] + c) = pack_row<T>(values + c);
-                }
+                if (there && !finite) spoilt = 1;
             }
         };
         KeyJob next(p, job0);
@@ -1028,6 +1121,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                     fine = fine && warp_wait(&full[stage], phase, &lost) && warp_wait(&s_full[b], n / F::kBuffers & 1, &lost);
                     if (!fine) break;
                     fence_after();
+                    if (F::kBuffers > 1 && (i < now.j0 || i + kStream > now.past(p))) clear_hidden<DP, F::kWorkers>(now.j0 - i, now.past(p) - i, shared + 2 * F::kTile + 2 * stage * F::kPart, lse[stage], delta[stage], half * kRows + row);
                     uint32_t probs[F::kPer / 2], grads[F::kPer / 2];
                     const float4 *l4 = reinterpret_cast<const float4*>(lse[stage]), *d4 = reinterpret_cast<const float4*>(delta[stage]);
                     const bool all = i >= all_low && i + kStream - 1 <= all_high;
@@ -1094,6 +1188,13 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         fence_after();
         leave();
         if (row == 0) wait_stores_done();
+        meet(1, F::kWorkers);
+        if (p.split == 1 && spoilt != 0 && lost == 0)
+            for (int job = job0; job < jobs; job += stride) {
+                const KeyJob done(p, job);
+                for (int j = done.j0 + half * 4 + warp % 4; j <= done.last; j += F::kWorkers / 32)
+                    for (int which = 0; which < 2; ++which) mend_key_grad<T>(p, j, done.head, which, lane);
+            }
     }
     __syncwarp();
     fence_before();
@@ -1114,16 +1215,16 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                 sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
             }
             if (j > job.last || c >= p.dim) continue;
-            float out[4] = {sum.x, sum.y, sum.z, sum.w};
-            if (!(fmaf(sum.x, 0.f, fmaf(sum.y, 0.f, fmaf(sum.z, 0.f, sum.w * 0.f))) == 0.f) && lost == 0) {
-                float values[DP];
-                slow_key_grad<T>(p, j, job.head, which, values);
-                for (int k = 0; k < 4; ++k) out[k] = values[c + k];
-            }
+            const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+            if (!(fmaf(sum.x, 0.f, fmaf(sum.y, 0.f, fmaf(sum.z, 0.f, sum.w * 0.f))) == 0.f)) spoilt = 1;
             store<T, 4>(static_cast<T*>(which ? p.dv : p.dk) + ((int64_t)j * p.heads_k + job.head) * p.dim + c, out);
         }
         __syncwarp();
         cluster_meet();                                 // nobody leaves while others read its shared memory
+        __syncthreads();
+        if (spoilt != 0 && lost == 0)
+            for (int x = warp; x < 2 * rows; x += F::kThreads / 32)
+                if (const int j = job.j0 + rank * rows + x % rows; j <= job.last) mend_key_grad<T>(p, j, job.head, x >= rows, lane);
     }
 }
 

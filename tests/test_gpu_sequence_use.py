@@ -98,3 +98,114 @@ def test_heads_of_tiny_values_and_tiny_eps():
     # row by row, whose gradients are of very different sizes; the eps itself is 2^-24 off in 32 bits
     off, size = (dq.double() - want).abs().amax(-1), want.abs().amax(-1)
     assert torch.isfinite(dq).all() and (off <= 16 * 2.0 ** -23 * size).all()
+
+
+# ---- attention next to what is not finite --------------------------------------------------------------------------------
+import math  # noqa: E402
+
+import test_gpu_attention as A  # noqa: E402
+
+
+@pytest.mark.parametrize("dim,heads_q,heads_k", [(64, 2, 1), (128, 2, 2), (64, 8, 1), (128, 8, 1), (40, 4, 4)])
+@pytest.mark.parametrize("what", ["q", "k", "v", "do"])
+@pytest.mark.parametrize("value", [math.nan, -math.inf])
+def test_neighbours_of_a_spoilt_episode(dim, heads_q, heads_k, what, value):
+    """A whole episode spoilt, in every head and in one column: the others of its tiles are what they are without it, with heads of a group in one block and dealt out over a cluster's."""
+    plan = A._plan_of([30, 40, 200, 24, 90])
+    names = ("q", "k", "v", "do")
+    clean = dict(zip(names, (x.clone() for x in A._inputs(_gen(dim + heads_q), plan.tokens, heads_q, heads_k, dim, torch.bfloat16))))
+    spoilt = {n: x.clone() for n, x in clean.items()}
+    spoilt[what][70:270, :, 3] = value
+    A.UNIT_OF[:] = [A.UNIT[torch.bfloat16] * 2.0 ** 7, A.UNIT[torch.bfloat16]]
+    w = A._reference(*(clean[n] for n in names[:3]), plan, dim ** -0.5, None, clean["do"])
+    q, k, v = (spoilt[n].requires_grad_() for n in names[:3])
+    o = S.episode_attention(q, k, v, plan)
+    outs = [o.detach(), *torch.autograd.grad(o, [q, k, v], spoilt["do"])]
+    other = torch.ones(plan.tokens, dtype=torch.bool, device="cuda")
+    other[70:270] = False
+    for (name, (want, bound)), got in zip(A._bounds(w, A.UNIT[torch.bfloat16], 0.0).items(), outs):
+        A._close(got[other], want[other], bound[other], name)
+    # of the spoilt episode what does not meet the spoilt column is what its definition gives, too
+    if what == "v" and dim == 64:
+        columns = [c for c in range(dim) if c != 3]
+        want, bound = A._bounds(w, A.UNIT[torch.bfloat16], 0.0)["o"]
+        A._close(outs[0][..., columns], want[..., columns], bound[..., columns], "o")
+        assert not torch.isfinite(outs[0][70:270, :, 3]).any()
+    if what == "do" and dim == 64:
+        columns = [c for c in range(dim) if c != 3]
+        want, bound = A._bounds(w, A.UNIT[torch.bfloat16], 0.0)["dv"]
+        A._close(outs[3][..., columns], want[..., columns], bound[..., columns], "dv")
+        assert not torch.isfinite(outs[1][70:270]).any() and not torch.isfinite(outs[2][70:270]).any()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("what", ["k", "v", "do"])
+def test_long_episodes_beside_a_long_spoilt_one(dim, what):
+    """30000 finite tokens share tiles with 20000 spoilt ones, which 700 finite ones follow.  The last rows of the first, whose tiles are mixed, against 64 bits, all others bit for bit
+    against the call without what is spoilt; no block gives up meanwhile.  Keys' gradients take D from the outputs of the mixed rows, which have other roundings where values are
+    spoilt: twice the outputs' bound, in D and in dS's rounding, and one rounding more."""
+    lengths, hq, hk = [30000, 20000, 700], 4, 2
+    plan = A._plan_of(lengths)
+    q, k, v, do = (x.clone() for x in A._inputs(_gen(dim), plan.tokens, hq, hk, dim, torch.bfloat16))
+
+    def run(q, k, v, do):
+        a, b, c = (x.detach().requires_grad_() for x in (q, k, v))
+        o = S.episode_attention(a, b, c, plan)
+        return [o.detach(), *torch.autograd.grad(o, [a, b, c], do)]
+
+    clean = run(q, k, v, do)
+    spoilt = {"q": q.clone(), "k": k.clone(), "v": v.clone(), "do": do.clone()}
+    spoilt[what][30000:50000:7] = math.inf                  # as a loss scale that is too large leaves them
+    got = run(**spoilt)
+    near = 256                                              # a tile of 128 rows, wherever it begins
+    for n, (x, y) in enumerate(zip(got, clean)):
+        assert torch.isfinite(x[:30000]).all() and torch.isfinite(x[50000:]).all()
+        if what != "v" or n != 2:
+            assert torch.equal(x[:30000 - near], y[:30000 - near]) and torch.equal(x[50000 + near:], y[50000 + near:])
+    u, sums = A.UNIT[torch.bfloat16], A.SUMS
+    rows = torch.arange(30000 - near, 30000, device="cuda")
+    seen = torch.arange(30000, device="cuda")[None, :] <= rows[:, None]
+    for h in range(hq):
+        g = h // (hq // hk)
+        kk, vv, qq, dd = k[:30000, g].double(), v[:30000, g].double(), q[rows, h].double(), do[rows, h].double()
+        p = torch.softmax((qq @ kk.t() * dim ** -0.5).masked_fill(~seen, -math.inf), -1)
+        o, size = p @ vv, p @ vv.abs()
+        assert ((got[0][rows, h].double() - o).abs() <= u * (o.abs() + size) + sums * size).all()
+        dp, delta = dd @ vv.t(), (dd * o).sum(-1, keepdim=True)
+        ds = p * (dp - delta) * dim ** -0.5
+        # as the module's bounds: rounding of dS and of the output that D is made of, 32-bit sums
+        each = ds.abs() * u + p * (dd.abs() @ vv.abs().t() + dp.abs() + delta.abs()) * sums * dim ** -0.5 + p * (dd.abs() * o.abs()).sum(-1, keepdim=True) * u * dim ** -0.5
+        dq = ds @ kk
+        assert ((got[1][rows, h].double() - dq).abs() <= u * dq.abs() + each @ kk.abs()).all()
+    for g in range(hk):                                     # the last keys are seen by the last queries only
+        dk, dv, bk, bv = (torch.zeros(near, dim, dtype=torch.float64, device="cuda") for _ in range(4))
+        far = torch.zeros(30000, dim, dtype=torch.float64, device="cuda")
+        for h in range(g * hq // hk, (g + 1) * hq // hk):
+            kk, vv, qq, dd = k[:30000, g].double(), v[:30000, g].double(), q[rows, h].double(), do[rows, h].double()
+            p = torch.softmax((qq @ kk.t() * dim ** -0.5).masked_fill(~seen, -math.inf), -1)
+            o, size = p @ vv, p @ vv.abs()
+            dp, delta = dd @ vv.t(), (dd * o).sum(-1, keepdim=True)
+            ds = p * (dp - delta) * dim ** -0.5
+            each = ds.abs() * u + p * (dd.abs() @ vv.abs().t() + dp.abs() + delta.abs()) * sums * dim ** -0.5 + p * (dd.abs() * o.abs()).sum(-1, keepdim=True) * u * dim ** -0.5
+            last = slice(30000 - near, 30000)
+            far += (2 * u * ds.abs() + p * 2 * (dd.abs() * (u * (o.abs() + size) + sums * size)).sum(-1, keepdim=True) * dim ** -0.5).t() @ qq.abs()
+            dk += ds[:, last].t() @ qq
+            dv += p[:, last].t() @ dd
+            bk += each[:, last].t() @ qq.abs()
+            bv += p[:, last].t() @ dd.abs()
+        assert ((got[2][rows, g].double() - dk).abs() <= u * dk.abs() + bk).all()
+        assert ((got[2][:30000 - near, g].double() - clean[2][:30000 - near, g].double()).abs() <= 2 * u * clean[2][:30000 - near, g].double().abs() + far[:30000 - near]).all()
+        assert ((got[3][rows, g].double() - dv).abs() <= u * (dv.abs() + bv) + sums * bv).all()
+
+
+@pytest.mark.parametrize("dim,heads_q,heads_k", [(64, 4, 2), (128, 4, 2), (64, 8, 1)])
+def test_f16_gradients_beyond_the_range_of_its_probabilities(dim, heads_q, heads_k):
+    """dS above 65504 is an infinity in f16; the gradients that it goes into are not, and come out as exact as ever."""
+    plan = A._plan_of([3, 200, 40, 1, 600])
+    q, k, v, do = A._inputs(_gen(5), plan.tokens, heads_q, heads_k, dim, torch.float16)
+    q, k, v, do = q * 0.25, k * 0.05, v * 4, do * 4096
+    s = (q.double().transpose(0, 1) @ k.double().repeat_interleave(heads_q // heads_k, 1).permute(1, 2, 0)) * dim ** -0.5
+    p = torch.softmax(s.masked_fill(~A._seen(plan, None), -math.inf), -1)
+    dp = do.double().transpose(0, 1) @ v.double().repeat_interleave(heads_q // heads_k, 1).permute(1, 2, 0)
+    assert (p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max() > 65504
+    A._check(q, k, v, plan, do)

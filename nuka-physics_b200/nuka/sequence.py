@@ -421,14 +421,17 @@ class HistoryCache:
         _call(self.device, _abi.lib().nuka_b200_history_advance, self.position.data_ptr(), _ptr(fresh), self.position.numel())
 
     def _workspace(self, heads):
-        """(address, bytes) of what a call with this many heads needs beside the cache, zeroed once."""
+        """(address, bytes, the tensor) of what a call with this many heads needs beside the cache, zeroed once.  One that is made while a graph is captured is that call's alone: its memory is the
+        graph's, and each replay zeroes it."""
         found = self._workspaces.get(heads)
         if found is None:
             envs, capacity, heads_k, dim = self.keys.shape
             need = _abi.lib().nuka_b200_history_workspace(ctypes.byref(_abi.HistoryDesc(_DTYPES[self.keys.dtype], envs, capacity, heads, heads_k, dim)))
             kept = torch.zeros(need, dtype=torch.uint8, device=self.device)
-            found = self._workspaces[heads] = (kept.data_ptr() or None, need, kept)
-        return found[:2]
+            found = (kept.data_ptr() or None, need, kept)
+            if not torch.cuda.is_current_stream_capturing():
+                self._workspaces[heads] = found
+        return found
 
 
 def history_attention(q, k, v, cache, scale=None):
@@ -446,8 +449,9 @@ def history_attention(q, k, v, cache, scale=None):
         raise ValueError(f"q, k and v must be {dtype}, as the cache is")
     q, k, v = _channels_last(q, 8, 16), _channels_last(k, 8, 16), _channels_last(v, 8, 16)
     out = torch.empty(q.shape, dtype=dtype, device=device)
+    workspace = cache._workspace(q.shape[1])
     desc = _abi.HistoryDesc(_DTYPES[dtype], envs, capacity, q.shape[1], heads_k, dim, dim ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                             _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), cache.keys.data_ptr(), cache.values.data_ptr(),
-                            cache.position.data_ptr(), out.data_ptr(), *cache._workspace(q.shape[1]))
+                            cache.position.data_ptr(), out.data_ptr(), *workspace[:2])
     _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
     return out

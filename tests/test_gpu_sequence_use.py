@@ -209,3 +209,56 @@ def test_f16_gradients_beyond_the_range_of_its_probabilities(dim, heads_q, heads
     dp = do.double().transpose(0, 1) @ v.double().repeat_interleave(heads_q // heads_k, 1).permute(1, 2, 0)
     assert (p * (dp - (p * dp).sum(-1, keepdim=True))).abs().max() > 65504
     A._check(q, k, v, plan, do)
+
+
+# ---- graphs ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("envs,capacity", [(1, 4096), (3, 1000), (2000, 40)])
+def test_an_acting_step_in_a_graph(envs, capacity):
+    """Captured before any call of these sizes: replays give what calls give, bit for bit, and so does a call outside between the capture and the first replay."""
+    gen = _gen(3)
+    f = S.rotary_frequencies(64).cuda()
+    state, fresh = _normal(gen, envs, 96), torch.zeros(envs, dtype=torch.bool, device="cuda")
+    x, both = _normal(gen, envs, 96), _normal(gen, envs, 12, 64, dtype=torch.bfloat16)
+
+    def made():
+        cache = S.HistoryCache(envs, capacity, 2, 64)
+        cache.keys.normal_(generator=_gen(4))
+        cache.values.normal_(generator=_gen(5))
+        cache.position.copy_(torch.arange(envs, device="cuda") * 2 + capacity // 2)
+        return cache, state.clone()
+
+    def step(cache, state):
+        cache.advance(fresh)
+        h = S.gated_recurrence_step(x, x, state, fresh)
+        q, k = S.rotate_heads(both[:, :8], both[:, 8:10], None, None, cache.position, f)
+        return h, S.history_attention(q, k, both[:, 10:], cache)
+
+    def inputs(t):
+        x.copy_(torch.sin(torch.arange(x.numel(), device="cuda") + t).view_as(x))
+        both.copy_(torch.cos(torch.arange(both.numel(), device="cuda") * 0.7 + t).view_as(both))
+        fresh.copy_(torch.arange(envs, device="cuda") % 5 == t)
+
+    captured, called = made(), made()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(*made())                                       # the library is loaded, and nothing of the captured cache is used
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        out = step(*captured)
+    inputs(9)
+    q = _normal(gen, envs, 8, 64, dtype=torch.bfloat16)
+    k = _normal(gen, envs, 2, 64, dtype=torch.bfloat16)
+    here = (captured[0].keys.clone(), captured[0].values.clone(), captured[0].position.clone())
+    first, second = S.history_attention(q, k, k, captured[0]), S.history_attention(q, k, k, S.HistoryCache(envs, capacity, 2, 64, buffers=here))
+    assert torch.equal(first, second) and torch.isfinite(first).all()
+    captured[0].keys.copy_(called[0].keys)
+    captured[0].values.copy_(called[0].values)
+    for t in range(4):
+        inputs(t)
+        graph.replay()
+        want = step(*called)
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        assert torch.equal(captured[1], called[1]) and torch.equal(captured[0].keys, called[0].keys) and torch.equal(captured[0].position, called[0].position)
+    del graph

@@ -1,4 +1,5 @@
 """What nuka.sequence hands to the library and to torch, without a GPU: its calls go to a recorder in the library's place."""
+import ctypes
 import os
 import re
 
@@ -83,3 +84,21 @@ def test_the_rows_of_an_attention_kernel_meet_at_one_barrier():
         kernels = f.read().split("__global__")[1:]
     met = [set(re.findall(r"\bmeet\(([^,]*),", body)) for body in kernels]
     assert len(kernels) == 3 and all(len(m) <= 1 for m in met) and any(met), met
+
+
+def test_a_workspace_made_while_a_graph_is_captured_is_not_kept(calls, monkeypatch):
+    """Its zeroing is a node of that graph: a call outside the graph, before the first replay, would count on what nothing zeroed."""
+    q, k = torch.zeros(1, 8, 64, dtype=torch.bfloat16), torch.zeros(1, 2, 64, dtype=torch.bfloat16)
+    cache = S.HistoryCache(1, 4096, 2, 64, device="cpu")
+    zeros, capturing = torch.zeros, [True]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: capturing[0])
+    monkeypatch.setattr(torch, "zeros", lambda *a, **b: zeros(*a, **b).fill_(7) if capturing[0] else zeros(*a, **b))         # zeroed by a replay, not now
+    S.history_attention(q, k, k, cache)
+    assert calls[-1][1].workspace_bytes > 0 and calls[-1][1].workspace
+    capturing[0] = False
+    S.history_attention(q, k, k, cache)
+    outside = calls[-1][1]
+    assert ctypes.string_at(outside.workspace, outside.workspace_bytes) == bytes(outside.workspace_bytes)
+    for capturing[0] in (False, True):                     # kept from then on, by captures too
+        S.history_attention(q, k, k, cache)
+        assert calls[-1][1].workspace == outside.workspace

@@ -15,6 +15,7 @@ rollouts take part in automatic differentiation (once).  Needs torch with CUDA.
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _abi, _check
 
@@ -174,6 +175,17 @@ def _recur(x, gate, initial, episodes):
     return h, state
 
 
+def _differentiated(*tensors):
+    """Whether the call goes through its autograd function: where a gradient may be asked for, and in forward mode, which that function refuses (a tangent would be lost otherwise)."""
+    if forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                return True
+    return False
+
+
 def _once(backward):
     """Gradients that cannot be differentiated again, at no cost where nobody asks for it."""
     guarded = torch.autograd.function.once_differentiable(backward)
@@ -227,7 +239,7 @@ def gated_recurrence(x, gate, episodes, initial=None):
         if initial.shape != (episodes.rows, x.shape[1]) or initial.dtype != torch.float32:
             raise ValueError(f"initial must be {episodes.rows} x {x.shape[1]} float32 on {device}")
         initial = initial.contiguous()
-    train = torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad or (initial is not None and initial.requires_grad))
+    train = _differentiated(x, gate, initial)
     x, gate = _channels_last(x), _channels_last(gate)
     return _Recurrence.apply(x, gate, initial, episodes) if train else _recur(x, gate, initial, episodes)
 
@@ -328,8 +340,7 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     q_weight, k_weight, frequencies = (None if x is None else x.contiguous() for x in (q_weight, k_weight, frequencies))
     size = 4 * q.element_size()
     q, k = _channels_last(q, 4, size), _channels_last(k, 4, size)
-    train = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, q_weight, k_weight))
-    if not train:
+    if not _differentiated(q, k, q_weight, k_weight):
         return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)[:2]
     return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
 
@@ -388,7 +399,7 @@ def episode_attention(q, k, v, episodes, scale=None, window=None):
     _expect(k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and q.shape[1] > 0, "the heads must be a multiple of the key heads")
     _expect(window is None or window >= 1, "window must be at least 1")
     scale, window = q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window)
-    train = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+    train = _differentiated(q, k, v)
     q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
     return _Attention.apply(q, k, v, episodes, scale, window) if train else _attend(q, k, v, episodes, scale, window, False)[0]
 

@@ -102,3 +102,21 @@ def test_a_workspace_made_while_a_graph_is_captured_is_not_kept(calls, monkeypat
     for capturing[0] in (False, True):                     # kept from then on, by captures too
         S.history_attention(q, k, k, cache)
         assert calls[-1][1].workspace == outside.workspace
+
+
+@pytest.mark.parametrize("operator", list(OPERATORS))
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused_and_not_dropped(calls, operator, grad):
+    """A tangent that an operator cannot carry on is an error, with or without gradients recorded; without a tangent the call is as ever."""
+    import torch.autograd.forward_ad as fwd
+    run, make, _ = OPERATORS[operator]
+    leaves = make()
+    with fwd.dual_level(), torch.set_grad_enabled(grad):
+        run(leaves)
+        for n in range(len(leaves)):
+            duals = [fwd.make_dual(x, torch.ones_like(x)) if n == i else x for i, x in enumerate(leaves)]
+            with pytest.raises(NotImplementedError):
+                run(duals)
+    run(leaves)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda x: run([x, *leaves[1:]]), (leaves[0],), (leaves[0],))

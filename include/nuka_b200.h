@@ -412,9 +412,11 @@ nuka_result_t nuka_b200_recurrence_step(uint32_t dtype, int64_t n, int64_t chann
 /* Queries and keys of every head: divided by their root mean square over the head's dim values (mean square plus eps), times a weight
  * per column (float, NULL = 1), then turned by the token's position: of the first `turned` columns the pairs (i, i + turned / 2), or with interleaved != 0
  * (2 i, 2 i + 1), turn by the angle position x frequencies[i] radians (double, turned / 2 of them), factors
- * and product rounded to 32 bits.
+ * and product rounded to 32 bits, as programs have them that train in 32 bits: off by up to about position x 2^-24 radians.  With NUKA_B200_EXACT_ANGLES added to
+ * interleaved the product is taken in 64 bits.
  * position[t] is t - plan->first[t], or positions[t] where positions is not NULL.  dim and turned are multiples of 8, dim at most 256.
  * The backward call takes dq_out / dk_out, writes dq / dk (contiguous) and the weights' gradients (float, NULL = not wanted). */
+#define NUKA_B200_EXACT_ANGLES 0x80000000u
 typedef struct nuka_b200_heads_t {
     const int32_t* first;                           /* the plan's, or NULL with positions */
     const int32_t* positions;

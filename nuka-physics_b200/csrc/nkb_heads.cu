@@ -31,7 +31,8 @@ struct HeadsParams {
     float* partial;                                     // blocks x 2 x dim, null where no weight's gradient is wanted
 };
 
-template <typename T, int LANES, bool INTERLEAVED, bool BACKWARD>
+// EXACT: angles are products in 64 bits; a build of its own, since both forms in one cost the other's registers (49999 x 20 x 128: 346 us in place of 287)
+template <typename T, int LANES, bool INTERLEAVED, bool BACKWARD, bool EXACT>
 __global__ void __launch_bounds__(kThreads, BACKWARD ? (sizeof(T) == 4 ? 4 : 6) : sizeof(T) == 4 ? 8 : 10) heads_kernel(const HeadsParams p) {
     constexpr int TOKENS = kThreads / LANES;
     using R = Raw<T, 4>;
@@ -71,9 +72,10 @@ __global__ void __launch_bounds__(kThreads, BACKWARD ? (sizeof(T) == 4 ? 4 : 6) 
             cosine[i] = 1.f;
             sine[i] = 0.f;
             if (turns) {
-                // The angle is the product in 32 bits, as programs have it that keep it in 32 bits: what they trained fits.  Of that angle in turns, taken
+                // The angle is the product in 32 bits unless asked otherwise, as programs have it that keep it in 32 bits: what they trained fits.  Of that angle in turns, taken
                 // in 64 bits, only the fraction is kept, so its sine and cosine are exact to 32 bits however large it is.
-                double angle = (double)((float)position * (float)p.frequencies[group * 4 + i]) * 0.15915494309189533577;
+                const double frequency = p.frequencies[group * 4 + i];
+                double angle = (EXACT ? (double)position * frequency : (double)((float)position * (float)frequency)) * 0.15915494309189533577;
                 angle -= rint(angle);
                 sincospif(2.f * (float)angle, &sine[i], &cosine[i]);
             }
@@ -204,19 +206,20 @@ template <typename T, int LANES, bool INTERLEAVED> static cudaError_t run_heads(
     p.q_weight = d.q_weight; p.k_weight = d.k_weight; p.eps = d.eps; p.q_out = d.q_out; p.k_out = d.k_out;
     p.dq_out = d.dq_out; p.dk_out = d.dk_out; p.dq = d.dq; p.dk = d.dk;
     const unsigned blocks = (unsigned)blocks_of(d.tokens, d.dim, backward);
+    const bool exact = (d.interleaved & NUKA_B200_EXACT_ANGLES) != 0;
     if (!backward) {
-        heads_kernel<T, LANES, INTERLEAVED, false><<<blocks, kThreads, 0, stream>>>(p);
+        exact ? heads_kernel<T, LANES, INTERLEAVED, false, true><<<blocks, kThreads, 0, stream>>>(p) : heads_kernel<T, LANES, INTERLEAVED, false, false><<<blocks, kThreads, 0, stream>>>(p);
         return cudaGetLastError();
     }
     const bool weights = d.dq_weight != nullptr || d.dk_weight != nullptr;
     p.partial = weights ? static_cast<float*>(d.workspace) : nullptr;
-    heads_kernel<T, LANES, INTERLEAVED, true><<<blocks, kThreads, 0, stream>>>(p);
+    exact ? heads_kernel<T, LANES, INTERLEAVED, true, true><<<blocks, kThreads, 0, stream>>>(p) : heads_kernel<T, LANES, INTERLEAVED, true, false><<<blocks, kThreads, 0, stream>>>(p);
     if (weights) weight_kernel<<<dim3((unsigned)((d.dim + 31) / 32), 2), 1024, 0, stream>>>(p.partial, (int)blocks, p.dim, d.dq_weight, d.dk_weight);
     return cudaGetLastError();
 }
 
 template <typename T, int LANES> static cudaError_t run_heads(const nuka_b200_heads_t& d, bool backward, cudaStream_t stream) {
-    return d.interleaved != 0 ? run_heads<T, LANES, true>(d, backward, stream) : run_heads<T, LANES, false>(d, backward, stream);
+    return (d.interleaved & ~NUKA_B200_EXACT_ANGLES) != 0 ? run_heads<T, LANES, true>(d, backward, stream) : run_heads<T, LANES, false>(d, backward, stream);
 }
 
 template <typename T> static cudaError_t run_heads(const nuka_b200_heads_t& d, bool backward, cudaStream_t stream) {

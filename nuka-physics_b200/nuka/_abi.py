@@ -73,6 +73,9 @@ class RecurrenceDesc(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
+EXACT_ANGLES = 0x80000000                # added to HeadsDesc.interleaved
+
+
 class HeadsDesc(ctypes.Structure):
     _fields_ = [("first", ctypes.c_void_p), ("positions", ctypes.c_void_p), ("frequencies", ctypes.c_void_p), ("dtype", ctypes.c_uint32), ("interleaved", ctypes.c_uint32),
                 ("tokens", ctypes.c_int64), ("heads_q", ctypes.c_int64), ("heads_k", ctypes.c_int64), ("dim", ctypes.c_int64), ("turned", ctypes.c_int64),

@@ -272,11 +272,11 @@ def rotary_frequencies(turned, base=10000.0, trained=0, context=0, low=1.0, high
     return f
 
 
-def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
+def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs):
     device = q.device
     tokens, heads_q, dim = q.shape
     q_out, k_out = _empty(q), _empty(k)
-    desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], bool(interleaved), tokens, heads_q, k.shape[1], dim,
+    desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], pairs, tokens, heads_q, k.shape[1], dim,
                           0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
                           _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
     _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
@@ -285,8 +285,8 @@ def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interlea
 
 class _Heads(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved):
-        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, interleaved)
+    def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs):
+        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs)
         tensors = {"q": q, "k": k, "q_weight": q_weight, "k_weight": k_weight, "first": first, "positions": positions, "frequencies": frequencies}
         ctx.names = [name for name, x in tensors.items() if x is not None]
         tensors = [tensors[name] for name in ctx.names]
@@ -317,12 +317,13 @@ class _Heads(torch.autograd.Function):
         return dq, dk, dw[0], dw[1], None, None, None, None, None
 
 
-def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, interleaved=False):
+def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, interleaved=False, exact_angles=False):
     """Each head's queries and keys divided by their root mean square, times a weight per column, then turned by their position.
 
     q: tokens x heads x dim, k: tokens x key heads x dim, f32, f16 or bf16, heads and tokens at any stride (views of one projection).  q_weight, k_weight: dim f32, or None.
     positions: an ``Episodes`` (each token's number in its episode) or int32 per token.  frequencies: float64 on the GPU, one per turned pair
-    (``rotary_frequencies``; twice as many columns are turned, the others only normed), or None; the angle is their product in 32 bits.  Pairs are (i, i + turned / 2), or with `interleaved` (2 i, 2 i + 1).
+    (``rotary_frequencies``; twice as many columns are turned, the others only normed), or None; the angle is their product in 32 bits, as programs
+    have it that train in 32 bits, and off by up to about position x 2^-24 radians; with `exact_angles` it is taken in 64 bits.  Pairs are (i, i + turned / 2), or with `interleaved` (2 i, 2 i + 1).
     dim and the number of turned columns are multiples of 8, dim at most 256.  Returns (q, k), contiguous."""
     episodes = positions if isinstance(positions, Episodes) else None
     _on_gpu(q, k, q_weight, k_weight, frequencies, episodes._plan if episodes is not None else positions)
@@ -338,11 +339,11 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
         _expect(positions.dtype == torch.int32 and positions.shape == q.shape[:1], "positions must be an Episodes or int32, one per token")
         first, positions = None, positions.contiguous()
     q_weight, k_weight, frequencies = (None if x is None else x.contiguous() for x in (q_weight, k_weight, frequencies))
-    size = 4 * q.element_size()
+    size, pairs = 4 * q.element_size(), bool(interleaved) | (_abi.EXACT_ANGLES if exact_angles else 0)
     q, k = _channels_last(q, 4, size), _channels_last(k, 4, size)
     if not _differentiated(q, k, q_weight, k_weight):
-        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)[:2]
-    return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), interleaved)
+        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), pairs)[:2]
+    return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), pairs)
 
 
 # ---- attention over packed episodes --------------------------------------------------------------------------------

@@ -262,3 +262,31 @@ def test_an_acting_step_in_a_graph(envs, capacity):
         assert all(torch.equal(a, b) for a, b in zip(out, want))
         assert torch.equal(captured[1], called[1]) and torch.equal(captured[0].keys, called[0].keys) and torch.equal(captured[0].position, called[0].position)
     del graph
+
+
+# ---- angles ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("turned", [64, 24])
+def test_exact_angles(interleaved, turned):
+    """Products of position and frequency in 64 bits, forwards and backwards, at positions that 32 bits do not tell apart; without them the angle is the 32-bit product's, as documented.
+    Norm, sine and turn in 32 bits: sixteen units in the last place."""
+    gen = _gen(6)
+    f = S.rotary_frequencies(turned, base=500.0).cuda()
+    positions = torch.tensor([0, 1, 700, 50000, 131071, 2 ** 24 + 1, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    q = _normal(gen, 7, 3, 64).requires_grad_()
+    cot = _normal(gen, 7, 3, 64)
+    x = q.detach().double().requires_grad_()
+    y = x / torch.sqrt((x * x).mean(-1, keepdim=True) + 1e-6)
+    worst = []
+    for exact in (True, False):
+        angle = positions.double()[:, None, None] * f if exact else (positions.float()[:, None, None] * f.float()).double()
+        u, v = (y[..., 0:turned:2], y[..., 1:turned:2]) if interleaved else (y[..., :turned // 2], y[..., turned // 2:turned])
+        a, b = u * angle.cos() - v * angle.sin(), u * angle.sin() + v * angle.cos()
+        want = torch.cat([torch.stack([a, b], -1).flatten(-2) if interleaved else torch.cat([a, b], -1), y[..., turned:]], -1)
+        got = S.rotate_heads(q, q, None, None, positions, f, interleaved=interleaved, exact_angles=exact)[1]
+        grad, = torch.autograd.grad(got, q, cot)
+        want_grad, = torch.autograd.grad(want, x, cot.double(), retain_graph=True)
+        for g, w in ((got, want), (grad, want_grad)):
+            assert ((g.double() - w).abs() <= 16 * 2.0 ** -23 * w.abs().max()).all()
+        worst.append(got.detach())
+    assert (worst[0] - worst[1])[:3].abs().max() < 1e-3 and (worst[0] - worst[1])[3:].abs().max() > 1e-3

@@ -18,7 +18,7 @@ nuka_result_t Ran(cudaError_t e) {
 cudaStream_t StreamOf(void* s) { return static_cast<cudaStream_t>(s); }
 bool Aligned(const void* p, uint64_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0u; }
 uint64_t SizeOf(uint32_t dtype) { return dtype == NUKA_B200_F32 ? 4u : 2u; }
-constexpr int64_t kMostTokens = (1ll << 31) - 1025;     // token indices, and a chunk past them, fit 32 bits
+constexpr int64_t kMostTokens = (1ll << 31) - 1025;     // token indices, and a tile past them, fit 32 bits
 
 const char* PlanFault(const nuka_b200_episodes_t* p) {
     if (p == nullptr) return "the plan is null";
@@ -26,6 +26,8 @@ const char* PlanFault(const nuka_b200_episodes_t* p) {
     if (p->tokens != 0 && p->rows == 0) return "tokens without a row";
     if (p->length < 0 || (p->length != 0 && p->length * p->rows != p->tokens)) return "rows of one length do not give the plan's tokens";
     if (p->tokens != 0 && (p->first == nullptr || p->end == nullptr || p->link == nullptr || p->tail == nullptr)) return "an array of the plan is null";
+    for (const int32_t* a : {p->first, p->end, p->link, p->tail})
+        if (!Aligned(a, 4)) return "an array of the plan does not lie on 4 bytes";
     return nullptr;
 }
 
@@ -35,7 +37,7 @@ extern "C" {
 
 nuka_result_t nuka_b200_episodes_from_offsets(const nuka_b200_episodes_t* plan, const int32_t* offsets, void* stream) {
     if (const char* fault = PlanFault(plan)) return Invalid(fault);
-    if (plan->tokens != 0 && offsets == nullptr) return Invalid("offsets are null");
+    if (plan->tokens != 0 && (offsets == nullptr || !Aligned(offsets, 4))) return Invalid("offsets are null or not on 4 bytes");
     return Ran(nkb::launch_episodes_from_offsets(*plan, offsets, StreamOf(stream)));
 }
 
@@ -96,6 +98,8 @@ static nuka_result_t Heads(const nuka_b200_heads_t* desc, bool backward, void* s
     if (d.dim < 8 || d.dim > 256 || d.dim % 8 != 0 || d.turned < 0 || d.turned > d.dim || d.turned % 8 != 0)
         return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dim and turned must be multiples of 8, dim 8 to 256, turned at most dim");
     if (!(d.eps >= 0.f)) return Invalid("eps must not be negative");
+    if (!Aligned(d.first, 4) || !Aligned(d.positions, 4)) return Invalid("the plan's first or positions do not lie on 4 bytes");
+    if (!Aligned(d.q_weight, 4) || !Aligned(d.k_weight, 4) || (backward && (!Aligned(d.dq_weight, 4) || !Aligned(d.dk_weight, 4)))) return Invalid("a weight or its gradient does not lie on 4 bytes");
     if (d.tokens == 0) return Ran(nkb::launch_heads(d, backward, StreamOf(stream)));
     if (d.turned != 0 && (d.frequencies == nullptr || !Aligned(d.frequencies, 8))) return Invalid("frequencies are null or not on 8 bytes");
     if (d.turned != 0 && d.first == nullptr && d.positions == nullptr) return Invalid("neither the plan's first nor positions are given");
@@ -110,7 +114,6 @@ static nuka_result_t Heads(const nuka_b200_heads_t* desc, bool backward, void* s
         if (!Aligned(need[i], four) || !Aligned(out[i], four) || (backward && !Aligned(grad[i], four))) return Invalid("queries and keys must lie on multiples of four values");
         if (strides[i] < 0 || head_strides[i] < 0 || strides[i] % 4 != 0 || head_strides[i] % 4 != 0) return Invalid("strides must be multiples of four values, not negative");
     }
-    if (!Aligned(d.q_weight, 4) || !Aligned(d.k_weight, 4)) return Invalid("a weight does not lie on 4 bytes");
     if (backward && (d.dq_weight != nullptr || d.dk_weight != nullptr) &&
         (d.workspace == nullptr || !Aligned(d.workspace, 4) || d.workspace_bytes < nkb::heads_workspace(d.tokens, d.dim))) return Invalid("the workspace is null, too small or not on 4 bytes");
     return Ran(nkb::launch_heads(d, backward, StreamOf(stream)));

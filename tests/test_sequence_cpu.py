@@ -6,7 +6,7 @@ import re
 import pytest
 
 torch = pytest.importorskip("torch")
-from nuka import sequence as S  # noqa: E402
+from nuka import _abi, sequence as S  # noqa: E402
 
 
 @pytest.fixture
@@ -120,3 +120,22 @@ def test_forward_mode_is_refused_and_not_dropped(calls, operator, grad):
     run(leaves)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda x: run([x, *leaves[1:]]), (leaves[0],), (leaves[0],))
+
+
+def test_the_c_entries_refuse_addresses_that_their_loads_cannot_take():
+    """Nothing is launched, so this needs no GPU; the addresses are never read."""
+    lib, at = _abi.lib(), 1 << 20
+    plan = lambda **change: _abi.EpisodesDesc(**{**dict(first=at, end=at, link=at, tail=at, tokens=8, rows=2, length=4), **change})
+    refused = lambda code: code == _abi.INVALID_ARG and b"byte" in lib.nuka_last_error_message()
+    for name in ("first", "end", "link", "tail"):
+        odd = ctypes.byref(plan(**{name: at + 2}))
+        assert refused(lib.nuka_b200_episodes_from_offsets(odd, at, None)) and refused(lib.nuka_b200_episodes_from_done(odd, at, None))
+    assert refused(lib.nuka_b200_episodes_from_offsets(ctypes.byref(plan()), at + 2, None))
+    ok = dict(first=at, dtype=0, tokens=8, heads_q=2, heads_k=1, dim=64, turned=0, q=at, k=at, q_stride=128, q_head_stride=64, k_stride=64, k_head_stride=64, eps=1e-6, q_out=at, k_out=at,
+              dq_out=at, dk_out=at, dq=at, dk=at, workspace=at, workspace_bytes=1 << 20)
+    heads = lambda back, **change: (lib.nuka_b200_heads_backward if back else lib.nuka_b200_heads)(ctypes.byref(_abi.HeadsDesc(**{**ok, **change})), None)
+    for change in (dict(first=at + 1), dict(first=None, positions=at + 2), dict(q_weight=at + 2)):
+        assert refused(heads(False, frequencies=at, turned=64, **change)), change
+    for change in (dict(dq_weight=at + 2), dict(dk_weight=at + 1)):
+        assert refused(heads(True, **change)), change
+        assert refused(heads(True, tokens=0, **change)), change             # zeroed in their place

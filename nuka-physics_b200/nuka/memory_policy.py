@@ -98,7 +98,7 @@ class Rollout:
     def __init__(self, env, policy, memory, obs, fresh, steps):
         self.states = memory.begin_rollout()
         if fresh is not None:                       # what ended with the last rollout does not go on into this one
-            self.states = [state * ~fresh[:, None] for state in self.states]
+            self.states = [state.masked_fill(fresh[:, None], 0.0) for state in self.states]
         kept = []
         for _ in range(steps):
             mean, _ = policy.act(obs, memory, fresh)

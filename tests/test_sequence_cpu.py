@@ -1,5 +1,6 @@
 """What nuka.sequence hands to the library and to torch, without a GPU: its calls go to a recorder in the library's place."""
 import ctypes
+import math
 import os
 import re
 
@@ -139,3 +140,17 @@ def test_the_c_entries_refuse_addresses_that_their_loads_cannot_take():
     for change in (dict(dq_weight=at + 2), dict(dk_weight=at + 1)):
         assert refused(heads(True, **change)), change
         assert refused(heads(True, tokens=0, **change)), change             # zeroed in their place
+
+
+def test_a_rollout_forgets_states_that_are_not_finite():
+    """What ended with the last rollout does not go on into this one, whatever it was: acting forgets it, and so does the state that the training form begins with."""
+    from types import SimpleNamespace
+    from nuka import memory_policy as M
+    state = torch.tensor([[1.0, math.nan], [math.inf, 2.0], [3.0, 4.0]])
+    fresh = torch.tensor([True, True, False])
+    memory = SimpleNamespace(begin_rollout=lambda: [state.clone(), state.clone()])
+    policy = SimpleNamespace(act=lambda obs, memory, fresh: (torch.zeros(3, 2), torch.zeros(3)), log_std=torch.zeros(2))
+    env = SimpleNamespace(step=lambda action: (torch.zeros(3, 4), torch.zeros(3), None, None, {"done": torch.zeros(3, dtype=torch.bool)}))
+    rollout = M.Rollout(env, policy, memory, torch.zeros(3, 4), fresh, 2)
+    for kept in rollout.states:
+        assert torch.equal(kept, torch.tensor([[0.0, 0.0], [0.0, 0.0], [3.0, 4.0]]))

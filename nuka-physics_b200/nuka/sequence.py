@@ -47,15 +47,17 @@ def _dtype(tensor, allowed, what):
 
 
 def _call(device, function, *args):
-    """One call of the library on torch's current stream of `device`."""
+    """One call of the library on torch's current stream of `device`, which it returns."""
     index = device.index
+    stream = torch.cuda.current_stream(index).cuda_stream
     if torch.cuda.current_device() != index:
         with torch.cuda.device(device):
-            code = function(*args, torch.cuda.current_stream(index).cuda_stream)
+            code = function(*args, stream)
     else:
-        code = function(*args, torch.cuda.current_stream(index).cuda_stream)
+        code = function(*args, stream)
     if code:
         _check(code)
+    return stream
 
 
 def _ptr(tensor):
@@ -121,7 +123,7 @@ class Episodes:
         device = _on_gpu(offsets)
         offsets = offsets.contiguous()
         plan = cls(tokens, offsets.numel() - 1, 0, device)
-        _call(device, _abi.lib().nuka_b200_episodes_from_offsets, plan._ref, offsets.data_ptr())
+        plan._stream = _call(device, _abi.lib().nuka_b200_episodes_from_offsets, plan._ref, offsets.data_ptr())
         return plan
 
     @classmethod
@@ -132,8 +134,13 @@ class Episodes:
         device = _on_gpu(done)
         done = _flags(done, done.shape, device, "done")
         plan = cls(done.numel(), done.shape[0], done.shape[1], device)
-        _call(device, _abi.lib().nuka_b200_episodes_from_done, plan._ref, done.data_ptr())
+        plan._stream = _call(device, _abi.lib().nuka_b200_episodes_from_done, plan._ref, done.data_ptr())
         return plan
+
+    def _read_on(self, stream):
+        """A call on `stream` reads the plan: its memory is kept from other use until that call has ended, wherever the plan was made."""
+        if stream != self._stream:
+            self._plan.record_stream(torch.cuda.current_stream(self.device))
 
     @property
     def first(self):
@@ -171,7 +178,7 @@ def _recur(x, gate, initial, episodes):
     workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), state.data_ptr(),
                                None, None, None, None, None, _ptr(workspace), need)
-    _call(device, lib.nuka_b200_recurrence, ctypes.byref(desc))
+    episodes._read_on(_call(device, lib.nuka_b200_recurrence, ctypes.byref(desc)))
     return h, state
 
 
@@ -221,7 +228,7 @@ class _Recurrence(torch.autograd.Function):
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         desc = _abi.RecurrenceDesc(episodes._ref, dtype, channels, x.data_ptr(), gate.data_ptr(), _stride(x, 0), _stride(gate, 0), _ptr(initial), h.data_ptr(), None,
                                    dh.data_ptr(), _ptr(dstate), dx.data_ptr(), dgate.data_ptr(), _ptr(dinitial), _ptr(workspace), need)
-        _call(device, lib.nuka_b200_recurrence_backward, ctypes.byref(desc))
+        episodes._read_on(_call(device, lib.nuka_b200_recurrence_backward, ctypes.byref(desc)))
         return dx, dgate, dinitial, None
 
 
@@ -272,26 +279,28 @@ def rotary_frequencies(turned, base=10000.0, trained=0, context=0, low=1.0, high
     return f
 
 
-def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs):
+def _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs, episodes):
     device = q.device
     tokens, heads_q, dim = q.shape
     q_out, k_out = _empty(q), _empty(k)
     desc = _abi.HeadsDesc(_ptr(first), _ptr(positions), _ptr(frequencies), _DTYPES[q.dtype], pairs, tokens, heads_q, k.shape[1], dim,
                           0 if frequencies is None else 2 * frequencies.numel(), q.data_ptr(), k.data_ptr(), _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1),
                           _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr())
-    _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
+    stream = _call(device, _abi.lib().nuka_b200_heads, ctypes.byref(desc))
+    if episodes is not None:
+        episodes._read_on(stream)
     return q_out, k_out, desc
 
 
 class _Heads(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs):
-        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs)
+    def forward(ctx, q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs, episodes):
+        q_out, k_out, desc = _turn(q, k, q_weight, k_weight, first, positions, frequencies, eps, pairs, episodes)
         tensors = {"q": q, "k": k, "q_weight": q_weight, "k_weight": k_weight, "first": first, "positions": positions, "frequencies": frequencies}
         ctx.names = [name for name, x in tensors.items() if x is not None]
         tensors = [tensors[name] for name in ctx.names]
         ctx.save_for_backward(*tensors)
-        ctx.desc, ctx.strides = desc, [x.stride() for x in tensors]
+        ctx.desc, ctx.strides, ctx.episodes = desc, [x.stride() for x in tensors], episodes
         ctx.set_materialize_grads(False)
         return q_out, k_out
 
@@ -313,8 +322,10 @@ class _Heads(torch.autograd.Function):
         workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         desc.dq_out, desc.dk_out, desc.dq, desc.dk = dq_out.data_ptr(), dk_out.data_ptr(), dq.data_ptr(), dk.data_ptr()
         desc.dq_weight, desc.dk_weight, desc.workspace, desc.workspace_bytes = _ptr(dw[0]), _ptr(dw[1]), _ptr(workspace), need
-        _call(device, lib.nuka_b200_heads_backward, ctypes.byref(desc))
-        return dq, dk, dw[0], dw[1], None, None, None, None, None
+        stream = _call(device, lib.nuka_b200_heads_backward, ctypes.byref(desc))
+        if ctx.episodes is not None:
+            ctx.episodes._read_on(stream)
+        return dq, dk, dw[0], dw[1], None, None, None, None, None, None
 
 
 def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, interleaved=False, exact_angles=False):
@@ -342,8 +353,8 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     size, pairs = 4 * q.element_size(), bool(interleaved) | (_abi.EXACT_ANGLES if exact_angles else 0)
     q, k = _channels_last(q, 4, size), _channels_last(k, 4, size)
     if not _differentiated(q, k, q_weight, k_weight):
-        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), pairs)[:2]
-    return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), pairs)
+        return _turn(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), pairs, episodes)[:2]
+    return _Heads.apply(q, k, q_weight, k_weight, first, positions, frequencies, float(eps), pairs, episodes)
 
 
 # ---- attention over packed episodes --------------------------------------------------------------------------------
@@ -355,7 +366,7 @@ def _attend(q, k, v, episodes, scale, window, train):
     lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device) if train else None
     desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
                               _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
-    _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
+    episodes._read_on(_call(device, lib.nuka_b200_attention, ctypes.byref(desc)))
     return out, lse, desc
 
 
@@ -381,7 +392,7 @@ class _Attention(torch.autograd.Function):
         dq, dk, dv = _empty(tensors[0]), _empty(tensors[1]), _empty(tensors[2])
         delta = _empty(lse)
         desc.dout, desc.delta, desc.dq, desc.dk, desc.dv = dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        _call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc))
+        ctx.episodes._read_on(_call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc)))
         return dq, dk, dv, None, None, None
 
 
@@ -433,14 +444,14 @@ class HistoryCache:
         _call(self.device, _abi.lib().nuka_b200_history_advance, self.position.data_ptr(), _ptr(fresh), self.position.numel())
 
     def _workspace(self, heads):
-        """(address, bytes, the tensor) of what a call with this many heads needs beside the cache, zeroed once.  One that is made while a graph is captured is that call's alone: its memory is the
+        """[address, bytes, the tensor, its stream] of what a call with this many heads needs beside the cache, zeroed once.  One that is made while a graph is captured is that call's alone: its memory is the
         graph's, and each replay zeroes it."""
         found = self._workspaces.get(heads)
         if found is None:
             envs, capacity, heads_k, dim = self.keys.shape
             need = _abi.lib().nuka_b200_history_workspace(ctypes.byref(_abi.HistoryDesc(_DTYPES[self.keys.dtype], envs, capacity, heads, heads_k, dim)))
             kept = torch.zeros(need, dtype=torch.uint8, device=self.device)
-            found = (kept.data_ptr() or None, need, kept)
+            found = [kept.data_ptr() or None, need, kept, None]             # the stream: the first call's, which comes next
             if not torch.cuda.is_current_stream_capturing():
                 self._workspaces[heads] = found
         return found
@@ -465,5 +476,9 @@ def history_attention(q, k, v, cache, scale=None):
     desc = _abi.HistoryDesc(_DTYPES[dtype], envs, capacity, q.shape[1], heads_k, dim, dim ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                             _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), cache.keys.data_ptr(), cache.values.data_ptr(),
                             cache.position.data_ptr(), out.data_ptr(), *workspace[:2])
-    _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
+    stream = _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
+    if workspace[3] is None:
+        workspace[3] = stream
+    elif workspace[1] and stream != workspace[3]:
+        workspace[2].record_stream(torch.cuda.current_stream(device))
     return out

@@ -290,3 +290,41 @@ def test_exact_angles(interleaved, turned):
             assert ((g.double() - w).abs() <= 16 * 2.0 ** -23 * w.abs().max()).all()
         worst.append(got.detach())
     assert (worst[0] - worst[1])[:3].abs().max() < 1e-3 and (worst[0] - worst[1])[3:].abs().max() > 1e-3
+
+
+# ---- streams ---------------------------------------------------------------------------------------------------------------
+def test_plans_and_workspaces_outlive_calls_on_other_streams():
+    """Memory that belongs to a plan or a cache alone is not handed out again while a call on a stream other than its own may still read it."""
+    q = _normal(_gen(7), 4000, 2, 64, dtype=torch.bfloat16)
+    f = S.rotary_frequencies(64).cuda()
+    x = _normal(_gen(8), 4000, 40)
+    calls = {"attention": lambda plan: S.episode_attention(q, q, q, plan), "recurrence": lambda plan: S.gated_recurrence(x, x, plan), "heads": lambda plan: S.rotate_heads(q, q, None, None, plan, f)}
+    side = torch.cuda.Stream()
+    for name, call in calls.items():
+        want = call(_plan_of([1500, 2500]))
+        plan = _plan_of([1500, 2500])
+        at, size = plan._plan.data_ptr(), plan._plan.numel()
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(20_000_000)                   # about 10 ms
+            got = call(plan)
+        del plan
+        taken = [torch.empty(size, dtype=torch.int32, device="cuda") for _ in range(8)]
+        assert not side.query() and all(t.data_ptr() != at for t in taken), name
+        torch.cuda.synchronize()
+        for a, b in zip(got, want) if isinstance(got, tuple) else ((got, want),):
+            assert torch.equal(a, b)
+    cache = S.HistoryCache(1, 4096, 2, 64)
+    first = S.history_attention(q[:1], q[:1], q[:1], cache)
+    (_, size, kept, _), = cache._workspaces.values()
+    at = kept.data_ptr()
+    del kept
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(20_000_000)
+        again = S.history_attention(q[:1], q[:1], q[:1], cache)
+    cache._workspaces.clear()
+    taken = [torch.empty(size, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    assert not side.query() and all(t.data_ptr() != at for t in taken)
+    torch.cuda.synchronize()
+    assert torch.equal(first, again)

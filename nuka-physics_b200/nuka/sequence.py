@@ -409,6 +409,7 @@ def episode_attention(q, k, v, episodes, scale=None, window=None):
         _tokens_of(x, episodes, 3, what)
     _expect(k.dtype == q.dtype and v.dtype == q.dtype and k.shape == v.shape and k.shape[2] == q.shape[2], "q, k and v must be of one type and dim, k and v of one shape")
     _expect(k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and q.shape[1] > 0, "the heads must be a multiple of the key heads")
+    _expect(q.shape[2] > 0, "heads must have columns")
     _expect(window is None or window >= 1, "window must be at least 1")
     scale, window = q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window)
     train = _differentiated(q, k, v)

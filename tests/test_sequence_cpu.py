@@ -154,3 +154,9 @@ def test_a_rollout_forgets_states_that_are_not_finite():
     rollout = M.Rollout(env, policy, memory, torch.zeros(3, 4), fresh, 2)
     for kept in rollout.states:
         assert torch.equal(kept, torch.tensor([[0.0, 0.0], [0.0, 0.0], [3.0, 4.0]]))
+
+
+def test_heads_without_columns_are_refused(calls):
+    q = torch.zeros(10, 2, 0, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        S.episode_attention(q, q, q, _plan())

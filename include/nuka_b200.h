@@ -385,7 +385,8 @@ nuka_result_t nuka_b200_episodes_from_done(const nuka_b200_episodes_t* plan, con
 
 /* The gated linear recurrence h_t = a_t h_{t-1} + (1 - a_t) x_t, a_t = sigmoid(gate_t), channel by channel.  An episode that begins
  * inside a row begins from 0, a row begins from initial (rows x channels float, NULL = 0).  state (rows x channels float) receives
- * h of each row's last token before it is rounded; empty rows are left as they are. */
+ * h of each row's last token before it is rounded; empty rows are left as they are.  The gate's gradient is formed from h as it was returned: where a 16-bit h is close to x, their
+ * difference is mostly h's rounding. */
 typedef struct nuka_b200_recurrence_t {
     const nuka_b200_episodes_t* plan;
     uint32_t dtype;                                 /* of x, gate, h, dh, dx, dgate */
@@ -462,7 +463,7 @@ nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, vo
 
 /* Attention of one token of each env over the env's cached history, for acting.  keys and values (envs x capacity x heads_k x dim, contiguous, on 16 bytes) are a
  * ring: the token's k and v are written to place position % capacity, then the token attends to the last min(position + 1, capacity) tokens, itself among
- * them: what nuka_b200_attention gives with window = capacity.  position[env]: the token's number in its episode (below 0 counts as 0).  Types, dims, strides and the heads'
+ * them: what nuka_b200_attention gives with window = capacity, probabilities rounded to the type of q as there.  position[env]: the token's number in its episode (below 0 counts as 0).  Types, dims, strides and the heads'
  * groups as in nuka_b200_attention; strides may also be 0.  The workspace (nuka_b200_history_workspace() bytes on 16 bytes, 0 bytes where an env is one block's work) is zeroed
  * once by the caller and kept for all later calls of these sizes; calls that share it, or a cache, must not run at the same time. */
 typedef struct nuka_b200_history_t {

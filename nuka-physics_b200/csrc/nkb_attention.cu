@@ -18,10 +18,10 @@
 //
 // Measured, bf16, causal (8 heads, 2 of keys):
 //                                                           forwards    queries     keys
-//   98304 tokens in rows of 24, dim 64                         80 us      111         99        252 MB of inputs and outputs forwards: 3.1 TB/s
-//   20011 tokens in 40 episodes, dim 64                        49          54         93
-//   16384 tokens, one episode, dim 128                        468          --         --        550 GFLOP of visible pairs: 1.17 PFLOP/s
-//   40000 tokens in 4 episodes, dim 128                       825        1220       2344        0.99, 1.01 and 0.70 PFLOP/s of visible pairs
+//   98304 tokens in rows of 24, dim 64                         73 us      106        100        252 MB of inputs and outputs forwards: 3.4 TB/s
+//   20011 tokens in 40 episodes, dim 64                        61          71        115
+//   16384 tokens, one episode, dim 128                        435          --         --        550 GFLOP of visible pairs: 1.26 PFLOP/s
+//   40000 tokens in 4 episodes, dim 128                       790        1200       2315        1.04, 1.02 and 0.71 PFLOP/s of visible pairs
 // Long episodes are bound by the chain of a step, scores to exponentials to product, that each tile walks through: the tensor cores are busy for half of it.
 // Short rows are bound by the same chain once a tile, with its loads and its rows' way out around it: 128 rows see 24 keys each, and a tile's product is
 // mostly mask, so there neither the bytes nor the products are near their limits.
@@ -633,7 +633,7 @@ template <int DP> struct Queries {
     // one block to an SM has columns for two steps' scores, the next ones multiplied while the present ones are worked on; where two share the SM, the other block's work goes on meanwhile
     static constexpr int kBlocks = DP == 64 ? 2 : 1, kBuffers = DP == 64 ? 1 : 2, kColumns = 512 / kBlocks;
     static constexpr int kStages = DP == 64 ? 2 : 3;
-    // threads of a row, with one block to an SM two, each with half of a step's columns (40000 tokens in 4 episodes, 8 heads, 2 of keys: 1309 us with one, 1220 so; keys' 2751 and 2344)
+    // threads of a row, with one block to an SM two, each with half of a step's columns (40000 tokens in 4 episodes, 8 heads, 2 of keys: 1309 us with one, 1220 with two; keys' 2751 and 2344)
     static constexpr int kHalves = DP == 64 ? 1 : 2, kWorkers = kHalves * kRows, kThreads = kBlock + kWorkers - kRows, kPer = kStream / kHalves;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
     // queries, dO and, for D = dO . O, O; steps of keys and values; the rows that leave
@@ -899,7 +899,7 @@ template <int DP> struct Keys {
     // one block to an SM has columns for two steps' scores; P and dS take their scores' place
     static constexpr int kBlocks = DP == 64 ? 2 : 1, kBuffers = DP == 64 ? 1 : 2, kColumns = 512 / kBlocks;
     static constexpr int kStages = DP == 64 ? 2 : 4;
-    // threads of a row, with one block to an SM two, each with half of a step's columns (40000 tokens in 4 episodes, 8 heads, 2 of keys: 1309 us with one, 1220 so; keys' 2751 and 2344)
+    // threads of a row, with one block to an SM two, each with half of a step's columns (40000 tokens in 4 episodes, 8 heads, 2 of keys: 1309 us with one, 1220 with two; keys' 2751 and 2344)
     static constexpr int kHalves = DP == 64 ? 1 : 2, kWorkers = kHalves * kRows, kThreads = kBlock + kWorkers - kRows, kPer = kStream / kHalves;
     static constexpr int kTile = kRows * DP * 2, kPart = kStream * DP * 2;
     static constexpr int kStaged = 2 * kTile + 2 * kStages * kPart, kShared = kStaged + (DP == 64 ? 2 * kTile : 0) + 1024;         // rows of wide heads leave without a staged tile

@@ -10,9 +10,9 @@ namespace nkb {
 // the turned part and their partners in the second, so that no value crosses lanes and a lane works out the sines and cosines of its four pairs once for all heads of the token;
 // columns behind the turned part lie as they are.
 //
-// Measured: 98304 tokens x 10 heads x 64, bf16, 60 us forwards (4.2 TB/s of its bytes) and 109 back (3.5 TB/s); 49999 x 20 x 128, f16, 106 us (4.8 TB/s) and 178 (4.3 TB/s).
-// A value costs some ten instructions forwards and sixteen back, 2.9 and 2.5 of which are issued a cycle and SM (of 4), and the memory is 40 % busy: more of either the instructions do not
-// leave.  Two values to an instruction need registers that are not there (128 and 204 us back).
+// Measured: 98304 tokens x 10 heads x 64, bf16, 63 us forwards (4.0 TB/s of its bytes) and 112 back (3.4 TB/s); 49999 x 20 x 128, f16, 108 us (4.7 TB/s) and 168 (4.6 TB/s).
+// A value costs some ten instructions forwards and sixteen back, 2.9 and 2.5 of which are issued a cycle and SM (of 4), and the memory is 40 % busy: forwards the instructions leave no more of
+// it, backwards the rows ahead, which fill the registers, leave 35 % of the warps' places in use.  Two values to an instruction need registers that are not there (128 and 204 us back).
 constexpr int kThreads = 128;
 constexpr int64_t kBlocksBack = 6 * 148;                // at most: they take their tokens in turn, and the weights' partial sums are as many
 

@@ -108,7 +108,8 @@ struct RecurrenceParams {
     uint32_t tiles;
 };
 
-// 1 / (1 + exp(-g)) and 1 minus it, each without cancellation.  16-bit inputs and outputs leave the fast form's 2^-21 far below their rounding; its clamp
+// 1 / (1 + exp(-g)) and 1 minus it, each without cancellation.  16-bit inputs and outputs leave the fast form's error, 2^-21 for small gates and, from the exponent's rounding, |g| 2^-24 for
+// large ones (2^-20.5 at 11, 2^-17.7 at 80), far below their rounding; its clamp
 // keeps exp(-g) finite, so that the product is 1 and not inf * 0 where the gate is closed.
 template <bool EXACT> __device__ __forceinline__ void sigmoid(float g, float& a, float& rest) {
     if (EXACT) {
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(kWalkers * 32, 4) recurrence_kernel(const Recu
                     }
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) {
-                        const float grad = h[v] + dv[v];
+                        const float grad = h[v] + dv[v];        // `before` was rounded to T: in 16 bits, where it is close to x, the difference below is mostly that
                         dx[v] = rest[v] * grad;
                         dg[v] = dx[v] * (before[v] - xv[v]) * a[v];
                         h[v] = a[v] * grad;

@@ -237,7 +237,8 @@ def gated_recurrence(x, gate, episodes, initial=None):
 
     x, gate: tokens x channels, f32, f16 or bf16.  initial: rows x channels f32, the state that each row begins with (the one its env had
     when the rollout began), None for 0; an episode that begins inside a row begins with 0.  Returns (h, state): h like x, state (rows x channels f32) the
-    state that each row ends with, not rounded."""
+    state that each row ends with, not rounded.  States and sums are in 32 bits; the gate's gradient is formed from the returned h, so where a 16-bit h is close to x it is off by
+    half a unit of h times its factor."""
     device = _on_gpu(x, gate, initial, episodes._plan)
     _dtype(x, _DTYPES, "x")
     _tokens_of(x, episodes, 2, "x")
@@ -332,7 +333,7 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
     """Each head's queries and keys divided by their root mean square, times a weight per column, then turned by their position.
 
     q: tokens x heads x dim, k: tokens x key heads x dim, f32, f16 or bf16, heads and tokens at any stride (views of one projection).  q_weight, k_weight: dim f32, or None.
-    positions: an ``Episodes`` (each token's number in its episode) or int32 per token.  frequencies: float64 on the GPU, one per turned pair
+    positions: an ``Episodes`` (each token's number in its episode) or int32 per token.  frequencies: float64 on the GPU, one per turned pair, no gradient
     (``rotary_frequencies``; twice as many columns are turned, the others only normed), or None; the angle is their product in 32 bits, as programs
     have it that train in 32 bits, and off by up to about position x 2^-24 radians; with `exact_angles` it is taken in 64 bits.  Pairs are (i, i + turned / 2), or with `interleaved` (2 i, 2 i + 1).
     dim and the number of turned columns are multiples of 8, dim at most 256.  Returns (q, k), contiguous."""
@@ -402,7 +403,7 @@ def episode_attention(q, k, v, episodes, scale=None, window=None):
     q: tokens x heads x dim, k and v: tokens x key heads x dim, f16 or bf16, tokens and heads at any stride (views of one projection); the heads are a multiple
     of the key heads, and as many heads share one key head.  dim: a multiple of 8, at most 128 (64 and 128 waste nothing).  scale: dim^-0.5 unless given.
     Returns tokens x heads x dim.  Sums and statistics are in 32 bits; probabilities and, backwards, their gradients are rounded to the inputs' type, so train in f16 with a
-    loss scale."""
+    loss scale. Gradients of a row whose probabilities' gradients leave f16's range are worked out in 32 bits, slowly."""
     _on_gpu(q, k, v, episodes._plan)
     _dtype(q, (torch.float16, torch.bfloat16), "q")
     for x, what in ((q, "q"), (k, "k"), (v, "v")):
@@ -461,7 +462,7 @@ class HistoryCache:
 def history_attention(q, k, v, cache, scale=None):
     """Attention of one token of each env over what `cache` holds of its episode, the token itself among it: what ``episode_attention`` gives for the
     episode's last token, with the cache's capacity as the window.  q: envs x heads x dim, k and v: envs x key heads x dim, in the cache's type, at any stride; k and v are
-    written into the cache.  scale: dim^-0.5 unless given.  Returns envs x heads x dim.  No gradient."""
+    written into the cache.  scale: dim^-0.5 unless given.  Returns envs x heads x dim.  Probabilities are rounded to the cache's type, sums are in 32 bits.  No gradient."""
     device = _on_gpu(q, k, v, cache.keys)
     envs, capacity, heads_k, dim = cache.keys.shape
     dtype = cache.keys.dtype

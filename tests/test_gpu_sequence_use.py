@@ -328,3 +328,42 @@ def test_plans_and_workspaces_outlive_calls_on_other_streams():
     assert not side.query() and all(t.data_ptr() != at for t in taken)
     torch.cuda.synchronize()
     assert torch.equal(first, again)
+
+
+def test_two_threads_differentiate_one_graph():
+    """A retained graph, differentiated by two threads at once, each on its stream with gradients of its own: what each gets alone."""
+    import threading
+    plan = _plan_of([700, 1300])
+    f = S.rotary_frequencies(64).cuda()
+    q, k, v = (_normal(_gen(9 + n), 2000, 2, 64, dtype=torch.bfloat16).requires_grad_() for n in range(3))
+    out = S.episode_attention(*S.rotate_heads(q, k, None, None, plan, f), v, plan)
+    cots = [_normal(_gen(20 + n), 2000, 2, 64, dtype=torch.bfloat16) for n in range(2)]
+    want = [torch.autograd.grad(out, [q, k, v], c, retain_graph=True) for c in cots]
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(n):
+        for _ in range(20):
+            got[n].append(torch.autograd.grad(out, [q, k, v], cots[n], retain_graph=True))
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for n in range(2):
+        assert len(got[n]) == 20 and all(torch.equal(a, b) for g in got[n] for a, b in zip(g, want[n]))
+
+
+@pytest.mark.parametrize("rows,length", [(1, 131071), (3, 40000)])
+def test_plans_of_very_long_rows(rows, length):
+    done = torch.rand((rows, length), generator=_gen(11), device="cuda") < 2e-4
+    plan = S.Episodes.from_done(done)
+    d = done.cpu()
+    at = torch.arange(rows * length, dtype=torch.int32).view(rows, length)
+    begins = torch.cat([torch.ones(rows, 1, dtype=torch.bool), d[:, :-1]], 1)
+    first = torch.where(begins, at, 0).cummax(1).values
+    ends = torch.cat([d[:, :-1], torch.ones(rows, 1, dtype=torch.bool)], 1)
+    end = torch.where(ends, at + 1, 2 ** 31 - 1).flip(1).cummin(1).values.flip(1)
+    assert torch.equal(plan.first.cpu(), first.flatten()) and torch.equal(plan.end.cpu(), end.flatten())

@@ -751,9 +751,9 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             unsigned char* const tile = shared + F::kStaged;
             if (threadIdx.x == 0) wait_stores_read();
             meet(1, F::kWorkers);
-            // the row's other thread has its part of D; where the block gave up, the keys' gradients become NaN by it
+            // the row's other thread has its part of D, unless it gave up, which `lost` then says; the keys' gradients become NaN by D
             if (F::kHalves > 1) leaving.delta += offs[0][row] + offs[1 % F::kHalves][row];
-            if (there && half == 0) p.delta[leaving.head * p.pitch + i] = fine ? leaving.delta : nan_value();
+            if (there && half == 0) p.delta[leaving.head * p.pitch + i] = fine && lost == 0 ? leaving.delta : nan_value();
             const bool finite = stage_row<T, DP / F::kHalves>(mine + F::kOut + half * (DP / 2), fine ? p.scale : nan_value(), tile + half * kRows * 128, row);
             if (!finite && there && isfinite(leaving.lse) && isfinite(leaving.delta)) spoilt = 1;
             fence_shared();

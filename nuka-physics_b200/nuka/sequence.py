@@ -108,7 +108,7 @@ class Episodes:
 
     def __init__(self, tokens, rows, length, device):
         self.tokens, self.rows, self.device = int(tokens), int(rows), torch.device(device)
-        self._rows_may_be_empty = length == 0
+        self._rows_may_be_empty, self._stream = length == 0, None
         self._plan = torch.empty((4, self.tokens), dtype=torch.int32, device=device)
         base, step = self._plan.data_ptr(), 4 * self.tokens
         self._desc = _abi.EpisodesDesc(base, base + step, base + 2 * step, base + 3 * step, self.tokens, self.rows, length)

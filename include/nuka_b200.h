@@ -410,6 +410,79 @@ nuka_result_t nuka_b200_recurrence_backward(const nuka_b200_recurrence_t* desc, 
 nuka_result_t nuka_b200_recurrence_step(uint32_t dtype, int64_t n, int64_t channels, const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
                                         const uint8_t* fresh, float* state, void* h, void* stream);
 
+/* The short causal convolution over the plan's episodes, channel by channel: y_t = bias + sum over j of weight[c][j] x_{t - width + 1 + j}, with silu != 0 times its logistic function.  Inputs before an
+ * episode are 0; before a row's first token they are initial (rows x (width - 1) x channels, the latest last, NULL = 0).  state (like initial) receives the last width - 1 inputs of each row's last episode;
+ * empty rows are left as they are.  width is 2, 3 or 4. */
+typedef struct nuka_b200_convolution_t {
+    const nuka_b200_episodes_t* plan;
+    uint32_t dtype, silu;                           /* dtype: of x, initial, y, state and their gradients */
+    int64_t channels, width;
+    const void* x;
+    int64_t x_stride;                               /* between tokens */
+    const float *weight, *bias;                     /* channels x width, and channels (NULL = 0) */
+    const void* initial;
+    void *y, *state;                                /* y: tokens x channels */
+    const void *dy, *dstate;                        /* the rest in the backward call only; dstate: NULL = 0 */
+    void *dx, *dinitial;                            /* dinitial: NULL = not wanted; empty rows are left as they are */
+    float *dweight, *dbias;                         /* NULL = not wanted */
+    void* workspace;                                /* nuka_b200_convolution_workspace() bytes, needed where a weight's or the bias's gradient is wanted */
+    uint64_t workspace_bytes;
+} nuka_b200_convolution_t;
+uint64_t nuka_b200_convolution_workspace(const nuka_b200_episodes_t* plan, int64_t channels, int64_t width);
+nuka_result_t nuka_b200_convolution(const nuka_b200_convolution_t* desc, void* stream);
+nuka_result_t nuka_b200_convolution_backward(const nuka_b200_convolution_t* desc, void* stream);
+/* Its form for one token of each env: state (envs x (width - 1) x channels, contiguous) is updated in place; envs with fresh[i] != 0 (NULL = none) begin from 0. */
+typedef struct nuka_b200_convolution_step_t {
+    uint32_t dtype, silu;
+    int64_t envs, channels, width;
+    const void* x;
+    int64_t x_stride;                               /* between envs */
+    const float *weight, *bias;
+    const uint8_t* fresh;
+    void *state, *y;                                /* y: envs x channels */
+} nuka_b200_convolution_step_t;
+nuka_result_t nuka_b200_convolution_step(const nuka_b200_convolution_step_t* desc, void* stream);
+
+/* The selective scan over the plan's episodes: dt = softplus(delta + delta_bias), h_t[c][n] = exp(dt decay[c][n]) h_{t-1}[c][n] + dt x b_t[n], y = sum over n of c_t[n] h_t[c][n] + skip[c] x, times
+ * gate / (1 + exp(-gate)) where a gate is given.  An episode that begins inside a row begins from 0, a row from initial (rows x channels x states, NULL = 0).  state (like initial) receives the h that each
+ * row ends with; empty rows are left as they are.  1 to 64 states.  Everything of dtype is rounded once, when it is written; rates, states and sums are in 32 bits. */
+typedef struct nuka_b200_scan_t {
+    const nuka_b200_episodes_t* plan;
+    uint32_t dtype;                                 /* of x, delta, gate, b, c, y and their gradients */
+    int64_t channels, states;
+    const void *x, *delta, *gate;                   /* tokens x channels; gate may be NULL */
+    const void *b, *c;                              /* tokens x states */
+    int64_t x_stride, delta_stride, gate_stride, b_stride, c_stride;         /* between tokens */
+    const float *decay, *skip, *delta_bias;         /* channels x states, channels, channels; the last two may be NULL */
+    const float* initial;
+    void* y;                                        /* tokens x channels */
+    float* state;
+    void* kept;                                     /* nuka_b200_scan_kept() bytes on 16 bytes that the backward call reads; the forward call writes them unless NULL */
+    uint64_t kept_bytes;
+    const void* dy;                                 /* the rest in the backward call only; gradients are contiguous */
+    const float* dstate;                            /* NULL = 0 */
+    void *dx, *ddelta, *dgate, *db, *dc;            /* dgate only where a gate is given */
+    float *ddecay, *dskip, *ddelta_bias, *dinitial; /* NULL = not wanted; of dinitial, empty rows are left as they are */
+    void* workspace;                                /* nuka_b200_scan_workspace() bytes on 16 bytes; may be NULL where that is 0 */
+    uint64_t workspace_bytes;
+} nuka_b200_scan_t;
+uint64_t nuka_b200_scan_kept(const nuka_b200_episodes_t* plan, int64_t channels, int64_t states);
+uint64_t nuka_b200_scan_workspace(const nuka_b200_episodes_t* plan, int64_t channels, int64_t states, uint32_t backward);
+nuka_result_t nuka_b200_scan(const nuka_b200_scan_t* desc, void* stream);
+nuka_result_t nuka_b200_scan_backward(const nuka_b200_scan_t* desc, void* stream);
+/* Its form for one token of each env: state (envs x channels x states float, contiguous) is updated in place; envs with fresh[i] != 0 (NULL = none) begin from 0. */
+typedef struct nuka_b200_scan_step_t {
+    uint32_t dtype;
+    int64_t envs, channels, states;
+    const void *x, *delta, *gate, *b, *c;
+    int64_t x_stride, delta_stride, gate_stride, b_stride, c_stride;         /* between envs */
+    const float *decay, *skip, *delta_bias;
+    const uint8_t* fresh;
+    float* state;
+    void* y;                                        /* envs x channels */
+} nuka_b200_scan_step_t;
+nuka_result_t nuka_b200_scan_step(const nuka_b200_scan_step_t* desc, void* stream);
+
 /* Queries and keys of every head: divided by their root mean square over the head's dim values (mean square plus eps), times a weight
  * per column (float, NULL = 1), then turned by the token's position: of the first `turned` columns the pairs (i, i + turned / 2), or with interleaved != 0
  * (2 i, 2 i + 1), turn by the angle position x frequencies[i] radians (double, turned / 2 of them), factors

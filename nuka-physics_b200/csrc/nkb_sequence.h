@@ -17,6 +17,16 @@ cudaError_t launch_recurrence(const nuka_b200_recurrence_t& d, bool backward, cu
 cudaError_t launch_recurrence_step(uint32_t dtype, int64_t n, int64_t channels, const void* x, int64_t x_stride, const void* gate, int64_t gate_stride,
                                    const uint8_t* fresh, float* state, void* h, cudaStream_t stream);
 
+uint64_t convolution_workspace(const nuka_b200_episodes_t& plan, int64_t channels, int64_t width);
+cudaError_t launch_convolution(const nuka_b200_convolution_t& d, bool backward, cudaStream_t stream);
+cudaError_t launch_convolution_step(const nuka_b200_convolution_step_t& d, cudaStream_t stream);
+
+uint64_t scan_kept(const nuka_b200_episodes_t& plan, int64_t channels, int64_t states);
+uint64_t scan_workspace(const nuka_b200_episodes_t& plan, int64_t channels, int64_t states, bool backward);
+int64_t scan_blocks(const nuka_b200_episodes_t& plan, int64_t channels, int64_t states);
+cudaError_t launch_scan(const nuka_b200_scan_t& d, bool backward, cudaStream_t stream);
+cudaError_t launch_scan_step(const nuka_b200_scan_step_t& d, cudaStream_t stream);
+
 uint64_t heads_workspace(int64_t tokens, int64_t dim);
 cudaError_t launch_heads(const nuka_b200_heads_t& d, bool backward, cudaStream_t stream);
 

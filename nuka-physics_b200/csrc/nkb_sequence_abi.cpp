@@ -88,6 +88,125 @@ nuka_result_t nuka_b200_recurrence_step(uint32_t dtype, int64_t n, int64_t chann
     return Ran(nkb::launch_recurrence_step(dtype, n, channels, x, x_stride, gate, gate_stride, fresh, state, h, StreamOf(stream)));
 }
 
+static const char* ConvolutionFault(uint32_t dtype, int64_t channels, int64_t width) {
+    if (dtype > NUKA_B200_BF16) return "dtype must be F32, F16 or BF16";
+    if (width < 2 || width > 4) return "width must be 2, 3 or 4";
+    if (channels < 0 || channels > (1 << 24)) return "channels must be 0 to 2^24";
+    return nullptr;
+}
+
+uint64_t nuka_b200_convolution_workspace(const nuka_b200_episodes_t* plan, int64_t channels, int64_t width) {
+    return PlanFault(plan) != nullptr || plan->tokens == 0 || channels <= 0 || ConvolutionFault(0, channels, width) != nullptr ? 0u : nkb::convolution_workspace(*plan, channels, width);
+}
+
+static nuka_result_t Convolution(const nuka_b200_convolution_t* desc, bool backward, void* stream) {
+    if (desc == nullptr) return Invalid("convolution desc is null");
+    const nuka_b200_convolution_t& d = *desc;
+    if (const char* fault = PlanFault(d.plan)) return Invalid(fault);
+    if (const char* fault = ConvolutionFault(d.dtype, d.channels, d.width)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, fault);
+    if (d.x_stride < 0) return Invalid("a stride is negative");
+    if (!Aligned(d.weight, 4) || !Aligned(d.bias, 4) || (backward && (!Aligned(d.dweight, 4) || !Aligned(d.dbias, 4)))) return Invalid("a weight or its gradient does not lie on 4 bytes");
+    if (d.channels == 0) return NUKA_RESULT_OK;
+    const uint64_t size = SizeOf(d.dtype);
+    if (d.plan->tokens != 0) {
+        if (d.x == nullptr || d.weight == nullptr) return Invalid("x or weight is null");
+        if (!backward && (d.y == nullptr || d.state == nullptr)) return Invalid("y or state is null");
+        if (backward && (d.dy == nullptr || d.dx == nullptr)) return Invalid("dy or dx is null");
+    }
+    for (const void* p : {d.x, d.initial, static_cast<const void*>(d.y), static_cast<const void*>(d.state)})
+        if (!Aligned(p, size)) return Invalid("a tensor does not lie on a multiple of its type's size");
+    if (backward)
+        for (const void* p : {d.dy, d.dstate, static_cast<const void*>(d.dx), static_cast<const void*>(d.dinitial)})
+            if (!Aligned(p, size)) return Invalid("a gradient does not lie on a multiple of its type's size");
+    if ((d.plan->tokens / 128 + 1) * (d.channels / 32 + 1) > (1ll << 30)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times channels");
+    if (backward && d.plan->tokens != 0 && (d.dweight != nullptr || d.dbias != nullptr) &&
+        (d.workspace == nullptr || !Aligned(d.workspace, 4) || d.workspace_bytes < nkb::convolution_workspace(*d.plan, d.channels, d.width))) return Invalid("the workspace is null, too small or not on 4 bytes");
+    return Ran(nkb::launch_convolution(d, backward, StreamOf(stream)));
+}
+
+nuka_result_t nuka_b200_convolution(const nuka_b200_convolution_t* desc, void* stream) { return Convolution(desc, false, stream); }
+nuka_result_t nuka_b200_convolution_backward(const nuka_b200_convolution_t* desc, void* stream) { return Convolution(desc, true, stream); }
+
+nuka_result_t nuka_b200_convolution_step(const nuka_b200_convolution_step_t* desc, void* stream) {
+    if (desc == nullptr) return Invalid("convolution step desc is null");
+    const nuka_b200_convolution_step_t& d = *desc;
+    if (const char* fault = ConvolutionFault(d.dtype, d.channels, d.width)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, fault);
+    if (d.envs < 0 || d.envs > kMostTokens || d.x_stride < 0) return Invalid("a size or stride is negative or too large");
+    if (d.envs == 0 || d.channels == 0) return NUKA_RESULT_OK;
+    if (d.x == nullptr || d.weight == nullptr || d.state == nullptr || d.y == nullptr) return Invalid("x, weight, state or y is null");
+    for (const void* p : {d.x, static_cast<const void*>(d.state), static_cast<const void*>(d.y)})
+        if (!Aligned(p, SizeOf(d.dtype))) return Invalid("a tensor does not lie on a multiple of its type's size");
+    if (!Aligned(d.weight, 4) || !Aligned(d.bias, 4)) return Invalid("a weight does not lie on 4 bytes");
+    if (d.envs * d.channels / 128 >= (1ll << 31) - 1) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many envs times channels");
+    return Ran(nkb::launch_convolution_step(d, StreamOf(stream)));
+}
+
+static const char* ScanFault(uint32_t dtype, int64_t channels, int64_t states) {
+    if (dtype > NUKA_B200_BF16) return "dtype must be F32, F16 or BF16";
+    if (states < 1 || states > 64) return "states must be 1 to 64";
+    if (channels < 0 || channels > (1 << 24)) return "channels must be 0 to 2^24";
+    return nullptr;
+}
+
+uint64_t nuka_b200_scan_kept(const nuka_b200_episodes_t* plan, int64_t channels, int64_t states) {
+    return PlanFault(plan) != nullptr || plan->tokens == 0 || channels <= 0 || ScanFault(0, channels, states) != nullptr ? 0u : nkb::scan_kept(*plan, channels, states);
+}
+uint64_t nuka_b200_scan_workspace(const nuka_b200_episodes_t* plan, int64_t channels, int64_t states, uint32_t backward) {
+    return PlanFault(plan) != nullptr || plan->tokens == 0 || channels <= 0 || ScanFault(0, channels, states) != nullptr ? 0u : nkb::scan_workspace(*plan, channels, states, backward != 0u);
+}
+
+static nuka_result_t Scan(const nuka_b200_scan_t* desc, bool backward, void* stream) {
+    if (desc == nullptr) return Invalid("scan desc is null");
+    const nuka_b200_scan_t& d = *desc;
+    if (const char* fault = PlanFault(d.plan)) return Invalid(fault);
+    if (const char* fault = ScanFault(d.dtype, d.channels, d.states)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, fault);
+    if (d.x_stride < 0 || d.delta_stride < 0 || d.gate_stride < 0 || d.b_stride < 0 || d.c_stride < 0) return Invalid("a stride is negative");
+    for (const float* p : {d.decay, d.skip, d.delta_bias, d.initial, static_cast<const float*>(d.state)})
+        if (!Aligned(p, 4)) return Invalid("a weight or state does not lie on 4 bytes");
+    if (backward)
+        for (const float* p : {d.dstate, static_cast<const float*>(d.ddecay), static_cast<const float*>(d.dskip), static_cast<const float*>(d.ddelta_bias), static_cast<const float*>(d.dinitial)})
+            if (!Aligned(p, 4)) return Invalid("a weight's or state's gradient does not lie on 4 bytes");
+    if (d.channels == 0) return NUKA_RESULT_OK;
+    if (d.plan->tokens == 0) return Ran(nkb::launch_scan(d, backward, StreamOf(stream)));
+    const uint64_t size = SizeOf(d.dtype);
+    for (const void* p : {d.x, d.delta, d.b, d.c, static_cast<const void*>(d.decay)})
+        if (p == nullptr) return Invalid("x, delta, b, c or decay is null");
+    if (!backward && (d.y == nullptr || d.state == nullptr)) return Invalid("y or state is null");
+    for (const void* p : {d.x, d.delta, d.gate, d.b, d.c, static_cast<const void*>(d.y)})
+        if (!Aligned(p, size)) return Invalid("a tensor does not lie on a multiple of its type's size");
+    if (backward) {
+        for (const void* p : {d.dy, static_cast<const void*>(d.dx), static_cast<const void*>(d.ddelta), static_cast<const void*>(d.db), static_cast<const void*>(d.dc)})
+            if (p == nullptr || !Aligned(p, size)) return Invalid("a gradient is null or does not lie on a multiple of its type's size");
+        if ((d.gate != nullptr && d.dgate == nullptr) || !Aligned(d.dgate, size)) return Invalid("dgate is null or does not lie on a multiple of its type's size");
+    }
+    if (nkb::scan_blocks(*d.plan, d.channels, d.states) > (1ll << 30)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times channels");
+    if ((backward || d.kept != nullptr) && (d.kept == nullptr || !Aligned(d.kept, 16) || d.kept_bytes < nkb::scan_kept(*d.plan, d.channels, d.states)))
+        return Invalid("what is kept for the gradient is null, too small or not on 16 bytes");
+    const uint64_t need = nkb::scan_workspace(*d.plan, d.channels, d.states, backward);
+    if (need != 0u && (d.workspace == nullptr || d.workspace_bytes < need || !Aligned(d.workspace, 16))) return Invalid("the workspace is null, too small or not on 16 bytes");
+    return Ran(nkb::launch_scan(d, backward, StreamOf(stream)));
+}
+
+nuka_result_t nuka_b200_scan(const nuka_b200_scan_t* desc, void* stream) { return Scan(desc, false, stream); }
+nuka_result_t nuka_b200_scan_backward(const nuka_b200_scan_t* desc, void* stream) { return Scan(desc, true, stream); }
+
+nuka_result_t nuka_b200_scan_step(const nuka_b200_scan_step_t* desc, void* stream) {
+    if (desc == nullptr) return Invalid("scan step desc is null");
+    const nuka_b200_scan_step_t& d = *desc;
+    if (const char* fault = ScanFault(d.dtype, d.channels, d.states)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, fault);
+    if (d.envs < 0 || d.envs > kMostTokens) return Invalid("envs are negative or too many");
+    if (d.x_stride < 0 || d.delta_stride < 0 || d.gate_stride < 0 || d.b_stride < 0 || d.c_stride < 0) return Invalid("a stride is negative");
+    if (d.envs == 0 || d.channels == 0) return NUKA_RESULT_OK;
+    for (const void* p : {d.x, d.delta, d.b, d.c, static_cast<const void*>(d.decay), static_cast<const void*>(d.state), static_cast<const void*>(d.y)})
+        if (p == nullptr) return Invalid("x, delta, b, c, decay, state or y is null");
+    for (const void* p : {d.x, d.delta, d.gate, d.b, d.c, static_cast<const void*>(d.y)})
+        if (!Aligned(p, SizeOf(d.dtype))) return Invalid("a tensor does not lie on a multiple of its type's size");
+    for (const float* p : {d.decay, d.skip, d.delta_bias, static_cast<const float*>(d.state)})
+        if (!Aligned(p, 4)) return Invalid("a weight or state does not lie on 4 bytes");
+    if (d.envs * d.channels / 8 >= (1ll << 31) - 1) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many envs times channels");
+    return Ran(nkb::launch_scan_step(d, StreamOf(stream)));
+}
+
 uint64_t nuka_b200_heads_workspace(int64_t tokens, int64_t dim) { return tokens <= 0 || dim <= 0 ? 0u : nkb::heads_workspace(tokens, dim); }
 
 static nuka_result_t Heads(const nuka_b200_heads_t* desc, bool backward, void* stream) {

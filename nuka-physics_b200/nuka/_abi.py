@@ -73,6 +73,35 @@ class RecurrenceDesc(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
 
 
+class ConvolutionDesc(ctypes.Structure):
+    _fields_ = [("plan", ctypes.POINTER(EpisodesDesc)), ("dtype", ctypes.c_uint32), ("silu", ctypes.c_uint32), ("channels", ctypes.c_int64), ("width", ctypes.c_int64),
+                ("x", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("initial", ctypes.c_void_p), ("y", ctypes.c_void_p),
+                ("state", ctypes.c_void_p), ("dy", ctypes.c_void_p), ("dstate", ctypes.c_void_p), ("dx", ctypes.c_void_p), ("dinitial", ctypes.c_void_p),
+                ("dweight", ctypes.c_void_p), ("dbias", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ConvolutionStepDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("silu", ctypes.c_uint32), ("envs", ctypes.c_int64), ("channels", ctypes.c_int64), ("width", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("x_stride", ctypes.c_int64), ("weight", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("fresh", ctypes.c_void_p), ("state", ctypes.c_void_p), ("y", ctypes.c_void_p)]
+
+
+class ScanDesc(ctypes.Structure):
+    _fields_ = [("plan", ctypes.POINTER(EpisodesDesc)), ("dtype", ctypes.c_uint32), ("channels", ctypes.c_int64), ("states", ctypes.c_int64), ("x", ctypes.c_void_p),
+                ("delta", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("b", ctypes.c_void_p), ("c", ctypes.c_void_p), ("x_stride", ctypes.c_int64),
+                ("delta_stride", ctypes.c_int64), ("gate_stride", ctypes.c_int64), ("b_stride", ctypes.c_int64), ("c_stride", ctypes.c_int64), ("decay", ctypes.c_void_p),
+                ("skip", ctypes.c_void_p), ("delta_bias", ctypes.c_void_p), ("initial", ctypes.c_void_p), ("y", ctypes.c_void_p), ("state", ctypes.c_void_p),
+                ("kept", ctypes.c_void_p), ("kept_bytes", ctypes.c_uint64), ("dy", ctypes.c_void_p), ("dstate", ctypes.c_void_p), ("dx", ctypes.c_void_p),
+                ("ddelta", ctypes.c_void_p), ("dgate", ctypes.c_void_p), ("db", ctypes.c_void_p), ("dc", ctypes.c_void_p), ("ddecay", ctypes.c_void_p), ("dskip", ctypes.c_void_p),
+                ("ddelta_bias", ctypes.c_void_p), ("dinitial", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64)]
+
+
+class ScanStepDesc(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_uint32), ("envs", ctypes.c_int64), ("channels", ctypes.c_int64), ("states", ctypes.c_int64), ("x", ctypes.c_void_p), ("delta", ctypes.c_void_p),
+                ("gate", ctypes.c_void_p), ("b", ctypes.c_void_p), ("c", ctypes.c_void_p), ("x_stride", ctypes.c_int64), ("delta_stride", ctypes.c_int64),
+                ("gate_stride", ctypes.c_int64), ("b_stride", ctypes.c_int64), ("c_stride", ctypes.c_int64), ("decay", ctypes.c_void_p), ("skip", ctypes.c_void_p),
+                ("delta_bias", ctypes.c_void_p), ("fresh", ctypes.c_void_p), ("state", ctypes.c_void_p), ("y", ctypes.c_void_p)]
+
+
 EXACT_ANGLES = 0x80000000                # added to HeadsDesc.interleaved
 
 
@@ -114,6 +143,8 @@ EXPORTS = [
     "nuka_b200_recurrence_backward", "nuka_b200_recurrence_step", "nuka_b200_heads_workspace", "nuka_b200_heads", "nuka_b200_heads_backward",
     "nuka_b200_attention_pitch", "nuka_b200_attention", "nuka_b200_attention_backward",
     "nuka_b200_history_workspace", "nuka_b200_history", "nuka_b200_history_advance",
+    "nuka_b200_convolution_workspace", "nuka_b200_convolution", "nuka_b200_convolution_backward", "nuka_b200_convolution_step",
+    "nuka_b200_scan_kept", "nuka_b200_scan_workspace", "nuka_b200_scan", "nuka_b200_scan_backward", "nuka_b200_scan_step",
 ]
 
 _LIB = None
@@ -201,5 +232,17 @@ def lib():
     L.nuka_b200_history_workspace.restype = u64
     L.nuka_b200_history.argtypes = [ctypes.POINTER(HistoryDesc), vp]
     L.nuka_b200_history_advance.argtypes = [vp, vp, i64, vp]
+    L.nuka_b200_convolution_workspace.argtypes = [ctypes.POINTER(EpisodesDesc), i64, i64]
+    L.nuka_b200_convolution_workspace.restype = u64
+    L.nuka_b200_convolution.argtypes = [ctypes.POINTER(ConvolutionDesc), vp]
+    L.nuka_b200_convolution_backward.argtypes = [ctypes.POINTER(ConvolutionDesc), vp]
+    L.nuka_b200_convolution_step.argtypes = [ctypes.POINTER(ConvolutionStepDesc), vp]
+    L.nuka_b200_scan_kept.argtypes = [ctypes.POINTER(EpisodesDesc), i64, i64]
+    L.nuka_b200_scan_kept.restype = u64
+    L.nuka_b200_scan_workspace.argtypes = [ctypes.POINTER(EpisodesDesc), i64, i64, u32]
+    L.nuka_b200_scan_workspace.restype = u64
+    L.nuka_b200_scan.argtypes = [ctypes.POINTER(ScanDesc), vp]
+    L.nuka_b200_scan_backward.argtypes = [ctypes.POINTER(ScanDesc), vp]
+    L.nuka_b200_scan_step.argtypes = [ctypes.POINTER(ScanStepDesc), vp]
     _LIB = L
     return L

@@ -6,6 +6,8 @@ every env, for acting:
 
     over a rollout (training)                      one token of every env (acting)
     gated_recurrence(x, gate, episodes, initial)   gated_recurrence_step(x, gate, state, fresh)
+    short_convolution(x, weight, bias, episodes)   short_convolution_step(x, weight, bias, state, fresh)
+    selective_scan(x, delta, ..., episodes)        selective_scan_step(x, delta, ..., state, fresh)
     rotate_heads(q, k, ..., episodes, ...)         rotate_heads(q, k, ..., positions, ...)
     episode_attention(q, k, v, episodes)           history_attention(q, k, v, cache)
 
@@ -265,6 +267,219 @@ def gated_recurrence_step(x, gate, state, fresh=None):
     h = torch.empty(x.shape, dtype=x.dtype, device=device)
     _call(device, _abi.lib().nuka_b200_recurrence_step, dtype, x.shape[0], x.shape[1], x.data_ptr(), _stride(x, 0), gate.data_ptr(), _stride(gate, 0), _ptr(fresh), state.data_ptr(), h.data_ptr())
     return h
+
+
+# ---- the short causal convolution -----------------------------------------------------------------------------------
+def _final_state(episodes, initial, shape, dtype, device):
+    """Where the state that each row ends with goes: an empty row ends with what it began with."""
+    if not episodes._rows_may_be_empty:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.zeros(shape, dtype=dtype, device=device) if initial is None else initial.clone(memory_format=torch.contiguous_format)
+
+
+def _workspace(need, device):
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def _convolve(x, weight, bias, initial, episodes, silu):
+    device, channels = x.device, x.shape[1]
+    y, state = torch.empty(x.shape, dtype=x.dtype, device=device), _final_state(episodes, initial, (episodes.rows, weight.shape[1] - 1, channels), x.dtype, device)
+    desc = _abi.ConvolutionDesc(episodes._ref, _DTYPES[x.dtype], silu, channels, weight.shape[1], x.data_ptr(), _stride(x, 0), weight.data_ptr(), _ptr(bias), _ptr(initial), y.data_ptr(), state.data_ptr())
+    episodes._read_on(_call(device, _abi.lib().nuka_b200_convolution, ctypes.byref(desc)))
+    return y, state
+
+
+class _Convolution(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, initial, episodes, silu):
+        ctx.episodes, ctx.silu, ctx.given = episodes, silu, (bias is not None, initial is not None)
+        ctx.save_for_backward(x, weight, *(v for v in (bias, initial) if v is not None))
+        ctx.set_materialize_grads(False)
+        return _convolve(x, weight, bias, initial, episodes, silu)
+
+    @_once
+    def backward(ctx, dy, dstate):
+        x, weight, *rest = ctx.saved_tensors
+        # what is saved may come back elsewhere and with other strides (offloaded, worked out again)
+        x, weight, rest = _channels_last(x), weight.contiguous(), [v.contiguous() for v in rest]
+        bias, initial = rest[0] if ctx.given[0] else None, rest[-1] if ctx.given[1] else None
+        episodes, device, channels, width = ctx.episodes, x.device, x.shape[1], weight.shape[1]
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=device) if dy is None else dy.contiguous()
+        dstate = None if dstate is None else dstate.contiguous()
+        dx, dinitial = _empty(x), None
+        if initial is not None and ctx.needs_input_grad[3]:
+            dinitial = _final_state(episodes, dstate, initial.shape, x.dtype, device)
+        dweight = _empty(weight) if ctx.needs_input_grad[1] else None
+        dbias = _empty(bias) if bias is not None and ctx.needs_input_grad[2] else None
+        lib = _abi.lib()
+        need = lib.nuka_b200_convolution_workspace(episodes._ref, channels, width) if dweight is not None or dbias is not None else 0
+        workspace = _workspace(need, device)
+        desc = _abi.ConvolutionDesc(episodes._ref, _DTYPES[x.dtype], ctx.silu, channels, width, x.data_ptr(), _stride(x, 0), weight.data_ptr(), _ptr(bias), _ptr(initial), None, None,
+                                    dy.data_ptr(), _ptr(dstate), dx.data_ptr(), _ptr(dinitial), _ptr(dweight), _ptr(dbias), _ptr(workspace), need)
+        episodes._read_on(_call(device, lib.nuka_b200_convolution_backward, ctypes.byref(desc)))
+        return dx, dweight, dbias, dinitial, None, None
+
+
+def _convolution_weights(weight, bias, channels):
+    if weight.dim() != 2 or weight.shape[0] != channels or not 2 <= weight.shape[1] <= 4 or weight.dtype != torch.float32:
+        raise ValueError(f"weight must be float32, {channels} channels x 2, 3 or 4 taps")
+    if bias is not None and (bias.shape != (channels,) or bias.dtype != torch.float32):
+        raise ValueError(f"bias must be float32, {channels} channels")
+    return weight.contiguous(), None if bias is None else bias.contiguous()
+
+
+def short_convolution(x, weight, bias, episodes, initial=None, silu=False):
+    """y_t = bias + sum over j of weight[:, j] x_{t - width + 1 + j}, channel by channel over each episode, with `silu` times its own logistic function.
+
+    x: tokens x channels, f32, f16 or bf16.  weight: channels x width float32, width 2 to 4, the present token's last.  bias: channels float32, or None.  Inputs before an episode are 0.
+    initial: rows x (width - 1) x channels in x's type, what came before each row (the state of its env when the rollout began), None for 0.  Returns (y, state): y like x,
+    state like initial, the last inputs of each row's last episode. Sums are in 32 bits."""
+    device = _on_gpu(x, weight, bias, initial, episodes._plan)
+    _dtype(x, _DTYPES, "x")
+    _tokens_of(x, episodes, 2, "x")
+    weight, bias = _convolution_weights(weight, bias, x.shape[1])
+    if initial is not None:
+        shape = (episodes.rows, weight.shape[1] - 1, x.shape[1])
+        if initial.shape != shape or initial.dtype != x.dtype:
+            raise ValueError(f"initial must be {' x '.join(map(str, shape))} of x's type on {device}")
+        initial = initial.contiguous()
+    train = _differentiated(x, weight, bias, initial)
+    x = _channels_last(x)
+    return _Convolution.apply(x, weight, bias, initial, episodes, bool(silu)) if train else _convolve(x, weight, bias, initial, episodes, bool(silu))
+
+
+def short_convolution_step(x, weight, bias, state, fresh=None, silu=False):
+    """The convolution for one token of each env.  x: envs x channels; state: envs x (width - 1) x channels of x's type, contiguous, updated in place; fresh: envs, bool or
+    uint8, set where the token begins an episode (the inputs before it count as 0).  Returns y like x.  No gradient."""
+    device = _on_gpu(x, weight, bias, state, fresh)
+    dtype = _dtype(x, _DTYPES, "x")
+    _expect(x.dim() == 2, "x must be envs x channels")
+    weight, bias = _convolution_weights(weight, bias, x.shape[1])
+    envs, channels, width = x.shape[0], x.shape[1], weight.shape[1]
+    if state.shape != (envs, width - 1, channels) or state.dtype != x.dtype or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous, {envs} x {width - 1} x {channels} of x's type")
+    x = _channels_last(x)
+    if fresh is not None:
+        fresh = _flags(fresh, x.shape[:1], device, "fresh")
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    desc = _abi.ConvolutionStepDesc(dtype, bool(silu), envs, channels, width, x.data_ptr(), _stride(x, 0), weight.data_ptr(), _ptr(bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
+    _call(device, _abi.lib().nuka_b200_convolution_step, ctypes.byref(desc))
+    return y
+
+
+# ---- the selective scan ----------------------------------------------------------------------------------------------
+_SCANNED = ("x", "delta", "gate", "b", "c")              # what has a stride of its own
+
+
+def _scan(tensors, episodes, train):
+    """`tensors`: by the descriptor's names, None where not given.  (y, state, what a backward pass needs beside the inputs)."""
+    x, decay, initial = tensors["x"], tensors["decay"], tensors["initial"]
+    device, (channels, states) = x.device, decay.shape
+    y, state = torch.empty(x.shape, dtype=x.dtype, device=device), _final_state(episodes, initial, (episodes.rows, channels, states), torch.float32, device)
+    lib = _abi.lib()
+    kept = torch.empty(lib.nuka_b200_scan_kept(episodes._ref, channels, states), dtype=torch.uint8, device=device) if train else None
+    need = lib.nuka_b200_scan_workspace(episodes._ref, channels, states, 0)
+    workspace = _workspace(need, device)
+    desc = _scan_desc(tensors, episodes)
+    desc.y, desc.state, desc.workspace, desc.workspace_bytes = y.data_ptr(), state.data_ptr(), _ptr(workspace), need
+    if train:
+        desc.kept, desc.kept_bytes = _ptr(kept), kept.numel()
+    episodes._read_on(_call(device, lib.nuka_b200_scan, ctypes.byref(desc)))
+    return y, state, kept
+
+
+def _scan_desc(t, episodes):
+    channels, states = t["decay"].shape
+    return _abi.ScanDesc(episodes._ref, _DTYPES[t["x"].dtype], channels, states, *(_ptr(t[name]) for name in _SCANNED), *(0 if t[name] is None else _stride(t[name], 0) for name in _SCANNED),
+                         t["decay"].data_ptr(), _ptr(t["skip"]), _ptr(t["delta_bias"]), _ptr(t["initial"]))
+
+
+_SCAN_INPUTS = ("x", "delta", "decay", "b", "c", "initial", "skip", "gate", "delta_bias")
+
+
+class _Scan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, episodes, *inputs):
+        y, state, kept = _scan(dict(zip(_SCAN_INPUTS, inputs)), episodes, True)
+        ctx.episodes, ctx.names = episodes, [name for name, x in zip(_SCAN_INPUTS, inputs) if x is not None]
+        ctx.save_for_backward(*(x for x in inputs if x is not None), kept)
+        ctx.set_materialize_grads(False)
+        return y, state
+
+    @_once
+    def backward(ctx, dy, dstate):
+        *saved, kept = ctx.saved_tensors
+        # what is saved may come back elsewhere and with other strides (offloaded, worked out again)
+        t = {name: _channels_last(x) if name in _SCANNED else x.contiguous() for name, x in zip(ctx.names, saved)}
+        t = {name: t.get(name) for name in _SCAN_INPUTS}
+        kept = _channels_last(kept.contiguous(), 1, 16)
+        x, episodes = t["x"], ctx.episodes
+        device, (channels, states) = x.device, t["decay"].shape
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=device) if dy is None else dy.contiguous()
+        dstate = None if dstate is None else dstate.contiguous()
+        wanted = dict(zip(_SCAN_INPUTS, ctx.needs_input_grad[1:]))
+        grads = {name: _empty(v) for name, v in t.items() if v is not None and (name in _SCANNED or wanted[name])}
+        if "initial" in grads:
+            grads["initial"] = _final_state(episodes, dstate, t["initial"].shape, torch.float32, device)
+        lib = _abi.lib()
+        need = lib.nuka_b200_scan_workspace(episodes._ref, channels, states, 1)
+        workspace = _workspace(need, device)
+        desc = _scan_desc(t, episodes)
+        desc.kept, desc.kept_bytes, desc.dy, desc.dstate, desc.workspace, desc.workspace_bytes = _ptr(kept), kept.numel(), dy.data_ptr(), _ptr(dstate), _ptr(workspace), need
+        for name, v in grads.items():
+            setattr(desc, "d" + name, v.data_ptr())
+        episodes._read_on(_call(device, lib.nuka_b200_scan_backward, ctypes.byref(desc)))
+        return (None, *(grads.get(name) for name in _SCAN_INPUTS))
+
+
+def _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias):
+    """Checks what the scan and its step have in common; the inputs as the kernels take them."""
+    _dtype(x, _DTYPES, "x")
+    if x.dim() != 2 or decay.dim() != 2 or decay.shape[0] != x.shape[1] or not 1 <= decay.shape[1] <= 64 or decay.dtype != torch.float32:
+        raise ValueError("x must have 2 dimensions, the second of channels, and decay must be float32, channels x 1 to 64 states")
+    for v, shape, what in ((delta, x.shape, "delta"), (gate, x.shape, "gate"), (b, (x.shape[0], decay.shape[1]), "b"), (c, (x.shape[0], decay.shape[1]), "c")):
+        if v is not None and (v.shape != shape or v.dtype != x.dtype):
+            raise ValueError(f"{what} must be {' x '.join(map(str, shape))}, of x's type")
+    for v, what in ((skip, "skip"), (delta_bias, "delta_bias")):
+        if v is not None and (v.shape != x.shape[1:] or v.dtype != torch.float32):
+            raise ValueError(f"{what} must be float32, one per channel")
+    x, delta, b, c = (_channels_last(v) for v in (x, delta, b, c))
+    gate = None if gate is None else _channels_last(gate)
+    return x, delta, decay.contiguous(), b, c, None if skip is None else skip.contiguous(), gate, None if delta_bias is None else delta_bias.contiguous()
+
+
+def selective_scan(x, delta, decay, b, c, episodes, initial=None, skip=None, gate=None, delta_bias=None):
+    """h_t = exp(dt decay) h_{t-1} + dt x_t b_t with dt = softplus(delta_t + delta_bias), a state of channels x states; y_t = h_t c_t + skip x_t, with `gate` times gate_t / (1 + exp(-gate_t)).
+
+    x, delta, gate: tokens x channels, f32, f16 or bf16.  b, c: tokens x states, of x's type; all at any stride (views of projections).  decay: channels x states float32, 1 to 64 states, below 0 where
+    a state fades.  skip, delta_bias: channels float32, or None.  initial: rows x channels x states float32, the state that each row begins with, None for 0; an episode that begins inside a row
+    begins with 0.  Returns (y, state): y like x, state like initial, what each row ends with.  Rates, states and sums are in 32 bits, exponentials are off by up to 2^-22 of themselves. Where a gradient may
+    be asked for, the states before each fourth or eighth token are kept (at 16 states 8 bytes for each value of x)."""
+    device = _on_gpu(x, delta, decay, b, c, initial, skip, gate, delta_bias, episodes._plan)
+    _tokens_of(x, episodes, 2, "x")
+    x, delta, decay, b, c, skip, gate, delta_bias = _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias)
+    if initial is not None:
+        if initial.shape != (episodes.rows, *decay.shape) or initial.dtype != torch.float32:
+            raise ValueError(f"initial must be {episodes.rows} x {decay.shape[0]} x {decay.shape[1]} float32 on {device}")
+        initial = initial.contiguous()
+    inputs = (x, delta, decay, b, c, initial, skip, gate, delta_bias)
+    return _Scan.apply(episodes, *inputs) if _differentiated(*inputs) else _scan(dict(zip(_SCAN_INPUTS, inputs)), episodes, False)[:2]
+
+
+def selective_scan_step(x, delta, decay, b, c, state, fresh=None, skip=None, gate=None, delta_bias=None):
+    """The scan for one token of each env.  x, delta, gate: envs x channels; b, c: envs x states; state: envs x channels x states float32, contiguous, updated in place; fresh: envs, bool or
+    uint8, set where the token begins an episode (the state before it counts as 0).  Returns y like x.  No gradient."""
+    device = _on_gpu(x, delta, decay, b, c, state, fresh, skip, gate, delta_bias)
+    x, delta, decay, b, c, skip, gate, delta_bias = _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias)
+    if state.shape != (x.shape[0], *decay.shape) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous float32, {x.shape[0]} x {decay.shape[0]} x {decay.shape[1]}")
+    if fresh is not None:
+        fresh = _flags(fresh, x.shape[:1], device, "fresh")
+    y = torch.empty(x.shape, dtype=x.dtype, device=device)
+    desc = _abi.ScanStepDesc(_DTYPES[x.dtype], x.shape[0], *decay.shape, x.data_ptr(), delta.data_ptr(), _ptr(gate), b.data_ptr(), c.data_ptr(), _stride(x, 0), _stride(delta, 0),
+                             0 if gate is None else _stride(gate, 0), _stride(b, 0), _stride(c, 0), decay.data_ptr(), _ptr(skip), _ptr(delta_bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
+    _call(device, _abi.lib().nuka_b200_scan_step, ctypes.byref(desc))
+    return y
 
 
 # ---- norms of queries and keys, and their rotation -----------------------------------------------------------------

@@ -533,6 +533,9 @@ typedef struct nuka_b200_attention_t {
 int64_t nuka_b200_attention_pitch(int64_t tokens);
 nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream);
 nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream);
+/* The same where, beside the window's, the first `sinks` tokens of an episode stay visible to all that come after them (without a window all are, whatever sinks is). */
+nuka_result_t nuka_b200_attention_sinks(const nuka_b200_attention_t* desc, int64_t sinks, void* stream);
+nuka_result_t nuka_b200_attention_sinks_backward(const nuka_b200_attention_t* desc, int64_t sinks, void* stream);
 
 /* Attention of one token of each env over the env's cached history, for acting.  keys and values (envs x capacity x heads_k x dim, contiguous, on 16 bytes) are a
  * ring: the token's k and v are written to place position % capacity, then the token attends to the last min(position + 1, capacity) tokens, itself among
@@ -553,6 +556,9 @@ typedef struct nuka_b200_history_t {
 } nuka_b200_history_t;
 uint64_t nuka_b200_history_workspace(const nuka_b200_history_t* desc);
 nuka_result_t nuka_b200_history(const nuka_b200_history_t* desc, void* stream);
+/* The same with a cache that keeps the first `sinks` tokens of an episode, fewer than its capacity, in its first places; the others are a ring behind them, token number p in place
+ * sinks + (p - sinks) % (capacity - sinks). What nuka_b200_attention_sinks gives with window = capacity - sinks. */
+nuka_result_t nuka_b200_history_sinks(const nuka_b200_history_t* desc, int64_t sinks, void* stream);
 /* position[env] = 0 where fresh[env] != 0 (NULL = nowhere), else one more than it was: the next token of every env. */
 nuka_result_t nuka_b200_history_advance(int32_t* position, const uint8_t* fresh, int64_t envs, void* stream);
 

@@ -41,7 +41,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct AttentionParams {
     const int32_t *first, *end;
     int64_t tokens, pitch;                              // pitch: floats between the heads' rows of lse and delta
-    int heads_q, heads_k, dim, window;                  // window 0: all of the episode
+    int heads_q, heads_k, dim, window, sinks;           // window 0: all of the episode; sinks: first tokens of an episode that stay visible, only with a window
     int span, tiles;                                    // tokens of a tile, at most 128, and how many tiles
     int split;                                          // blocks of a key job, a cluster, each with an equal share of the group's heads
     int by_heads, across, along;                        // of the forward kernel's jobs: tiles of two heads or of two stretches of tokens; jobs side by side, and behind one another
@@ -55,6 +55,45 @@ struct AttentionParams {
 
 __device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
 
+// The keys that a tile of queries goes through, `step` at a time: from the first query's own first one to the last query, and with sinks, before these, what of its episode's first tokens lies
+// before that. The sinks of an episode that begins in the tile, or among the tile's keys, lie among those anyway: there is never more than one episode with some before.
+template <bool SINKS> struct KeySteps {
+    int near, count, far, far_steps, far_end;           // far to far_end: the sinks before; their steps come first
+    __device__ __forceinline__ KeySteps(const AttentionParams& p, int first, int i0, int last, int step) {
+        near = p.window > 0 ? max(first, i0 - p.window + 1) : first;
+        far = first;
+        far_end = SINKS ? first + min(p.sinks, near - first) : first;
+        far_steps = SINKS ? (far_end - far + step - 1) / step : 0;
+        count = (last - near) / step + 1 + far_steps;
+    }
+    __device__ __forceinline__ bool is_far(int j) const { return SINKS && j < far_steps; }
+    __device__ __forceinline__ int at(int j, int step) const { return !SINKS ? near + j * step : j < far_steps ? far + j * step : near + (j - far_steps) * step; }
+};
+
+// The keys that a row sees, and what its warp's rows see: the window's, and those of the episode's first tokens, which may overlap it or lie before.
+template <bool SINKS> struct RowKeys {
+    int low, high, first, sink;                         // low to high, and first to sink
+    int any_low, any_high, all_low, all_high, any_first, any_sink;
+    __device__ __forceinline__ RowKeys(const AttentionParams& p, bool live, int i, int episode) {
+        high = live ? i : -1;
+        low = !live ? 0 : p.window > 0 ? max(episode, i - p.window + 1) : episode;
+        any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff); any_high = __reduce_max_sync(~0u, high);
+        all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff); all_high = __reduce_min_sync(~0u, high);
+        if (SINKS) {
+            first = live ? episode : 0;
+            sink = live ? episode + min(p.sinks - 1, i - episode) : -1;
+            any_first = __reduce_min_sync(~0u, live ? episode : 0x7fffffff); any_sink = __reduce_max_sync(~0u, sink);
+        }
+    }
+    // The keys k0 to k0 + n - 1 of a step, of which `far_end` and on are another's where it is a far one: seen by all rows; hidden from all; the ones of 32 that the row sees
+    __device__ __forceinline__ bool all(int k0, int n, bool far) const { return !(SINKS && far) && k0 >= all_low && k0 + n - 1 <= all_high; }
+    __device__ __forceinline__ bool hidden(int k0, int n, bool far, int far_end) const {
+        const bool window = k0 > any_high || k0 + n - 1 < any_low;
+        return !SINKS ? window : (far || window) && (k0 > any_sink || k0 + n - 1 < any_first || (far && k0 >= far_end));
+    }
+    __device__ __forceinline__ uint32_t seen(int k0, bool far, int far_end) const;
+};
+
 // A tile of queries and a head; the longest of one long row first.  What it reads of the plan is looked at only when it is used, a job after it was asked for.
 struct QueryJob {
     int i0, last, head, first;                          // queries i0 to last; first: the plan's, of the first
@@ -65,8 +104,7 @@ struct QueryJob {
         last = (int)min((int64_t)i0 + p.span, p.tokens) - 1;
         first = p.first[i0];
     }
-    __device__ __forceinline__ int begin(const AttentionParams& p) const { return p.window > 0 ? max(first, i0 - p.window + 1) : first; }             // of its keys
-    __device__ __forceinline__ int steps(const AttentionParams& p) const { return (last - begin(p)) / kStream + 1; }
+    template <bool SINKS> __device__ __forceinline__ KeySteps<SINKS> steps(const AttentionParams& p) const { return KeySteps<SINKS>(p, first, i0, last, kStream); }
 };
 
 // One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T; whether all are finite.
@@ -119,6 +157,10 @@ __device__ __forceinline__ uint32_t columns_between(int from, int to) {
     const uint32_t above = from <= 0 ? ~0u : from > 31 ? 0u : ~0u << from, below = to < 0 ? 0u : to >= 31 ? ~0u : (2u << to) - 1u;
     return above & below;
 }
+template <bool SINKS> __device__ __forceinline__ uint32_t RowKeys<SINKS>::seen(int k0, bool far, int far_end) const {
+    if (!SINKS) return columns_between(low - k0, high - k0);
+    return far ? columns_between(first - k0, min(sink, far_end - 1) - k0) : columns_between(low - k0, high - k0) | columns_between(first - k0, sink - k0);
+}
 
 // A row of 64-column panels of 128 rows, swizzled as TMA takes it: 16 bytes number `k` of row `row`.
 __device__ __forceinline__ unsigned char* staged(unsigned char* tile, int row, int k) { return tile + k / 8 * kRows * 128 + row * 128 + ((k % 8) ^ (row % 8)) * 16; }
@@ -170,7 +212,13 @@ template <typename T> __device__ __forceinline__ const T* key_row(const Attentio
 template <typename T> __device__ __forceinline__ const T* value_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.v) + j * p.v_stride + head * p.v_head_stride; }
 template <typename T> __device__ __forceinline__ const T* dout_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.dout) + ((int64_t)i * p.heads_q + head) * p.dim; }
 __device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
-__device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+__device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 && j - p.first[j] >= p.sinks ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+// The keys that query i sees, in one range or, its sinks first, in two.
+template <typename Use> __device__ __forceinline__ void each_range(const AttentionParams& p, int i, Use use) {
+    const int low = first_key(p, i);
+    if (p.sinks > 0 && p.first[i] < low) use(p.first[i], p.first[i] + min(p.sinks, low - p.first[i]) - 1);
+    use(low, i);
+}
 
 // Which of a lane's four values are not finite.
 template <typename T> __device__ __forceinline__ uint32_t spoilt_of(uint2 v) {
@@ -207,14 +255,17 @@ template <typename T> __device__ __noinline__ void mend_out(const AttentionParam
     const uint2 is = result_of(out, p.dim, lane);
     uint32_t which = spoilt_of<T>(is);
     if (!__any_sync(~0u, which != 0u) || (__shfl_sync(~0u, is.x, 0) & 0xffffu) == kFinal) return;
-    const int key_head = head / (p.heads_q / p.heads_k), low = first_key(p, i);
-    for (int j = low; j <= i && __any_sync(~0u, which != 0u); j += 8)
+    const int key_head = head / (p.heads_q / p.heads_k);
+    each_range(p, i, [&](int low, int high) {
+        for (int j = low; j <= high && __any_sync(~0u, which != 0u); j += 8)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) which &= ~spoilt_of<T>(result_of(value_row<T>(p, min(j + k, i), key_head), p.dim, lane));
+            for (int k = 0; k < 8; ++k) which &= ~spoilt_of<T>(result_of(value_row<T>(p, min(j + k, high), key_head), p.dim, lane));
+    });
     if (!__any_sync(~0u, which != 0u)) return;
     float top = -INFINITY, total = 0.f, sum[4] = {};
-    for (int j = low; j <= i; j += 32) {
-        const int count = min(32, i - j + 1);
+    each_range(p, i, [&](int low, int high) {
+    for (int j = low; j <= high; j += 32) {
+        const int count = min(32, high - j + 1);
         const float score = lane < count ? dot(query_row<T>(p, i, head), key_row<T>(p, j + lane, key_head), p.dim) * p.scale2 : -INFINITY;
         float best = score;
 #pragma unroll
@@ -227,6 +278,7 @@ template <typename T> __device__ __noinline__ void mend_out(const AttentionParam
         add_rows<T>(sum, weight, count, p.dim, lane, [&](int k) { return value_row<T>(p, j + k, key_head); });
         top = best;
     }
+    });
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) total += __shfl_xor_sync(~0u, total, d);
     give_columns(out, which, sum, 1.f / total, lane);
@@ -240,12 +292,14 @@ template <typename T> __device__ __noinline__ void mend_query_grad(const Attenti
     if (!__any_sync(~0u, which != 0u)) return;
     const int key_head = head / (p.heads_q / p.heads_k);
     float sum[4] = {};
-    for (int j = first_key(p, i); j <= i; j += 32) {
-        const int count = min(32, i - j + 1), own = min(j + lane, i);
+    each_range(p, i, [&](int low, int high) {
+    for (int j = low; j <= high; j += 32) {
+        const int count = min(32, high - j + 1), own = min(j + lane, high);
         const float prob = exp2f(fmaf(dot(query_row<T>(p, i, head), key_row<T>(p, own, key_head), p.dim), p.scale2, -lse));
         const float weight = prob * (dot(dout_row<T>(p, i, head), value_row<T>(p, own, key_head), p.dim) - delta);
         add_rows<T>(sum, weight, count, p.dim, lane, [&](int k) { return key_row<T>(p, j + k, key_head); });
     }
+    });
     give_columns(dq, which, sum, p.scale, lane);
 }
 
@@ -321,13 +375,12 @@ struct ForwardJob {
         }
         first = p.first[i0[0]];
     }
-    __device__ __forceinline__ int begin(const AttentionParams& p) const { return p.window > 0 ? max(first, i0[0] - p.window + 1) : first; }          // of its keys
-    __device__ __forceinline__ int steps(const AttentionParams& p, int step) const { return (max(last[0], last[1]) - begin(p)) / step + 1; }
+    template <bool SINKS> __device__ __forceinline__ KeySteps<SINKS> steps(const AttentionParams& p, int step) const { return KeySteps<SINKS>(p, first, i0[0], max(last[0], last[1]), step); }
     // Every other round backwards, so that the longest of one round goes with the shortest of the next.
     static __device__ __forceinline__ int of_turn(int turn) { return turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                 const __grid_constant__ CUtensorMap map_o, const __grid_constant__ AttentionParams p) {
     using F = Forward<DP>;
@@ -372,16 +425,17 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 const ForwardJob now = next;
                 const int after = ForwardJob::of_turn(turn + 1);
                 if (after < jobs) next = ForwardJob(p, after);
-                const int b = queries % F::kQueries, key_head = now.head[0] / (p.heads_q / p.heads_k), j0 = now.begin(p), count = now.steps(p, F::kStep);
+                const int b = queries % F::kQueries, key_head = now.head[0] / (p.heads_q / p.heads_k);
+                const KeySteps<SINKS> through = now.steps<SINKS>(p, F::kStep);
                 if (queries >= F::kQueries && !(fine = barrier_wait(&q_empty[b], (queries / F::kQueries - 1) & 1, &lost))) break;
                 barrier_expect(&q_full[b], 2 * F::kTile);
                 for (int s = 0; s < 2; ++s) load_panels<kRows, DP>(shared + (2 * b + s) * F::kTile, &map_q, &q_full[b], now.head[s], now.i0[s]);
                 ++queries;
-                for (int j = 0; j < count; ++j, ++keys) {
+                for (int j = 0; j < through.count; ++j, ++keys) {
                     const int s = keys % F::kStages, round = keys / F::kStages;
                     if (round > 0 && !(fine = barrier_wait(&k_empty[s], (round - 1) & 1, &lost))) break;
                     barrier_expect(&k_full[s], F::kPart);
-                    load_panels<F::kStep, DP>(shared + F::kKeys + s * F::kPart, &map_k, &k_full[s], key_head, j0 + j * F::kStep);
+                    load_panels<F::kStep, DP>(shared + F::kKeys + s * F::kPart, &map_k, &k_full[s], key_head, through.at(j, F::kStep));
                 }
             }
             drain_ring(q_full, F::kQueries, queries);
@@ -396,12 +450,13 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 const ForwardJob now = next;
                 const int after = ForwardJob::of_turn(turn + 1);
                 if (after < jobs) next = ForwardJob(p, after);
-                const int key_head = now.head[0] / (p.heads_q / p.heads_k), j0 = now.begin(p), count = now.steps(p, F::kStep);
-                for (int j = 0; j < count; ++j, ++values) {
+                const int key_head = now.head[0] / (p.heads_q / p.heads_k);
+                const KeySteps<SINKS> through = now.steps<SINKS>(p, F::kStep);
+                for (int j = 0; j < through.count; ++j, ++values) {
                     const int s = values % F::kStages, round = values / F::kStages;
                     if (round > 0 && !(fine = barrier_wait(&v_empty[s], (round - 1) & 1, &lost))) break;
                     barrier_expect(&v_full[s], F::kPart);
-                    load_panels<F::kStep, DP>(shared + F::kKeys + (F::kStages + s) * F::kPart, &map_v, &v_full[s], key_head, j0 + j * F::kStep);
+                    load_panels<F::kStep, DP>(shared + F::kKeys + (F::kStages + s) * F::kPart, &map_v, &v_full[s], key_head, through.at(j, F::kStep));
                 }
             }
             drain_ring(v_full, F::kStages, values);
@@ -415,7 +470,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         int k_stage = 0, k_phase = 0, v_stage = 0, v_phase = 0, q_buffer = 0, q_phase = 0;
         auto scores = [&]() {
             if (j == 0) {
-                count = __shfl_sync(~0u, next.steps(p, F::kStep), 0);
+                count = __shfl_sync(~0u, next.steps<SINKS>(p, F::kStep).count, 0);
                 const int after = ForwardJob::of_turn(turn + 1);
                 if (after < jobs) next = ForwardJob(p, after);
                 if (!warp_wait(&q_full[q_buffer], q_phase, &lost)) return false;
@@ -491,18 +546,17 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         auto first_of = [&](const ForwardJob& job) { return p.first[min(job.i0[set] + row, job.last[set] >= job.i0[set] ? job.last[set] : 0)]; };
         int next_first = first_of(next);
         for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
-            const int first = next.i0[set], last = next.last[set], i = first + row, head = next.head[set], j0 = next.begin(p), count = next.steps(p, F::kStep);
-            const bool live = i <= last;
-            const int high = live ? i : -1, low = !live ? 0 : p.window > 0 ? max(next_first, i - p.window + 1) : next_first;
+            const int first = next.i0[set], last = next.last[set], i = first + row, head = next.head[set];
+            const KeySteps<SINKS> through = next.steps<SINKS>(p, F::kStep);
+            // keys that any and that all of the warp's rows see; a row that is not there sees none
+            const RowKeys<SINKS> keys(p, i <= last, i, next_first);
             const int after = ForwardJob::of_turn(turn + 1);
             if (after < jobs) { next = ForwardJob(p, after); next_first = first_of(next); }
-            // keys that any and that all of the warp's rows see; a row that is not there sees none
-            const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
-            const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
             bool left = false;
-            for (int j = 0; j < count; ++j, ++n) {
-                const int k0 = j0 + j * F::kStep;
+            for (int j = 0; j < through.count; ++j, ++n) {
+                const int k0 = through.at(j, F::kStep);
+                const bool far = through.is_far(j);
                 fine = fine && warp_wait(&s_full[set], n & 1, &lost);
                 if (!fine) break;
                 fence_after();
@@ -530,13 +584,13 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                 auto rows = [&](auto all) {
                     constexpr bool ALL = decltype(all)::value != 0;
                     constexpr int CHUNK = DP == 64 ? 32 : 16;
-                    auto hidden = [&](int c) { return !ALL && (k0 + c > any_high || k0 + c + CHUNK - 1 < any_low); };
+                    auto hidden = [&](int c) { return !ALL && keys.hidden(k0 + c, CHUNK, far, through.far_end); };
                     float best[4] = {top, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
                     for (int c = 0; c < F::kStep; c += CHUNK) {
                         if (hidden(c)) continue;
-                        if (!ALL && (k0 + c < all_low || k0 + c + CHUNK - 1 > all_high)) {
-                            const uint32_t seen = columns_between(low - k0 - c, high - k0 - c);
+                        if (!ALL && !keys.all(k0 + c, CHUNK, far)) {
+                            const uint32_t seen = keys.seen(k0 + c, far, through.far_end);
 #pragma unroll
                             for (int k = 0; k < CHUNK; ++k) r[c + k] = seen >> k & 1u ? r[c + k] : 0xff800000u;
                         }
@@ -579,7 +633,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
                     }
                     return true;
                 };
-                if (!(fine = k0 >= all_low && k0 + F::kStep - 1 <= all_high ? rows(Number<1>{}) : rows(Number<0>{}))) break;
+                if (!(fine = keys.all(k0, F::kStep, far) ? rows(Number<1>{}) : rows(Number<0>{}))) break;
                 float x, y;
                 split(add_pair(part[0], part[1]), x, y);
                 sum += x + y;
@@ -641,7 +695,7 @@ template <int DP> struct Queries {
     static constexpr int kGrad = kStream, kScores = 2 * kStream, kOut = kBuffers * kScores, kProb = kOut + DP;
 };
 
-template <typename T, int DP>
+template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
                                                                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq,
                                                                const AttentionParams p) {
@@ -685,14 +739,15 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
                 load_panels<kRows, DP>(shared + F::kTile, &map_do, &q_full, now.head, now.i0);
                 load_panels<kRows, DP>(shared + 2 * F::kTile, &map_o, &q_full, now.head, now.i0);
                 ++queries;
-                const int j0 = now.begin(p), count = now.steps(p), key_head = now.head / group;
-                for (int j = 0; j < count; ++j, ++steps) {
+                const int key_head = now.head / group;
+                const KeySteps<SINKS> through = now.steps<SINKS>(p);
+                for (int j = 0; j < through.count; ++j, ++steps) {
                     const int s = steps % F::kStages, turn = steps / F::kStages;
                     if (turn > 0 && !(fine = barrier_wait(&empty[s], (turn - 1) & 1, &lost))) break;
                     barrier_expect(&full[s], 2 * F::kPart);
                     unsigned char* to = shared + F::kKeys + 2 * s * F::kPart;
-                    load_panels<kStream, DP>(to, &map_k, &full[s], key_head, j0 + j * kStream);
-                    load_panels<kStream, DP>(to + F::kPart, &map_v, &full[s], key_head, j0 + j * kStream);
+                    load_panels<kStream, DP>(to, &map_k, &full[s], key_head, through.at(j, kStream));
+                    load_panels<kStream, DP>(to + F::kPart, &map_v, &full[s], key_head, through.at(j, kStream));
                 }
             }
             drain_ring(&q_full, 1, queries);
@@ -703,7 +758,7 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
         QueryJob next(p, job);
         auto scores = [&]() {
             if (j == 0) {
-                count = __shfl_sync(~0u, next.steps(p), 0);
+                count = __shfl_sync(~0u, next.steps<SINKS>(p).count, 0);
                 if (job + stride < jobs) next = QueryJob(p, job + stride);
                 if (!warp_wait(&q_full, queries & 1, &lost)) return false;
             }
@@ -771,13 +826,11 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
         float next_lse = lse_of(next);
         for (int job = blockIdx.x; job < jobs; job += stride, ++queries) {
             const QueryJob now = next;
-            const int i = now.i0 + row, j0 = now.begin(p), count = now.steps(p);
-            const bool live = i <= now.last;
-            const int high = live ? i : -1, low = !live ? 0 : p.window > 0 ? max(next_first, i - p.window + 1) : next_first;
+            const int i = now.i0 + row;
+            const KeySteps<SINKS> through = now.steps<SINKS>(p);
+            const RowKeys<SINKS> sees(p, i <= now.last, i, next_first);
             const float lse = next_lse;
             if (job + stride < jobs) { next = QueryJob(p, job + stride); next_first = first_of(next); next_lse = lse_of(next); }
-            const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
-            const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             // D = dO . O of the thread's row.  O has the error of its own rounding and of P's, which the sum of dS over the row, 0 by definition, shows: the keys' kernel, which runs
             // after this one, gets D without it. Where a step holds all keys of a row D is summed from its own P and dP before dS, which matters where few keys share a row (dq of
             // 24-token episodes was off by 1.8 times its rounding; with many keys the error averages out).
@@ -796,23 +849,24 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             const Pair scale2 = pair_of(p.scale2, p.scale2), shift = pair_of(-lse, -lse);
             Pair off = pair_of(0.f, 0.f);
             bool left = false;
-            for (int j = 0; j < count; ++j, ++n) {
-                const int k0 = j0 + j * kStream;
+            for (int j = 0; j < through.count; ++j, ++n) {
+                const int k0 = through.at(j, kStream);
+                const bool far = through.is_far(j);
                 const int b = n % F::kBuffers;
                 const uint32_t here = mine + b * F::kScores;
                 fine = fine && warp_wait(&s_full[b], n / F::kBuffers & 1, &lost);
                 if (!fine) break;
                 fence_after();
                 uint32_t packed[F::kPer / 2];
-                const bool all = k0 >= all_low && k0 + kStream - 1 <= all_high;
-                auto hidden = [&](int c0) { return k0 + c0 > any_high || k0 + c0 + 31 < any_low; };          // from all of the warp's rows
+                const bool all = sees.all(k0, kStream, far);
+                auto hidden = [&](int c0) { return sees.hidden(k0 + c0, 32, far, through.far_end); };         // from all of the warp's rows
                 // P and P (dP - D) of 32 keys
                 auto part = [&](int c0, Pair minus, auto use) {
                     uint32_t r[32], d[32];
                     tensor_load(here + c0, r);
                     tensor_load(here + F::kGrad + c0, d);
                     wait_loads();
-                    const uint32_t seen = all ? ~0u : columns_between(low - k0 - c0, high - k0 - c0);
+                    const uint32_t seen = all ? ~0u : sees.seen(k0 + c0, far, through.far_end);
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         float a, b, x, y;
@@ -827,7 +881,7 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
                         use(c, x, y);
                     }
                 };
-                const bool whole = live && low >= k0 && high < k0 + kStream;
+                const bool whole = !far && (SINKS ? sees.first : sees.low) >= k0 && sees.high >= 0 && sees.high < k0 + kStream;
                 if (__any_sync(~0u, whole)) {
                     float own = 0.f;
 #pragma unroll 1
@@ -907,17 +961,21 @@ template <int DP> struct Keys {
 };
 
 // A tile of keys and a key head; the longest of one long row are the first ones.
-struct KeyJob {
-    int j0, last, head, end;                            // keys j0 to last; end: the plan's, of the last
+template <bool SINKS> struct KeyJob {
+    int j0, last, head, end, first;                     // keys j0 to last; end, first: the plan's, of the last
     __device__ __forceinline__ KeyJob(const AttentionParams& p, int job) {
         const int tile = job / p.heads_k;
         head = job - tile * p.heads_k;
         j0 = tile * p.span;
         last = (int)min((int64_t)j0 + p.span, p.tokens) - 1;
         end = p.end[last];
+        if (SINKS) first = p.first[last];
     }
     __device__ __forceinline__ int begin() const { return j0 & ~3; }               // of its queries: a multiple of 16 bytes of their statistics
-    __device__ __forceinline__ int past(const AttentionParams& p) const { return p.window > 0 ? (int)min((int64_t)end, (int64_t)last + p.window) : end; }
+    // behind the last query that sees one of the keys: sinks of the last key's episode are seen to its end
+    __device__ __forceinline__ int past(const AttentionParams& p) const {
+        return p.window > 0 && !(SINKS && j0 - first < p.sinks) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
+    }
     __device__ __forceinline__ int steps(const AttentionParams& p) const { return (past(p) - 1 - begin()) / kStream + 1; }            // for one head
 };
 
@@ -938,7 +996,7 @@ template <int DP, int THREADS> __device__ __noinline__ void clear_hidden(int fro
     __syncwarp();
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                                                                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
                                                                             const __grid_constant__ CUtensorMap map_dv, const AttentionParams p) {
@@ -973,10 +1031,10 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         if (lane == 0) {
             int steps = 0, keys = 0;                    // loads begun so far
             bool fine = true;
-            KeyJob next(p, job0);
+            KeyJob<SINKS> next(p, job0);
             for (int job = job0; fine && job < jobs; job += stride) {
-                const KeyJob now = next;
-                if (job + stride < jobs) next = KeyJob(p, job + stride);
+                const KeyJob<SINKS> now = next;
+                if (job + stride < jobs) next = KeyJob<SINKS>(p, job + stride);
                 if (keys > 0 && !(fine = barrier_wait(&k_empty, (keys - 1) & 1, &lost))) break;
                 barrier_expect(&k_full, 2 * F::kTile);
                 load_panels<kRows, DP>(shared, &map_k, &k_full, now.head, now.j0);
@@ -1000,11 +1058,11 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         }
     } else if (warp == 5) {
         int job = job0, j = 0, count = 0, ahead = 0, keys = 0, stage = 0, phase = 0;         // of the scores
-        KeyJob next(p, job);
+        KeyJob<SINKS> next(p, job);
         auto scores = [&]() {
             if (j == 0) {
                 count = __shfl_sync(~0u, next.steps(p) * group, 0);
-                if (job + stride < jobs) next = KeyJob(p, job + stride);
+                if (job + stride < jobs) next = KeyJob<SINKS>(p, job + stride);
                 if (!warp_wait(&k_full, keys & 1, &lost)) return false;
             }
             if (!warp_wait(&full[stage], phase, &lost)) return false;
@@ -1023,7 +1081,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         bool fine = scores();
         for (int own = job0; fine && own < jobs; own += stride) {
             const int steps = count;                    // of the job that the scores have just begun
-            const KeyJob now(p, own);
+            const KeyJob<SINKS> now(p, own);
             const int each = steps / group;
             for (int i = 0, m = 0; i < steps; ++i, ++n) {
                 // the other buffer's P and dS are free when the products before have ended
@@ -1098,17 +1156,19 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                 if (there && !finite) spoilt = 1;
             }
         };
-        KeyJob next(p, job0);
-        auto end_of = [&](const KeyJob& job) { return p.end[min(job.j0 + row, job.last)]; };
+        KeyJob<SINKS> next(p, job0);
+        auto end_of = [&](const KeyJob<SINKS>& job) { return p.end[min(job.j0 + row, job.last)]; };
+        auto sink_of = [&](const KeyJob<SINKS>& job) { const int j = min(job.j0 + row, job.last); return SINKS && j - p.first[j] < p.sinks; };
         int next_end = end_of(next);
+        bool next_sink = sink_of(next);
         const Pair scale2 = pair_of(p.scale2, p.scale2), minus_one = pair_of(-1.f, -1.f);
         for (int job = job0; job < jobs; job += stride, ++keys) {
-            const KeyJob now = next;
+            const KeyJob<SINKS> now = next;
             const int j = now.j0 + row, each = now.steps(p);
             const bool live = j <= now.last;
             // the queries that see the key
-            const int low = live ? j : 0, high = !live ? -1 : (p.window > 0 ? (int)min((int64_t)next_end, (int64_t)j + p.window) : next_end) - 1;
-            if (job + stride < jobs) { next = KeyJob(p, job + stride); next_end = end_of(next); }
+            const int low = live ? j : 0, high = !live ? -1 : (p.window > 0 && !next_sink ? (int)min((int64_t)next_end, (int64_t)j + p.window) : next_end) - 1;
+            if (job + stride < jobs) { next = KeyJob<SINKS>(p, job + stride); next_end = end_of(next); next_sink = sink_of(next); }
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             bool first = true, left = false;
@@ -1191,7 +1251,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         meet(1, F::kWorkers);
         if (p.split == 1 && spoilt != 0 && lost == 0)
             for (int job = job0; job < jobs; job += stride) {
-                const KeyJob done(p, job);
+                const KeyJob<SINKS> done(p, job);
                 for (int j = done.j0 + half * 4 + warp % 4; j <= done.last; j += F::kWorkers / 32)
                     for (int which = 0; which < 2; ++which) mend_key_grad<T>(p, j, done.head, which, lane);
             }
@@ -1205,7 +1265,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         __syncwarp();
         cluster_meet();
         // each block takes its share of the rows of the cluster's one job
-        const KeyJob job(p, job0);
+        const KeyJob<SINKS> job(p, job0);
         const int rows = kRows / p.split;
         for (int x = threadIdx.x; x < 2 * rows * (DP / 4); x += F::kThreads) {
             const int which = x / (rows * (DP / 4)), row = rank * rows + x / (DP / 4) % rows, c = x % (DP / 4) * 4, j = job.j0 + row;
@@ -1261,11 +1321,11 @@ static int tile_span(const nuka_b200_episodes_t& plan) {
 
 template <typename K> static cudaError_t with_shared(K kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 
-template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_attention_t& d, bool backward, cudaStream_t stream) {
+template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream) {
     AttentionParams p{};
     const nuka_b200_episodes_t& e = *d.plan;
     p.first = e.first; p.end = e.end; p.tokens = e.tokens; p.pitch = attention_pitch(e.tokens);
-    p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens);
+    p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens); p.sinks = (int)std::min(sinks, e.tokens);
     p.span = tile_span(e); p.tiles = (int)((e.tokens + p.span - 1) / p.span);
     p.by_heads = p.heads_q / p.heads_k % 2 == 0;
     p.across = p.by_heads ? p.heads_q / 2 : p.heads_q; p.along = p.by_heads ? p.tiles : (p.tiles + 1) / 2;
@@ -1277,18 +1337,18 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
     CUtensorMap q, k, v, g, o;
     if (!backward) {
         // first, because it makes the device's context the thread's own: maps cannot be encoded without one
-        cudaError_t set = with_shared(attention_kernel<T, DP>, Forward<DP>::kShared);
+        cudaError_t set = with_shared(attention_kernel<T, DP, SINKS>, Forward<DP>::kShared);
         if (set != cudaSuccess) return set;
         if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, kRows) || !map_of(&k, d.dtype, d.k, d.dim, d.heads_k, e.tokens, d.k_head_stride, d.k_stride, Forward<DP>::kStep) ||
             !map_of(&v, d.dtype, d.v, d.dim, d.heads_k, e.tokens, d.v_head_stride, d.v_stride, Forward<DP>::kStep) || !map_of(&o, d.dtype, d.out, d.dim, d.heads_q, e.tokens, d.dim, d.dim * d.heads_q, p.span))
             return cudaErrorInvalidValue;
-        attention_kernel<T, DP><<<(unsigned)std::min(p.across * p.along, 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
+        attention_kernel<T, DP, SINKS><<<(unsigned)std::min(p.across * p.along, 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();
     }
     CUtensorMap dq, dk, dv;
     for (int keys = 0; keys < 2; ++keys) {
         const int own = keys ? kStream : kRows, other = keys ? kRows : kStream;
-        cudaError_t set = keys ? with_shared(key_grad_kernel<T, DP>, Keys<DP>::kShared) : with_shared(query_grad_kernel<T, DP>, Queries<DP>::kShared);
+        cudaError_t set = keys ? with_shared(key_grad_kernel<T, DP, SINKS>, Keys<DP>::kShared) : with_shared(query_grad_kernel<T, DP, SINKS>, Queries<DP>::kShared);
         if (set != cudaSuccess) return set;
         const int64_t wide = d.dim * d.heads_q, narrow = d.dim * d.heads_k;
         if (!map_of(&q, d.dtype, d.q, d.dim, d.heads_q, e.tokens, d.q_head_stride, d.q_stride, own) || !map_of(&g, d.dtype, d.dout, d.dim, d.heads_q, e.tokens, d.dim, wide, own) ||
@@ -1302,9 +1362,9 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
         p.split = 1;
         while (keys && p.split < 8 && group % (2 * p.split) == 0 && 2 * p.split * (int64_t)jobs <= places) p.split *= 2;
         if (!keys) {
-            query_grad_kernel<T, DP><<<(unsigned)blocks, Queries<DP>::kThreads, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
+            query_grad_kernel<T, DP, SINKS><<<(unsigned)blocks, Queries<DP>::kThreads, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         } else if (p.split == 1) {
-            key_grad_kernel<T, DP><<<(unsigned)blocks, Keys<DP>::kThreads, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
+            key_grad_kernel<T, DP, SINKS><<<(unsigned)blocks, Keys<DP>::kThreads, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
         } else {
             cudaLaunchAttribute cluster{};
             cluster.id = cudaLaunchAttributeClusterDimension;
@@ -1312,7 +1372,7 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
             cudaLaunchConfig_t config{};
             config.gridDim = dim3((unsigned)(jobs * p.split)); config.blockDim = dim3(Keys<DP>::kThreads); config.dynamicSmemBytes = Keys<DP>::kShared; config.stream = stream;
             config.attrs = &cluster; config.numAttrs = 1u;
-            set = cudaLaunchKernelEx(&config, key_grad_kernel<T, DP>, q, g, k, v, dk, dv, p);
+            set = cudaLaunchKernelEx(&config, key_grad_kernel<T, DP, SINKS>, q, g, k, v, dk, dv, p);
             if (set != cudaSuccess) return set;
         }
         set = cudaGetLastError();
@@ -1321,10 +1381,14 @@ template <typename T, int DP> static cudaError_t run_attention(const nuka_b200_a
     return cudaSuccess;
 }
 
-cudaError_t launch_attention(const nuka_b200_attention_t& d, bool backward, cudaStream_t stream) {
+template <bool SINKS> static cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream) {
+    if (d.dtype == NUKA_B200_F16) return d.dim <= 64 ? run_attention<__half, 64, SINKS>(d, sinks, backward, stream) : run_attention<__half, 128, SINKS>(d, sinks, backward, stream);
+    return d.dim <= 64 ? run_attention<__nv_bfloat16, 64, SINKS>(d, sinks, backward, stream) : run_attention<__nv_bfloat16, 128, SINKS>(d, sinks, backward, stream);
+}
+
+cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream) {
     if (d.plan->tokens == 0) return cudaSuccess;
-    if (d.dtype == NUKA_B200_F16) return d.dim <= 64 ? run_attention<__half, 64>(d, backward, stream) : run_attention<__half, 128>(d, backward, stream);
-    return d.dim <= 64 ? run_attention<__nv_bfloat16, 64>(d, backward, stream) : run_attention<__nv_bfloat16, 128>(d, backward, stream);
+    return sinks > 0 && d.window > 0 ? launch_attention<true>(d, sinks, backward, stream) : launch_attention<false>(d, 0, backward, stream);
 }
 
 }  // namespace nkb

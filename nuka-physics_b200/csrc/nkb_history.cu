@@ -24,7 +24,7 @@ constexpr int kHistoryWarps = 4, kQueries = 8, kSplits = 32;
 constexpr float kHistoryLog2e = 1.4426950408889634f;
 
 struct HistoryParams {
-    int64_t jobs, capacity, q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
+    int64_t jobs, capacity, sinks, q_stride, q_head_stride, k_stride, k_head_stride, v_stride, v_head_stride;
     int heads_q, heads_k, dim, splits, parts;           // parts: sets of 8 query heads of a key head; jobs: envs x key heads x parts
     float scale2;
     const void *q, *k, *v;
@@ -64,7 +64,8 @@ __global__ void __launch_bounds__(kHistoryWarps * 32, DP == 64 ? 4 : 3) history_
     const int64_t env = job / p.parts / p.heads_k;
     const int group = p.heads_q / p.heads_k, queries = min(kQueries, group - part * kQueries), first = head * group + part * kQueries;
     const int32_t position = max(p.position[env], 0);
-    const int slot = (int)(position % p.capacity), held = (int)min((int64_t)position + 1, p.capacity);
+    // the first `sinks` tokens of an episode stay where they are, the others are a ring behind them
+    const int slot = position < p.capacity ? position : (int)(p.sinks + (position - p.sinks) % (p.capacity - p.sinks)), held = (int)min((int64_t)position + 1, p.capacity);
     const int each = (held + p.splits * 16 - 1) / (p.splits * 16) * 16, begin = (int)min((int64_t)held, (int64_t)split * each), end = min(held, begin + each);
 
     const int64_t row = (int64_t)p.heads_k * p.dim;     // between an env's keys
@@ -276,10 +277,10 @@ template <typename T, int DP> static void run_history(const HistoryParams& p, bo
     else history_kernel<T, DP, kHistoryWarps><<<(unsigned)(p.jobs * p.splits), kHistoryWarps * 32, 0, stream>>>(p);
 }
 
-cudaError_t launch_history(const nuka_b200_history_t& d, cudaStream_t stream) {
+cudaError_t launch_history(const nuka_b200_history_t& d, int64_t sinks, cudaStream_t stream) {
     if (d.envs == 0) return cudaSuccess;
     HistoryParams p{};
-    p.jobs = history_jobs(d); p.capacity = d.capacity; p.q_stride = d.q_stride; p.q_head_stride = d.q_head_stride; p.k_stride = d.k_stride; p.k_head_stride = d.k_head_stride;
+    p.jobs = history_jobs(d); p.capacity = d.capacity; p.sinks = sinks; p.q_stride = d.q_stride; p.q_head_stride = d.q_head_stride; p.k_stride = d.k_stride; p.k_head_stride = d.k_head_stride;
     p.v_stride = d.v_stride; p.v_head_stride = d.v_head_stride; p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.splits = history_splits(d);
     p.parts = (int)(p.jobs / d.envs / d.heads_k);
     p.scale2 = d.scale * kHistoryLog2e; p.q = d.q; p.k = d.k; p.v = d.v; p.keys = d.keys; p.values = d.values; p.out = d.out; p.position = d.position;

@@ -31,10 +31,10 @@ uint64_t heads_workspace(int64_t tokens, int64_t dim);
 cudaError_t launch_heads(const nuka_b200_heads_t& d, bool backward, cudaStream_t stream);
 
 int64_t attention_pitch(int64_t tokens);
-cudaError_t launch_attention(const nuka_b200_attention_t& d, bool backward, cudaStream_t stream);
+cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream);
 
 uint64_t history_workspace(const nuka_b200_history_t& d);
-cudaError_t launch_history(const nuka_b200_history_t& d, cudaStream_t stream);
+cudaError_t launch_history(const nuka_b200_history_t& d, int64_t sinks, cudaStream_t stream);
 cudaError_t launch_history_advance(int32_t* position, const uint8_t* fresh, int64_t envs, cudaStream_t stream);
 
 }  // namespace nkb

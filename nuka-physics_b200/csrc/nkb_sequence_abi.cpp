@@ -243,14 +243,14 @@ nuka_result_t nuka_b200_heads_backward(const nuka_b200_heads_t* desc, void* stre
 
 int64_t nuka_b200_attention_pitch(int64_t tokens) { return tokens <= 0 ? 0 : nkb::attention_pitch(tokens); }
 
-static nuka_result_t Attention(const nuka_b200_attention_t* desc, bool backward, void* stream) {
+static nuka_result_t Attention(const nuka_b200_attention_t* desc, int64_t sinks, bool backward, void* stream) {
     if (desc == nullptr) return Invalid("attention desc is null");
     const nuka_b200_attention_t& d = *desc;
     if (const char* fault = PlanFault(d.plan)) return Invalid(fault);
     if (d.dtype != NUKA_B200_F16 && d.dtype != NUKA_B200_BF16) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dtype must be F16 or BF16");
     if (d.heads_k < 1 || d.heads_q < 1 || d.heads_q > 65536 || d.heads_q % d.heads_k != 0) return Invalid("heads_q must be a positive multiple of heads_k, at most 65536");
     if (d.dim < 8 || d.dim > 128 || d.dim % 8 != 0) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dim must be a multiple of 8, 8 to 128");
-    if (d.window < 0) return Invalid("window must not be negative");
+    if (d.window < 0 || sinks < 0) return Invalid("window and sinks must not be negative");
     if (!(d.scale > 0.f) || d.scale > 3.0e38f) return Invalid("scale must be greater than 0 and finite");
     if (d.plan->tokens == 0) return NUKA_RESULT_OK;
     if ((d.plan->tokens / 64 + 1) * d.heads_q > (1ll << 30)) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many tokens times heads");
@@ -267,11 +267,13 @@ static nuka_result_t Attention(const nuka_b200_attention_t* desc, bool backward,
                                                         {d.plan->tokens, d.v_stride}, {d.heads_k, d.v_head_stride}};
     for (const auto& s : strides)
         if (s.size > 1 && (s.stride < d.dim || s.stride % 8 != 0 || s.stride >= (1ll << 38))) return Invalid("strides must be multiples of 8 values, at least dim");
-    return Ran(nkb::launch_attention(d, backward, StreamOf(stream)));
+    return Ran(nkb::launch_attention(d, sinks, backward, StreamOf(stream)));
 }
 
-nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, false, stream); }
-nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, true, stream); }
+nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, 0, false, stream); }
+nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, 0, true, stream); }
+nuka_result_t nuka_b200_attention_sinks(const nuka_b200_attention_t* desc, int64_t sinks, void* stream) { return Attention(desc, sinks, false, stream); }
+nuka_result_t nuka_b200_attention_sinks_backward(const nuka_b200_attention_t* desc, int64_t sinks, void* stream) { return Attention(desc, sinks, true, stream); }
 
 static const char* HistoryFault(const nuka_b200_history_t& d) {
     if (d.envs < 0 || d.envs > kMostTokens || d.capacity < 1 || d.capacity > (1 << 30)) return "envs must not be negative, capacity 1 to 2^30";
@@ -283,13 +285,14 @@ uint64_t nuka_b200_history_workspace(const nuka_b200_history_t* desc) {
     return desc == nullptr || HistoryFault(*desc) != nullptr || desc->envs == 0 ? 0u : nkb::history_workspace(*desc);
 }
 
-nuka_result_t nuka_b200_history(const nuka_b200_history_t* desc, void* stream) {
+static nuka_result_t History(const nuka_b200_history_t* desc, int64_t sinks, void* stream) {
     if (desc == nullptr) return Invalid("history desc is null");
     const nuka_b200_history_t& d = *desc;
     if (d.dtype != NUKA_B200_F16 && d.dtype != NUKA_B200_BF16) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dtype must be F16 or BF16");
     if (const char* fault = HistoryFault(d)) return Invalid(fault);
     if (d.dim < 8 || d.dim > 128 || d.dim % 8 != 0) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "dim must be a multiple of 8, 8 to 128");
     if (!(d.scale > 0.f) || d.scale > 3.0e38f) return Invalid("scale must be greater than 0 and finite");
+    if (sinks < 0 || sinks >= d.capacity) return Invalid("sinks must not be negative, and fewer than the capacity");
     if (d.envs == 0) return NUKA_RESULT_OK;
     if (d.envs * d.heads_q > (1ll << 31) - 1024) return Refuse(NUKA_RESULT_NOT_SUPPORTED, "too many envs times heads");
     for (const void* p : {d.q, d.k, d.v, static_cast<const void*>(d.keys), static_cast<const void*>(d.values), static_cast<const void*>(d.out)}) {
@@ -301,8 +304,11 @@ nuka_result_t nuka_b200_history(const nuka_b200_history_t* desc, void* stream) {
         if (s < 0 || s % 8 != 0) return Invalid("strides must be multiples of 8 values, not negative");
     const uint64_t need = nkb::history_workspace(d);
     if (need != 0u && (d.workspace == nullptr || d.workspace_bytes < need || !Aligned(d.workspace, 16))) return Invalid("the workspace is null, too small or not on 16 bytes");
-    return Ran(nkb::launch_history(d, StreamOf(stream)));
+    return Ran(nkb::launch_history(d, sinks, StreamOf(stream)));
 }
+
+nuka_result_t nuka_b200_history(const nuka_b200_history_t* desc, void* stream) { return History(desc, 0, stream); }
+nuka_result_t nuka_b200_history_sinks(const nuka_b200_history_t* desc, int64_t sinks, void* stream) { return History(desc, sinks, stream); }
 
 nuka_result_t nuka_b200_history_advance(int32_t* position, const uint8_t* fresh, int64_t envs, void* stream) {
     if (envs < 0 || envs > kMostTokens) return Invalid("envs are negative or too many");

@@ -574,7 +574,7 @@ def rotate_heads(q, k, q_weight, k_weight, positions, frequencies, eps=1e-6, int
 
 
 # ---- attention over packed episodes --------------------------------------------------------------------------------
-def _attend(q, k, v, episodes, scale, window, train):
+def _attend(q, k, v, episodes, scale, window, sinks, train):
     """(out, the statistics that a backward pass needs beside it, the call's descriptor)."""
     device = q.device
     out = torch.empty(q.shape, dtype=q.dtype, device=device)
@@ -582,17 +582,21 @@ def _attend(q, k, v, episodes, scale, window, train):
     lse = torch.empty((q.shape[1], lib.nuka_b200_attention_pitch(episodes.tokens)), dtype=torch.float32, device=device) if train else None
     desc = _abi.AttentionDesc(episodes._ref, _DTYPES[q.dtype], q.shape[1], k.shape[1], q.shape[2], window, scale, q.data_ptr(), k.data_ptr(), v.data_ptr(), _stride(q, 0), _stride(q, 1),
                               _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), out.data_ptr(), _ptr(lse))
-    episodes._read_on(_call(device, lib.nuka_b200_attention, ctypes.byref(desc)))
+    if sinks:
+        stream = _call(device, lib.nuka_b200_attention_sinks, ctypes.byref(desc), sinks)
+    else:
+        stream = _call(device, lib.nuka_b200_attention, ctypes.byref(desc))
+    episodes._read_on(stream)
     return out, lse, desc
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, episodes, scale, window):
-        out, lse, desc = _attend(q, k, v, episodes, scale, window, True)
+    def forward(ctx, q, k, v, episodes, scale, window, sinks):
+        out, lse, desc = _attend(q, k, v, episodes, scale, window, sinks, True)
         tensors = (q, k, v, out, lse)
         ctx.save_for_backward(*tensors)
-        ctx.desc, ctx.strides, ctx.episodes = desc, [x.stride() for x in tensors], episodes
+        ctx.desc, ctx.strides, ctx.episodes, ctx.sinks = desc, [x.stride() for x in tensors], episodes, sinks
         return out
 
     @_once
@@ -608,12 +612,17 @@ class _Attention(torch.autograd.Function):
         dq, dk, dv = _empty(tensors[0]), _empty(tensors[1]), _empty(tensors[2])
         delta = _empty(lse)
         desc.dout, desc.delta, desc.dq, desc.dk, desc.dv = dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
-        ctx.episodes._read_on(_call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc)))
-        return dq, dk, dv, None, None, None
+        if ctx.sinks:
+            stream = _call(device, _abi.lib().nuka_b200_attention_sinks_backward, ctypes.byref(desc), ctx.sinks)
+        else:
+            stream = _call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc))
+        ctx.episodes._read_on(stream)
+        return dq, dk, dv, None, None, None, None
 
 
-def episode_attention(q, k, v, episodes, scale=None, window=None):
-    """Causal attention over each episode: a token sees itself and the tokens of its episode before it, with `window` at most the last `window` of these.
+def episode_attention(q, k, v, episodes, scale=None, window=None, sinks=0):
+    """Causal attention over each episode: a token sees itself and the tokens of its episode before it, with `window` at most the last `window` of these, and beside them the
+    episode's first `sinks` ones (which without a window are seen anyway).
 
     q: tokens x heads x dim, k and v: tokens x key heads x dim, f16 or bf16, tokens and heads at any stride (views of one projection); the heads are a multiple
     of the key heads, and as many heads share one key head.  dim: a multiple of 8, at most 128 (64 and 128 waste nothing).  scale: dim^-0.5 unless given.
@@ -627,22 +636,26 @@ def episode_attention(q, k, v, episodes, scale=None, window=None):
     _expect(k.shape[1] > 0 and q.shape[1] % k.shape[1] == 0 and q.shape[1] > 0, "the heads must be a multiple of the key heads")
     _expect(q.shape[2] > 0, "heads must have columns")
     _expect(window is None or window >= 1, "window must be at least 1")
-    scale, window = q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window)
+    _expect(sinks >= 0, "sinks must not be negative")
+    scale, window, sinks = q.shape[2] ** -0.5 if scale is None else float(scale), 0 if window is None else int(window), 0 if window is None else int(sinks)
     train = _differentiated(q, k, v)
     q, k, v = (_channels_last(x, 8, 16, x.shape[2]) for x in (q, k, v))
-    return _Attention.apply(q, k, v, episodes, scale, window) if train else _attend(q, k, v, episodes, scale, window, False)[0]
+    return _Attention.apply(q, k, v, episodes, scale, window, sinks) if train else _attend(q, k, v, episodes, scale, window, sinks, False)[0]
 
 
 # ---- attention of one token over a cached history ------------------------------------------------------------------
 class HistoryCache:
-    """Keys and values of the last `capacity` tokens of each env, for one layer: a ring of envs x capacity x key heads x dim.
+    """Keys and values of the last `capacity` tokens of each env, for one layer: a ring of envs x capacity x key heads x dim. With `sinks`, fewer than the capacity, its first
+    places keep the first tokens of the env's episode, and the last `capacity` - `sinks` of the others are a ring behind them.
 
     ``position`` (envs, int32) is the number of each env's present token in its episode; ``advance(fresh)`` moves on to the next token of every env.  Layers of one
     policy share it: give one cache's ``position`` to the others and advance once per control step.  `buffers`: (keys, values, position) to use in place of new ones."""
 
-    def __init__(self, envs, capacity, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", position=None, buffers=None):
+    def __init__(self, envs, capacity, kv_heads, head_dim, dtype=torch.bfloat16, device="cuda", position=None, buffers=None, sinks=0):
         _expect(dtype in (torch.float16, torch.bfloat16), "dtype must be float16 or bfloat16")
         _expect(envs >= 0 and capacity >= 1 and kv_heads >= 1 and head_dim >= 8, "envs must not be negative, capacity and kv_heads at least 1, head_dim at least 8")
+        _expect(0 <= sinks < capacity, "sinks must not be negative, and fewer than the capacity")
+        self.sinks = int(sinks)
         shape = (int(envs), int(capacity), int(kv_heads), int(head_dim))
         if buffers is None:
             buffers = (torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device),
@@ -676,7 +689,7 @@ class HistoryCache:
 
 def history_attention(q, k, v, cache, scale=None):
     """Attention of one token of each env over what `cache` holds of its episode, the token itself among it: what ``episode_attention`` gives for the
-    episode's last token, with the cache's capacity as the window.  q: envs x heads x dim, k and v: envs x key heads x dim, in the cache's type, at any stride; k and v are
+    episode's last token, with the cache's capacity as the window (less its sinks, where it has some, and with them as sinks).  q: envs x heads x dim, k and v: envs x key heads x dim, in the cache's type, at any stride; k and v are
     written into the cache.  scale: dim^-0.5 unless given.  Returns envs x heads x dim.  Probabilities are rounded to the cache's type, sums are in 32 bits.  No gradient."""
     device = _on_gpu(q, k, v, cache.keys)
     envs, capacity, heads_k, dim = cache.keys.shape
@@ -693,7 +706,10 @@ def history_attention(q, k, v, cache, scale=None):
     desc = _abi.HistoryDesc(_DTYPES[dtype], envs, capacity, q.shape[1], heads_k, dim, dim ** -0.5 if scale is None else float(scale), q.data_ptr(), k.data_ptr(), v.data_ptr(),
                             _stride(q, 0), _stride(q, 1), _stride(k, 0), _stride(k, 1), _stride(v, 0), _stride(v, 1), cache.keys.data_ptr(), cache.values.data_ptr(),
                             cache.position.data_ptr(), out.data_ptr(), *workspace[:2])
-    stream = _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
+    if cache.sinks:
+        stream = _call(device, _abi.lib().nuka_b200_history_sinks, ctypes.byref(desc), cache.sinks)
+    else:
+        stream = _call(device, _abi.lib().nuka_b200_history, ctypes.byref(desc))
     if workspace[3] is None:
         workspace[3] = stream
     elif workspace[1] and stream != workspace[3]:

@@ -23,15 +23,8 @@ struct ConvolutionParams {
     const void *x, *initial, *dy, *dstate;
     void *y, *state, *dx, *dinitial;
     float* partial;                                     // of the weights' gradients: across x (K + 1) x channels
-    bool silu, sums;
+    bool act, sums;
 };
-
-// s / (1 + exp(-s)) and its derivative.
-__device__ __forceinline__ float silu_of(float s) { return s / (1.f + expf(-s)); }
-__device__ __forceinline__ float silu_slope(float s) {
-    const float r = 1.f / (1.f + expf(-s));
-    return r * fmaf(s, 1.f - r, 1.f);
-}
 
 template <typename T, int K, int VEC> struct Line {
     float w[K][VEC], bias[VEC];
@@ -112,9 +105,9 @@ __global__ void __launch_bounds__(kLines * 32) convolution_kernel(const Convolut
             window[K - 1] = next[i];
             float s[VEC];
             f.sum(window, s);
-            if (p.silu)
+            if (p.act)
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) s[v] = silu_of(s[v]);
+                for (int v = 0; v < VEC; ++v) s[v] = silu<sizeof(T) == 4>(s[v]);
             store<T, VEC>(static_cast<T*>(p.y) + t * C + c, s);
             if (tail[i] >= 0)
 #pragma unroll
@@ -197,11 +190,11 @@ __global__ void __launch_bounds__(kLines * 32) convolution_grad_kernel(const Con
                 window[K - 1] = xs[i];
                 float ds[VEC];
                 unpack<T, VEC>(dys[i], ds);
-                if (p.silu) {
+                if (p.act) {
                     float s[VEC];
                     f.sum(window, s);
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) ds[v] *= silu_slope(s[v]);
+                    for (int v = 0; v < VEC; ++v) ds[v] *= silu_slope<sizeof(T) == 4>(s[v]);
                 }
 #pragma unroll
                 for (int j = 0; j < K; ++j)
@@ -297,7 +290,7 @@ template <typename T, int VEC> static ConvolutionParams convolution_params(const
     p.stretches = (p.plan.tokens + p.stretch - 1) / p.stretch;
     p.tiles = (uint32_t)((d.channels + 32 * VEC - 1) / (32 * VEC));
     p.across = (uint32_t)((p.stretches + kLines - 1) / kLines);
-    p.weight = d.weight; p.bias = d.bias; p.silu = d.silu != 0u;
+    p.weight = d.weight; p.bias = d.bias; p.act = d.silu != 0u;
     p.x = d.x; p.initial = d.initial; p.dy = d.dy; p.dstate = d.dstate;
     p.y = d.y; p.state = d.state; p.dx = d.dx; p.dinitial = d.dinitial;
     return p;
@@ -370,7 +363,7 @@ __global__ void convolution_step_kernel(int64_t groups, uint32_t per_env, const 
     }
     if (d.silu)
 #pragma unroll
-        for (int v = 0; v < VEC; ++v) sum[v] = silu_of(sum[v]);
+        for (int v = 0; v < VEC; ++v) sum[v] = silu<sizeof(T) == 4>(sum[v]);
     store<T, VEC>(static_cast<T*>(d.y) + env * d.channels + c, sum);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) *reinterpret_cast<Raw<T, VEC>*>(state + j * d.channels) = window[j + 1];

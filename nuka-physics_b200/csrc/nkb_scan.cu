@@ -16,14 +16,17 @@
 namespace nkb {
 
 constexpr int kScanWarps = 4;                           // of a block
+template <int N> struct Flag { static constexpr int value = N; };
 constexpr float kToBase2 = 1.4426950408889634f, kFromBase2 = 0.6931471805599453f;
 
 // LN: lanes over the states
 template <int LN> struct ScanTile {
     static constexpr int kChannelLanes = 32 / LN, kChannels = 4 * kChannelLanes, kStates = 4 * LN;
-    static constexpr int kChunk = LN == 4 || LN == 8 ? 8 : 4;
-    static constexpr int kEach = kChunk * kChannels / 32, kNarrow = kChunk * kStates / 32;          // of a lane: values of a chunk, and of its B
-    static constexpr int kCells = kChunk * kChannels;
+    static constexpr int kChunk = LN == 2 ? 4 : 8;
+    // what a lane loads and works out of a chunk before and after the states: neighbouring channels of one token; of B and C neighbouring states
+    static constexpr int kEach = kChunk * kChannels / 32, kNarrow = kChunk * kStates / 32;
+    static constexpr int kRow = kChannels + 4;          // floats between a chunk's tokens in shared memory: neighbouring tokens' reads meet different banks
+    static constexpr int kCells = kChunk * kRow;
 };
 
 struct ScanParams {
@@ -31,18 +34,17 @@ struct ScanParams {
     int64_t channels, states, x_stride, delta_stride, gate_stride, b_stride, c_stride, segment, segments, chunks;           // chunks: of a segment
     uint32_t tiles, workers;                            // of the channels; warps of a tile backwards
     bool alone;                                         // every segment is whole rows
+    bool wide, wide_states;                             // a lane's loads and stores of a chunk go in one piece; those of states two at a time
     const void *x, *delta, *gate, *b, *c, *dy;
     const float *decay, *skip, *delta_bias, *initial, *dstate;
     void *y, *dx, *ddelta, *dgate;
     float *state, *dinitial;
     float4* kept;                                       // segments x chunks x tiles x 4 x 32
     float *maps, *sums;                                 // segments x tiles x 512, and segments x tiles x channels of a tile; below 0 where what came before is forgotten
-    float *db, *dc;                                     // tiles x tokens x states of a tile, each
+    float* db;                                          // tiles x tokens x states of a tile, and the same of C
+    int64_t dc_after;
     float *ddecay, *dskip, *dbias;                      // workers x tiles x 512, and workers x tiles x channels of a tile
 };
-
-__device__ __forceinline__ float softplus(float u) { return u > 20.f ? u : log1pf(expf(u)); }                 // above, exp(-u) is less than half a unit of u
-__device__ __forceinline__ float logistic(float u) { return 1.f / (1.f + expf(-u)); }
 
 // Sums over the LANES lanes that lie STRIDE apart: each time a lane keeps half of its values, as long as it has some to give. Afterwards it has max(1, COUNT / LANES) of them, from `first` on.
 template <int COUNT, int LANES, int STRIDE> __device__ __forceinline__ void sum_lanes(float (&v)[COUNT], int lane) {
@@ -62,93 +64,247 @@ template <int COUNT, int LANES, int STRIDE> __device__ __forceinline__ void sum_
         }
     }
 }
+// The same of four values whose first two are the lane's to keep (States).
+template <int LN> __device__ __forceinline__ void sum_states(Pair low, Pair high, float (&v)[2], int lane) {
+    float give[2];
+    split(low, v[0], v[1]);
+    split(high, give[0], give[1]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) v[i] += __shfl_xor_sync(~0u, give[i], LN / 2);
+    sum_lanes<2, LN / 2, 1>(v, lane);
+}
 template <int COUNT, int LANES> struct Kept {
     static constexpr int kCount = COUNT > LANES ? COUNT / LANES : 1, kShare = LANES > COUNT ? LANES / COUNT : 1;
     static __device__ __forceinline__ int first(int group) { return group / kShare * kCount; }
     static __device__ __forceinline__ bool owner(int group) { return group % kShare == 0; }
 };
 
+// N neighbouring values, in pieces of at most 16 bytes.
+template <typename T, int N> struct Piece {
+    static constexpr int kPer = sizeof(T) * N > 16 ? 16 / sizeof(T) : N, kCount = N / kPer;
+    Raw<T, kPer> raw[kCount];
+    __device__ __forceinline__ void load(const T* from, int there, bool wide) {
+        if (wide && there >= N) {
+#pragma unroll
+            for (int k = 0; k < kCount; ++k) raw[k] = load_raw<T, kPer>(from + k * kPer);
+        } else {
+            T v[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) v[k] = k < there ? from[k] : from_float<T>(0.f);
+#pragma unroll
+            for (int k = 0; k < kCount; ++k) {
+                float f[kPer];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) f[e] = to_float<T>(v[k * kPer + e]);
+                nkb::store<T, kPer>(reinterpret_cast<T*>(&raw[k]), f);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[N]) const {
+#pragma unroll
+        for (int k = 0; k < kCount; ++k) {
+            float f[kPer];
+            unpack<T, kPer>(raw[k], f);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[k * kPer + e] = f[e];
+        }
+    }
+    static __device__ __forceinline__ void store(T* to, const float (&v)[N], int there, bool wide) {
+        if (wide && there >= N) {
+#pragma unroll
+            for (int k = 0; k < kCount; ++k) {
+                float f[kPer];
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) f[e] = v[k * kPer + e];
+                nkb::store<T, kPer>(to + k * kPer, f);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k)
+                if (k < there) to[k] = from_float<T>(v[k]);
+        }
+    }
+};
+
+// A lane's sixteen states: h[j][i] are those of its pair j of channels for its state i. The lanes of the upper half of a channel group have its two pairs in the other order, and those of the upper half of the
+// channel groups the two halves of their four states: what a lane gives away first of its sums then lies in the same registers in all lanes.
+struct States {
+    Pair h[2][4];
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) h[j][i] = pair_of(0.f, 0.f);
+    }
+    // in the lanes' order: four times 32 x 16 bytes, one of each state
+    __device__ __forceinline__ void load(const float4* from) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(from + 32 * i);
+            h[0][i] = v.x; h[1][i] = v.y;
+        }
+    }
+    __device__ __forceinline__ void store(float4* to) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<ulonglong2*>(to + 32 * i) = make_ulonglong2(h[0][i], h[1][i]);
+    }
+};
+__device__ __forceinline__ Pair exp2_pair(Pair v) {
+    float a, b;
+    split(v, a, b);
+    return pair_of(exp2_fast(a), exp2_fast(b));
+}
+// How a lane's own order goes through its channels and states: upper_j, upper_i 0 or 2.
+struct Order {
+    int upper_j, upper_i;
+    __device__ __forceinline__ void two_pairs(const float* from, Pair (&v)[2]) const {
+        v[0] = *reinterpret_cast<const Pair*>(from + upper_j); v[1] = *reinterpret_cast<const Pair*>(from + 2 - upper_j);
+    }
+    __device__ __forceinline__ void four_pairs(const float2* from, Pair (&v)[4]) const {
+        const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(from + upper_i), q = *reinterpret_cast<const ulonglong2*>(from + 2 - upper_i);
+        v[0] = r.x; v[1] = r.y; v[2] = q.x; v[3] = q.y;
+    }
+};
+
 template <typename T, int LN> struct ScanLane {
     using S = ScanTile<LN>;
+    using Each = Piece<T, S::kEach>;
+    using Narrow = Piece<T, S::kNarrow>;
     int lane, nl, cl;
     int64_t c0;                                         // the tile's first channel
     int count, states;                                  // channels and states that there are of the tile
-    float rate[4][4];                                   // A log2(e)
+    int token, channel, own;                            // of the lane's share of a chunk: its token, its first channel, and how many there are
+    int narrow_token, narrow_state, narrow_own;
+    Order order;
+    States rate;                                        // A log2(e)
     __device__ __forceinline__ ScanLane(const ScanParams& p, int64_t tile) {
         lane = threadIdx.x % 32; nl = lane % LN; cl = lane / LN;
+        order.upper_j = nl / (LN / 2) * 2; order.upper_i = cl / (S::kChannelLanes / 2) * 2;
         c0 = tile * S::kChannels;
         count = (int)min((int64_t)S::kChannels, p.channels - c0); states = (int)p.states;
-        each(p.decay, 0, rate);
+        token = lane * S::kEach / S::kChannels; channel = lane * S::kEach % S::kChannels; own = count - channel;
+        narrow_token = lane * S::kNarrow / S::kStates; narrow_state = lane * S::kNarrow % S::kStates; narrow_own = states - narrow_state;
+        each(p, p.decay, 0, rate);
+        const Pair to = pair_of(kToBase2, kToBase2);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) rate[j][i] *= kToBase2;
+            for (int i = 0; i < 4; ++i) rate.h[j][i] = mul_pair(rate.h[j][i], to);
     }
     // the lane's values of row `row` of rows x channels x states; 0 where there are none
-    __device__ __forceinline__ void each(const float* from, int64_t row, float (&v)[4][4], int64_t channels = 0) const {
+    __device__ __forceinline__ void each(const ScanParams& p, const float* from, int64_t row, States& v) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 2; ++j) {
+            float f[2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = 4 * cl + j, n = 4 * nl + i;
-                v[j][i] = from != nullptr && c < count && n < states ? from[(row * channels + c0 + c) * states + n] : 0.f;
+            for (int e = 0; e < 2; ++e) {
+                const int c = 4 * cl + (2 * j ^ order.upper_j) + e;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const int n = 4 * nl + (i ^ order.upper_i);
+                    const float* const at = from + (row * p.channels + c0 + c) * states + n;
+                    const int there = from != nullptr && c < count ? states - n : 0;
+                    if (p.wide_states && there >= 2) {
+                        const float2 q = *reinterpret_cast<const float2*>(at);
+                        f[e][i] = q.x; f[e][i + 1] = q.y;
+                    } else {
+                        f[e][i] = there > 0 ? at[0] : 0.f; f[e][i + 1] = there > 1 ? at[1] : 0.f;
+                    }
+                }
             }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v.h[j][i] = pair_of(f[0][i], f[1][i]);
+        }
     }
-    __device__ __forceinline__ void give(float* to, int64_t row, const float (&v)[4][4], int64_t channels) const {
+    __device__ __forceinline__ void give(const ScanParams& p, float* to, int64_t row, const States& v) const {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int j = 0; j < 2; ++j) {
+            float f[2][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int c = 4 * cl + j, n = 4 * nl + i;
-                if (c < count && n < states) to[(row * channels + c0 + c) * states + n] = v[j][i];
+            for (int i = 0; i < 4; ++i) split(v.h[j][i], f[0][i], f[1][i]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int c = 4 * cl + (2 * j ^ order.upper_j) + e;
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const int n = 4 * nl + (i ^ order.upper_i);
+                    float* const at = to + (row * p.channels + c0 + c) * states + n;
+                    const int there = c < count ? states - n : 0;
+                    if (p.wide_states && there >= 2) {
+                        *reinterpret_cast<float2*>(at) = make_float2(f[e][i], f[e][i + 1]);
+                    } else {
+                        if (there > 0) at[0] = f[e][i];
+                        if (there > 1) at[1] = f[e][i + 1];
+                    }
+                }
             }
+        }
     }
-    // value number k of the lane's share of a chunk: its token and channel; of B or C: its token and state
-    __device__ __forceinline__ int token_of(int k) const { return (lane + 32 * k) / S::kChannels; }
-    __device__ __forceinline__ int channel_of(int k) const { return (lane + 32 * k) % S::kChannels; }
-    __device__ __forceinline__ int narrow_token(int k) const { return (lane + 32 * k) / S::kStates; }
-    __device__ __forceinline__ int narrow_state(int k) const { return (lane + 32 * k) % S::kStates; }
     // tokens t0 to t0 + left - 1
-    __device__ __forceinline__ void load(const void* from, int64_t stride, int64_t t0, int left, T (&v)[S::kEach]) const {
+    __device__ __forceinline__ void load(const ScanParams& p, const void* from, int64_t stride, int64_t t0, int left, Each& v) const {
+        v.load(static_cast<const T*>(from) + (t0 + token) * stride + c0 + channel, token < left ? own : 0, p.wide);
+    }
+    __device__ __forceinline__ void load_narrow(const ScanParams& p, const void* from, int64_t stride, int64_t t0, int left, Narrow& v) const {
+        v.load(static_cast<const T*>(from) + (t0 + narrow_token) * stride + narrow_state, narrow_token < left ? narrow_own : 0, p.wide);
+    }
+    __device__ __forceinline__ void store(const ScanParams& p, void* to, int64_t t0, int left, const float (&v)[S::kEach]) const {
+        Each::store(static_cast<T*>(to) + (t0 + token) * p.channels + c0 + channel, v, token < left ? own : 0, p.wide);
+    }
+    // values per channel, of the lane's
+    __device__ __forceinline__ void of_channels(const float* from, float (&v)[S::kEach]) const {
 #pragma unroll
-        for (int k = 0; k < S::kEach; ++k) {
-            const int t = token_of(k), c = channel_of(k);
-            v[k] = t < left && c < count ? static_cast<const T*>(from)[(t0 + t) * stride + c0 + c] : from_float<T>(0.f);
+        for (int k = 0; k < S::kEach; ++k) v[k] = from != nullptr && k < own ? from[c0 + channel + k] : 0.f;
+    }
+    __device__ __forceinline__ float* cell(float* of) const { return of + token * S::kRow + channel; }
+    // each value of B or C twice, as it meets two channels
+    __device__ __forceinline__ void put_narrow(float2* to, const Narrow& v) const {
+        float f[S::kNarrow];
+        v.get(f);
+        float2* const at = to + narrow_token * S::kStates + narrow_state;
+        if constexpr (S::kNarrow % 2 == 0) {
+#pragma unroll
+            for (int k = 0; k < S::kNarrow; k += 2) *reinterpret_cast<float4*>(at + k) = make_float4(f[k], f[k], f[k + 1], f[k + 1]);
+        } else {
+#pragma unroll
+            for (int k = 0; k < S::kNarrow; ++k) at[k] = make_float2(f[k], f[k]);
         }
     }
-    __device__ __forceinline__ void load_narrow(const void* from, int64_t stride, int64_t t0, int left, T (&v)[S::kNarrow]) const {
-#pragma unroll
-        for (int k = 0; k < S::kNarrow; ++k) {
-            const int t = narrow_token(k), n = narrow_state(k);
-            v[k] = t < left && n < states ? static_cast<const T*>(from)[(t0 + t) * stride + n] : from_float<T>(0.f);
-        }
-    }
-    __device__ __forceinline__ float bias(const ScanParams& p, int k) const { const int c = channel_of(k); return p.delta_bias != nullptr && c < count ? p.delta_bias[c0 + c] : 0.f; }
-    __device__ __forceinline__ float skip(const ScanParams& p, int k) const { const int c = channel_of(k); return p.skip != nullptr && c < count ? p.skip[c0 + c] : 0.f; }
-    __device__ __forceinline__ bool there(int k, int left) const { return token_of(k) < left && channel_of(k) < count; }
 };
+template <int N> __device__ __forceinline__ void put(float* to, const float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(to + k) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) to[k] = v[k];
+    }
+}
+template <int N> __device__ __forceinline__ void take(const float* from, float (&v)[N]) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int k = 0; k < N; k += 4) { const float4 q = *reinterpret_cast<const float4*>(from + k); v[k] = q.x; v[k + 1] = q.y; v[k + 2] = q.z; v[k + 3] = q.w; }
+    } else {
+#pragma unroll
+        for (int k = 0; k < N; ++k) v[k] = from[k];
+    }
+}
 
-// What a warp's states read of a chunk.
+// What a warp's states read of a chunk, and what they give.
 template <int LN> struct __align__(16) ScanShared {
     using S = ScanTile<LN>;
     float dt[S::kCells], in[S::kCells], out[S::kCells];
-    float b[S::kChunk * S::kStates], c[S::kChunk * S::kStates];
+    float2 b[S::kChunk * S::kStates], c[S::kChunk * S::kStates];
 };
-__device__ __forceinline__ void four(const float* from, float (&v)[4]) {
-    const float4 f = *reinterpret_cast<const float4*>(from);
-    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
-}
 
-// A segment's sums of dt, of each channel those that lie in the lanes and numbers that have it.
-template <int LN> __device__ __forceinline__ void give_totals(const ScanParams& p, ScanShared<LN>& m, const float (&total)[ScanTile<LN>::kEach], int lane, int64_t map, bool closed) {
+// A segment's sums of dt: of each channel those of the lanes that have it.
+template <int LN> __device__ __forceinline__ void give_totals(const ScanParams& p, ScanShared<LN>& m, float* cell, const float (&total)[ScanTile<LN>::kEach], int lane, int64_t map, bool closed) {
     using S = ScanTile<LN>;
     __syncwarp();
-#pragma unroll
-    for (int k = 0; k < S::kEach; ++k) m.out[lane + 32 * k] = total[k];
+    put(cell, total);
     __syncwarp();
     for (int ch = lane; ch < S::kChannels; ch += 32) {
         float sum = 0.f;
-        for (int t = 0; t < S::kChunk; ++t) sum += m.out[t * S::kChannels + ch];
+        for (int t = 0; t < S::kChunk; ++t) sum += m.out[t * S::kRow + ch];
         p.sums[map * S::kChannels + ch] = closed ? -1.f : sum;
     }
 }
@@ -156,104 +312,137 @@ template <int LN> __device__ __forceinline__ void give_totals(const ScanParams& 
 // ---- forwards ----------------------------------------------------------------------------------------------------------
 // MAPS: only what the segment does to the state
 template <typename T, int LN, bool MAPS>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanParams p) {
     using S = ScanTile<LN>;
+    constexpr int E = S::kEach;
     __shared__ ScanShared<LN> all[kScanWarps];
     ScanShared<LN>& m = all[threadIdx.x / 32];
     const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, segment = job / p.tiles, tile = job % p.tiles;
     if (segment >= p.segments) return;
     const ScanLane<T, LN> l(p, tile);
     const int64_t begin = segment * p.segment, end = min(begin + p.segment, p.plan.tokens);
-    float h[4][4] = {}, total[S::kEach] = {};           // total: of dt, of the lane's own values
+    States h;
+    h.clear();
+    float total[E] = {}, bias[E], skip[E];              // total: of dt, of the lane's own values
+    l.of_channels(p.delta_bias, bias);
+    l.of_channels(p.skip, skip);
     bool closed = false;
     float4* const maps = p.alone ? nullptr : reinterpret_cast<float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane;
-    if (!MAPS && maps != nullptr)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) { const float4 v = maps[32 * j]; h[j][0] = v.x; h[j][1] = v.y; h[j][2] = v.z; h[j][3] = v.w; }
-    T x[S::kEach], delta[S::kEach], gate[S::kEach], b[S::kNarrow], c[S::kNarrow];
+    if (!MAPS && maps != nullptr) h.load(maps);
+    typename ScanLane<T, LN>::Each x, delta, gate;
+    typename ScanLane<T, LN>::Narrow b, c;
     int32_t link, tail;                                 // of token number `lane` of the chunk
     auto fetch = [&](int64_t t0) {
         const int left = (int)min((int64_t)S::kChunk, end - t0);
         if (left <= 0) return;
-        l.load(p.x, p.x_stride, t0, left, x);
-        l.load(p.delta, p.delta_stride, t0, left, delta);
-        l.load_narrow(p.b, p.b_stride, t0, left, b);
-        if (!MAPS) l.load_narrow(p.c, p.c_stride, t0, left, c);
-        if (!MAPS && p.gate != nullptr) l.load(p.gate, p.gate_stride, t0, left, gate);
+        l.load(p, p.x, p.x_stride, t0, left, x);
+        l.load(p, p.delta, p.delta_stride, t0, left, delta);
+        l.load_narrow(p, p.b, p.b_stride, t0, left, b);
+        if (!MAPS) l.load_narrow(p, p.c, p.c_stride, t0, left, c);
+        if (!MAPS && p.gate != nullptr) l.load(p, p.gate, p.gate_stride, t0, left, gate);
         link = l.lane < left ? p.plan.link[t0 + l.lane] : -1;
         tail = l.lane < left ? p.plan.tail[t0 + l.lane] : -1;
     };
     fetch(begin);
     int64_t chunk = segment * p.chunks;
     for (int64_t t0 = begin; t0 < end; t0 += S::kChunk, ++chunk) {
-        const int left = (int)min((int64_t)S::kChunk, end - t0);
+        const int left = (int)min((int64_t)S::kChunk, end - t0), there = l.token < left ? l.own : 0;
         const uint32_t begins = __ballot_sync(~0u, link != -1), ends = __ballot_sync(~0u, tail >= 0);
         const int32_t links = link, tails = tail;
-        float xs[S::kEach], zs[S::kEach];
+        typename ScanLane<T, LN>::Each x_now = x, gate_now = gate;
+        {
+            float xs[E], us[E];
+            x.get(xs);
+            delta.get(us);
 #pragma unroll
-        for (int k = 0; k < S::kEach; ++k) {
-            xs[k] = to_float<T>(x[k]);
-            if (!MAPS && p.gate != nullptr) zs[k] = to_float<T>(gate[k]);
-            const float dt = l.there(k, left) ? softplus(to_float<T>(delta[k]) + l.bias(p, k)) : 0.f;
-            if (MAPS) total[k] += dt;
-            m.dt[l.lane + 32 * k] = dt;
-            m.in[l.lane + 32 * k] = dt * xs[k];
+            for (int k = 0; k < E; ++k) {
+                const float u = us[k] + bias[k];
+                us[k] = softplus(u, fading<true>(u));
+                xs[k] *= us[k];
+                if (MAPS && there > 0) total[k] += us[k];
+            }
+            put(l.cell(m.dt), us);
+            put(l.cell(m.in), xs);
         }
-#pragma unroll
-        for (int k = 0; k < S::kNarrow; ++k) {
-            m.b[l.lane + 32 * k] = to_float<T>(b[k]);
-            if (!MAPS) m.c[l.lane + 32 * k] = to_float<T>(c[k]);
-        }
+        l.put_narrow(m.b, b);
+        if (!MAPS) l.put_narrow(m.c, c);
         __syncwarp();
         fetch(t0 + S::kChunk);
-        if (!MAPS && p.kept != nullptr)
+        if (!MAPS && p.kept != nullptr) h.store(p.kept + (chunk * p.tiles + tile) * 128 + l.lane);
+        auto begin_at = [&](int t) {
+            const int32_t row = __shfl_sync(~0u, links, t);
+            if (row >= 0) l.each(p, p.initial, row, h); else h.clear();
+            closed = true;
+        };
+        auto token = [&](int t) {
+            Pair dt[2], in[2], bs[4];
+            l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
+            l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, in);
+            l.order.four_pairs(m.b + t * S::kStates + 4 * l.nl, bs);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p.kept[((chunk * p.tiles + tile) * 4 + j) * 32 + l.lane] = make_float4(h[j][0], h[j][1], h[j][2], h[j][3]);
-#pragma unroll 2
-        for (int t = 0; t < left; ++t) {
-            if (begins >> t & 1u) {
-                const int32_t row = __shfl_sync(~0u, links, t);
-                l.each(row >= 0 ? p.initial : nullptr, row, h, p.channels);
-                closed = true;
-            }
-            float dt[4], in[4], bs[4];
-            four(m.dt + t * S::kChannels + 4 * l.cl, dt);
-            four(m.in + t * S::kChannels + 4 * l.cl, in);
-            four(m.b + t * S::kStates + 4 * l.nl, bs);
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) h[j][i] = fmaf(exp2_fast(dt[j] * l.rate[j][i]), h[j][i], in[j] * bs[i]);
+                for (int i = 0; i < 4; ++i) h.h[j][i] = fma_pair(exp2_pair(mul_pair(dt[j], l.rate.h[j][i])), h.h[j][i], mul_pair(in[j], bs[i]));
             if constexpr (!MAPS) {
-                float cs[4], y[4] = {};
-                four(m.c + t * S::kStates + 4 * l.nl, cs);
+                Pair cs[4];
+                l.order.four_pairs(m.c + t * S::kStates + 4 * l.nl, cs);
+                Pair sum[2];
+                float y[2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 2; ++j) {
+                    sum[j] = mul_pair(cs[0], h.h[j][0]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) y[j] = fmaf(cs[i], h[j][i], y[j]);
-                sum_lanes<4, LN, 1>(y, l.lane);
+                    for (int i = 1; i < 4; ++i) sum[j] = fma_pair(cs[i], h.h[j][i], sum[j]);
+                }
+                sum_states<LN>(sum[0], sum[1], y, l.lane);
                 using K = Kept<4, LN>;
                 if (K::owner(l.nl))
 #pragma unroll
-                    for (int i = 0; i < K::kCount; ++i) m.out[t * S::kChannels + 4 * l.cl + K::first(l.nl) + i] = y[i];
-                if (ends >> t & 1u) l.give(p.state, __shfl_sync(~0u, tails, t), h, p.channels);
+                    for (int i = 0; i < K::kCount; ++i) m.out[t * S::kRow + 4 * l.cl + K::first(l.nl) + i] = y[i];
+            }
+        };
+        // most chunks are whole, and nothing begins or ends but at their edges
+        if (left == S::kChunk && (begins & ~1u) == 0u && (ends & ~(1u << (S::kChunk - 1))) == 0u) {
+            if (begins != 0u) begin_at(0);
+#pragma unroll
+            for (int t = 0; t < S::kChunk; ++t) token(t);
+            if (!MAPS && ends != 0u) l.give(p, p.state, __shfl_sync(~0u, tails, S::kChunk - 1), h);
+        } else {
+#pragma unroll 1
+            for (int t = 0; t < left; ++t) {
+                if (begins >> t & 1u) begin_at(t);
+                token(t);
+                if (!MAPS && ends >> t & 1u) l.give(p, p.state, __shfl_sync(~0u, tails, t), h);
             }
         }
         __syncwarp();
-        if constexpr (!MAPS)
+        if constexpr (!MAPS) {
+            float y[E], xs[E];
+            take(l.cell(m.out), y);
+            x_now.get(xs);
 #pragma unroll
-            for (int k = 0; k < S::kEach; ++k)
-                if (l.there(k, left)) {
-                    float y = fmaf(l.skip(p, k), xs[k], m.out[l.lane + 32 * k]);
-                    if (p.gate != nullptr) y *= zs[k] * logistic(zs[k]);
-                    static_cast<T*>(p.y)[(t0 + l.token_of(k)) * p.channels + l.c0 + l.channel_of(k)] = from_float<T>(y);
-                }
+            for (int k = 0; k < E; ++k) y[k] = fmaf(skip[k], xs[k], y[k]);
+            if (p.gate != nullptr) {
+                float z[E];
+                gate_now.get(z);
+#pragma unroll
+                for (int k = 0; k < E; ++k) y[k] *= silu<sizeof(T) == 4>(z[k]);
+            }
+            l.store(p, p.y, t0, left, y);
+            __syncwarp();
+        }
     }
     if constexpr (MAPS) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) maps[32 * j] = make_float4(h[j][0], h[j][1], h[j][2], h[j][3]);
-        give_totals<LN>(p, m, total, l.lane, segment * p.tiles + tile, closed);
+        h.store(maps);
+        give_totals<LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
     }
+}
+
+// Of the 512 states of a tile in the lanes' order, number `place`: its channel and state.
+template <int LN> __device__ __forceinline__ void place_of(int place, int& c, int& n) {
+    const int of = place % 128 / 4, upper_j = of % LN / (LN / 2) * 2, upper_i = of / LN / (16 / LN) * 2;
+    c = 4 * (of / LN) + (place % 4 ^ upper_j);
+    n = 4 * (of % LN) + (place / 128 ^ upper_i);
 }
 
 // What each segment begins with (backwards: what goes back into its last token), in place of its map: a block per 32 of a tile's 512 states, its warps a run of segments each, joined, then walked again.
@@ -261,8 +450,10 @@ template <int LN, bool BACKWARD> __global__ void __launch_bounds__(1024) scan_ca
     using S = ScanTile<LN>;
     __shared__ float2 runs[32][32];
     const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    const int64_t tile = blockIdx.x / 16, place = (blockIdx.x % 16) * 32 + lane, each = (p.segments + 31) / 32, begin = min(p.segments, warp * each), end = min(p.segments, begin + each);
-    const int j = (int)place / 128, of = (int)place % 128 / 4, c = 4 * (of / LN) + j, n = 4 * (of % LN) + (int)place % 4;
+    const int64_t tile = blockIdx.x / 16, each = (p.segments + 31) / 32, begin = min(p.segments, warp * each), end = min(p.segments, begin + each);
+    const int place = (int)(blockIdx.x % 16) * 32 + lane;
+    int c, n;
+    place_of<LN>(place, c, n);
     const int64_t channel = tile * S::kChannels + c;
     const float rate = channel < p.channels && n < p.states ? p.decay[channel * p.states + n] * kToBase2 : 0.f;
     auto map_of = [&](int64_t k) -> float& { return p.maps[((BACKWARD ? p.segments - 1 - k : k) * p.tiles + tile) * 512 + place]; };
@@ -289,252 +480,334 @@ template <int LN, bool BACKWARD> __global__ void __launch_bounds__(1024) scan_ca
 template <int LN> struct __align__(16) ScanGradShared {
     using S = ScanTile<LN>;
     float4 before[S::kChunk * 4 * 32];                  // the states before each token, in the lanes' order
-    float dt[S::kCells], in[S::kCells], dy[S::kCells], out[S::kCells], by_b[S::kCells], by_a[S::kCells];
-    float b[S::kChunk * S::kStates], c[S::kChunk * S::kStates];
+    float dt[S::kCells], dy[S::kCells], slope[S::kCells], gate[S::kCells], out[S::kCells], by_a[S::kCells];         // slope: of dt; gate: what y's gradient of the gate is multiplied with
+    float in[S::kCells];                                // dt x, and when the token is done sum of m B
+    float2 b[S::kChunk * S::kStates], c[S::kChunk * S::kStates];
 };
 
 // What goes back through a segment from 0: m_t = C dy + a_{t+1} m_{t+1}, times a_t of its first token
 template <typename T, int LN>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_back_maps_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(const ScanParams p) {
     using S = ScanTile<LN>;
+    constexpr int E = S::kEach;
     __shared__ ScanShared<LN> all[kScanWarps];
     ScanShared<LN>& m = all[threadIdx.x / 32];
     const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, segment = job / p.tiles, tile = job % p.tiles;
     if (segment >= p.segments) return;
     const ScanLane<T, LN> l(p, tile);
     const int64_t begin = segment * p.segment, end = min(begin + p.segment, p.plan.tokens), chunks = (end - begin + S::kChunk - 1) / S::kChunk;
-    float back[4][4] = {}, total[S::kEach] = {};
+    States back;
+    back.clear();
+    float total[E] = {}, bias[E];
+    l.of_channels(p.delta_bias, bias);
     bool closed = false;
-    T dy[S::kEach], delta[S::kEach], gate[S::kEach], c[S::kNarrow];
+    typename ScanLane<T, LN>::Each dy, delta, gate;
+    typename ScanLane<T, LN>::Narrow c;
     int32_t link, tail;
     auto fetch = [&](int64_t k) {
         if (k < 0) return;
         const int64_t t0 = begin + k * S::kChunk;
         const int left = (int)min((int64_t)S::kChunk, end - t0);
-        l.load(p.dy, p.channels, t0, left, dy);
-        l.load(p.delta, p.delta_stride, t0, left, delta);
-        if (p.gate != nullptr) l.load(p.gate, p.gate_stride, t0, left, gate);
-        l.load_narrow(p.c, p.c_stride, t0, left, c);
+        l.load(p, p.dy, p.channels, t0, left, dy);
+        l.load(p, p.delta, p.delta_stride, t0, left, delta);
+        if (p.gate != nullptr) l.load(p, p.gate, p.gate_stride, t0, left, gate);
+        l.load_narrow(p, p.c, p.c_stride, t0, left, c);
         link = l.lane < left ? p.plan.link[t0 + l.lane] : -1;
         tail = l.lane < left ? p.plan.tail[t0 + l.lane] : -1;
     };
     fetch(chunks - 1);
     for (int64_t k0 = chunks - 1; k0 >= 0; --k0) {
         const int64_t t0 = begin + k0 * S::kChunk;
-        const int left = (int)min((int64_t)S::kChunk, end - t0);
+        const int left = (int)min((int64_t)S::kChunk, end - t0), there = l.token < left ? l.own : 0;
         const uint32_t begins = __ballot_sync(~0u, link != -1), ends = __ballot_sync(~0u, tail >= 0);
         const int32_t tails = tail;
+        {
+            float us[E], ds[E];
+            delta.get(us);
+            dy.get(ds);
 #pragma unroll
-        for (int k = 0; k < S::kEach; ++k) {
-            const float dt = l.there(k, left) ? softplus(to_float<T>(delta[k]) + l.bias(p, k)) : 0.f;
-            float d = to_float<T>(dy[k]);
-            if (p.gate != nullptr) { const float z = to_float<T>(gate[k]); d *= z * logistic(z); }
-            total[k] += dt;
-            m.dt[l.lane + 32 * k] = dt;
-            m.in[l.lane + 32 * k] = d;
+            for (int k = 0; k < E; ++k) {
+                const float u = us[k] + bias[k];
+                us[k] = softplus(u, fading<true>(u));
+                if (there > 0) total[k] += us[k];
+            }
+            if (p.gate != nullptr) {
+                float z[E];
+                gate.get(z);
+#pragma unroll
+                for (int k = 0; k < E; ++k) ds[k] *= silu<sizeof(T) == 4>(z[k]);
+            }
+            put(l.cell(m.dt), us);
+            put(l.cell(m.in), ds);
         }
-#pragma unroll
-        for (int k = 0; k < S::kNarrow; ++k) m.c[l.lane + 32 * k] = to_float<T>(c[k]);
+        l.put_narrow(m.c, c);
         __syncwarp();
         fetch(k0 - 1);
-#pragma unroll 2
-        for (int t = left - 1; t >= 0; --t) {
-            if (ends >> t & 1u) {
-                float more[4][4];
-                l.each(p.dstate, __shfl_sync(~0u, tails, t), more, p.channels);
+        auto end_at = [&](int t) {
+            const int32_t row = __shfl_sync(~0u, tails, t);
+            if (p.dstate == nullptr) return;
+            States more;
+            l.each(p, p.dstate, row, more);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) back[j][i] += more[j][i];
-            }
-            float dt[4], d[4], cs[4];
-            four(m.dt + t * S::kChannels + 4 * l.cl, dt);
-            four(m.in + t * S::kChannels + 4 * l.cl, d);
-            four(m.c + t * S::kStates + 4 * l.nl, cs);
+                for (int i = 0; i < 4; ++i) back.h[j][i] = add_pair(back.h[j][i], more.h[j][i]);
+        };
+        auto back_through = [&](int t) {
+            Pair dt[2], d[2], cs[4];
+            l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
+            l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, d);
+            l.order.four_pairs(m.c + t * S::kStates + 4 * l.nl, cs);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) back[j][i] = exp2_fast(dt[j] * l.rate[j][i]) * fmaf(d[j], cs[i], back[j][i]);
-            if (begins >> t & 1u) {
-                closed = true;
+                for (int i = 0; i < 4; ++i) back.h[j][i] = mul_pair(exp2_pair(mul_pair(dt[j], l.rate.h[j][i])), fma_pair(d[j], cs[i], back.h[j][i]));
+        };
+        if (left == S::kChunk && (begins & ~1u) == 0u && (ends & ~(1u << (S::kChunk - 1))) == 0u) {
+            if (ends != 0u) end_at(S::kChunk - 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) back[j][i] = 0.f;
+            for (int t = S::kChunk - 1; t >= 0; --t) back_through(t);
+            if (begins != 0u) { closed = true; back.clear(); }
+        } else {
+#pragma unroll 1
+            for (int t = left - 1; t >= 0; --t) {
+                if (ends >> t & 1u) end_at(t);
+                back_through(t);
+                if (begins >> t & 1u) { closed = true; back.clear(); }
             }
         }
         __syncwarp();
     }
-    float4* const maps = reinterpret_cast<float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) maps[32 * j] = make_float4(back[j][0], back[j][1], back[j][2], back[j][3]);
-    give_totals<LN>(p, m, total, l.lane, segment * p.tiles + tile, closed);
+    back.store(reinterpret_cast<float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane);
+    give_totals<LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
 }
 
 template <typename T, int LN>
-__global__ void __launch_bounds__(kScanWarps * 32) scan_grad_kernel(const ScanParams p) {
+__global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const ScanParams p) {
     using S = ScanTile<LN>;
+    constexpr int E = S::kEach;
     extern __shared__ __align__(16) unsigned char raw[];
     ScanGradShared<LN>& m = reinterpret_cast<ScanGradShared<LN>*>(raw)[threadIdx.x / 32];
     const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, worker = job / p.tiles, tile = job % p.tiles;
     if (worker >= p.workers) return;
     const ScanLane<T, LN> l(p, tile);
-    constexpr int OWN = S::kChannels > 32 ? S::kChannels / 32 : 1;         // channels of a lane where it has values
-    float ddecay[4][4] = {}, dskip[OWN] = {}, dbias[OWN] = {};
+    States ddecay;
+    ddecay.clear();
+    float dskip[E] = {}, dbias[E] = {};
     for (int64_t segment = worker; segment < p.segments; segment += p.workers) {
         const int64_t begin = segment * p.segment, end = min(begin + p.segment, p.plan.tokens), chunks = (end - begin + S::kChunk - 1) / S::kChunk;
-        float back[4][4] = {};                          // a_{t+1} m_{t+1}
-        if (!p.alone) {
-            const float4* const maps = reinterpret_cast<const float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { const float4 v = maps[32 * j]; back[j][0] = v.x; back[j][1] = v.y; back[j][2] = v.z; back[j][3] = v.w; }
-        }
+        States back;                                    // a_{t+1} m_{t+1}
+        back.clear();
+        if (!p.alone) back.load(reinterpret_cast<const float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane);
         for (int64_t k0 = chunks - 1; k0 >= 0; --k0) {
             const int64_t t0 = begin + k0 * S::kChunk, chunk = segment * p.chunks + k0;
-            const int left = (int)min((int64_t)S::kChunk, end - t0);
-            T x[S::kEach], delta[S::kEach], gate[S::kEach], dy[S::kEach], b[S::kNarrow], c[S::kNarrow];
-            l.load(p.x, p.x_stride, t0, left, x);
-            l.load(p.delta, p.delta_stride, t0, left, delta);
-            l.load(p.dy, p.channels, t0, left, dy);
-            if (p.gate != nullptr) l.load(p.gate, p.gate_stride, t0, left, gate);
-            l.load_narrow(p.b, p.b_stride, t0, left, b);
-            l.load_narrow(p.c, p.c_stride, t0, left, c);
+            const int left = (int)min((int64_t)S::kChunk, end - t0), there = l.token < left ? l.own : 0;
+            typename ScanLane<T, LN>::Each x, delta, gate, dy;
+            typename ScanLane<T, LN>::Narrow b, c;
+            l.load(p, p.x, p.x_stride, t0, left, x);
+            l.load(p, p.delta, p.delta_stride, t0, left, delta);
+            l.load(p, p.dy, p.channels, t0, left, dy);
+            if (p.gate != nullptr) l.load(p, p.gate, p.gate_stride, t0, left, gate);
+            l.load_narrow(p, p.b, p.b_stride, t0, left, b);
+            l.load_narrow(p, p.c, p.c_stride, t0, left, c);
             const int32_t links = l.lane < left ? p.plan.link[t0 + l.lane] : -1, tails = l.lane < left ? p.plan.tail[t0 + l.lane] : -1;
             const uint32_t begins = __ballot_sync(~0u, links != -1), ends = __ballot_sync(~0u, tails >= 0);
-            float h[4][4];
+            const float4* const kept = p.kept + (chunk * p.tiles + tile) * 128 + l.lane;
+            States h;
+            h.load(kept);
+            {
+                float xs[E], us[E], ds[E], bias[E];
+                x.get(xs);
+                delta.get(us);
+                l.of_channels(p.delta_bias, bias);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) { const float4 v = p.kept[((chunk * p.tiles + tile) * 4 + j) * 32 + l.lane]; h[j][0] = v.x; h[j][1] = v.y; h[j][2] = v.z; h[j][3] = v.w; }
-            float slope[S::kEach], silu[S::kEach];      // softplus'(delta + bias), silu(gate)
+                for (int k = 0; k < E; ++k) {
+                    const float u = us[k] + bias[k];
+                    const Fading f = fading<true>(u);
+                    us[k] = softplus(u, f);
+                    bias[k] = logistic(u, f);
+                    xs[k] *= us[k];
+                }
+                put(l.cell(m.dt), us);
+                put(l.cell(m.slope), bias);
+                put(l.cell(m.in), xs);
+                dy.get(ds);
+                if (p.gate != nullptr) {
+                    float z[E];
+                    gate.get(z);
 #pragma unroll
-            for (int k = 0; k < S::kEach; ++k) {
-                const bool there = l.there(k, left);
-                const float u = to_float<T>(delta[k]) + l.bias(p, k), dt = there ? softplus(u) : 0.f;
-                slope[k] = logistic(u);
-                silu[k] = 1.f;
-                if (p.gate != nullptr) { const float z = to_float<T>(gate[k]); silu[k] = z * logistic(z); }
-                m.dt[l.lane + 32 * k] = dt;
-                m.in[l.lane + 32 * k] = dt * to_float<T>(x[k]);
-                m.dy[l.lane + 32 * k] = there ? to_float<T>(dy[k]) * silu[k] : 0.f;
+                    for (int k = 0; k < E; ++k) {
+                        const Fading f = fading<sizeof(T) == 4>(z[k]);
+                        const float r = logistic(z[k], f);
+                        us[k] = ds[k] * (r * fmaf(z[k], one_less(z[k], f), 1.f));
+                        ds[k] *= z[k] * r;
+                    }
+                    put(l.cell(m.gate), us);
+                }
+                put(l.cell(m.dy), ds);
             }
-#pragma unroll
-            for (int k = 0; k < S::kNarrow; ++k) { m.b[l.lane + 32 * k] = to_float<T>(b[k]); m.c[l.lane + 32 * k] = to_float<T>(c[k]); }
+            l.put_narrow(m.b, b);
+            l.put_narrow(m.c, c);
             __syncwarp();
-#pragma unroll 2
-            for (int t = 0; t < left; ++t) {
-                if (begins >> t & 1u) {
-                    const int32_t row = __shfl_sync(~0u, links, t);
-                    l.each(row >= 0 ? p.initial : nullptr, row, h, p.channels);
-                }
-                float dt[4], in[4], bs[4];
-                four(m.dt + t * S::kChannels + 4 * l.cl, dt);
-                four(m.in + t * S::kChannels + 4 * l.cl, in);
-                four(m.b + t * S::kStates + 4 * l.nl, bs);
+            auto begin_at = [&](int t) {
+                const int32_t row = __shfl_sync(~0u, links, t);
+                if (row >= 0) l.each(p, p.initial, row, h); else h.clear();
+            };
+            auto forth = [&](int t) {
+                h.store(m.before + t * 128 + l.lane);
+                Pair dt[2], in[2], bs[4];
+                l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
+                l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, in);
+                l.order.four_pairs(m.b + t * S::kStates + 4 * l.nl, bs);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    m.before[(t * 4 + j) * 32 + l.lane] = make_float4(h[j][0], h[j][1], h[j][2], h[j][3]);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) h[j][i] = fmaf(exp2_fast(dt[j] * l.rate[j][i]), h[j][i], in[j] * bs[i]);
-                }
-            }
-#pragma unroll 1
-            for (int t = left - 1; t >= 0; --t) {
-                if (ends >> t & 1u) {
-                    float more[4][4];
-                    l.each(p.dstate, __shfl_sync(~0u, tails, t), more, p.channels);
+                    for (int i = 0; i < 4; ++i) h.h[j][i] = fma_pair(exp2_pair(mul_pair(dt[j], l.rate.h[j][i])), h.h[j][i], mul_pair(in[j], bs[i]));
+            };
+            auto end_at = [&](int t) {
+                const int32_t row = __shfl_sync(~0u, tails, t);
+                if (p.dstate == nullptr) return;
+                States more;
+                l.each(p, p.dstate, row, more);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) back[j][i] += more[j][i];
-                }
-                float dt[4], in[4], d[4], bs[4], cs[4];
-                four(m.dt + t * S::kChannels + 4 * l.cl, dt);
-                four(m.in + t * S::kChannels + 4 * l.cl, in);
-                four(m.dy + t * S::kChannels + 4 * l.cl, d);
-                four(m.b + t * S::kStates + 4 * l.nl, bs);
-                four(m.c + t * S::kStates + 4 * l.nl, cs);
-                float y[4] = {}, by_b[4] = {}, by_a[4] = {}, narrow[8] = {};
+                    for (int i = 0; i < 4; ++i) back.h[j][i] = add_pair(back.h[j][i], more.h[j][i]);
+            };
+            auto begun_at = [&](int t) {
+                const int32_t row = __shfl_sync(~0u, links, t);
+                if (row >= 0 && p.dinitial != nullptr) l.give(p, p.dinitial, row, back);
+                back.clear();
+            };
+            // where a lane's sums over the channels go: B's gradient or C's
+            constexpr int HALF = S::kChannelLanes / 2;
+            using N = Kept<4, HALF>;
+            const int which = N::first(l.cl % HALF);
+            float* const narrow_to = p.db + (which < 2 ? 0 : p.dc_after) + (tile * p.plan.tokens + t0) * S::kStates + 4 * l.nl + l.order.upper_i + which % 2;
+            auto back_through = [&](int t) {
+                Pair dt[2], in[2], d[2], bs[4], cs[4];
+                l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
+                l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, in);
+                l.order.two_pairs(m.dy + t * S::kRow + 4 * l.cl, d);
+                l.order.four_pairs(m.b + t * S::kStates + 4 * l.nl, bs);
+                l.order.four_pairs(m.c + t * S::kStates + 4 * l.nl, cs);
+                States before;
+                before.load(m.before + t * 128 + l.lane);
+                Pair y[2], by_b[2], by_a[2], to_b[4], to_c[4];
+                auto add = [](bool first, Pair a, Pair b, Pair& sum) { sum = first ? mul_pair(a, b) : fma_pair(a, b, sum); };
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    float before[4];
-                    four(reinterpret_cast<const float*>(m.before + (t * 4 + j) * 32 + l.lane), before);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const float grad = fmaf(d[j], cs[i], back[j][i]), a = exp2_fast(dt[j] * l.rate[j][i]);
-                        const float kept = a * before[i], now = fmaf(in[j], bs[i], kept), through = grad * kept;
-                        y[j] = fmaf(cs[i], now, y[j]);
-                        narrow[4 + i] = fmaf(d[j], now, narrow[4 + i]);
-                        narrow[i] = fmaf(in[j], grad, narrow[i]);
-                        by_b[j] = fmaf(grad, bs[i], by_b[j]);
-                        by_a[j] = fmaf(through, l.rate[j][i], by_a[j]);
-                        ddecay[j][i] = fmaf(through, dt[j], ddecay[j][i]);
-                        back[j][i] = a * grad;
+                        const Pair grad = fma_pair(d[j], cs[i], back.h[j][i]), a = exp2_pair(mul_pair(dt[j], l.rate.h[j][i]));
+                        const Pair kept = mul_pair(a, before.h[j][i]), now = fma_pair(in[j], bs[i], kept), through = mul_pair(grad, kept);
+                        add(i == 0, cs[i], now, y[j]);
+                        add(j == 0, d[j], now, to_c[i]);
+                        add(j == 0, in[j], grad, to_b[i]);
+                        add(i == 0, grad, bs[i], by_b[j]);
+                        add(i == 0, through, l.rate.h[j][i], by_a[j]);
+                        ddecay.h[j][i] = fma_pair(through, dt[j], ddecay.h[j][i]);
+                        back.h[j][i] = mul_pair(a, grad);
                     }
-                }
-                if (begins >> t & 1u) {
-                    const int32_t row = __shfl_sync(~0u, links, t);
-                    if (row >= 0 && p.dinitial != nullptr) l.give(p.dinitial, row, back, p.channels);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) back[j][i] = 0.f;
-                }
-                sum_lanes<4, LN, 1>(y, l.lane);
-                sum_lanes<4, LN, 1>(by_b, l.lane);
-                sum_lanes<4, LN, 1>(by_a, l.lane);
+                float sums[3][2], narrow[4];
+                sum_states<LN>(y[0], y[1], sums[0], l.lane);
+                sum_states<LN>(by_b[0], by_b[1], sums[1], l.lane);
+                sum_states<LN>(by_a[0], by_a[1], sums[2], l.lane);
+                __syncwarp();                           // all have read the token's dt x, whose place is written
                 using K = Kept<4, LN>;
                 if (K::owner(l.nl))
 #pragma unroll
                     for (int i = 0; i < K::kCount; ++i) {
-                        const int at = t * S::kChannels + 4 * l.cl + K::first(l.nl) + i;
-                        m.out[at] = y[i];
-                        m.by_b[at] = by_b[i];
-                        m.by_a[at] = by_a[i] * kFromBase2;
+                        const int at = t * S::kRow + 4 * l.cl + K::first(l.nl) + i;
+                        m.out[at] = sums[0][i];
+                        m.in[at] = sums[1][i];
+                        m.by_a[at] = sums[2][i];
                     }
-                sum_lanes<8, S::kChannelLanes, LN>(narrow, l.lane);
-                using N = Kept<8, S::kChannelLanes>;
-                if (N::owner(l.cl))
+                // of the channels' two halves the states' upper or lower two, then B's or C's
 #pragma unroll
-                    for (int i = 0; i < N::kCount; ++i) {
-                        const int which = N::first(l.cl) + i;
-                        float* const to = which < 4 ? p.db : p.dc;
-                        to[(tile * p.plan.tokens + t0 + t) * S::kStates + 4 * l.nl + which % 4] = narrow[i];
-                    }
-            }
-            __syncwarp();
-#pragma unroll
-            for (int k = 0; k < S::kEach; ++k) {
-                if (!l.there(k, left)) continue;
-                const int at = l.lane + 32 * k;
-                const int64_t to = (t0 + l.token_of(k)) * p.channels + l.c0 + l.channel_of(k);
-                const float xv = to_float<T>(x[k]), dyv = m.dy[at], skip = l.skip(p, k);
-                if (p.gate != nullptr) {
-                    const float z = to_float<T>(gate[k]), r = logistic(z), y = fmaf(skip, xv, m.out[at]);
-                    static_cast<T*>(p.dgate)[to] = from_float<T>(to_float<T>(dy[k]) * y * (r * fmaf(z, 1.f - r, 1.f)));
+                for (int i = 0; i < 2; ++i) {
+                    float u, v, x, z;
+                    split(to_b[i], u, v);
+                    split(to_b[i + 2], x, z);
+                    narrow[i] = u + v + __shfl_xor_sync(~0u, x + z, 16);
+                    split(to_c[i], u, v);
+                    split(to_c[i + 2], x, z);
+                    narrow[2 + i] = u + v + __shfl_xor_sync(~0u, x + z, 16);
                 }
-                const float du = fmaf(m.by_b[at], xv, m.by_a[at]) * slope[k];
-                static_cast<T*>(p.dx)[to] = from_float<T>(fmaf(m.by_b[at], m.dt[at], skip * dyv));
-                static_cast<T*>(p.ddelta)[to] = from_float<T>(du);
-                dskip[k % OWN] = fmaf(dyv, xv, dskip[k % OWN]);
-                dbias[k % OWN] += du;
+                sum_lanes<4, HALF, LN>(narrow, l.lane);
+                if (N::owner(l.cl % HALF))
+#pragma unroll
+                    for (int i = 0; i < N::kCount; ++i) (i < 2 ? narrow_to : narrow_to + p.dc_after)[t * S::kStates + i % 2] = narrow[i];
+            };
+            // the states again, then back through the tokens. CHECKED: something may begin or end in the midst, or the chunk end early
+            auto walk = [&](auto checked) {
+                constexpr bool CHECKED = decltype(checked)::value != 0;
+                const int to = CHECKED ? left : S::kChunk;
+                if (!CHECKED && begins != 0u) begin_at(0);
+#pragma unroll 4
+                for (int t = 0; t < to; ++t) {
+                    if (CHECKED && begins >> t & 1u) begin_at(t);
+                    forth(t);
+                }
+                if (!CHECKED && ends != 0u) end_at(S::kChunk - 1);
+#pragma unroll 2
+                for (int t = to - 1; t >= 0; --t) {
+                    if (CHECKED && ends >> t & 1u) end_at(t);
+                    back_through(t);
+                    if (CHECKED && begins >> t & 1u) begun_at(t);
+                }
+                if (!CHECKED && begins != 0u) begun_at(0);
+            };
+            // most chunks are whole, and nothing begins or ends but at their edges
+            if (left == S::kChunk && (begins & ~1u) == 0u && (ends & ~(1u << (S::kChunk - 1))) == 0u) walk(Flag<0>{}); else walk(Flag<1>{});
+            __syncwarp();
+            {
+                float xs[E], us[E], ds[E], dt[E], by_b[E], out[E], skip[E];
+                x.get(xs);
+                take(l.cell(m.in), by_b);
+                take(l.cell(m.by_a), us);
+                take(l.cell(m.slope), out);
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    us[k] = fmaf(by_b[k], xs[k], us[k] * kFromBase2) * out[k];
+                    if (there > 0) dbias[k] += us[k];
+                }
+                l.store(p, p.ddelta, t0, left, us);
+                take(l.cell(m.dy), ds);
+                take(l.cell(m.dt), dt);
+                l.of_channels(p.skip, skip);
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    dskip[k] = fmaf(ds[k], xs[k], dskip[k]);       // 0 where there is no token
+                    out[k] = fmaf(by_b[k], dt[k], skip[k] * ds[k]);
+                }
+                l.store(p, p.dx, t0, left, out);
+                if (p.gate != nullptr) {
+                    take(l.cell(m.out), out);
+                    take(l.cell(m.gate), us);
+#pragma unroll
+                    for (int k = 0; k < E; ++k) out[k] = us[k] * fmaf(skip[k], xs[k], out[k]);
+                    l.store(p, p.dgate, t0, left, out);
+                }
             }
             __syncwarp();
         }
     }
-    // lanes that have values of one channel
+    // lanes that have values of the same channels, which lie as many apart as a token has
+    constexpr int APART = S::kChannels / E;
 #pragma unroll
-    for (int d = S::kChannels; d < 32; d *= 2) {
-        dskip[0] += __shfl_xor_sync(~0u, dskip[0], d);
-        dbias[0] += __shfl_xor_sync(~0u, dbias[0], d);
-    }
-    const int64_t at = worker * p.tiles + tile;
+    for (int d = APART; d < 32; d *= 2)
 #pragma unroll
-    for (int k = 0; k < OWN; ++k)
-        if (l.lane + 32 * k < S::kChannels) {
-            p.dskip[at * S::kChannels + l.lane + 32 * k] = dskip[k];
-            p.dbias[at * S::kChannels + l.lane + 32 * k] = dbias[k];
+        for (int k = 0; k < E; ++k) {
+            dskip[k] += __shfl_xor_sync(~0u, dskip[k], d);
+            dbias[k] += __shfl_xor_sync(~0u, dbias[k], d);
         }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) reinterpret_cast<float4*>(p.ddecay)[at * 128 + j * 32 + l.lane] = make_float4(ddecay[j][0], ddecay[j][1], ddecay[j][2], ddecay[j][3]);
+    const int64_t at = worker * p.tiles + tile;
+    if (l.lane < APART) {
+        put(p.dskip + at * S::kChannels + l.channel, dskip);
+        put(p.dbias + at * S::kChannels + l.channel, dbias);
+    }
+    ddecay.store(reinterpret_cast<float4*>(p.ddecay) + at * 128 + l.lane);
 }
 
 // The workers' sums into one: a block per 32 of a tile's 512 decays and their channels' other sums.
@@ -557,9 +830,9 @@ template <int LN> __global__ void __launch_bounds__(1024) scan_sums_kernel(const
     sum = 0.f;
     for (int w = 0; w < 32; ++w) sum += part[w][lane];
     if (which < 16) {
-        const int place = which * 32 + lane, of = place % 128 / 4, n = 4 * (of % LN) + place % 4;
-        const int64_t c = tile * S::kChannels + 4 * (of / LN) + place / 128;
-        if (c < p.channels && n < p.states && ddecay != nullptr) ddecay[c * p.states + n] = sum;
+        int c, n;
+        place_of<LN>(which * 32 + lane, c, n);
+        if (const int64_t channel = tile * S::kChannels + c; channel < p.channels && n < p.states && ddecay != nullptr) ddecay[channel * p.states + n] = sum;
     } else if (const int64_t c = tile * S::kChannels + other; c < p.channels) {
         float* const to = extra % 2 ? ddelta_bias : dskip;
         if (to != nullptr) to[c] = sum;
@@ -572,7 +845,7 @@ template <typename T> __global__ void __launch_bounds__(256) scan_narrow_kernel(
     if (at >= n || at % width >= p.states) return;
     float b = 0.f, c = 0.f;
 #pragma unroll 4
-    for (uint32_t k = 0; k < p.tiles; ++k) { b += p.db[k * n + at]; c += p.dc[k * n + at]; }
+    for (uint32_t k = 0; k < p.tiles; ++k) { b += p.db[k * n + at]; c += p.db[p.dc_after + k * n + at]; }
     const int64_t to = at / width * p.states + at % width;
     db[to] = from_float<T>(b);
     dc[to] = from_float<T>(c);
@@ -580,7 +853,7 @@ template <typename T> __global__ void __launch_bounds__(256) scan_narrow_kernel(
 
 // ---- host ------------------------------------------------------------------------------------------------------------------
 static int scan_lanes(int64_t states) { return states <= 8 ? 2 : states <= 16 ? 4 : states <= 32 ? 8 : 16; }
-static int64_t scan_chunk(int lanes) { return lanes == 4 || lanes == 8 ? 8 : 4; }
+static int64_t scan_chunk(int lanes) { return lanes == 2 ? 4 : 8; }
 
 struct ScanShape {
     int lanes;
@@ -596,7 +869,7 @@ struct ScanShape {
         segments = (plan.tokens + segment - 1) / segment;
         alone = plan.tokens <= segment || segment == plan.length;
         chunks = (segment + chunk - 1) / chunk;
-        workers = std::max<int64_t>(1, std::min<int64_t>(segments, (12 * 148 + tiles - 1) / tiles));
+        workers = std::max<int64_t>(1, std::min<int64_t>(segments, 8 * 148 / tiles));
     }
     uint64_t kept() const { return (uint64_t)(segments * chunks * tiles) * 2048u; }
     uint64_t maps() const { return alone ? 0u : (uint64_t)(segments * tiles) * (512u + (uint64_t)channels) * 4u; }
@@ -620,6 +893,19 @@ template <typename T, int LN> static cudaError_t run_scan(const nuka_b200_scan_t
     p.decay = d.decay; p.skip = d.skip; p.delta_bias = d.delta_bias; p.initial = d.initial; p.dstate = d.dstate;
     p.y = d.y; p.dx = d.dx; p.ddelta = d.ddelta; p.dgate = d.dgate; p.state = d.state; p.dinitial = d.dinitial;
     p.kept = static_cast<float4*>(d.kept);
+    // a lane's share of a chunk: eight values (four with 32 states, two with 64), and of B and C four (one, eight, sixteen with 8, 32 and 64 states)
+    using S = ScanTile<LN>;
+    auto lies = [](const void* at, uint64_t on) { return reinterpret_cast<uintptr_t>(at) % on == 0u; };
+    constexpr uint64_t EACH = std::min<uint64_t>(16, S::kEach * sizeof(T)), NARROW = std::min<uint64_t>(16, S::kNarrow * sizeof(T));
+    p.wide = d.channels % S::kEach == 0 && d.states % S::kNarrow == 0 && d.b_stride % S::kNarrow == 0 && d.c_stride % S::kNarrow == 0 && lies(d.b, NARROW) && lies(d.c, NARROW);
+    for (int64_t stride : {d.x_stride, d.delta_stride, d.gate_stride}) p.wide = p.wide && stride % S::kEach == 0;
+    for (const void* at : {d.x, d.delta, d.gate, static_cast<const void*>(d.y)}) p.wide = p.wide && lies(at, EACH);
+    if (backward)
+        for (const void* at : {d.dy, static_cast<const void*>(d.dx), static_cast<const void*>(d.ddelta), static_cast<const void*>(d.dgate)}) p.wide = p.wide && lies(at, EACH);
+    p.wide_states = d.states % 2 == 0;
+    for (const float* at : {d.decay, d.initial, static_cast<const float*>(d.state)}) p.wide_states = p.wide_states && lies(at, 8);
+    if (backward)
+        for (const float* at : {d.dstate, static_cast<const float*>(d.dinitial)}) p.wide_states = p.wide_states && lies(at, 8);
     float* work = static_cast<float*>(d.workspace);
     if (!s.alone) { p.maps = work; p.sums = work + s.segments * s.tiles * 512; work += s.maps() / 4; }
     const unsigned jobs = (unsigned)((s.segments * s.tiles + kScanWarps - 1) / kScanWarps), carries = (unsigned)(s.tiles * 16);
@@ -632,7 +918,7 @@ template <typename T, int LN> static cudaError_t run_scan(const nuka_b200_scan_t
         return cudaGetLastError();
     }
     const int64_t narrow = s.tiles * p.plan.tokens * s.states;
-    p.db = work; p.dc = work + narrow; p.ddecay = work + 2 * narrow; p.dskip = p.ddecay + s.workers * s.tiles * 512; p.dbias = p.dskip + s.workers * s.tiles * s.channels;
+    p.db = work; p.dc_after = narrow; p.ddecay = work + 2 * narrow; p.dskip = p.ddecay + s.workers * s.tiles * 512; p.dbias = p.dskip + s.workers * s.tiles * s.channels;
     constexpr int SHARED = sizeof(ScanGradShared<LN>) * kScanWarps;
     const cudaError_t set = cudaFuncSetAttribute(scan_grad_kernel<T, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED);
     if (set != cudaSuccess) return set;
@@ -680,14 +966,14 @@ template <typename T, int LN, bool FOUR> __global__ void __launch_bounds__(128) 
     const int count = live ? min(4, (int)d.states - 4 * nl) : 0;                  // below 1: none
     float h[4], rate[4];
     if (FOUR && count > 0) {
-        four(state, h);
-        four(decay, rate);
+        take(state, h);
+        take(decay, rate);
     } else {
 #pragma unroll
         for (int i = 0; i < 4; ++i) { h[i] = i < count ? state[i] : 0.f; rate[i] = i < count ? decay[i] : 0.f; }
     }
     const float x = to_float<T>(static_cast<const T*>(d.x)[env * d.x_stride + ch]);
-    const float dt = softplus(to_float<T>(static_cast<const T*>(d.delta)[env * d.delta_stride + ch]) + (d.delta_bias != nullptr ? d.delta_bias[ch] : 0.f));
+    const float u = to_float<T>(static_cast<const T*>(d.delta)[env * d.delta_stride + ch]) + (d.delta_bias != nullptr ? d.delta_bias[ch] : 0.f), dt = softplus(u, fading<true>(u));
     float y = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -706,7 +992,7 @@ template <typename T, int LN, bool FOUR> __global__ void __launch_bounds__(128) 
     }
     if (!live || nl != 0) return;
     if (d.skip != nullptr) y = fmaf(d.skip[ch], x, y);
-    if (d.gate != nullptr) { const float z = to_float<T>(static_cast<const T*>(d.gate)[env * d.gate_stride + ch]); y *= z * logistic(z); }
+    if (d.gate != nullptr) { const float z = to_float<T>(static_cast<const T*>(d.gate)[env * d.gate_stride + ch]); y *= silu<sizeof(T) == 4>(z); }
     static_cast<T*>(d.y)[env * d.channels + ch] = from_float<T>(y);
 }
 

@@ -9,10 +9,14 @@
 #include <algorithm>
 #include "nkb_sequence.cuh"
 #include "nkb_sequence.h"
+#include "nkb_tcgen.cuh"
 
 namespace nkb {
 
-constexpr int kLines = 8;                               // warps of a block: stretches side by side
+constexpr int kLines = 4;                               // warps of a block: stretches side by side
+constexpr int kForthBlocks = 5, kBackBlocks = 4;        // blocks of an SM
+constexpr int kForthBatch = 4, kBackBatch = 4;          // tokens whose loads are under way; a multiple of the longest window, so that its shift is a change of names
+constexpr int kBytes = 8;                               // of a thread's channels
 constexpr int kSms = 148;
 
 struct ConvolutionParams {
@@ -26,6 +30,17 @@ struct ConvolutionParams {
     bool act, sums;
 };
 
+// sum += a b, two values at a time where there are two
+template <int N> __device__ __forceinline__ void add_products(float (&sum)[N], const float (&a)[N], const float (&b)[N]) {
+    if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int v = 0; v < N; v += 2) split(fma_pair(pair_of(a[v], a[v + 1]), pair_of(b[v], b[v + 1]), pair_of(sum[v], sum[v + 1])), sum[v], sum[v + 1]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < N; ++v) sum[v] = fmaf(a[v], b[v], sum[v]);
+    }
+}
+
 template <typename T, int K, int VEC> struct Line {
     float w[K][VEC], bias[VEC];
     __device__ __forceinline__ Line(const ConvolutionParams& p, int64_t c) {
@@ -37,157 +52,179 @@ template <typename T, int K, int VEC> struct Line {
         }
     }
     // the sum for a window of inputs, the present one the last
-    __device__ __forceinline__ void sum(const Raw<T, VEC> (&window)[K], float (&s)[VEC]) const {
+    __device__ __forceinline__ void sum(const float (&window)[K][VEC], float (&s)[VEC]) const {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) s[v] = bias[v];
 #pragma unroll
-        for (int j = 0; j < K; ++j) {
-            float x[VEC];
-            unpack<T, VEC>(window[j], x);
-#pragma unroll
-            for (int v = 0; v < VEC; ++v) s[v] = fmaf(w[j][v], x[v], s[v]);
-        }
+        for (int j = 0; j < K; ++j) add_products(s, w[j], window[j]);
     }
 };
 
-template <typename T, int VEC> __device__ __forceinline__ Raw<T, VEC> nothing() {
-    const float zero[VEC] = {};
-    Raw<T, VEC> r;
-    store<T, VEC>(reinterpret_cast<T*>(&r), zero);
-    return r;
+// VEC inputs, or zeros.
+template <typename T, int VEC> __device__ __forceinline__ void input(const void* from, int64_t at, bool there, float (&v)[VEC]) {
+    if (there) {
+        unpack<T, VEC>(load_raw<T, VEC>(static_cast<const T*>(from) + at), v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) v[k] = 0.f;
+    }
 }
 
 // The inputs before token t, which does not begin an episode: zeros before its first token, or what the row began with.
-template <typename T, int K, int VEC> __device__ __forceinline__ void window_before(const ConvolutionParams& p, int64_t t, int64_t c, Raw<T, VEC> (&window)[K]) {
+template <typename T, int K, int VEC> __device__ __forceinline__ void window_before(const ConvolutionParams& p, int64_t t, int64_t c, float (&window)[K][VEC]) {
     const int64_t first = p.plan.first[t];
     const int32_t row = t - first < K - 1 ? p.plan.link[first] : -1;
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) {
         const int64_t at = t - (K - 1) + j, early = at - first + K - 1;          // number among the row's initial inputs where below K - 1
-        window[j + 1] = at >= first ? load_raw<T, VEC>(static_cast<const T*>(p.x) + at * p.x_stride + c)
-                      : row >= 0 && p.initial != nullptr ? load_raw<T, VEC>(static_cast<const T*>(p.initial) + ((int64_t)row * (K - 1) + early) * p.channels + c) : nothing<T, VEC>();
+        if (at >= first) input<T, VEC>(p.x, at * p.x_stride + c, true, window[j + 1]);
+        else input<T, VEC>(p.initial, ((int64_t)row * (K - 1) + early) * p.channels + c, row >= 0 && p.initial != nullptr, window[j + 1]);
     }
 }
-template <typename T, int K, int VEC> __device__ __forceinline__ void window_begins(const ConvolutionParams& p, int32_t row, int64_t c, Raw<T, VEC> (&window)[K]) {
+template <typename T, int K, int VEC> __device__ __forceinline__ void window_begins(const ConvolutionParams& p, int32_t row, int64_t c, float (&window)[K][VEC]) {
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j)
-        window[j + 1] = row >= 0 && p.initial != nullptr ? load_raw<T, VEC>(static_cast<const T*>(p.initial) + ((int64_t)row * (K - 1) + j) * p.channels + c) : nothing<T, VEC>();
+    for (int j = 0; j < K - 1; ++j) input<T, VEC>(p.initial, ((int64_t)row * (K - 1) + j) * p.channels + c, row >= 0 && p.initial != nullptr, window[j + 1]);
 }
 
+// A warp's next tokens, number `lane` to a lane: which of them begin an episode, and which end a row.
+struct Marks {
+    int32_t link, tail;
+    uint32_t begins, ends;
+    __device__ __forceinline__ Marks(const ConvolutionParams& p, int64_t t0, int count) {
+        const int lane = threadIdx.x % 32;
+        link = lane < count ? p.plan.link[t0 + lane] : -1;
+        tail = lane < count ? p.plan.tail[t0 + lane] : -1;
+        begins = __ballot_sync(~0u, link != -1);
+        ends = __ballot_sync(~0u, tail >= 0);
+    }
+    __device__ __forceinline__ int32_t row_of(int i) const { return __shfl_sync(~0u, link, i); }
+    __device__ __forceinline__ int32_t end_of(int i) const { return __shfl_sync(~0u, tail, i); }
+};
+
 template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(kLines * 32) convolution_kernel(const ConvolutionParams p) {
-    constexpr int BATCH = 8;                            // tokens whose loads are under way
-    const int64_t c = ((int64_t)(blockIdx.x % p.tiles) * 32 + threadIdx.x % 32) * VEC, C = p.channels;
+__global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(const ConvolutionParams p) {
+    constexpr int BATCH = kForthBatch;                  // tokens whose loads are under way
+    const int64_t own = ((int64_t)(blockIdx.x % p.tiles) * 32 + threadIdx.x % 32) * VEC, C = p.channels;
     const int64_t line = (int64_t)(blockIdx.x / p.tiles) * kLines + threadIdx.x / 32;
-    if (c >= C || line >= p.stretches) return;          // VEC divides the channels
+    if (line >= p.stretches) return;
+    const bool live = own < C;                          // VEC divides the channels; lanes behind the last read the first ones, and write nothing
+    const int64_t c = live ? own : 0;
     const Line<T, K, VEC> f(p, c);
-    const T* const x = static_cast<const T*>(p.x) + c;
-    const int64_t begin = line * p.stretch, end = min(begin + p.stretch, p.plan.tokens);
-    Raw<T, VEC> window[K];                              // after the shift at the loop's begin: the last inputs, 0 the oldest
+    const int64_t begin = line * p.stretch;
+    const int count = (int)min(p.stretch, p.plan.tokens - begin);
+    const T* const x = static_cast<const T*>(p.x) + begin * p.x_stride + c;
+    T* y = static_cast<T*>(p.y) + begin * C + c;
+    Raw<T, VEC> ahead[BATCH];
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) ahead[i] = load_raw<T, VEC>(x + min(t0 + i, count - 1) * p.x_stride);
+    };
+    fetch(0);
+    float window[K][VEC];                               // after the shift at a token's begin: the last inputs, 0 the oldest
     if (p.plan.link[begin] == -1) window_before<T, K, VEC>(p, begin, c, window);
-    for (int64_t t0 = begin; t0 < end; t0 += BATCH) {
-        Raw<T, VEC> next[BATCH];
-        int32_t link[BATCH], tail[BATCH];
+    for (int t0 = 0; t0 < count; t0 += BATCH) {
+        const int left = min(BATCH, count - t0);
+        Raw<T, VEC> now[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) now[i] = ahead[i];
+        const Marks marks(p, begin + t0, left);
+        if (t0 + BATCH < count) fetch(t0 + BATCH);
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-            const int64_t t = min(t0 + i, end - 1);
-            next[i] = load_raw<T, VEC>(x + t * p.x_stride);
-            link[i] = p.plan.link[t];
-            tail[i] = p.plan.tail[t];
-        }
+            if (i >= left) break;
+            if (marks.begins >> i & 1u) window_begins<T, K, VEC>(p, marks.row_of(i), c, window);
 #pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            const int64_t t = t0 + i;
-            if (t >= end) break;
-            if (link[i] != -1) window_begins<T, K, VEC>(p, link[i], c, window);
+            for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-            for (int j = 0; j < K - 1; ++j) window[j] = window[j + 1];
-            window[K - 1] = next[i];
+                for (int v = 0; v < VEC; ++v) window[j][v] = window[j + 1][v];
+            unpack<T, VEC>(now[i], window[K - 1]);
             float s[VEC];
             f.sum(window, s);
             if (p.act)
 #pragma unroll
                 for (int v = 0; v < VEC; ++v) s[v] = silu<sizeof(T) == 4>(s[v]);
-            store<T, VEC>(static_cast<T*>(p.y) + t * C + c, s);
-            if (tail[i] >= 0)
+            if (live) store<T, VEC>(y, s);
+            y += C;
+            if (marks.ends >> i & 1u) {
+                T* const to = static_cast<T*>(p.state) + (int64_t)marks.end_of(i) * (K - 1) * C + c;
 #pragma unroll
-                for (int j = 0; j < K - 1; ++j) *reinterpret_cast<Raw<T, VEC>*>(static_cast<T*>(p.state) + ((int64_t)tail[i] * (K - 1) + j) * C + c) = window[j + 1];
+                for (int j = 0; j < K - 1; ++j)
+                    if (live) store<T, VEC>(to + j * C, window[j + 1]);
+            }
         }
     }
 }
 
 template <typename T, int K, int VEC>
-__global__ void __launch_bounds__(kLines * 32) convolution_grad_kernel(const ConvolutionParams p) {
+__global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_kernel(const ConvolutionParams p) {
     __shared__ float sums[kLines / 2][(K + 1) * VEC * 32];
+    constexpr int BATCH = kBackBatch;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t own = ((int64_t)(blockIdx.x % p.tiles) * 32 + lane) * VEC, C = p.channels;
     const bool live = own < C;
     const int64_t c = live ? own : 0;
     const Line<T, K, VEC> f(p, c);
-    const T *const x = static_cast<const T*>(p.x) + c, *const dy = static_cast<const T*>(p.dy) + c;
     float dw[K][VEC] = {}, db[VEC] = {};
-    for (int64_t line = (int64_t)(blockIdx.x / p.tiles) * kLines + warp; live && line < p.stretches; line += (int64_t)p.across * kLines) {
-        const int64_t begin = line * p.stretch, end = min(begin + p.stretch, p.plan.tokens), past = min(end + K - 1, p.plan.tokens);
-        Raw<T, VEC> window[K];
-        float grad[K][VEC];                             // of the inputs in the window, as far as they are complete
-        int64_t first = begin;                          // of the episode
-        int32_t row = -1;                               // that it began, within this walk
+    for (int64_t line = (int64_t)(blockIdx.x / p.tiles) * kLines + warp; line < p.stretches; line += (int64_t)p.across * kLines) {
+        // tokens by their number from the walk's first one
+        const int64_t begin = line * p.stretch;
+        const int end = (int)min(p.stretch, p.plan.tokens - begin), past = (int)min((int64_t)end + K - 1, p.plan.tokens - begin);
+        float window[K][VEC], grad[K][VEC];             // grad: of the inputs in the window, as far as they are complete
+        int first = 0, row = -1;                        // of the episode; the row that it began, within this walk
 #pragma unroll
         for (int j = 0; j < K; ++j)
 #pragma unroll
             for (int v = 0; v < VEC; ++v) grad[j][v] = 0.f;
         if (p.plan.link[begin] == -1) {
             window_before<T, K, VEC>(p, begin, c, window);
-            first = p.plan.first[begin];
+            first = (int)max(p.plan.first[begin] - begin, (int64_t)-K);          // K before the walk is as far as any
         }
+        const T *const x = static_cast<const T*>(p.x) + begin * p.x_stride + c, *const dy = static_cast<const T*>(p.dy) + begin * C + c;
+        T* const dx = static_cast<T*>(p.dx) + begin * C + c;
         // the gradient of input number `at`, one of the row's initial ones where that is before the episode
-        auto leave = [&](int64_t at, const float (&g)[VEC]) {
+        auto leave = [&](int at, const float (&g)[VEC]) {
             if (at >= first) {
-                if (at >= begin && at < end) store<T, VEC>(static_cast<T*>(p.dx) + at * C + c, g);
+                if (live && (unsigned)at < (unsigned)end) store<T, VEC>(dx + at * C, g);
             } else if (row >= 0 && p.dinitial != nullptr) {
-                const int64_t early = at - first + K - 1;
-                if (early >= 0) store<T, VEC>(static_cast<T*>(p.dinitial) + ((int64_t)row * (K - 1) + early) * C + c, g);
+                const int early = at - first + K - 1;
+                if (live && early >= 0) store<T, VEC>(static_cast<T*>(p.dinitial) + ((int64_t)row * (K - 1) + early) * C + c, g);
             }
         };
-        int64_t t = begin;
-        constexpr int BATCH = 4;
-        bool goes = true;
-        for (int64_t t0 = begin; goes && t0 < past; t0 += BATCH) {
+        int last = past;                                // behind the last token walked
+        for (int t0 = 0; t0 < past && last == past; t0 += BATCH) {
+            const int left = min(BATCH, past - t0);
             Raw<T, VEC> xs[BATCH], dys[BATCH];
-            int32_t link[BATCH], tail[BATCH];
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                const int64_t u = min(t0 + i, past - 1);
-                xs[i] = load_raw<T, VEC>(x + u * p.x_stride);
-                dys[i] = load_raw<T, VEC>(dy + u * C);
-                link[i] = p.plan.link[u];
-                tail[i] = p.plan.tail[u];
+                const int t = min(t0 + i, past - 1);
+                xs[i] = load_raw<T, VEC>(x + t * p.x_stride);
+                dys[i] = load_raw<T, VEC>(dy + t * C);
             }
+            const Marks marks(p, begin + t0, left);
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
-                t = t0 + i;
-                if (t >= past || (t >= end && link[i] != -1)) { goes = false; break; }
-                if (link[i] != -1) {
-                    if (t > begin)
+                const int t = t0 + i;
+                if (i >= left) break;
+                if (marks.begins >> i & 1u) {
+                    if (t >= end) { last = t; break; }
+                    if (t > 0)
 #pragma unroll
                         for (int j = 0; j < K; ++j) leave(t - K + j, grad[j]);
-                    window_begins<T, K, VEC>(p, link[i], c, window);
                     first = t;
-                    row = link[i];
+                    row = marks.row_of(i);
+                    window_begins<T, K, VEC>(p, row, c, window);
 #pragma unroll
                     for (int j = 0; j < K; ++j)
 #pragma unroll
                         for (int v = 0; v < VEC; ++v) grad[j][v] = 0.f;
-                } else if (t > begin) {
+                } else if (t > 0) {
                     leave(t - K, grad[0]);
                 }
 #pragma unroll
-                for (int j = 0; j < K - 1; ++j) {
-                    window[j] = window[j + 1];
+                for (int j = 0; j < K - 1; ++j)
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) grad[j][v] = grad[j + 1][v];
-                }
-                window[K - 1] = xs[i];
+                    for (int v = 0; v < VEC; ++v) { window[j][v] = window[j + 1][v]; grad[j][v] = grad[j + 1][v]; }
+                unpack<T, VEC>(xs[i], window[K - 1]);
                 float ds[VEC];
                 unpack<T, VEC>(dys[i], ds);
                 if (p.act) {
@@ -197,33 +234,29 @@ __global__ void __launch_bounds__(kLines * 32) convolution_grad_kernel(const Con
                     for (int v = 0; v < VEC; ++v) ds[v] *= silu_slope<sizeof(T) == 4>(s[v]);
                 }
 #pragma unroll
-                for (int j = 0; j < K; ++j)
+                for (int j = 0; j < K - 1; ++j) add_products(grad[j], f.w[j], ds);
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) grad[j][v] = fmaf(f.w[j][v], ds[v], j < K - 1 ? grad[j][v] : 0.f);
-                if (p.sums && t < end) {
+                for (int v = 0; v < VEC; ++v) grad[K - 1][v] = f.w[K - 1][v] * ds[v];
+                if (t < end) {
 #pragma unroll
-                    for (int j = 0; j < K; ++j) {
-                        float xv[VEC];
-                        unpack<T, VEC>(window[j], xv);
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) dw[j][v] = fmaf(ds[v], xv[v], dw[j][v]);
-                    }
+                    for (int j = 0; j < K; ++j) add_products(dw[j], ds, window[j]);
 #pragma unroll
                     for (int v = 0; v < VEC; ++v) db[v] += ds[v];
                 }
-                if (tail[i] >= 0 && p.dstate != nullptr)
+                if (marks.ends >> i & 1u && p.dstate != nullptr) {
+                    const int32_t ended = marks.end_of(i);
 #pragma unroll
                     for (int j = 0; j < K - 1; ++j) {
                         float more[VEC];
-                        unpack<T, VEC>(load_raw<T, VEC>(static_cast<const T*>(p.dstate) + ((int64_t)tail[i] * (K - 1) + j) * C + c), more);
+                        input<T, VEC>(p.dstate, ((int64_t)ended * (K - 1) + j) * C + c, true, more);
 #pragma unroll
                         for (int v = 0; v < VEC; ++v) grad[j + 1][v] += more[v];
                     }
+                }
             }
         }
-        if (goes) t = past;                             // the token after the last one walked
 #pragma unroll
-        for (int j = 0; j < K; ++j) leave(t - K + j, grad[j]);
+        for (int j = 0; j < K; ++j) leave(last - K + j, grad[j]);
     }
     if (!p.sums) return;
     // the block's warps into one, half of them at a time
@@ -277,16 +310,18 @@ template <int K> __global__ void __launch_bounds__(1024) convolution_sums_kernel
     if (j < K) { if (dweight != nullptr) dweight[c * K + j] = sum; } else if (dbias != nullptr) dbias[c] = sum;
 }
 
-// Tokens of a walk: whole rows where they are of one short length, else 32, for which K - 1 are read twice.
-static int64_t stretch_of(const nuka_b200_episodes_t& plan) {
-    return plan.length > 0 && plan.length <= 64 ? plan.length * std::max<int64_t>(1, 32 / plan.length) : std::min<int64_t>(32, plan.tokens);
+// Tokens of a walk: whole rows where they are of one short length; else as many as leave every SM sixty-four walks of 128 channels, 32 to 128, for which K - 1 are read twice.
+static int64_t stretch_of(const nuka_b200_episodes_t& plan, int64_t channels) {
+    if (plan.length > 0 && plan.length <= 64) return plan.length * std::max<int64_t>(1, 32 / plan.length);
+    const int64_t tiles = (channels + 127) / 128;
+    return std::min<int64_t>(plan.tokens, std::max<int64_t>(32, std::min<int64_t>(128, plan.tokens * tiles / (64 * kSms) / 4 * 4)));
 }
 
 template <typename T, int VEC> static ConvolutionParams convolution_params(const nuka_b200_convolution_t& d) {
     ConvolutionParams p{};
     p.plan = *d.plan;
     p.channels = d.channels; p.x_stride = d.x_stride;
-    p.stretch = stretch_of(p.plan);
+    p.stretch = stretch_of(p.plan, d.channels);
     p.stretches = (p.plan.tokens + p.stretch - 1) / p.stretch;
     p.tiles = (uint32_t)((d.channels + 32 * VEC - 1) / (32 * VEC));
     p.across = (uint32_t)((p.stretches + kLines - 1) / kLines);
@@ -296,10 +331,10 @@ template <typename T, int VEC> static ConvolutionParams convolution_params(const
     return p;
 }
 
-// Blocks along the tokens of the backward pass, each of which leaves a set of partial sums: four to an SM.
+// Blocks along the tokens of the backward pass, each of which leaves a set of partial sums: as many as run at a time.
 static int64_t convolution_across(const nuka_b200_episodes_t& plan, int64_t channels) {
-    const int64_t stretches = (plan.tokens + stretch_of(plan) - 1) / stretch_of(plan), tiles = (channels + 255) / 256;
-    return std::max<int64_t>(1, std::min<int64_t>((stretches + kLines - 1) / kLines, (4 * kSms + tiles - 1) / tiles));
+    const int64_t stretch = stretch_of(plan, channels), stretches = (plan.tokens + stretch - 1) / stretch, tiles = (channels + 127) / 128;
+    return std::max<int64_t>(1, std::min<int64_t>((stretches + kLines - 1) / kLines, std::max<int64_t>(1, kBackBlocks * kSms / tiles)));
 }
 uint64_t convolution_workspace(const nuka_b200_episodes_t& plan, int64_t channels, int64_t width) { return (uint64_t)(convolution_across(plan, channels) * (width + 1) * channels) * sizeof(float); }
 
@@ -321,12 +356,14 @@ template <typename T, int VEC> static cudaError_t run_convolution(const nuka_b20
     return d.width == 2 ? run_convolution<T, 2, VEC>(d, backward, stream) : d.width == 3 ? run_convolution<T, 3, VEC>(d, backward, stream) : run_convolution<T, 4, VEC>(d, backward, stream);
 }
 
-// 16 bytes to a thread where everything lies so, else a value.
+// kBytes to a thread where everything lies so, else a value.
 template <typename T> static cudaError_t run_convolution(const nuka_b200_convolution_t& d, bool backward, cudaStream_t stream) {
-    constexpr int W = 16 / sizeof(T);
+    constexpr int W = kBytes / sizeof(T);
     bool wide = d.channels % W == 0 && d.x_stride % W == 0;
-    for (const void* p : {d.x, d.initial, d.dy, d.dstate, static_cast<const void*>(d.y), static_cast<const void*>(d.state), static_cast<const void*>(d.dx), static_cast<const void*>(d.dinitial)})
-        wide = wide && reinterpret_cast<uintptr_t>(p) % 16 == 0;
+    auto lies = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % kBytes == 0; };
+    for (const void* p : {d.x, d.initial, static_cast<const void*>(d.y), static_cast<const void*>(d.state)}) wide = wide && lies(p);
+    if (backward)
+        for (const void* p : {d.dy, d.dstate, static_cast<const void*>(d.dx), static_cast<const void*>(d.dinitial)}) wide = wide && lies(p);
     return wide ? run_convolution<T, W>(d, backward, stream) : run_convolution<T, 1>(d, backward, stream);
 }
 
@@ -348,25 +385,22 @@ __global__ void convolution_step_kernel(int64_t groups, uint32_t per_env, const 
     const int64_t env = g / per_env, c = (g - env * per_env) * VEC;
     T* const state = static_cast<T*>(d.state) + env * (K - 1) * d.channels + c;
     const bool begins = d.fresh != nullptr && d.fresh[env] != 0;
-    float sum[VEC], x[VEC];
-    Raw<T, VEC> window[K];
+    float sum[VEC], window[K][VEC];
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) window[j] = begins ? nothing<T, VEC>() : load_raw<T, VEC>(state + j * d.channels);
-    window[K - 1] = load_raw<T, VEC>(static_cast<const T*>(d.x) + env * d.x_stride + c);
+    for (int j = 0; j < K - 1; ++j) input<T, VEC>(state, j * d.channels, !begins, window[j]);
+    input<T, VEC>(d.x, env * d.x_stride + c, true, window[K - 1]);
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) sum[v] = d.bias != nullptr ? d.bias[c + v] : 0.f;
+    for (int v = 0; v < VEC; ++v) {
+        sum[v] = d.bias != nullptr ? d.bias[c + v] : 0.f;
 #pragma unroll
-    for (int j = 0; j < K; ++j) {
-        unpack<T, VEC>(window[j], x);
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) sum[v] = fmaf(d.weight[(c + v) * K + j], x[v], sum[v]);
+        for (int j = 0; j < K; ++j) sum[v] = fmaf(d.weight[(c + v) * K + j], window[j][v], sum[v]);
     }
     if (d.silu)
 #pragma unroll
         for (int v = 0; v < VEC; ++v) sum[v] = silu<sizeof(T) == 4>(sum[v]);
     store<T, VEC>(static_cast<T*>(d.y) + env * d.channels + c, sum);
 #pragma unroll
-    for (int j = 0; j < K - 1; ++j) *reinterpret_cast<Raw<T, VEC>*>(state + j * d.channels) = window[j + 1];
+    for (int j = 0; j < K - 1; ++j) store<T, VEC>(state + j * d.channels, window[j + 1]);
 }
 
 template <typename T, int VEC> static cudaError_t run_convolution_step(const nuka_b200_convolution_step_t& d, cudaStream_t stream) {

@@ -953,55 +953,89 @@ cudaError_t launch_scan(const nuka_b200_scan_t& d, bool backward, cudaStream_t s
 }
 
 // ---- one token per env ---------------------------------------------------------------------------------------------
-// The states' bytes bound it: four states of a channel to a lane, LN lanes to a channel.
-template <typename T, int LN, bool FOUR> __global__ void __launch_bounds__(128) scan_step_kernel(int64_t cells, const nuka_b200_scan_step_t d) {
-    const int64_t at = (int64_t)blockIdx.x * 128 + threadIdx.x, cell = at / LN;
-    const int nl = threadIdx.x % LN;
-    const bool live = cell < cells;
-    const int64_t env = live ? cell / d.channels : 0, ch = live ? cell % d.channels : 0;
+// The states' bytes bound it. A warp has an env and a tile of channels, its lanes four channels of four states each, as over rollouts; what a channel's states share is worked out by one lane.
+template <typename T, int LN> __global__ void __launch_bounds__(kScanWarps * 32) scan_step_kernel(int64_t jobs, uint32_t tiles, bool wide, const nuka_b200_scan_step_t d) {
+    constexpr int CHANNELS = 128 / LN, OWN = (CHANNELS + 31) / 32;
+    __shared__ __align__(16) float shared[kScanWarps][3][CHANNELS];
+    const int lane = threadIdx.x % 32, nl = lane % LN, cl = lane / LN;
+    const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, env = job / tiles, c0 = job % tiles * CHANNELS;
+    if (job >= jobs) return;
+    float(&m)[3][CHANNELS] = shared[threadIdx.x / 32];
+    const int count = (int)min((int64_t)CHANNELS, d.channels - c0), states = (int)d.states, there = states - 4 * nl;
     const bool begins = d.fresh != nullptr && d.fresh[env] != 0;
-    float* const state = d.state + (env * d.channels + ch) * d.states + 4 * nl;
-    const float* const decay = d.decay + ch * d.states + 4 * nl;
-    const T *const b = static_cast<const T*>(d.b) + env * d.b_stride + 4 * nl, *const c = static_cast<const T*>(d.c) + env * d.c_stride + 4 * nl;
-    const int count = live ? min(4, (int)d.states - 4 * nl) : 0;                  // below 1: none
-    float h[4], rate[4];
-    if (FOUR && count > 0) {
-        take(state, h);
-        take(decay, rate);
-    } else {
+    float* const state = d.state + (env * d.channels + c0 + 4 * cl) * states + 4 * nl;
+    const float* const decay = d.decay + (c0 + 4 * cl) * states + 4 * nl;
+    float h[4][4], rate[4][4], b[4], c[4], x[OWN], z[OWN];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) { h[i] = i < count ? state[i] : 0.f; rate[i] = i < count ? decay[i] : 0.f; }
-    }
-    const float x = to_float<T>(static_cast<const T*>(d.x)[env * d.x_stride + ch]);
-    const float u = to_float<T>(static_cast<const T*>(d.delta)[env * d.delta_stride + ch]) + (d.delta_bias != nullptr ? d.delta_bias[ch] : 0.f), dt = softplus(u, fading<true>(u));
-    float y = 0.f;
+    for (int j = 0; j < 4; ++j)
+        if (wide && 4 * cl + j < count && there >= 4) {
+            if (begins) { h[j][0] = h[j][1] = h[j][2] = h[j][3] = 0.f; } else take(state + j * states, h[j]);
+            take(decay + j * states, rate[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool is = 4 * cl + j < count && i < there;
+                h[j][i] = is && !begins ? state[j * states + i] : 0.f;
+                rate[j][i] = is ? decay[j * states + i] : 0.f;
+            }
+        }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float bv = i < count ? to_float<T>(b[i]) : 0.f, cv = i < count ? to_float<T>(c[i]) : 0.f, into = dt * x * bv;
-        h[i] = begins ? into : fmaf(exp2_fast(dt * (rate[i] * kToBase2)), h[i], into);
-        if (i < count) y = fmaf(cv, h[i], y);
+        b[i] = i < there ? to_float<T>(static_cast<const T*>(d.b)[env * d.b_stride + 4 * nl + i]) : 0.f;
+        c[i] = i < there ? to_float<T>(static_cast<const T*>(d.c)[env * d.c_stride + 4 * nl + i]) : 0.f;
     }
 #pragma unroll
-    for (int m = 1; m < LN; m *= 2) y += __shfl_xor_sync(~0u, y, m);
-    if (FOUR && count > 0) {
-        *reinterpret_cast<float4*>(state) = make_float4(h[0], h[1], h[2], h[3]);
-    } else {
+    for (int k = 0; k < OWN; ++k)
+        if (const int ch = lane + 32 * k; ch < count) {
+            x[k] = to_float<T>(static_cast<const T*>(d.x)[env * d.x_stride + c0 + ch]);
+            if (d.gate != nullptr) z[k] = to_float<T>(static_cast<const T*>(d.gate)[env * d.gate_stride + c0 + ch]);
+            const float u = to_float<T>(static_cast<const T*>(d.delta)[env * d.delta_stride + c0 + ch]) + (d.delta_bias != nullptr ? d.delta_bias[c0 + ch] : 0.f), dt = softplus(u, fading<true>(u));
+            m[0][ch] = dt * kToBase2;
+            m[1][ch] = dt * x[k];
+        } else if (ch < CHANNELS) {
+            m[0][ch] = m[1][ch] = 0.f;
+        }
+    __syncwarp();
+    float dt[4], in[4], y[4];
+    take(m[0] + 4 * cl, dt);
+    take(m[1] + 4 * cl, in);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (i < count) state[i] = h[i];
+    for (int j = 0; j < 4; ++j) {
+        y[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            h[j][i] = fmaf(exp2_fast(dt[j] * rate[j][i]), h[j][i], in[j] * b[i]);
+            if (begins) h[j][i] = in[j] * b[i];
+            y[j] = fmaf(c[i], h[j][i], y[j]);
+        }
+        if (wide && 4 * cl + j < count && there >= 4) {
+            put(state + j * states, h[j]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (4 * cl + j < count && i < there) state[j * states + i] = h[j][i];
+        }
     }
-    if (!live || nl != 0) return;
-    if (d.skip != nullptr) y = fmaf(d.skip[ch], x, y);
-    if (d.gate != nullptr) { const float z = to_float<T>(static_cast<const T*>(d.gate)[env * d.gate_stride + ch]); y *= silu<sizeof(T) == 4>(z); }
-    static_cast<T*>(d.y)[env * d.channels + ch] = from_float<T>(y);
+    sum_lanes<4, LN, 1>(y, lane);
+    using K = Kept<4, LN>;
+    if (K::owner(nl))
+#pragma unroll
+        for (int i = 0; i < K::kCount; ++i) m[2][4 * cl + K::first(nl) + i] = y[i];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < OWN; ++k)
+        if (const int ch = lane + 32 * k; ch < count) {
+            float out = m[2][ch];
+            if (d.skip != nullptr) out = fmaf(d.skip[c0 + ch], x[k], out);
+            if (d.gate != nullptr) out *= silu<sizeof(T) == 4>(z[k]);
+            static_cast<T*>(d.y)[env * d.channels + c0 + ch] = from_float<T>(out);
+        }
 }
 
 template <typename T, int LN> static cudaError_t run_scan_step(const nuka_b200_scan_step_t& d, cudaStream_t stream) {
-    const int64_t cells = d.envs * d.channels;
-    const unsigned blocks = (unsigned)((cells * LN + 127) / 128);
-    const bool by_four = d.states % 4 == 0 && reinterpret_cast<uintptr_t>(d.state) % 16 == 0 && reinterpret_cast<uintptr_t>(d.decay) % 16 == 0;
-    if (by_four) scan_step_kernel<T, LN, true><<<blocks, 128, 0, stream>>>(cells, d);
-    else scan_step_kernel<T, LN, false><<<blocks, 128, 0, stream>>>(cells, d);
+    const int64_t tiles = (d.channels + 128 / LN - 1) / (128 / LN), jobs = d.envs * tiles;
+    const bool wide = d.states % 4 == 0 && reinterpret_cast<uintptr_t>(d.state) % 16 == 0 && reinterpret_cast<uintptr_t>(d.decay) % 16 == 0;
+    scan_step_kernel<T, LN><<<(unsigned)((jobs + kScanWarps - 1) / kScanWarps), kScanWarps * 32, 0, stream>>>(jobs, (uint32_t)tiles, wide, d);
     return cudaGetLastError();
 }
 

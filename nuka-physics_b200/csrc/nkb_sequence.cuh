@@ -74,9 +74,20 @@ template <bool EXACT> __device__ __forceinline__ Fading fading(float u) {
 }
 __device__ __forceinline__ float logistic(float u, Fading f) { return u >= 0.f ? f.r : f.e * f.r; }
 __device__ __forceinline__ float one_less(float u, Fading f) { return u >= 0.f ? f.e * f.r : f.r; }             // 1 - logistic(u)
-template <bool EXACT> __device__ __forceinline__ float silu(float s) { return s * logistic(s, fading<EXACT>(s)); }
+// Where 16 bits are the result: 1 / (1 + exp(-s)) at once, the exponential kept finite.
+__device__ __forceinline__ float logistic_fast(float s) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(s * -1.4426950408889634f, 126.f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
+template <bool EXACT> __device__ __forceinline__ float silu(float s) { return s * (EXACT ? logistic(s, fading<true>(s)) : logistic_fast(s)); }
 template <bool EXACT> __device__ __forceinline__ float silu_slope(float s) {
-    const Fading f = fading<EXACT>(s);
+    if (!EXACT) {
+        const float r = logistic_fast(s);
+        return r * fmaf(s, 1.f - r, 1.f);
+    }
+    const Fading f = fading<true>(s);
     return logistic(s, f) * fmaf(s, one_less(s, f), 1.f);
 }
 // log(1 + exp(u)) = max(u, 0) + log(1 + e), the latter by the series of 2 artanh(e / (2 + e)): its argument is 1/3 at most, the first term left out 2^-26 of the sum.

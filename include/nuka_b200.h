@@ -535,7 +535,9 @@ nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* strea
 nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream);
 /* The same where, beside the window's, the first `sinks` tokens of an episode stay visible to all that come after them (without a window all are, whatever sinks is). */
 nuka_result_t nuka_b200_attention_sinks(const nuka_b200_attention_t* desc, int64_t sinks, void* stream);
-nuka_result_t nuka_b200_attention_sinks_backward(const nuka_b200_attention_t* desc, int64_t sinks, void* stream);
+/* The backward call's workspace: bytes on 16 bytes, of which nothing is read before it is written; the desc needs its plan, heads, dim and window for this. */
+uint64_t nuka_b200_attention_sinks_workspace(const nuka_b200_attention_t* desc, int64_t sinks);
+nuka_result_t nuka_b200_attention_sinks_backward(const nuka_b200_attention_t* desc, int64_t sinks, void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Attention of one token of each env over the env's cached history, for acting.  keys and values (envs x capacity x heads_k x dim, contiguous, on 16 bytes) are a
  * ring: the token's k and v are written to place position % capacity, then the token attends to the last min(position + 1, capacity) tokens, itself among

@@ -29,6 +29,7 @@
 #include <algorithm>
 #include "nkb_sequence.cuh"
 #include "nkb_sequence.h"
+#include "nkb_sinks.cuh"
 #include "nkb_tcgen.cuh"
 
 namespace nkb {
@@ -51,6 +52,7 @@ struct AttentionParams {
     void *out, *dq, *dk, *dv;
     const void* dout;
     float *lse, *delta;
+    FarSinks far;                                       // slots 0: the keys' kernel goes through all queries of its sinks itself
 };
 
 __device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
@@ -107,8 +109,8 @@ struct QueryJob {
     template <bool SINKS> __device__ __forceinline__ KeySteps<SINKS> steps(const AttentionParams& p) const { return KeySteps<SINKS>(p, first, i0, last, kStream); }
 };
 
-// One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T; whether all are finite.
-template <typename T, int DP> __device__ __forceinline__ bool store_row(uint32_t at, float by, int dim, T* to) {
+// One thread's row of 32-bit accumulators, times `by`, into DP or fewer values of T; whether all are finite. `more`: sums from elsewhere that belong to them.
+template <typename T, int DP> __device__ __forceinline__ bool store_row(uint32_t at, float by, int dim, T* to, const FarRow& more = FarRow{}) {
     float probe = 0.f;                                  // becomes NaN where a value is not finite
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
@@ -116,6 +118,7 @@ template <typename T, int DP> __device__ __forceinline__ bool store_row(uint32_t
         __syncwarp();
         tensor_load(at + c, r);
         wait_loads();
+        more.add(r, c);
 #pragma unroll
         for (int k = 0; k < 32; k += 8)
             if (to != nullptr && c + k < dim) {
@@ -165,13 +168,14 @@ template <bool SINKS> __device__ __forceinline__ uint32_t RowKeys<SINKS>::seen(i
 // A row of 64-column panels of 128 rows, swizzled as TMA takes it: 16 bytes number `k` of row `row`.
 __device__ __forceinline__ unsigned char* staged(unsigned char* tile, int row, int k) { return tile + k / 8 * kRows * 128 + row * 128 + ((k % 8) ^ (row % 8)) * 16; }
 // A thread's row of 32-bit accumulators, times `by`, into a staged tile of T; whether all are finite.
-template <typename T, int DP> __device__ __forceinline__ bool stage_row(uint32_t at, float by, unsigned char* tile, int row) {
+template <typename T, int DP> __device__ __forceinline__ bool stage_row(uint32_t at, float by, unsigned char* tile, int row, const FarRow& more = FarRow{}) {
     float probe = 0.f;                                  // becomes NaN where a value is not finite
 #pragma unroll
     for (int c = 0; c < DP; c += 32) {
         uint32_t r[32];
         tensor_load(at + c, r);
         wait_loads();
+        more.add(r, c);
 #pragma unroll
         for (int k = 0; k < 32; k += 8) {
 #pragma unroll
@@ -972,9 +976,9 @@ template <bool SINKS> struct KeyJob {
         if (SINKS) first = p.first[last];
     }
     __device__ __forceinline__ int begin() const { return j0 & ~3; }               // of its queries: a multiple of 16 bytes of their statistics
-    // behind the last query that sees one of the keys: sinks of the last key's episode are seen to its end
+    // behind the last query that sees one of the keys: sinks of the last key's episode are seen to its end, by queries of which another kernel may have the far ones
     __device__ __forceinline__ int past(const AttentionParams& p) const {
-        return p.window > 0 && !(SINKS && j0 - first < p.sinks) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
+        return p.window > 0 && !(SINKS && p.far.slots == 0 && j0 - first < p.sinks) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
     }
     __device__ __forceinline__ int steps(const AttentionParams& p) const { return (past(p) - 1 - begin()) / kStream + 1; }            // for one head
 };
@@ -1122,6 +1126,9 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         auto leave = [&]() {
             const int j = leaving.first + row;
             const bool there = j <= leaving.last;
+            FarRow more[2];                             // of the key's gradient and the value's
+            if (SINKS && there && rank == 0)
+                for (int which = 0; which < 2; ++which) more[which] = p.far.row_of(leaving.first / p.span, j - max(leaving.first, p.first[leaving.last]), leaving.head, which, DP);
             if (p.split > 1) {
                 // in 32 bits where the operands were, 16 bytes at a time, rows turned against each other so that lanes meet different banks
 #pragma unroll
@@ -1131,6 +1138,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                         uint32_t r[32];
                         tensor_load(mine + (which ? F::kValue : F::kKey) + c, r);
                         wait_loads();
+                        if (SINKS) more[which].add(r, c);
                         const float by = !fine ? nan_value() : which ? 1.f : p.scale;
 #pragma unroll
                         for (int k = 0; k < 32; k += 4)
@@ -1141,7 +1149,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                 unsigned char *const dv = shared + F::kStaged, *const dk = dv + F::kTile;
                 if (row == 0) wait_stores_read();
                 meet(1, kRows);
-                const bool keys_finite = stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row), values_finite = stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row);
+                const bool keys_finite = stage_row<T, DP>(mine + F::kKey, fine ? p.scale : nan_value(), dk, row, more[0]), values_finite = stage_row<T, DP>(mine + F::kValue, fine ? 1.f : nan_value(), dv, row, more[1]);
                 if (there && !(keys_finite && values_finite)) spoilt = 1;
                 fence_shared();
                 meet(1, kRows);
@@ -1152,7 +1160,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                 }
             } else {
                 T* const to[2] = {static_cast<T*>(p.dk) + ((int64_t)j * p.heads_k + leaving.head) * p.dim, static_cast<T*>(p.dv) + ((int64_t)j * p.heads_k + leaving.head) * p.dim};
-                const bool finite = store_row<T, DP>(mine + (half ? F::kValue : F::kKey), !fine ? nan_value() : half ? 1.f : p.scale, p.dim, there ? to[half] : nullptr);
+                const bool finite = store_row<T, DP>(mine + (half ? F::kValue : F::kKey), !fine ? nan_value() : half ? 1.f : p.scale, p.dim, there ? to[half] : nullptr, half ? more[1] : more[0]);
                 if (there && !finite) spoilt = 1;
             }
         };
@@ -1167,7 +1175,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
             const int j = now.j0 + row, each = now.steps(p);
             const bool live = j <= now.last;
             // the queries that see the key
-            const int low = live ? j : 0, high = !live ? -1 : (p.window > 0 && !next_sink ? (int)min((int64_t)next_end, (int64_t)j + p.window) : next_end) - 1;
+            const int low = live ? j : 0, high = !live ? -1 : SINKS && next_sink ? min(next_end, now.past(p)) - 1 : (p.window > 0 ? (int)min((int64_t)next_end, (int64_t)j + p.window) : next_end) - 1;
             if (job + stride < jobs) { next = KeyJob<SINKS>(p, job + stride); next_end = end_of(next); next_sink = sink_of(next); }
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
@@ -1321,7 +1329,7 @@ static int tile_span(const nuka_b200_episodes_t& plan) {
 
 template <typename K> static cudaError_t with_shared(K kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 
-template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream) {
+template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const nuka_b200_attention_t& d, int64_t sinks, void* workspace, bool backward, cudaStream_t stream) {
     AttentionParams p{};
     const nuka_b200_episodes_t& e = *d.plan;
     p.first = e.first; p.end = e.end; p.tokens = e.tokens; p.pitch = attention_pitch(e.tokens);
@@ -1345,6 +1353,7 @@ template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const
         attention_kernel<T, DP, SINKS><<<(unsigned)std::min(p.across * p.along, 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();
     }
+    if (SINKS) p.far = far_sinks(d, sinks, p.span, p.tiles, workspace);
     CUtensorMap dq, dk, dv;
     for (int keys = 0; keys < 2; ++keys) {
         const int own = keys ? kStream : kRows, other = keys ? kRows : kStream;
@@ -1361,6 +1370,8 @@ template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const
         const int64_t row = e.tokens / std::max<int64_t>(e.rows, 1), reach = d.window > 0 ? std::min<int64_t>(row, d.window) : row, places = reach >= 1024 ? 4 * slots : slots;
         p.split = 1;
         while (keys && p.split < 8 && group % (2 * p.split) == 0 && 2 * p.split * (int64_t)jobs <= places) p.split *= 2;
+        if (keys && p.far.slots > 0)
+            if (const cudaError_t far = launch_far_sinks(d, p.window, p.sinks, p.span, p.tiles, p.pitch, p.far, stream); far != cudaSuccess) return far;
         if (!keys) {
             query_grad_kernel<T, DP, SINKS><<<(unsigned)blocks, Queries<DP>::kThreads, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         } else if (p.split == 1) {
@@ -1381,14 +1392,21 @@ template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const
     return cudaSuccess;
 }
 
-template <bool SINKS> static cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream) {
-    if (d.dtype == NUKA_B200_F16) return d.dim <= 64 ? run_attention<__half, 64, SINKS>(d, sinks, backward, stream) : run_attention<__half, 128, SINKS>(d, sinks, backward, stream);
-    return d.dim <= 64 ? run_attention<__nv_bfloat16, 64, SINKS>(d, sinks, backward, stream) : run_attention<__nv_bfloat16, 128, SINKS>(d, sinks, backward, stream);
+template <bool SINKS> static cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, void* workspace, bool backward, cudaStream_t stream) {
+    if (d.dtype == NUKA_B200_F16)
+        return d.dim <= 64 ? run_attention<__half, 64, SINKS>(d, sinks, workspace, backward, stream) : run_attention<__half, 128, SINKS>(d, sinks, workspace, backward, stream);
+    return d.dim <= 64 ? run_attention<__nv_bfloat16, 64, SINKS>(d, sinks, workspace, backward, stream) : run_attention<__nv_bfloat16, 128, SINKS>(d, sinks, workspace, backward, stream);
 }
 
-cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream) {
+cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, void* workspace, bool backward, cudaStream_t stream) {
     if (d.plan->tokens == 0) return cudaSuccess;
-    return sinks > 0 && d.window > 0 ? launch_attention<true>(d, sinks, backward, stream) : launch_attention<false>(d, 0, backward, stream);
+    return sinks > 0 && d.window > 0 ? launch_attention<true>(d, sinks, workspace, backward, stream) : launch_attention<false>(d, 0, nullptr, backward, stream);
+}
+
+uint64_t attention_workspace(const nuka_b200_attention_t& d, int64_t sinks) {
+    if (sinks <= 0 || d.window <= 0 || d.plan->tokens == 0) return 0u;
+    const int span = tile_span(*d.plan);
+    return far_sinks_bytes(d, sinks, span, (int)((d.plan->tokens + span - 1) / span));
 }
 
 }  // namespace nkb

@@ -31,7 +31,8 @@ uint64_t heads_workspace(int64_t tokens, int64_t dim);
 cudaError_t launch_heads(const nuka_b200_heads_t& d, bool backward, cudaStream_t stream);
 
 int64_t attention_pitch(int64_t tokens);
-cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, bool backward, cudaStream_t stream);
+uint64_t attention_workspace(const nuka_b200_attention_t& d, int64_t sinks);
+cudaError_t launch_attention(const nuka_b200_attention_t& d, int64_t sinks, void* workspace, bool backward, cudaStream_t stream);
 
 uint64_t history_workspace(const nuka_b200_history_t& d);
 cudaError_t launch_history(const nuka_b200_history_t& d, int64_t sinks, cudaStream_t stream);

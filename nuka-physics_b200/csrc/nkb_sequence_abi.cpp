@@ -243,7 +243,7 @@ nuka_result_t nuka_b200_heads_backward(const nuka_b200_heads_t* desc, void* stre
 
 int64_t nuka_b200_attention_pitch(int64_t tokens) { return tokens <= 0 ? 0 : nkb::attention_pitch(tokens); }
 
-static nuka_result_t Attention(const nuka_b200_attention_t* desc, int64_t sinks, bool backward, void* stream) {
+static nuka_result_t Attention(const nuka_b200_attention_t* desc, int64_t sinks, void* workspace, uint64_t workspace_bytes, bool backward, void* stream) {
     if (desc == nullptr) return Invalid("attention desc is null");
     const nuka_b200_attention_t& d = *desc;
     if (const char* fault = PlanFault(d.plan)) return Invalid(fault);
@@ -267,13 +267,20 @@ static nuka_result_t Attention(const nuka_b200_attention_t* desc, int64_t sinks,
                                                         {d.plan->tokens, d.v_stride}, {d.heads_k, d.v_head_stride}};
     for (const auto& s : strides)
         if (s.size > 1 && (s.stride < d.dim || s.stride % 8 != 0 || s.stride >= (1ll << 38))) return Invalid("strides must be multiples of 8 values, at least dim");
-    return Ran(nkb::launch_attention(d, sinks, backward, StreamOf(stream)));
+    const uint64_t need = backward ? nkb::attention_workspace(d, sinks) : 0u;
+    if (need != 0u && (workspace == nullptr || workspace_bytes < need || !Aligned(workspace, 16))) return Invalid("the workspace is null, too small or not on 16 bytes");
+    return Ran(nkb::launch_attention(d, sinks, workspace, backward, StreamOf(stream)));
 }
 
-nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, 0, false, stream); }
-nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, 0, true, stream); }
-nuka_result_t nuka_b200_attention_sinks(const nuka_b200_attention_t* desc, int64_t sinks, void* stream) { return Attention(desc, sinks, false, stream); }
-nuka_result_t nuka_b200_attention_sinks_backward(const nuka_b200_attention_t* desc, int64_t sinks, void* stream) { return Attention(desc, sinks, true, stream); }
+nuka_result_t nuka_b200_attention(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, 0, nullptr, 0, false, stream); }
+nuka_result_t nuka_b200_attention_backward(const nuka_b200_attention_t* desc, void* stream) { return Attention(desc, 0, nullptr, 0, true, stream); }
+nuka_result_t nuka_b200_attention_sinks(const nuka_b200_attention_t* desc, int64_t sinks, void* stream) { return Attention(desc, sinks, nullptr, 0, false, stream); }
+uint64_t nuka_b200_attention_sinks_workspace(const nuka_b200_attention_t* desc, int64_t sinks) {
+    return desc == nullptr || PlanFault(desc->plan) != nullptr || desc->heads_k < 1 || desc->heads_k > 65536 || desc->dim < 8 || desc->dim > 128 ? 0u : nkb::attention_workspace(*desc, sinks);
+}
+nuka_result_t nuka_b200_attention_sinks_backward(const nuka_b200_attention_t* desc, int64_t sinks, void* workspace, uint64_t workspace_bytes, void* stream) {
+    return Attention(desc, sinks, workspace, workspace_bytes, true, stream);
+}
 
 static const char* HistoryFault(const nuka_b200_history_t& d) {
     if (d.envs < 0 || d.envs > kMostTokens || d.capacity < 1 || d.capacity > (1 << 30)) return "envs must not be negative, capacity 1 to 2^30";

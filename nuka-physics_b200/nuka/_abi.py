@@ -144,7 +144,7 @@ EXPORTS = [
     "nuka_b200_attention_pitch", "nuka_b200_attention", "nuka_b200_attention_backward",
     "nuka_b200_history_workspace", "nuka_b200_history", "nuka_b200_history_advance",
     "nuka_b200_convolution_workspace", "nuka_b200_convolution", "nuka_b200_convolution_backward", "nuka_b200_convolution_step",
-    "nuka_b200_attention_sinks", "nuka_b200_attention_sinks_backward", "nuka_b200_history_sinks", "nuka_b200_scan_kept", "nuka_b200_scan_workspace", "nuka_b200_scan", "nuka_b200_scan_backward", "nuka_b200_scan_step",
+    "nuka_b200_attention_sinks", "nuka_b200_attention_sinks_workspace", "nuka_b200_attention_sinks_backward", "nuka_b200_history_sinks", "nuka_b200_scan_kept", "nuka_b200_scan_workspace", "nuka_b200_scan", "nuka_b200_scan_backward", "nuka_b200_scan_step",
 ]
 
 _LIB = None
@@ -238,7 +238,9 @@ def lib():
     L.nuka_b200_convolution_backward.argtypes = [ctypes.POINTER(ConvolutionDesc), vp]
     L.nuka_b200_convolution_step.argtypes = [ctypes.POINTER(ConvolutionStepDesc), vp]
     L.nuka_b200_attention_sinks.argtypes = [ctypes.POINTER(AttentionDesc), i64, vp]
-    L.nuka_b200_attention_sinks_backward.argtypes = [ctypes.POINTER(AttentionDesc), i64, vp]
+    L.nuka_b200_attention_sinks_workspace.argtypes = [ctypes.POINTER(AttentionDesc), i64]
+    L.nuka_b200_attention_sinks_workspace.restype = u64
+    L.nuka_b200_attention_sinks_backward.argtypes = [ctypes.POINTER(AttentionDesc), i64, vp, u64, vp]
     L.nuka_b200_history_sinks.argtypes = [ctypes.POINTER(HistoryDesc), i64, vp]
     L.nuka_b200_scan_kept.argtypes = [ctypes.POINTER(EpisodesDesc), i64, i64]
     L.nuka_b200_scan_kept.restype = u64

@@ -613,7 +613,10 @@ class _Attention(torch.autograd.Function):
         delta = _empty(lse)
         desc.dout, desc.delta, desc.dq, desc.dk, desc.dv = dout.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
         if ctx.sinks:
-            stream = _call(device, _abi.lib().nuka_b200_attention_sinks_backward, ctypes.byref(desc), ctx.sinks)
+            lib = _abi.lib()
+            need = lib.nuka_b200_attention_sinks_workspace(ctypes.byref(desc), ctx.sinks)
+            workspace = _workspace(need, device)
+            stream = _call(device, lib.nuka_b200_attention_sinks_backward, ctypes.byref(desc), ctx.sinks, _ptr(workspace), need)
         else:
             stream = _call(device, _abi.lib().nuka_b200_attention_backward, ctypes.byref(desc))
         ctx.episodes._read_on(stream)

@@ -204,7 +204,7 @@ def test_wrong_arguments_are_refused():
     ok = dict(plan=plan._ref, dtype=2, heads_q=4, heads_k=4, dim=64, window=4, scale=0.125, q=q.data_ptr(), k=q.data_ptr(), v=q.data_ptr(), q_stride=256, q_head_stride=64, k_stride=256,
               k_head_stride=64, v_stride=256, v_head_stride=64, out=q.data_ptr())
     assert lib.nuka_b200_attention_sinks(ctypes.byref(_abi.AttentionDesc(**ok)), -1, None) == _abi.INVALID_ARG
-    assert lib.nuka_b200_attention_sinks_backward(ctypes.byref(_abi.AttentionDesc(**ok)), 2, None) == _abi.INVALID_ARG
+    assert lib.nuka_b200_attention_sinks_backward(ctypes.byref(_abi.AttentionDesc(**ok)), 2, None, 0, None) == _abi.INVALID_ARG
     ring = dict(dtype=2, envs=1, capacity=8, heads_q=1, heads_k=1, dim=64, scale=1.0, q=q.data_ptr(), k=q.data_ptr(), v=q.data_ptr(), keys=q.data_ptr(), values=q.data_ptr(), position=q.data_ptr(), out=q.data_ptr())
     for sinks in (-1, 8):
         assert lib.nuka_b200_history_sinks(ctypes.byref(_abi.HistoryDesc(**ring)), sinks, None) == _abi.INVALID_ARG

@@ -16,7 +16,7 @@ namespace nkb {
 constexpr int kLines = 4;                               // warps of a block: stretches side by side
 constexpr int kForthBlocks = 5, kBackBlocks = 4;        // blocks of an SM
 constexpr int kForthBatch = 4, kBackBatch = 4;          // tokens whose loads are under way; a multiple of the longest window, so that its shift is a change of names
-constexpr int kBytes = 8;                               // of a thread's channels
+constexpr int kWide = 4;                                // channels of a thread
 constexpr int kSms = 148;
 
 struct ConvolutionParams {
@@ -356,15 +356,14 @@ template <typename T, int VEC> static cudaError_t run_convolution(const nuka_b20
     return d.width == 2 ? run_convolution<T, 2, VEC>(d, backward, stream) : d.width == 3 ? run_convolution<T, 3, VEC>(d, backward, stream) : run_convolution<T, 4, VEC>(d, backward, stream);
 }
 
-// kBytes to a thread where everything lies so, else a value.
+// kWide channels to a thread where everything lies on as many, else one.
 template <typename T> static cudaError_t run_convolution(const nuka_b200_convolution_t& d, bool backward, cudaStream_t stream) {
-    constexpr int W = kBytes / sizeof(T);
-    bool wide = d.channels % W == 0 && d.x_stride % W == 0;
-    auto lies = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % kBytes == 0; };
+    bool wide = d.channels % kWide == 0 && d.x_stride % kWide == 0;
+    auto lies = [](const void* at) { return reinterpret_cast<uintptr_t>(at) % (kWide * sizeof(T)) == 0; };
     for (const void* p : {d.x, d.initial, static_cast<const void*>(d.y), static_cast<const void*>(d.state)}) wide = wide && lies(p);
     if (backward)
         for (const void* p : {d.dy, d.dstate, static_cast<const void*>(d.dx), static_cast<const void*>(d.dinitial)}) wide = wide && lies(p);
-    return wide ? run_convolution<T, W>(d, backward, stream) : run_convolution<T, 1>(d, backward, stream);
+    return wide ? run_convolution<T, kWide>(d, backward, stream) : run_convolution<T, 1>(d, backward, stream);
 }
 
 cudaError_t launch_convolution(const nuka_b200_convolution_t& d, bool backward, cudaStream_t stream) {

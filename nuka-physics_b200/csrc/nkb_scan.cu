@@ -954,7 +954,7 @@ cudaError_t launch_scan(const nuka_b200_scan_t& d, bool backward, cudaStream_t s
 
 // ---- one token per env ---------------------------------------------------------------------------------------------
 // The states' bytes bound it. A warp has an env and a tile of channels, its lanes four channels of four states each, as over rollouts; what a channel's states share is worked out by one lane.
-template <typename T, int LN> __global__ void __launch_bounds__(kScanWarps * 32) scan_step_kernel(int64_t jobs, uint32_t tiles, bool wide, const nuka_b200_scan_step_t d) {
+template <typename T, int LN> __global__ void __launch_bounds__(kScanWarps * 32, 6) scan_step_kernel(int64_t jobs, uint32_t tiles, bool wide, const nuka_b200_scan_step_t d) {
     constexpr int CHANNELS = 128 / LN, OWN = (CHANNELS + 31) / 32;
     __shared__ __align__(16) float shared[kScanWarps][3][CHANNELS];
     const int lane = threadIdx.x % 32, nl = lane % LN, cl = lane / LN;

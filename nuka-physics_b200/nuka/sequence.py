@@ -93,6 +93,11 @@ def _channels_last(tensor, multiple=1, size=1, least=0):
     return tensor.clone(memory_format=torch.contiguous_format)
 
 
+def _rows(tensor):
+    """The tensor as it is where its last dimension is contiguous, else a copy."""
+    return tensor if tensor.stride(-1) == 1 else _channels_last(tensor)
+
+
 def _point(desc, names, tensors, strides=None, size=1):
     """Sets the descriptor's addresses to those that the tensors have. What a backward pass finds saved may lie elsewhere than in the forward call, and otherwise (offloaded, worked
     out again): False where a stride is not what it was or an address is not on `size` bytes."""
@@ -354,15 +359,16 @@ def short_convolution_step(x, weight, bias, state, fresh=None, silu=False):
     device = _on_gpu(x, weight, bias, state, fresh)
     dtype = _dtype(x, _DTYPES, "x")
     _expect(x.dim() == 2, "x must be envs x channels")
-    weight, bias = _convolution_weights(weight, bias, x.shape[1])
-    envs, channels, width = x.shape[0], x.shape[1], weight.shape[1]
+    envs, channels = x.shape
+    weight, bias = _convolution_weights(weight, bias, channels)
+    width = weight.shape[1]
     if state.shape != (envs, width - 1, channels) or state.dtype != x.dtype or not state.is_contiguous():
         raise ValueError(f"state must be contiguous, {envs} x {width - 1} x {channels} of x's type")
-    x = _channels_last(x)
+    x = _rows(x)
     if fresh is not None:
         fresh = _flags(fresh, x.shape[:1], device, "fresh")
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    desc = _abi.ConvolutionStepDesc(dtype, bool(silu), envs, channels, width, x.data_ptr(), _stride(x, 0), weight.data_ptr(), _ptr(bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
+    y = torch.empty((envs, channels), dtype=x.dtype, device=device)
+    desc = _abi.ConvolutionStepDesc(dtype, bool(silu), envs, channels, width, x.data_ptr(), x.stride(0) if envs > 1 else 0, weight.data_ptr(), _ptr(bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
     _call(device, _abi.lib().nuka_b200_convolution_step, ctypes.byref(desc))
     return y
 
@@ -434,18 +440,18 @@ class _Scan(torch.autograd.Function):
 
 def _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias):
     """Checks what the scan and its step have in common; the inputs as the kernels take them."""
+    dtype, shape = x.dtype, x.shape
     _dtype(x, _DTYPES, "x")
-    if x.dim() != 2 or decay.dim() != 2 or decay.shape[0] != x.shape[1] or not 1 <= decay.shape[1] <= 64 or decay.dtype != torch.float32:
+    if len(shape) != 2 or decay.dim() != 2 or decay.shape[0] != shape[1] or not 1 <= decay.shape[1] <= 64 or decay.dtype != torch.float32:
         raise ValueError("x must have 2 dimensions, the second of channels, and decay must be float32, channels x 1 to 64 states")
-    for v, shape, what in ((delta, x.shape, "delta"), (gate, x.shape, "gate"), (b, (x.shape[0], decay.shape[1]), "b"), (c, (x.shape[0], decay.shape[1]), "c")):
-        if v is not None and (v.shape != shape or v.dtype != x.dtype):
-            raise ValueError(f"{what} must be {' x '.join(map(str, shape))}, of x's type")
-    for v, what in ((skip, "skip"), (delta_bias, "delta_bias")):
-        if v is not None and (v.shape != x.shape[1:] or v.dtype != torch.float32):
-            raise ValueError(f"{what} must be float32, one per channel")
-    x, delta, b, c = (_channels_last(v) for v in (x, delta, b, c))
-    gate = None if gate is None else _channels_last(gate)
-    return x, delta, decay.contiguous(), b, c, None if skip is None else skip.contiguous(), gate, None if delta_bias is None else delta_bias.contiguous()
+    narrow = (shape[0], decay.shape[1])
+    if not (delta.shape == shape and delta.dtype == dtype and b.shape == narrow and b.dtype == dtype and c.shape == narrow and c.dtype == dtype and (gate is None or (gate.shape == shape and gate.dtype == dtype))):
+        raise ValueError(f"delta and gate must be like x, b and c {' x '.join(map(str, narrow))}, of x's type")
+    for v in (skip, delta_bias):
+        if v is not None and (v.shape != shape[1:] or v.dtype != torch.float32):
+            raise ValueError("skip and delta_bias must be float32, one per channel")
+    return (_rows(x), _rows(delta), decay.contiguous(), _rows(b), _rows(c), None if skip is None else skip.contiguous(), None if gate is None else _rows(gate),
+            None if delta_bias is None else delta_bias.contiguous())
 
 
 def selective_scan(x, delta, decay, b, c, episodes, initial=None, skip=None, gate=None, delta_bias=None):
@@ -471,13 +477,15 @@ def selective_scan_step(x, delta, decay, b, c, state, fresh=None, skip=None, gat
     uint8, set where the token begins an episode (the state before it counts as 0).  Returns y like x.  No gradient."""
     device = _on_gpu(x, delta, decay, b, c, state, fresh, skip, gate, delta_bias)
     x, delta, decay, b, c, skip, gate, delta_bias = _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias)
-    if state.shape != (x.shape[0], *decay.shape) or state.dtype != torch.float32 or not state.is_contiguous():
-        raise ValueError(f"state must be contiguous float32, {x.shape[0]} x {decay.shape[0]} x {decay.shape[1]}")
+    (envs, channels), states = x.shape, decay.shape[1]
+    if state.shape != (envs, channels, states) or state.dtype != torch.float32 or not state.is_contiguous():
+        raise ValueError(f"state must be contiguous float32, {envs} x {channels} x {states}")
     if fresh is not None:
         fresh = _flags(fresh, x.shape[:1], device, "fresh")
-    y = torch.empty(x.shape, dtype=x.dtype, device=device)
-    desc = _abi.ScanStepDesc(_DTYPES[x.dtype], x.shape[0], *decay.shape, x.data_ptr(), delta.data_ptr(), _ptr(gate), b.data_ptr(), c.data_ptr(), _stride(x, 0), _stride(delta, 0),
-                             0 if gate is None else _stride(gate, 0), _stride(b, 0), _stride(c, 0), decay.data_ptr(), _ptr(skip), _ptr(delta_bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
+    y = torch.empty((envs, channels), dtype=x.dtype, device=device)
+    strides = (x.stride(0), delta.stride(0), 0 if gate is None else gate.stride(0), b.stride(0), c.stride(0)) if envs > 1 else (0, 0, 0, 0, 0)
+    desc = _abi.ScanStepDesc(_DTYPES[x.dtype], envs, channels, states, x.data_ptr(), delta.data_ptr(), None if gate is None else gate.data_ptr(), b.data_ptr(), c.data_ptr(), *strides,
+                             decay.data_ptr(), _ptr(skip), _ptr(delta_bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
     _call(device, _abi.lib().nuka_b200_scan_step, ctypes.byref(desc))
     return y
 

@@ -27,7 +27,7 @@ struct ConvolutionParams {
     const void *x, *initial, *dy, *dstate;
     void *y, *state, *dx, *dinitial;
     float* partial;                                     // of the weights' gradients: across x (K + 1) x channels
-    bool act, sums;
+    bool act, sums, whole;                              // whole: every stretch ends with an episode
 };
 
 // sum += a b, two values at a time where there are two
@@ -129,10 +129,7 @@ __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(
         for (int i = 0; i < BATCH; ++i) now[i] = ahead[i];
         const Marks marks(p, begin + t0, left);
         if (t0 + BATCH < count) fetch(t0 + BATCH);
-#pragma unroll
-        for (int i = 0; i < BATCH; ++i) {
-            if (i >= left) break;
-            if (marks.begins >> i & 1u) window_begins<T, K, VEC>(p, marks.row_of(i), c, window);
+        auto token = [&](int i) {
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
 #pragma unroll
@@ -145,11 +142,27 @@ __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(
                 for (int v = 0; v < VEC; ++v) s[v] = silu<sizeof(T) == 4>(s[v]);
             if (live) store<T, VEC>(y, s);
             y += C;
-            if (marks.ends >> i & 1u) {
-                T* const to = static_cast<T*>(p.state) + (int64_t)marks.end_of(i) * (K - 1) * C + c;
+        };
+        auto begin_at = [&](int i) { window_begins<T, K, VEC>(p, marks.row_of(i), c, window); };
+        auto end_at = [&](int i) {
+            T* const to = static_cast<T*>(p.state) + (int64_t)marks.end_of(i) * (K - 1) * C + c;
 #pragma unroll
-                for (int j = 0; j < K - 1; ++j)
-                    if (live) store<T, VEC>(to + j * C, window[j + 1]);
+            for (int j = 0; j < K - 1; ++j)
+                if (live) store<T, VEC>(to + j * C, window[j + 1]);
+        };
+        // mostly nothing begins or ends but at the edges
+        if (left == BATCH && (marks.begins & ~1u) == 0u && (marks.ends & ~(1u << (BATCH - 1))) == 0u) {
+            if (marks.begins != 0u) begin_at(0);
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) token(i);
+            if (marks.ends != 0u) end_at(BATCH - 1);
+        } else {
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) {
+                if (i >= left) break;
+                if (marks.begins >> i & 1u) begin_at(i);
+                token(i);
+                if (marks.ends >> i & 1u) end_at(i);
             }
         }
     }
@@ -168,7 +181,7 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
     for (int64_t line = (int64_t)(blockIdx.x / p.tiles) * kLines + warp; line < p.stretches; line += (int64_t)p.across * kLines) {
         // tokens by their number from the walk's first one
         const int64_t begin = line * p.stretch;
-        const int end = (int)min(p.stretch, p.plan.tokens - begin), past = (int)min((int64_t)end + K - 1, p.plan.tokens - begin);
+        const int end = (int)min(p.stretch, p.plan.tokens - begin), past = p.whole ? end : (int)min((int64_t)end + K - 1, p.plan.tokens - begin);
         float window[K][VEC], grad[K][VEC];             // grad: of the inputs in the window, as far as they are complete
         int first = 0, row = -1;                        // of the episode; the row that it began, within this walk
 #pragma unroll
@@ -201,6 +214,53 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
                 dys[i] = load_raw<T, VEC>(dy + t * C);
             }
             const Marks marks(p, begin + t0, left);
+            // one input further, whose gradient the others' are added to; own: the token is the walk's
+            auto token = [&](int i, bool own) {
+#pragma unroll
+                for (int j = 0; j < K - 1; ++j)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) { window[j][v] = window[j + 1][v]; grad[j][v] = grad[j + 1][v]; }
+                unpack<T, VEC>(xs[i], window[K - 1]);
+                float ds[VEC];
+                unpack<T, VEC>(dys[i], ds);
+                if (p.act) {
+                    float s[VEC];
+                    f.sum(window, s);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) ds[v] *= silu_slope<sizeof(T) == 4>(s[v]);
+                }
+#pragma unroll
+                for (int j = 0; j < K - 1; ++j) add_products(grad[j], f.w[j], ds);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) grad[K - 1][v] = f.w[K - 1][v] * ds[v];
+                if (own) {
+#pragma unroll
+                    for (int j = 0; j < K; ++j) add_products(dw[j], ds, window[j]);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) db[v] += ds[v];
+                }
+            };
+            auto end_at = [&](int i) {
+                const int32_t ended = marks.end_of(i);
+                if (p.dstate == nullptr) return;
+#pragma unroll
+                for (int j = 0; j < K - 1; ++j) {
+                    float more[VEC];
+                    input<T, VEC>(p.dstate, ((int64_t)ended * (K - 1) + j) * C + c, true, more);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) grad[j + 1][v] += more[v];
+                }
+            };
+            // mostly nothing begins, or ends but at the edge, and what leaves is the walk's and the episode's
+            if (t0 >= K && first <= t0 - K && t0 + BATCH <= end && marks.begins == 0u && (marks.ends & ~(1u << (BATCH - 1))) == 0u) {
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    if (live) store<T, VEC>(dx + (t0 + i - K) * C, grad[0]);
+                    token(i, true);
+                }
+                if (marks.ends != 0u) end_at(BATCH - 1);
+                continue;
+            }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
                 const int t = t0 + i;
@@ -220,39 +280,8 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
                 } else if (t > 0) {
                     leave(t - K, grad[0]);
                 }
-#pragma unroll
-                for (int j = 0; j < K - 1; ++j)
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) { window[j][v] = window[j + 1][v]; grad[j][v] = grad[j + 1][v]; }
-                unpack<T, VEC>(xs[i], window[K - 1]);
-                float ds[VEC];
-                unpack<T, VEC>(dys[i], ds);
-                if (p.act) {
-                    float s[VEC];
-                    f.sum(window, s);
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) ds[v] *= silu_slope<sizeof(T) == 4>(s[v]);
-                }
-#pragma unroll
-                for (int j = 0; j < K - 1; ++j) add_products(grad[j], f.w[j], ds);
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) grad[K - 1][v] = f.w[K - 1][v] * ds[v];
-                if (t < end) {
-#pragma unroll
-                    for (int j = 0; j < K; ++j) add_products(dw[j], ds, window[j]);
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) db[v] += ds[v];
-                }
-                if (marks.ends >> i & 1u && p.dstate != nullptr) {
-                    const int32_t ended = marks.end_of(i);
-#pragma unroll
-                    for (int j = 0; j < K - 1; ++j) {
-                        float more[VEC];
-                        input<T, VEC>(p.dstate, ((int64_t)ended * (K - 1) + j) * C + c, true, more);
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) grad[j + 1][v] += more[v];
-                    }
-                }
+                token(i, t < end);
+                if (marks.ends >> i & 1u) end_at(i);
             }
         }
 #pragma unroll
@@ -325,7 +354,7 @@ template <typename T, int VEC> static ConvolutionParams convolution_params(const
     p.stretches = (p.plan.tokens + p.stretch - 1) / p.stretch;
     p.tiles = (uint32_t)((d.channels + 32 * VEC - 1) / (32 * VEC));
     p.across = (uint32_t)((p.stretches + kLines - 1) / kLines);
-    p.weight = d.weight; p.bias = d.bias; p.act = d.silu != 0u;
+    p.weight = d.weight; p.bias = d.bias; p.act = d.silu != 0u; p.whole = p.plan.length > 0 && p.stretch % p.plan.length == 0;
     p.x = d.x; p.initial = d.initial; p.dy = d.dy; p.dstate = d.dstate;
     p.y = d.y; p.state = d.state; p.dx = d.dx; p.dinitial = d.dinitial;
     return p;

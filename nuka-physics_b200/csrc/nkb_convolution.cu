@@ -27,7 +27,7 @@ struct ConvolutionParams {
     const void *x, *initial, *dy, *dstate;
     void *y, *state, *dx, *dinitial;
     float* partial;                                     // of the weights' gradients: across x (K + 1) x channels
-    bool act, sums, whole;                              // whole: every stretch ends with an episode
+    bool act, sums, whole, wide_weights;                // whole: every stretch ends with an episode; wide_weights: they lie on 16 bytes
 };
 
 // sum += a b, two values at a time where there are two
@@ -44,10 +44,18 @@ template <int N> __device__ __forceinline__ void add_products(float (&sum)[N], c
 template <typename T, int K, int VEC> struct Line {
     float w[K][VEC], bias[VEC];
     __device__ __forceinline__ Line(const ConvolutionParams& p, int64_t c) {
+        float all[VEC * K];
+        if (VEC % 4 == 0 && p.wide_weights) {
+#pragma unroll
+            for (int k = 0; k < VEC * K; k += 4) { const float4 q = *reinterpret_cast<const float4*>(p.weight + c * K + k); all[k] = q.x; all[k + 1] = q.y; all[k + 2] = q.z; all[k + 3] = q.w; }
+        } else {
+#pragma unroll
+            for (int k = 0; k < VEC * K; ++k) all[k] = p.weight[c * K + k];
+        }
 #pragma unroll
         for (int v = 0; v < VEC; ++v) {
 #pragma unroll
-            for (int j = 0; j < K; ++j) w[j][v] = p.weight[(c + v) * K + j];
+            for (int j = 0; j < K; ++j) w[j][v] = all[v * K + j];
             bias[v] = p.bias != nullptr ? p.bias[c + v] : 0.f;
         }
     }
@@ -339,22 +347,26 @@ template <int K> __global__ void __launch_bounds__(1024) convolution_sums_kernel
     if (j < K) { if (dweight != nullptr) dweight[c * K + j] = sum; } else if (dbias != nullptr) dbias[c] = sum;
 }
 
-// Tokens of a walk: whole rows where they are of one short length; else as many as leave every SM sixty-four walks of 128 channels, 32 to 128, for which K - 1 are read twice.
-static int64_t stretch_of(const nuka_b200_episodes_t& plan, int64_t channels) {
-    if (plan.length > 0 && plan.length <= 64) return plan.length * std::max<int64_t>(1, 32 / plan.length);
-    const int64_t tiles = (channels + 127) / 128;
-    return std::min<int64_t>(plan.tokens, std::max<int64_t>(32, std::min<int64_t>(128, plan.tokens * tiles / (64 * kSms) / 4 * 4)));
+// Tokens of a walk. Whole rows where they are of one short length; else forwards as many as leave every SM sixty-four walks of 128 channels, 32 to 128, for which K - 1 are read twice; backwards, where a warp takes
+// walks in turn, equal shares of about as many.
+static int64_t walkers_of(int64_t channels) { return std::max<int64_t>(1, kBackBlocks * kSms / ((channels + 32 * kWide - 1) / (32 * kWide))) * kLines; }
+static int64_t stretch_of(const nuka_b200_episodes_t& plan, int64_t channels, bool backward) {
+    const int64_t tiles = (channels + 32 * kWide - 1) / (32 * kWide), fit = std::max<int64_t>(32, std::min<int64_t>(128, plan.tokens * tiles / (64 * kSms) / 4 * 4));
+    if (plan.length > 0 && plan.length <= 64) return plan.length * std::max<int64_t>(1, ((backward ? 32 : fit) + plan.length / 2) / plan.length);
+    if (!backward) return std::min<int64_t>(plan.tokens, fit);
+    const int64_t walkers = walkers_of(channels), turns = (plan.tokens + 128 * walkers - 1) / (128 * walkers);
+    return std::min<int64_t>(plan.tokens, std::max<int64_t>(32, (plan.tokens + turns * walkers - 1) / (turns * walkers)));
 }
 
-template <typename T, int VEC> static ConvolutionParams convolution_params(const nuka_b200_convolution_t& d) {
+template <typename T, int VEC> static ConvolutionParams convolution_params(const nuka_b200_convolution_t& d, bool backward) {
     ConvolutionParams p{};
     p.plan = *d.plan;
     p.channels = d.channels; p.x_stride = d.x_stride;
-    p.stretch = stretch_of(p.plan, d.channels);
+    p.stretch = stretch_of(p.plan, d.channels, backward);
     p.stretches = (p.plan.tokens + p.stretch - 1) / p.stretch;
     p.tiles = (uint32_t)((d.channels + 32 * VEC - 1) / (32 * VEC));
     p.across = (uint32_t)((p.stretches + kLines - 1) / kLines);
-    p.weight = d.weight; p.bias = d.bias; p.act = d.silu != 0u; p.whole = p.plan.length > 0 && p.stretch % p.plan.length == 0;
+    p.weight = d.weight; p.bias = d.bias; p.act = d.silu != 0u; p.whole = p.plan.length > 0 && p.stretch % p.plan.length == 0; p.wide_weights = reinterpret_cast<uintptr_t>(d.weight) % 16 == 0;
     p.x = d.x; p.initial = d.initial; p.dy = d.dy; p.dstate = d.dstate;
     p.y = d.y; p.state = d.state; p.dx = d.dx; p.dinitial = d.dinitial;
     return p;
@@ -362,13 +374,13 @@ template <typename T, int VEC> static ConvolutionParams convolution_params(const
 
 // Blocks along the tokens of the backward pass, each of which leaves a set of partial sums: as many as run at a time.
 static int64_t convolution_across(const nuka_b200_episodes_t& plan, int64_t channels) {
-    const int64_t stretch = stretch_of(plan, channels), stretches = (plan.tokens + stretch - 1) / stretch, tiles = (channels + 127) / 128;
-    return std::max<int64_t>(1, std::min<int64_t>((stretches + kLines - 1) / kLines, std::max<int64_t>(1, kBackBlocks * kSms / tiles)));
+    const int64_t stretch = stretch_of(plan, channels, true), stretches = (plan.tokens + stretch - 1) / stretch;
+    return std::min<int64_t>((stretches + kLines - 1) / kLines, walkers_of(channels) / kLines);
 }
 uint64_t convolution_workspace(const nuka_b200_episodes_t& plan, int64_t channels, int64_t width) { return (uint64_t)(convolution_across(plan, channels) * (width + 1) * channels) * sizeof(float); }
 
 template <typename T, int K, int VEC> static cudaError_t run_convolution(const nuka_b200_convolution_t& d, bool backward, cudaStream_t stream) {
-    ConvolutionParams p = convolution_params<T, VEC>(d);
+    ConvolutionParams p = convolution_params<T, VEC>(d, backward);
     if (!backward) {
         convolution_kernel<T, K, VEC><<<p.tiles * p.across, kLines * 32, 0, stream>>>(p);
         return cudaGetLastError();

@@ -7,9 +7,9 @@
 // and the sums that become the gradients of the last K inputs travel with them; the walk goes K - 1 tokens past its stretch (as far as the episode does) to complete them.
 // Weights' gradients are summed in registers over all stretches of a thread, then over a block's warps, then over the blocks, always in the same order.
 #include <algorithm>
+#include "nkb_gates.cuh"
 #include "nkb_sequence.cuh"
 #include "nkb_sequence.h"
-#include "nkb_tcgen.cuh"
 
 namespace nkb {
 
@@ -145,9 +145,7 @@ __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(
             unpack<T, VEC>(now[i], window[K - 1]);
             float s[VEC];
             f.sum(window, s);
-            if (p.act)
-#pragma unroll
-                for (int v = 0; v < VEC; ++v) s[v] = silu<sizeof(T) == 4>(s[v]);
+            if (p.act) silu_all<sizeof(T) == 4>(s);
             if (live) store<T, VEC>(y, s);
             y += C;
         };
@@ -234,8 +232,7 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
                 if (p.act) {
                     float s[VEC];
                     f.sum(window, s);
-#pragma unroll
-                    for (int v = 0; v < VEC; ++v) ds[v] *= silu_slope<sizeof(T) == 4>(s[v]);
+                    by_silu_slope<sizeof(T) == 4>(s, ds);
                 }
 #pragma unroll
                 for (int j = 0; j < K - 1; ++j) add_products(grad[j], f.w[j], ds);
@@ -435,9 +432,7 @@ __global__ void convolution_step_kernel(int64_t groups, uint32_t per_env, const 
 #pragma unroll
         for (int j = 0; j < K; ++j) sum[v] = fmaf(d.weight[(c + v) * K + j], window[j][v], sum[v]);
     }
-    if (d.silu)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) sum[v] = silu<sizeof(T) == 4>(sum[v]);
+    if (d.silu) silu_all<sizeof(T) == 4>(sum);
     store<T, VEC>(static_cast<T*>(d.y) + env * d.channels + c, sum);
 #pragma unroll
     for (int j = 0; j < K - 1; ++j) store<T, VEC>(state + j * d.channels, window[j + 1]);

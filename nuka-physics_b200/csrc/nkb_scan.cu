@@ -9,9 +9,9 @@
 // Segments and maps are as in the gated recurrence: rows where they are short or many, else equal shares, walked once for what each does to the state, (exp(A sum dt), h), and a second time for the values.
 // For a gradient the states before each chunk are kept, in the lanes' order; backwards a chunk's states are worked out again from them, into shared memory, and its tokens then walked back.
 #include <algorithm>
+#include "nkb_gates.cuh"
 #include "nkb_sequence.cuh"
 #include "nkb_sequence.h"
-#include "nkb_tcgen.cuh"
 
 namespace nkb {
 
@@ -355,9 +355,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanPara
             x.get(xs);
             delta.get(us);
 #pragma unroll
+            for (int k = 0; k < E; ++k) us[k] += bias[k];
+            softplus_all(us, us);
+#pragma unroll
             for (int k = 0; k < E; ++k) {
-                const float u = us[k] + bias[k];
-                us[k] = softplus(u, fading<true>(u));
                 xs[k] *= us[k];
                 if (MAPS && there > 0) total[k] += us[k];
             }
@@ -425,8 +426,9 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanPara
             if (p.gate != nullptr) {
                 float z[E];
                 gate_now.get(z);
+                silu_all<sizeof(T) == 4>(z);
 #pragma unroll
-                for (int k = 0; k < E; ++k) y[k] *= silu<sizeof(T) == 4>(z[k]);
+                for (int k = 0; k < E; ++k) y[k] *= z[k];
             }
             l.store(p, p.y, t0, left, y);
             __syncwarp();
@@ -526,16 +528,17 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(cons
             delta.get(us);
             dy.get(ds);
 #pragma unroll
-            for (int k = 0; k < E; ++k) {
-                const float u = us[k] + bias[k];
-                us[k] = softplus(u, fading<true>(u));
-                if (there > 0) total[k] += us[k];
-            }
+            for (int k = 0; k < E; ++k) us[k] += bias[k];
+            softplus_all(us, us);
+            if (there > 0)
+#pragma unroll
+                for (int k = 0; k < E; ++k) total[k] += us[k];
             if (p.gate != nullptr) {
                 float z[E];
                 gate.get(z);
+                silu_all<sizeof(T) == 4>(z);
 #pragma unroll
-                for (int k = 0; k < E; ++k) ds[k] *= silu<sizeof(T) == 4>(z[k]);
+                for (int k = 0; k < E; ++k) ds[k] *= z[k];
             }
             put(l.cell(m.dt), us);
             put(l.cell(m.in), ds);
@@ -621,13 +624,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                 delta.get(us);
                 l.of_channels(p.delta_bias, bias);
 #pragma unroll
-                for (int k = 0; k < E; ++k) {
-                    const float u = us[k] + bias[k];
-                    const Fading f = fading<true>(u);
-                    us[k] = softplus(u, f);
-                    bias[k] = logistic(u, f);
-                    xs[k] *= us[k];
-                }
+                for (int k = 0; k < E; ++k) us[k] += bias[k];
+                softplus_all(us, us, bias);
+#pragma unroll
+                for (int k = 0; k < E; ++k) xs[k] *= us[k];
                 put(l.cell(m.dt), us);
                 put(l.cell(m.slope), bias);
                 put(l.cell(m.in), xs);
@@ -636,12 +636,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                     float z[E];
                     gate.get(z);
 #pragma unroll
-                    for (int k = 0; k < E; ++k) {
-                        const Fading f = fading<sizeof(T) == 4>(z[k]);
-                        const float r = logistic(z[k], f);
-                        us[k] = ds[k] * (r * fmaf(z[k], one_less(z[k], f), 1.f));
-                        ds[k] *= z[k] * r;
-                    }
+                    for (int k = 0; k < E; ++k) us[k] = ds[k];
+                    by_silu_slope<sizeof(T) == 4>(z, us, ds);
                     put(l.cell(m.gate), us);
                 }
                 put(l.cell(m.dy), ds);

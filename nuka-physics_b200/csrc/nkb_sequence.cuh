@@ -61,43 +61,4 @@ template <typename T, int N> __device__ __forceinline__ void store(T* p, const f
     *reinterpret_cast<Raw<T, N>*>(p) = raw;
 }
 
-// ---- logistic function and its kin -------------------------------------------------------------------------------------
-// exp(-|u|) and 1 / (1 + it), of which the others are made. The exponent's product with log2(e) is rounded to 2^-24 of itself; EXACT adds what that lost. What is not a number has to come with a factor of its own.
-struct Fading { float e, r; };
-template <bool EXACT> __device__ __forceinline__ Fading fading(float u) {
-    const float a = fminf(fabsf(u), 100.f), t = a * -1.4426950408889634f;
-    Fading f;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(f.e) : "f"(t));
-    if (EXACT) f.e = fmaf(f.e, fmaf(a, -1.4426950408889634f, -t) * 0.6931471805599453f + a * -1.3352e-8f, f.e);       // the last: log2(e)'s own rounding, 1.9263e-8, times ln(2)
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f.r) : "f"(1.f + f.e));
-    return f;
-}
-__device__ __forceinline__ float logistic(float u, Fading f) { return u >= 0.f ? f.r : f.e * f.r; }
-__device__ __forceinline__ float one_less(float u, Fading f) { return u >= 0.f ? f.e * f.r : f.r; }             // 1 - logistic(u)
-// Where 16 bits are the result: 1 / (1 + exp(-s)) at once, the exponential kept finite.
-__device__ __forceinline__ float logistic_fast(float s) {
-    float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(s * -1.4426950408889634f, 126.f)));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
-    return r;
-}
-template <bool EXACT> __device__ __forceinline__ float silu(float s) { return s * (EXACT ? logistic(s, fading<true>(s)) : logistic_fast(s)); }
-template <bool EXACT> __device__ __forceinline__ float silu_slope(float s) {
-    if (!EXACT) {
-        const float r = logistic_fast(s);
-        return r * fmaf(s, 1.f - r, 1.f);
-    }
-    const Fading f = fading<true>(s);
-    return logistic(s, f) * fmaf(s, one_less(s, f), 1.f);
-}
-// log(1 + exp(u)) = max(u, 0) + log(1 + e), the latter by the series of 2 artanh(e / (2 + e)): its argument is 1/3 at most, the first term left out 2^-26 of the sum.
-__device__ __forceinline__ float softplus(float u, Fading f) {
-    float most, q;
-    asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(most) : "f"(u));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(q) : "f"(2.f + f.e));
-    const float z = f.e * q, s = z * z;
-    const float series = fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, 1.f / 13.f, 1.f / 11.f), 1.f / 9.f), 1.f / 7.f), 1.f / 5.f), 1.f / 3.f), 1.f);
-    return fmaf(z + z, series, most);
-}
-
 }  // namespace nkb

@@ -160,9 +160,49 @@ struct Order {
     __device__ __forceinline__ void two_pairs(const float* from, Pair (&v)[2]) const {
         v[0] = *reinterpret_cast<const Pair*>(from + upper_j); v[1] = *reinterpret_cast<const Pair*>(from + 2 - upper_j);
     }
-    __device__ __forceinline__ void four_pairs(const float2* from, Pair (&v)[4]) const {
-        const ulonglong2 r = *reinterpret_cast<const ulonglong2*>(from + upper_i), q = *reinterpret_cast<const ulonglong2*>(from + 2 - upper_i);
-        v[0] = r.x; v[1] = r.y; v[2] = q.x; v[3] = q.y;
+};
+// B and C of a chunk as they come, four states of each one behind the other, once in each of the two orders of a lane's states.
+template <typename T, int LN> struct __align__(16) NarrowShared {
+    T of[2][ScanTile<LN>::kChunk][LN][8];
+    // what a lane has of B (which 0) or C (1), from state `first` of token `t` on
+    template <int N> __device__ __forceinline__ void put(int which, int t, int first, const T (&v)[N]) {
+        if constexpr (N % 4 == 0) {
+#pragma unroll
+            for (int k = 0; k < N; k += 4) {
+                T turned[4] = {v[k + 2], v[k + 3], v[k], v[k + 1]}, same[4] = {v[k], v[k + 1], v[k + 2], v[k + 3]};
+                *reinterpret_cast<Raw<T, 4>*>(&of[0][t][first / 4 + k / 4][4 * which]) = *reinterpret_cast<const Raw<T, 4>*>(same);
+                *reinterpret_cast<Raw<T, 4>*>(&of[1][t][first / 4 + k / 4][4 * which]) = *reinterpret_cast<const Raw<T, 4>*>(turned);
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const int n = first + k;
+                of[0][t][n / 4][4 * which + n % 4] = v[k];
+                of[1][t][n / 4][4 * which + (n % 4 ^ 2)] = v[k];
+            }
+        }
+    }
+    // each twice, as it meets two channels
+    __device__ __forceinline__ void get(int upper, int t, int nl, Pair (&b)[4], Pair (&c)[4]) const {
+        float f[8];
+        if constexpr (sizeof(T) == 2) {
+            unpack<T, 8>(load_raw<T, 8>(of[upper][t][nl]), f);
+        } else {
+            take4(of[upper][t][nl], f);
+            take4(of[upper][t][nl] + 4, f + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { b[i] = both(f[i]); c[i] = both(f[4 + i]); }
+    }
+    __device__ __forceinline__ void get(int which, int upper, int t, int nl, Pair (&v)[4]) const {
+        float f[4];
+        unpack<T, 4>(load_raw<T, 4>(of[upper][t][nl] + 4 * which), f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = both(f[i]);
+    }
+    static __device__ __forceinline__ void take4(const float* from, float* v) {
+        const float4 q = *reinterpret_cast<const float4*>(from);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
     }
 };
 
@@ -256,18 +296,11 @@ template <typename T, int LN> struct ScanLane {
         for (int k = 0; k < S::kEach; ++k) v[k] = from != nullptr && k < own ? from[c0 + channel + k] : 0.f;
     }
     __device__ __forceinline__ float* cell(float* of) const { return of + token * S::kRow + channel; }
-    // each value of B or C twice, as it meets two channels
-    __device__ __forceinline__ void put_narrow(float2* to, const Narrow& v) const {
-        float f[S::kNarrow];
-        v.get(f);
-        float2* const at = to + narrow_token * S::kStates + narrow_state;
-        if constexpr (S::kNarrow % 2 == 0) {
+    __device__ __forceinline__ void put_narrow(NarrowShared<T, LN>& to, int which, const Narrow& v) const {
+        T f[S::kNarrow];
 #pragma unroll
-            for (int k = 0; k < S::kNarrow; k += 2) *reinterpret_cast<float4*>(at + k) = make_float4(f[k], f[k], f[k + 1], f[k + 1]);
-        } else {
-#pragma unroll
-            for (int k = 0; k < S::kNarrow; ++k) at[k] = make_float2(f[k], f[k]);
-        }
+        for (int k = 0; k < S::kNarrow; ++k) f[k] = reinterpret_cast<const T*>(&v.raw)[k];
+        to.put(which, narrow_token, narrow_state, f);
     }
 };
 template <int N> __device__ __forceinline__ void put(float* to, const float (&v)[N]) {
@@ -290,14 +323,14 @@ template <int N> __device__ __forceinline__ void take(const float* from, float (
 }
 
 // What a warp's states read of a chunk, and what they give.
-template <int LN> struct __align__(16) ScanShared {
+template <typename T, int LN> struct __align__(16) ScanShared {
     using S = ScanTile<LN>;
     float dt[S::kCells], in[S::kCells], out[S::kCells];
-    float2 b[S::kChunk * S::kStates], c[S::kChunk * S::kStates];
+    NarrowShared<T, LN> narrow;
 };
 
 // A segment's sums of dt: of each channel those of the lanes that have it.
-template <int LN> __device__ __forceinline__ void give_totals(const ScanParams& p, ScanShared<LN>& m, float* cell, const float (&total)[ScanTile<LN>::kEach], int lane, int64_t map, bool closed) {
+template <typename T, int LN> __device__ __forceinline__ void give_totals(const ScanParams& p, ScanShared<T, LN>& m, float* cell, const float (&total)[ScanTile<LN>::kEach], int lane, int64_t map, bool closed) {
     using S = ScanTile<LN>;
     __syncwarp();
     put(cell, total);
@@ -315,8 +348,8 @@ template <typename T, int LN, bool MAPS>
 __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanParams p) {
     using S = ScanTile<LN>;
     constexpr int E = S::kEach;
-    __shared__ ScanShared<LN> all[kScanWarps];
-    ScanShared<LN>& m = all[threadIdx.x / 32];
+    __shared__ ScanShared<T, LN> all[kScanWarps];
+    ScanShared<T, LN>& m = all[threadIdx.x / 32];
     const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, segment = job / p.tiles, tile = job % p.tiles;
     if (segment >= p.segments) return;
     const ScanLane<T, LN> l(p, tile);
@@ -365,8 +398,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanPara
             put(l.cell(m.dt), us);
             put(l.cell(m.in), xs);
         }
-        l.put_narrow(m.b, b);
-        if (!MAPS) l.put_narrow(m.c, c);
+        l.put_narrow(m.narrow, 0, b);
+        if (!MAPS) l.put_narrow(m.narrow, 1, c);
         __syncwarp();
         fetch(t0 + S::kChunk);
         if (!MAPS && p.kept != nullptr) h.store(p.kept + (chunk * p.tiles + tile) * 128 + l.lane);
@@ -379,14 +412,13 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanPara
             Pair dt[2], in[2], bs[4];
             l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
             l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, in);
-            l.order.four_pairs(m.b + t * S::kStates + 4 * l.nl, bs);
+            Pair cs[4];
+            if constexpr (MAPS) m.narrow.get(0, l.order.upper_i / 2, t, l.nl, bs); else m.narrow.get(l.order.upper_i / 2, t, l.nl, bs, cs);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) h.h[j][i] = fma_pair(exp2_pair(mul_pair(dt[j], l.rate.h[j][i])), h.h[j][i], mul_pair(in[j], bs[i]));
             if constexpr (!MAPS) {
-                Pair cs[4];
-                l.order.four_pairs(m.c + t * S::kStates + 4 * l.nl, cs);
                 Pair sum[2];
                 float y[2];
 #pragma unroll
@@ -436,7 +468,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_kernel(const ScanPara
     }
     if constexpr (MAPS) {
         h.store(maps);
-        give_totals<LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
+        give_totals<T, LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
     }
 }
 
@@ -479,12 +511,12 @@ template <int LN, bool BACKWARD> __global__ void __launch_bounds__(1024) scan_ca
 }
 
 // ---- backwards -----------------------------------------------------------------------------------------------------------
-template <int LN> struct __align__(16) ScanGradShared {
+template <typename T, int LN> struct __align__(16) ScanGradShared {
     using S = ScanTile<LN>;
     float4 before[S::kChunk * 4 * 32];                  // the states before each token, in the lanes' order
     float dt[S::kCells], dy[S::kCells], slope[S::kCells], gate[S::kCells], out[S::kCells], by_a[S::kCells];         // slope: of dt; gate: what y's gradient of the gate is multiplied with
     float in[S::kCells];                                // dt x, and when the token is done sum of m B
-    float2 b[S::kChunk * S::kStates], c[S::kChunk * S::kStates];
+    NarrowShared<T, LN> narrow;
 };
 
 // What goes back through a segment from 0: m_t = C dy + a_{t+1} m_{t+1}, times a_t of its first token
@@ -492,8 +524,8 @@ template <typename T, int LN>
 __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(const ScanParams p) {
     using S = ScanTile<LN>;
     constexpr int E = S::kEach;
-    __shared__ ScanShared<LN> all[kScanWarps];
-    ScanShared<LN>& m = all[threadIdx.x / 32];
+    __shared__ ScanShared<T, LN> all[kScanWarps];
+    ScanShared<T, LN>& m = all[threadIdx.x / 32];
     const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, segment = job / p.tiles, tile = job % p.tiles;
     if (segment >= p.segments) return;
     const ScanLane<T, LN> l(p, tile);
@@ -543,7 +575,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(cons
             put(l.cell(m.dt), us);
             put(l.cell(m.in), ds);
         }
-        l.put_narrow(m.c, c);
+        l.put_narrow(m.narrow, 1, c);
         __syncwarp();
         fetch(k0 - 1);
         auto end_at = [&](int t) {
@@ -560,7 +592,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(cons
             Pair dt[2], d[2], cs[4];
             l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
             l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, d);
-            l.order.four_pairs(m.c + t * S::kStates + 4 * l.nl, cs);
+            m.narrow.get(1, l.order.upper_i / 2, t, l.nl, cs);
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -582,7 +614,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(cons
         __syncwarp();
     }
     back.store(reinterpret_cast<float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane);
-    give_totals<LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
+    give_totals<T, LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
 }
 
 template <typename T, int LN>
@@ -590,7 +622,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
     using S = ScanTile<LN>;
     constexpr int E = S::kEach;
     extern __shared__ __align__(16) unsigned char raw[];
-    ScanGradShared<LN>& m = reinterpret_cast<ScanGradShared<LN>*>(raw)[threadIdx.x / 32];
+    ScanGradShared<T, LN>& m = reinterpret_cast<ScanGradShared<T, LN>*>(raw)[threadIdx.x / 32];
     const int64_t job = (int64_t)blockIdx.x * kScanWarps + threadIdx.x / 32, worker = job / p.tiles, tile = job % p.tiles;
     if (worker >= p.workers) return;
     const ScanLane<T, LN> l(p, tile);
@@ -642,8 +674,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                 }
                 put(l.cell(m.dy), ds);
             }
-            l.put_narrow(m.b, b);
-            l.put_narrow(m.c, c);
+            l.put_narrow(m.narrow, 0, b);
+            l.put_narrow(m.narrow, 1, c);
             __syncwarp();
             auto begin_at = [&](int t) {
                 const int32_t row = __shfl_sync(~0u, links, t);
@@ -654,7 +686,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                 Pair dt[2], in[2], bs[4];
                 l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
                 l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, in);
-                l.order.four_pairs(m.b + t * S::kStates + 4 * l.nl, bs);
+                m.narrow.get(0, l.order.upper_i / 2, t, l.nl, bs);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -685,8 +717,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                 l.order.two_pairs(m.dt + t * S::kRow + 4 * l.cl, dt);
                 l.order.two_pairs(m.in + t * S::kRow + 4 * l.cl, in);
                 l.order.two_pairs(m.dy + t * S::kRow + 4 * l.cl, d);
-                l.order.four_pairs(m.b + t * S::kStates + 4 * l.nl, bs);
-                l.order.four_pairs(m.c + t * S::kStates + 4 * l.nl, cs);
+                m.narrow.get(l.order.upper_i / 2, t, l.nl, bs, cs);
                 States before;
                 before.load(m.before + t * 128 + l.lane);
                 Pair y[2], by_b[2], by_a[2], to_b[4], to_c[4];
@@ -915,7 +946,7 @@ template <typename T, int LN> static cudaError_t run_scan(const nuka_b200_scan_t
     }
     const int64_t narrow = s.tiles * p.plan.tokens * s.states;
     p.db = work; p.dc_after = narrow; p.ddecay = work + 2 * narrow; p.dskip = p.ddecay + s.workers * s.tiles * 512; p.dbias = p.dskip + s.workers * s.tiles * s.channels;
-    constexpr int SHARED = sizeof(ScanGradShared<LN>) * kScanWarps;
+    constexpr int SHARED = sizeof(ScanGradShared<T, LN>) * kScanWarps;
     const cudaError_t set = cudaFuncSetAttribute(scan_grad_kernel<T, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED);
     if (set != cudaSuccess) return set;
     if (!s.alone) {

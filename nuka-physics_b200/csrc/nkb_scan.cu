@@ -516,6 +516,7 @@ template <typename T, int LN> struct __align__(16) ScanGradShared {
     float4 before[S::kChunk * 4 * 32];                  // the states before each token, in the lanes' order
     float dt[S::kCells], dy[S::kCells], slope[S::kCells], gate[S::kCells], out[S::kCells], by_a[S::kCells];         // slope: of dt; gate: what y's gradient of the gate is multiplied with
     float in[S::kCells];                                // dt x, and when the token is done sum of m B
+    float bias[S::kChannels], skip[S::kChannels];       // of the tile's channels
     NarrowShared<T, LN> narrow;
 };
 
@@ -629,32 +630,45 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
     States ddecay;
     ddecay.clear();
     float dskip[E] = {}, dbias[E] = {};
+    for (int ch = l.lane; ch < S::kChannels; ch += 32) {
+        m.bias[ch] = p.delta_bias != nullptr && ch < l.count ? p.delta_bias[l.c0 + ch] : 0.f;
+        m.skip[ch] = p.skip != nullptr && ch < l.count ? p.skip[l.c0 + ch] : 0.f;
+    }
+    __syncwarp();
+    // a chunk's inputs and the states before it: asked for while the last one's outputs are worked out
+    typename ScanLane<T, LN>::Each x, delta, gate, dy;
+    typename ScanLane<T, LN>::Narrow b, c;
+    int32_t links, tails;
+    States h, back;                                     // back: a_{t+1} m_{t+1}
+    auto end_of = [&](int64_t segment) { return min((segment + 1) * p.segment, p.plan.tokens); };
+    auto last_of = [&](int64_t segment) { return (end_of(segment) - segment * p.segment + S::kChunk - 1) / S::kChunk - 1; };
+    auto fetch = [&](int64_t segment, int64_t k) {
+        const int64_t t0 = segment * p.segment + k * S::kChunk;
+        const int left = (int)min((int64_t)S::kChunk, end_of(segment) - t0);
+        l.load(p, p.x, p.x_stride, t0, left, x);
+        l.load(p, p.delta, p.delta_stride, t0, left, delta);
+        l.load(p, p.dy, p.channels, t0, left, dy);
+        if (p.gate != nullptr) l.load(p, p.gate, p.gate_stride, t0, left, gate);
+        l.load_narrow(p, p.b, p.b_stride, t0, left, b);
+        l.load_narrow(p, p.c, p.c_stride, t0, left, c);
+        links = l.lane < left ? p.plan.link[t0 + l.lane] : -1;
+        tails = l.lane < left ? p.plan.tail[t0 + l.lane] : -1;
+        h.load(p.kept + ((segment * p.chunks + k) * p.tiles + tile) * 128 + l.lane);
+    };
+    fetch(worker, last_of(worker));                     // workers are no more than segments
     for (int64_t segment = worker; segment < p.segments; segment += p.workers) {
-        const int64_t begin = segment * p.segment, end = min(begin + p.segment, p.plan.tokens), chunks = (end - begin + S::kChunk - 1) / S::kChunk;
-        States back;                                    // a_{t+1} m_{t+1}
+        const int64_t begin = segment * p.segment, end = end_of(segment);
         back.clear();
         if (!p.alone) back.load(reinterpret_cast<const float4*>(p.maps) + (segment * p.tiles + tile) * 128 + l.lane);
-        for (int64_t k0 = chunks - 1; k0 >= 0; --k0) {
-            const int64_t t0 = begin + k0 * S::kChunk, chunk = segment * p.chunks + k0;
+        for (int64_t k0 = last_of(segment); k0 >= 0; --k0) {
+            const int64_t t0 = begin + k0 * S::kChunk;
             const int left = (int)min((int64_t)S::kChunk, end - t0), there = l.token < left ? l.own : 0;
-            typename ScanLane<T, LN>::Each x, delta, gate, dy;
-            typename ScanLane<T, LN>::Narrow b, c;
-            l.load(p, p.x, p.x_stride, t0, left, x);
-            l.load(p, p.delta, p.delta_stride, t0, left, delta);
-            l.load(p, p.dy, p.channels, t0, left, dy);
-            if (p.gate != nullptr) l.load(p, p.gate, p.gate_stride, t0, left, gate);
-            l.load_narrow(p, p.b, p.b_stride, t0, left, b);
-            l.load_narrow(p, p.c, p.c_stride, t0, left, c);
-            const int32_t links = l.lane < left ? p.plan.link[t0 + l.lane] : -1, tails = l.lane < left ? p.plan.tail[t0 + l.lane] : -1;
             const uint32_t begins = __ballot_sync(~0u, links != -1), ends = __ballot_sync(~0u, tails >= 0);
-            const float4* const kept = p.kept + (chunk * p.tiles + tile) * 128 + l.lane;
-            States h;
-            h.load(kept);
             {
                 float xs[E], us[E], ds[E], bias[E];
                 x.get(xs);
                 delta.get(us);
-                l.of_channels(p.delta_bias, bias);
+                take(m.bias + l.channel, bias);
 #pragma unroll
                 for (int k = 0; k < E; ++k) us[k] += bias[k];
                 softplus_all(us, us, bias);
@@ -791,6 +805,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
             {
                 float xs[E], us[E], ds[E], dt[E], by_b[E], out[E], skip[E];
                 x.get(xs);
+                if (k0 > 0) fetch(segment, k0 - 1);
+                else if (const int64_t next = segment + p.workers; next < p.segments) fetch(next, last_of(next));
                 take(l.cell(m.in), by_b);
                 take(l.cell(m.by_a), us);
                 take(l.cell(m.slope), out);
@@ -802,7 +818,7 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                 l.store(p, p.ddelta, t0, left, us);
                 take(l.cell(m.dy), ds);
                 take(l.cell(m.dt), dt);
-                l.of_channels(p.skip, skip);
+                take(m.skip + l.channel, skip);
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     dskip[k] = fmaf(ds[k], xs[k], dskip[k]);       // 0 where there is no token

@@ -12,6 +12,7 @@
 //
 // Measured, bf16, 8 heads, 2 of keys, dim 64: 4096 envs of 256 tokens 86 us, 4.8 TB/s of cached keys and values (0.73 of what a copy reaches): a warp's loads under way are as many as its registers
 // hold, and 13 warps an SM (20 %) leave the memory idle between them.  One env of 8192 tokens 9.5 us, of which its 4 MB are 1: it is bound by the chain of launch, loads and join.
+// The first tokens of an episode may have places of their own before the ring: which place a token takes is all that changes, the order of keys being free.
 #include <cuda_runtime.h>
 #include <algorithm>
 #include "nkb_sequence.cuh"

@@ -32,13 +32,13 @@ def _expect(ok, text):
 
 def _on_gpu(first, *others):
     """The GPU that all of the tensors are on (None is left out)."""
-    device = first.device
-    if device.type != "cuda":
+    index = first.get_device()
+    if not first.is_cuda:
         raise ValueError("tensors must be on the GPU")
     for tensor in others:
-        if tensor is not None and tensor.device != device:
+        if tensor is not None and tensor.get_device() != index:
             raise ValueError("tensors must be on one GPU")
-    return device
+    return first.device
 
 
 def _dtype(tensor, allowed, what):
@@ -48,11 +48,17 @@ def _dtype(tensor, allowed, what):
     return _DTYPES[tensor.dtype]
 
 
+# what torch.cuda.current_stream(index).cuda_stream and torch.cuda.current_device() give, without the objects on the way
+_raw_stream, _current_device = getattr(torch._C, "_cuda_getCurrentRawStream", None), getattr(torch._C, "_cuda_getDevice", None)
+if _raw_stream is None or _current_device is None:
+    _raw_stream, _current_device = (lambda index: torch.cuda.current_stream(index).cuda_stream), torch.cuda.current_device
+
+
 def _call(device, function, *args):
     """One call of the library on torch's current stream of `device`, which it returns."""
     index = device.index
-    stream = torch.cuda.current_stream(index).cuda_stream
-    if torch.cuda.current_device() != index:
+    stream = _raw_stream(index)
+    if _current_device() != index:
         with torch.cuda.device(device):
             code = function(*args, stream)
     else:

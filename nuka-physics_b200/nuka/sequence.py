@@ -332,7 +332,7 @@ class _Convolution(torch.autograd.Function):
 
 
 def _convolution_weights(weight, bias, channels):
-    if weight.dim() != 2 or weight.shape[0] != channels or not 2 <= weight.shape[1] <= 4 or weight.dtype != torch.float32:
+    if weight.dim() != 2 or weight.dtype is not torch.float32 or weight.shape[0] != channels or not 2 <= weight.shape[1] <= 4:
         raise ValueError(f"weight must be float32, {channels} channels x 2, 3 or 4 taps")
     if bias is not None and (bias.shape != (channels,) or bias.dtype != torch.float32):
         raise ValueError(f"bias must be float32, {channels} channels")
@@ -444,20 +444,28 @@ class _Scan(torch.autograd.Function):
         return (None, *(grads.get(name) for name in _SCAN_INPUTS))
 
 
-def _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias):
-    """Checks what the scan and its step have in common; the inputs as the kernels take them."""
+def _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias, strides=None):
+    """Checks what the scan and its step have in common; the inputs as the kernels take them. `strides`: those of x, delta, b and c where the caller has them, made those of what is returned."""
     dtype, shape = x.dtype, x.shape
-    _dtype(x, _DTYPES, "x")
-    if len(shape) != 2 or decay.dim() != 2 or decay.shape[0] != shape[1] or not 1 <= decay.shape[1] <= 64 or decay.dtype != torch.float32:
+    if dtype not in _DTYPES:
+        _dtype(x, _DTYPES, "x")
+    if len(shape) != 2 or decay.dim() != 2 or decay.dtype != torch.float32:
         raise ValueError("x must have 2 dimensions, the second of channels, and decay must be float32, channels x 1 to 64 states")
-    narrow = (shape[0], decay.shape[1])
-    if not (delta.shape == shape and delta.dtype == dtype and b.shape == narrow and b.dtype == dtype and c.shape == narrow and c.dtype == dtype and (gate is None or (gate.shape == shape and gate.dtype == dtype))):
-        raise ValueError(f"delta and gate must be like x, b and c {' x '.join(map(str, narrow))}, of x's type")
+    (count, channels), (rows, states) = shape, decay.shape
+    if rows != channels or not 1 <= states <= 64:
+        raise ValueError("x must have 2 dimensions, the second of channels, and decay must be float32, channels x 1 to 64 states")
+    narrow = (count, states)
+    if not (delta.shape == shape and delta.dtype is dtype and b.shape == narrow and b.dtype is dtype and c.shape == narrow and c.dtype is dtype and (gate is None or (gate.shape == shape and gate.dtype is dtype))):
+        raise ValueError(f"delta and gate must be like x, b and c {count} x {states}, of x's type")
     for v in (skip, delta_bias):
-        if v is not None and (v.shape != shape[1:] or v.dtype != torch.float32):
+        if v is not None and (v.dtype is not torch.float32 or v.shape != (channels,)):
             raise ValueError("skip and delta_bias must be float32, one per channel")
-    return (_rows(x), _rows(delta), decay.contiguous(), _rows(b), _rows(c), None if skip is None else skip.contiguous(), None if gate is None else _rows(gate),
-            None if delta_bias is None else delta_bias.contiguous())
+    # kept as they are where their last dimension is contiguous
+    if strides is None or not strides[0][-1] == strides[1][-1] == strides[2][-1] == strides[3][-1] == 1:
+        x, delta, b, c = _rows(x), _rows(delta), _rows(b), _rows(c)
+        if strides is not None:
+            strides[:] = x.stride(), delta.stride(), b.stride(), c.stride()
+    return (x, delta, decay.contiguous(), b, c, None if skip is None else skip.contiguous(), None if gate is None else _rows(gate), None if delta_bias is None else delta_bias.contiguous())
 
 
 def selective_scan(x, delta, decay, b, c, episodes, initial=None, skip=None, gate=None, delta_bias=None):
@@ -482,16 +490,17 @@ def selective_scan_step(x, delta, decay, b, c, state, fresh=None, skip=None, gat
     """The scan for one token of each env.  x, delta, gate: envs x channels; b, c: envs x states; state: envs x channels x states float32, contiguous, updated in place; fresh: envs, bool or
     uint8, set where the token begins an episode (the state before it counts as 0).  Returns y like x.  No gradient."""
     device = _on_gpu(x, delta, decay, b, c, state, fresh, skip, gate, delta_bias)
-    x, delta, decay, b, c, skip, gate, delta_bias = _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias)
+    strides = [x.stride(), delta.stride(), b.stride(), c.stride()]
+    x, delta, decay, b, c, skip, gate, delta_bias = _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias, strides)
     (envs, channels), states = x.shape, decay.shape[1]
     if state.shape != (envs, channels, states) or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"state must be contiguous float32, {envs} x {channels} x {states}")
     if fresh is not None:
         fresh = _flags(fresh, x.shape[:1], device, "fresh")
     y = torch.empty((envs, channels), dtype=x.dtype, device=device)
-    strides = (x.stride(0), delta.stride(0), 0 if gate is None else gate.stride(0), b.stride(0), c.stride(0)) if envs > 1 else (0, 0, 0, 0, 0)
-    desc = _abi.ScanStepDesc(_DTYPES[x.dtype], envs, channels, states, x.data_ptr(), delta.data_ptr(), None if gate is None else gate.data_ptr(), b.data_ptr(), c.data_ptr(), *strides,
-                             decay.data_ptr(), _ptr(skip), _ptr(delta_bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
+    by = (strides[0][0], strides[1][0], 0 if gate is None else gate.stride(0), strides[2][0], strides[3][0]) if envs > 1 else (0, 0, 0, 0, 0)
+    desc = _abi.ScanStepDesc(_DTYPES[x.dtype], envs, channels, states, x.data_ptr(), delta.data_ptr(), None if gate is None else gate.data_ptr(), b.data_ptr(), c.data_ptr(), *by, decay.data_ptr(),
+                             None if skip is None else skip.data_ptr(), None if delta_bias is None else delta_bias.data_ptr(), None if fresh is None else fresh.data_ptr(), state.data_ptr(), y.data_ptr())
     _call(device, _abi.lib().nuka_b200_scan_step, ctypes.byref(desc))
     return y
 

@@ -36,11 +36,6 @@ __device__ __forceinline__ float softplus(float u, Fading f) {
 
 // ---- several values, two to an instruction ---------------------------------------------------------------------------------
 __device__ __forceinline__ Pair both(float v) { return pair_of(v, v); }
-__device__ __forceinline__ float exp2_of(float x) {
-    float e;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(x));
-    return e;
-}
 __device__ __forceinline__ float inverse_of(float x) {
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -50,7 +45,7 @@ __device__ __forceinline__ float inverse_of(float x) {
 __device__ __forceinline__ Pair logistic_pair(Pair s) {
     float a, b, x, y;
     split(mul_pair(s, both(-1.4426950408889634f)), a, b);
-    split(add_pair(pair_of(exp2_of(fminf(a, 126.f)), exp2_of(fminf(b, 126.f))), both(1.f)), x, y);
+    split(add_pair(pair_of(exp2_fast(fminf(a, 126.f)), exp2_fast(fminf(b, 126.f))), both(1.f)), x, y);
     return pair_of(inverse_of(x), inverse_of(y));
 }
 // s = silu(s)
@@ -94,7 +89,7 @@ template <int N> __device__ __forceinline__ void softplus_all(const float (&u)[N
             // fading<true>, its sign turned round
             const Pair a = pair_of(fminf(fabsf(u[k]), 100.f), fminf(fabsf(u[k + 1]), 100.f)), t = mul_pair(a, both(1.4426950408889634f));
             split(t, x, y);
-            Pair e = pair_of(exp2_of(-x), exp2_of(-y));
+            Pair e = pair_of(exp2_fast(-x), exp2_fast(-y));
             e = fma_pair(e, fma_pair(fma_pair(a, both(-1.4426950408889634f), t), both(0.6931471805599453f), mul_pair(a, both(-1.3352e-8f))), e);
             if (slope != nullptr) {
                 split(add_pair(e, both(1.f)), x, y);

@@ -480,3 +480,42 @@ def test_offsets_that_lie_stay_inside_the_tensors():
         y, state = S.short_convolution(x, _normal(_gen(16), 8, 4), None, plan, _normal(_gen(17), 3, 3, 8), silu=True)
         torch.autograd.grad(y.sum(), x)
     torch.cuda.synchronize()
+
+
+def test_more_values_than_32_bits_count():
+    """Tensors of more than 2^31 values: the last rows of a batch, and their gradients, are what they are in a batch of their own, bit for bit (rows of one short length are worked out alike)."""
+    rows, length, channels, states, few = 34000, 32, 2048, 4, 3
+    assert rows * length * channels > 2 ** 31
+    gen, dtype = _gen(20), torch.bfloat16
+    cut = slice((rows - few) * length, None)
+
+    def make(n):
+        return torch.empty(rows * length, n, dtype=dtype, device="cuda")
+
+    x, delta = make(channels), make(channels)
+    b, c = (_normal(gen, rows * length, states, dtype=dtype) for _ in range(2))
+    decay, taps = -torch.rand((channels, states), generator=gen, device="cuda"), _normal(gen, channels, 4)
+    x.zero_(), delta.zero_()
+    x[cut], delta[cut] = _normal(gen, few * length, channels, dtype=dtype), _normal(gen, few * length, channels, dtype=dtype)
+    done = torch.rand((rows, length), generator=gen, device="cuda") < 0.05
+    whole, part = S.Episodes.from_done(done), S.Episodes.from_done(done[-few:].contiguous())
+
+    def run(plan, x, delta, b, c, at):
+        x, delta, b, c = (v.detach().requires_grad_() for v in (x, delta, b, c))
+        y, state = S.selective_scan(x, delta, decay, b, c, plan)
+        dy = torch.zeros_like(y)
+        dy[at] = 1.0
+        out = [y[at], state[-few:], *(g[at] for g in torch.autograd.grad(y, [x, delta, b, c], dy))]
+        out = [v.detach().clone() for v in out]
+        del y, dy
+        y, state = S.short_convolution(x, taps, None, plan, silu=True)
+        dy = torch.zeros_like(y)
+        dy[at] = 1.0
+        return out + [y[at].detach().clone(), state[-few:].detach(), torch.autograd.grad(y, x, dy)[0][at].clone()]
+
+    want = run(part, x[cut].clone(), delta[cut].clone(), b[cut].clone(), c[cut].clone(), slice(None))
+    got = run(whole, x, delta, b, c, cut)
+    del x, delta
+    torch.cuda.empty_cache()
+    for n, (a, w) in enumerate(zip(got, want)):
+        assert torch.isfinite(a).all() and a.abs().sum() > 0 and torch.equal(a, w), n

@@ -50,17 +50,16 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     return r;
 }
 
-// WARPS: of a job, 1 or all of the block's
+// WARPS: of a job and of a block. A warp with a job to itself is a block to itself, too: its place is then free when its own env's history ends, not the longest of four.
 template <typename T, int DP, int WARPS>
-__global__ void __launch_bounds__(kHistoryWarps * 32, DP == 64 ? 4 : 3) history_kernel(const HistoryParams p) {
+__global__ void __launch_bounds__(WARPS * 32, (DP == 64 ? 4 : 3) * kHistoryWarps / WARPS) history_kernel(const HistoryParams p) {
     constexpr int SETS = DP == 64 ? 2 : 1, KEYS = 16 * SETS, CHUNKS = DP / 32, HALVES = DP / 64, ROW = DP + 2;
     __shared__ __align__(16) float sums[WARPS == 1 ? 1 : WARPS][kQueries][DP];
     __shared__ float tops[WARPS][kQueries], totals[WARPS][kQueries], weights[WARPS == 1 ? 1 : kSplits][kQueries];
     __shared__ uint32_t order;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3, rank = WARPS == 1 ? 0 : warp;
     const int split = WARPS == 1 ? 0 : blockIdx.x % p.splits;
-    const int64_t job = WARPS == 1 ? (int64_t)blockIdx.x * kHistoryWarps + warp : blockIdx.x / p.splits;
-    if (job >= p.jobs) return;                          // a whole warp, and only where warps do not meet
+    const int64_t job = WARPS == 1 ? blockIdx.x : blockIdx.x / p.splits;
     const int part = (int)(job % p.parts), head = (int)(job / p.parts % p.heads_k);
     const int64_t env = job / p.parts / p.heads_k;
     const int group = p.heads_q / p.heads_k, queries = min(kQueries, group - part * kQueries), first = head * group + part * kQueries;
@@ -274,7 +273,7 @@ uint64_t history_workspace(const nuka_b200_history_t& d) {
 }
 
 template <typename T, int DP> static void run_history(const HistoryParams& p, bool by_warps, cudaStream_t stream) {
-    if (by_warps) history_kernel<T, DP, 1><<<(unsigned)((p.jobs + kHistoryWarps - 1) / kHistoryWarps), kHistoryWarps * 32, 0, stream>>>(p);
+    if (by_warps) history_kernel<T, DP, 1><<<(unsigned)p.jobs, 32, 0, stream>>>(p);
     else history_kernel<T, DP, kHistoryWarps><<<(unsigned)(p.jobs * p.splits), kHistoryWarps * 32, 0, stream>>>(p);
 }
 

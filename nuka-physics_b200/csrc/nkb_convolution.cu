@@ -7,9 +7,9 @@
 // and the sums that become the gradients of the last K inputs travel with them; the walk goes K - 1 tokens past its stretch (as far as the episode does) to complete them.
 // Weights' gradients are summed in registers over all stretches of a thread, then over a block's warps, then over the blocks, always in the same order.
 //
-// Measured, K = 4 with silu: 4096 rows of 24 x 512, bf16, 55 us forwards (3.7 TB/s of its 2 tensors) and 105 back (2.9 TB/s of 3); 3 long rows, 131071 x 1024, f16, 131 us (4.1 TB/s) and 245 (3.3 TB/s).
+// Measured, K = 4 with silu: 4096 rows of 24 x 512, bf16, 55 us forwards (3.7 TB/s of its 2 tensors) and 103 back (2.9 TB/s of 3); 3 long rows, 131071 x 1024, f16, 131 us (4.1 TB/s) and 242 (3.3 TB/s).
 // Memory is half busy; the instructions, 2.0 of 4 a cycle (exponentials' unit 47 % forwards, multiplications' 40 % back), and the few loads that registers leave room for share the rest. Eight channels to a thread were
-// slower both ways (fewer warps), two slower back.
+// slower both ways (fewer warps), two slower back; so was a batch asked for before the one in hand is walked (115 back: registers run out, and with them free, 3 blocks to an SM, 123).
 #include <algorithm>
 #include "nkb_gates.cuh"
 #include "nkb_sequence.cuh"
@@ -217,11 +217,20 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
         for (int t0 = 0; t0 < past && last == past; t0 += BATCH) {
             const int left = min(BATCH, past - t0);
             Raw<T, VEC> xs[BATCH], dys[BATCH];
+            const T *const xb = x + t0 * p.x_stride, *const dyb = dy + t0 * C;
+            if (left == BATCH) {                        // no clamp between the loads of a full batch: 3% of this kernel
 #pragma unroll
-            for (int i = 0; i < BATCH; ++i) {
-                const int t = min(t0 + i, past - 1);
-                xs[i] = load_raw<T, VEC>(x + t * p.x_stride);
-                dys[i] = load_raw<T, VEC>(dy + t * C);
+                for (int i = 0; i < BATCH; ++i) {
+                    xs[i] = load_raw<T, VEC>(xb + i * p.x_stride);
+                    dys[i] = load_raw<T, VEC>(dyb + i * C);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < BATCH; ++i) {
+                    const int t = min(i, left - 1);
+                    xs[i] = load_raw<T, VEC>(xb + t * p.x_stride);
+                    dys[i] = load_raw<T, VEC>(dyb + t * C);
+                }
             }
             const Marks marks(p, begin + t0, left);
             // one input further, whose gradient the others' are added to; own: the token is the walk's

@@ -10,8 +10,8 @@
 // warps, and over several blocks, evenly over the keys that the env has; the last block of an env to end joins their partial sums, always in the same order, so
 // the same call gives the same bits.
 //
-// Measured, bf16, 8 heads, 2 of keys, dim 64: 4096 envs of 256 tokens 86 us, 4.8 TB/s of cached keys and values (0.73 of what a copy reaches): a warp's loads under way are as many as its registers
-// hold, and 13 warps an SM (20 %) leave the memory idle between them.  One env of 8192 tokens 9.5 us, of which its 4 MB are 1: it is bound by the chain of launch, loads and join.
+// Measured, bf16, 8 heads, 2 of keys, dim 64: 4096 envs of up to 256 tokens 80 us, 5.2 TB/s of cached keys and values (0.79 of what a copy reaches; 89 us where the L2 holds what others wrote): a warp's
+// loads under way are as many as its registers hold, and with at most 16 warps to an SM the memory idles between them (18 and 20 with spilled registers: 94 us).  One env of 8192 tokens 9.5 us, of which its 4 MB are 1: it is bound by the chain of launch, loads and join.
 // The first tokens of an episode may have places of their own before the ring: which place a token takes is all that changes, the order of keys being free.
 #include <cuda_runtime.h>
 #include <algorithm>

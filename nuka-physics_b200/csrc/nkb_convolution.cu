@@ -18,8 +18,8 @@
 namespace nkb {
 
 constexpr int kLines = 4;                               // warps of a block: stretches side by side
-constexpr int kForthBlocks = 5, kBackBlocks = 4;        // blocks of an SM
-constexpr int kForthBatch = 4, kBackBatch = 4;          // tokens whose loads are under way; a multiple of the longest window, so that its shift is a change of names
+constexpr int kForthBlocks = 4, kBackBlocks = 3;        // blocks of an SM
+constexpr int kForthBatch = 8, kBackBatch = 4;          // tokens whose loads are under way; a multiple of the longest window, so that its shift is a change of names
 constexpr int kWide = 4;                                // channels of a thread
 constexpr int kSms = 148;
 
@@ -98,24 +98,30 @@ template <typename T, int K, int VEC> __device__ __forceinline__ void window_beg
     for (int j = 0; j < K - 1; ++j) input<T, VEC>(p.initial, ((int64_t)row * (K - 1) + j) * p.channels + c, row >= 0 && p.initial != nullptr, window[j + 1]);
 }
 
-// A warp's next tokens, number `lane` to a lane: which of them begin an episode, and which end a row.
+// 32 tokens of a warp's walk, number `lane` to a lane: which of them begin an episode, and which end a row. The next 32 are under way meanwhile, so that no batch waits for its own.
 struct Marks {
-    int32_t link, tail;
+    int32_t link, tail, next_link, next_tail;
     uint32_t begins, ends;
-    __device__ __forceinline__ Marks(const ConvolutionParams& p, int64_t t0, int count) {
-        const int lane = threadIdx.x % 32;
-        link = lane < count ? p.plan.link[t0 + lane] : -1;
-        tail = lane < count ? p.plan.tail[t0 + lane] : -1;
+    __device__ __forceinline__ void ask(const ConvolutionParams& p, int64_t begin, int t0, int count) {
+        const int t = t0 + threadIdx.x % 32;
+        next_link = t < count ? p.plan.link[begin + t] : -1;
+        next_tail = t < count ? p.plan.tail[begin + t] : -1;
+    }
+    __device__ __forceinline__ void turn(const ConvolutionParams& p, int64_t begin, int t0, int count) {
+        link = next_link;
+        tail = next_tail;
         begins = __ballot_sync(~0u, link != -1);
         ends = __ballot_sync(~0u, tail >= 0);
+        ask(p, begin, t0 + 32, count);
     }
-    __device__ __forceinline__ int32_t row_of(int i) const { return __shfl_sync(~0u, link, i); }
-    __device__ __forceinline__ int32_t end_of(int i) const { return __shfl_sync(~0u, tail, i); }
+    __device__ __forceinline__ int32_t row_of(int t) const { return __shfl_sync(~0u, link, t & 31); }
+    __device__ __forceinline__ int32_t end_of(int t) const { return __shfl_sync(~0u, tail, t & 31); }
 };
 
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(const ConvolutionParams p) {
     constexpr int BATCH = kForthBatch;                  // tokens whose loads are under way
+    constexpr uint32_t kBatchBits = (1u << BATCH) - 1u;
     const int64_t own = ((int64_t)(blockIdx.x % p.tiles) * 32 + threadIdx.x % 32) * VEC, C = p.channels;
     const int64_t line = (int64_t)(blockIdx.x / p.tiles) * kLines + threadIdx.x / 32;
     if (line >= p.stretches) return;
@@ -132,6 +138,8 @@ __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(
         for (int i = 0; i < BATCH; ++i) ahead[i] = load_raw<T, VEC>(x + min(t0 + i, count - 1) * p.x_stride);
     };
     fetch(0);
+    Marks marks;
+    marks.ask(p, begin, 0, count);
     float window[K][VEC];                               // after the shift at a token's begin: the last inputs, 0 the oldest
     if (p.plan.link[begin] == -1) window_before<T, K, VEC>(p, begin, c, window);
     for (int t0 = 0; t0 < count; t0 += BATCH) {
@@ -139,8 +147,9 @@ __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(
         Raw<T, VEC> now[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) now[i] = ahead[i];
-        const Marks marks(p, begin + t0, left);
         if (t0 + BATCH < count) fetch(t0 + BATCH);
+        if (t0 % 32 == 0) marks.turn(p, begin, t0, count);
+        const uint32_t begins = marks.begins >> (t0 & 31) & kBatchBits, ends = marks.ends >> (t0 & 31) & kBatchBits;
         auto token = [&](int i) {
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
@@ -153,26 +162,26 @@ __global__ void __launch_bounds__(kLines * 32, kForthBlocks) convolution_kernel(
             if (live) store<T, VEC>(y, s);
             y += C;
         };
-        auto begin_at = [&](int i) { window_begins<T, K, VEC>(p, marks.row_of(i), c, window); };
+        auto begin_at = [&](int i) { window_begins<T, K, VEC>(p, marks.row_of(t0 + i), c, window); };
         auto end_at = [&](int i) {
-            T* const to = static_cast<T*>(p.state) + (int64_t)marks.end_of(i) * (K - 1) * C + c;
+            T* const to = static_cast<T*>(p.state) + (int64_t)marks.end_of(t0 + i) * (K - 1) * C + c;
 #pragma unroll
             for (int j = 0; j < K - 1; ++j)
                 if (live) store<T, VEC>(to + j * C, window[j + 1]);
         };
         // mostly nothing begins or ends but at the edges
-        if (left == BATCH && (marks.begins & ~1u) == 0u && (marks.ends & ~(1u << (BATCH - 1))) == 0u) {
-            if (marks.begins != 0u) begin_at(0);
+        if (left == BATCH && (begins & ~1u) == 0u && (ends & ~(1u << (BATCH - 1))) == 0u) {
+            if (begins != 0u) begin_at(0);
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) token(i);
-            if (marks.ends != 0u) end_at(BATCH - 1);
+            if (ends != 0u) end_at(BATCH - 1);
         } else {
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
                 if (i >= left) break;
-                if (marks.begins >> i & 1u) begin_at(i);
+                if (begins >> i & 1u) begin_at(i);
                 token(i);
-                if (marks.ends >> i & 1u) end_at(i);
+                if (ends >> i & 1u) end_at(i);
             }
         }
     }
@@ -182,6 +191,7 @@ template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_kernel(const ConvolutionParams p) {
     __shared__ float sums[kLines / 2][(K + 1) * VEC * 32];
     constexpr int BATCH = kBackBatch;
+    constexpr uint32_t kBatchBits = (1u << BATCH) - 1u;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const int64_t own = ((int64_t)(blockIdx.x % p.tiles) * 32 + lane) * VEC, C = p.channels;
     const bool live = own < C;
@@ -213,26 +223,36 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
                 if (live && early >= 0) store<T, VEC>(static_cast<T*>(p.dinitial) + ((int64_t)row * (K - 1) + early) * C + c, g);
             }
         };
-        int last = past;                                // behind the last token walked
-        for (int t0 = 0; t0 < past && last == past; t0 += BATCH) {
-            const int left = min(BATCH, past - t0);
-            Raw<T, VEC> xs[BATCH], dys[BATCH];
+        Raw<T, VEC> x_ahead[BATCH], dy_ahead[BATCH];
+        auto fetch = [&](int t0) {
             const T *const xb = x + t0 * p.x_stride, *const dyb = dy + t0 * C;
-            if (left == BATCH) {                        // no clamp between the loads of a full batch: 3% of this kernel
+            if (t0 + BATCH <= past) {                   // no clamps between the loads of a full batch
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    xs[i] = load_raw<T, VEC>(xb + i * p.x_stride);
-                    dys[i] = load_raw<T, VEC>(dyb + i * C);
+                    x_ahead[i] = load_raw<T, VEC>(xb + i * p.x_stride);
+                    dy_ahead[i] = load_raw<T, VEC>(dyb + i * C);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    const int t = min(i, left - 1);
-                    xs[i] = load_raw<T, VEC>(xb + t * p.x_stride);
-                    dys[i] = load_raw<T, VEC>(dyb + t * C);
+                    const int t = min(i, past - 1 - t0);
+                    x_ahead[i] = load_raw<T, VEC>(xb + t * p.x_stride);
+                    dy_ahead[i] = load_raw<T, VEC>(dyb + t * C);
                 }
             }
-            const Marks marks(p, begin + t0, left);
+        };
+        fetch(0);
+        Marks marks;
+        marks.ask(p, begin, 0, past);
+        int last = past;                                // behind the last token walked
+        for (int t0 = 0; t0 < past && last == past; t0 += BATCH) {
+            const int left = min(BATCH, past - t0);
+            Raw<T, VEC> xs[BATCH], dys[BATCH];
+#pragma unroll
+            for (int i = 0; i < BATCH; ++i) { xs[i] = x_ahead[i]; dys[i] = dy_ahead[i]; }
+            if (t0 + BATCH < past) fetch(t0 + BATCH);
+            if (t0 % 32 == 0) marks.turn(p, begin, t0, past);
+            const uint32_t begins = marks.begins >> (t0 & 31) & kBatchBits, ends = marks.ends >> (t0 & 31) & kBatchBits;
             // one input further, whose gradient the others' are added to; own: the token is the walk's
             auto token = [&](int i, bool own) {
 #pragma unroll
@@ -259,7 +279,7 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
                 }
             };
             auto end_at = [&](int i) {
-                const int32_t ended = marks.end_of(i);
+                const int32_t ended = marks.end_of(t0 + i);
                 if (p.dstate == nullptr) return;
 #pragma unroll
                 for (int j = 0; j < K - 1; ++j) {
@@ -269,37 +289,47 @@ __global__ void __launch_bounds__(kLines * 32, kBackBlocks) convolution_grad_ker
                     for (int v = 0; v < VEC; ++v) grad[j + 1][v] += more[v];
                 }
             };
-            // mostly nothing begins, or ends but at the edge, and what leaves is the walk's and the episode's
-            if (t0 >= K && first <= t0 - K && t0 + BATCH <= end && marks.begins == 0u && (marks.ends & ~(1u << (BATCH - 1))) == 0u) {
+            // an episode begins at token t: what the last one leaves, and an empty window
+            auto begin_at = [&](int t) {
+                if (t > 0)
+#pragma unroll
+                    for (int j = 0; j < K; ++j) leave(t - K + j, grad[j]);
+                first = t;
+                row = marks.row_of(t);
+                window_begins<T, K, VEC>(p, row, c, window);
+#pragma unroll
+                for (int j = 0; j < K; ++j)
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) grad[j][v] = 0.f;
+            };
+            // mostly nothing begins or ends but at the edges, and what leaves is the walk's and the episode's, or the initial inputs' of the row that begins here
+            const bool fresh = begins == 1u;
+            if (t0 + BATCH <= end && (fresh || (begins == 0u && t0 >= K && first <= t0 - K)) && (ends & ~(1u << (BATCH - 1))) == 0u) {
+                T* to = dx + (t0 - K) * C;
+                if (fresh) {
+                    begin_at(t0);
+                    to = row >= 0 && p.dinitial != nullptr ? static_cast<T*>(p.dinitial) + ((int64_t)row * (K - 1) - 1) * C + c : nullptr;
+                }
 #pragma unroll
                 for (int i = 0; i < BATCH; ++i) {
-                    if (live) store<T, VEC>(dx + (t0 + i - K) * C, grad[0]);
+                    if (i >= K ? live : live && to != nullptr && !(fresh && i == 0)) store<T, VEC>((i >= K ? dx + (t0 - K) * C : to) + i * C, grad[0]);
                     token(i, true);
                 }
-                if (marks.ends != 0u) end_at(BATCH - 1);
+                if (ends != 0u) end_at(BATCH - 1);
                 continue;
             }
 #pragma unroll
             for (int i = 0; i < BATCH; ++i) {
                 const int t = t0 + i;
                 if (i >= left) break;
-                if (marks.begins >> i & 1u) {
+                if (begins >> i & 1u) {
                     if (t >= end) { last = t; break; }
-                    if (t > 0)
-#pragma unroll
-                        for (int j = 0; j < K; ++j) leave(t - K + j, grad[j]);
-                    first = t;
-                    row = marks.row_of(i);
-                    window_begins<T, K, VEC>(p, row, c, window);
-#pragma unroll
-                    for (int j = 0; j < K; ++j)
-#pragma unroll
-                        for (int v = 0; v < VEC; ++v) grad[j][v] = 0.f;
+                    begin_at(t);
                 } else if (t > 0) {
                     leave(t - K, grad[0]);
                 }
                 token(i, t < end);
-                if (marks.ends >> i & 1u) end_at(i);
+                if (ends >> i & 1u) end_at(i);
             }
         }
 #pragma unroll

@@ -16,10 +16,10 @@ template <bool EXACT> __device__ __forceinline__ Fading fading(float u) {
 }
 __device__ __forceinline__ float logistic(float u, Fading f) { return u >= 0.f ? f.r : f.e * f.r; }
 __device__ __forceinline__ float one_less(float u, Fading f) { return u >= 0.f ? f.e * f.r : f.r; }             // 1 - logistic(u)
-// Where 16 bits are the result: 1 / (1 + exp(-s)) at once, the exponential kept finite.
+// Where 16 bits are the result: 1 / (1 + exp(-s)) at once. The exponential may be infinite, and the result 0, as it has to be next to an s of that size.
 __device__ __forceinline__ float logistic_fast(float s) {
     float e, r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(fminf(s * -1.4426950408889634f, 126.f)));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(s * -1.4426950408889634f));
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
     return r;
 }
@@ -45,7 +45,7 @@ __device__ __forceinline__ float inverse_of(float x) {
 __device__ __forceinline__ Pair logistic_pair(Pair s) {
     float a, b, x, y;
     split(mul_pair(s, both(-1.4426950408889634f)), a, b);
-    split(add_pair(pair_of(exp2_fast(fminf(a, 126.f)), exp2_fast(fminf(b, 126.f))), both(1.f)), x, y);
+    split(add_pair(pair_of(exp2_fast(a), exp2_fast(b)), both(1.f)), x, y);
     return pair_of(inverse_of(x), inverse_of(y));
 }
 // s = silu(s)

@@ -349,6 +349,30 @@ def test_gradients_against_differences():
 
 
 # ---- what programs do around a call ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(UNIT))
+def test_sums_and_gates_of_any_size(dtype):
+    """s / (1 + exp(-s)) and its slope where the exponential ends at infinity or 0: the slope's and the value's own size is then that of TINY or of s, 1 or 0, times products of at most one such factor."""
+    top = float(torch.finfo(dtype).max)
+    s = torch.tensor([-top, -top / 4, -top / 64, -1000.0, -200.0, -100.0, -20.0, 0.0, 20.0, 100.0, 1000.0, top / 64, top / 4], device="cuda").to(dtype)[:, None].expand(-1, 8).contiguous().requires_grad_()
+    plan, tokens = _plan_of([s.shape[0]]), s.shape[0]
+    dy = _normal(_gen(1), tokens, 8, dtype=dtype)
+    value, slope = _silu(s.detach().double())
+    unit = UNIT[dtype] + SLIP
+    weight = torch.tensor([0.0, 1.0], device="cuda").expand(8, 2).contiguous()
+    y, _ = S.short_convolution(s, weight, None, plan, silu=True)
+    dx, = torch.autograd.grad(y, s, dy)
+    _close(y.detach(), value, 64 * TINY, "y", unit, STEP[dtype])
+    _close(dx, dy.double() * slope, 64 * TINY + SLIP * dy.double().abs(), "dx", unit, STEP[dtype])
+    # states of nothing, so that y = x / 2 silu(gate)
+    x, none = torch.ones(tokens, 8, device="cuda", dtype=dtype, requires_grad=True), torch.zeros(tokens, 4, device="cuda", dtype=dtype)
+    y, _ = S.selective_scan(x, torch.zeros_like(x), -torch.ones(8, 4, device="cuda"), none, none, plan, skip=torch.full((8,), 0.5, device="cuda"), gate=s)
+    _close(y.detach(), value / 2, 64 * TINY, "scan's y", unit, STEP[dtype])
+    small = s.detach().double() <= 1000
+    dx, dgate = torch.autograd.grad(y, (x, s), dy * small.to(dtype))            # of x's gradient only what fits the type
+    _close(dx, dy.double() * small * value / 2, 64 * TINY, "scan's dx", unit, STEP[dtype])
+    _close(dgate, dy.double() * small * slope / 2, 64 * TINY + SLIP * dy.double().abs(), "dgate", unit, STEP[dtype])
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_what_is_not_finite_stays_in_its_episode(bad):
     """A value of one episode's input: outputs, states and gradients of the other episodes keep their bits."""

@@ -7,9 +7,10 @@
 // and the sums that become the gradients of the last K inputs travel with them; the walk goes K - 1 tokens past its stretch (as far as the episode does) to complete them.
 // Weights' gradients are summed in registers over all stretches of a thread, then over a block's warps, then over the blocks, always in the same order.
 //
-// Measured, K = 4 with silu: 4096 rows of 24 x 512, bf16, 55 us forwards (3.7 TB/s of its 2 tensors) and 103 back (2.9 TB/s of 3); 3 long rows, 131071 x 1024, f16, 131 us (4.1 TB/s) and 242 (3.3 TB/s).
-// Memory is half busy; the instructions, 2.0 of 4 a cycle (exponentials' unit 47 % forwards, multiplications' 40 % back), and the few loads that registers leave room for share the rest. Eight channels to a thread were
-// slower both ways (fewer warps), two slower back; so was a batch asked for before the one in hand is walked (115 back: registers run out, and with them free, 3 blocks to an SM, 123).
+// Measured, K = 4 with silu: 4096 rows of 24 x 512, bf16, 52 us forwards (3.9 TB/s of its 2 tensors) and 87 back (3.5 TB/s of 3); 3 long rows, 131071 x 1024, f16, 113 us (4.8 TB/s) and 204 (3.9 TB/s).
+// The loads of the next tokens, and the plan's marks of the next 32, are under way while these are walked: with marks asked for by the batch, 55, 103, 133 and 243 us. Instructions, 1.9 to 2.0 of 4 a cycle, are some 15 a value
+// forwards and 28 back, the exponentials' unit is busy for half of the time forwards and the multiplications' for 40 % back; 16 and 12 warps an SM is what the registers leave. More warps with four tokens ahead forwards: 52 and
+// 124; back, four blocks to an SM spill (109 and 242), eight tokens ahead too (100 and 259). Eight channels to a thread were slower both ways (fewer warps), two slower back; blocks that take walks in turn forwards the same.
 #include <algorithm>
 #include "nkb_gates.cuh"
 #include "nkb_sequence.cuh"

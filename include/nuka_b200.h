@@ -445,7 +445,8 @@ nuka_result_t nuka_b200_convolution_step(const nuka_b200_convolution_step_t* des
 
 /* The selective scan over the plan's episodes: dt = softplus(delta + delta_bias), h_t[c][n] = exp(dt decay[c][n]) h_{t-1}[c][n] + dt x b_t[n], y = sum over n of c_t[n] h_t[c][n] + skip[c] x, times
  * gate / (1 + exp(-gate)) where a gate is given.  An episode that begins inside a row begins from 0, a row from initial (rows x channels x states, NULL = 0).  state (like initial) receives the h that each
- * row ends with; empty rows are left as they are.  1 to 64 states.  Everything of dtype is rounded once, when it is written; rates, states and sums are in 32 bits. */
+ * row ends with; empty rows are left as they are.  1 to 64 states; without channels (or without tokens) gradients that are sums over none are 0.
+ * Everything of dtype is rounded once, when it is written; rates, states and sums are in 32 bits. */
 typedef struct nuka_b200_scan_t {
     const nuka_b200_episodes_t* plan;
     uint32_t dtype;                                 /* of x, delta, gate, b, c, y and their gradients */

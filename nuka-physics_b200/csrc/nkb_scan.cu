@@ -994,11 +994,14 @@ template <typename T> static cudaError_t run_scan(const nuka_b200_scan_t& d, boo
 }
 
 cudaError_t launch_scan(const nuka_b200_scan_t& d, bool backward, cudaStream_t stream) {
-    if (d.plan->tokens == 0) {                          // weights' gradients are sums of nothing
+    const int64_t tokens = d.plan->tokens;
+    if (tokens == 0 || d.channels == 0) {               // weights' gradients, and those of B and C, are sums of nothing; what has no values is left alone
+        const size_t size = d.dtype == NUKA_B200_F32 ? 4 : 2;
         cudaError_t set = cudaSuccess;
-        const struct { float* at; int64_t count; } sums[] = {{d.ddecay, d.channels * d.states}, {d.dskip, d.channels}, {d.ddelta_bias, d.channels}};
+        const struct { void* at; size_t bytes; } sums[] = {{d.ddecay, (size_t)(d.channels * d.states) * 4}, {d.dskip, (size_t)d.channels * 4}, {d.ddelta_bias, (size_t)d.channels * 4},
+                                                           {d.db, (size_t)(tokens * d.states) * size}, {d.dc, (size_t)(tokens * d.states) * size}};
         for (const auto& s : sums)
-            if (backward && s.at != nullptr && set == cudaSuccess) set = cudaMemsetAsync(s.at, 0, (size_t)s.count * 4, stream);
+            if (backward && s.at != nullptr && s.bytes != 0 && set == cudaSuccess) set = cudaMemsetAsync(s.at, 0, s.bytes, stream);
         return set;
     }
     return d.dtype == NUKA_B200_F32 ? run_scan<float>(d, backward, stream) : d.dtype == NUKA_B200_F16 ? run_scan<__half>(d, backward, stream) : run_scan<__nv_bfloat16>(d, backward, stream);

@@ -166,9 +166,11 @@ static nuka_result_t Scan(const nuka_b200_scan_t* desc, bool backward, void* str
     if (backward)
         for (const float* p : {d.dstate, static_cast<const float*>(d.ddecay), static_cast<const float*>(d.dskip), static_cast<const float*>(d.ddelta_bias), static_cast<const float*>(d.dinitial)})
             if (!Aligned(p, 4)) return Invalid("a weight's or state's gradient does not lie on 4 bytes");
-    if (d.channels == 0) return NUKA_RESULT_OK;
-    if (d.plan->tokens == 0) return Ran(nkb::launch_scan(d, backward, StreamOf(stream)));
     const uint64_t size = SizeOf(d.dtype);
+    if (d.channels == 0 && backward && d.plan->tokens != 0)                // of what a call without channels is asked for, B's and C's gradients alone are not empty
+        for (const void* p : {static_cast<const void*>(d.db), static_cast<const void*>(d.dc)})
+            if (p == nullptr || !Aligned(p, size)) return Invalid("a gradient is null or does not lie on a multiple of its type's size");
+    if (d.channels == 0 || d.plan->tokens == 0) return Ran(nkb::launch_scan(d, backward, StreamOf(stream)));
     for (const void* p : {d.x, d.delta, d.b, d.c, static_cast<const void*>(d.decay)})
         if (p == nullptr) return Invalid("x, delta, b, c or decay is null");
     if (!backward && (d.y == nullptr || d.state == nullptr)) return Invalid("y or state is null");

@@ -220,11 +220,11 @@ template <typename T> __device__ __forceinline__ const T* key_row(const Attentio
 template <typename T> __device__ __forceinline__ const T* value_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.v) + j * p.v_stride + head * p.v_head_stride; }
 template <typename T> __device__ __forceinline__ const T* dout_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.dout) + ((int64_t)i * p.heads_q + head) * p.dim; }
 __device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
-__device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 && j - p.first[j] >= p.sinks ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+template <bool SINKS> __device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 && !(SINKS && j - p.first[j] < p.sinks) ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
 // The keys that query i sees, in one range or, its sinks first, in two.
-template <typename Use> __device__ __forceinline__ void each_range(const AttentionParams& p, int i, Use use) {
+template <bool SINKS, typename Use> __device__ __forceinline__ void each_range(const AttentionParams& p, int i, Use use) {
     const int low = first_key(p, i);
-    if (p.sinks > 0 && p.first[i] < low) use(p.first[i], p.first[i] + min(p.sinks, low - p.first[i]) - 1);
+    if (SINKS && p.first[i] < low) use(p.first[i], p.first[i] + min(p.sinks, low - p.first[i]) - 1);
     use(low, i);
 }
 
@@ -258,20 +258,20 @@ template <typename T, typename Row> __device__ __forceinline__ void add_rows(flo
 }
 constexpr uint32_t kFinal = 0xffffu;                    // first value of an output row whose lse is not finite: NaN as no conversion gives it
 
-template <typename T> __device__ __noinline__ void mend_out(const AttentionParams& p, int i, int head, int lane) {
+template <typename T, bool SINKS> __device__ __noinline__ void mend_out(const AttentionParams& p, int i, int head, int lane) {
     T* const out = static_cast<T*>(p.out) + ((int64_t)i * p.heads_q + head) * p.dim;
     const uint2 is = result_of(out, p.dim, lane);
     uint32_t which = spoilt_of<T>(is);
     if (!__any_sync(~0u, which != 0u) || (__shfl_sync(~0u, is.x, 0) & 0xffffu) == kFinal) return;
     const int key_head = head / (p.heads_q / p.heads_k);
-    each_range(p, i, [&](int low, int high) {
+    each_range<SINKS>(p, i, [&](int low, int high) {
         for (int j = low; j <= high && __any_sync(~0u, which != 0u); j += 8)
 #pragma unroll
             for (int k = 0; k < 8; ++k) which &= ~spoilt_of<T>(result_of(value_row<T>(p, min(j + k, high), key_head), p.dim, lane));
     });
     if (!__any_sync(~0u, which != 0u)) return;
     float top = -INFINITY, total = 0.f, sum[4] = {};
-    each_range(p, i, [&](int low, int high) {
+    each_range<SINKS>(p, i, [&](int low, int high) {
     for (int j = low; j <= high; j += 32) {
         const int count = min(32, high - j + 1);
         const float score = lane < count ? dot(query_row<T>(p, i, head), key_row<T>(p, j + lane, key_head), p.dim) * p.scale2 : -INFINITY;
@@ -292,7 +292,7 @@ template <typename T> __device__ __noinline__ void mend_out(const AttentionParam
     give_columns(out, which, sum, 1.f / total, lane);
 }
 
-template <typename T> __device__ __noinline__ void mend_query_grad(const AttentionParams& p, int i, int head, int lane) {
+template <typename T, bool SINKS> __device__ __noinline__ void mend_query_grad(const AttentionParams& p, int i, int head, int lane) {
     const float lse = p.lse[head * p.pitch + i], delta = __ldcg(p.delta + head * p.pitch + i);
     if (!isfinite(lse) || !isfinite(delta)) return;
     T* const dq = static_cast<T*>(p.dq) + ((int64_t)i * p.heads_q + head) * p.dim;
@@ -300,7 +300,7 @@ template <typename T> __device__ __noinline__ void mend_query_grad(const Attenti
     if (!__any_sync(~0u, which != 0u)) return;
     const int key_head = head / (p.heads_q / p.heads_k);
     float sum[4] = {};
-    each_range(p, i, [&](int low, int high) {
+    each_range<SINKS>(p, i, [&](int low, int high) {
     for (int j = low; j <= high; j += 32) {
         const int count = min(32, high - j + 1), own = min(j + lane, high);
         const float prob = exp2f(fmaf(dot(query_row<T>(p, i, head), key_row<T>(p, own, key_head), p.dim), p.scale2, -lse));
@@ -312,11 +312,11 @@ template <typename T> __device__ __noinline__ void mend_query_grad(const Attenti
 }
 
 // values: the value's gradient, else the key's
-template <typename T> __device__ __noinline__ void mend_key_grad(const AttentionParams& p, int j, int key_head, bool values, int lane) {
+template <typename T, bool SINKS> __device__ __noinline__ void mend_key_grad(const AttentionParams& p, int j, int key_head, bool values, int lane) {
     T* const to = static_cast<T*>(values ? p.dv : p.dk) + ((int64_t)j * p.heads_k + key_head) * p.dim;
     uint32_t which = spoilt_of<T>(result_of(to, p.dim, lane));
     if (!__any_sync(~0u, which != 0u)) return;
-    const int group = p.heads_q / p.heads_k, past = past_query(p, j);
+    const int group = p.heads_q / p.heads_k, past = past_query<SINKS>(p, j);
     for (int head = key_head * group; head < (key_head + 1) * group; ++head)
         for (int i = j; i < past; i += 32) {
             const int64_t at = head * p.pitch + min(i + lane, past - 1);
@@ -556,10 +556,10 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
             const int first = next.i0[set], last = next.last[set], i = first + row, head = next.head[set];
             const KeySteps<SINKS> through = next.steps<SINKS>(p, F::kStep);
-            // keys that any and that all of the warp's rows see; a row that is not there sees none
-            const RowKeys<SINKS> keys(p, i <= last, i, next_first);
-            const int after = ForwardJob::of_turn(turn + 1);
+            const int episode = next_first, after = ForwardJob::of_turn(turn + 1);
             if (after < jobs) { next = ForwardJob(p, after); next_first = first_of(next); }
+            // keys that any and that all of the warp's rows see; a row that is not there sees none
+            const RowKeys<SINKS> keys(p, i <= last, i, episode);
             float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
             bool left = false;
             for (int j = 0; j < through.count; ++j, ++n) {
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
         if (spoilt[set] != 0 && lost == 0)
             for (int turn = 0, job = blockIdx.x; job < jobs; job = ForwardJob::of_turn(++turn)) {
                 const ForwardJob done(p, job);
-                for (int i = done.i0[set] + warp % 4; i <= done.last[set]; i += 4) mend_out<T>(p, i, done.head[set], lane);
+                for (int i = done.i0[set] + warp % 4; i <= done.last[set]; i += 4) mend_out<T, SINKS>(p, i, done.head[set], lane);
             }
     }
     __syncwarp();
@@ -706,7 +706,7 @@ template <int DP> struct Queries {
 template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
                                                                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq,
-                                                               const AttentionParams p) {
+                                                               const __grid_constant__ AttentionParams p) {
     using F = Queries<DP>;
     __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], s_empty[F::kBuffers], p_full, o_done, ended;
     __shared__ uint32_t tensor;
@@ -941,7 +941,7 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
         if (spoilt != 0 && lost == 0)
             for (int job = blockIdx.x; job < jobs; job += stride) {
                 const QueryJob done(p, job);
-                for (int i = done.i0 + half * 4 + warp % 4; i <= done.last; i += F::kWorkers / 32) mend_query_grad<T>(p, i, done.head, lane);
+                for (int i = done.i0 + half * 4 + warp % 4; i <= done.last; i += F::kWorkers / 32) mend_query_grad<T, SINKS>(p, i, done.head, lane);
             }
     }
     __syncwarp();
@@ -1007,7 +1007,7 @@ template <int DP, int THREADS> __device__ __noinline__ void clear_hidden(int fro
 template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                                                                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
-                                                                            const __grid_constant__ CUtensorMap map_dv, const AttentionParams p) {
+                                                                            const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ AttentionParams p) {
     using F = Keys<DP>;
     __shared__ uint64_t k_full, k_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], p_full, o_done, ended;
     __shared__ __align__(16) float lse[F::kStages][kStream], delta[F::kStages][kStream];
@@ -1265,7 +1265,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
             for (int job = job0; job < jobs; job += stride) {
                 const KeyJob<SINKS> done(p, job);
                 for (int j = done.j0 + half * 4 + warp % 4; j <= done.last; j += F::kWorkers / 32)
-                    for (int which = 0; which < 2; ++which) mend_key_grad<T>(p, j, done.head, which, lane);
+                    for (int which = 0; which < 2; ++which) mend_key_grad<T, SINKS>(p, j, done.head, which, lane);
             }
     }
     __syncwarp();
@@ -1296,7 +1296,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         __syncthreads();
         if (spoilt != 0 && lost == 0)
             for (int x = warp; x < 2 * rows; x += F::kThreads / 32)
-                if (const int j = job.j0 + rank * rows + x % rows; j <= job.last) mend_key_grad<T>(p, j, job.head, x >= rows, lane);
+                if (const int j = job.j0 + rank * rows + x % rows; j <= job.last) mend_key_grad<T, SINKS>(p, j, job.head, x >= rows, lane);
     }
 }
 

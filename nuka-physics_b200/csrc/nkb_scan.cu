@@ -26,6 +26,9 @@ namespace nkb {
 constexpr int kScanWarps = 4;                           // of a block
 template <int N> struct Flag { static constexpr int value = N; };
 constexpr float kToBase2 = 1.4426950408889634f, kFromBase2 = 0.6931471805599453f;
+// Sums over tokens of one warp, term by term in 32 bits, are off by up to n 2^-24 of the terms' sizes. A warp with more than kLongSum tokens adds what it has to its share in memory every kFold tokens.
+constexpr int64_t kLongSum = 4096;
+constexpr int kFold = 1024;
 
 // LN: lanes over the states
 template <int LN> struct ScanTile {
@@ -626,7 +629,8 @@ __global__ void __launch_bounds__(kScanWarps * 32, 4) scan_back_maps_kernel(cons
     give_totals<T, LN>(p, m, l.cell(m.out), total, l.lane, segment * p.tiles + tile, closed);
 }
 
-template <typename T, int LN>
+// FOLD: the weights' sums go to memory every kFold tokens, not only at the end. The check after each chunk costs 2 % (4096 rows of 24 x 512 1574 us in all, forwards too, and 1541 without), so where sums are short it is left out.
+template <typename T, int LN, bool FOLD>
 __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const ScanParams p) {
     using S = ScanTile<LN>;
     constexpr int E = S::kEach;
@@ -662,6 +666,45 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
         links = l.lane < left ? p.plan.link[t0 + l.lane] : -1;
         tails = l.lane < left ? p.plan.tail[t0 + l.lane] : -1;
         h.load(p.kept + ((segment * p.chunks + k) * p.tiles + tile) * 128 + l.lane);
+    };
+    int since = 0;                                      // tokens in the weights' sums
+    bool before = false;                                // some are in the warp's share already
+    auto leave = [&]() {
+        // lanes that have values of the same channels, which lie as many apart as a token has
+        constexpr int APART = S::kChannels / E;
+#pragma unroll
+        for (int d = APART; d < 32; d *= 2)
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                dskip[k] += __shfl_xor_sync(~0u, dskip[k], d);
+                dbias[k] += __shfl_xor_sync(~0u, dbias[k], d);
+            }
+        const int64_t at = worker * p.tiles + tile;
+        float4* const decays = reinterpret_cast<float4*>(p.ddecay) + at * 128 + l.lane;
+        float *const skips = p.dskip + at * S::kChannels + l.channel, *const biases = p.dbias + at * S::kChannels + l.channel;
+        if (FOLD && before) {
+            States sofar;
+            sofar.load(decays);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ddecay.h[j][i] = add_pair(ddecay.h[j][i], sofar.h[j][i]);
+            if (l.lane < APART)
+#pragma unroll
+                for (int k = 0; k < E; ++k) { dskip[k] += skips[k]; dbias[k] += biases[k]; }
+        }
+        if (l.lane < APART) {
+            put(skips, dskip);
+            put(biases, dbias);
+        }
+        ddecay.store(decays);
+        if (FOLD) {
+            ddecay.clear();
+#pragma unroll
+            for (int k = 0; k < E; ++k) dskip[k] = dbias[k] = 0.f;
+            since = 0;
+            before = true;
+        }
     };
     fetch(worker, last_of(worker));                     // workers are no more than segments
     for (int64_t segment = worker; segment < p.segments; segment += p.workers) {
@@ -842,23 +885,10 @@ __global__ void __launch_bounds__(kScanWarps * 32, 2) scan_grad_kernel(const Sca
                 }
             }
             __syncwarp();
+            if (FOLD && ((since += S::kChunk) >= kFold || (k0 == 0 && segment + p.workers >= p.segments))) leave();
         }
     }
-    // lanes that have values of the same channels, which lie as many apart as a token has
-    constexpr int APART = S::kChannels / E;
-#pragma unroll
-    for (int d = APART; d < 32; d *= 2)
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            dskip[k] += __shfl_xor_sync(~0u, dskip[k], d);
-            dbias[k] += __shfl_xor_sync(~0u, dbias[k], d);
-        }
-    const int64_t at = worker * p.tiles + tile;
-    if (l.lane < APART) {
-        put(p.dskip + at * S::kChannels + l.channel, dskip);
-        put(p.dbias + at * S::kChannels + l.channel, dbias);
-    }
-    ddecay.store(reinterpret_cast<float4*>(p.ddecay) + at * 128 + l.lane);
+    if (!FOLD) leave();
 }
 
 // The workers' sums into one: a block per 32 of a tile's 512 decays and their channels' other sums.
@@ -972,13 +1002,14 @@ template <typename T, int LN> static cudaError_t run_scan(const nuka_b200_scan_t
     const int64_t narrow = s.tiles * p.plan.tokens * s.states;
     p.db = work; p.dc_after = narrow; p.ddecay = work + 2 * narrow; p.dskip = p.ddecay + s.workers * s.tiles * 512; p.dbias = p.dskip + s.workers * s.tiles * s.channels;
     constexpr int SHARED = sizeof(ScanGradShared<T, LN>) * kScanWarps;
-    const cudaError_t set = cudaFuncSetAttribute(scan_grad_kernel<T, LN>, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED);
+    const auto grad = (s.segments + s.workers - 1) / s.workers * s.segment > kLongSum ? scan_grad_kernel<T, LN, true> : scan_grad_kernel<T, LN, false>;
+    const cudaError_t set = cudaFuncSetAttribute(grad, cudaFuncAttributeMaxDynamicSharedMemorySize, SHARED);
     if (set != cudaSuccess) return set;
     if (!s.alone) {
         scan_back_maps_kernel<T, LN><<<jobs, kScanWarps * 32, 0, stream>>>(p);
         scan_carries_kernel<LN, true><<<carries, 1024, 0, stream>>>(p);
     }
-    scan_grad_kernel<T, LN><<<(unsigned)((s.workers * s.tiles + kScanWarps - 1) / kScanWarps), kScanWarps * 32, SHARED, stream>>>(p);
+    grad<<<(unsigned)((s.workers * s.tiles + kScanWarps - 1) / kScanWarps), kScanWarps * 32, SHARED, stream>>>(p);
     scan_sums_kernel<LN><<<(unsigned)(s.tiles * (16 + 2 * ((s.channels + 31) / 32))), 1024, 0, stream>>>(p, d.ddecay, d.dskip, d.ddelta_bias);
     scan_narrow_kernel<T><<<(unsigned)((p.plan.tokens * s.states + 255) / 256), 256, 0, stream>>>(p, (int)s.states, static_cast<T*>(d.db), static_cast<T*>(d.dc));
     return cudaGetLastError();

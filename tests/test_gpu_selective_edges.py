@@ -1,4 +1,5 @@
-"""Calls of the selective operators at the ends of what they take: no channels."""
+"""Calls of the selective operators at the ends of what they take: no channels, and sums over many tokens."""
+import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -6,6 +7,8 @@ import nuka  # noqa: E402,F401
 from nuka import sequence as S  # noqa: E402
 
 pytestmark = pytest.mark.gpu
+
+SLIP = 2.0 ** -20                       # of what the few roundings of a formula in 32 bits come to, an exponential's (and its argument's) among them
 
 
 def _rows_of(*lengths):
@@ -30,3 +33,46 @@ def test_a_scan_without_channels(dtype, lengths):
     leaves = [x, delta, decay, b, c, first, skip, gate, bias]
     for leaf, grad in zip(leaves, torch.autograd.grad([y, state], leaves, [torch.ones_like(y), torch.ones_like(state)])):
         assert grad.shape == leaf.shape and not grad.any()
+
+
+def _sums_of_equal_tokens(rows, length, states, dt, slope, decay, gate):
+    """{name: (value, bound)} of a channel's sums over all tokens, where x, b, c and dy are 1 in all of them: the terms' own error by the recurrences that the states follow."""
+    a, loss = np.exp(dt * decay), SLIP * (1 + dt * np.abs(decay))
+    h, E = np.zeros(states), np.zeros(states)
+    before, slips = np.zeros((length, states)), np.zeros((length, states))
+    for t in range(length):
+        before[t], slips[t] = h, E
+        h, E = a * h + dt, a * (E + loss * h) + SLIP * dt
+    back, EB = np.zeros(states), np.zeros(states)
+    ddecay, ddecay_slip, dbias, dbias_slip = np.zeros(states), np.zeros(states), 0.0, 0.0
+    for t in range(length - 1, -1, -1):
+        m, EM = back + gate, EB + SLIP * (back + gate)
+        through, slip = m * a * before[t], a * (EM * before[t] + m * slips[t] + loss * m * before[t])
+        ddecay += through * dt
+        ddecay_slip += slip * dt + SLIP * through * dt
+        dbias += (np.sum(through * decay) + np.sum(m)) * slope
+        dbias_slip += (np.sum((slip + SLIP * through) * np.abs(decay)) + np.sum(EM + SLIP * m) + SLIP * abs(np.sum(through * decay) + np.sum(m))) * slope
+        back, EB = a * m, a * (EM + loss * m)
+    return {"decay": (rows * ddecay, rows * ddecay_slip), "delta_bias": (rows * dbias, rows * dbias_slip), "skip": (rows * length * gate, SLIP * rows * length * gate)}
+
+
+@pytest.mark.parametrize("dtype,rows,length,channels,states", [(torch.bfloat16, 1, 16381, 4744, 64), (torch.bfloat16, 4, 4100, 4744, 64), (torch.float16, 1, 4200, 18960, 32), (torch.bfloat16, 1, 4200, 37920, 16),
+                                                               (torch.float32, 3, 1400, 37920, 12), (torch.bfloat16, 1, 4200, 75904, 8)])
+def test_weights_gradients_of_many_tokens(dtype, rows, length, channels, states):
+    """So many channels that one warp has all tokens of its own.  Sums of n terms of one sign, one by one, are off by up to n 2^-24 of themselves: n is the 1024 terms of a warp's registers, as many parts as these make of
+    all tokens, and the 32 of the last sum, and not all the tokens (of 16381, the gradients of decays were off by 2^-12.1)."""
+    tokens = rows * length
+    plan = S.Episodes.from_done(torch.zeros(rows, length, dtype=torch.bool, device="cuda")) if rows > 1 else _rows_of(length)
+    full = lambda value, *shape: torch.full(shape, value, dtype=dtype, device="cuda")
+    decay = torch.linspace(-0.3, -1.7, states, device="cuda").expand(channels, states).contiguous().requires_grad_()
+    skip, bias = (torch.zeros(channels, device="cuda", requires_grad=True) for _ in range(2))
+    x, delta, gate = full(1.0, tokens, channels), full(0.5, tokens, channels), full(0.7, tokens, channels)
+    y, _ = S.selective_scan(x, delta, decay, full(1.0, tokens, states), full(1.0, tokens, states), plan, skip=skip, gate=gate, delta_bias=bias)
+    got = dict(zip(("decay", "skip", "delta_bias"), torch.autograd.grad(y, [decay, skip, bias], torch.ones_like(y))))
+    z, u = gate[0, 0].item(), 0.5
+    want = _sums_of_equal_tokens(rows, length, states, np.log1p(np.exp(u)), 1 / (1 + np.exp(-u)), decay[0].detach().double().cpu().numpy(), z / (1 + np.exp(-z)))
+    chain = (1024 + -(-tokens // 1024) + 32) * 2.0 ** -24
+    for name, grad in got.items():
+        value, bound = (torch.as_tensor(v, dtype=torch.float64, device="cuda") for v in want[name])
+        off = (grad.double() - value).abs() - bound - chain * value.abs()       # of every channel
+        assert off.max().item() <= 0, f"{name}: off by {((grad.double() - value).abs() / value.abs()).max().item():.3e} of itself"

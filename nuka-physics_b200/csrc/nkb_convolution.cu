@@ -413,10 +413,13 @@ template <typename T, int VEC> static ConvolutionParams convolution_params(const
     return p;
 }
 
-// Blocks along the tokens of the backward pass, each of which leaves a set of partial sums: as many as run at a time.
+// Blocks along the tokens of the backward pass, each of which leaves a set of partial sums: as many as run at a time, or several times that where a warp would sum more than kLongSum tokens one by one
+// (n terms in 32 bits are off by up to n 2^-24 of their sizes).
+constexpr int64_t kLongSum = 1024;
 static int64_t convolution_across(const nuka_b200_episodes_t& plan, int64_t channels) {
-    const int64_t stretch = stretch_of(plan, channels, true), stretches = (plan.tokens + stretch - 1) / stretch;
-    return std::min<int64_t>((stretches + kLines - 1) / kLines, walkers_of(channels) / kLines);
+    const int64_t stretch = stretch_of(plan, channels, true), stretches = (plan.tokens + stretch - 1) / stretch, walkers = walkers_of(channels);
+    const int64_t tokens = (stretches + walkers - 1) / walkers * stretch;
+    return std::min<int64_t>((stretches + kLines - 1) / kLines, walkers / kLines * ((tokens + kLongSum - 1) / kLongSum));
 }
 uint64_t convolution_workspace(const nuka_b200_episodes_t& plan, int64_t channels, int64_t width) { return (uint64_t)(convolution_across(plan, channels) * (width + 1) * channels) * sizeof(float); }
 

@@ -76,3 +76,19 @@ def test_weights_gradients_of_many_tokens(dtype, rows, length, channels, states)
         value, bound = (torch.as_tensor(v, dtype=torch.float64, device="cuda") for v in want[name])
         off = (grad.double() - value).abs() - bound - chain * value.abs()       # of every channel
         assert off.max().item() <= 0, f"{name}: off by {((grad.double() - value).abs() / value.abs()).max().item():.3e} of itself"
+
+
+def test_the_convolutions_weights_gradients_of_many_tokens():
+    """So many channels that four warps have all tokens.  n terms of one sign, one by one: 1024 tokens of a warp and a walk of 128 at most more, the block's four warps, the blocks."""
+    tokens, channels, width = 65536, 28420, 4
+    plan = _rows_of(tokens)
+    x, weight, bias = torch.ones(tokens, channels, dtype=torch.bfloat16, device="cuda"), torch.zeros(channels, width, device="cuda", requires_grad=True), torch.linspace(-2.0, 2.0, channels, device="cuda", requires_grad=True)
+    y, _ = S.short_convolution(x, weight, bias, plan, silu=True)
+    dw, db = torch.autograd.grad(y, [weight, bias], torch.ones_like(y))
+    s = bias.detach().double()
+    r = torch.special.expit(s)
+    ds = r * (1 + s * (1 - r))
+    loss = SLIP * r * (1 + s.abs() * (1 + s.abs())) + (1024 + 128 + 4 + 64) * 2.0 ** -24 * ds.abs()
+    for got, count in [(db, tokens), *((dw[:, j], tokens - width + 1 + j) for j in range(width))]:          # inputs before the episode are 0
+        off = (got.double() - ds * count).abs() - loss * count
+        assert off.max().item() <= 0, f"off by {((got.double() - ds * count).abs() / (ds * count).abs()).max().item():.3e}"

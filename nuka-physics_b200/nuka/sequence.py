@@ -68,6 +68,10 @@ def _call(device, function, *args):
     return stream
 
 
+# A kernel has written the tensor: told to autograd, which refuses a gradient that would read what it was.
+_written = torch.autograd.graph.increment_version
+
+
 def _ptr(tensor):
     return None if tensor is None else tensor.data_ptr()
 
@@ -277,6 +281,7 @@ def gated_recurrence_step(x, gate, state, fresh=None):
         fresh = _flags(fresh, x.shape[:1], device, "fresh")
     h = torch.empty(x.shape, dtype=x.dtype, device=device)
     _call(device, _abi.lib().nuka_b200_recurrence_step, dtype, x.shape[0], x.shape[1], x.data_ptr(), _stride(x, 0), gate.data_ptr(), _stride(gate, 0), _ptr(fresh), state.data_ptr(), h.data_ptr())
+    _written(state)
     return h
 
 
@@ -376,6 +381,7 @@ def short_convolution_step(x, weight, bias, state, fresh=None, silu=False):
     y = torch.empty((envs, channels), dtype=x.dtype, device=device)
     desc = _abi.ConvolutionStepDesc(dtype, bool(silu), envs, channels, width, x.data_ptr(), x.stride(0) if envs > 1 else 0, weight.data_ptr(), _ptr(bias), _ptr(fresh), state.data_ptr(), y.data_ptr())
     _call(device, _abi.lib().nuka_b200_convolution_step, ctypes.byref(desc))
+    _written(state)
     return y
 
 
@@ -502,6 +508,7 @@ def selective_scan_step(x, delta, decay, b, c, state, fresh=None, skip=None, gat
     desc = _abi.ScanStepDesc(_DTYPES[x.dtype], envs, channels, states, x.data_ptr(), delta.data_ptr(), None if gate is None else gate.data_ptr(), b.data_ptr(), c.data_ptr(), *by, decay.data_ptr(),
                              None if skip is None else skip.data_ptr(), None if delta_bias is None else delta_bias.data_ptr(), None if fresh is None else fresh.data_ptr(), state.data_ptr(), y.data_ptr())
     _call(device, _abi.lib().nuka_b200_scan_step, ctypes.byref(desc))
+    _written(state)
     return y
 
 

@@ -1,10 +1,10 @@
-"""What the selective operators' entries refuse at the ends of what they take, without a GPU."""
+"""What the selective operators' entries refuse at the ends of what they take, and what autograd is told, without a GPU."""
 import ctypes
 
 import pytest
 
-pytest.importorskip("torch")
-from nuka import _abi  # noqa: E402
+torch = pytest.importorskip("torch")
+from nuka import _abi, sequence as S  # noqa: E402
 
 AT = 1 << 20
 
@@ -20,3 +20,25 @@ def test_a_scan_without_channels_has_gradients_of_b_and_c():
         assert lib.nuka_b200_scan_backward(ctypes.byref(_abi.ScanDesc(**{**ok, **change})), None) == _abi.INVALID_ARG, change
     assert lib.nuka_b200_scan(ctypes.byref(_abi.ScanDesc(**ok)), None) == 0
     assert lib.nuka_b200_scan_backward(ctypes.byref(_abi.ScanDesc(**{**ok, "plan": _plan(tokens=0, rows=2, length=0)})), None) == 0
+
+
+@pytest.mark.parametrize("kind", ["recurrence", "convolution", "scan"])
+def test_a_state_that_was_stepped_on_has_no_gradients_of_what_it_was(kind, monkeypatch):
+    """A step writes the state in place. Autograd, which keeps what a row began with for the backward pass, refuses the gradient then, as for torch's own operators in place."""
+    monkeypatch.setattr(S, "_on_gpu", lambda first, *others: first.device)
+    monkeypatch.setattr(S, "_call", lambda device, function, *args: None)
+    plan, x = S.Episodes.from_offsets(torch.arange(3, dtype=torch.int32) * 5, 10), torch.randn(10, 8, requires_grad=True)
+    b, decay, taps, one = torch.randn(10, 4), -torch.rand(8, 4), torch.randn(8, 4), torch.randn(2, 8)
+    state = torch.zeros({"recurrence": (2, 8), "convolution": (2, 3, 8), "scan": (2, 8, 4)}[kind])
+    over = {"recurrence": lambda: S.gated_recurrence(x, x, plan, state), "convolution": lambda: S.short_convolution(x, taps, None, plan, state), "scan": lambda: S.selective_scan(x, x, decay, b, b, plan, state)}[kind]
+    step = {"recurrence": lambda: S.gated_recurrence_step(one, one, state), "convolution": lambda: S.short_convolution_step(one, taps, None, state),
+            "scan": lambda: S.selective_scan_step(one, one, decay, b[:2], b[:2], state)}[kind]
+    y, _ = over()
+    torch.autograd.grad(y.sum(), x)
+    y, _ = over()
+    step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y.sum(), x)
+    with torch.inference_mode():                            # where nothing is counted
+        state = torch.zeros_like(state)
+        step()

@@ -88,13 +88,17 @@ class SelectiveLayer(Layer):
 
     def remember(self, x, episodes, states):
         x, gate = self.inputs(x)
-        x, _ = sequence.short_convolution(x, self.taps, self.taps_bias, episodes, states[0], silu=True)
+        first = None if states[0] is None else states[0].to(x.dtype)        # the convolution's state has its inputs' type, which autocast may have made 16 bits
+        x, _ = sequence.short_convolution(x, self.taps, self.taps_bias, episodes, first, silu=True)
         y, _ = sequence.selective_scan(x, *self._selected(x), episodes, states[1], self.skip, gate, self.rates_bias)
         return self.recurrence_out(y)
 
     def remember_step(self, x, states, fresh):
         x, gate = self.inputs(x)
-        x = sequence.short_convolution_step(x, self.taps, self.taps_bias, states[0], fresh, silu=True)
+        kept = states[0].to(x.dtype)
+        x = sequence.short_convolution_step(x, self.taps, self.taps_bias, kept, fresh, silu=True)
+        if kept is not states[0]:
+            states[0].copy_(kept)
         return self.recurrence_out(sequence.selective_scan_step(x, *self._selected(x), states[1], fresh, self.skip, gate, self.rates_bias))
 
 

@@ -1,10 +1,10 @@
-"""Calls of the selective operators at the ends of what they take: no channels, and sums over many tokens."""
+"""Calls of the selective operators at the ends of what they take: no channels, sums over many tokens, and a policy whose layers are worked out in 16 bits."""
 import numpy as np
 import pytest
 
 torch = pytest.importorskip("torch")
 import nuka  # noqa: E402,F401
-from nuka import sequence as S  # noqa: E402
+from nuka import memory_policy as M, sequence as S  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -92,3 +92,27 @@ def test_the_convolutions_weights_gradients_of_many_tokens():
     for got, count in [(db, tokens), *((dw[:, j], tokens - width + 1 + j) for j in range(width))]:          # inputs before the episode are 0
         off = (got.double() - ds * count).abs() - loss * count
         assert off.max().item() <= 0, f"off by {((got.double() - ds * count).abs() / (ds * count).abs()).max().item():.3e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("states", [0, 16])
+def test_a_policy_under_autocast(dtype, states):
+    """Both kinds of layer, over two rollouts: acting and training are one policy, and it has gradients.  A layer has eight results that are rounded to 16 bits (inputs, taps, rates, scan, products, scores, attention,
+    its product) and there are two: where both forms' values of about 1 fall on different sides each time, actions are 16 x 2^-8 apart."""
+    torch.manual_seed(states)
+    envs, steps = 5, 11
+    policy = M.MemoryPolicy(12, 3, width=128, heads=4, kv_heads=2, history=16, states=states, sinks=2).cuda()
+    memory, fresh = M.Memory(policy, envs, "cuda"), None
+    with torch.autocast("cuda", dtype=dtype):
+        for _ in range(2):
+            obs, done = torch.randn(envs, steps, 12, device="cuda"), torch.rand(envs, steps, device="cuda") < 0.2
+            first = [s if fresh is None else s.masked_fill(fresh.view(-1, *[1] * (s.dim() - 1)), 0.0) for s in memory.begin_rollout()]
+            acted = []
+            for t in range(steps):
+                acted.append(policy.act(obs[:, t], memory, fresh)[0].float())
+                fresh = done[:, t]
+            mean, value = policy(obs, done, first)
+            assert mean.dtype == dtype and all(s.dtype == torch.float32 for s in memory.states)
+            assert (torch.stack(acted, 1) - mean.float()).abs().max().item() <= 16 * 2.0 ** -8 * max(1.0, mean.abs().max().item())
+    (mean.float().square().sum() + value.float().sum()).backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in policy.parameters() if p is not policy.log_std)

@@ -1,8 +1,9 @@
 """A policy with memory over ``nuka.vec_env.NukaVecEnv``: what ``nuka.sequence`` is for, in one small model.
 
 A layer is a gated linear recurrence, which remembers for as long as it likes in a state of fixed size, and attention over the last ``history`` control
-steps, which remembers those exactly, and with ``sinks`` an episode's first ones beside them. With ``states`` a selective scan behind a short convolution takes the recurrence's place: as many values of state a
-channel, and rates, inputs and outputs that depend on the token. The policy acts token by token (``act``, on a ``Memory``) and trains on whole rollouts (calling it), with the
+steps, which remembers those exactly. With ``sinks`` some of the ``history`` are the first control steps that it has of an episode, beside the last ones: histories begin anew with every rollout, in which a policy
+trains, so those are the episode's own first steps where it began in the rollout, else the rollout's first ones, and a rollout of no more than ``history`` - ``sinks`` steps is all seen anyway. With ``states`` a selective
+scan behind a short convolution takes the recurrence's place: as many values of state a channel, and rates, inputs and outputs that depend on the token. The policy acts token by token (``act``, on a ``Memory``) and trains on whole rollouts (calling it), with the
 same result; episodes end at any control step of any env.
 
     python -m nuka.memory_policy [--envs 1024] [--steps 24] [--rollouts 20] [--states 0] [--sinks 0]

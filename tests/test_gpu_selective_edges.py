@@ -116,3 +116,19 @@ def test_a_policy_under_autocast(dtype, states):
             assert (torch.stack(acted, 1) - mean.float()).abs().max().item() <= 16 * 2.0 ** -8 * max(1.0, mean.abs().max().item())
     (mean.float().square().sum() + value.float().sum()).backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in policy.parameters() if p is not policy.log_std)
+
+
+def test_histories_begin_anew_with_a_rollout():
+    """First control steps that stay are those of the rollout's part of an episode: of a rollout before only the states go on."""
+    torch.manual_seed(1)
+    policy = M.MemoryPolicy(12, 3, width=64, heads=2, kv_heads=1, history=8, states=4, sinks=3).cuda()
+    obs, outs = torch.randn(4, 20, 12, device="cuda"), []
+    for before in (0, 5, 13):
+        memory = M.Memory(policy, 4, "cuda")
+        for t in range(before):
+            policy.act(-obs[:, t], memory)
+        memory.begin_rollout()
+        for state in memory.states:
+            state.zero_()
+        outs.append(torch.stack([policy.act(obs[:, t], memory)[0] for t in range(20)]))
+    assert torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])

@@ -479,7 +479,8 @@ def selective_scan(x, delta, decay, b, c, episodes, initial=None, skip=None, gat
 
     x, delta, gate: tokens x channels, f32, f16 or bf16.  b, c: tokens x states, of x's type; all at any stride (views of projections).  decay: channels x states float32, 1 to 64 states, below 0 where
     a state fades.  skip, delta_bias: channels float32, or None.  initial: rows x channels x states float32, the state that each row begins with, None for 0; an episode that begins inside a row
-    begins with 0.  Returns (y, state): y like x, state like initial, what each row ends with.  Rates, states and sums are in 32 bits, exponentials are off by up to 2^-22 of themselves. Where a gradient may
+    begins with 0.  Returns (y, state): y like x, state like initial, what each row ends with.  Rates, states and sums are in 32 bits; exp(dt decay) is off by up to 2^-22 (1 + |dt decay|) of itself, as its argument is rounded
+    to 32 bits, and 0 below 2^-126. Where a gradient may
     be asked for, the states before each fourth or eighth token are kept (at 16 states 8 bytes for each value of x)."""
     device = _on_gpu(x, delta, decay, b, c, initial, skip, gate, delta_bias, episodes._plan)
     _tokens_of(x, episodes, 2, "x")

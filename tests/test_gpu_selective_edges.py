@@ -132,3 +132,23 @@ def test_histories_begin_anew_with_a_rollout():
             state.zero_()
         outs.append(torch.stack([policy.act(obs[:, t], memory)[0] for t in range(20)]))
     assert torch.equal(outs[1], outs[0]) and torch.equal(outs[2], outs[0])
+
+
+@pytest.mark.parametrize("size", [2.0, 16.0, 60.0, 80.0])
+@pytest.mark.parametrize("states", [8, 16, 64])
+def test_exponentials_of_large_arguments(size, states):
+    """What a state of 1 fades to, forwards, as a gradient and in a step.  The argument is a product of three factors, dt, decay and log2(e), the last off by 2^-26 of itself, two products rounded by 2^-24 each: 2.3 x 2^-24 of it
+    in all, and dt itself, above 20, by half a unit; the exponential is off by as much as its argument, and by the instruction's own 2^-22: below 2^-22 (1 + |dt decay|)."""
+    channels, dt = 512, 24.0
+    decay = -torch.linspace(size / 16, size, channels * states, device="cuda").view(channels, states) / dt
+    plan, none, narrow = _rows_of(1), torch.zeros(1, channels, device="cuda"), torch.zeros(1, states, device="cuda")
+    first = torch.ones(1, channels, states, device="cuda", requires_grad=True)
+    _, state = S.selective_scan(none, none + dt, decay, narrow, narrow, plan, first)
+    back, = torch.autograd.grad(state, first, torch.ones_like(state))
+    stepped = torch.ones(1, channels, states, device="cuda")
+    S.selective_scan_step(none, none + dt, decay, narrow, narrow, stepped)
+    argument = decay.double() * np.logaddexp(dt, 0.0)
+    want = argument.exp()
+    for what, got in (("state", state.detach()), ("gradient", back), ("step", stepped)):
+        off = (got[0].double() - want).abs() / want - 2.0 ** -22 * (1 + argument.abs())
+        assert off.max().item() <= 0, what

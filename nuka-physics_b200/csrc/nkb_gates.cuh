@@ -10,7 +10,7 @@ template <bool EXACT> __device__ __forceinline__ Fading fading(float u) {
     const float a = fminf(fabsf(u), 100.f), t = a * -1.4426950408889634f;
     Fading f;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(f.e) : "f"(t));
-    if (EXACT) f.e = fmaf(f.e, fmaf(a, -1.4426950408889634f, -t) * 0.6931471805599453f + a * -1.3352e-8f, f.e);       // the last: log2(e)'s own rounding, 1.9263e-8, times ln(2)
+    if (EXACT) f.e = fmaf(f.e, fmaf(a, -1.4426950408889634f, -t) * 0.6931471805599453f + a * -1.33498e-8f, f.e);       // the last: what log2(e) lost, 1.92596e-8, times ln(2)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(f.r) : "f"(1.f + f.e));
     return f;
 }
@@ -90,7 +90,7 @@ template <int N> __device__ __forceinline__ void softplus_all(const float (&u)[N
             const Pair a = pair_of(fminf(fabsf(u[k]), 100.f), fminf(fabsf(u[k + 1]), 100.f)), t = mul_pair(a, both(1.4426950408889634f));
             split(t, x, y);
             Pair e = pair_of(exp2_fast(-x), exp2_fast(-y));
-            e = fma_pair(e, fma_pair(fma_pair(a, both(-1.4426950408889634f), t), both(0.6931471805599453f), mul_pair(a, both(-1.3352e-8f))), e);
+            e = fma_pair(e, fma_pair(fma_pair(a, both(-1.4426950408889634f), t), both(0.6931471805599453f), mul_pair(a, both(-1.33498e-8f))), e);
             if (slope != nullptr) {
                 split(add_pair(e, both(1.f)), x, y);
                 const Pair r = pair_of(inverse_of(x), inverse_of(y));

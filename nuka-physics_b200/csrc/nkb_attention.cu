@@ -56,7 +56,7 @@ struct AttentionParams {
     void *out, *dq, *dk, *dv;
     const void* dout;
     float *lse, *delta;
-    FarSinks far;                                       // slots 0: the keys' kernel goes through all queries of its sinks itself
+    FarSinks far;                                       // slots 0: none
 };
 
 __device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
@@ -971,18 +971,19 @@ template <int DP> struct Keys {
 // A tile of keys and a key head; the longest of one long row are the first ones.
 template <bool SINKS> struct KeyJob {
     int j0, last, head, end, first;                     // keys j0 to last; end, first: the plan's, of the last
+    bool shared;                                        // the last key's sinks have their far queries elsewhere
     __device__ __forceinline__ KeyJob(const AttentionParams& p, int job) {
         const int tile = job / p.heads_k;
         head = job - tile * p.heads_k;
         j0 = tile * p.span;
         last = (int)min((int64_t)j0 + p.span, p.tokens) - 1;
         end = p.end[last];
-        if (SINKS) first = p.first[last];
+        if (SINKS) { first = p.first[last]; shared = p.far.slots > 0 && p.far.slot_of[tile] >= 0; }
     }
     __device__ __forceinline__ int begin() const { return j0 & ~3; }               // of its queries: a multiple of 16 bytes of their statistics
     // behind the last query that sees one of the keys: sinks of the last key's episode are seen to its end, by queries of which another kernel may have the far ones
     __device__ __forceinline__ int past(const AttentionParams& p) const {
-        return p.window > 0 && !(SINKS && p.far.slots == 0 && j0 - first < p.sinks) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
+        return p.window > 0 && !(SINKS && !shared && j0 - first < p.sinks) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
     }
     __device__ __forceinline__ int steps(const AttentionParams& p) const { return (past(p) - 1 - begin()) / kStream + 1; }            // for one head
 };

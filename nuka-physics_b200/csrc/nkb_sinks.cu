@@ -45,7 +45,7 @@ __global__ void __launch_bounds__(1024) far_plan_kernel(const FarParams p) {
         bool is = false;
         if (tile < p.tiles) {
             const FarRange r = far_range(p, tile);
-            is = r.count > 0 && r.from < r.past;
+            is = r.count > 0 && r.past - r.from >= p.far.least;
         }
         const uint32_t which = __ballot_sync(~0u, is);
         if (lane == 0) part[warp] = __popc(which);
@@ -201,15 +201,18 @@ __global__ void __launch_bounds__(256) far_join_kernel(const FarSinks far, int w
     *reinterpret_cast<float4*>(to) = sum;
 }
 
-// Sinks that are worth it; with more, the keys' kernel has all queries of its sinks. Each eight read the far queries once more, which pays where those are many. All gradients, 8 heads, 2 of keys, with 4, 16, 32 and 64
-// sinks: one episode of 16384, dim 64, window 256: 153 to 181 us here, 1630 to 1555 there; dim 128, window 1024: 409 to 460 and 753 to 707; 40 episodes of 500, dim 64, window 64: 128, 138, 157 and 183, and 145 to 147.
-static int64_t most_sinks(const nuka_b200_episodes_t& e) { return e.tokens / std::max<int64_t>(e.rows, 1) >= 1024 ? 64 : 16; }
+// Far queries that a tile must have for its sinks to be worked out here, else the keys' kernel has all queries of its sinks: there a job is as long as the longest of them, here each eight sinks read all far queries once
+// more. Up to 16 sinks a step of that kernel is enough, with more only those of long rows are worth it. Whole training steps in us, 8 heads, 2 of keys, dim 64, with 16, 32 and 64 sinks, here and there: one episode of 16384,
+// window 256, 165, 175 and 196, and 1600; the same among twenty of 50 tokens 174, 188 and 220, and 1770; 8 of 4000, window 128, 214, 231 and 301, and 570; 40 of 500, window 64, 149 here, 169 and 174 there; 4096 of 24, window 8, 4 sinks, 390 here and 370 there; dim 128, 16384, window 1024, 473, 493 and 532, and 790. With more than 64 sinks always there.
+constexpr int64_t kMostSinks = 64, kFewSinks = 16, kFewFar = 64, kManyFar = 1024;
+static int64_t far_least(int64_t sinks) { return sinks <= kFewSinks ? kFewFar : kManyFar; }
 
-// Slots at most: tiles whose last key's episode is longer than the window and has sinks in the tile.
+// Slots at most: tiles whose last key's episode is so much longer than the window and has sinks in the tile.
 static int64_t far_slots(const nuka_b200_attention_t& d, int64_t sinks, int span, int tiles) {
     const nuka_b200_episodes_t& e = *d.plan;
-    if (sinks > most_sinks(e) || (e.length > 0 && (span % e.length == 0 || d.window >= e.length))) return 0;       // a tile's rows are whole, or no longer than the window
-    const int64_t episodes = std::min(e.tokens / (d.window + 1), e.length == 0 ? e.rows : e.tokens);
+    const int64_t reach = std::min(d.window, e.tokens) + far_least(sinks);      // tokens of such an episode, at least
+    if (sinks > kMostSinks || (e.length > 0 && (span % e.length == 0 || reach > e.length))) return 0;         // a tile's rows are whole, or too short
+    const int64_t episodes = std::min(e.tokens / reach, e.length == 0 ? e.rows : e.tokens);
     return std::min<int64_t>(tiles, episodes * 2);      // fewer sinks than a tile has keys lie in two tiles at most
 }
 // As many jobs as there may be slots for, and room to split them where the GPU has more places.
@@ -225,6 +228,7 @@ uint64_t far_sinks_bytes(const nuka_b200_attention_t& d, int64_t sinks, int span
 FarSinks far_sinks(const nuka_b200_attention_t& d, int64_t sinks, int span, int tiles, void* workspace) {
     FarSinks f;
     f.slots = (int)far_slots(d, sinks, span, tiles);
+    f.least = (int)far_least(sinks);
     if (f.slots == 0) return f;
     f.groups = (int)((sinks + kSinkRows - 1) / kSinkRows);
     f.heads_k = (int)d.heads_k;

@@ -23,9 +23,9 @@ struct FarRow {
     }
 };
 
-// A tile of keys has far queries where its last key's episode has sinks in it and goes on behind what the window reaches; such tiles have a slot.
+// A tile of keys has far queries where its last key's episode has sinks in it and goes on behind what the window reaches; tiles with `least` of them have a slot, the keys' kernel works out the others itself.
 struct FarSinks {
-    int slots = 0, groups = 0, heads_k = 0;             // slots: at most; groups: of kSinkRows sinks
+    int slots = 0, groups = 0, heads_k = 0, least = 1;             // slots: at most; groups: of kSinkRows sinks
     int64_t jobs = 0;                                   // there is room for, slots x groups x heads_k or more
     int32_t *slot_of = nullptr, *tile_of = nullptr, *count = nullptr;           // of tiles, of slots, and how many; behind it into how many parts each one's far queries are split
     float* sums = nullptr;                              // slots x groups x heads_k x splits x 2 x kSinkRows x DP: of keys, then values, not scaled; the splits joined in the first

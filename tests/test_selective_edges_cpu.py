@@ -42,3 +42,17 @@ def test_a_state_that_was_stepped_on_has_no_gradients_of_what_it_was(kind, monke
     with torch.inference_mode():                            # where nothing is counted
         state = torch.zeros_like(state)
         step()
+
+
+def test_far_queries_of_one_long_row_among_short_ones():
+    """Sinks of long rows have their far queries worked out apart, however short the rows beside them are on average; those of short rows only where there are few sinks."""
+    lib = _abi.lib()
+    ok = dict(dtype=2, heads_q=8, heads_k=2, dim=64, window=256, scale=0.125)
+    need = lambda sinks, **plan: lib.nuka_b200_attention_sinks_workspace(ctypes.byref(_abi.AttentionDesc(**{**ok, "plan": _plan(**plan)})), sinks)
+    for sinks in (4, 16, 17, 64):
+        assert need(sinks, tokens=17384, rows=21, length=0) > 0, sinks
+        assert need(sinks, tokens=20000, rows=5, length=4000) > 0 and need(sinks, tokens=16384, rows=1, length=0) > 0
+        assert (need(sinks, tokens=20000, rows=40, length=500) > 0) == (sinks <= 16)
+    assert need(65, tokens=16384, rows=1, length=0) == 0
+    ok["window"] = 2 ** 63 - 1                              # without end
+    assert need(4, tokens=16384, rows=1, length=0) == 0

@@ -45,7 +45,7 @@ struct ScanParams {
     int64_t channels, states, x_stride, delta_stride, gate_stride, b_stride, c_stride, segment, segments, chunks;           // chunks: of a segment
     uint32_t tiles, workers;                            // of the channels; warps of a tile backwards
     bool alone;                                         // every segment is whole rows
-    bool wide, wide_states;                             // a lane's loads and stores of a chunk go in one piece; those of states two at a time
+    bool wide, wide_narrow, wide_states;                // a lane's loads and stores of a chunk go in one piece: of channels, and of B and C; those of states two at a time
     const void *x, *delta, *gate, *b, *c, *dy;
     const float *decay, *skip, *delta_bias, *initial, *dstate;
     void *y, *dx, *ddelta, *dgate;
@@ -296,7 +296,7 @@ template <typename T, int LN> struct ScanLane {
         v.load(static_cast<const T*>(from) + (t0 + token) * stride + c0 + channel, token < left ? own : 0, p.wide);
     }
     __device__ __forceinline__ void load_narrow(const ScanParams& p, const void* from, int64_t stride, int64_t t0, int left, Narrow& v) const {
-        v.load(static_cast<const T*>(from) + (t0 + narrow_token) * stride + narrow_state, narrow_token < left ? narrow_own : 0, p.wide);
+        v.load(static_cast<const T*>(from) + (t0 + narrow_token) * stride + narrow_state, narrow_token < left ? narrow_own : 0, p.wide_narrow);
     }
     __device__ __forceinline__ void store(const ScanParams& p, void* to, int64_t t0, int left, const float (&v)[S::kEach]) const {
         Each::store(static_cast<T*>(to) + (t0 + token) * p.channels + c0 + channel, v, token < left ? own : 0, p.wide);
@@ -979,7 +979,8 @@ template <typename T, int LN> static cudaError_t run_scan(const nuka_b200_scan_t
     using S = ScanTile<LN>;
     auto lies = [](const void* at, uint64_t on) { return reinterpret_cast<uintptr_t>(at) % on == 0u; };
     constexpr uint64_t EACH = std::min<uint64_t>(16, S::kEach * sizeof(T)), NARROW = std::min<uint64_t>(16, S::kNarrow * sizeof(T));
-    p.wide = d.channels % S::kEach == 0 && d.states % S::kNarrow == 0 && d.b_stride % S::kNarrow == 0 && d.c_stride % S::kNarrow == 0 && lies(d.b, NARROW) && lies(d.c, NARROW);
+    p.wide_narrow = d.states % S::kNarrow == 0 && d.b_stride % S::kNarrow == 0 && d.c_stride % S::kNarrow == 0 && lies(d.b, NARROW) && lies(d.c, NARROW);
+    p.wide = d.channels % S::kEach == 0;
     for (int64_t stride : {d.x_stride, d.delta_stride, d.gate_stride}) p.wide = p.wide && stride % S::kEach == 0;
     for (const void* at : {d.x, d.delta, d.gate, static_cast<const void*>(d.y)}) p.wide = p.wide && lies(at, EACH);
     if (backward)

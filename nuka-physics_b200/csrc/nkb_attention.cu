@@ -31,6 +31,7 @@
 // mostly mask, so there neither the bytes nor the products are near their limits.
 #include <cuda_runtime.h>
 #include <algorithm>
+#include <type_traits>
 #include "nkb_sequence.cuh"
 #include "nkb_sequence.h"
 #include "nkb_sinks.cuh"
@@ -46,7 +47,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 struct AttentionParams {
     const int32_t *first, *end;
     int64_t tokens, pitch;                              // pitch: floats between the heads' rows of lse and delta
-    int heads_q, heads_k, dim, window, sinks;           // window 0: all of the episode; sinks: first tokens of an episode that stay visible, only with a window
+    int heads_q, heads_k, dim, window;                  // window 0: all of the episode
     int span, tiles;                                    // tokens of a tile, at most 128, and how many tiles
     int split;                                          // blocks of a key job, a cluster, each with an equal share of the group's heads
     int by_heads, across, along;                        // of the forward kernel's jobs: tiles of two heads or of two stretches of tokens; jobs side by side, and behind one another
@@ -56,8 +57,13 @@ struct AttentionParams {
     void *out, *dq, *dk, *dv;
     const void* dout;
     float *lse, *delta;
-    FarSinks far;                                       // slots 0: none
 };
+// What the kernels with first tokens that stay visible have beside that. Others are not handed it: the gradients' kernels copy what they are handed to each thread's stack.
+struct SinkParams : AttentionParams { int sinks; };
+template <bool SINKS> using ParamsOf = std::conditional_t<SINKS, SinkParams, AttentionParams>;
+template <bool SINKS> __device__ __forceinline__ int sinks_of(const AttentionParams& p) {
+    if constexpr (SINKS) return static_cast<const SinkParams&>(p).sinks; else return 0;
+}
 
 __device__ __forceinline__ float nan_value() { return __uint_as_float(0x7fffffffu); }
 
@@ -68,7 +74,7 @@ template <bool SINKS> struct KeySteps {
     __device__ __forceinline__ KeySteps(const AttentionParams& p, int first, int i0, int last, int step) {
         near = p.window > 0 ? max(first, i0 - p.window + 1) : first;
         far = first;
-        far_end = SINKS ? first + min(p.sinks, near - first) : first;
+        far_end = SINKS ? first + min(sinks_of<SINKS>(p), near - first) : first;
         far_steps = SINKS ? (far_end - far + step - 1) / step : 0;
         count = (last - near) / step + 1 + far_steps;
     }
@@ -87,7 +93,7 @@ template <bool SINKS> struct RowKeys {
         all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff); all_high = __reduce_min_sync(~0u, high);
         if (SINKS) {
             first = live ? episode : 0;
-            sink = live ? episode + min(p.sinks - 1, i - episode) : -1;
+            sink = live ? episode + min(sinks_of<SINKS>(p) - 1, i - episode) : -1;
             any_first = __reduce_min_sync(~0u, live ? episode : 0x7fffffff); any_sink = __reduce_max_sync(~0u, sink);
         }
     }
@@ -220,11 +226,11 @@ template <typename T> __device__ __forceinline__ const T* key_row(const Attentio
 template <typename T> __device__ __forceinline__ const T* value_row(const AttentionParams& p, int j, int head) { return static_cast<const T*>(p.v) + j * p.v_stride + head * p.v_head_stride; }
 template <typename T> __device__ __forceinline__ const T* dout_row(const AttentionParams& p, int i, int head) { return static_cast<const T*>(p.dout) + ((int64_t)i * p.heads_q + head) * p.dim; }
 __device__ __forceinline__ int first_key(const AttentionParams& p, int i) { return p.window > 0 ? max(p.first[i], i - p.window + 1) : p.first[i]; }
-template <bool SINKS> __device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 && !(SINKS && j - p.first[j] < p.sinks) ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
+template <bool SINKS> __device__ __forceinline__ int past_query(const AttentionParams& p, int j) { return p.window > 0 && !(SINKS && j - p.first[j] < sinks_of<SINKS>(p)) ? (int)min((int64_t)p.end[j], (int64_t)j + p.window) : p.end[j]; }
 // The keys that query i sees, in one range or, its sinks first, in two.
 template <bool SINKS, typename Use> __device__ __forceinline__ void each_range(const AttentionParams& p, int i, Use use) {
     const int low = first_key(p, i);
-    if (SINKS && p.first[i] < low) use(p.first[i], p.first[i] + min(p.sinks, low - p.first[i]) - 1);
+    if (SINKS && p.first[i] < low) use(p.first[i], p.first[i] + min(sinks_of<SINKS>(p), low - p.first[i]) - 1);
     use(low, i);
 }
 
@@ -390,7 +396,7 @@ struct ForwardJob {
 
 template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                const __grid_constant__ CUtensorMap map_o, const __grid_constant__ AttentionParams p) {
+                                                                const __grid_constant__ CUtensorMap map_o, const __grid_constant__ ParamsOf<SINKS> p) {
     using F = Forward<DP>;
     __shared__ uint64_t q_full[F::kQueries], q_empty[F::kQueries], k_full[F::kStages], k_empty[F::kStages], v_full[F::kStages], v_empty[F::kStages];
     __shared__ uint64_t s_full[2], s_empty[2], p_full[2], o_done[2], ended[2];
@@ -706,7 +712,7 @@ template <int DP> struct Queries {
 template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) query_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_o,
                                                                const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dq,
-                                                               const __grid_constant__ AttentionParams p) {
+                                                               const ParamsOf<SINKS> p) {
     using F = Queries<DP>;
     __shared__ uint64_t q_full, q_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], s_empty[F::kBuffers], p_full, o_done, ended;
     __shared__ uint32_t tensor;
@@ -836,9 +842,10 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             const QueryJob now = next;
             const int i = now.i0 + row;
             const KeySteps<SINKS> through = now.steps<SINKS>(p);
-            const RowKeys<SINKS> sees(p, i <= now.last, i, next_first);
+            const int episode = next_first;
             const float lse = next_lse;
             if (job + stride < jobs) { next = QueryJob(p, job + stride); next_first = first_of(next); next_lse = lse_of(next); }
+            const RowKeys<SINKS> sees(p, i <= now.last, i, episode);
             // D = dO . O of the thread's row.  O has the error of its own rounding and of P's, which the sum of dS over the row, 0 by definition, shows: the keys' kernel, which runs
             // after this one, gets D without it. Where a step holds all keys of a row D is summed from its own P and dP before dS, which matters where few keys share a row (dq of
             // 24-token episodes was off by 1.8 times its rounding; with many keys the error averages out).
@@ -972,18 +979,18 @@ template <int DP> struct Keys {
 template <bool SINKS> struct KeyJob {
     int j0, last, head, end, first;                     // keys j0 to last; end, first: the plan's, of the last
     bool shared;                                        // the last key's sinks have their far queries elsewhere
-    __device__ __forceinline__ KeyJob(const AttentionParams& p, int job) {
+    __device__ __forceinline__ KeyJob(const AttentionParams& p, const FarSinks& far, int job) {
         const int tile = job / p.heads_k;
         head = job - tile * p.heads_k;
         j0 = tile * p.span;
         last = (int)min((int64_t)j0 + p.span, p.tokens) - 1;
         end = p.end[last];
-        if (SINKS) { first = p.first[last]; shared = p.far.slots > 0 && p.far.slot_of[tile] >= 0; }
+        if (SINKS) { first = p.first[last]; shared = far.slots > 0 && far.slot_of[tile] >= 0; }
     }
     __device__ __forceinline__ int begin() const { return j0 & ~3; }               // of its queries: a multiple of 16 bytes of their statistics
     // behind the last query that sees one of the keys: sinks of the last key's episode are seen to its end, by queries of which another kernel may have the far ones
     __device__ __forceinline__ int past(const AttentionParams& p) const {
-        return p.window > 0 && !(SINKS && !shared && j0 - first < p.sinks) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
+        return p.window > 0 && !(SINKS && !shared && j0 - first < sinks_of<SINKS>(p)) ? (int)min((int64_t)end, (int64_t)last + p.window) : end;
     }
     __device__ __forceinline__ int steps(const AttentionParams& p) const { return (past(p) - 1 - begin()) / kStream + 1; }            // for one head
 };
@@ -1008,7 +1015,7 @@ template <int DP, int THREADS> __device__ __noinline__ void clear_hidden(int fro
 template <typename T, int DP, bool SINKS>
 __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_grad_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const __grid_constant__ CUtensorMap map_k,
                                                                             const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_dk,
-                                                                            const __grid_constant__ CUtensorMap map_dv, const __grid_constant__ AttentionParams p) {
+                                                                            const __grid_constant__ CUtensorMap map_dv, const ParamsOf<SINKS> p, const __grid_constant__ FarSinks far) {
     using F = Keys<DP>;
     __shared__ uint64_t k_full, k_empty, full[F::kStages], empty[F::kStages], s_full[F::kBuffers], p_full, o_done, ended;
     __shared__ __align__(16) float lse[F::kStages][kStream], delta[F::kStages][kStream];
@@ -1040,10 +1047,10 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         if (lane == 0) {
             int steps = 0, keys = 0;                    // loads begun so far
             bool fine = true;
-            KeyJob<SINKS> next(p, job0);
+            KeyJob<SINKS> next(p, far, job0);
             for (int job = job0; fine && job < jobs; job += stride) {
                 const KeyJob<SINKS> now = next;
-                if (job + stride < jobs) next = KeyJob<SINKS>(p, job + stride);
+                if (job + stride < jobs) next = KeyJob<SINKS>(p, far, job + stride);
                 if (keys > 0 && !(fine = barrier_wait(&k_empty, (keys - 1) & 1, &lost))) break;
                 barrier_expect(&k_full, 2 * F::kTile);
                 load_panels<kRows, DP>(shared, &map_k, &k_full, now.head, now.j0);
@@ -1067,11 +1074,11 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         }
     } else if (warp == 5) {
         int job = job0, j = 0, count = 0, ahead = 0, keys = 0, stage = 0, phase = 0;         // of the scores
-        KeyJob<SINKS> next(p, job);
+        KeyJob<SINKS> next(p, far, job);
         auto scores = [&]() {
             if (j == 0) {
                 count = __shfl_sync(~0u, next.steps(p) * group, 0);
-                if (job + stride < jobs) next = KeyJob<SINKS>(p, job + stride);
+                if (job + stride < jobs) next = KeyJob<SINKS>(p, far, job + stride);
                 if (!warp_wait(&k_full, keys & 1, &lost)) return false;
             }
             if (!warp_wait(&full[stage], phase, &lost)) return false;
@@ -1090,7 +1097,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         bool fine = scores();
         for (int own = job0; fine && own < jobs; own += stride) {
             const int steps = count;                    // of the job that the scores have just begun
-            const KeyJob<SINKS> now(p, own);
+            const KeyJob<SINKS> now(p, far, own);
             const int each = steps / group;
             for (int i = 0, m = 0; i < steps; ++i, ++n) {
                 // the other buffer's P and dS are free when the products before have ended
@@ -1133,7 +1140,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
             const bool there = j <= leaving.last;
             FarRow more[2];                             // of the key's gradient and the value's
             if (SINKS && there && rank == 0)
-                for (int which = 0; which < 2; ++which) more[which] = p.far.row_of(leaving.first / p.span, j - max(leaving.first, p.first[leaving.last]), leaving.head, which, DP);
+                for (int which = 0; which < 2; ++which) more[which] = far.row_of(leaving.first / p.span, j - max(leaving.first, p.first[leaving.last]), leaving.head, which, DP);
             if (p.split > 1) {
                 // in 32 bits where the operands were, 16 bytes at a time, rows turned against each other so that lanes meet different banks
 #pragma unroll
@@ -1169,9 +1176,9 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
                 if (there && !finite) spoilt = 1;
             }
         };
-        KeyJob<SINKS> next(p, job0);
+        KeyJob<SINKS> next(p, far, job0);
         auto end_of = [&](const KeyJob<SINKS>& job) { return p.end[min(job.j0 + row, job.last)]; };
-        auto sink_of = [&](const KeyJob<SINKS>& job) { const int j = min(job.j0 + row, job.last); return SINKS && j - p.first[j] < p.sinks; };
+        auto sink_of = [&](const KeyJob<SINKS>& job) { const int j = min(job.j0 + row, job.last); return SINKS && j - p.first[j] < sinks_of<SINKS>(p); };
         int next_end = end_of(next);
         bool next_sink = sink_of(next);
         const Pair scale2 = pair_of(p.scale2, p.scale2), minus_one = pair_of(-1.f, -1.f);
@@ -1181,7 +1188,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
             const bool live = j <= now.last;
             // the queries that see the key
             const int low = live ? j : 0, high = !live ? -1 : SINKS && next_sink ? min(next_end, now.past(p)) - 1 : (p.window > 0 ? (int)min((int64_t)next_end, (int64_t)j + p.window) : next_end) - 1;
-            if (job + stride < jobs) { next = KeyJob<SINKS>(p, job + stride); next_end = end_of(next); next_sink = sink_of(next); }
+            if (job + stride < jobs) { next = KeyJob<SINKS>(p, far, job + stride); next_end = end_of(next); next_sink = sink_of(next); }
             const int any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff), any_high = __reduce_max_sync(~0u, high);
             const int all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff), all_high = __reduce_min_sync(~0u, high);
             bool first = true, left = false;
@@ -1264,7 +1271,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         meet(1, F::kWorkers);
         if (p.split == 1 && spoilt != 0 && lost == 0)
             for (int job = job0; job < jobs; job += stride) {
-                const KeyJob<SINKS> done(p, job);
+                const KeyJob<SINKS> done(p, far, job);
                 for (int j = done.j0 + half * 4 + warp % 4; j <= done.last; j += F::kWorkers / 32)
                     for (int which = 0; which < 2; ++which) mend_key_grad<T, SINKS>(p, j, done.head, which, lane);
             }
@@ -1278,7 +1285,7 @@ __global__ void __launch_bounds__(Keys<DP>::kThreads, Keys<DP>::kBlocks) key_gra
         __syncwarp();
         cluster_meet();
         // each block takes its share of the rows of the cluster's one job
-        const KeyJob<SINKS> job(p, job0);
+        const KeyJob<SINKS> job(p, far, job0);
         const int rows = kRows / p.split;
         for (int x = threadIdx.x; x < 2 * rows * (DP / 4); x += F::kThreads) {
             const int which = x / (rows * (DP / 4)), row = rank * rows + x / (DP / 4) % rows, c = x % (DP / 4) * 4, j = job.j0 + row;
@@ -1335,10 +1342,11 @@ static int tile_span(const nuka_b200_episodes_t& plan) {
 template <typename K> static cudaError_t with_shared(K kernel, int bytes) { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes); }
 
 template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const nuka_b200_attention_t& d, int64_t sinks, void* workspace, bool backward, cudaStream_t stream) {
-    AttentionParams p{};
+    ParamsOf<SINKS> p{};
     const nuka_b200_episodes_t& e = *d.plan;
     p.first = e.first; p.end = e.end; p.tokens = e.tokens; p.pitch = attention_pitch(e.tokens);
-    p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens); p.sinks = (int)std::min(sinks, e.tokens);
+    p.heads_q = (int)d.heads_q; p.heads_k = (int)d.heads_k; p.dim = (int)d.dim; p.window = (int)std::min(d.window, e.tokens);
+    if constexpr (SINKS) p.sinks = (int)std::min(sinks, e.tokens);
     p.span = tile_span(e); p.tiles = (int)((e.tokens + p.span - 1) / p.span);
     p.by_heads = p.heads_q / p.heads_k % 2 == 0;
     p.across = p.by_heads ? p.heads_q / 2 : p.heads_q; p.along = p.by_heads ? p.tiles : (p.tiles + 1) / 2;
@@ -1358,7 +1366,8 @@ template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const
         attention_kernel<T, DP, SINKS><<<(unsigned)std::min(p.across * p.along, 148), kForward, Forward<DP>::kShared, stream>>>(q, k, v, o, p);
         return cudaGetLastError();
     }
-    if (SINKS) p.far = far_sinks(d, sinks, p.span, p.tiles, workspace);
+    FarSinks far;
+    if (SINKS) far = far_sinks(d, sinks, p.span, p.tiles, workspace);
     CUtensorMap dq, dk, dv;
     for (int keys = 0; keys < 2; ++keys) {
         const int own = keys ? kStream : kRows, other = keys ? kRows : kStream;
@@ -1375,12 +1384,12 @@ template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const
         const int64_t row = e.tokens / std::max<int64_t>(e.rows, 1), reach = d.window > 0 ? std::min<int64_t>(row, d.window) : row, places = reach >= 1024 ? 4 * slots : slots;
         p.split = 1;
         while (keys && p.split < 8 && group % (2 * p.split) == 0 && 2 * p.split * (int64_t)jobs <= places) p.split *= 2;
-        if (keys && p.far.slots > 0)
-            if (const cudaError_t far = launch_far_sinks(d, p.window, p.sinks, p.span, p.tiles, p.pitch, p.far, stream); far != cudaSuccess) return far;
+        if (keys && far.slots > 0)
+            if (const cudaError_t ran = launch_far_sinks(d, p.window, (int)std::min(sinks, e.tokens), p.span, p.tiles, p.pitch, far, stream); ran != cudaSuccess) return ran;
         if (!keys) {
             query_grad_kernel<T, DP, SINKS><<<(unsigned)blocks, Queries<DP>::kThreads, Queries<DP>::kShared, stream>>>(q, g, o, k, v, dq, p);
         } else if (p.split == 1) {
-            key_grad_kernel<T, DP, SINKS><<<(unsigned)blocks, Keys<DP>::kThreads, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p);
+            key_grad_kernel<T, DP, SINKS><<<(unsigned)blocks, Keys<DP>::kThreads, Keys<DP>::kShared, stream>>>(q, g, k, v, dk, dv, p, far);
         } else {
             cudaLaunchAttribute cluster{};
             cluster.id = cudaLaunchAttributeClusterDimension;
@@ -1388,7 +1397,7 @@ template <typename T, int DP, bool SINKS> static cudaError_t run_attention(const
             cudaLaunchConfig_t config{};
             config.gridDim = dim3((unsigned)(jobs * p.split)); config.blockDim = dim3(Keys<DP>::kThreads); config.dynamicSmemBytes = Keys<DP>::kShared; config.stream = stream;
             config.attrs = &cluster; config.numAttrs = 1u;
-            set = cudaLaunchKernelEx(&config, key_grad_kernel<T, DP, SINKS>, q, g, k, v, dk, dv, p);
+            set = cudaLaunchKernelEx(&config, key_grad_kernel<T, DP, SINKS>, q, g, k, v, dk, dv, p, far);
             if (set != cudaSuccess) return set;
         }
         set = cudaGetLastError();

@@ -944,12 +944,12 @@ struct ScanShape {
         lanes = scan_lanes(all_states); states = 4 * lanes; channels = 128 / lanes; chunk = scan_chunk(lanes);
         tiles = (all_channels + channels - 1) / channels;
         // rows of one length where they give every SM sixteen warps, or are so short that a second walk would cost more than the first (64 rows of 24 x 64 14 us whole and 23 cut, 16 of 48 x 512 21 and 27,
-        // 8 of 64 x 64 23 and 21); else equal shares for sixteen warps an SM, 16 tokens at least
+        // 8 of 64 x 64 23 and 21), of less than a chunk several together; else equal shares for sixteen warps an SM, 16 tokens at least
         const int64_t wanted = 16 * 148;
-        if (plan.length > 0 && (plan.length <= 64 || plan.rows * tiles >= wanted)) segment = plan.length;
+        if (plan.length > 0 && (plan.length <= 64 || plan.rows * tiles >= wanted)) segment = plan.length < 8 ? (15 + plan.length) / plan.length * plan.length : plan.length;
         else segment = plan.tokens <= 16 ? plan.tokens : std::max<int64_t>(16, (plan.tokens * tiles / wanted + 7) / 8 * 8);
         segments = (plan.tokens + segment - 1) / segment;
-        alone = plan.tokens <= segment || segment == plan.length;
+        alone = plan.tokens <= segment || (plan.length > 0 && segment % plan.length == 0);
         chunks = (segment + chunk - 1) / chunk;
         workers = std::max<int64_t>(1, std::min<int64_t>(segments, 8 * 148 / tiles));
     }

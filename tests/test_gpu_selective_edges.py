@@ -5,6 +5,7 @@ import pytest
 torch = pytest.importorskip("torch")
 import nuka  # noqa: E402,F401
 from nuka import memory_policy as M, sequence as S  # noqa: E402
+from test_gpu_selective import _check_scan, _done_plan  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +153,11 @@ def test_exponentials_of_large_arguments(size, states):
     for what, got in (("state", state.detach()), ("gradient", back), ("step", stepped)):
         off = (got[0].double() - want).abs() / want - 2.0 ** -22 * (1 + argument.abs())
         assert off.max().item() <= 0, what
+
+
+@pytest.mark.parametrize("length", [1, 2, 3, 5, 7])
+@pytest.mark.parametrize("states", [5, 16, 33])
+def test_rows_of_less_than_a_chunk(length, states):
+    """Several rows to a walk: each begins with its own initial state, and leaves its own."""
+    for rows, dtype in ((41, torch.bfloat16), (1, torch.float32), (23, torch.float16)):
+        _check_scan(_done_plan(rows, length, 0.2, seed=length), 37, states, dtype, seed=length)

@@ -56,3 +56,14 @@ def test_far_queries_of_one_long_row_among_short_ones():
     assert need(65, tokens=16384, rows=1, length=0) == 0
     ok["window"] = 2 ** 63 - 1                              # without end
     assert need(4, tokens=16384, rows=1, length=0) == 0
+
+
+@pytest.mark.parametrize("length", [1, 2, 3, 5, 7, 8, 15, 24, 64])
+@pytest.mark.parametrize("states", [8, 16, 64])
+def test_what_is_kept_for_short_rows(length, states):
+    """States before each fourth (up to 8 states) or eighth token, in 32 bits; chunks of tokens begin anew with rows of eight tokens and more, and with every sixteen or so of shorter ones."""
+    rows, channels, chunk = 840, 512, 4 if states == 8 else 8
+    kept = _abi.lib().nuka_b200_scan_kept(_plan(tokens=rows * length, rows=rows, length=length), channels, states)
+    together = length if length >= 8 else -(-16 // length) * length
+    assert kept == -(-rows * length // together) * -(-together // chunk) * channels * states * 4
+    assert kept <= 2 * rows * length * channels * states * 4 // chunk

@@ -11,7 +11,7 @@
 // The backward pass works the scores out twice, once for the queries' gradients and once for the keys': 7 products in place of 5, and in return no gradient is summed
 // through atomics, so that the same call gives the same bits, and the shared heads' sum stays in tensor memory.
 // With a window an episode's first tokens may stay visible (sinks): a tile of queries then goes through those of its first query's episode that lie before its keys, in steps of their own at the job's begin, and rows see two
-// ranges of keys, the window's and the sinks'; a second set of the kernels, so that what has no sinks is as it was. The keys' kernel leaves a sink's far queries to another (nkb_sinks.cu).
+// ranges of keys, the window's and the sinks'; a second set of the kernels, so that what has no sinks is as it was (queries' gradients 1 to 2 % slower, the others the same). The keys' kernel leaves a sink's far queries to another (nkb_sinks.cu).
 // Warps have roles: one or two load tiles by TMA, one or two issue products, four for each tile turn scores into probabilities, a row to a thread;
 // P and dS go back to tensor memory as the next product's operand in the inputs' type (their one rounding more; sums and statistics are in 32 bits).
 // One tile's products run under the other's exponentials: forwards the two are one block's, backwards those of two blocks on an SM, and with wide heads, of which one block fills an SM,
@@ -23,9 +23,9 @@
 //   98304 tokens in rows of 24, dim 64                         73 us      106        100        252 MB of inputs and outputs forwards: 3.4 TB/s
 //   20011 tokens in 40 episodes, dim 64                        61          71        115
 //   16384 tokens, one episode, dim 128                        435          --         --        550 GFLOP of visible pairs: 1.26 PFLOP/s
-//   40000 tokens in 4 episodes, dim 128                       790        1200       2315        1.04, 1.02 and 0.71 PFLOP/s of visible pairs
-//   20011 tokens in 40 episodes, dim 64, window 64, 4 sinks    35          39         61        and 21 for the far queries
-//   16384 tokens, one episode, dim 128, window 1024, 16 sinks 100         137        224        and 37
+//   40000 tokens in 4 episodes, dim 128                       790        1190       2313        1.04, 1.02 and 0.71 PFLOP/s of visible pairs
+//   20011 tokens in 40 episodes, dim 64, window 64, 4 sinks    35          39         60        and 21 for the far queries
+//   16384 tokens, one episode, dim 128, window 1024, 16 sinks  97         139        218        and 38
 // Long episodes are bound by the chain of a step, scores to exponentials to product, that each tile walks through: the tensor cores are busy for half of it.
 // Short rows are bound by the same chain once a tile, with its loads and its rows' way out around it: 128 rows see 24 keys each, and a tile's product is
 // mostly mask, so there neither the bytes nor the products are near their limits.

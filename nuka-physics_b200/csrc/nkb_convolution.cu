@@ -7,7 +7,7 @@
 // and the sums that become the gradients of the last K inputs travel with them; the walk goes K - 1 tokens past its stretch (as far as the episode does) to complete them.
 // Weights' gradients are summed in registers over all stretches of a thread, then over a block's warps, then over the blocks, always in the same order.
 //
-// Measured, K = 4 with silu: 4096 rows of 24 x 512, bf16, 52 us forwards (3.9 TB/s of its 2 tensors) and 87 back (3.5 TB/s of 3); 3 long rows, 131071 x 1024, f16, 113 us (4.8 TB/s) and 204 (3.9 TB/s).
+// Measured, K = 4 with silu: 4096 rows of 24 x 512, bf16, 51 us forwards (3.9 TB/s of its 2 tensors) and 86 back (3.5 TB/s of 3); 3 long rows, 131071 x 1024, f16, 112 us (4.8 TB/s) and 203 (4.0 TB/s); in f32 76, 135, 192 and 339. One token of 4096 envs x 512 22 us, in f32 15.
 // The loads of the next tokens, and the plan's marks of the next 32, are under way while these are walked: with marks asked for by the batch, 55, 103, 133 and 243 us. Instructions, 1.9 to 2.0 of 4 a cycle, are some 15 a value
 // forwards and 28 back, the exponentials' unit is busy for half of the time forwards and the multiplications' for 40 % back; 16 and 12 warps an SM is what the registers leave. More warps with four tokens ahead forwards: 52 and
 // 124; back, four blocks to an SM spill (109 and 242), eight tokens ahead too (100 and 259). Eight channels to a thread were slower both ways (fewer warps), two slower back; blocks that take walks in turn forwards the same.

@@ -8,14 +8,14 @@
 // go through one instruction.
 // It walks a segment of tokens, kChunk at a time: first what needs no state, eight values to a lane (rates, gates), into shared memory, then the states token by token, then the outputs, eight to a lane again.
 // Segments and maps are as in the gated recurrence: rows where they are short or many, else equal shares, walked once for what each does to the state, (exp(A sum dt), h), and a second time for the values.
-// For a gradient the states before each chunk are kept, in the lanes' order (at 16 states 8 bytes for each value of x); backwards a chunk's states are worked out again from them, into shared memory, and its tokens then
+// For a gradient the states before each chunk are kept, in the lanes' order (2048 bytes for each chunk and tile: at 16 states 8 bytes for each value of x where rows are multiples of 8 tokens and channels of 32); backwards a chunk's states are worked out again from them, into shared memory, and its tokens then
 // walked back. B's and C's gradients are sums over the channels: each tile leaves its own, in 32 bits, and a last kernel adds them up; so are A's and the other weights', by the warps' shares of the tokens. No atomics, every
 // order is fixed.
 //
-// Measured, bf16, 16 states: 4096 rows of 24 x 512 371 us forwards and 1122 back, 51 more for B's and C's sums; 3 long rows, 32749 x 1024, 174 for the maps, 15 for the scan over them and 221 for the values, back 190, 16, 703 and 36;
-// 1000 rows of 37 x 200, f32, 8 states 64 us; one token of 4096 envs x 512 63 us, 4.6 TB/s of its states.
-// Exponentials bound it from below: one for each value and state forwards, two back, and a few for rates and gates, sixteen a cycle and SM, that is 224 us of the 371 and 414 of the 1122; their unit is busy for 61 % and 37 % of the time, the multiplying ones
-// for 42 and 43 %. Forwards 16 warps share an SM, backwards 8 (226 KB of shared memory and all registers), which leaves each warp's own chain of instructions in view: 1.9 of 4 a cycle.
+// Measured, bf16, 16 states: 4096 rows of 24 x 512 370 us forwards and 1115 back, 51 more for B's and C's sums; 3 long rows, 32749 x 1024, 171 for the maps, 15 for the scan over them and 221 for the values, back 190, 17, 702 and 36;
+// the same in f32 448, 1155 and 52, and 170, 17, 254, 213, 17, 721 and 36 (kernels of 8 and 16 states spill up to 80 bytes there); 1000 rows of 37 x 200, f32, 8 states 64 us; one token of 4096 envs x 512 63 us, 4.6 TB/s of its states.
+// Exponentials bound it from below: one for each value and state forwards, two back, and a few for rates and gates, sixteen a cycle and SM, that is 224 us of the 370 and 414 of the 1115; their unit is busy for 61 % and 37 % of the time, the multiplying ones
+// for 42 and 43 %. Forwards 16 warps share an SM, backwards 8 (201 KB of shared memory, with f32 and 64 states 214, and all registers), which leaves each warp's own chain of instructions in view: 1.9 of 4 a cycle.
 #include <algorithm>
 #include "nkb_gates.cuh"
 #include "nkb_sequence.cuh"

@@ -6,8 +6,8 @@
 // The queries' bytes bound it, q and dO once for each eight sinks; what it takes is the chain of loads, scores, exponentials and products of sixteen queries, so a slot's queries and heads are dealt out over blocks and
 // their warps, as many as the slots leave places for, and the sums joined in a fixed order: a block's warps in shared memory, then the splits.
 //
-// Measured, bf16, 8 heads, 2 of keys: 20011 tokens in 40 episodes, dim 64, window 64, 4 sinks: 15 us, 3 each for the slots before and the join behind (keys' kernel 61; with all queries of its sinks 115);
-// 16384 tokens, one episode, dim 128, window 1024, 16 sinks: 30, 3 and 4 (keys' 224; 543). The second products' operands are the first ones', turned over by 8 x 8 in registers; loaded again in the other order they took 40 in place of 30.
+// Measured, bf16, 8 heads, 2 of keys: 20011 tokens in 40 episodes, dim 64, window 64, 4 sinks: 15 us, 3 each for the slots before and the join behind (keys' kernel 60; with all queries of its sinks 115);
+// 16384 tokens, one episode, dim 128, window 1024, 16 sinks: 30, 4 and 4 (keys' 218; 543). The second products' operands are the first ones', turned over by 8 x 8 in registers; loaded again in the other order they took 40 in place of 30.
 #include <algorithm>
 #include "nkb_sequence.cuh"
 #include "nkb_sinks.cuh"

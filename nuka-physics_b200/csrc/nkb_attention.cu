@@ -11,7 +11,7 @@
 // The backward pass works the scores out twice, once for the queries' gradients and once for the keys': 7 products in place of 5, and in return no gradient is summed
 // through atomics, so that the same call gives the same bits, and the shared heads' sum stays in tensor memory.
 // With a window an episode's first tokens may stay visible (sinks): a tile of queries then goes through those of its first query's episode that lie before its keys, in steps of their own at the job's begin, and rows see two
-// ranges of keys, the window's and the sinks'; a second set of the kernels, so that what has no sinks is as it was (queries' gradients 1 to 2 % slower, the others the same). The keys' kernel leaves a sink's far queries to another (nkb_sinks.cu).
+// ranges of keys, the window's and the sinks'; a second set of the kernels, so that what has no sinks is as it was (queries' gradients 1 % slower, the others the same). The keys' kernel leaves a sink's far queries to another (nkb_sinks.cu).
 // Warps have roles: one or two load tiles by TMA, one or two issue products, four for each tile turn scores into probabilities, a row to a thread;
 // P and dS go back to tensor memory as the next product's operand in the inputs' type (their one rounding more; sums and statistics are in 32 bits).
 // One tile's products run under the other's exponentials: forwards the two are one block's, backwards those of two blocks on an SM, and with wide heads, of which one block fills an SM,
@@ -89,6 +89,9 @@ template <bool SINKS> struct RowKeys {
     __device__ __forceinline__ RowKeys(const AttentionParams& p, bool live, int i, int episode) {
         high = live ? i : -1;
         low = !live ? 0 : p.window > 0 ? max(episode, i - p.window + 1) : episode;
+    }
+    // The warp's, which has time after the next job is asked for (queries' gradients of wide heads 1185 us in place of 1202).
+    __device__ __forceinline__ void among_warp(const AttentionParams& p, bool live, int i, int episode) {
         any_low = __reduce_min_sync(~0u, live ? low : 0x7fffffff); any_high = __reduce_max_sync(~0u, high);
         all_low = __reduce_max_sync(~0u, live ? low : 0x7fffffff); all_high = __reduce_min_sync(~0u, high);
         if (SINKS) {
@@ -565,7 +568,8 @@ __global__ void __launch_bounds__(kForward, 1) attention_kernel(const __grid_con
             const int episode = next_first, after = ForwardJob::of_turn(turn + 1);
             if (after < jobs) { next = ForwardJob(p, after); next_first = first_of(next); }
             // keys that any and that all of the warp's rows see; a row that is not there sees none
-            const RowKeys<SINKS> keys(p, i <= last, i, episode);
+            RowKeys<SINKS> keys(p, i <= last, i, episode);
+            keys.among_warp(p, i <= last, i, episode);
             float top = -INFINITY, sum = 0.f;           // of the scores as they are; the sum of exp2(scale2 (S - top))
             bool left = false;
             for (int j = 0; j < through.count; ++j, ++n) {
@@ -842,10 +846,12 @@ __global__ void __launch_bounds__(Queries<DP>::kThreads, Queries<DP>::kBlocks) q
             const QueryJob now = next;
             const int i = now.i0 + row;
             const KeySteps<SINKS> through = now.steps<SINKS>(p);
+            const bool live = i <= now.last;
             const int episode = next_first;
+            RowKeys<SINKS> sees(p, live, i, episode);
             const float lse = next_lse;
             if (job + stride < jobs) { next = QueryJob(p, job + stride); next_first = first_of(next); next_lse = lse_of(next); }
-            const RowKeys<SINKS> sees(p, i <= now.last, i, episode);
+            sees.among_warp(p, live, i, episode);
             // D = dO . O of the thread's row.  O has the error of its own rounding and of P's, which the sum of dS over the row, 0 by definition, shows: the keys' kernel, which runs
             // after this one, gets D without it. Where a step holds all keys of a row D is summed from its own P and dP before dS, which matters where few keys share a row (dq of
             // 24-token episodes was off by 1.8 times its rounding; with many keys the error averages out).

@@ -481,7 +481,7 @@ def selective_scan(x, delta, decay, b, c, episodes, initial=None, skip=None, gat
     a state fades.  skip, delta_bias: channels float32, or None.  initial: rows x channels x states float32, the state that each row begins with, None for 0; an episode that begins inside a row
     begins with 0.  Returns (y, state): y like x, state like initial, what each row ends with.  Rates, states and sums are in 32 bits; exp(dt decay) is off by up to 2^-22 (1 + |dt decay|) of itself, as its argument is rounded
     to 32 bits, and 0 below 2^-126. Where a gradient may
-    be asked for, the states before each fourth or eighth token are kept (at 16 states 8 bytes for each value of x)."""
+    be asked for, the states before each fourth or eighth token are kept (at 16 states 8 bytes for each value of x, up to twice that where rows are short)."""
     device = _on_gpu(x, delta, decay, b, c, initial, skip, gate, delta_bias, episodes._plan)
     _tokens_of(x, episodes, 2, "x")
     x, delta, decay, b, c, skip, gate, delta_bias = _scan_inputs(x, delta, decay, b, c, skip, gate, delta_bias)
